@@ -94,7 +94,8 @@ typedef struct ksmm_tile {
  * projections of the ViT feed-forward block (src/ksmm_py/model/vit.py:416-431). */
 typedef enum ksmm_act {
     KSMM_ACT_NONE = 0,
-    KSMM_ACT_GELU = 1 /* x * Phi(x), the erf form (torch.nn.GELU() default)                 */
+    KSMM_ACT_GELU = 1, /* x * Phi(x), the erf form (torch.nn.GELU() default)                */
+    KSMM_ACT_SILU = 2  /* x / (1 + exp(-x)): ksmm_gated_* only                              */
 } ksmm_act;
 
 typedef struct ksmm_epilogue {
@@ -314,6 +315,70 @@ int64_t ksmm_static_scratch_bytes(void);
 int ksmm_chain_forward_static(const ksmm_factor_desc *factors, int n_factors, const void *x, void *y,
                               int64_t batch, int x_dtype, int y_dtype, int bs_last, int fuse,
                               const ksmm_epilogue *epilogue, void *stream);
+
+/* ---- operators around a Kronecker-sparse feed-forward block (fp32 and fp16) -----------------------
+ * All of them launch on the caller's stream, allocate nothing, keep nothing, and compute in fp32; results are
+ * rounded once.  Every pointer needs the alignment of its elements only; workspaces 16 bytes.  Outputs must not
+ * overlap inputs unless said so. */
+
+/* Gated projection: two factors of one pattern (a, b, c, d) that share their input x,
+ *     h = act(G x + bias_g) * (U x + bias_u)
+ * w holds both side by side, (a*d*c, 2*b), gate columns first: the kernel-format weights of ONE factor with pattern
+ * (a, 2b, c, d).  bias (NULL: none) has that factor's 2*a*b*d output features; h has a*b*d.  act: any ksmm_act.
+ * The backward pass computes the projections again from x, and writes what is not NULL of dx (x's shape), dw (w's)
+ * and dbias (bias's).  Tensors of 2^31 elements and more (2*a*b*d x batch among them) are refused.
+ * dw and dbias are sums in a fixed order: the same bits on every call. */
+int ksmm_gated_forward(const void *x, const void *w, const void *bias, void *h, int64_t batch, int a, int b,
+                       int c, int d, int dtype, int bs_last, int act, void *stream);
+int64_t ksmm_gated_backward_workspace(int64_t batch, int a, int b, int c, int d, int dtype, int bs_last);
+int ksmm_gated_backward(const void *dh, const void *x, const void *w, const void *bias, void *dx, void *dw,
+                        void *dbias, void *workspace, int64_t workspace_bytes, int64_t batch, int a, int b, int c,
+                        int d, int dtype, int bs_last, int act, void *stream);
+
+/* Norms around a residual connection:
+ *     r_out = residual + alpha * gate * P(x),   P(x) = x, or norm(x) * post_weight where that is given
+ *     n_out = norm(r_out) * weight + bias
+ * with norm(t) = t / sqrt(mean(t^2) + eps) (KSMM_NORM_RMS) or (t - mean) / sqrt(var + eps) (KSMM_NORM_LAYER) over
+ * the features of a row.  Tensors are (batch, features), or (features, batch) with bs_last.  gate has `groups` rows of
+ * features, each for batch / groups consecutive rows of the tensors.  x NULL: r_out is the residual and is not
+ * written.  n_out NULL: not wanted.  NULL gate and weight count as ones, NULL bias as zeros.
+ * stats (NULL: not wanted): 4 x batch floats for the backward pass.
+ * Batch-size-first rows of up to 32768 bytes; batch-size-last any number of features. */
+typedef enum ksmm_norm_kind { KSMM_NORM_RMS = 0, KSMM_NORM_LAYER = 1 } ksmm_norm_kind;
+typedef struct ksmm_norm_desc {
+    const void *x, *residual, *gate, *post_weight, *weight, *bias;
+    int64_t groups;
+    float alpha, eps;
+    int kind; /* ksmm_norm_kind */
+} ksmm_norm_desc;
+int ksmm_residual_norm_forward(const ksmm_norm_desc *desc, void *r_out, void *n_out, float *stats, int64_t batch,
+                               int64_t features, int dtype, int bs_last, void *stream);
+/* Gradients from those of the results (either may be NULL: zero).  What is not wanted is NULL; dgate of more than one
+ * group in batch-size-last layout needs dresidual.  dgate, dpost_weight, dweight and dbias are sums in a fixed order. */
+int64_t ksmm_residual_norm_backward_workspace(int64_t batch, int64_t features, int64_t groups, int dtype,
+                                              int bs_last);
+int ksmm_residual_norm_backward(const ksmm_norm_desc *desc, const float *stats, const void *dr_out,
+                                const void *dn_out, void *dx, void *dresidual, void *dgate, void *dpost_weight,
+                                void *dweight, void *dbias, void *workspace, int64_t workspace_bytes, int64_t batch,
+                                int64_t features, int dtype, int bs_last, void *stream);
+
+/* Update of a factor in kernel format, (blocks * c, parts * b), whose every c x b matrix is made orthogonal by
+ * Newton-Schulz steps:
+ *     m' = beta m + g,   u = nesterov ? g + beta m' : m'        (momentum NULL: u = g)
+ *     X = u / (|u|_F + eps);   steps times:  A = X X^T,  X = p0 X + (p1 A + p2 A A) X
+ *     out = keep * weight - rate * X                            (weight NULL: out = X)
+ * grad, weight and out have `dtype`; momentum is fp32.  master (NULL: none): fp32 values that the weights are
+ * rounded from; they are read in place of weight, and written too.  momentum_out, master_out and out may be
+ * momentum, master and weight themselves. */
+typedef struct ksmm_muon_desc {
+    float coefficients[3];
+    float eps, beta, keep, rate;
+    int steps, nesterov;
+} ksmm_muon_desc;
+int64_t ksmm_muon_workspace(int64_t blocks, int c, int b, int parts);
+int ksmm_muon_update(const ksmm_muon_desc *desc, const void *grad, const float *momentum, float *momentum_out,
+                     const void *weight, const float *master, float *master_out, void *out, void *workspace,
+                     int64_t workspace_bytes, int64_t blocks, int c, int b, int parts, int dtype, void *stream);
 
 #ifdef __cplusplus
 }

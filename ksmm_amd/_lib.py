@@ -13,7 +13,8 @@ LIB_PATH = os.path.join(HERE, "libksmm_hip.so")
 KSMM_F32, KSMM_F16, KSMM_FP8_E4M3 = 0, 1, 2
 ALGO_AUTO, ALGO_GENERIC, ALGO_WAVE, ALGO_TILE = 0, 1, 2, 3
 MAX_FACTORS = 16
-ACT_NONE, ACT_GELU = 0, 1
+ACT_NONE, ACT_GELU, ACT_SILU = 0, 1, 2
+NORM_RMS, NORM_LAYER = 0, 1
 ABI_VERSION = 2
 
 c_i64 = ctypes.c_int64
@@ -37,6 +38,16 @@ class KsmmFactorDesc(ctypes.Structure):
 
 class KsmmEpilogue(ctypes.Structure):
     _fields_ = [("bias", c_vp), ("act", c_int)]
+
+
+class KsmmNormDesc(ctypes.Structure):
+    _fields_ = [("x", c_vp), ("residual", c_vp), ("gate", c_vp), ("post_weight", c_vp), ("weight", c_vp), ("bias", c_vp),
+                ("groups", c_i64), ("alpha", ctypes.c_float), ("eps", ctypes.c_float), ("kind", c_int)]
+
+
+class KsmmMuonDesc(ctypes.Structure):
+    _fields_ = [("coefficients", ctypes.c_float * 3), ("eps", ctypes.c_float), ("beta", ctypes.c_float),
+                ("keep", ctypes.c_float), ("rate", ctypes.c_float), ("steps", c_int), ("nesterov", c_int)]
 
 
 # name -> (restype, argtypes); every symbol include/ksmm_hip.h declares
@@ -91,6 +102,17 @@ SIGNATURES = {
     "ksmm_static_scratch_bytes": (c_i64, []),
     "ksmm_chain_forward_static": (c_int, [ctypes.POINTER(KsmmFactorDesc), c_int, c_vp, c_vp, c_i64, c_int,
                                           c_int, c_int, c_int, ctypes.POINTER(KsmmEpilogue), c_vp]),
+    "ksmm_gated_forward": (c_int, [c_vp, c_vp, c_vp, c_vp, c_i64, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_vp]),
+    "ksmm_gated_backward_workspace": (c_i64, [c_i64, c_int, c_int, c_int, c_int, c_int, c_int]),
+    "ksmm_gated_backward": (c_int, [c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_i64, c_i64, c_int, c_int, c_int, c_int,
+                                    c_int, c_int, c_int, c_vp]),
+    "ksmm_residual_norm_forward": (c_int, [ctypes.POINTER(KsmmNormDesc), c_vp, c_vp, c_vp, c_i64, c_i64, c_int, c_int, c_vp]),
+    "ksmm_residual_norm_backward_workspace": (c_i64, [c_i64, c_i64, c_i64, c_int, c_int]),
+    "ksmm_residual_norm_backward": (c_int, [ctypes.POINTER(KsmmNormDesc), c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp,
+                                            c_vp, c_i64, c_i64, c_i64, c_int, c_int, c_vp]),
+    "ksmm_muon_workspace": (c_i64, [c_i64, c_int, c_int, c_int]),
+    "ksmm_muon_update": (c_int, [ctypes.POINTER(KsmmMuonDesc), c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_i64, c_i64,
+                                 c_int, c_int, c_int, c_int, c_vp]),
 }
 
 _lib = None

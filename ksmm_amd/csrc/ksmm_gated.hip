@@ -1,0 +1,606 @@
+// Gated projection: two factors of one pattern that share their input, the activation of one and the product in one
+// kernel.
+//
+//     z[a_i, p, b_i, d_i, n] = sum_c W[a_i, p, b_i, c_i, d_i] x[a_i, c_i, d_i, n] + bias[a_i, p, b_i, d_i]    (p = 0, 1)
+//     h[a_i, b_i, d_i, n]    = act(z[a_i, 0, b_i, d_i, n]) * z[a_i, 1, b_i, d_i, n]
+//
+// The weights of both lie side by side, (a*d*c, 2*b), gate columns first: as kernel-format weights they are ONE factor
+// with pattern (a, 2b, c, d), which is what the gradients of input and weights run as, on the kernels that any factor
+// has.  z itself never reaches memory on the way forward; backward it is computed again, and
+//     dz[0] = dh * z1 * act'(z0),  dz[1] = dh * act(z0)
+// leave the kernel in its place (MODE 1).  Sums are fp32; h and dz are rounded once, from fp32.
+//
+// An MFMA tile has 32 rows of weights.  Batch-size-first these are 16 gate and 16 up columns of the same outputs, dealt
+// so that a lane (which holds rows 8j + 4*(lane/32) + i) has gate and up of 8 outputs in a row: the product needs no
+// other lane's values and leaves as whole vectors.  Batch-size-last the operands swap sides: a lane holds one output's
+// gate (or up) at 16 batch elements in a row, and gate and up are two tiles of the same lanes.
+#include "ksmm_mfma.h"
+
+namespace ksmm {
+
+namespace {
+
+struct GatedArgs {
+    const void *x, *w, *bias, *dh;
+    void *out;  // h, or dz (MODE 1)
+    int64_t batch;
+    int a, b, c, d;
+    int act;
+};
+
+constexpr float LOG2E = 1.4426950408889634f;
+
+// act(z), and act'(z) where wanted.  fp32: the library's functions; fp16: the forms of one or two transcendentals whose
+// error (3e-7 of the value) is far below the type's
+template <typename T, bool SLOPE> __device__ __forceinline__ float activate(int act, float z, float &slope)
+{
+    if (act == KSMM_ACT_SILU) {
+        float s;
+        if constexpr (sizeof(T) == 4)
+            s = 1.f / (1.f + expf(-z));
+        else
+            s = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-LOG2E * z));
+        if constexpr (SLOPE) slope = s * fmaf(z, 1.f - s, 1.f);
+        return z * s;
+    }
+    if (act == KSMM_ACT_GELU) {
+        float phi, ex;
+        if constexpr (sizeof(T) == 4) {
+            phi = 0.5f * erfcf(-0.70710678118654752f * z);
+            ex = SLOPE ? expf(-0.5f * z * z) : 0.f;
+        } else {
+            const float q = fabsf(z) * 0.84932180028801907f;
+            const float t = __builtin_amdgcn_rcpf(fmaf(0.2727374808792225f, q, 1.0f));
+            float poly = fmaf(0.5307027145f, t, -0.7265760135f);
+            poly = fmaf(poly, t, 0.7107068705f);
+            poly = fmaf(poly, t, -0.142248368f);
+            poly = fmaf(poly, t, 0.127414796f);
+            ex = __builtin_amdgcn_exp2f(-(q * q));
+            const float tail = poly * t * ex;
+            phi = z >= 0.f ? 1.f - tail : tail;
+        }
+        if constexpr (SLOPE) slope = fmaf(z * 0.39894228040143268f, ex, phi);
+        return z * phi;
+    }
+    if constexpr (SLOPE) slope = 1.f;
+    return z;
+}
+
+// ---- MFMA operands: KS k values of one row or column a lane --------------------------------------------
+// fp16: 8 k in a row from 8 * (lane / 32) on, one 32x32x16.  fp32: 4 k in a row from 4 * (lane / 32) on, four 32x32x2
+// (the order of k within a sum is free, as long as both operands have the same)
+template <typename T> struct op;
+template <> struct op<half_t> {
+    static constexpr int KS = 16, PER = 8;
+    typedef half8_t type;
+    __device__ static __forceinline__ float16_t mfma(type a, type b, float16_t c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+};
+template <> struct op<float> {
+    static constexpr int KS = 8, PER = 4;
+    typedef float4_t type;
+    __device__ static __forceinline__ float16_t mfma(type a, type b, float16_t c)
+    {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[i], b[i], c, 0, 0, 0);
+        return c;
+    }
+};
+
+// column of a weight row (gate columns 0..tb-1, up columns tb..) that row r of the 16 + 16 tile holds
+__device__ __forceinline__ int mixed_col(int r, int tb)
+{
+    const int rg = r >> 2, hh = rg & 1, j = rg >> 1;
+    return (j >> 1) * tb + 8 * hh + 4 * (j & 1) + (r & 3);
+}
+// batch element that row r of a batch-size-last tile holds: a lane ends up with 16 in a row
+__device__ __forceinline__ int run_col(int r)
+{
+    const int rg = r >> 2;
+    return 16 * (rg & 1) + 4 * (rg >> 1) + (r & 3);
+}
+
+// k-outer operand S[k][col], columns by groups of 4: group rg (0..7) of the operand at column at(rg)
+template <typename F> __device__ __forceinline__ half8_t k_outer(const half_t *s, int ld, int k0, int lane, F at)
+{
+    const int kq = lane >> 5, i16 = lane & 15, rg = 4 * ((lane >> 4) & 1) + (i16 & 3);
+    const half_t *p = s + (k0 + 8 * kq + (i16 >> 2)) * ld + at(rg);
+    typedef short4_t __attribute__((address_space(3))) * lds_ptr;
+    typedef short short8_t __attribute__((ext_vector_type(8)));
+    const short4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(p));
+    const short4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(p + 4 * ld));
+    return __builtin_bit_cast(half8_t, short8_t{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]});
+}
+template <typename F> __device__ __forceinline__ float4_t k_outer(const float *s, int ld, int k0, int lane, F at)
+{
+    const float *p = s + (k0 + 4 * (lane >> 5)) * ld + at((lane & 31) >> 2) + (lane & 3);
+    return float4_t{p[0], p[ld], p[2 * ld], p[3 * ld]};
+}
+// k-inner operand S[idx][k]
+template <typename T> __device__ __forceinline__ typename op<T>::type k_inner(const T *s, int ld, int idx0, int k0, int lane)
+{
+    return *(const typename op<T>::type *)(s + (idx0 + (lane & 31)) * ld + k0 + op<T>::PER * (lane >> 5));
+}
+
+template <typename T> constexpr int EPV = 16 / (int)sizeof(T);
+template <typename T, int N> struct Run {
+    T e[N];
+};
+// count (<= N) elements from p on, the rest zeros; all of them in one or more 16-byte loads at element alignment
+template <typename T, int N> __device__ __forceinline__ Run<T, N> load_run(const T *p, int count)
+{
+    Run<T, N> r;
+    if (count >= N) {
+        __builtin_memcpy(&r, p, sizeof(r));
+    } else {
+#pragma unroll
+        for (int e = 0; e < N; ++e) r.e[e] = e < count ? p[e] : (T)0.f;
+    }
+    return r;
+}
+template <typename T, int N> __device__ __forceinline__ void store_run(T *p, int count, const Run<T, N> &r)
+{
+    if (count >= N) {
+        __builtin_memcpy(p, &r, sizeof(r));
+    } else {
+#pragma unroll
+        for (int e = 0; e < N; ++e)
+            if (e < count) p[e] = r.e[e];
+    }
+}
+
+// ---- tiles ---------------------------------------------------------------------------------------------
+// Workgroup: TB outputs (2 * TB weight columns) of D neighbouring d_i of one a_i x TN rows of the batch; WB x WN waves.
+// x and W arrive in slabs of TK, through registers into two LDS buffers in turn.  Batch-size-first a thread takes D * PER
+// values of a row, the PER k of D neighbouring d_i, and writes them as D chunks of one d_i each.
+template <typename T, bool LAST, int D, int TB, int TN, int TK, int WB, int WN> struct Tile {
+    static constexpr int THREADS = 64 * WB * WN, E = EPV<T>;
+    static constexpr int BT = TB / WB / (LAST ? 32 : 16), NT = TN / WN / 32;  // MFMA tiles a wave: outputs (16, or 32 as gate and up), rows
+    static constexpr int LDW = pads<T>::outer(2 * TB), LDX = LAST ? pads<T>::outer(TN) : pads<T>::inner(TK);
+    static constexpr int W_PLANE = TK * LDW, X_PLANE = LAST ? TK * LDX : TN * LDX;
+    static constexpr int BUF = D * (W_PLANE + X_PLANE), LDS_BYTES = 2 * BUF * (int)sizeof(T);
+    static constexpr int W_UNITS = D * TK * 2 * TB / E, X_UNITS = TK * TN / E;
+    static constexpr int W_PER = W_UNITS / THREADS, X_PER = X_UNITS / THREADS;
+    static_assert(W_UNITS % THREADS == 0 && X_UNITS % THREADS == 0 && TK % op<T>::KS == 0 && (!LAST || D == 1), "shape");
+    static_assert(LDS_BYTES <= 160 * 1024, "LDS");
+};
+
+template <typename T, bool LAST, int D, int TB, int TN, int TK, int WB, int WN, int MODE>
+__global__ __launch_bounds__(64 * WB *WN) void ks_gated_kernel(GatedArgs g, int b_tiles, int n_tiles, int blocks)
+{
+    typedef Tile<T, LAST, D, TB, TN, TK, WB, WN> C;
+    typedef op<T> O;
+    constexpr int E = C::E;
+    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+    T *const lds = (T *)smem;
+    auto ws = [&](int buf, int p) { return lds + buf * C::BUF + p * C::W_PLANE; };
+    auto xs = [&](int buf, int p) { return lds + buf * C::BUF + D * C::W_PLANE + p * C::X_PLANE; };
+
+    // each XCD gets a contiguous range of tiles: those that share rows of x share an L2
+    const int per_xcd = (blocks + 7) / 8, lid = (blockIdx.x % 8) * per_xcd + blockIdx.x / 8;
+    if (lid >= blocks) return;
+    const int a = g.a, b = g.b, c = g.c, d = g.d, dg = d / D;
+    const int bt = lid % b_tiles, rest = lid / b_tiles;
+    // (batch-size-first the d_i of an a_i share cache lines of x and h: they are neighbours)
+    const int grp = LAST ? rest / n_tiles : rest % (a * dg), nt = LAST ? rest % n_tiles : rest / (a * dg);
+    const int a_i = grp / dg, d0 = (grp - a_i * dg) * D;
+    const int b0 = bt * TB;
+    const int64_t n0 = (int64_t)nt * TN, B = g.batch;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wb = wave / WN, wn = wave % WN;
+    const int64_t in_size = (int64_t)a * c * d;
+    const T *const w = (const T *)g.w + (int64_t)(a_i * d + d0) * c * 2 * b;
+    const T *const x = LAST ? (const T *)g.x + ((int64_t)a_i * c * d + d0) * B : (const T *)g.x + (int64_t)a_i * c * d + d0;
+
+    Run<T, E> wr[C::W_PER];
+    Run<T, D * E> xr[C::X_PER];
+    auto gload = [&](int k0) {
+#pragma unroll
+        for (int i = 0; i < C::W_PER; ++i) {
+            const int v = tid + i * C::THREADS, cv = v % (2 * TB / E), row = v / (2 * TB / E);
+            const int p = row / TK, k = k0 + row % TK;
+            const int col = cv * E, part = col / TB, bi = b0 + col % TB;
+            // past the block's rows: zeros.  Past its outputs: anything (they are not stored), here zeros
+            const int count = k < c ? min(max(b - bi, 0), E) : 0;
+            wr[i] = load_run<T, E>(w + ((int64_t)p * c + k) * 2 * b + part * b + bi, count);
+        }
+#pragma unroll
+        for (int i = 0; i < C::X_PER; ++i) {
+            const int v = tid + i * C::THREADS;
+            if constexpr (LAST) {
+                const int k = k0 + v / (TN / E);
+                const int64_t n = n0 + v % (TN / E) * E;
+                const int count = k < c ? (int)min(max(B - n, (int64_t)0), (int64_t)E) : 0;
+                xr[i] = load_run<T, E>(x + (int64_t)k * d * B + n, count);
+            } else {
+                const int k = k0 + v % (TK / E) * E;
+                const int64_t n = min(n0 + v / (TK / E), B - 1);  // (rows past the batch: the last one again, not stored)
+                const int count = min(max(c - k, 0), E);
+                const T *const from = x + n * in_size + (int64_t)k * d;
+                if (d == D) {
+                    xr[i] = load_run<T, D * E>(from, count * D);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < E; ++e) {
+                        const Run<T, D> s = load_run<T, D>(from + (int64_t)e * d, e < count ? D : 0);
+#pragma unroll
+                        for (int p = 0; p < D; ++p) xr[i].e[e * D + p] = s.e[p];
+                    }
+                }
+            }
+        }
+    };
+    auto lstore = [&](int buf) {
+#pragma unroll
+        for (int i = 0; i < C::W_PER; ++i) {
+            const int v = tid + i * C::THREADS, cv = v % (2 * TB / E), row = v / (2 * TB / E);
+            *(Run<T, E> *)__builtin_assume_aligned(ws(buf, row / TK) + (row % TK) * C::LDW + cv * E, 16) = wr[i];
+        }
+#pragma unroll
+        for (int i = 0; i < C::X_PER; ++i) {
+            const int v = tid + i * C::THREADS;
+            if constexpr (LAST) {
+                *(Run<T, E> *)__builtin_assume_aligned(xs(buf, 0) + v / (TN / E) * C::LDX + v % (TN / E) * E, 16) = xr[i];
+            } else {
+#pragma unroll
+                for (int p = 0; p < D; ++p) {
+                    Run<T, E> s;
+#pragma unroll
+                    for (int e = 0; e < E; ++e) s.e[e] = xr[i].e[e * D + p];
+                    *(Run<T, E> *)__builtin_assume_aligned(xs(buf, p) + v / (TK / E) * C::LDX + v % (TK / E) * E, 16) = s;
+                }
+            }
+        }
+    };
+
+    constexpr int PARTS = LAST ? 2 : 1;  // accumulators an output tile: gate and up apart, or both in one
+    float16_t acc[D][PARTS][C::BT][C::NT];
+#pragma unroll
+    for (int p = 0; p < D; ++p)
+#pragma unroll
+        for (int q = 0; q < PARTS; ++q)
+#pragma unroll
+            for (int i = 0; i < C::BT; ++i)
+#pragma unroll
+                for (int j = 0; j < C::NT; ++j)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) acc[p][q][i][j][e] = 0.f;
+
+    const int steps = (c + TK - 1) / TK;
+    gload(0);
+    lstore(0);
+    __syncthreads();
+    for (int s = 0; s < steps; ++s) {
+        const int buf = s & 1;
+        if (s + 1 < steps) gload((s + 1) * TK);
+#pragma unroll
+        for (int k0 = 0; k0 < TK; k0 += O::KS)
+#pragma unroll
+            for (int p = 0; p < D; ++p) {
+                const T *wp = ws(buf, p), *xp = xs(buf, p);
+                typename O::type fw[PARTS][C::BT], fx[C::NT];
+#pragma unroll
+                for (int q = 0; q < PARTS; ++q)
+#pragma unroll
+                    for (int i = 0; i < C::BT; ++i) {
+                        if constexpr (LAST) {
+                            const int col = q * TB + (wb * C::BT + i) * 32;
+                            fw[q][i] = k_outer(wp, C::LDW, k0, lane, [&](int rg) { return col + 4 * rg; });
+                        } else {
+                            const int col = (wb * C::BT + i) * 16;
+                            fw[q][i] = k_outer(wp, C::LDW, k0, lane, [&](int rg) { return col + mixed_col(4 * rg, TB); });
+                        }
+                    }
+#pragma unroll
+                for (int j = 0; j < C::NT; ++j) {
+                    const int n = (wn * C::NT + j) * 32;
+                    if constexpr (LAST)
+                        fx[j] = k_outer(xp, C::LDX, k0, lane, [&](int rg) { return n + run_col(4 * rg); });
+                    else
+                        fx[j] = k_inner<T>(xp, C::LDX, n, k0, lane);
+                }
+#pragma unroll
+                for (int q = 0; q < PARTS; ++q)
+#pragma unroll
+                    for (int i = 0; i < C::BT; ++i)
+#pragma unroll
+                        for (int j = 0; j < C::NT; ++j)
+                            acc[p][q][i][j] = LAST ? O::mfma(fx[j], fw[q][i], acc[p][q][i][j]) : O::mfma(fw[q][i], fx[j], acc[p][q][i][j]);
+            }
+        if (s + 1 < steps) lstore(buf ^ 1);
+        __syncthreads();
+    }
+
+    const T *const bias = (const T *)g.bias, *const dh = (const T *)g.dh;
+    T *const out = (T *)g.out;
+    const int lq = lane >> 5, l32 = lane & 31;
+    if constexpr (LAST) {
+        // a lane: one output, 16 rows of the batch in a row
+#pragma unroll
+        for (int i = 0; i < C::BT; ++i) {
+            const int bi = b0 + (wb * C::BT + i) * 32 + l32;
+            if (bi >= b) continue;
+            const int64_t zg = ((int64_t)(a_i * 2) * b + bi) * d + d0, zu = zg + (int64_t)b * d, hf = ((int64_t)a_i * b + bi) * d + d0;
+            const float bg = bias ? (float)bias[zg] : 0.f, bu = bias ? (float)bias[zu] : 0.f;
+#pragma unroll
+            for (int j = 0; j < C::NT; ++j) {
+                const int64_t n = n0 + (wn * C::NT + j) * 32 + 16 * lq;
+                if (n >= B) continue;
+                const int count = (int)min(B - n, (int64_t)16);
+                Run<T, 16> r0, r1, in;
+                if (MODE == 1) in = load_run<T, 16>(dh + hf * B + n, count);
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const float zgv = acc[0][0][i][j][e] + bg, zuv = acc[0][PARTS - 1][i][j][e] + bu;
+                    float slope = 0.f;
+                    const float act = activate<T, MODE == 1>(g.act, zgv, slope);
+                    if (MODE == 0) {
+                        r0.e[e] = (T)(act * zuv);
+                    } else {
+                        const float v = (float)in.e[e];
+                        r0.e[e] = (T)(v * zuv * slope);
+                        r1.e[e] = (T)(v * act);
+                    }
+                }
+                if (MODE == 0) {
+                    store_run<T, 16>(out + hf * B + n, count, r0);
+                } else {
+                    store_run<T, 16>(out + zg * B + n, count, r0);
+                    store_run<T, 16>(out + zu * B + n, count, r1);
+                }
+            }
+        }
+    } else {
+        // a lane: one row of the batch, 8 outputs of D neighbouring d_i
+        const int64_t out_size = (int64_t)a * b * d;
+#pragma unroll
+        for (int i = 0; i < C::BT; ++i) {
+            const int bi = b0 + (wb * C::BT + i) * 16 + 8 * lq;
+            const int count = min(b - bi, 8);
+            if (count <= 0) continue;
+            const int64_t zg = ((int64_t)(a_i * 2) * b + bi) * d + d0, zu = zg + (int64_t)b * d, hf = ((int64_t)a_i * b + bi) * d + d0;
+            // 8 x D values: b_i * d + d_i, in a row where D is all of d
+            auto load = [&](const T *from) {
+                if (d == D) return load_run<T, 8 * D>(from, count * D);
+                Run<T, 8 * D> r;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const Run<T, D> s = load_run<T, D>(from + (int64_t)e * d, e < count ? D : 0);
+#pragma unroll
+                    for (int p = 0; p < D; ++p) r.e[e * D + p] = s.e[p];
+                }
+                return r;
+            };
+            auto store = [&](T *to, const Run<T, 8 * D> &r) {
+                if (d == D) {
+                    store_run<T, 8 * D>(to, count * D, r);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        Run<T, D> s;
+#pragma unroll
+                        for (int p = 0; p < D; ++p) s.e[p] = r.e[e * D + p];
+                        store_run<T, D>(to + (int64_t)e * d, e < count ? D : 0, s);
+                    }
+                }
+            };
+            Run<T, 8 * D> bg, bu;
+            if (bias) {
+                bg = load(bias + zg);
+                bu = load(bias + zu);
+            }
+#pragma unroll
+            for (int j = 0; j < C::NT; ++j) {
+                const int64_t n = n0 + (wn * C::NT + j) * 32 + l32;
+                if (n >= B) continue;
+                Run<T, 8 * D> r0, r1, in;
+                if (MODE == 1) in = load(dh + n * out_size + hf);
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+#pragma unroll
+                    for (int p = 0; p < D; ++p) {
+                        float zgv = acc[p][0][i][j][e], zuv = acc[p][0][i][j][8 + e], slope = 0.f;
+                        if (bias) {
+                            zgv += (float)bg.e[e * D + p];
+                            zuv += (float)bu.e[e * D + p];
+                        }
+                        const float act = activate<T, MODE == 1>(g.act, zgv, slope);
+                        if (MODE == 0) {
+                            r0.e[e * D + p] = (T)(act * zuv);
+                        } else {
+                            const float v = (float)in.e[e * D + p];
+                            r0.e[e * D + p] = (T)(v * zuv * slope);
+                            r1.e[e * D + p] = (T)(v * act);
+                        }
+                    }
+                if (MODE == 0) {
+                    store(out + n * out_size + hf, r0);
+                } else {
+                    store(out + n * 2 * out_size + zg, r0);
+                    store(out + n * 2 * out_size + zu, r1);
+                }
+            }
+        }
+    }
+}
+
+// ---- few rows ------------------------------------------------------------------------------------------
+// A workgroup takes 16 outputs of one block x 32 rows of the batch; its waves share c and add their sums in LDS, one
+// output and row a thread.  Operands come straight from global memory, element by element: any shape and alignment.
+constexpr int FEW_WAVES = 8;
+template <typename T, bool LAST, int MODE>
+__global__ __launch_bounds__(64 * FEW_WAVES) void ks_gated_few_kernel(GatedArgs g, int b_tiles, int blocks)
+{
+    typedef op<T> O;
+    __shared__ float red[FEW_WAVES][16 * 64];
+    const int per_xcd = (blocks + 7) / 8, lid = (blockIdx.x % 8) * per_xcd + blockIdx.x / 8;
+    if (lid >= blocks) return;
+    const int a = g.a, b = g.b, c = g.c, d = g.d, groups = a * d;
+    const int bt = lid % b_tiles, rest = lid / b_tiles, grp = rest % groups, nt = rest / groups;
+    const int a_i = grp / d, d_i = grp - a_i * d, b0 = bt * 16;
+    const int64_t B = g.batch, n0 = (int64_t)nt * 32;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l32 = lane & 31, lq = lane >> 5;
+    const int64_t kstride = LAST ? (int64_t)d * B : d;
+    const T *const w = (const T *)g.w + (int64_t)grp * c * 2 * b;
+    const int64_t n_in = min(n0 + l32, B - 1);
+    const T *const x = LAST ? (const T *)g.x + ((int64_t)a_i * c * d + d_i) * B + n_in
+                            : (const T *)g.x + n_in * a * c * d + (int64_t)a_i * c * d + d_i;
+    const int col = mixed_col(l32, 16);  // 16 of gate, 16 of up
+    const T *const wl = w + (col >> 4) * b + min(b0 + (col & 15), b - 1);
+    float16_t acc;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) acc[e] = 0.f;
+    for (int k0 = wave * O::KS; k0 < c; k0 += FEW_WAVES * O::KS) {
+        typename O::type fw, fx;
+#pragma unroll
+        for (int e = 0; e < O::PER; ++e) {
+            const int k = k0 + O::PER * lq + e;
+            fw[e] = k < c ? wl[(int64_t)k * 2 * b] : (T)0.f;
+            fx[e] = k < c ? x[(int64_t)k * kstride] : (T)0.f;
+        }
+        acc = O::mfma(fw, fx, acc);
+    }
+#pragma unroll
+    for (int e = 0; e < 16; ++e) red[wave][e * 64 + lane] = acc[e];
+    __syncthreads();
+    // thread: lane's row of the batch, output 8 * (lane / 32) + e
+    const int e = wave, bi = b0 + 8 * lq + e;
+    const int64_t n = n0 + l32;
+    if (bi >= b || n >= B) return;
+    float zg = 0.f, zu = 0.f;
+#pragma unroll
+    for (int i = 0; i < FEW_WAVES; ++i) {
+        zg += red[i][e * 64 + lane];
+        zu += red[i][(8 + e) * 64 + lane];
+    }
+    const int64_t fg = ((int64_t)(a_i * 2) * b + bi) * d + d_i, fu = fg + (int64_t)b * d, fh = ((int64_t)a_i * b + bi) * d + d_i;
+    if (g.bias) {
+        zg += (float)((const T *)g.bias)[fg];
+        zu += (float)((const T *)g.bias)[fu];
+    }
+    const int64_t out_size = (int64_t)a * b * d;
+    auto at = [&](int64_t f, int64_t size) { return LAST ? f * B + n : n * size + f; };
+    float slope = 0.f;
+    const float act = activate<T, MODE == 1>(g.act, zg, slope);
+    T *const out = (T *)g.out;
+    if (MODE == 0) {
+        out[at(fh, out_size)] = (T)(act * zu);
+    } else {
+        const float v = (float)((const T *)g.dh)[at(fh, out_size)];
+        out[at(fg, 2 * out_size)] = (T)(v * zu * slope);
+        out[at(fu, 2 * out_size)] = (T)(v * act);
+    }
+}
+
+// ---- choices -------------------------------------------------------------------------------------------
+int launched() { return hipGetLastError() == hipSuccess ? KSMM_OK : KSMM_ERR_LAUNCH; }
+
+template <typename T, bool LAST, int MODE> int run_few(const GatedArgs &g, hipStream_t s)
+{
+    const int b_tiles = (g.b + 15) / 16;
+    const int64_t blocks = (int64_t)b_tiles * g.a * g.d * ((g.batch + 31) / 32);
+    if (blocks > 0x7ffffff0LL) return KSMM_ERR_TOO_LARGE;
+    hipLaunchKernelGGL((ks_gated_few_kernel<T, LAST, MODE>), dim3((unsigned)((blocks + 7) / 8 * 8)), dim3(64 * FEW_WAVES), 0, s, g, b_tiles, (int)blocks);
+    return launched();
+}
+
+template <typename T, bool LAST, int D, int TB, int TN, int TK, int WB, int WN, int MODE> int run_tile(const GatedArgs &g, hipStream_t s)
+{
+    typedef Tile<T, LAST, D, TB, TN, TK, WB, WN> C;
+    const int b_tiles = (g.b + TB - 1) / TB;
+    const int64_t n_tiles = (g.batch + TN - 1) / TN, blocks = (int64_t)b_tiles * g.a * (g.d / D) * n_tiles;
+    if (blocks > 0x7ffffff0LL) return KSMM_ERR_TOO_LARGE;
+    const auto fn = &ks_gated_kernel<T, LAST, D, TB, TN, TK, WB, WN, MODE>;
+    if (C::LDS_BYTES > 64 * 1024) {
+        const int rc = ensure_dynamic_lds((const void *)fn, C::LDS_BYTES);
+        if (rc != KSMM_OK) return rc;
+    }
+    hipLaunchKernelGGL(fn, dim3((unsigned)((blocks + 7) / 8 * 8)), dim3(C::THREADS), C::LDS_BYTES, s, g, b_tiles, (int)n_tiles, (int)blocks);
+    return launched();
+}
+
+template <typename T, bool LAST, int MODE> int run(const GatedArgs &g, hipStream_t s)
+{
+    constexpr int TK = sizeof(T) == 4 ? 16 : 32;
+    if (g.batch <= 128) return run_few<T, LAST, MODE>(g, s);
+    if constexpr (LAST) return run_tile<T, true, 1, 64, 128, TK, 2, 2, MODE>(g, s);
+    if constexpr (!LAST) {
+        if (g.d == 1) return run_tile<T, false, 1, 64, 128, TK, 2, 2, MODE>(g, s);
+        if (g.d % 4 == 0) return run_tile<T, false, 4, 32, 64, TK, 2, 2, MODE>(g, s);
+        if (g.d % 3 == 0) return run_tile<T, false, 3, 32, 128, TK, 2, 2, MODE>(g, s);
+        if (g.d % 2 == 0) return run_tile<T, false, 2, 64, 128, TK, 2, 2, MODE>(g, s);
+        return run_tile<T, false, 1, 64, 128, TK, 2, 2, MODE>(g, s);
+    }
+    return KSMM_ERR_BAD_ALGO;
+}
+
+}  // namespace
+
+int gated_run(const void *x, const void *w, const void *bias, const void *dh, void *out, int64_t batch, int a, int b, int c, int d,
+              int dtype, int bs_last, int act, int mode, hipStream_t s)
+{
+    const GatedArgs g{x, w, bias, dh, out, batch, a, b, c, d, act};
+    if (dtype == KSMM_F32) {
+        if (bs_last) return mode ? run<float, true, 1>(g, s) : run<float, true, 0>(g, s);
+        return mode ? run<float, false, 1>(g, s) : run<float, false, 0>(g, s);
+    }
+    if (bs_last) return mode ? run<half_t, true, 1>(g, s) : run<half_t, true, 0>(g, s);
+    return mode ? run<half_t, false, 1>(g, s) : run<half_t, false, 0>(g, s);
+}
+
+}  // namespace ksmm
+
+using namespace ksmm;
+
+namespace {
+
+int check(int64_t batch, int a, int b, int c, int d, int dtype, int act)
+{
+    if (b > 0x3fffffff) return KSMM_ERR_TOO_LARGE;
+    if (dtype != KSMM_F32 && dtype != KSMM_F16) return KSMM_ERR_BAD_DTYPE;
+    const int rc = ksmm_validate(batch, a, 2 * b, c, d, dtype, dtype, dtype, 0);
+    if (rc != KSMM_OK) return rc;
+    return act == KSMM_ACT_NONE || act == KSMM_ACT_GELU || act == KSMM_ACT_SILU ? KSMM_OK : KSMM_ERR_BAD_EPILOGUE;
+}
+
+int64_t align256(int64_t v) { return (v + 255) / 256 * 256; }
+
+}  // namespace
+
+extern "C" {
+
+int ksmm_gated_forward(const void *x, const void *w, const void *bias, void *h, int64_t batch, int a, int b, int c, int d, int dtype,
+                       int bs_last, int act, void *stream)
+{
+    const int rc = check(batch, a, b, c, d, dtype, act);
+    if (rc != KSMM_OK) return rc;
+    if (!x || !w || !h) return KSMM_ERR_NULL_POINTER;
+    return gated_run(x, w, bias, nullptr, h, batch, a, b, c, d, dtype, bs_last, act, 0, (hipStream_t)stream);
+}
+
+int64_t ksmm_gated_backward_workspace(int64_t batch, int a, int b, int c, int d, int dtype, int bs_last)
+{
+    const int rc = check(batch, a, b, c, d, dtype, KSMM_ACT_NONE);
+    if (rc != KSMM_OK) return rc;
+    const ksmm_factor_desc f{nullptr, a, 2 * b, c, d, dtype, 1.f};
+    const int64_t layer = ksmm_layer_backward_workspace(&f, 1, batch, dtype, bs_last, KSMM_ACT_NONE);
+    return layer < 0 ? layer : layer + align256(2 * (int64_t)a * b * d * batch * (int64_t)dtype_size(dtype));
+}
+
+int ksmm_gated_backward(const void *dh, const void *x, const void *w, const void *bias, void *dx, void *dw, void *dbias, void *workspace,
+                        int64_t workspace_bytes, int64_t batch, int a, int b, int c, int d, int dtype, int bs_last, int act, void *stream)
+{
+    int rc = check(batch, a, b, c, d, dtype, act);
+    if (rc != KSMM_OK) return rc;
+    if (!dh || !x || !w) return KSMM_ERR_NULL_POINTER;
+    const int64_t need = ksmm_gated_backward_workspace(batch, a, b, c, d, dtype, bs_last);
+    if (need < 0) return (int)need;
+    if (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15) != 0) return KSMM_ERR_WORKSPACE;
+    if (!dx && !dw && !dbias) return KSMM_OK;
+    rc = gated_run(x, w, bias, dh, workspace, batch, a, b, c, d, dtype, bs_last, act, 1, (hipStream_t)stream);
+    if (rc != KSMM_OK) return rc;
+    const int64_t dz = align256(2 * (int64_t)a * b * d * batch * (int64_t)dtype_size(dtype));
+    const ksmm_factor_desc f{w, a, 2 * b, c, d, dtype, 1.f};
+    return ksmm_layer_backward(&f, 1, &x, nullptr, workspace, dx, &dw, dbias, (char *)workspace + dz, workspace_bytes - dz, batch, dtype,
+                               bs_last, KSMM_ACT_NONE, stream);
+}
+
+}  // extern "C"

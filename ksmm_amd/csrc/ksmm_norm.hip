@@ -1,0 +1,876 @@
+// Norms around a residual connection: what follows a block, what precedes the next one, and the gated, scaled
+// addition between them in one pass over the tensors.
+//
+//     r' = r + alpha * gate * P(x)      P(x) = x, or norm(x) * post_weight
+//     n  = norm(r') * weight + bias     norm(t) = (t - mean) / sqrt(var + eps), or t / sqrt(mean(t^2) + eps)
+//
+// Backward, with u = norm(x) before its weight, v = norm(r') before its weight, rho the factors 1 / sqrt(..):
+//     dv = dn * weight,  D = dr' + rho_r (dv - v mean(dv v) - [mean(dv)])     ([..]: with a mean only)
+//     dr = D,  dgate = sum alpha D P(x),  dP = alpha gate D,  dpost = sum dP u,  dweight = sum dn v,  dbias = sum dn
+//     du = dP post_weight,  dx = rho_x (du - u mean(du u) - [mean(du)])
+// r' and v are computed again from x and r (the same bytes as reading r', and not rounded), the statistics (fp32,
+// four a row) come from the forward pass.
+//
+// What bounds it: HBM; four tensors forward, six backward.  Everything is computed in fp32; a tensor's values are
+// rounded once, when they are stored.  The sums over rows are fp32 partial sums that are added in a fixed order.
+#include "ksmm_common.h"
+#include "ksmm_norm.h"
+
+namespace ksmm {
+
+namespace {
+
+constexpr int MAX_WAVES = 16;
+
+// ---- sums over lanes ------------------------------------------------------------------------------
+template <int CTRL> __device__ __forceinline__ float dpp_add(float v)
+{
+    return v + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true));
+}
+// every lane of 16 gets the sum over the 16
+__device__ __forceinline__ float sum16(float v)
+{
+    v = dpp_add<0xB1>(v);   // the other one of a pair
+    v = dpp_add<0x4E>(v);   // the other pair of four
+    v = dpp_add<0x141>(v);  // the other four of eight, mirrored
+    return dpp_add<0x140>(v);
+}
+// every lane gets the sum over the wave
+__device__ __forceinline__ float sum64(float v)
+{
+    v = sum16(v);
+    auto lane = [&](int l) { return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), l)); };
+    return (lane(0) + lane(16)) + (lane(32) + lane(48));
+}
+
+// Sums over the TPR threads of a row.  Rows wider than a wave add up through LDS, two buffers in turn: one barrier a sum.
+template <int TPR> struct RowSum {
+    float *red;  // 2 x 2 x MAX_WAVES floats
+    int turn = 0;
+    __device__ __forceinline__ void two(float &a, float &b)
+    {
+        if constexpr (TPR == 16) {
+            a = sum16(a);
+            b = sum16(b);
+        } else {
+            a = sum64(a);
+            b = sum64(b);
+            if constexpr (TPR > 64) {
+                constexpr int W = TPR / 64;
+                float *const at = red + turn * 2 * MAX_WAVES;
+                turn ^= 1;
+                if ((threadIdx.x & 63) == 0) {
+                    at[threadIdx.x >> 6] = a;
+                    at[MAX_WAVES + (threadIdx.x >> 6)] = b;
+                }
+                __syncthreads();
+                a = b = 0.f;
+#pragma unroll
+                for (int i = 0; i < W; ++i) {
+                    a += at[i];
+                    b += at[MAX_WAVES + i];
+                }
+            }
+        }
+    }
+    __device__ __forceinline__ float one(float a)
+    {
+        float b = 0.f;
+        if constexpr (TPR == 16) return sum16(a);
+        if constexpr (TPR == 64) return sum64(a);
+        two(a, b);
+        return a;
+    }
+};
+
+// What a gradient dv of v = norm(t) leaves of itself: dv - v mean(dv v) - mean(dv), given the means.  (A row of one feature
+// has v^2 = 1 - eps rho^2 without a mean, which the difference would lose.)
+__device__ __forceinline__ float project(const NormArgs &a, float dv, float v, float m1, float m2, float rho)
+{
+    return a.features == 1 && !a.layer ? dv * (a.eps * rho * rho) : fmaf(-v, m2, dv) - m1;
+}
+
+// ---- 16 bytes of a row, at element alignment; past its end: zeros, and nothing stored --------------
+template <typename T> constexpr int EPV = 16 / (int)sizeof(T);
+template <typename T> union Piece {
+    uint4_t v;
+    T e[EPV<T>];
+};
+template <typename T> __device__ __forceinline__ Piece<T> load_piece(const T *row, int col, int end)
+{
+    Piece<T> p;
+    if (col + EPV<T> <= end) {
+        __builtin_memcpy(&p.v, row + col, 16);
+    } else {
+        p.v = uint4_t{0u, 0u, 0u, 0u};
+#pragma unroll
+        for (int e = 0; e < EPV<T>; ++e)
+            if (col + e < end) p.e[e] = row[col + e];
+    }
+    return p;
+}
+template <typename T> __device__ __forceinline__ void store_piece(T *row, int col, int end, const Piece<T> &p)
+{
+    if (col + EPV<T> <= end) {
+        __builtin_memcpy(row + col, &p.v, 16);
+    } else {
+#pragma unroll
+        for (int e = 0; e < EPV<T>; ++e)
+            if (col + e < end) row[col + e] = p.e[e];
+    }
+}
+
+// ---- batch-size-first -------------------------------------------------------------------------------
+// A row is held by TPR threads, VPL pieces each: TPR * VPL pieces are enough for it.  Rows are dealt in ranges: the
+// workgroup's row r of a range starts at range * range_rows.  (Threads past the end of a row hold zeros.)
+template <typename T, int TPR, int VPL>
+__global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void ks_norm_rows_kernel(NormArgs a, int64_t range_rows)
+{
+    constexpr int E = EPV<T>, ROWS = TPR < 256 ? 256 / TPR : 1;
+    __shared__ float red[4 * MAX_WAVES];
+    RowSum<TPR> sum{red};
+    const int t = threadIdx.x % TPR, H = a.features;
+    const float inv = 1.f / (float)H;
+    const T *x = (const T *)a.x, *res = (const T *)a.residual, *gate = (const T *)a.gate, *post = (const T *)a.post_weight;
+    const int64_t first = (int64_t)blockIdx.x * range_rows, last = min(a.batch, first + range_rows);
+    Piece<T> w[VPL], b[VPL], pw[VPL], g[VPL];
+    int64_t group = -1;
+#pragma unroll
+    for (int j = 0; j < VPL; ++j) {
+        const int col = (j * TPR + t) * E;
+        if (a.n_out && a.weight) w[j] = load_piece<T>((const T *)a.weight, col, H);
+        if (a.n_out && a.bias) b[j] = load_piece<T>((const T *)a.bias, col, H);
+        if (x && post) pw[j] = load_piece<T>(post, col, H);
+    }
+    // (rows of a workgroup wider than a wave add up behind barriers: all of its threads take the same ones)
+    for (int64_t row = first + threadIdx.x / TPR; row < last; row += ROWS) {
+        Piece<T> rp[VPL], xp[VPL];
+#pragma unroll
+        for (int j = 0; j < VPL; ++j) {
+            const int col = (j * TPR + t) * E;
+            rp[j] = load_piece<T>(res + row * H, col, H);
+            if (x) xp[j] = load_piece<T>(x + row * H, col, H);
+        }
+        if (x && gate && row / a.group_rows != group) {
+            group = row / a.group_rows;
+#pragma unroll
+            for (int j = 0; j < VPL; ++j) g[j] = load_piece<T>(gate + group * H, (j * TPR + t) * E, H);
+        }
+        float r[VPL][E];
+        float mean_x = 0.f, rho_x = 1.f;
+        if (x) {
+            if (post) {
+                if (a.layer) {
+                    float s = 0.f;
+#pragma unroll
+                    for (int j = 0; j < VPL; ++j)
+#pragma unroll
+                        for (int e = 0; e < E; ++e) s += (float)xp[j].e[e];
+                    mean_x = sum.one(s) * inv;
+                }
+                float s = 0.f;
+#pragma unroll
+                for (int j = 0; j < VPL; ++j)
+#pragma unroll
+                    for (int e = 0; e < E; ++e) {
+                        const float c = (j * TPR + t) * E + e < H ? (float)xp[j].e[e] - mean_x : 0.f;
+                        s = fmaf(c, c, s);
+                    }
+                rho_x = rsqrtf(fmaf(sum.one(s), inv, a.eps));
+            }
+#pragma unroll
+            for (int j = 0; j < VPL; ++j)
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    float p = (float)xp[j].e[e];
+                    if (post) p = (p - mean_x) * rho_x * (float)pw[j].e[e];
+                    r[j][e] = fmaf(gate ? a.alpha * (float)g[j].e[e] : a.alpha, p, (float)rp[j].e[e]);
+                }
+            if (a.r_out) {
+#pragma unroll
+                for (int j = 0; j < VPL; ++j) {
+                    Piece<T> o;
+#pragma unroll
+                    for (int e = 0; e < E; ++e) o.e[e] = (T)r[j][e];
+                    store_piece<T>((T *)a.r_out + row * H, (j * TPR + t) * E, H, o);
+                }
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < VPL; ++j)
+#pragma unroll
+                for (int e = 0; e < E; ++e) r[j][e] = (float)rp[j].e[e];
+        }
+        float mean_r = 0.f, rho_r = 1.f;
+        if (a.n_out) {
+            if (a.layer) {
+                float s = 0.f;
+#pragma unroll
+                for (int j = 0; j < VPL; ++j)
+#pragma unroll
+                    for (int e = 0; e < E; ++e) s += r[j][e];  // (zeros past the end: x and r are)
+                mean_r = sum.one(s) * inv;
+            }
+            float s = 0.f;
+#pragma unroll
+            for (int j = 0; j < VPL; ++j)
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    const float c = (j * TPR + t) * E + e < H ? r[j][e] - mean_r : 0.f;
+                    s = fmaf(c, c, s);
+                }
+            rho_r = rsqrtf(fmaf(sum.one(s), inv, a.eps));
+#pragma unroll
+            for (int j = 0; j < VPL; ++j) {
+                Piece<T> o;
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    float v = (r[j][e] - mean_r) * rho_r;
+                    if (a.weight) v *= (float)w[j].e[e];
+                    if (a.bias) v += (float)b[j].e[e];
+                    o.e[e] = (T)v;
+                }
+                store_piece<T>((T *)a.n_out + row * H, (j * TPR + t) * E, H, o);
+            }
+        }
+        if (a.stats && t == 0) {
+            a.stats[row] = mean_x;
+            a.stats[a.batch + row] = rho_x;
+            a.stats[2 * a.batch + row] = mean_r;
+            a.stats[3 * a.batch + row] = rho_r;
+        }
+    }
+}
+
+// Gradients.  Workgroup = range of rows: `parts` ranges share a gate's group, or a range is `groups_per` whole groups
+// (parts == 1).  Partial sums: slice blockIdx.x of each quantity; dgate's lie [part][group][feature].
+template <typename T, int TPR, int VPL>
+__global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void ks_norm_rows_bwd_kernel(NormArgs a, NormGrads d, NormSplit sp)
+{
+    constexpr int E = EPV<T>, ROWS = TPR < 256 ? 256 / TPR : 1, WIDE = VPL * E;
+    __shared__ float red[4 * MAX_WAVES];
+    __shared__ float wide[ROWS > 1 ? 256 * WIDE : 1];
+    RowSum<TPR> sum{red};
+    const int t = threadIdx.x % TPR, slot = threadIdx.x / TPR, H = a.features;
+    const float inv = 1.f / (float)H;
+    const T *x = (const T *)a.x, *gate = (const T *)a.gate, *post = (const T *)a.post_weight;
+    const T *dr_in = (const T *)d.dr_out, *dn = (const T *)d.dn_out;
+    Piece<T> w[VPL], pw[VPL], g[VPL];
+#pragma unroll
+    for (int j = 0; j < VPL; ++j) {
+        const int col = (j * TPR + t) * E;
+        if (dn && a.weight) w[j] = load_piece<T>((const T *)a.weight, col, H);
+        if (x && post) pw[j] = load_piece<T>(post, col, H);
+    }
+    float s_w[WIDE], s_b[WIDE], s_p[WIDE], s_g[WIDE];
+#pragma unroll
+    for (int i = 0; i < WIDE; ++i) s_w[i] = s_b[i] = s_p[i] = s_g[i] = 0.f;
+
+    // the workgroup's sum of one quantity, stored to a row of floats
+    auto flush = [&](const float *s, float *to) {
+        if constexpr (ROWS > 1) {
+#pragma unroll
+            for (int i = 0; i < WIDE; ++i) wide[i * 256 + threadIdx.x] = s[i];
+            __syncthreads();
+            for (int i = threadIdx.x; i < TPR * WIDE; i += 256) {
+                const int tt = i % TPR, k = i / TPR, col = (k / E * TPR + tt) * E + k % E;
+                float v = 0.f;
+#pragma unroll
+                for (int q = 0; q < ROWS; ++q) v += wide[k * 256 + q * TPR + tt];
+                if (col < H) to[col] = v;
+            }
+            __syncthreads();
+        } else {
+#pragma unroll
+            for (int j = 0; j < VPL; ++j)
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    const int col = (j * TPR + t) * E + e;
+                    if (col < H) to[col] = s[j * E + e];
+                }
+        }
+    };
+
+    const int64_t unit = (int64_t)blockIdx.x / sp.parts;
+    const int part = (int)(blockIdx.x - unit * sp.parts);
+    const int64_t g_first = unit * sp.groups_per, g_last = min(sp.groups, g_first + sp.groups_per);
+    for (int64_t group = g_first; group < g_last; ++group) {
+        const int64_t base = group * a.group_rows, first = base + part * sp.part_rows;
+        const int64_t last = min(base + a.group_rows, first + sp.part_rows);
+        if (x && gate) {
+#pragma unroll
+            for (int j = 0; j < VPL; ++j) g[j] = load_piece<T>(gate + (sp.one_gate ? 0 : group * H), (j * TPR + t) * E, H);
+        }
+        for (int64_t row = first + slot; row < last; row += ROWS) {
+            Piece<T> rp[VPL], xp[VPL], np[VPL], dp[VPL];
+#pragma unroll
+            for (int j = 0; j < VPL; ++j) {
+                const int col = (j * TPR + t) * E;
+                if (dn) {
+                    np[j] = load_piece<T>(dn + row * H, col, H);
+                    rp[j] = load_piece<T>((const T *)a.residual + row * H, col, H);
+                }
+                if (x) xp[j] = load_piece<T>(x + row * H, col, H);
+                if (dr_in) dp[j] = load_piece<T>(dr_in + row * H, col, H);
+            }
+            const float mean_x = a.stats[row], rho_x = a.stats[a.batch + row];
+            const float mean_r = a.stats[2 * a.batch + row], rho_r = a.stats[3 * a.batch + row];
+            float u[VPL][E], D[VPL][E];
+#pragma unroll
+            for (int j = 0; j < VPL; ++j)
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    u[j][e] = 0.f;
+                    if (x) u[j][e] = post ? ((float)xp[j].e[e] - mean_x) * rho_x : (float)xp[j].e[e];
+                    D[j][e] = dr_in ? (float)dp[j].e[e] : 0.f;
+                }
+            if (dn) {
+                float v[VPL][E], dv[VPL][E], m1 = 0.f, m2 = 0.f;
+#pragma unroll
+                for (int j = 0; j < VPL; ++j)
+#pragma unroll
+                    for (int e = 0; e < E; ++e) {
+                        const float p = x ? (post ? u[j][e] * (float)pw[j].e[e] : u[j][e]) : 0.f;
+                        const float r = x ? fmaf(gate ? a.alpha * (float)g[j].e[e] : a.alpha, p, (float)rp[j].e[e]) : (float)rp[j].e[e];
+                        const float n = (float)np[j].e[e];  // (zero past the end, and so is what it multiplies)
+                        v[j][e] = (r - mean_r) * rho_r;
+                        dv[j][e] = a.weight ? n * (float)w[j].e[e] : n;
+                        m1 += dv[j][e];
+                        m2 = fmaf(dv[j][e], v[j][e], m2);
+                        s_w[j * E + e] = fmaf(n, v[j][e], s_w[j * E + e]);
+                        s_b[j * E + e] += n;
+                    }
+                sum.two(m1, m2);
+                m1 = a.layer ? m1 * inv : 0.f;
+                m2 *= inv;
+#pragma unroll
+                for (int j = 0; j < VPL; ++j)
+#pragma unroll
+                    for (int e = 0; e < E; ++e) D[j][e] = fmaf(rho_r, project(a, dv[j][e], v[j][e], m1, m2, rho_r), D[j][e]);
+            }
+            if (d.dresidual) {
+#pragma unroll
+                for (int j = 0; j < VPL; ++j) {
+                    Piece<T> o;
+#pragma unroll
+                    for (int e = 0; e < E; ++e) o.e[e] = (T)D[j][e];
+                    store_piece<T>((T *)d.dresidual + row * H, (j * TPR + t) * E, H, o);
+                }
+            }
+            if (x && (d.dx || d.dgate || d.dpost_weight)) {
+                float m1 = 0.f, m2 = 0.f;
+#pragma unroll
+                for (int j = 0; j < VPL; ++j)
+#pragma unroll
+                    for (int e = 0; e < E; ++e) {
+                        // (past the end D holds the rest of a mean: nothing may be added there)
+                        const float D0 = (j * TPR + t) * E + e < H ? D[j][e] : 0.f;
+                        const float p = post ? u[j][e] * (float)pw[j].e[e] : u[j][e];
+                        s_g[j * E + e] = fmaf(a.alpha * D0, p, s_g[j * E + e]);
+                        float q = (gate ? a.alpha * (float)g[j].e[e] : a.alpha) * D0;
+                        if (post) {
+                            s_p[j * E + e] = fmaf(q, u[j][e], s_p[j * E + e]);
+                            q *= (float)pw[j].e[e];
+                            m1 += q;
+                            m2 = fmaf(q, u[j][e], m2);
+                        }
+                        D[j][e] = q;
+                    }
+                if (post) {
+                    sum.two(m1, m2);
+                    m1 = a.layer ? m1 * inv : 0.f;
+                    m2 *= inv;
+                }
+                if (d.dx) {
+#pragma unroll
+                    for (int j = 0; j < VPL; ++j) {
+                        Piece<T> o;
+#pragma unroll
+                        for (int e = 0; e < E; ++e) o.e[e] = (T)(post ? rho_x * project(a, D[j][e], u[j][e], m1, m2, rho_x) : D[j][e]);
+                        store_piece<T>((T *)d.dx + row * H, (j * TPR + t) * E, H, o);
+                    }
+                }
+            }
+        }
+        if (d.dgate && !sp.one_gate) {
+            flush(s_g, d.dgate + ((int64_t)part * sp.groups + group) * H);
+#pragma unroll
+            for (int i = 0; i < WIDE; ++i) s_g[i] = 0.f;
+        }
+    }
+    if (d.dweight) flush(s_w, d.dweight + (int64_t)blockIdx.x * H);
+    if (d.dbias) flush(s_b, d.dbias + (int64_t)blockIdx.x * H);
+    if (d.dpost_weight) flush(s_p, d.dpost_weight + (int64_t)blockIdx.x * H);
+    if (d.dgate && sp.one_gate) flush(s_g, d.dgate + (int64_t)blockIdx.x * H);
+}
+
+// ---- batch-size-last --------------------------------------------------------------------------------
+// A workgroup takes CT neighbouring rows of the batch (columns of the tensors) and all features: thread = one column
+// and every GROUPS-th feature.  FPT > 0: a thread's values of a tensor (at most FPT) stay in registers; FPT == 0, for
+// any number of features: they are read again for each of the passes that the statistics need.
+template <int CT, int GROUPS> struct ColSum {
+    float *red;  // 2 x GROUPS x CT floats
+    __device__ __forceinline__ void two(float &a, float &b)
+    {
+        const int col = threadIdx.x % CT, grp = threadIdx.x / CT;
+        __syncthreads();
+        red[grp * CT + col] = a;
+        red[(GROUPS + grp) * CT + col] = b;
+        __syncthreads();
+        a = b = 0.f;
+        for (int i = 0; i < GROUPS; ++i) {
+            a += red[i * CT + col];
+            b += red[(GROUPS + i) * CT + col];
+        }
+    }
+    __device__ __forceinline__ float one(float a)
+    {
+        float b = 0.f;
+        two(a, b);
+        return a;
+    }
+};
+// the sum over the CT lanes side by side that hold one feature
+template <int CT> __device__ __forceinline__ float sum_lanes(float v)
+{
+    v = sum16(v);
+    if constexpr (CT > 16) v += __shfl_xor(v, 16, 64);
+    if constexpr (CT > 32) v += __shfl_xor(v, 32, 64);
+    return v;
+}
+
+template <typename T, int CT, int THREADS, int FPT>
+__global__ __launch_bounds__(THREADS) void ks_norm_cols_kernel(NormArgs a)
+{
+    constexpr int GROUPS = THREADS / CT, N = FPT > 0 ? FPT : 1;
+    __shared__ float red[2 * THREADS];
+    ColSum<CT, GROUPS> sum{red};
+    const int H = a.features, grp = threadIdx.x / CT;
+    const int64_t B = a.batch, col = (int64_t)blockIdx.x * CT + threadIdx.x % CT;
+    const bool in = col < B;
+    const float inv = 1.f / (float)H;
+    const T *x = (const T *)a.x, *res = (const T *)a.residual, *post = (const T *)a.post_weight;
+    const T *gate = a.gate ? (const T *)a.gate + (in ? col / a.group_rows : 0) * H : nullptr;
+    float xv[N], rv[N];
+    // every feature of the thread in turn
+    auto each = [&](auto f) {
+        if constexpr (FPT > 0) {
+#pragma unroll
+            for (int i = 0; i < FPT; ++i)
+                if (in && grp + i * GROUPS < H) f(i, grp + i * GROUPS);
+        } else if (in) {
+            for (int h = grp; h < H; h += GROUPS) f(0, h);
+        }
+    };
+    if constexpr (FPT > 0) {
+        each([&](int i, int h) {
+            rv[i] = (float)res[h * B + col];
+            if (x) xv[i] = (float)x[h * B + col];
+        });
+    }
+    auto get_x = [&](int i, int h) { return FPT > 0 ? xv[i] : (float)x[h * B + col]; };
+    float mean_x = 0.f, rho_x = 1.f, mean_r = 0.f, rho_r = 1.f;
+    if (x && post) {
+        if (a.layer) {
+            float s = 0.f;
+            each([&](int i, int h) { s += get_x(i, h); });
+            mean_x = sum.one(s) * inv;
+        }
+        float s = 0.f;
+        each([&](int i, int h) {
+            const float c = get_x(i, h) - mean_x;
+            s = fmaf(c, c, s);
+        });
+        rho_x = rsqrtf(fmaf(sum.one(s), inv, a.eps));
+    }
+    auto get_r = [&](int i, int h) {  // r', from the inputs
+        float r = FPT > 0 ? rv[i] : (float)res[h * B + col];
+        if (x) {
+            float p = get_x(i, h);
+            if (post) p = (p - mean_x) * rho_x * (float)post[h];
+            r = fmaf(gate ? a.alpha * (float)gate[h] : a.alpha, p, r);
+        }
+        return r;
+    };
+    float s = 0.f;
+    each([&](int i, int h) {
+        const float r = get_r(i, h);
+        if constexpr (FPT > 0) rv[i] = r;
+        if (x && a.r_out) ((T *)a.r_out)[h * B + col] = (T)r;
+        s += a.layer ? r : r * r;
+    });
+    if (a.n_out) {
+        auto again = [&](int i, int h) { return FPT > 0 ? rv[i] : get_r(i, h); };
+        s = sum.one(s) * inv;
+        if (a.layer) {
+            mean_r = s;
+            s = 0.f;
+            each([&](int i, int h) {
+                const float c = again(i, h) - mean_r;
+                s = fmaf(c, c, s);
+            });
+            s = sum.one(s) * inv;
+        }
+        rho_r = rsqrtf(s + a.eps);
+        each([&](int i, int h) {
+            float v = (again(i, h) - mean_r) * rho_r;
+            if (a.weight) v *= (float)((const T *)a.weight)[h];
+            if (a.bias) v += (float)((const T *)a.bias)[h];
+            ((T *)a.n_out)[h * B + col] = (T)v;
+        });
+    }
+    if (a.stats && in && grp == 0) {
+        a.stats[col] = mean_x;
+        a.stats[B + col] = rho_x;
+        a.stats[2 * B + col] = mean_r;
+        a.stats[3 * B + col] = rho_r;
+    }
+}
+
+template <typename T, int CT, int THREADS, int FPT>
+__global__ __launch_bounds__(THREADS) void ks_norm_cols_bwd_kernel(NormArgs a, NormGrads d)
+{
+    constexpr int GROUPS = THREADS / CT, N = FPT > 0 ? FPT : 1;
+    __shared__ float red[2 * THREADS];
+    ColSum<CT, GROUPS> sum{red};
+    const int H = a.features, grp = threadIdx.x / CT;
+    const int64_t B = a.batch, col = (int64_t)blockIdx.x * CT + threadIdx.x % CT, at = col < B ? col : B - 1;
+    const bool in = col < B;
+    const float inv = 1.f / (float)H;
+    const T *x = (const T *)a.x, *res = (const T *)a.residual, *post = (const T *)a.post_weight;
+    const T *gate = a.gate ? (const T *)a.gate + at / a.group_rows * H : nullptr;
+    const T *dr_in = (const T *)d.dr_out, *dn = (const T *)d.dn_out;
+    const float mean_x = a.stats[at], rho_x = a.stats[B + at], mean_r = a.stats[2 * B + at], rho_r = a.stats[3 * B + at];
+    float uv[N], vv[N], nv[N], dv_[N];
+    // every feature of the thread in turn, columns past the end too (their values count as zero: lanes add up)
+    auto each = [&](auto f) {
+        if constexpr (FPT > 0) {
+#pragma unroll
+            for (int i = 0; i < FPT; ++i)
+                if (grp + i * GROUPS < H) f(i, grp + i * GROUPS);
+        } else {
+            for (int h = grp; h < H; h += GROUPS) f(0, h);
+        }
+    };
+    auto load_u = [&](int h) { return !x ? 0.f : post ? ((float)x[h * B + at] - mean_x) * rho_x : (float)x[h * B + at]; };
+    auto load_v = [&](int h, float u) {
+        float r = (float)res[h * B + at];
+        if (x) r = fmaf(gate ? a.alpha * (float)gate[h] : a.alpha, post ? u * (float)post[h] : u, r);
+        return (r - mean_r) * rho_r;
+    };
+    if constexpr (FPT > 0) {
+        each([&](int i, int h) {
+            uv[i] = load_u(h);
+            if (dn) {
+                vv[i] = load_v(h, uv[i]);
+                nv[i] = in ? (float)dn[h * B + at] : 0.f;
+            }
+            dv_[i] = dr_in ? (float)dr_in[h * B + at] : 0.f;
+        });
+    }
+    auto get_u = [&](int i, int h) { return FPT > 0 ? uv[i] : load_u(h); };
+    auto get_v = [&](int i, int h, float u) { return FPT > 0 ? vv[i] : load_v(h, u); };
+    auto get_n = [&](int i, int h) { return FPT > 0 ? nv[i] : in ? (float)dn[h * B + at] : 0.f; };
+    float m1 = 0.f, m2 = 0.f;
+    if (dn) {
+        each([&](int i, int h) {
+            const float v = get_v(i, h, get_u(i, h)), n = get_n(i, h), dv = a.weight ? n * (float)((const T *)a.weight)[h] : n;
+            m1 += dv;
+            m2 = fmaf(dv, v, m2);
+            if (d.dweight) {
+                const float q = sum_lanes<CT>(n * v);
+                if (threadIdx.x % CT == 0) d.dweight[(int64_t)blockIdx.x * H + h] = q;
+            }
+            if (d.dbias) {
+                const float q = sum_lanes<CT>(n);
+                if (threadIdx.x % CT == 0) d.dbias[(int64_t)blockIdx.x * H + h] = q;
+            }
+        });
+        sum.two(m1, m2);
+        m1 = a.layer ? m1 * inv : 0.f;
+        m2 *= inv;
+    }
+    // D of one feature
+    auto get_D = [&](int i, int h, float u) {
+        float D = FPT > 0 ? dv_[i] : dr_in ? (float)dr_in[h * B + at] : 0.f;
+        if (dn) {
+            const float n = get_n(i, h), dv = a.weight ? n * (float)((const T *)a.weight)[h] : n;
+            D = fmaf(rho_r, project(a, dv, get_v(i, h, u), m1, m2, rho_r), D);
+        }
+        return in ? D : 0.f;
+    };
+    float k1 = 0.f, k2 = 0.f;
+    each([&](int i, int h) {
+        const float u = get_u(i, h), D = get_D(i, h, u);
+        if (d.dresidual && in) ((T *)d.dresidual)[h * B + col] = (T)D;
+        if (!x) return;
+        const float pw = post ? (float)post[h] : 1.f;
+        float q = (gate ? a.alpha * (float)gate[h] : a.alpha) * D;
+        if (d.dgate) {
+            const float s = sum_lanes<CT>(a.alpha * D * (post ? u * pw : u));
+            if (threadIdx.x % CT == 0) d.dgate[(int64_t)blockIdx.x * H + h] = s;
+        }
+        if (post) {
+            if (d.dpost_weight) {
+                const float s = sum_lanes<CT>(q * u);
+                if (threadIdx.x % CT == 0) d.dpost_weight[(int64_t)blockIdx.x * H + h] = s;
+            }
+            q *= pw;
+            k1 += q;
+            k2 = fmaf(q, u, k2);
+        }
+        if constexpr (FPT > 0) dv_[i] = q;
+        if (!post && d.dx && in) ((T *)d.dx)[h * B + col] = (T)q;
+    });
+    if (x && post && d.dx) {
+        sum.two(k1, k2);
+        k1 = a.layer ? k1 * inv : 0.f;
+        k2 *= inv;
+        each([&](int i, int h) {
+            const float u = get_u(i, h);
+            float q;
+            if constexpr (FPT > 0)
+                q = dv_[i];
+            else
+                q = (gate ? a.alpha * (float)gate[h] : a.alpha) * get_D(i, h, u) * (float)post[h];
+            if (in) ((T *)d.dx)[h * B + col] = (T)(rho_x * project(a, q, u, k1, k2, rho_x));
+        });
+    }
+}
+
+// Gradients of gates that belong to groups of columns: a wave sums a feature over a group, from the stored dr.
+template <typename T>
+__global__ __launch_bounds__(256) void ks_norm_cols_gate_kernel(NormArgs a, const T *__restrict__ dr, T *__restrict__ dgate, int64_t groups)
+{
+    const int64_t wave = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6), B = a.batch;
+    const int64_t group = wave / a.features;
+    const int h = (int)(wave - group * a.features);
+    if (group >= groups) return;
+    const T *x = (const T *)a.x, *post = (const T *)a.post_weight;
+    const float pw = post ? (float)post[h] : 1.f;
+    float s = 0.f;
+    for (int64_t c = group * a.group_rows + (threadIdx.x & 63); c < (group + 1) * a.group_rows; c += 64) {
+        float p = (float)x[h * B + c];
+        if (post) p = (p - a.stats[c]) * a.stats[B + c] * pw;
+        s = fmaf((float)dr[h * B + c], p, s);
+    }
+    s = sum64(s);
+    if ((threadIdx.x & 63) == 0) dgate[group * a.features + h] = (T)(a.alpha * s);
+}
+
+// ---- choices ------------------------------------------------------------------------------------------
+// ranges of rows that fill the chip: workgroups of 4 waves, 2 of which fit a CU in the backward pass
+constexpr int64_t FWD_RANGES = 2048, BWD_RANGES = 768;
+// widest batch-size-first row that the kernels hold (elements of 4 bytes)
+constexpr int64_t WIDEST = 8192;
+
+int row_threads(int64_t features, int dtype)
+{
+    const int64_t pieces = (features * (int64_t)dtype_size(dtype) + 15) / 16;
+    return pieces <= 16 ? 16 : pieces <= 128 ? 64 : pieces <= 512 ? 256 : pieces <= 2048 ? 1024 : 0;
+}
+
+template <typename T, typename F> int with_rows(int64_t features, int dtype, F f)
+{
+    const int tpr = row_threads(features, dtype);
+    const bool one = features * (int64_t)sizeof(T) <= (int64_t)tpr * 16;
+    switch (tpr) {
+    case 16: return f(std::integral_constant<int, 16>(), std::integral_constant<int, 1>());
+    case 64: return one ? f(std::integral_constant<int, 64>(), std::integral_constant<int, 1>()) : f(std::integral_constant<int, 64>(), std::integral_constant<int, 2>());
+    case 256: return one ? f(std::integral_constant<int, 256>(), std::integral_constant<int, 1>()) : f(std::integral_constant<int, 256>(), std::integral_constant<int, 2>());
+    case 1024: return one ? f(std::integral_constant<int, 1024>(), std::integral_constant<int, 1>()) : f(std::integral_constant<int, 1024>(), std::integral_constant<int, 2>());
+    }
+    return KSMM_ERR_TOO_LARGE;
+}
+
+constexpr int COLS = 32, COL_THREADS = 512;
+template <typename F> int with_cols(int64_t features, F f)
+{
+    const int64_t per = (features + COL_THREADS / COLS - 1) / (COL_THREADS / COLS);
+    if (per <= 8) return f(std::integral_constant<int, 8>());
+    if (per <= 24) return f(std::integral_constant<int, 24>());
+    if (per <= 48) return f(std::integral_constant<int, 48>());
+    return f(std::integral_constant<int, 0>());
+}
+
+NormSplit split_rows(int64_t batch, int64_t groups)
+{
+    NormSplit s;
+    s.one_gate = groups <= 1;
+    s.groups = groups < 1 ? 1 : groups;
+    const int64_t rows = batch / s.groups;
+    s.parts = (int)std::max<int64_t>(1, std::min<int64_t>(BWD_RANGES / s.groups, (rows + 7) / 8));
+    s.part_rows = (rows + s.parts - 1) / s.parts;
+    s.parts = (int)((rows + s.part_rows - 1) / s.part_rows);
+    s.groups_per = s.parts > 1 ? 1 : (s.groups + BWD_RANGES - 1) / BWD_RANGES;
+    s.ranges = (s.groups + s.groups_per - 1) / s.groups_per * s.parts;
+    return s;
+}
+
+int launched() { return hipGetLastError() == hipSuccess ? KSMM_OK : KSMM_ERR_LAUNCH; }
+
+template <typename T> int forward(const NormArgs &a, int dtype, int bs_last, hipStream_t stream)
+{
+    if (bs_last)
+        return with_cols(a.features, [&](auto fpt) {
+            hipLaunchKernelGGL((ks_norm_cols_kernel<T, COLS, COL_THREADS, decltype(fpt)::value>), dim3((unsigned)((a.batch + COLS - 1) / COLS)),
+                               dim3(COL_THREADS), 0, stream, a);
+            return launched();
+        });
+    return with_rows<T>(a.features, dtype, [&](auto tpr, auto vpl) {
+        constexpr int TPR = decltype(tpr)::value, ROWS = TPR < 256 ? 256 / TPR : 1;
+        const int64_t steps = (a.batch + ROWS - 1) / ROWS, per = (steps + FWD_RANGES - 1) / FWD_RANGES * ROWS;
+        hipLaunchKernelGGL((ks_norm_rows_kernel<T, TPR, decltype(vpl)::value>), dim3((unsigned)((a.batch + per - 1) / per)),
+                           dim3(TPR < 256 ? 256 : TPR), 0, stream, a, per);
+        return launched();
+    });
+}
+
+template <typename T> int backward(const NormArgs &a, const NormGrads &partial, const NormSplit &sp, int dtype, int bs_last, hipStream_t stream)
+{
+    if (bs_last)
+        return with_cols(a.features, [&](auto fpt) {
+            hipLaunchKernelGGL((ks_norm_cols_bwd_kernel<T, COLS, COL_THREADS, decltype(fpt)::value>), dim3((unsigned)((a.batch + COLS - 1) / COLS)),
+                               dim3(COL_THREADS), 0, stream, a, partial);
+            return launched();
+        });
+    return with_rows<T>(a.features, dtype, [&](auto tpr, auto vpl) {
+        constexpr int TPR = decltype(tpr)::value;
+        hipLaunchKernelGGL((ks_norm_rows_bwd_kernel<T, TPR, decltype(vpl)::value>), dim3((unsigned)sp.ranges), dim3(TPR < 256 ? 256 : TPR), 0,
+                           stream, a, partial, sp);
+        return launched();
+    });
+}
+
+int64_t align256(int64_t v) { return (v + 255) / 256 * 256; }
+
+// where the partial sums of each quantity lie
+struct Layout {
+    int64_t slices, slice_bytes, gate_bytes, total;
+    NormSplit split;
+};
+Layout layout(int64_t batch, int64_t features, int64_t groups, int bs_last)
+{
+    Layout l;
+    l.split = split_rows(batch, groups);
+    l.slices = bs_last ? (batch + COLS - 1) / COLS : l.split.ranges;
+    l.slice_bytes = align256(4 * l.slices * features);
+    l.gate_bytes = l.split.one_gate ? l.slice_bytes : bs_last ? 0 : align256(4 * l.split.parts * l.split.groups * features);
+    l.total = 3 * l.slice_bytes + l.gate_bytes;
+    return l;
+}
+
+int check(const ksmm_norm_desc *d, int64_t batch, int64_t features, int dtype, int bs_last)
+{
+    if (!d) return KSMM_ERR_NULL_POINTER;
+    if (batch < 1 || features < 1 || d->groups < 1 || batch % d->groups) return KSMM_ERR_BAD_BATCH;
+    if (dtype != KSMM_F32 && dtype != KSMM_F16) return KSMM_ERR_BAD_DTYPE;
+    if (d->kind != KSMM_NORM_RMS && d->kind != KSMM_NORM_LAYER) return KSMM_ERR_BAD_EPILOGUE;
+    if (!d->residual) return KSMM_ERR_NULL_POINTER;
+    if (features > (bs_last ? 0x7fffffffLL / 64 : WIDEST * 4 / (int64_t)dtype_size(dtype))) return KSMM_ERR_TOO_LARGE;
+    if (batch > (1LL << 31) || batch * features > (1LL << 40)) return KSMM_ERR_TOO_LARGE;
+    return KSMM_OK;
+}
+
+NormArgs args_of(const ksmm_norm_desc *d, int64_t batch, int64_t features)
+{
+    NormArgs a;
+    a.x = d->x;
+    a.residual = d->residual;
+    a.gate = d->x ? d->gate : nullptr;
+    a.post_weight = d->x ? d->post_weight : nullptr;
+    a.weight = d->weight;
+    a.bias = d->bias;
+    a.alpha = d->alpha;
+    a.eps = d->eps;
+    a.layer = d->kind == KSMM_NORM_LAYER;
+    a.batch = batch;
+    a.features = (int)features;
+    a.group_rows = batch / d->groups;
+    return a;
+}
+
+}  // namespace
+
+}  // namespace ksmm
+
+using namespace ksmm;
+
+extern "C" {
+
+int ksmm_residual_norm_forward(const ksmm_norm_desc *desc, void *r_out, void *n_out, float *stats, int64_t batch, int64_t features,
+                               int dtype, int bs_last, void *stream)
+{
+    const int rc = check(desc, batch, features, dtype, bs_last);
+    if (rc != KSMM_OK) return rc;
+    if ((desc->x && !r_out) || (!desc->x && !n_out)) return KSMM_ERR_NULL_POINTER;
+    NormArgs a = args_of(desc, batch, features);
+    a.r_out = desc->x ? r_out : nullptr;
+    a.n_out = n_out;
+    a.stats = stats;
+    return dtype == KSMM_F32 ? forward<float>(a, dtype, bs_last, (hipStream_t)stream) : forward<half_t>(a, dtype, bs_last, (hipStream_t)stream);
+}
+
+int64_t ksmm_residual_norm_backward_workspace(int64_t batch, int64_t features, int64_t groups, int dtype, int bs_last)
+{
+    if (batch < 1 || features < 1 || groups < 1 || batch % groups) return KSMM_ERR_BAD_BATCH;
+    if (dtype != KSMM_F32 && dtype != KSMM_F16) return KSMM_ERR_BAD_DTYPE;
+    return layout(batch, features, groups, bs_last).total;
+}
+
+int ksmm_residual_norm_backward(const ksmm_norm_desc *desc, const float *stats, const void *dr_out, const void *dn_out, void *dx,
+                                void *dresidual, void *dgate, void *dpost_weight, void *dweight, void *dbias, void *workspace,
+                                int64_t workspace_bytes, int64_t batch, int64_t features, int dtype, int bs_last, void *stream)
+{
+    const int rc = check(desc, batch, features, dtype, bs_last);
+    if (rc != KSMM_OK) return rc;
+    if (!stats || (!dr_out && !dn_out)) return KSMM_ERR_NULL_POINTER;
+    if ((!desc->x && (dx || dgate || dpost_weight)) || (dgate && !desc->gate) || (dpost_weight && !desc->post_weight) ||
+        (dweight && !desc->weight) || (dbias && !desc->bias))
+        return KSMM_ERR_NULL_POINTER;
+    const Layout l = layout(batch, features, desc->groups, bs_last);
+    if (!workspace || workspace_bytes < l.total || ((uintptr_t)workspace & 15) != 0) return KSMM_ERR_WORKSPACE;
+    const bool gate_alone = dgate && bs_last && !l.split.one_gate;
+    if (gate_alone && !dresidual) return KSMM_ERR_NULL_POINTER;  // its sums read it
+    const hipStream_t s = (hipStream_t)stream;
+    NormArgs a = args_of(desc, batch, features);
+    a.stats = (float *)stats;
+    char *const ws = (char *)workspace;
+    NormGrads p;
+    p.dr_out = dr_out;
+    p.dn_out = dn_out;
+    p.dx = dx;
+    p.dresidual = dresidual;
+    p.dweight = dweight && dn_out ? (float *)ws : nullptr;
+    p.dbias = dbias && dn_out ? (float *)(ws + l.slice_bytes) : nullptr;
+    p.dpost_weight = dpost_weight ? (float *)(ws + 2 * l.slice_bytes) : nullptr;
+    p.dgate = dgate && !gate_alone ? (float *)(ws + 3 * l.slice_bytes) : nullptr;
+    int st = dtype == KSMM_F32 ? backward<float>(a, p, l.split, dtype, bs_last, s) : backward<half_t>(a, p, l.split, dtype, bs_last, s);
+    if (st != KSMM_OK) return st;
+    if (gate_alone) {
+        const unsigned blocks = (unsigned)((l.split.groups * features + 3) / 4);
+        if (dtype == KSMM_F32)
+            hipLaunchKernelGGL((ks_norm_cols_gate_kernel<float>), dim3(blocks), dim3(256), 0, s, a, (const float *)dresidual, (float *)dgate, l.split.groups);
+        else
+            hipLaunchKernelGGL((ks_norm_cols_gate_kernel<half_t>), dim3(blocks), dim3(256), 0, s, a, (const half_t *)dresidual, (half_t *)dgate, l.split.groups);
+        st = launched();
+        if (st != KSMM_OK) return st;
+    }
+    FinishJob jobs[4];
+    int n = 0;
+    auto finish = [&](const float *from, void *to, int64_t values, int64_t slices) {
+        if (from) jobs[n++] = FinishJob{from, to, values, (int)slices, 1.f};
+    };
+    finish(p.dweight, dweight, features, l.slices);
+    finish(p.dbias, dbias, features, l.slices);
+    finish(p.dpost_weight, dpost_weight, features, l.slices);
+    if (p.dgate) {
+        if (l.split.one_gate)
+            finish(p.dgate, dgate, features, l.slices);
+        else
+            finish(p.dgate, dgate, l.split.groups * features, l.split.parts);
+    }
+    return finish_run(jobs, n, dtype, s);
+}
+
+}  // extern "C"
