@@ -32,9 +32,9 @@ constexpr float LOG2E = 1.4426950408889634f;
 
 // act(z), and act'(z) where wanted.  fp32: the library's functions; fp16: the forms of one or two transcendentals whose
 // error (3e-7 of the value) is far below the type's
-template <typename T, bool SLOPE> __device__ __forceinline__ float activate(int act, float z, float &slope)
+template <typename T, int ACT, bool SLOPE> __device__ __forceinline__ float activate(float z, float &slope)
 {
-    if (act == KSMM_ACT_SILU) {
+    if constexpr (ACT == KSMM_ACT_SILU) {
         float s;
         if constexpr (sizeof(T) == 4)
             s = 1.f / (1.f + expf(-z));
@@ -43,7 +43,7 @@ template <typename T, bool SLOPE> __device__ __forceinline__ float activate(int 
         if constexpr (SLOPE) slope = s * fmaf(z, 1.f - s, 1.f);
         return z * s;
     }
-    if (act == KSMM_ACT_GELU) {
+    if constexpr (ACT == KSMM_ACT_GELU) {
         float phi, ex;
         if constexpr (sizeof(T) == 4) {
             phi = 0.5f * erfcf(-0.70710678118654752f * z);
@@ -64,6 +64,17 @@ template <typename T, bool SLOPE> __device__ __forceinline__ float activate(int 
     }
     if constexpr (SLOPE) slope = 1.f;
     return z;
+}
+
+// one branch on the activation around all of a tile's values
+template <typename F> __device__ __forceinline__ void with_act(int act, F f)
+{
+    if (act == KSMM_ACT_SILU)
+        f(std::integral_constant<int, KSMM_ACT_SILU>());
+    else if (act == KSMM_ACT_GELU)
+        f(std::integral_constant<int, KSMM_ACT_GELU>());
+    else
+        f(std::integral_constant<int, KSMM_ACT_NONE>());
 }
 
 // ---- MFMA operands: KS k values of one row or column a lane --------------------------------------------
@@ -150,8 +161,11 @@ template <typename T, int N> __device__ __forceinline__ void store_run(T *p, int
 
 // ---- tiles ---------------------------------------------------------------------------------------------
 // Workgroup: TB outputs (2 * TB weight columns) of D neighbouring d_i of one a_i x TN rows of the batch; WB x WN waves.
-// x and W arrive in slabs of TK, through registers into two LDS buffers in turn.  Batch-size-first a thread takes D * PER
-// values of a row, the PER k of D neighbouring d_i, and writes them as D chunks of one d_i each.
+// x and W arrive in slabs of TK, through registers into two LDS buffers in turn.  Batch-size-first a thread takes D * E
+// values of a row, the E k of D neighbouring d_i, and writes them as D chunks of one d_i each (ALL: D is all of d, and
+// these values lie in a row).
+// Vectors that would cross the end of a row of weights, or of a batch-size-last row, are moved back to end with it, and
+// so are their results: some outputs are computed, and stored, twice, the same.  (b >= 8, batch-size-last batch >= 16.)
 template <typename T, bool LAST, int D, int TB, int TN, int TK, int WB, int WN> struct Tile {
     static constexpr int THREADS = 64 * WB * WN, E = EPV<T>;
     static constexpr int BT = TB / WB / (LAST ? 32 : 16), NT = TN / WN / 32;  // MFMA tiles a wave: outputs (16, or 32 as gate and up), rows
@@ -164,8 +178,8 @@ template <typename T, bool LAST, int D, int TB, int TN, int TK, int WB, int WN> 
     static_assert(LDS_BYTES <= 160 * 1024, "LDS");
 };
 
-template <typename T, bool LAST, int D, int TB, int TN, int TK, int WB, int WN, int MODE>
-__global__ __launch_bounds__(64 * WB *WN) void ks_gated_kernel(GatedArgs g, int b_tiles, int n_tiles, int blocks)
+template <typename T, bool LAST, int D, bool ALL, int TB, int TN, int TK, int WB, int WN, int MODE>
+__global__ __launch_bounds__(64 * WB *WN, 2) void ks_gated_kernel(GatedArgs g, int b_tiles, int n_tiles, int blocks)
 {
     typedef Tile<T, LAST, D, TB, TN, TK, WB, WN> C;
     typedef op<T> O;
@@ -178,51 +192,61 @@ __global__ __launch_bounds__(64 * WB *WN) void ks_gated_kernel(GatedArgs g, int 
     // each XCD gets a contiguous range of tiles: those that share rows of x share an L2
     const int per_xcd = (blocks + 7) / 8, lid = (blockIdx.x % 8) * per_xcd + blockIdx.x / 8;
     if (lid >= blocks) return;
-    const int a = g.a, b = g.b, c = g.c, d = g.d, dg = d / D;
+    const int a = g.a, b = g.b, c = g.c, d = ALL ? D : g.d, dg = ALL ? 1 : d / D;
     const int bt = lid % b_tiles, rest = lid / b_tiles;
     // (batch-size-first the d_i of an a_i share cache lines of x and h: they are neighbours)
     const int grp = LAST ? rest / n_tiles : rest % (a * dg), nt = LAST ? rest % n_tiles : rest / (a * dg);
-    const int a_i = grp / dg, d0 = (grp - a_i * dg) * D;
-    const int b0 = bt * TB;
-    const int64_t n0 = (int64_t)nt * TN, B = g.batch;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wb = wave / WN, wn = wave % WN;
+    const int a_i = grp / dg, d0 = ALL ? 0 : (grp - a_i * dg) * D;
+    const int b0 = bt * TB, B = (int)g.batch, n0 = nt * TN;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), wb = wave / WN, wn = wave % WN;
+    const int lq = lane >> 5, l32 = lane & 31;
     const int64_t in_size = (int64_t)a * c * d;
     const T *const w = (const T *)g.w + (int64_t)(a_i * d + d0) * c * 2 * b;
     const T *const x = LAST ? (const T *)g.x + ((int64_t)a_i * c * d + d0) * B : (const T *)g.x + (int64_t)a_i * c * d + d0;
 
+    // what a thread loads: places in the first slab
+    const T *wp[C::W_PER], *xp[C::X_PER];
+#pragma unroll
+    for (int i = 0; i < C::W_PER; ++i) {
+        const int v = tid + i * C::THREADS, col = v % (2 * TB / E) * E, row = v / (2 * TB / E);
+        wp[i] = w + ((int64_t)(row / TK) * c + row % TK) * 2 * b + col / TB * b + min(b0 + col % TB, b - E);
+    }
+#pragma unroll
+    for (int i = 0; i < C::X_PER; ++i) {
+        const int v = tid + i * C::THREADS;
+        if constexpr (LAST)
+            xp[i] = x + (int64_t)(v / (TN / E)) * d * B + min(n0 + v % (TN / E) * E, B - E);
+        else  // (rows past the batch: the last one again, not stored)
+            xp[i] = x + min(n0 + v / (TK / E), B - 1) * in_size + (int64_t)(v % (TK / E) * E) * d;
+    }
+    const int64_t w_step = (int64_t)TK * 2 * b, x_step = LAST ? (int64_t)TK * d * B : (int64_t)TK * d;
     Run<T, E> wr[C::W_PER];
     Run<T, D * E> xr[C::X_PER];
-    auto gload = [&](int k0) {
+    auto gload = [&](int s, bool whole) {
 #pragma unroll
         for (int i = 0; i < C::W_PER; ++i) {
-            const int v = tid + i * C::THREADS, cv = v % (2 * TB / E), row = v / (2 * TB / E);
-            const int p = row / TK, k = k0 + row % TK;
-            const int col = cv * E, part = col / TB, bi = b0 + col % TB;
-            // past the block's rows: zeros.  Past its outputs: anything (they are not stored), here zeros
-            const int count = k < c ? min(max(b - bi, 0), E) : 0;
-            wr[i] = load_run<T, E>(w + ((int64_t)p * c + k) * 2 * b + part * b + bi, count);
+            const T *const from = wp[i] + s * w_step;
+            if (whole)
+                wr[i] = load_run<T, E>(from, E);
+            else  // past the block's rows: zeros
+                wr[i] = load_run<T, E>(from, s * TK + (tid + i * C::THREADS) / (2 * TB / E) % TK < c ? E : 0);
         }
 #pragma unroll
         for (int i = 0; i < C::X_PER; ++i) {
             const int v = tid + i * C::THREADS;
+            const T *const from = xp[i] + s * x_step;
             if constexpr (LAST) {
-                const int k = k0 + v / (TN / E);
-                const int64_t n = n0 + v % (TN / E) * E;
-                const int count = k < c ? (int)min(max(B - n, (int64_t)0), (int64_t)E) : 0;
-                xr[i] = load_run<T, E>(x + (int64_t)k * d * B + n, count);
+                xr[i] = load_run<T, E>(from, whole || s * TK + v / (TN / E) < c ? E : 0);
             } else {
-                const int k = k0 + v % (TK / E) * E;
-                const int64_t n = min(n0 + v / (TK / E), B - 1);  // (rows past the batch: the last one again, not stored)
-                const int count = min(max(c - k, 0), E);
-                const T *const from = x + n * in_size + (int64_t)k * d;
-                if (d == D) {
+                const int count = whole ? E : min(max(c - s * TK - v % (TK / E) * E, 0), E);
+                if constexpr (ALL) {
                     xr[i] = load_run<T, D * E>(from, count * D);
                 } else {
 #pragma unroll
                     for (int e = 0; e < E; ++e) {
-                        const Run<T, D> s = load_run<T, D>(from + (int64_t)e * d, e < count ? D : 0);
+                        const Run<T, D> q = load_run<T, D>(from + (int64_t)e * d, e < count ? D : 0);
 #pragma unroll
-                        for (int p = 0; p < D; ++p) xr[i].e[e * D + p] = s.e[p];
+                        for (int p = 0; p < D; ++p) xr[i].e[e * D + p] = q.e[p];
                     }
                 }
             }
@@ -242,10 +266,10 @@ __global__ __launch_bounds__(64 * WB *WN) void ks_gated_kernel(GatedArgs g, int 
             } else {
 #pragma unroll
                 for (int p = 0; p < D; ++p) {
-                    Run<T, E> s;
+                    Run<T, E> q;
 #pragma unroll
-                    for (int e = 0; e < E; ++e) s.e[e] = xr[i].e[e * D + p];
-                    *(Run<T, E> *)__builtin_assume_aligned(xs(buf, p) + v / (TK / E) * C::LDX + v % (TK / E) * E, 16) = s;
+                    for (int e = 0; e < E; ++e) q.e[e] = xr[i].e[e * D + p];
+                    *(Run<T, E> *)__builtin_assume_aligned(xs(buf, p) + v / (TK / E) * C::LDX + v % (TK / E) * E, 16) = q;
                 }
             }
         }
@@ -253,29 +277,61 @@ __global__ __launch_bounds__(64 * WB *WN) void ks_gated_kernel(GatedArgs g, int 
 
     constexpr int PARTS = LAST ? 2 : 1;  // accumulators an output tile: gate and up apart, or both in one
     float16_t acc[D][PARTS][C::BT][C::NT];
+    const T *const bias = (const T *)g.bias;
+    // the lane's outputs of tile i: a run of 8 (E at a time, each moved back on its own), or one
+    auto run_at = [&](int i, int e) { return min(b0 + (wb * C::BT + i) * 16 + 8 * lq + e, b - E); };
+    auto one_at = [&](int i) {
+        const int at = b0 + (wb * C::BT + i) * 32 + l32 / E * E;
+        return min(at, b - E) + l32 % E;
+    };
 #pragma unroll
     for (int p = 0; p < D; ++p)
 #pragma unroll
-        for (int q = 0; q < PARTS; ++q)
+        for (int q = 0; q < 2; ++q)
 #pragma unroll
-            for (int i = 0; i < C::BT; ++i)
+            for (int i = 0; i < C::BT; ++i) {
+                float v[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] = 0.f;
+                if (bias) {
+                    const T *const from = bias + ((int64_t)(a_i * 2 + q) * b) * d + d0 + p;
+                    if constexpr (LAST) {
+                        const float t = (float)from[(int64_t)one_at(i) * d];
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) v[e] = t;
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) v[e] = (float)from[(int64_t)(run_at(i, e / E * E) + e % E) * d];
+                    }
+                }
 #pragma unroll
                 for (int j = 0; j < C::NT; ++j)
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) acc[p][q][i][j][e] = 0.f;
+                    for (int e = 0; e < 8; ++e) {
+                        if constexpr (LAST)
+                            acc[p][q * (PARTS - 1)][i][j][e] = acc[p][q * (PARTS - 1)][i][j][8 + e] = v[e];
+                        else
+                            acc[p][0][i][j][8 * q + e] = v[e];
+                    }
+            }
 
     const int steps = (c + TK - 1) / TK;
-    gload(0);
+    gload(0, TK <= c);
     lstore(0);
     __syncthreads();
     for (int s = 0; s < steps; ++s) {
         const int buf = s & 1;
-        if (s + 1 < steps) gload((s + 1) * TK);
+        if (s + 1 < steps) {
+            if ((s + 2) * TK <= c)
+                gload(s + 1, true);
+            else
+                gload(s + 1, false);
+        }
 #pragma unroll
         for (int k0 = 0; k0 < TK; k0 += O::KS)
 #pragma unroll
             for (int p = 0; p < D; ++p) {
-                const T *wp = ws(buf, p), *xp = xs(buf, p);
+                const T *wl = ws(buf, p), *xl = xs(buf, p);
                 typename O::type fw[PARTS][C::BT], fx[C::NT];
 #pragma unroll
                 for (int q = 0; q < PARTS; ++q)
@@ -283,19 +339,19 @@ __global__ __launch_bounds__(64 * WB *WN) void ks_gated_kernel(GatedArgs g, int 
                     for (int i = 0; i < C::BT; ++i) {
                         if constexpr (LAST) {
                             const int col = q * TB + (wb * C::BT + i) * 32;
-                            fw[q][i] = k_outer(wp, C::LDW, k0, lane, [&](int rg) { return col + 4 * rg; });
+                            fw[q][i] = k_outer(wl, C::LDW, k0, lane, [&](int rg) { return col + 4 * rg; });
                         } else {
                             const int col = (wb * C::BT + i) * 16;
-                            fw[q][i] = k_outer(wp, C::LDW, k0, lane, [&](int rg) { return col + mixed_col(4 * rg, TB); });
+                            fw[q][i] = k_outer(wl, C::LDW, k0, lane, [&](int rg) { return col + mixed_col(4 * rg, TB); });
                         }
                     }
 #pragma unroll
                 for (int j = 0; j < C::NT; ++j) {
                     const int n = (wn * C::NT + j) * 32;
                     if constexpr (LAST)
-                        fx[j] = k_outer(xp, C::LDX, k0, lane, [&](int rg) { return n + run_col(4 * rg); });
+                        fx[j] = k_outer(xl, C::LDX, k0, lane, [&](int rg) { return n + run_col(4 * rg); });
                     else
-                        fx[j] = k_inner<T>(xp, C::LDX, n, k0, lane);
+                        fx[j] = k_inner<T>(xl, C::LDX, n, k0, lane);
                 }
 #pragma unroll
                 for (int q = 0; q < PARTS; ++q)
@@ -309,117 +365,84 @@ __global__ __launch_bounds__(64 * WB *WN) void ks_gated_kernel(GatedArgs g, int 
         __syncthreads();
     }
 
-    const T *const bias = (const T *)g.bias, *const dh = (const T *)g.dh;
+    const T *const dh = (const T *)g.dh;
     T *const out = (T *)g.out;
-    const int lq = lane >> 5, l32 = lane & 31;
-    if constexpr (LAST) {
-        // a lane: one output, 16 rows of the batch in a row
+    const int64_t out_size = (int64_t)a * b * d;
+    with_act(g.act, [&](auto act_of) {
+        constexpr int ACT = decltype(act_of)::value;
+        // N values of gate and up (and of dh) at a time: a vector of the result
+        auto finish = [&](auto zg, auto zu, const T *dh_at, T *to_g, T *to_u, auto count) {
+            constexpr int N = decltype(count)::value;
+            Run<T, N> in, r0, r1;
+            if constexpr (MODE == 1) in = load_run<T, N>(dh_at, N);
 #pragma unroll
-        for (int i = 0; i < C::BT; ++i) {
-            const int bi = b0 + (wb * C::BT + i) * 32 + l32;
-            if (bi >= b) continue;
-            const int64_t zg = ((int64_t)(a_i * 2) * b + bi) * d + d0, zu = zg + (int64_t)b * d, hf = ((int64_t)a_i * b + bi) * d + d0;
-            const float bg = bias ? (float)bias[zg] : 0.f, bu = bias ? (float)bias[zu] : 0.f;
+            for (int e = 0; e < N; ++e) {
+                const float gate = zg(e), up = zu(e);
+                float slope = 0.f;
+                const float v = activate<T, ACT, MODE == 1>(gate, slope);
+                if constexpr (MODE == 0) {
+                    r0.e[e] = (T)(v * up);
+                } else {
+                    const float t = (float)in.e[e];
+                    r0.e[e] = (T)(t * up * slope);
+                    r1.e[e] = (T)(t * v);
+                }
+            }
+            store_run<T, N>(to_g, N, r0);
+            if constexpr (MODE == 1) store_run<T, N>(to_u, N, r1);
+        };
+        if constexpr (LAST) {
+            // a lane: one output, 16 rows of the batch in a row, E at a time
+#pragma unroll
+            for (int i = 0; i < C::BT; ++i) {
+                if (b0 + (wb * C::BT + i) * 32 >= b) continue;
+                const int64_t bi = one_at(i);
+                const int64_t fg = (a_i * 2 * (int64_t)b + bi) * d + d0, fh = (a_i * (int64_t)b + bi) * d + d0;
+#pragma unroll
+                for (int j = 0; j < C::NT; ++j)
+#pragma unroll
+                    for (int v = 0; v < 16; v += E) {
+                        const int at = n0 + (wn * C::NT + j) * 32 + 16 * lq + v;
+                        if (at >= B) continue;
+                        const int n = min(at, B - E);
+                        finish([&](int e) { return acc[0][0][i][j][v + e]; }, [&](int e) { return acc[0][PARTS - 1][i][j][v + e]; },
+                               dh + fh * B + n, out + (MODE == 0 ? fh : fg) * B + n, out + (fg + (int64_t)b * d) * B + n,
+                               std::integral_constant<int, E>());
+                    }
+            }
+        } else {
+            // a lane: one row of the batch, 8 outputs of D neighbouring d_i
 #pragma unroll
             for (int j = 0; j < C::NT; ++j) {
-                const int64_t n = n0 + (wn * C::NT + j) * 32 + 16 * lq;
+                const int n = n0 + (wn * C::NT + j) * 32 + l32;
                 if (n >= B) continue;
-                const int count = (int)min(B - n, (int64_t)16);
-                Run<T, 16> r0, r1, in;
-                if (MODE == 1) in = load_run<T, 16>(dh + hf * B + n, count);
+                const T *const dh_n = dh + n * out_size + d0;
+                T *const out_n = out + n * (MODE + 1) * out_size + d0;
 #pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    const float zgv = acc[0][0][i][j][e] + bg, zuv = acc[0][PARTS - 1][i][j][e] + bu;
-                    float slope = 0.f;
-                    const float act = activate<T, MODE == 1>(g.act, zgv, slope);
-                    if (MODE == 0) {
-                        r0.e[e] = (T)(act * zuv);
+                for (int i = 0; i < C::BT; ++i) {
+                    if (b0 + (wb * C::BT + i) * 16 + 8 * lq >= b) continue;
+                    if constexpr (ALL) {
+#pragma unroll
+                        for (int h = 0; h < 8; h += E) {
+                            const int64_t fh = ((int64_t)a_i * b + run_at(i, h)) * D, fg = fh + (int64_t)a_i * b * D * MODE;
+#pragma unroll
+                            for (int q = 0; q < D; ++q)  // vector q of the E * D values
+                                finish([&](int e) { return acc[(q * E + e) % D][0][i][j][h + (q * E + e) / D]; },
+                                       [&](int e) { return acc[(q * E + e) % D][0][i][j][8 + h + (q * E + e) / D]; }, dh_n + fh + q * E,
+                                       out_n + fg + q * E, out_n + fg + (int64_t)b * D + q * E, std::integral_constant<int, E>());
+                        }
                     } else {
-                        const float v = (float)in.e[e];
-                        r0.e[e] = (T)(v * zuv * slope);
-                        r1.e[e] = (T)(v * act);
+#pragma unroll
+                        for (int h = 0; h < 8; ++h) {
+                            const int64_t at = run_at(i, h / E * E) + h % E, fh = ((int64_t)a_i * b + at) * d, fg = fh + (int64_t)a_i * b * d * MODE;
+                            finish([&](int e) { return acc[e][0][i][j][h]; }, [&](int e) { return acc[e][0][i][j][8 + h]; }, dh_n + fh,
+                                   out_n + fg, out_n + fg + (int64_t)b * d, std::integral_constant<int, D>());
+                        }
                     }
-                }
-                if (MODE == 0) {
-                    store_run<T, 16>(out + hf * B + n, count, r0);
-                } else {
-                    store_run<T, 16>(out + zg * B + n, count, r0);
-                    store_run<T, 16>(out + zu * B + n, count, r1);
                 }
             }
         }
-    } else {
-        // a lane: one row of the batch, 8 outputs of D neighbouring d_i
-        const int64_t out_size = (int64_t)a * b * d;
-#pragma unroll
-        for (int i = 0; i < C::BT; ++i) {
-            const int bi = b0 + (wb * C::BT + i) * 16 + 8 * lq;
-            const int count = min(b - bi, 8);
-            if (count <= 0) continue;
-            const int64_t zg = ((int64_t)(a_i * 2) * b + bi) * d + d0, zu = zg + (int64_t)b * d, hf = ((int64_t)a_i * b + bi) * d + d0;
-            // 8 x D values: b_i * d + d_i, in a row where D is all of d
-            auto load = [&](const T *from) {
-                if (d == D) return load_run<T, 8 * D>(from, count * D);
-                Run<T, 8 * D> r;
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const Run<T, D> s = load_run<T, D>(from + (int64_t)e * d, e < count ? D : 0);
-#pragma unroll
-                    for (int p = 0; p < D; ++p) r.e[e * D + p] = s.e[p];
-                }
-                return r;
-            };
-            auto store = [&](T *to, const Run<T, 8 * D> &r) {
-                if (d == D) {
-                    store_run<T, 8 * D>(to, count * D, r);
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        Run<T, D> s;
-#pragma unroll
-                        for (int p = 0; p < D; ++p) s.e[p] = r.e[e * D + p];
-                        store_run<T, D>(to + (int64_t)e * d, e < count ? D : 0, s);
-                    }
-                }
-            };
-            Run<T, 8 * D> bg, bu;
-            if (bias) {
-                bg = load(bias + zg);
-                bu = load(bias + zu);
-            }
-#pragma unroll
-            for (int j = 0; j < C::NT; ++j) {
-                const int64_t n = n0 + (wn * C::NT + j) * 32 + l32;
-                if (n >= B) continue;
-                Run<T, 8 * D> r0, r1, in;
-                if (MODE == 1) in = load(dh + n * out_size + hf);
-#pragma unroll
-                for (int e = 0; e < 8; ++e)
-#pragma unroll
-                    for (int p = 0; p < D; ++p) {
-                        float zgv = acc[p][0][i][j][e], zuv = acc[p][0][i][j][8 + e], slope = 0.f;
-                        if (bias) {
-                            zgv += (float)bg.e[e * D + p];
-                            zuv += (float)bu.e[e * D + p];
-                        }
-                        const float act = activate<T, MODE == 1>(g.act, zgv, slope);
-                        if (MODE == 0) {
-                            r0.e[e * D + p] = (T)(act * zuv);
-                        } else {
-                            const float v = (float)in.e[e * D + p];
-                            r0.e[e * D + p] = (T)(v * zuv * slope);
-                            r1.e[e * D + p] = (T)(v * act);
-                        }
-                    }
-                if (MODE == 0) {
-                    store(out + n * out_size + hf, r0);
-                } else {
-                    store(out + n * 2 * out_size + zg, r0);
-                    store(out + n * 2 * out_size + zu, r1);
-                }
-            }
-        }
-    }
+    });
 }
 
 // ---- few rows ------------------------------------------------------------------------------------------
@@ -478,16 +501,18 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void ks_gated_few_kernel(GatedArgs 
     }
     const int64_t out_size = (int64_t)a * b * d;
     auto at = [&](int64_t f, int64_t size) { return LAST ? f * B + n : n * size + f; };
-    float slope = 0.f;
-    const float act = activate<T, MODE == 1>(g.act, zg, slope);
     T *const out = (T *)g.out;
-    if (MODE == 0) {
-        out[at(fh, out_size)] = (T)(act * zu);
-    } else {
-        const float v = (float)((const T *)g.dh)[at(fh, out_size)];
-        out[at(fg, 2 * out_size)] = (T)(v * zu * slope);
-        out[at(fu, 2 * out_size)] = (T)(v * act);
-    }
+    with_act(g.act, [&](auto act_of) {
+        float slope = 0.f;
+        const float act = activate<T, decltype(act_of)::value, MODE == 1>(zg, slope);
+        if (MODE == 0) {
+            out[at(fh, out_size)] = (T)(act * zu);
+        } else {
+            const float v = (float)((const T *)g.dh)[at(fh, out_size)];
+            out[at(fg, 2 * out_size)] = (T)(v * zu * slope);
+            out[at(fu, 2 * out_size)] = (T)(v * act);
+        }
+    });
 }
 
 // ---- choices -------------------------------------------------------------------------------------------
@@ -502,13 +527,13 @@ template <typename T, bool LAST, int MODE> int run_few(const GatedArgs &g, hipSt
     return launched();
 }
 
-template <typename T, bool LAST, int D, int TB, int TN, int TK, int WB, int WN, int MODE> int run_tile(const GatedArgs &g, hipStream_t s)
+template <typename T, bool LAST, int D, bool ALL, int TB, int TN, int TK, int WB, int WN, int MODE> int run_tile(const GatedArgs &g, hipStream_t s)
 {
     typedef Tile<T, LAST, D, TB, TN, TK, WB, WN> C;
     const int b_tiles = (g.b + TB - 1) / TB;
     const int64_t n_tiles = (g.batch + TN - 1) / TN, blocks = (int64_t)b_tiles * g.a * (g.d / D) * n_tiles;
     if (blocks > 0x7ffffff0LL) return KSMM_ERR_TOO_LARGE;
-    const auto fn = &ks_gated_kernel<T, LAST, D, TB, TN, TK, WB, WN, MODE>;
+    const auto fn = &ks_gated_kernel<T, LAST, D, ALL, TB, TN, TK, WB, WN, MODE>;
     if (C::LDS_BYTES > 64 * 1024) {
         const int rc = ensure_dynamic_lds((const void *)fn, C::LDS_BYTES);
         if (rc != KSMM_OK) return rc;
@@ -520,16 +545,19 @@ template <typename T, bool LAST, int D, int TB, int TN, int TK, int WB, int WN, 
 template <typename T, bool LAST, int MODE> int run(const GatedArgs &g, hipStream_t s)
 {
     constexpr int TK = sizeof(T) == 4 ? 16 : 32;
-    if (g.batch <= 128) return run_few<T, LAST, MODE>(g, s);
-    if constexpr (LAST) return run_tile<T, true, 1, 64, 128, TK, 2, 2, MODE>(g, s);
-    if constexpr (!LAST) {
-        if (g.d == 1) return run_tile<T, false, 1, 64, 128, TK, 2, 2, MODE>(g, s);
-        if (g.d % 4 == 0) return run_tile<T, false, 4, 32, 64, TK, 2, 2, MODE>(g, s);
-        if (g.d % 3 == 0) return run_tile<T, false, 3, 32, 128, TK, 2, 2, MODE>(g, s);
-        if (g.d % 2 == 0) return run_tile<T, false, 2, 64, 128, TK, 2, 2, MODE>(g, s);
-        return run_tile<T, false, 1, 64, 128, TK, 2, 2, MODE>(g, s);
+    if (g.batch <= 128 || g.b < 8) return run_few<T, LAST, MODE>(g, s);
+    if constexpr (LAST) {
+        return run_tile<T, true, 1, false, 64, 128, TK, 2, 2, MODE>(g, s);
+    } else {
+        if (g.d == 1) return run_tile<T, false, 1, true, 64, 128, TK, 2, 2, MODE>(g, s);
+        if (g.d == 2) return run_tile<T, false, 2, true, 64, 128, TK, 2, 2, MODE>(g, s);
+        if (g.d == 3) return run_tile<T, false, 3, true, 32, 128, TK, 2, 2, MODE>(g, s);
+        if (g.d == 4) return run_tile<T, false, 4, true, 32, 64, TK, 2, 2, MODE>(g, s);
+        if (g.d % 4 == 0) return run_tile<T, false, 4, false, 32, 64, TK, 2, 2, MODE>(g, s);
+        if (g.d % 3 == 0) return run_tile<T, false, 3, false, 32, 128, TK, 2, 2, MODE>(g, s);
+        if (g.d % 2 == 0) return run_tile<T, false, 2, false, 64, 128, TK, 2, 2, MODE>(g, s);
+        return run_tile<T, false, 1, false, 64, 128, TK, 2, 2, MODE>(g, s);
     }
-    return KSMM_ERR_BAD_ALGO;
 }
 
 }  // namespace
@@ -554,7 +582,7 @@ namespace {
 
 int check(int64_t batch, int a, int b, int c, int d, int dtype, int act)
 {
-    if (b > 0x3fffffff) return KSMM_ERR_TOO_LARGE;
+    if (b > 0x3fffffff || batch > 0x7fffff00) return KSMM_ERR_TOO_LARGE;  // (a tile's rows past the end are counted in 32 bits)
     if (dtype != KSMM_F32 && dtype != KSMM_F16) return KSMM_ERR_BAD_DTYPE;
     const int rc = ksmm_validate(batch, a, 2 * b, c, d, dtype, dtype, dtype, 0);
     if (rc != KSMM_OK) return rc;
