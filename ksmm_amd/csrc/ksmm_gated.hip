@@ -284,39 +284,50 @@ __global__ __launch_bounds__(64 * WB *WN, 2) void ks_gated_kernel(GatedArgs g, i
         const int at = b0 + (wb * C::BT + i) * 32 + l32 / E * E;
         return min(at, b - E) + l32 % E;
     };
-#pragma unroll
-    for (int p = 0; p < D; ++p)
+    // the sums start at the bias: its loads go out before those of the first slab
+    constexpr int BIAS = LAST ? 1 : 8 * D;
+    T bv[2][C::BT][BIAS];
+    if (bias) {
 #pragma unroll
         for (int q = 0; q < 2; ++q)
 #pragma unroll
             for (int i = 0; i < C::BT; ++i) {
-                float v[8];
+                const T *const from = bias + ((int64_t)(a_i * 2 + q) * b) * d + d0;
+                if constexpr (LAST) {
+                    bv[q][i][0] = from[(int64_t)one_at(i) * d];
+                } else if constexpr (ALL) {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) v[e] = 0.f;
-                if (bias) {
-                    const T *const from = bias + ((int64_t)(a_i * 2 + q) * b) * d + d0 + p;
-                    if constexpr (LAST) {
-                        const float t = (float)from[(int64_t)one_at(i) * d];
+                    for (int h = 0; h < 8; h += E) __builtin_memcpy(&bv[q][i][h * D], from + (int64_t)run_at(i, h) * D, E * D * sizeof(T));
+                } else {
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) v[e] = t;
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) v[e] = (float)from[(int64_t)(run_at(i, e / E * E) + e % E) * d];
-                    }
+                    for (int h = 0; h < 8; ++h) __builtin_memcpy(&bv[q][i][h * D], from + (int64_t)(run_at(i, h / E * E) + h % E) * d, D * sizeof(T));
                 }
-#pragma unroll
-                for (int j = 0; j < C::NT; ++j)
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        if constexpr (LAST)
-                            acc[p][q * (PARTS - 1)][i][j][e] = acc[p][q * (PARTS - 1)][i][j][8 + e] = v[e];
-                        else
-                            acc[p][0][i][j][8 * q + e] = v[e];
-                    }
             }
-
+    } else {
+#pragma unroll
+        for (int q = 0; q < 2; ++q)
+#pragma unroll
+            for (int i = 0; i < C::BT; ++i)
+#pragma unroll
+                for (int e = 0; e < BIAS; ++e) bv[q][i][e] = (T)0.f;
+    }
     const int steps = (c + TK - 1) / TK;
     gload(0, TK <= c);
+#pragma unroll
+    for (int p = 0; p < D; ++p)
+#pragma unroll
+        for (int i = 0; i < C::BT; ++i)
+#pragma unroll
+            for (int j = 0; j < C::NT; ++j)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    if constexpr (LAST) {
+                        acc[p][0][i][j][e] = (float)bv[0][i][0];
+                        acc[p][PARTS - 1][i][j][e] = (float)bv[1][i][0];
+                    } else {
+                        acc[p][0][i][j][e] = (float)bv[e / 8][i][e % 8 * D + p];
+                    }
+                }
     lstore(0);
     __syncthreads();
     for (int s = 0; s < steps; ++s) {
