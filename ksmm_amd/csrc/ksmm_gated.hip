@@ -456,6 +456,379 @@ __global__ __launch_bounds__(64 * WB *WN, 2) void ks_gated_kernel(GatedArgs g, i
     });
 }
 
+// ---- fp16 in aligned vectors: a ring of slabs ----------------------------------------------------------
+// The tile above spends its time waiting: a slab of 32 k is a quarter of a microsecond of products, its loads take two.
+// Here they go straight to LDS (no registers), three slabs of 16 k ahead; a workgroup stays for many tiles, and the first
+// slabs of the next one are on their way while this one's results leave.  Two workgroups a CU: one multiplies while the
+// other finishes a tile (GLU in the vector ALU takes as long as the products of c = 192).
+//
+// What counts as landed is counted by hand: a slab's loads are followed by those of two more (2 * L of them), and, for three
+// iterations each, by the loads that a tile's end needs (bias of the next tile, dh; EARLY of them) and by its stores.
+//
+// d_i = 2: a row's (k, d_i) pairs are split into the operands of both d_i when they are read (one v_perm a register).
+// The sums start at the bias: one product of (bias, 0, ..) and (1, 0, ..).  Results go through 4 KB of LDS a wave, and
+// leave as rows of 128 bytes.
+//
+// (1,768,192,2), 25088 rows: see the table of measurements in the host code below.
+constexpr int vmcnt_imm(int n) { return (n & 15) | (7 << 4) | (15 << 8) | (((n >> 4) & 3) << 14); }
+typedef __attribute__((address_space(3))) unsigned char *lds_bytes_t;
+
+// 16 bytes a lane from base (uniform) + offset to LDS, 1024 bytes a wave from `to` on
+__device__ __forceinline__ void to_lds(const void *base, uint32_t offset, uint32_t to)
+{
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(offset), "s"(base), "s"(to) : "memory", "m0");
+}
+
+template <bool LAST, int D, int TB, int MODE> struct Ring {
+    static constexpr int WB = 2, WN = 2, TN = 128, TK = 16, ST = 4, THREADS = 256;
+    static constexpr int BT = TB / WB / (LAST ? 32 : 16), NT = 2, PARTS = LAST ? 2 : 1;
+    static constexpr int W_CPR = 2 * TB / 8, X_CPR = LAST ? TN / 8 : TK * D / 8, X_ROWS = LAST ? TK : TN;  // 16-byte chunks a row
+    static constexpr int W_PLANE = TK * W_CPR * 16, W_BYTES = D * W_PLANE, X_BYTES = X_ROWS * X_CPR * 16, STAGE = W_BYTES + X_BYTES;
+    static constexpr int LW = W_BYTES / 16 / THREADS, LX = X_BYTES / 16 / THREADS, L = LW + LX;
+    static constexpr int UNITS = LAST ? BT : NT;                       // pieces of 32 rows that a wave's results leave in
+    static constexpr int O_CPR = LAST ? 8 : TB / WB * D * 2 / 16;      // chunks a row of them
+    static constexpr int O_IT = 32 * O_CPR / 64, PIECE = 32 * O_CPR * 16;
+    static constexpr int LDS_BYTES = ST * STAGE + 4 * PIECE;
+    static constexpr int STORES = UNITS * O_IT * (MODE + 1), BIASES = LAST ? 2 * BT : D * BT, EARLY = BIASES + (MODE ? UNITS * O_IT : 0);
+    static constexpr int WAIT = (ST - 2) * L;
+    static_assert(W_BYTES % (16 * THREADS) == 0 && X_BYTES % (16 * THREADS) == 0 && (!LAST || D == 1) && D <= 2, "loads");
+    static_assert(TB == 64 || TB == 128, "weight swizzle");
+    static_assert(WAIT + STORES + EARLY <= 63 && LDS_BYTES <= 80 * 1024, "ring");
+    static_assert(BT * PARTS * NT * D * 16 <= 128, "accumulators");
+};
+
+// where chunk cc of row `row` lies (and, as these are their own inverses, what the chunk that lies there is)
+template <int TB, bool LAST> __device__ __forceinline__ int w_swizzle(int row, int cc)
+{
+    if (LAST) return cc ^ (4 * (row & 3));                  // operands of 32 columns in a row: 4 rows x 64 bytes at a time
+    const int r = cc ^ (2 * (row & 3));                     // 16 gate and 16 up columns: 4 rows x (32 + 32)
+    return TB == 128 ? r ^ ((r >> 4) * 8) : r;
+}
+template <bool LAST, int CPR> __device__ __forceinline__ int x_swizzle(int row, int cc)
+{
+    if (LAST) return cc ^ (4 * (row & 3));
+    return cc ^ (CPR == 2 ? (row >> 3) & 1 : (row >> 2) & 3);
+}
+template <int CPR> __device__ __forceinline__ int o_swizzle(int row, int cc) { return cc ^ (CPR == 8 ? (row >> 1) & 7 : (row >> 2) & 3); }
+
+template <bool LAST, int D, int TB, int MODE>
+__global__ __launch_bounds__(256, 2) void ks_gated_ring_kernel(GatedArgs g, int b_tiles, int tiles)
+{
+    typedef Ring<LAST, D, TB, MODE> C;
+    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_bytes_t)smem;
+    const int a = g.a, b = g.b, c = g.c, d = LAST ? g.d : D, groups = LAST ? a * d : a, B = (int)g.batch;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), wb = wave / C::WN, wn = wave % C::WN;
+    const int l32 = lane & 31, lq = lane >> 5, steps = c / C::TK;
+    // each XCD has a range of tiles, dealt to its workgroups in turn: those at work share rows of x in their L2
+    const int per_xcd = (tiles + 7) / 8, first = (blockIdx.x & 7) * per_xcd, last = min(tiles, first + per_xcd), stride = gridDim.x / 8;
+    const int mine = first + (blockIdx.x >> 3);
+    if (mine >= last) return;
+    const half_t *const x = (const half_t *)g.x, *const w = (const half_t *)g.w, *const bias = (const half_t *)g.bias;
+    const half_t *const dh = (const half_t *)g.dh;
+    half_t *const out = (half_t *)g.out;
+    const int64_t in_size = (int64_t)a * c * d, out_size = (int64_t)a * b * d;
+
+    struct At {
+        int grp, b0, n0;
+    };
+    auto at = [&](int t) {
+        const int bt = t % b_tiles, rest = t / b_tiles;
+        return At{rest % groups, bt * TB, rest / groups * C::TN};
+    };
+
+    // ---- loads: slab `ls` of tile `lt` next
+    uint32_t woff[C::LW], xoff[C::LX];
+    const char *wsrc, *xsrc;
+    const int64_t w_step = (int64_t)C::TK * 2 * b * 2, x_step = LAST ? (int64_t)C::TK * d * B * 2 : (int64_t)C::TK * D * 2;
+    int lt = mine, ls = 0;
+    auto begin_loads = [&]() {
+        const At p = at(lt);
+#pragma unroll
+        for (int i = 0; i < C::LW; ++i) {
+            const int v = tid + i * C::THREADS, row = v / C::W_CPR, cc = w_swizzle<TB, LAST>(row, v % C::W_CPR);
+            const int part = cc / (TB / 8), col = p.b0 + cc % (TB / 8) * 8;
+            woff[i] = (uint32_t)((((row / C::TK) * c + row % C::TK) * 2 * b + part * b + min(col, b - 8)) * 2);
+        }
+#pragma unroll
+        for (int i = 0; i < C::LX; ++i) {
+            const int v = tid + i * C::THREADS, row = v / C::X_CPR, cc = x_swizzle<LAST, C::X_CPR>(row, v % C::X_CPR);
+            xoff[i] = LAST ? (uint32_t)((row * d * B + min(cc * 8, B - 8 - p.n0)) * 2)
+                           : (uint32_t)((min(row, B - 1 - p.n0) * (int)in_size + cc * 8) * 2);
+        }
+        const int a_i = LAST ? p.grp / d : p.grp, d_i = LAST ? p.grp - a_i * d : 0;
+        wsrc = (const char *)(w + (int64_t)(a_i * d + d_i) * c * 2 * b);
+        xsrc = (const char *)(LAST ? x + ((int64_t)a_i * c * d + d_i) * B + p.n0 : x + p.n0 * in_size + (int64_t)a_i * c * D);
+    };
+    uint32_t to = lds0 + wave * 1024;
+    int slot = 0;
+    auto issue = [&]() {
+#pragma unroll
+        for (int i = 0; i < C::LW; ++i) to_lds(wsrc, woff[i], to + i * (C::THREADS * 16));
+#pragma unroll
+        for (int i = 0; i < C::LX; ++i) to_lds(xsrc, xoff[i], to + C::W_BYTES + i * (C::THREADS * 16));
+        slot = slot + 1 == C::ST ? 0 : slot + 1;
+        to = lds0 + wave * 1024 + slot * C::STAGE;
+        wsrc += w_step;
+        xsrc += x_step;
+        if (++ls == steps) {
+            // (behind the last tile its loads are repeated: the counts stay what they are)
+            ls = 0;
+            lt = lt + stride < last ? lt + stride : lt;
+            begin_loads();
+        }
+    };
+
+    // ---- operands
+    uint32_t wa[C::PARTS][C::BT], xa[LAST ? C::NT : D];
+    {
+        const int i16 = lane & 15, hs = (lane >> 4) & 1, row = 8 * lq + (i16 >> 2);
+#pragma unroll
+        for (int q = 0; q < C::PARTS; ++q)
+#pragma unroll
+            for (int i = 0; i < C::BT; ++i) {
+                int cc, half;
+                if (LAST) {
+                    cc = q * (TB / 8) + (wb * C::BT + i) * 4 + 2 * hs + ((i16 & 3) >> 1);
+                    half = i16 & 1;
+                } else {  // mixed_col: rows of the operand 4 * (4 * hs + (i16 & 3)) ..
+                    cc = hs * (TB / 8) + (wb * C::BT + i) * 2 + (i16 & 1);
+                    half = (i16 >> 1) & 1;
+                }
+                wa[q][i] = lds0 + row * (C::W_CPR * 16) + w_swizzle<TB, LAST>(row, cc) * 16 + half * 8;
+            }
+        if (LAST) {
+#pragma unroll
+            for (int j = 0; j < C::NT; ++j) {  // run_col
+                const int cc = (wn * C::NT + j) * 4 + 2 * (i16 & 1) + hs, half = (i16 >> 1) & 1;
+                xa[j % (LAST ? C::NT : D)] = lds0 + C::W_BYTES + row * (C::X_CPR * 16) + x_swizzle<LAST, C::X_CPR>(row, cc) * 16 + half * 8;
+            }
+        } else {
+#pragma unroll
+            for (int p = 0; p < D; ++p) {
+                const int r = wn * C::NT * 32 + l32;
+                xa[p] = lds0 + C::W_BYTES + r * (C::X_CPR * 16) + x_swizzle<LAST, C::X_CPR>(r, lq * D + p) * 16;
+            }
+        }
+    }
+    auto outer = [&](uint32_t addr, int row_bytes) {
+        typedef short4_t __attribute__((address_space(3))) * lds_ptr;
+        typedef short short8_t __attribute__((ext_vector_type(8)));
+        const short4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(lds_bytes_t)(uintptr_t)addr);
+        const short4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(lds_bytes_t)(uintptr_t)(addr + 4 * row_bytes));
+        return __builtin_bit_cast(half8_t, short8_t{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]});
+    };
+    auto inner = [&](uint32_t addr) {
+        typedef uint4_t __attribute__((address_space(3))) * lds_ptr;
+        return *(lds_ptr)(lds_bytes_t)(uintptr_t)addr;
+    };
+
+    // ---- bias: of row lane % 32 of each weight tile (of column lane % 32, batch-size-last)
+    half_t bv[C::BIASES];
+    auto load_bias = [&](int t) {
+        const At p = at(t);
+        const int a_i = LAST ? p.grp / d : p.grp, d_i = LAST ? p.grp - a_i * d : 0;
+        const half_t *const from = bias ? bias + (int64_t)a_i * 2 * b * d + d_i : w;  // (no bias: anything, not used)
+#pragma unroll
+        for (int i = 0; i < C::BT; ++i)
+#pragma unroll
+            for (int q = 0; q < C::BIASES / C::BT; ++q) {
+                int64_t k;
+                if (LAST) {
+                    k = ((int64_t)q * b + min(p.b0 + (wb * C::BT + i) * 32 + l32, b - 1)) * d;
+                } else {
+                    const int col = mixed_col(l32, 16);
+                    k = ((int64_t)(col >> 4) * b + min(p.b0 + (wb * C::BT + i) * 16 + (col & 15), b - 1)) * D + q;
+                }
+                bv[i * (C::BIASES / C::BT) + q] = from[bias ? k : 0];
+            }
+    };
+    auto unit_operand = [&](half_t v) { return half8_t{lq == 0 ? v : (half_t)0.f, (half_t)0.f, (half_t)0.f, (half_t)0.f, (half_t)0.f, (half_t)0.f, (half_t)0.f, (half_t)0.f}; };
+
+    // ---- results: rows of a unit, 16 bytes a lane
+    unsigned char *const piece = smem + C::ST * C::STAGE + wave * C::PIECE;
+    const int o_row = lane / C::O_CPR, o_cc = lane % C::O_CPR;
+    constexpr int O_STEP = 64 / C::O_CPR;
+    // where chunk o_cc of row `row` of unit u lies in the result's layout with `parts` blocks of outputs an a_i; valid?
+    auto place = [&](const At &p, int u, int row, int parts, int part, int64_t *k) {
+        if (LAST) {
+            const int a_i = p.grp / d, d_i = p.grp - a_i * d, bi = p.b0 + (wb * C::BT + u) * 32 + row, n = p.n0 + wn * 64 + o_cc * 8;
+            *k = (((int64_t)(a_i * parts + part) * b + min(bi, b - 1)) * d + d_i) * B + min(n, B - 8);
+            return bi < b && n < B;
+        }
+        const int n = p.n0 + (wn * C::NT + u) * 32 + row, bi = p.b0 + wb * (TB / C::WB) + o_cc * 8 / D;
+        *k = (int64_t)min(n, B - 1) * out_size * parts + ((int64_t)(p.grp * parts + part) * b + min(bi, b - 8 / D)) * D;
+        return n < B && bi < b;
+    };
+    uint4_t dhv[MODE ? C::UNITS : 1][C::O_IT];
+    auto load_dh = [&](int t) {
+        const At p = at(t);
+#pragma unroll
+        for (int u = 0; u < C::UNITS; ++u)
+#pragma unroll
+            for (int i = 0; i < C::O_IT; ++i) {
+                int64_t k;
+                place(p, u, i * O_STEP + o_row, 1, 0, &k);
+                dhv[MODE ? u : 0][i] = *(const uint4_t *)(dh + k);
+            }
+    };
+    auto wave_sync = [&]() {
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_wave_barrier();
+    };
+    // the lane's chunk q of its row in a piece
+    auto mine_at = [&](int q) { return (uint4_t *)(piece + l32 * (C::O_CPR * 16) + o_swizzle<C::O_CPR>(l32, q) * 16); };
+
+    float16_t acc[D][C::PARTS][C::BT][C::NT];
+    auto finish = [&](int t) {
+        const At p = at(t);
+        with_act(g.act, [&](auto act_of) {
+            constexpr int ACT = decltype(act_of)::value;
+#pragma unroll
+            for (int u = 0; u < C::UNITS; ++u) {
+                if constexpr (MODE == 1) {
+#pragma unroll
+                    for (int i = 0; i < C::O_IT; ++i) {
+                        const int row = i * O_STEP + o_row;
+                        *(uint4_t *)(piece + row * (C::O_CPR * 16) + o_swizzle<C::O_CPR>(row, o_cc) * 16) = dhv[u][i];
+                    }
+                    wave_sync();
+                }
+                // the lane's values of the unit: chunks of 8
+                constexpr int CHUNKS = LAST ? 4 : C::BT * D;
+                Run<half_t, 8> r1[MODE ? CHUNKS : 1];
+#pragma unroll
+                for (int k = 0; k < CHUNKS; ++k) {
+                    // LAST: j = k / 2, values 8 * (k % 2) ..; else tile i = k / D, values 8 q .. of (8 outputs x D)
+                    const int q = LAST ? k / 2 * 4 + lq * 2 + k % 2 : (k / D * 2 + lq) * D + k % D;
+                    Run<half_t, 8> in, r0;
+                    if constexpr (MODE == 1) in = __builtin_bit_cast(Run<half_t, 8>, *mine_at(q));
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const int m = LAST ? k % 2 * 8 + e : (k % D * 8 + e) / D, pl = LAST ? 0 : (k % D * 8 + e) % D;
+                        const float gate = LAST ? acc[0][0][u % C::BT][k / 2 % C::NT][m] : acc[pl][0][k / D % C::BT][u % C::NT][m];
+                        const float up = LAST ? acc[0][C::PARTS - 1][u % C::BT][k / 2 % C::NT][m] : acc[pl][0][k / D % C::BT][u % C::NT][8 + m];
+                        float slope = 0.f;
+                        const float v = activate<half_t, ACT, MODE == 1>(gate, slope);
+                        if constexpr (MODE == 0) {
+                            r0.e[e] = (half_t)(v * up);
+                        } else {
+                            const float f = (float)in.e[e];
+                            r0.e[e] = (half_t)(f * up * slope);
+                            r1[MODE ? k : 0].e[e] = (half_t)(f * v);
+                        }
+                    }
+                    *mine_at(q) = __builtin_bit_cast(uint4_t, r0);
+                }
+#pragma unroll
+                for (int part = 0; part <= MODE; ++part) {
+                    if (part == 1) {
+#pragma unroll
+                        for (int k = 0; k < CHUNKS; ++k) {
+                            const int q = LAST ? k / 2 * 4 + lq * 2 + k % 2 : (k / D * 2 + lq) * D + k % D;
+                            *mine_at(q) = __builtin_bit_cast(uint4_t, r1[MODE ? k : 0]);
+                        }
+                    }
+                    wave_sync();
+#pragma unroll
+                    for (int i = 0; i < C::O_IT; ++i) {
+                        const int row = i * O_STEP + o_row;
+                        const uint4_t v = *(const uint4_t *)(piece + row * (C::O_CPR * 16) + o_swizzle<C::O_CPR>(row, o_cc) * 16);
+                        int64_t k;
+                        if (place(p, u, row, MODE + 1, part, &k)) *(uint4_t *)(out + k) = v;
+                    }
+                    wave_sync();
+                }
+            }
+        });
+        return p.n0 + C::TN <= B && p.b0 + TB <= b;  // all of its stores went out
+    };
+
+    begin_loads();
+    load_bias(mine);
+#pragma unroll
+    for (int s = 0; s < C::ST - 1; ++s) issue();
+    int read = 0;        // slot that is multiplied next
+    int after = 0;       // stores of the tile before that may still be counted
+    bool early = false;  // so may the loads made early in it
+    for (int t = mine; t < last; t += stride) {
+        const half8_t one = unit_operand((half_t)1.f);
+#pragma unroll
+        for (int p = 0; p < D; ++p)
+#pragma unroll
+            for (int q = 0; q < C::PARTS; ++q)
+#pragma unroll
+                for (int i = 0; i < C::BT; ++i) {
+                    const half8_t v = unit_operand(bias ? bv[i * (C::BIASES / C::BT) + (LAST ? q : p)] : (half_t)0.f);
+#pragma unroll
+                    for (int j = 0; j < C::NT; ++j) {
+                        float16_t z;
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) z[e] = 0.f;
+                        acc[p][q][i][j] = LAST ? op<half_t>::mfma(one, v, z) : op<half_t>::mfma(v, one, z);
+                    }
+                }
+        for (int s = 0; s < steps; ++s) {
+            const bool st = s < C::ST - 1 && after > 0, ea = s > steps - C::ST + 1 || (s == 0 && early);
+            if (st && ea)
+                __builtin_amdgcn_s_waitcnt(vmcnt_imm(C::WAIT + C::STORES + C::EARLY));
+            else if (st)
+                __builtin_amdgcn_s_waitcnt(vmcnt_imm(C::WAIT + C::STORES));
+            else if (ea)
+                __builtin_amdgcn_s_waitcnt(vmcnt_imm(C::WAIT + C::EARLY));
+            else
+                __builtin_amdgcn_s_waitcnt(vmcnt_imm(C::WAIT));
+            __syncthreads();  // the slab landed for every wave, and everyone left the one before, whose place is filled next
+            issue();
+            if (s == steps - C::ST + 1) {
+                load_bias(t + stride < last ? t + stride : t);
+                if constexpr (MODE == 1) load_dh(t);
+            }
+            const uint32_t base = read * C::STAGE;
+            read = read + 1 == C::ST ? 0 : read + 1;
+            half8_t fx[D][C::NT];
+            if constexpr (LAST) {
+#pragma unroll
+                for (int j = 0; j < C::NT; ++j) fx[0][j] = outer(xa[j % (LAST ? C::NT : D)] + base, C::X_CPR * 16);
+            } else {
+#pragma unroll
+                for (int j = 0; j < C::NT; ++j) {
+                    uint4_t raw[D];
+#pragma unroll
+                    for (int p = 0; p < D; ++p) raw[p] = inner(xa[p] + base + j * 32 * C::X_CPR * 16);
+                    if constexpr (D == 1) {
+                        fx[0][j] = __builtin_bit_cast(half8_t, raw[0]);
+                    } else {
+                        uint4_t lo, hi;
+#pragma unroll
+                        for (int m = 0; m < 4; ++m) {
+                            const uint32_t even = raw[m / 2][2 * m % 4], odd = raw[m / 2][2 * m % 4 + 1];
+                            lo[m] = __builtin_amdgcn_perm(odd, even, 0x05040100u);
+                            hi[m] = __builtin_amdgcn_perm(odd, even, 0x07060302u);
+                        }
+                        fx[0][j] = __builtin_bit_cast(half8_t, lo);
+                        fx[D - 1][j] = __builtin_bit_cast(half8_t, hi);
+                    }
+                }
+            }
+#pragma unroll
+            for (int p = 0; p < D; ++p)
+#pragma unroll
+                for (int q = 0; q < C::PARTS; ++q)
+#pragma unroll
+                    for (int i = 0; i < C::BT; ++i) {
+                        const half8_t fw = outer(wa[q][i] + base + p * C::W_PLANE, C::W_CPR * 16);
+#pragma unroll
+                        for (int j = 0; j < C::NT; ++j)
+                            acc[p][q][i][j] = LAST ? op<half_t>::mfma(fx[p][j], fw, acc[p][q][i][j]) : op<half_t>::mfma(fw, fx[p][j], acc[p][q][i][j]);
+                    }
+        }
+        after = finish(t) ? 1 : 0;
+        early = true;
+    }
+    __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));  // repeated loads land before LDS goes to someone else
+}
+
 // ---- few rows ------------------------------------------------------------------------------------------
 // A workgroup takes 16 outputs of one block x 32 rows of the batch; its waves share c and add their sums in LDS, one
 // output and row a thread.  Operands come straight from global memory, element by element: any shape and alignment.
@@ -553,10 +926,43 @@ template <typename T, bool LAST, int D, bool ALL, int TB, int TN, int TK, int WB
     return launched();
 }
 
+template <bool LAST, int D, int TB, int MODE> int run_ring(const GatedArgs &g, hipStream_t s)
+{
+    typedef Ring<LAST, D, TB, MODE> C;
+    const int b_tiles = (g.b + TB - 1) / TB;
+    const int64_t tiles = (int64_t)b_tiles * g.a * (LAST ? g.d : 1) * ((g.batch + C::TN - 1) / C::TN);
+    if (tiles > 0x7ffffff0LL) return KSMM_ERR_TOO_LARGE;
+    const auto fn = &ks_gated_ring_kernel<LAST, D, TB, MODE>;
+    const int rc = ensure_dynamic_lds((const void *)fn, C::LDS_BYTES);
+    if (rc != KSMM_OK) return rc;
+    const int64_t grid = std::min<int64_t>(512, (tiles + 7) / 8 * 8);  // two workgroups a CU
+    hipLaunchKernelGGL(fn, dim3((unsigned)grid), dim3(C::THREADS), C::LDS_BYTES, s, g, b_tiles, (int)tiles);
+    return launched();
+}
+// vectors of 16 bytes everywhere, and offsets inside a tile that fit 32 bits
+bool ring_ok(const GatedArgs &g, bool last)
+{
+    const uintptr_t p = (uintptr_t)g.x | (uintptr_t)g.w | (uintptr_t)g.out | (uintptr_t)g.dh;
+    if ((p & 15) || g.b % 8 || g.c % 16 || g.c < 64 || (int64_t)g.d * g.c * 2 * g.b >= 1 << 29) return false;
+    if (last) return g.batch % 8 == 0 && 16 * (int64_t)g.d * g.batch < 1 << 29;
+    return g.d <= 2 && (int64_t)g.a * g.c * g.d * 128 < 1 << 29;
+}
+
 template <typename T, bool LAST, int MODE> int run(const GatedArgs &g, hipStream_t s)
 {
     constexpr int TK = sizeof(T) == 4 ? 16 : 32;
     if (g.batch <= 128 || g.b < 8) return run_few<T, LAST, MODE>(g, s);
+    if constexpr (sizeof(T) == 2) {
+        if (ring_ok(g, LAST)) {
+            const bool wide = g.b % 128 == 0 || g.b > 256;
+            if constexpr (LAST) {
+                return wide ? run_ring<true, 1, 128, MODE>(g, s) : run_ring<true, 1, 64, MODE>(g, s);
+            } else {
+                if (g.d == 2) return run_ring<false, 2, 64, MODE>(g, s);
+                return wide ? run_ring<false, 1, 128, MODE>(g, s) : run_ring<false, 1, 64, MODE>(g, s);
+            }
+        }
+    }
     if constexpr (LAST) {
         return run_tile<T, true, 1, false, 64, 128, TK, 2, 2, MODE>(g, s);
     } else {

@@ -88,6 +88,17 @@ def test_larger_batches(pattern, batch, bs_last, prec, act):
     check(pattern, batch, prec, act, True, bs_last)
 
 
+@pytest.mark.parametrize("bias", [True, False])
+@pytest.mark.parametrize("pattern,batch,bs_last", [
+    ((1, 64, 64, 2), 129, False), ((1, 72, 80, 2), 300, False), ((3, 136, 96, 2), 2000, False), ((1, 8, 64, 2), 9000, False),
+    ((1, 128, 64, 1), 1300, False), ((3, 72, 80, 1), 517, False), ((1, 264, 176, 1), 3001, False), ((2, 640, 128, 1), 4500, False),
+    ((1, 128, 64, 1), 1304, True), ((3, 72, 80, 2), 520, True), ((1, 264, 176, 1), 3008, True), ((2, 640, 128, 3), 1504, True),
+    ((1, 8, 64, 2), 136, True)])
+def test_aligned_fp16(pattern, batch, bs_last, bias):
+    """The ring of slabs: few and many tiles a workgroup, outputs and rows that end inside a tile, few and many slabs."""
+    check(pattern, batch, "fp16", "silu" if bias else "gelu", bias, bs_last)
+
+
 @pytest.mark.parametrize("bs_last", [False, True])
 def test_no_rows_and_more_axes(bs_last):
     from ksmm_amd import GatedKernel, KSGatedLinear
