@@ -343,7 +343,7 @@ int ksmm_gated_backward(const void *dh, const void *x, const void *w, const void
  * features, each for batch / groups consecutive rows of the tensors.  x NULL: r_out is the residual and is not
  * written.  n_out NULL: not wanted.  NULL gate and weight count as ones, NULL bias as zeros.
  * stats (NULL: not wanted): 4 x batch floats for the backward pass.
- * Batch-size-first rows of up to 32768 bytes; batch-size-last any number of features. */
+ * Batch-size-first rows of up to 8192 features; batch-size-last any number. */
 typedef enum ksmm_norm_kind { KSMM_NORM_RMS = 0, KSMM_NORM_LAYER = 1 } ksmm_norm_kind;
 typedef struct ksmm_norm_desc {
     const void *x, *residual, *gate, *post_weight, *weight, *bias;

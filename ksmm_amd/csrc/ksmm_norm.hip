@@ -90,71 +90,99 @@ __device__ __forceinline__ float project(const NormArgs &a, float dv, float v, f
     return a.features == 1 && !a.layer ? dv * (a.eps * rho * rho) : fmaf(-v, m2, dv) - m1;
 }
 
-// ---- 16 bytes of a row, at element alignment; past its end: zeros, and nothing stored --------------
-template <typename T> constexpr int EPV = 16 / (int)sizeof(T);
-template <typename T> union Piece {
-    uint4_t v;
-    T e[EPV<T>];
+// ---- E elements of a row, at element alignment; past its end: zeros, and nothing stored ------------
+// (WHOLE: E divides the row, and a piece is inside or past its end as a whole)
+template <typename T, int E> struct Piece {
+    T e[E];
 };
-template <typename T> __device__ __forceinline__ Piece<T> load_piece(const T *row, int col, int end)
+template <bool WHOLE, typename T, int E> __device__ __forceinline__ void load_piece(Piece<T, E> &p, const T *row, int col, int end)
 {
-    Piece<T> p;
-    if (col + EPV<T> <= end) {
-        __builtin_memcpy(&p.v, row + col, 16);
+    if (WHOLE ? col < end : col + E <= end) {
+        __builtin_memcpy(&p, row + col, sizeof(p));
     } else {
-        p.v = uint4_t{0u, 0u, 0u, 0u};
 #pragma unroll
-        for (int e = 0; e < EPV<T>; ++e)
-            if (col + e < end) p.e[e] = row[col + e];
+        for (int e = 0; e < E; ++e) p.e[e] = !WHOLE && col + e < end ? row[col + e] : (T)0.f;
     }
-    return p;
 }
-template <typename T> __device__ __forceinline__ void store_piece(T *row, int col, int end, const Piece<T> &p)
+template <bool WHOLE, typename T, int E> __device__ __forceinline__ void store_piece(T *row, int col, int end, const Piece<T, E> &p)
 {
-    if (col + EPV<T> <= end) {
-        __builtin_memcpy(row + col, &p.v, 16);
-    } else {
+    if (WHOLE ? col < end : col + E <= end) {
+        __builtin_memcpy(row + col, &p, sizeof(p));
+    } else if (!WHOLE) {
 #pragma unroll
-        for (int e = 0; e < EPV<T>; ++e)
+        for (int e = 0; e < E; ++e)
             if (col + e < end) row[col + e] = p.e[e];
     }
 }
+// keeps a loop's invariant pieces as they were loaded: the compiler would hold 16-bit ones converted, in twice the registers
+template <typename T, int E> __device__ __forceinline__ void opaque(Piece<T, E> &p)
+{
+    typedef uint32_t words __attribute__((ext_vector_type(E * sizeof(T) / 4)));
+    words w = __builtin_bit_cast(words, p);
+    asm volatile("" : "+v"(w));
+    p = __builtin_bit_cast(Piece<T, E>, w);
+}
 
 // ---- batch-size-first -------------------------------------------------------------------------------
-// A row is held by TPR threads, VPL pieces each: TPR * VPL pieces are enough for it.  Rows are dealt in ranges: the
-// workgroup's row r of a range starts at range * range_rows.  (Threads past the end of a row hold zeros.)
-template <typename T, int TPR, int VPL>
+// A row is held by TPR threads, VPL pieces of E elements each: TPR * VPL * E are enough for it.  Rows are dealt in ranges:
+// the workgroup's range starts at range * range_rows.  (Threads past the end of a row hold zeros.)
+template <int TPR> __device__ __forceinline__ int row_slot()
+{
+    const int s = threadIdx.x / TPR;
+    return TPR >= 64 ? __builtin_amdgcn_readfirstlane(s) : s;  // a row's address is uniform
+}
+
+template <typename T, int E, int TPR, int VPL, bool WHOLE>
 __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void ks_norm_rows_kernel(NormArgs a, int64_t range_rows)
 {
-    constexpr int E = EPV<T>, ROWS = TPR < 256 ? 256 / TPR : 1;
+    constexpr int ROWS = TPR < 256 ? 256 / TPR : 1;
     __shared__ float red[4 * MAX_WAVES];
     RowSum<TPR> sum{red};
     const int t = threadIdx.x % TPR, H = a.features;
     const float inv = 1.f / (float)H;
     const T *x = (const T *)a.x, *res = (const T *)a.residual, *gate = (const T *)a.gate, *post = (const T *)a.post_weight;
     const int64_t first = (int64_t)blockIdx.x * range_rows, last = min(a.batch, first + range_rows);
-    Piece<T> w[VPL], b[VPL], pw[VPL], g[VPL];
-    int64_t group = -1;
+    Piece<T, E> w[VPL], b[VPL], pw[VPL], g[VPL];
+    int64_t group_end = first;  // the gate that is held is good for rows before this one
 #pragma unroll
     for (int j = 0; j < VPL; ++j) {
         const int col = (j * TPR + t) * E;
-        if (a.n_out && a.weight) w[j] = load_piece<T>((const T *)a.weight, col, H);
-        if (a.n_out && a.bias) b[j] = load_piece<T>((const T *)a.bias, col, H);
-        if (x && post) pw[j] = load_piece<T>(post, col, H);
+#pragma unroll
+        for (int e = 0; e < E; ++e) w[j].e[e] = b[j].e[e] = pw[j].e[e] = g[j].e[e] = (T)0.f;  // (not used where they are not loaded)
+        if (a.n_out && a.weight) load_piece<WHOLE>(w[j], (const T *)a.weight, col, H);
+        if (a.n_out && a.bias) load_piece<WHOLE>(b[j], (const T *)a.bias, col, H);
+        if (x && post) load_piece<WHOLE>(pw[j], post, col, H);
     }
     // (rows of a workgroup wider than a wave add up behind barriers: all of its threads take the same ones)
-    for (int64_t row = first + threadIdx.x / TPR; row < last; row += ROWS) {
-        Piece<T> rp[VPL], xp[VPL];
+    struct Operands {
+        Piece<T, E> r[VPL], x[VPL];
+    };
+    auto fetch = [&](Operands &o, int64_t row) {
 #pragma unroll
         for (int j = 0; j < VPL; ++j) {
             const int col = (j * TPR + t) * E;
-            rp[j] = load_piece<T>(res + row * H, col, H);
-            if (x) xp[j] = load_piece<T>(x + row * H, col, H);
+            load_piece<WHOLE>(o.r[j], res + row * H, col, H);
+            if (x) load_piece<WHOLE>(o.x[j], x + row * H, col, H);
         }
-        if (x && gate && row / a.group_rows != group) {
-            group = row / a.group_rows;
+    };
+    Operands next;  // a row's operands are asked for while the one before is worked on
+    const int64_t start = first + row_slot<TPR>();
+    if (start < last) fetch(next, start);
+    for (int64_t row = start; row < last; row += ROWS) {
+        const Operands now = next;
+        if (row + ROWS < last) fetch(next, row + ROWS);
+        const auto &rp = now.r, &xp = now.x;
 #pragma unroll
-            for (int j = 0; j < VPL; ++j) g[j] = load_piece<T>(gate + group * H, (j * TPR + t) * E, H);
+        for (int j = 0; j < VPL; ++j) {
+            opaque(w[j]);
+            opaque(b[j]);
+            opaque(pw[j]);
+        }
+        if (x && gate && row >= group_end) {
+            const int64_t group = row / a.group_rows;
+            group_end = (group + 1) * a.group_rows;
+#pragma unroll
+            for (int j = 0; j < VPL; ++j) load_piece<WHOLE>(g[j], gate + group * H, (j * TPR + t) * E, H);
         }
         float r[VPL][E];
         float mean_x = 0.f, rho_x = 1.f;
@@ -179,20 +207,22 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void ks_norm_rows_kernel(Nor
                 rho_x = rsqrtf(fmaf(sum.one(s), inv, a.eps));
             }
 #pragma unroll
-            for (int j = 0; j < VPL; ++j)
+            for (int j = 0; j < VPL; ++j) {
+                opaque(g[j]);
 #pragma unroll
                 for (int e = 0; e < E; ++e) {
                     float p = (float)xp[j].e[e];
                     if (post) p = (p - mean_x) * rho_x * (float)pw[j].e[e];
                     r[j][e] = fmaf(gate ? a.alpha * (float)g[j].e[e] : a.alpha, p, (float)rp[j].e[e]);
                 }
+            }
             if (a.r_out) {
 #pragma unroll
                 for (int j = 0; j < VPL; ++j) {
-                    Piece<T> o;
+                    Piece<T, E> o;
 #pragma unroll
                     for (int e = 0; e < E; ++e) o.e[e] = (T)r[j][e];
-                    store_piece<T>((T *)a.r_out + row * H, (j * TPR + t) * E, H, o);
+                    store_piece<WHOLE>((T *)a.r_out + row * H, (j * TPR + t) * E, H, o);
                 }
             }
         } else {
@@ -222,7 +252,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void ks_norm_rows_kernel(Nor
             rho_r = rsqrtf(fmaf(sum.one(s), inv, a.eps));
 #pragma unroll
             for (int j = 0; j < VPL; ++j) {
-                Piece<T> o;
+                Piece<T, E> o;
 #pragma unroll
                 for (int e = 0; e < E; ++e) {
                     float v = (r[j][e] - mean_r) * rho_r;
@@ -230,7 +260,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void ks_norm_rows_kernel(Nor
                     if (a.bias) v += (float)b[j].e[e];
                     o.e[e] = (T)v;
                 }
-                store_piece<T>((T *)a.n_out + row * H, (j * TPR + t) * E, H, o);
+                store_piece<WHOLE>((T *)a.n_out + row * H, (j * TPR + t) * E, H, o);
             }
         }
         if (a.stats && t == 0) {
@@ -243,34 +273,44 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void ks_norm_rows_kernel(Nor
 }
 
 // Gradients.  Workgroup = range of rows: `parts` ranges share a gate's group, or a range is `groups_per` whole groups
-// (parts == 1).  Partial sums: slice blockIdx.x of each quantity; dgate's lie [part][group][feature].
-template <typename T, int TPR, int VPL>
+// (parts == 1).  Partial sums: slice blockIdx.x of each quantity; dgate's lie [part][group][feature].  POST: x has a norm;
+// MEAN: there is a bias, or a mean is taken.
+// One sum serves two gradients: with S = sum D u over the rows of a gate, dgate = alpha post_weight S and, of these rows,
+// dpost_weight = alpha gate S.  What a row needs twice is converted, or computed, twice: registers decide how many
+// rows are on their way from memory.
+template <typename T, int E, int TPR, int VPL, bool WHOLE, bool POST, bool MEAN>
 __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void ks_norm_rows_bwd_kernel(NormArgs a, NormGrads d, NormSplit sp)
 {
-    constexpr int E = EPV<T>, ROWS = TPR < 256 ? 256 / TPR : 1, WIDE = VPL * E;
+    constexpr int THREADS = TPR < 256 ? 256 : TPR, ROWS = TPR < 256 ? 256 / TPR : 1, WIDE = VPL * E;
     __shared__ float red[4 * MAX_WAVES];
     __shared__ float wide[ROWS > 1 ? 256 * WIDE : 1];
+    __shared__ float post_sum[POST ? THREADS * WIDE : 1];  // of the groups before
     RowSum<TPR> sum{red};
-    const int t = threadIdx.x % TPR, slot = threadIdx.x / TPR, H = a.features;
+    const int t = threadIdx.x % TPR, slot = row_slot<TPR>(), H = a.features;
     const float inv = 1.f / (float)H;
-    const T *x = (const T *)a.x, *gate = (const T *)a.gate, *post = (const T *)a.post_weight;
-    const T *dr_in = (const T *)d.dr_out, *dn = (const T *)d.dn_out;
-    Piece<T> w[VPL], pw[VPL], g[VPL];
+    const T *const x = (const T *)a.x, *const gate = (const T *)a.gate;
+    const T *const dr_in = (const T *)d.dr_out, *const dn = (const T *)d.dn_out;
+    Piece<T, E> w[VPL], pw[VPL], g[VPL];
 #pragma unroll
     for (int j = 0; j < VPL; ++j) {
         const int col = (j * TPR + t) * E;
-        if (dn && a.weight) w[j] = load_piece<T>((const T *)a.weight, col, H);
-        if (x && post) pw[j] = load_piece<T>(post, col, H);
-    }
-    float s_w[WIDE], s_b[WIDE], s_p[WIDE], s_g[WIDE];
 #pragma unroll
-    for (int i = 0; i < WIDE; ++i) s_w[i] = s_b[i] = s_p[i] = s_g[i] = 0.f;
+        for (int e = 0; e < E; ++e) w[j].e[e] = pw[j].e[e] = g[j].e[e] = (T)1.f;
+        if (dn && a.weight) load_piece<WHOLE>(w[j], (const T *)a.weight, col, H);
+        if (POST) load_piece<WHOLE>(pw[j], (const T *)a.post_weight, col, H);
+    }
+    float s_w[WIDE], s_b[MEAN ? WIDE : 1], s_u[WIDE];
+#pragma unroll
+    for (int i = 0; i < WIDE; ++i) {
+        s_w[i] = s_b[MEAN ? i : 0] = s_u[i] = 0.f;
+        if (POST) post_sum[i * THREADS + threadIdx.x] = 0.f;
+    }
 
-    // the workgroup's sum of one quantity, stored to a row of floats
-    auto flush = [&](const float *s, float *to) {
+    // the workgroup's sum of one quantity (value i of each thread), stored to a row of floats
+    auto flush = [&](auto value, float *to) {
         if constexpr (ROWS > 1) {
 #pragma unroll
-            for (int i = 0; i < WIDE; ++i) wide[i * 256 + threadIdx.x] = s[i];
+            for (int i = 0; i < WIDE; ++i) wide[i * 256 + threadIdx.x] = value(i);
             __syncthreads();
             for (int i = threadIdx.x; i < TPR * WIDE; i += 256) {
                 const int tt = i % TPR, k = i / TPR, col = (k / E * TPR + tt) * E + k % E;
@@ -286,7 +326,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void ks_norm_rows_bwd_kernel
 #pragma unroll
                 for (int e = 0; e < E; ++e) {
                     const int col = (j * TPR + t) * E + e;
-                    if (col < H) to[col] = s[j * E + e];
+                    if (col < H) to[col] = value(j * E + e);
                 }
         }
     };
@@ -299,109 +339,127 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void ks_norm_rows_bwd_kernel
         const int64_t last = min(base + a.group_rows, first + sp.part_rows);
         if (x && gate) {
 #pragma unroll
-            for (int j = 0; j < VPL; ++j) g[j] = load_piece<T>(gate + (sp.one_gate ? 0 : group * H), (j * TPR + t) * E, H);
+            for (int j = 0; j < VPL; ++j) load_piece<WHOLE>(g[j], gate + (sp.one_gate ? 0 : group * H), (j * TPR + t) * E, H);
         }
-        for (int64_t row = first + slot; row < last; row += ROWS) {
-            Piece<T> rp[VPL], xp[VPL], np[VPL], dp[VPL];
+        // a row's operands are asked for while the one before is worked on
+        struct Operands {
+            Piece<T, E> r[VPL], x[VPL], n[VPL], d[VPL];
+            float mean_x, rho_x, mean_r, rho_r;
+        };
+        auto fetch = [&](Operands &o, int64_t row) {
 #pragma unroll
             for (int j = 0; j < VPL; ++j) {
                 const int col = (j * TPR + t) * E;
+                if (x) load_piece<WHOLE>(o.x[j], x + row * H, col, H);
                 if (dn) {
-                    np[j] = load_piece<T>(dn + row * H, col, H);
-                    rp[j] = load_piece<T>((const T *)a.residual + row * H, col, H);
+                    load_piece<WHOLE>(o.r[j], (const T *)a.residual + row * H, col, H);
+                    load_piece<WHOLE>(o.n[j], dn + row * H, col, H);
                 }
-                if (x) xp[j] = load_piece<T>(x + row * H, col, H);
-                if (dr_in) dp[j] = load_piece<T>(dr_in + row * H, col, H);
+                if (dr_in) load_piece<WHOLE>(o.d[j], dr_in + row * H, col, H);
             }
-            const float mean_x = a.stats[row], rho_x = a.stats[a.batch + row];
-            const float mean_r = a.stats[2 * a.batch + row], rho_r = a.stats[3 * a.batch + row];
-            float u[VPL][E], D[VPL][E];
-#pragma unroll
-            for (int j = 0; j < VPL; ++j)
-#pragma unroll
-                for (int e = 0; e < E; ++e) {
-                    u[j][e] = 0.f;
-                    if (x) u[j][e] = post ? ((float)xp[j].e[e] - mean_x) * rho_x : (float)xp[j].e[e];
-                    D[j][e] = dr_in ? (float)dp[j].e[e] : 0.f;
-                }
+            o.mean_x = a.stats[row];
+            o.rho_x = a.stats[a.batch + row];
+            o.mean_r = a.stats[2 * a.batch + row];
+            o.rho_r = a.stats[3 * a.batch + row];
+        };
+        Operands next;
+        if (first + slot < last) fetch(next, first + slot);
+        for (int64_t row = first + slot; row < last; row += ROWS) {
+            const Operands now = next;
+            if (row + ROWS < last) fetch(next, row + ROWS);
+            const auto &rp = now.r, &xp = now.x, &np = now.n, &dp = now.d;
+            const float mean_x = now.mean_x, rho_x = now.rho_x, mean_r = now.mean_r, rho_r = now.rho_r;
+            auto u_of = [&](int j, int e) { return POST ? ((float)xp[j].e[e] - mean_x) * rho_x : (float)xp[j].e[e]; };
+            auto gate_of = [&](int j, int e) { return a.alpha * (float)g[j].e[e]; };  // (ones without a gate)
+            float v[VPL][E], m1 = 0.f, m2 = 0.f;
             if (dn) {
-                float v[VPL][E], dv[VPL][E], m1 = 0.f, m2 = 0.f;
-#pragma unroll
-                for (int j = 0; j < VPL; ++j)
-#pragma unroll
-                    for (int e = 0; e < E; ++e) {
-                        const float p = x ? (post ? u[j][e] * (float)pw[j].e[e] : u[j][e]) : 0.f;
-                        const float r = x ? fmaf(gate ? a.alpha * (float)g[j].e[e] : a.alpha, p, (float)rp[j].e[e]) : (float)rp[j].e[e];
-                        const float n = (float)np[j].e[e];  // (zero past the end, and so is what it multiplies)
-                        v[j][e] = (r - mean_r) * rho_r;
-                        dv[j][e] = a.weight ? n * (float)w[j].e[e] : n;
-                        m1 += dv[j][e];
-                        m2 = fmaf(dv[j][e], v[j][e], m2);
-                        s_w[j * E + e] = fmaf(n, v[j][e], s_w[j * E + e]);
-                        s_b[j * E + e] += n;
-                    }
-                sum.two(m1, m2);
-                m1 = a.layer ? m1 * inv : 0.f;
-                m2 *= inv;
-#pragma unroll
-                for (int j = 0; j < VPL; ++j)
-#pragma unroll
-                    for (int e = 0; e < E; ++e) D[j][e] = fmaf(rho_r, project(a, dv[j][e], v[j][e], m1, m2, rho_r), D[j][e]);
-            }
-            if (d.dresidual) {
 #pragma unroll
                 for (int j = 0; j < VPL; ++j) {
-                    Piece<T> o;
-#pragma unroll
-                    for (int e = 0; e < E; ++e) o.e[e] = (T)D[j][e];
-                    store_piece<T>((T *)d.dresidual + row * H, (j * TPR + t) * E, H, o);
-                }
-            }
-            if (x && (d.dx || d.dgate || d.dpost_weight)) {
-                float m1 = 0.f, m2 = 0.f;
-#pragma unroll
-                for (int j = 0; j < VPL; ++j)
+                    opaque(w[j]);
+                    opaque(pw[j]);
+                    opaque(g[j]);
 #pragma unroll
                     for (int e = 0; e < E; ++e) {
-                        // (past the end D holds the rest of a mean: nothing may be added there)
-                        const float D0 = (j * TPR + t) * E + e < H ? D[j][e] : 0.f;
-                        const float p = post ? u[j][e] * (float)pw[j].e[e] : u[j][e];
-                        s_g[j * E + e] = fmaf(a.alpha * D0, p, s_g[j * E + e]);
-                        float q = (gate ? a.alpha * (float)g[j].e[e] : a.alpha) * D0;
-                        if (post) {
-                            s_p[j * E + e] = fmaf(q, u[j][e], s_p[j * E + e]);
-                            q *= (float)pw[j].e[e];
-                            m1 += q;
-                            m2 = fmaf(q, u[j][e], m2);
-                        }
-                        D[j][e] = q;
+                        float r = (float)rp[j].e[e];
+                        if (x) r = fmaf(gate_of(j, e), POST ? u_of(j, e) * (float)pw[j].e[e] : u_of(j, e), r);
+                        const float n = (float)np[j].e[e];  // (zero past the end, and so is what it multiplies)
+                        v[j][e] = (r - mean_r) * rho_r;
+                        const float dv = n * (float)w[j].e[e];
+                        if (MEAN) m1 += dv;
+                        m2 = fmaf(dv, v[j][e], m2);
+                        s_w[j * E + e] = fmaf(n, v[j][e], s_w[j * E + e]);
+                        if (MEAN) s_b[MEAN ? j * E + e : 0] += n;
                     }
-                if (post) {
-                    sum.two(m1, m2);
-                    m1 = a.layer ? m1 * inv : 0.f;
-                    m2 *= inv;
                 }
-                if (d.dx) {
+                if (MEAN)
+                    sum.two(m1, m2);
+                else
+                    m2 = sum.one(m2);
+                m1 = MEAN && a.layer ? m1 * inv : 0.f;
+                m2 *= inv;
+            }
+            float k1 = 0.f, k2 = 0.f;
 #pragma unroll
-                    for (int j = 0; j < VPL; ++j) {
-                        Piece<T> o;
+            for (int j = 0; j < VPL; ++j) {
+                opaque(w[j]);
+                opaque(pw[j]);
+                opaque(g[j]);
+                Piece<T, E> o;
 #pragma unroll
-                        for (int e = 0; e < E; ++e) o.e[e] = (T)(post ? rho_x * project(a, D[j][e], u[j][e], m1, m2, rho_x) : D[j][e]);
-                        store_piece<T>((T *)d.dx + row * H, (j * TPR + t) * E, H, o);
+                for (int e = 0; e < E; ++e) {
+                    float D = dr_in ? (float)dp[j].e[e] : 0.f;
+                    if (dn) D = fmaf(rho_r, project(a, (float)np[j].e[e] * (float)w[j].e[e], v[j][e], m1, m2, rho_r), D);
+                    o.e[e] = (T)D;
+                    // (past the end D holds the rest of a mean: nothing may be added there)
+                    const bool in = WHOLE ? (j * TPR + t) * E < H : (j * TPR + t) * E + e < H;
+                    D = in ? D : 0.f;
+                    if (x) {
+                        const float u = u_of(j, e);
+                        s_u[j * E + e] = fmaf(D, u, s_u[j * E + e]);
+                        float q = gate_of(j, e) * D;
+                        if (POST) {
+                            q *= (float)pw[j].e[e];
+                            if (MEAN) k1 += q;
+                            k2 = fmaf(q, u, k2);
+                        }
+                        v[j][e] = q;
                     }
+                }
+                if (d.dresidual) store_piece<WHOLE>((T *)d.dresidual + row * H, (j * TPR + t) * E, H, o);
+            }
+            if (x && d.dx) {
+                if (POST) {
+                    if (MEAN)
+                        sum.two(k1, k2);
+                    else
+                        k2 = sum.one(k2);
+                    k1 = MEAN && a.layer ? k1 * inv : 0.f;
+                    k2 *= inv;
+                }
+#pragma unroll
+                for (int j = 0; j < VPL; ++j) {
+                    Piece<T, E> o;
+#pragma unroll
+                    for (int e = 0; e < E; ++e) o.e[e] = (T)(POST ? rho_x * project(a, v[j][e], u_of(j, e), k1, k2, rho_x) : v[j][e]);
+                    store_piece<WHOLE>((T *)d.dx + row * H, (j * TPR + t) * E, H, o);
                 }
             }
         }
-        if (d.dgate && !sp.one_gate) {
-            flush(s_g, d.dgate + ((int64_t)part * sp.groups + group) * H);
+        if (x) {
+            if (d.dgate)
+                flush([&](int i) { return a.alpha * (POST ? (float)pw[i / E].e[i % E] : 1.f) * s_u[i]; },
+                      d.dgate + (sp.one_gate ? (int64_t)blockIdx.x : (int64_t)part * sp.groups + group) * H);
+            if (POST) {
 #pragma unroll
-            for (int i = 0; i < WIDE; ++i) s_g[i] = 0.f;
+                for (int i = 0; i < WIDE; ++i) post_sum[i * THREADS + threadIdx.x] += a.alpha * (float)g[i / E].e[i % E] * s_u[i];
+            }
+#pragma unroll
+            for (int i = 0; i < WIDE; ++i) s_u[i] = 0.f;
         }
     }
-    if (d.dweight) flush(s_w, d.dweight + (int64_t)blockIdx.x * H);
-    if (d.dbias) flush(s_b, d.dbias + (int64_t)blockIdx.x * H);
-    if (d.dpost_weight) flush(s_p, d.dpost_weight + (int64_t)blockIdx.x * H);
-    if (d.dgate && sp.one_gate) flush(s_g, d.dgate + (int64_t)blockIdx.x * H);
+    if (d.dweight) flush([&](int i) { return s_w[i]; }, d.dweight + (int64_t)blockIdx.x * H);
+    if (MEAN && d.dbias) flush([&](int i) { return s_b[MEAN ? i : 0]; }, d.dbias + (int64_t)blockIdx.x * H);
+    if (POST && d.dpost_weight) flush([&](int i) { return post_sum[POST ? i * THREADS + threadIdx.x : 0]; }, d.dpost_weight + (int64_t)blockIdx.x * H);
 }
 
 // ---- batch-size-last --------------------------------------------------------------------------------
@@ -661,24 +719,34 @@ __global__ __launch_bounds__(256) void ks_norm_cols_gate_kernel(NormArgs a, cons
 // ---- choices ------------------------------------------------------------------------------------------
 // ranges of rows that fill the chip: workgroups of 4 waves, 2 of which fit a CU in the backward pass
 constexpr int64_t FWD_RANGES = 2048, BWD_RANGES = 768;
-// widest batch-size-first row that the kernels hold (elements of 4 bytes)
+// widest batch-size-first row that the kernels hold
 constexpr int64_t WIDEST = 8192;
 
-int row_threads(int64_t features, int dtype)
+template <int E, int TPR, int VPL> struct Rows {
+    static constexpr int e = E, tpr = TPR, vpl = VPL;
+};
+// The kernel that holds a row in the fewest values a thread (8 to 16): fp16 768 features in 12 a lane, 3 pieces of 8 bytes,
+// are 54 us backward with both norms, in 2 pieces of 16 bytes, a third of them empty, 152.
+template <typename T, typename F> int with_rows(int64_t features, F f)
 {
-    const int64_t pieces = (features * (int64_t)dtype_size(dtype) + 15) / 16;
-    return pieces <= 16 ? 16 : pieces <= 128 ? 64 : pieces <= 512 ? 256 : pieces <= 2048 ? 1024 : 0;
-}
-
-template <typename T, typename F> int with_rows(int64_t features, int dtype, F f)
-{
-    const int tpr = row_threads(features, dtype);
-    const bool one = features * (int64_t)sizeof(T) <= (int64_t)tpr * 16;
-    switch (tpr) {
-    case 16: return f(std::integral_constant<int, 16>(), std::integral_constant<int, 1>());
-    case 64: return one ? f(std::integral_constant<int, 64>(), std::integral_constant<int, 1>()) : f(std::integral_constant<int, 64>(), std::integral_constant<int, 2>());
-    case 256: return one ? f(std::integral_constant<int, 256>(), std::integral_constant<int, 1>()) : f(std::integral_constant<int, 256>(), std::integral_constant<int, 2>());
-    case 1024: return one ? f(std::integral_constant<int, 1024>(), std::integral_constant<int, 1>()) : f(std::integral_constant<int, 1024>(), std::integral_constant<int, 2>());
+    constexpr int E = 16 / (int)sizeof(T);
+    if constexpr (sizeof(T) == 2) {
+        if (features <= 128) return f(Rows<E, 16, 1>());
+        if (features <= 512) return f(Rows<E, 64, 1>());
+        if (features <= 768) return f(Rows<4, 64, 3>());
+        if (features <= 1024) return f(Rows<E, 64, 2>());
+        if (features <= 2048) return f(Rows<E, 256, 1>());
+        if (features <= 4096) return f(Rows<E, 256, 2>());
+        if (features <= 8192) return f(Rows<E, 1024, 1>());
+    } else {
+        if (features <= 64) return f(Rows<E, 16, 1>());
+        if (features <= 256) return f(Rows<E, 64, 1>());
+        if (features <= 512) return f(Rows<E, 64, 2>());
+        if (features <= 768) return f(Rows<E, 64, 3>());
+        if (features <= 1024) return f(Rows<E, 256, 1>());
+        if (features <= 2048) return f(Rows<E, 256, 2>());
+        if (features <= 4096) return f(Rows<E, 1024, 1>());
+        if (features <= 8192) return f(Rows<E, 1024, 2>());
     }
     return KSMM_ERR_TOO_LARGE;
 }
@@ -709,7 +777,7 @@ NormSplit split_rows(int64_t batch, int64_t groups)
 
 int launched() { return hipGetLastError() == hipSuccess ? KSMM_OK : KSMM_ERR_LAUNCH; }
 
-template <typename T> int forward(const NormArgs &a, int dtype, int bs_last, hipStream_t stream)
+template <typename T> int forward(const NormArgs &a, int bs_last, hipStream_t stream)
 {
     if (bs_last)
         return with_cols(a.features, [&](auto fpt) {
@@ -717,16 +785,18 @@ template <typename T> int forward(const NormArgs &a, int dtype, int bs_last, hip
                                dim3(COL_THREADS), 0, stream, a);
             return launched();
         });
-    return with_rows<T>(a.features, dtype, [&](auto tpr, auto vpl) {
-        constexpr int TPR = decltype(tpr)::value, ROWS = TPR < 256 ? 256 / TPR : 1;
+    return with_rows<T>(a.features, [&](auto how) {
+        typedef decltype(how) R;
+        constexpr int TPR = R::tpr, ROWS = TPR < 256 ? 256 / TPR : 1;
         const int64_t steps = (a.batch + ROWS - 1) / ROWS, per = (steps + FWD_RANGES - 1) / FWD_RANGES * ROWS;
-        hipLaunchKernelGGL((ks_norm_rows_kernel<T, TPR, decltype(vpl)::value>), dim3((unsigned)((a.batch + per - 1) / per)),
+        const auto fn = a.features % R::e ? &ks_norm_rows_kernel<T, R::e, TPR, R::vpl, false> : &ks_norm_rows_kernel<T, R::e, TPR, R::vpl, true>;
+        hipLaunchKernelGGL(fn, dim3((unsigned)((a.batch + per - 1) / per)),
                            dim3(TPR < 256 ? 256 : TPR), 0, stream, a, per);
         return launched();
     });
 }
 
-template <typename T> int backward(const NormArgs &a, const NormGrads &partial, const NormSplit &sp, int dtype, int bs_last, hipStream_t stream)
+template <typename T> int backward(const NormArgs &a, const NormGrads &partial, const NormSplit &sp, int bs_last, hipStream_t stream)
 {
     if (bs_last)
         return with_cols(a.features, [&](auto fpt) {
@@ -734,10 +804,19 @@ template <typename T> int backward(const NormArgs &a, const NormGrads &partial, 
                                dim3(COL_THREADS), 0, stream, a, partial);
             return launched();
         });
-    return with_rows<T>(a.features, dtype, [&](auto tpr, auto vpl) {
-        constexpr int TPR = decltype(tpr)::value;
-        hipLaunchKernelGGL((ks_norm_rows_bwd_kernel<T, TPR, decltype(vpl)::value>), dim3((unsigned)sp.ranges), dim3(TPR < 256 ? 256 : TPR), 0,
-                           stream, a, partial, sp);
+    return with_rows<T>(a.features, [&](auto how) {
+        typedef decltype(how) R;
+        const bool post = a.post_weight != nullptr, mean = a.layer || partial.dbias;
+        constexpr int E = R::e, TPR = R::tpr, VPL = R::vpl;
+        auto fn = &ks_norm_rows_bwd_kernel<T, E, TPR, VPL, false, true, true>;
+        if (a.features % E) {
+            if (!post) fn = &ks_norm_rows_bwd_kernel<T, E, TPR, VPL, false, false, true>;
+        } else if (mean) {
+            fn = post ? &ks_norm_rows_bwd_kernel<T, E, TPR, VPL, true, true, true> : &ks_norm_rows_bwd_kernel<T, E, TPR, VPL, true, false, true>;
+        } else {
+            fn = post ? &ks_norm_rows_bwd_kernel<T, E, TPR, VPL, true, true, false> : &ks_norm_rows_bwd_kernel<T, E, TPR, VPL, true, false, false>;
+        }
+        hipLaunchKernelGGL(fn, dim3((unsigned)sp.ranges), dim3(R::tpr < 256 ? 256 : R::tpr), 0, stream, a, partial, sp);
         return launched();
     });
 }
@@ -767,7 +846,7 @@ int check(const ksmm_norm_desc *d, int64_t batch, int64_t features, int dtype, i
     if (dtype != KSMM_F32 && dtype != KSMM_F16) return KSMM_ERR_BAD_DTYPE;
     if (d->kind != KSMM_NORM_RMS && d->kind != KSMM_NORM_LAYER) return KSMM_ERR_BAD_EPILOGUE;
     if (!d->residual) return KSMM_ERR_NULL_POINTER;
-    if (features > (bs_last ? 0x7fffffffLL / 64 : WIDEST * 4 / (int64_t)dtype_size(dtype))) return KSMM_ERR_TOO_LARGE;
+    if (features > (bs_last ? 0x7fffffffLL / 64 : WIDEST)) return KSMM_ERR_TOO_LARGE;
     if (batch > (1LL << 31) || batch * features > (1LL << 40)) return KSMM_ERR_TOO_LARGE;
     return KSMM_OK;
 }
@@ -808,7 +887,7 @@ int ksmm_residual_norm_forward(const ksmm_norm_desc *desc, void *r_out, void *n_
     a.r_out = desc->x ? r_out : nullptr;
     a.n_out = n_out;
     a.stats = stats;
-    return dtype == KSMM_F32 ? forward<float>(a, dtype, bs_last, (hipStream_t)stream) : forward<half_t>(a, dtype, bs_last, (hipStream_t)stream);
+    return dtype == KSMM_F32 ? forward<float>(a, bs_last, (hipStream_t)stream) : forward<half_t>(a, bs_last, (hipStream_t)stream);
 }
 
 int64_t ksmm_residual_norm_backward_workspace(int64_t batch, int64_t features, int64_t groups, int dtype, int bs_last)
@@ -845,7 +924,7 @@ int ksmm_residual_norm_backward(const ksmm_norm_desc *desc, const float *stats, 
     p.dbias = dbias && dn_out ? (float *)(ws + l.slice_bytes) : nullptr;
     p.dpost_weight = dpost_weight ? (float *)(ws + 2 * l.slice_bytes) : nullptr;
     p.dgate = dgate && !gate_alone ? (float *)(ws + 3 * l.slice_bytes) : nullptr;
-    int st = dtype == KSMM_F32 ? backward<float>(a, p, l.split, dtype, bs_last, s) : backward<half_t>(a, p, l.split, dtype, bs_last, s);
+    int st = dtype == KSMM_F32 ? backward<float>(a, p, l.split, bs_last, s) : backward<half_t>(a, p, l.split, bs_last, s);
     if (st != KSMM_OK) return st;
     if (gate_alone) {
         const unsigned blocks = (unsigned)((l.split.groups * features + 3) / 4);
