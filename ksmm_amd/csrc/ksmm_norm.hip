@@ -463,235 +463,408 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void ks_norm_rows_bwd_kernel
 }
 
 // ---- batch-size-last --------------------------------------------------------------------------------
-// A workgroup takes CT neighbouring rows of the batch (columns of the tensors) and all features: thread = one column
-// and every GROUPS-th feature.  FPT > 0: a thread's values of a tensor (at most FPT) stay in registers; FPT == 0, for
-// any number of features: they are read again for each of the passes that the statistics need.
-template <int CT, int GROUPS> struct ColSum {
-    float *red;  // 2 x GROUPS x CT floats
-    __device__ __forceinline__ void two(float &a, float &b)
-    {
-        const int col = threadIdx.x % CT, grp = threadIdx.x / CT;
-        __syncthreads();
-        red[grp * CT + col] = a;
-        red[(GROUPS + grp) * CT + col] = b;
-        __syncthreads();
-        a = b = 0.f;
-        for (int i = 0; i < GROUPS; ++i) {
-            a += red[i * CT + col];
-            b += red[(GROUPS + i) * CT + col];
-        }
-    }
-    __device__ __forceinline__ float one(float a)
-    {
-        float b = 0.f;
-        two(a, b);
-        return a;
-    }
+// A workgroup takes 4 * LANES neighbouring rows of the batch (columns of the tensors) and all features: thread = four
+// columns, one vector, and every GROUPS-th feature, FPT of them at a time, as they are stored, in registers.  ONE: that is all
+// of them, and they are read once; else they are read again in each pass that the statistics need.
+constexpr int COL_THREADS = 512, COL_WAVES = COL_THREADS / 64;
+struct Four {
+    float v[4];
 };
-// the sum over the CT lanes side by side that hold one feature
-template <int CT> __device__ __forceinline__ float sum_lanes(float v)
+template <typename T> struct Raw {
+    T v[4];
+};
+// each XCD gets a contiguous range of column tiles: neighbours share cache lines
+__device__ __forceinline__ int col_tile(int tiles) { return (blockIdx.x & 7) * ((tiles + 7) / 8) + (blockIdx.x >> 3); }
+template <typename T> __device__ __forceinline__ Four wide_of(const Raw<T> &r)
 {
-    v = sum16(v);
-    if constexpr (CT > 16) v += __shfl_xor(v, 16, 64);
-    if constexpr (CT > 32) v += __shfl_xor(v, 32, 64);
-    return v;
+    return Four{{(float)r.v[0], (float)r.v[1], (float)r.v[2], (float)r.v[3]}};
+}
+template <typename T> __device__ __forceinline__ void opaque(Raw<T> &r)
+{
+    typedef uint32_t words __attribute__((ext_vector_type(sizeof(T))));
+    words w = __builtin_bit_cast(words, r);
+    asm volatile("" : "+v"(w));
+    r = __builtin_bit_cast(Raw<T>, w);
+}
+// alpha * gate, post_weight, weight and bias of every feature, as far as they fit LDS: a feature's four are one read.
+// (gates of groups: alpha alone)
+constexpr int PARAMS = 2048;
+struct Params {
+    float gate, post, weight, bias;
+};
+template <typename T> __device__ __forceinline__ Params params_of(const NormArgs &a, bool one_gate, int h)
+{
+    Params p;
+    p.gate = a.gate && one_gate ? a.alpha * (float)((const T *)a.gate)[h] : a.alpha;
+    p.post = a.post_weight ? (float)((const T *)a.post_weight)[h] : 1.f;
+    p.weight = a.weight ? (float)((const T *)a.weight)[h] : 1.f;
+    p.bias = a.bias ? (float)((const T *)a.bias)[h] : 0.f;
+    return p;
+}
+// one row's four columns; past the last column: zeros, and nothing stored
+template <typename T> __device__ __forceinline__ Raw<T> load_four(const T *row, int count)
+{
+    Raw<T> r;
+    if (count >= 4) {
+        __builtin_memcpy(&r, row, sizeof(r));
+    } else {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) r.v[c] = c < count ? row[c] : (T)0.f;
+    }
+    return r;
+}
+template <typename T> __device__ __forceinline__ void store_four(T *row, int count, const Four &f)
+{
+    if (count >= 4) {
+        const Raw<T> r{{(T)f.v[0], (T)f.v[1], (T)f.v[2], (T)f.v[3]}};
+        __builtin_memcpy(row, &r, sizeof(r));
+    } else {
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+            if (c < count) row[c] = (T)f.v[c];
+    }
 }
 
-template <typename T, int CT, int THREADS, int FPT>
-__global__ __launch_bounds__(THREADS) void ks_norm_cols_kernel(NormArgs a)
-{
-    constexpr int GROUPS = THREADS / CT, N = FPT > 0 ? FPT : 1;
-    __shared__ float red[2 * THREADS];
-    ColSum<CT, GROUPS> sum{red};
-    const int H = a.features, grp = threadIdx.x / CT;
-    const int64_t B = a.batch, col = (int64_t)blockIdx.x * CT + threadIdx.x % CT;
-    const bool in = col < B;
-    const float inv = 1.f / (float)H;
-    const T *x = (const T *)a.x, *res = (const T *)a.residual, *post = (const T *)a.post_weight;
-    const T *gate = a.gate ? (const T *)a.gate + (in ? col / a.group_rows : 0) * H : nullptr;
-    float xv[N], rv[N];
-    // every feature of the thread in turn
-    auto each = [&](auto f) {
-        if constexpr (FPT > 0) {
+// every thread gets the sums of its columns over all features
+template <int LANES> struct ColSum {
+    float *red;  // 2 x COL_WAVES x 4 * LANES floats
+    __device__ __forceinline__ void add(Four &f, int q)
+    {
 #pragma unroll
-            for (int i = 0; i < FPT; ++i)
-                if (in && grp + i * GROUPS < H) f(i, grp + i * GROUPS);
-        } else if (in) {
-            for (int h = grp; h < H; h += GROUPS) f(0, h);
+        for (int c = 0; c < 4; ++c) {
+            if (LANES <= 4) f.v[c] += __shfl_xor(f.v[c], 4, 64);
+            if (LANES <= 8) f.v[c] = dpp_add<0x128>(f.v[c]);  // the other eight of sixteen
+            f.v[c] += __shfl_xor(f.v[c], 16, 64);
+            f.v[c] += __shfl_xor(f.v[c], 32, 64);
+        }
+        if ((threadIdx.x & 63) < LANES) *(Four *)(red + ((q * COL_WAVES + (threadIdx.x >> 6)) * LANES + threadIdx.x % LANES) * 4) = f;
+    }
+    __device__ __forceinline__ void get(Four &f, int q)
+    {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) f.v[c] = 0.f;
+#pragma unroll
+        for (int w = 0; w < COL_WAVES; ++w) {
+            const Four o = *(const Four *)(red + ((q * COL_WAVES + w) * LANES + threadIdx.x % LANES) * 4);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) f.v[c] += o.v[c];
+        }
+    }
+    __device__ __forceinline__ void two(Four &a, Four &b)
+    {
+        __syncthreads();
+        add(a, 0);
+        add(b, 1);
+        __syncthreads();
+        get(a, 0);
+        get(b, 1);
+    }
+    __device__ __forceinline__ void one(Four &a)
+    {
+        __syncthreads();
+        add(a, 0);
+        __syncthreads();
+        get(a, 0);
+    }
+};
+// the sum over the LANES lanes side by side that hold one feature
+template <int LANES> __device__ __forceinline__ float sum_lanes(const Four &f)
+{
+    float v = (f.v[0] + f.v[1]) + (f.v[2] + f.v[3]);
+    v = dpp_add<0xB1>(v);
+    v = dpp_add<0x4E>(v);
+    if (LANES > 4) v = dpp_add<0x141>(v);
+    return LANES > 8 ? dpp_add<0x140>(v) : v;
+}
+
+template <typename T, int LANES, int FPT, bool ONE>
+__global__ __launch_bounds__(COL_THREADS) void ks_norm_cols_kernel(NormArgs a, int tiles)
+{
+    const int tile = col_tile(tiles);
+    if (tile >= tiles) return;
+    constexpr int GROUPS = COL_THREADS / LANES;
+    __shared__ float red[2 * COL_WAVES * 4 * LANES];
+    __shared__ Params held[PARAMS];
+    ColSum<LANES> sum{red};
+    const int H = a.features, grp = threadIdx.x / LANES;
+    const int64_t B = a.batch, col = ((int64_t)tile * LANES + threadIdx.x % LANES) * 4;
+    const int count = (int)max((int64_t)0, min((int64_t)4, B - col));  // (none: the thread adds zeros)
+    const float inv = 1.f / (float)H;
+    const T *const x = (const T *)a.x, *const res = (const T *)a.residual;
+    const bool post = a.post_weight != nullptr, one_gate = a.group_rows == B, in_lds = H <= PARAMS;
+    if (in_lds) {
+        for (int h = threadIdx.x; h < H; h += COL_THREADS) held[h] = params_of<T>(a, one_gate, h);
+    }
+    auto params = [&](int h) { return in_lds ? held[h] : params_of<T>(a, one_gate, h); };
+    const bool own_gates = a.gate && !one_gate;  // each column that of its group
+    const T *gate[4];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) gate[c] = own_gates ? (const T *)a.gate + min(col + c, B - 1) / a.group_rows * H : nullptr;
+    auto factor = [&](const Params &p, int c, int h) { return own_gates ? a.alpha * (float)gate[c][h] : p.gate; };
+    Raw<T> xv[FPT] = {}, rv[FPT] = {};
+    auto load = [&](int first, bool with_r) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < FPT; ++i) {
+            const int h = first + i * GROUPS;
+            if (h < H) {
+                if (with_r) rv[i] = load_four(res + h * B + col, count);
+                if (x) xv[i] = load_four(x + h * B + col, count);
+            }
         }
     };
-    if constexpr (FPT > 0) {
-        each([&](int i, int h) {
-            rv[i] = (float)res[h * B + col];
-            if (x) xv[i] = (float)x[h * B + col];
-        });
-    }
-    auto get_x = [&](int i, int h) { return FPT > 0 ? xv[i] : (float)x[h * B + col]; };
-    float mean_x = 0.f, rho_x = 1.f, mean_r = 0.f, rho_r = 1.f;
+    // every feature of the thread in turn, f(i, h): its values are xv[i] and (WITH_R) rv[i]
+    auto each = [&](bool with_r, auto f) __attribute__((always_inline)) {
+        int first = grp;
+        asm volatile("" : "+v"(first));  // (addresses are made anew in each pass, not held)
+        for (; first < H; first += FPT * GROUPS) {
+            if (!ONE) load(first, with_r);
+#pragma unroll
+            for (int i = 0; i < FPT; ++i) {
+                opaque(xv[i]);  // (each pass starts from the values as they are stored: kept wide they would not fit)
+                opaque(rv[i]);
+                if (first + i * GROUPS < H) f(i, first + i * GROUPS);
+            }
+            if (ONE) break;
+        }
+    };
+    if (ONE) load(grp, true);
+    __syncthreads();
+    Four mean_x = {}, rho_x = {{1.f, 1.f, 1.f, 1.f}}, mean_r = {}, rho_r = {{1.f, 1.f, 1.f, 1.f}};
     if (x && post) {
         if (a.layer) {
-            float s = 0.f;
-            each([&](int i, int h) { s += get_x(i, h); });
-            mean_x = sum.one(s) * inv;
+            each(false, [&](int i, int) {
+#pragma unroll
+                for (int c = 0; c < 4; ++c) mean_x.v[c] += (float)xv[i].v[c];
+            });
+            sum.one(mean_x);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) mean_x.v[c] *= inv;
         }
-        float s = 0.f;
-        each([&](int i, int h) {
-            const float c = get_x(i, h) - mean_x;
-            s = fmaf(c, c, s);
+        Four s = {};
+        each(false, [&](int i, int) {
+#pragma unroll
+            for (int c = 0; c < 4; ++c) s.v[c] = fmaf((float)xv[i].v[c] - mean_x.v[c], (float)xv[i].v[c] - mean_x.v[c], s.v[c]);
         });
-        rho_x = rsqrtf(fmaf(sum.one(s), inv, a.eps));
+        sum.one(s);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) rho_x.v[c] = rsqrtf(fmaf(s.v[c], inv, a.eps));
     }
     auto get_r = [&](int i, int h) {  // r', from the inputs
-        float r = FPT > 0 ? rv[i] : (float)res[h * B + col];
+        Four r = wide_of(rv[i]);
         if (x) {
-            float p = get_x(i, h);
-            if (post) p = (p - mean_x) * rho_x * (float)post[h];
-            r = fmaf(gate ? a.alpha * (float)gate[h] : a.alpha, p, r);
+            const Params q = params(h);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                const float f = (float)xv[i].v[c], p = post ? (f - mean_x.v[c]) * rho_x.v[c] * q.post : f;
+                r.v[c] = fmaf(factor(q, c, h), p, r.v[c]);
+            }
         }
         return r;
     };
-    float s = 0.f;
-    each([&](int i, int h) {
-        const float r = get_r(i, h);
-        if constexpr (FPT > 0) rv[i] = r;
-        if (x && a.r_out) ((T *)a.r_out)[h * B + col] = (T)r;
-        s += a.layer ? r : r * r;
+    Four s = {};
+    each(true, [&](int i, int h) {
+        const Four r = get_r(i, h);
+        if (x && a.r_out) store_four((T *)a.r_out + h * B + col, count, r);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) s.v[c] += a.layer ? r.v[c] : r.v[c] * r.v[c];
     });
     if (a.n_out) {
-        auto again = [&](int i, int h) { return FPT > 0 ? rv[i] : get_r(i, h); };
-        s = sum.one(s) * inv;
+        sum.one(s);
         if (a.layer) {
-            mean_r = s;
-            s = 0.f;
-            each([&](int i, int h) {
-                const float c = again(i, h) - mean_r;
-                s = fmaf(c, c, s);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                mean_r.v[c] = s.v[c] * inv;
+                s.v[c] = 0.f;
+            }
+            each(true, [&](int i, int h) {
+                const Four r = get_r(i, h);
+#pragma unroll
+                for (int c = 0; c < 4; ++c) s.v[c] = fmaf(r.v[c] - mean_r.v[c], r.v[c] - mean_r.v[c], s.v[c]);
             });
-            s = sum.one(s) * inv;
+            sum.one(s);
         }
-        rho_r = rsqrtf(s + a.eps);
-        each([&](int i, int h) {
-            float v = (again(i, h) - mean_r) * rho_r;
-            if (a.weight) v *= (float)((const T *)a.weight)[h];
-            if (a.bias) v += (float)((const T *)a.bias)[h];
-            ((T *)a.n_out)[h * B + col] = (T)v;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) rho_r.v[c] = rsqrtf(fmaf(s.v[c], inv, a.eps));
+        each(true, [&](int i, int h) {
+            const Four r = get_r(i, h);
+            const Params p = params(h);
+            Four o;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) o.v[c] = fmaf((r.v[c] - mean_r.v[c]) * rho_r.v[c], p.weight, p.bias);
+            store_four((T *)a.n_out + h * B + col, count, o);
         });
     }
-    if (a.stats && in && grp == 0) {
-        a.stats[col] = mean_x;
-        a.stats[B + col] = rho_x;
-        a.stats[2 * B + col] = mean_r;
-        a.stats[3 * B + col] = rho_r;
+    if (a.stats && grp == 0) {
+        store_four(a.stats + col, count, mean_x);
+        store_four(a.stats + B + col, count, rho_x);
+        store_four(a.stats + 2 * B + col, count, mean_r);
+        store_four(a.stats + 3 * B + col, count, rho_r);
     }
 }
 
-template <typename T, int CT, int THREADS, int FPT>
-__global__ __launch_bounds__(THREADS) void ks_norm_cols_bwd_kernel(NormArgs a, NormGrads d)
+// Gradients; the sums over a workgroup's columns are its slice of the partial sums.  With one gate for all rows, S = sum D u
+// serves dgate and dpost_weight (see above); gates of groups have a kernel of their own.
+template <typename T, int LANES, int FPT, bool ONE>
+__global__ __launch_bounds__(COL_THREADS) void ks_norm_cols_bwd_kernel(NormArgs a, NormGrads d, int tiles)
 {
-    constexpr int GROUPS = THREADS / CT, N = FPT > 0 ? FPT : 1;
-    __shared__ float red[2 * THREADS];
-    ColSum<CT, GROUPS> sum{red};
-    const int H = a.features, grp = threadIdx.x / CT;
-    const int64_t B = a.batch, col = (int64_t)blockIdx.x * CT + threadIdx.x % CT, at = col < B ? col : B - 1;
-    const bool in = col < B;
+    const int tile = col_tile(tiles);
+    if (tile >= tiles) return;
+    constexpr int GROUPS = COL_THREADS / LANES;
+    __shared__ float red[2 * COL_WAVES * 4 * LANES];
+    __shared__ Params held[PARAMS];
+    ColSum<LANES> sum{red};
+    const int H = a.features, grp = threadIdx.x / LANES;
+    const int64_t B = a.batch, col = ((int64_t)tile * LANES + threadIdx.x % LANES) * 4;
+    const int count = (int)max((int64_t)0, min((int64_t)4, B - col));  // (past the end: zeros, which no sum minds)
     const float inv = 1.f / (float)H;
-    const T *x = (const T *)a.x, *res = (const T *)a.residual, *post = (const T *)a.post_weight;
-    const T *gate = a.gate ? (const T *)a.gate + at / a.group_rows * H : nullptr;
-    const T *dr_in = (const T *)d.dr_out, *dn = (const T *)d.dn_out;
-    const float mean_x = a.stats[at], rho_x = a.stats[B + at], mean_r = a.stats[2 * B + at], rho_r = a.stats[3 * B + at];
-    float uv[N], vv[N], nv[N], dv_[N];
-    // every feature of the thread in turn, columns past the end too (their values count as zero: lanes add up)
-    auto each = [&](auto f) {
-        if constexpr (FPT > 0) {
+    const T *const x = (const T *)a.x, *const res = (const T *)a.residual;
+    const bool post = a.post_weight != nullptr, one_gate = a.group_rows == B, in_lds = H <= PARAMS;
+    if (in_lds) {
+        for (int h = threadIdx.x; h < H; h += COL_THREADS) held[h] = params_of<T>(a, one_gate, h);
+    }
+    auto params = [&](int h) { return in_lds ? held[h] : params_of<T>(a, one_gate, h); };
+    const bool own_gates = a.gate && !one_gate, writes = threadIdx.x % LANES == 0;
+    const T *gate[4];
 #pragma unroll
-            for (int i = 0; i < FPT; ++i)
-                if (grp + i * GROUPS < H) f(i, grp + i * GROUPS);
-        } else {
-            for (int h = grp; h < H; h += GROUPS) f(0, h);
+    for (int c = 0; c < 4; ++c) gate[c] = own_gates ? (const T *)a.gate + min(col + c, B - 1) / a.group_rows * H : nullptr;
+    auto factor = [&](const Params &p, int c, int h) { return own_gates ? a.alpha * (float)gate[c][h] : p.gate; };
+    const T *const dr_in = (const T *)d.dr_out, *const dn = (const T *)d.dn_out;
+    Four mean_x = {}, rho_x = {}, mean_r = {}, rho_r = {};
+    if (count > 0) {
+        mean_x = wide_of(load_four(a.stats + col, count));
+        rho_x = wide_of(load_four(a.stats + B + col, count));
+        mean_r = wide_of(load_four(a.stats + 2 * B + col, count));
+        rho_r = wide_of(load_four(a.stats + 3 * B + col, count));
+    }
+    Raw<T> xv[FPT] = {}, rv[FPT] = {}, nv[FPT] = {}, dv[FPT] = {};
+    auto load = [&](int first, bool with_d) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < FPT; ++i) {
+            const int h = first + i * GROUPS;
+            if (h < H) {
+                if (x) xv[i] = load_four(x + h * B + col, count);
+                if (dn) {
+                    rv[i] = load_four(res + h * B + col, count);
+                    nv[i] = load_four(dn + h * B + col, count);
+                }
+                if (with_d && dr_in) dv[i] = load_four(dr_in + h * B + col, count);
+            }
         }
     };
-    auto load_u = [&](int h) { return !x ? 0.f : post ? ((float)x[h * B + at] - mean_x) * rho_x : (float)x[h * B + at]; };
-    auto load_v = [&](int h, float u) {
-        float r = (float)res[h * B + at];
-        if (x) r = fmaf(gate ? a.alpha * (float)gate[h] : a.alpha, post ? u * (float)post[h] : u, r);
-        return (r - mean_r) * rho_r;
-    };
-    if constexpr (FPT > 0) {
-        each([&](int i, int h) {
-            uv[i] = load_u(h);
-            if (dn) {
-                vv[i] = load_v(h, uv[i]);
-                nv[i] = in ? (float)dn[h * B + at] : 0.f;
+    auto each = [&](bool with_d, auto f) __attribute__((always_inline)) {
+        int first = grp;
+        asm volatile("" : "+v"(first));  // (addresses are made anew in each pass, not held)
+        for (; first < H; first += FPT * GROUPS) {
+            if (!ONE) load(first, with_d);
+#pragma unroll
+            for (int i = 0; i < FPT; ++i) {
+                opaque(xv[i]);  // (each pass starts from the values as they are stored: kept wide they would not fit)
+                opaque(rv[i]);
+                opaque(nv[i]);
+                opaque(dv[i]);
+                if (first + i * GROUPS < H) f(i, first + i * GROUPS);
             }
-            dv_[i] = dr_in ? (float)dr_in[h * B + at] : 0.f;
-        });
-    }
-    auto get_u = [&](int i, int h) { return FPT > 0 ? uv[i] : load_u(h); };
-    auto get_v = [&](int i, int h, float u) { return FPT > 0 ? vv[i] : load_v(h, u); };
-    auto get_n = [&](int i, int h) { return FPT > 0 ? nv[i] : in ? (float)dn[h * B + at] : 0.f; };
-    float m1 = 0.f, m2 = 0.f;
+            if (ONE) break;
+        }
+    };
+    if (ONE) load(grp, true);
+    __syncthreads();
+    auto get_u = [&](int i) {
+        Four u = {};
+        if (x) {
+#pragma unroll
+            for (int c = 0; c < 4; ++c) u.v[c] = post ? ((float)xv[i].v[c] - mean_x.v[c]) * rho_x.v[c] : (float)xv[i].v[c];
+        }
+        return u;
+    };
+    auto get_v = [&](int i, int h, const Params &p, const Four &u) {
+        Four r = wide_of(rv[i]);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) r.v[c] = ((x ? fmaf(factor(p, c, h), u.v[c] * p.post, r.v[c]) : r.v[c]) - mean_r.v[c]) * rho_r.v[c];
+        return r;
+    };
+    Four m1 = {}, m2 = {};
     if (dn) {
-        each([&](int i, int h) {
-            const float v = get_v(i, h, get_u(i, h)), n = get_n(i, h), dv = a.weight ? n * (float)((const T *)a.weight)[h] : n;
-            m1 += dv;
-            m2 = fmaf(dv, v, m2);
+        each(false, [&](int i, int h) {
+            const Params p = params(h);
+            const Four v = get_v(i, h, p, get_u(i)), n = wide_of(nv[i]);
+            Four nw;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                m1.v[c] = fmaf(n.v[c], p.weight, m1.v[c]);
+                m2.v[c] = fmaf(n.v[c] * p.weight, v.v[c], m2.v[c]);
+                nw.v[c] = n.v[c] * v.v[c];
+            }
             if (d.dweight) {
-                const float q = sum_lanes<CT>(n * v);
-                if (threadIdx.x % CT == 0) d.dweight[(int64_t)blockIdx.x * H + h] = q;
+                const float q = sum_lanes<LANES>(nw);
+                if (writes) d.dweight[(int64_t)tile * H + h] = q;
             }
             if (d.dbias) {
-                const float q = sum_lanes<CT>(n);
-                if (threadIdx.x % CT == 0) d.dbias[(int64_t)blockIdx.x * H + h] = q;
+                const float q = sum_lanes<LANES>(n);
+                if (writes) d.dbias[(int64_t)tile * H + h] = q;
             }
         });
-        sum.two(m1, m2);
-        m1 = a.layer ? m1 * inv : 0.f;
-        m2 *= inv;
+        if (a.layer)
+            sum.two(m1, m2);
+        else
+            sum.one(m2);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            m1.v[c] = a.layer ? m1.v[c] * inv : 0.f;
+            m2.v[c] *= inv;
+        }
     }
     // D of one feature
-    auto get_D = [&](int i, int h, float u) {
-        float D = FPT > 0 ? dv_[i] : dr_in ? (float)dr_in[h * B + at] : 0.f;
+    auto get_D = [&](int i, int h, const Params &p, const Four &u) {
+        Four D = dr_in ? wide_of(dv[i]) : Four{};
         if (dn) {
-            const float n = get_n(i, h), dv = a.weight ? n * (float)((const T *)a.weight)[h] : n;
-            D = fmaf(rho_r, project(a, dv, get_v(i, h, u), m1, m2, rho_r), D);
+            const Four v = get_v(i, h, p, u);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) D.v[c] = fmaf(rho_r.v[c], project(a, (float)nv[i].v[c] * p.weight, v.v[c], m1.v[c], m2.v[c], rho_r.v[c]), D.v[c]);
         }
-        return in ? D : 0.f;
+        return D;
     };
-    float k1 = 0.f, k2 = 0.f;
-    each([&](int i, int h) {
-        const float u = get_u(i, h), D = get_D(i, h, u);
-        if (d.dresidual && in) ((T *)d.dresidual)[h * B + col] = (T)D;
+    Four k1 = {}, k2 = {};
+    each(true, [&](int i, int h) {
+        const Params p = params(h);
+        const Four u = get_u(i), D = get_D(i, h, p, u);
+        if (d.dresidual) store_four((T *)d.dresidual + h * B + col, count, D);
         if (!x) return;
-        const float pw = post ? (float)post[h] : 1.f;
-        float q = (gate ? a.alpha * (float)gate[h] : a.alpha) * D;
-        if (d.dgate) {
-            const float s = sum_lanes<CT>(a.alpha * D * (post ? u * pw : u));
-            if (threadIdx.x % CT == 0) d.dgate[(int64_t)blockIdx.x * H + h] = s;
-        }
-        if (post) {
-            if (d.dpost_weight) {
-                const float s = sum_lanes<CT>(q * u);
-                if (threadIdx.x % CT == 0) d.dpost_weight[(int64_t)blockIdx.x * H + h] = s;
+        Four q, s;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            q.v[c] = factor(p, c, h) * D.v[c];
+            s.v[c] = (one_gate ? D.v[c] : q.v[c]) * u.v[c];
+            if (post) {
+                q.v[c] *= p.post;
+                k1.v[c] += q.v[c];
+                k2.v[c] = fmaf(q.v[c], u.v[c], k2.v[c]);
             }
-            q *= pw;
-            k1 += q;
-            k2 = fmaf(q, u, k2);
         }
-        if constexpr (FPT > 0) dv_[i] = q;
-        if (!post && d.dx && in) ((T *)d.dx)[h * B + col] = (T)q;
+        if (d.dgate || d.dpost_weight) {
+            const float S = sum_lanes<LANES>(s);
+            if (writes && d.dgate) d.dgate[(int64_t)tile * H + h] = a.alpha * p.post * S;
+            if (writes && d.dpost_weight) d.dpost_weight[(int64_t)tile * H + h] = one_gate ? p.gate * S : S;
+        }
+        if (!post && d.dx) store_four((T *)d.dx + h * B + col, count, q);
     });
     if (x && post && d.dx) {
-        sum.two(k1, k2);
-        k1 = a.layer ? k1 * inv : 0.f;
-        k2 *= inv;
-        each([&](int i, int h) {
-            const float u = get_u(i, h);
-            float q;
-            if constexpr (FPT > 0)
-                q = dv_[i];
-            else
-                q = (gate ? a.alpha * (float)gate[h] : a.alpha) * get_D(i, h, u) * (float)post[h];
-            if (in) ((T *)d.dx)[h * B + col] = (T)(rho_x * project(a, q, u, k1, k2, rho_x));
+        if (a.layer)
+            sum.two(k1, k2);
+        else
+            sum.one(k2);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            k1.v[c] = a.layer ? k1.v[c] * inv : 0.f;
+            k2.v[c] *= inv;
+        }
+        each(true, [&](int i, int h) {
+            const Params p = params(h);
+            const Four u = get_u(i);
+            Four q = get_D(i, h, p, u);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) q.v[c] = rho_x.v[c] * project(a, q.v[c] * factor(p, c, h) * p.post, u.v[c], k1.v[c], k2.v[c], rho_x.v[c]);
+            store_four((T *)d.dx + h * B + col, count, q);
         });
     }
 }
@@ -751,14 +924,22 @@ template <typename T, typename F> int with_rows(int64_t features, F f)
     return KSMM_ERR_TOO_LARGE;
 }
 
-constexpr int COLS = 32, COL_THREADS = 512;
-template <typename F> int with_cols(int64_t features, F f)
+// Lanes side by side (four columns each) of a workgroup: 8, or 4 where that would leave CUs without work
+int col_lanes(int64_t batch) { return batch >= 32 * 192 ? 8 : 4; }
+template <typename T, typename F> int with_cols(int64_t batch, int64_t features, F f)
 {
-    const int64_t per = (features + COL_THREADS / COLS - 1) / (COL_THREADS / COLS);
-    if (per <= 8) return f(std::integral_constant<int, 8>());
-    if (per <= 24) return f(std::integral_constant<int, 24>());
-    if (per <= 48) return f(std::integral_constant<int, 48>());
-    return f(std::integral_constant<int, 0>());
+    // features a thread holds: 12 in 16 bits and 6 in 32 are what the backward pass has registers for (with 24 and 12 it
+    // spills, and takes twice the time)
+    constexpr int MOST = sizeof(T) == 2 ? 12 : 6;
+    const int lanes = col_lanes(batch);
+    const int64_t groups = COL_THREADS / lanes, per = (features + groups - 1) / groups;
+    auto held = [&](auto lanes_of) {
+        typedef std::integral_constant<bool, true> one;
+        if (per <= MOST / 2) return f(lanes_of, std::integral_constant<int, MOST / 2>(), one());
+        if (per <= MOST) return f(lanes_of, std::integral_constant<int, MOST>(), one());
+        return f(lanes_of, std::integral_constant<int, MOST / 2>(), std::integral_constant<bool, false>());
+    };
+    return lanes == 8 ? held(std::integral_constant<int, 8>()) : held(std::integral_constant<int, 4>());
 }
 
 NormSplit split_rows(int64_t batch, int64_t groups)
@@ -780,9 +961,11 @@ int launched() { return hipGetLastError() == hipSuccess ? KSMM_OK : KSMM_ERR_LAU
 template <typename T> int forward(const NormArgs &a, int bs_last, hipStream_t stream)
 {
     if (bs_last)
-        return with_cols(a.features, [&](auto fpt) {
-            hipLaunchKernelGGL((ks_norm_cols_kernel<T, COLS, COL_THREADS, decltype(fpt)::value>), dim3((unsigned)((a.batch + COLS - 1) / COLS)),
-                               dim3(COL_THREADS), 0, stream, a);
+        return with_cols<T>(a.batch, a.features, [&](auto lanes, auto fpt, auto one) {
+            constexpr int LANES = decltype(lanes)::value;
+            const int tiles = (int)((a.batch + 4 * LANES - 1) / (4 * LANES));
+            hipLaunchKernelGGL((ks_norm_cols_kernel<T, LANES, decltype(fpt)::value, decltype(one)::value>), dim3((tiles + 7) / 8 * 8),
+                               dim3(COL_THREADS), 0, stream, a, tiles);
             return launched();
         });
     return with_rows<T>(a.features, [&](auto how) {
@@ -799,9 +982,11 @@ template <typename T> int forward(const NormArgs &a, int bs_last, hipStream_t st
 template <typename T> int backward(const NormArgs &a, const NormGrads &partial, const NormSplit &sp, int bs_last, hipStream_t stream)
 {
     if (bs_last)
-        return with_cols(a.features, [&](auto fpt) {
-            hipLaunchKernelGGL((ks_norm_cols_bwd_kernel<T, COLS, COL_THREADS, decltype(fpt)::value>), dim3((unsigned)((a.batch + COLS - 1) / COLS)),
-                               dim3(COL_THREADS), 0, stream, a, partial);
+        return with_cols<T>(a.batch, a.features, [&](auto lanes, auto fpt, auto one) {
+            constexpr int LANES = decltype(lanes)::value;
+            const int tiles = (int)((a.batch + 4 * LANES - 1) / (4 * LANES));
+            hipLaunchKernelGGL((ks_norm_cols_bwd_kernel<T, LANES, decltype(fpt)::value, decltype(one)::value>), dim3((tiles + 7) / 8 * 8),
+                               dim3(COL_THREADS), 0, stream, a, partial, tiles);
             return launched();
         });
     return with_rows<T>(a.features, [&](auto how) {
@@ -832,7 +1017,8 @@ Layout layout(int64_t batch, int64_t features, int64_t groups, int bs_last)
 {
     Layout l;
     l.split = split_rows(batch, groups);
-    l.slices = bs_last ? (batch + COLS - 1) / COLS : l.split.ranges;
+    const int cols = 4 * col_lanes(batch);
+    l.slices = bs_last ? (batch + cols - 1) / cols : l.split.ranges;
     l.slice_bytes = align256(4 * l.slices * features);
     l.gate_bytes = l.split.one_gate ? l.slice_bytes : bs_last ? 0 : align256(4 * l.split.parts * l.split.groups * features);
     l.total = 3 * l.slice_bytes + l.gate_bytes;
