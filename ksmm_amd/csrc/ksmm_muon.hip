@@ -202,153 +202,220 @@ __global__ __launch_bounds__(64 * WAVES) void ks_muon_block_kernel(MuonArgs a)
 }
 
 // ---- larger blocks: a launch a product --------------------------------------------------------------------
-// In the workspace each matrix lies as M x N, both multiples of 64 (zeros past its own sides).
-constexpr int TILE = 64, CHUNKS = 16;
+// fp32 values as two fp16 ones, x = hi + lo / 2048: 22 bits.  A product of two such is three matrix instructions
+// (hi hi, and hi lo + lo hi in sums of their own; what lo lo would add is below the last bit), 96 clocks for 32 x 32 x 16
+// where the 32-bit instructions take 512.  |X| <= 1 here, so that no part leaves fp16's range.
+// In the workspace each matrix lies as X (M x N) and as its transpose, M and N multiples of 64 (zeros past its own
+// sides): with G and Q symmetric, every product is one of rows with rows, and its operands come straight from memory.  They
+// lie there as the instructions take them: 32 rows x 16 k are 1 KB in a row, 16 bytes a lane (operands gathered from plain
+// rows took 58 us a product of (1,1536,384,2) pairs, bound by addresses).
+constexpr int TILE = 64, STEP = 16;
+constexpr float SPLIT = 2048.f;
 __host__ __device__ constexpr int up64(int v) { return (v + 63) / 64 * 64; }
 
-// u into the workspace, and the sums of its squares, CHUNKS a matrix
+// where element (r, k) of a matrix of K columns lies: lane r % 32 + 32 * (k % 16 / 8) of piece (r / 32, k / 16)
+__device__ __forceinline__ int64_t operand_at(int r, int k, int K)
+{
+    return ((int64_t)(r >> 5) * (K >> 4) + (k >> 4)) * 512 + (((k >> 3) & 1) * 32 + (r & 31)) * 8 + (k & 7);
+}
+struct Split {
+    half_t *hi, *lo;
+    // four values, k to k + 3 (4 divides k)
+    __device__ __forceinline__ void put(int64_t at, const f4 &v) const
+    {
+        half4_t h, l;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            h[i] = (half_t)v[i];
+            l[i] = (half_t)((v[i] - (float)h[i]) * SPLIT);
+        }
+        *(half4_t *)(hi + at) = h;
+        *(half4_t *)(lo + at) = l;
+    }
+    __device__ __forceinline__ f4 get(int64_t at) const
+    {
+        const half4_t h = *(const half4_t *)(hi + at), l = *(const half4_t *)(lo + at);
+        f4 v;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = fmaf((float)l[i], 1.f / SPLIT, (float)h[i]);
+        return v;
+    }
+};
+
+// u (fp32, as it is stored in memory, blocks next to each other) and the sums of its squares, `chunks` a matrix
 template <typename T>
-__global__ __launch_bounds__(256) void ks_muon_load_kernel(MuonArgs a, float *__restrict__ x, float *__restrict__ squares, int M, int N)
+__global__ __launch_bounds__(256) void ks_muon_load_kernel(MuonArgs a, float *__restrict__ u, float *__restrict__ squares, int chunks)
 {
     __shared__ float red[4];
-    const int64_t id = blockIdx.x / CHUNKS, chunk = blockIdx.x % CHUNKS;
-    const bool flip = a.c > a.b;
+    const int64_t id = blockIdx.x / chunks, chunk = blockIdx.x - id * chunks;
     const int64_t base = matrix_base(a, id), pitch = (int64_t)a.parts * a.b;
-    // in the order of memory: rows and columns as they are stored, padded alike
-    const int R = flip ? N : M, K = flip ? M : N;
-    const int64_t total = (int64_t)R * K, per = (total + CHUNKS - 1) / CHUNKS, end = min(total, (chunk + 1) * per);
-    x += id * M * N;
+    const int total = a.c * a.b, per = (total + chunks - 1) / chunks, end = min((int64_t)total, (chunk + 1) * per);
+    u += id * total;
     float ss = 0.f;
-    for (int64_t i = chunk * per + threadIdx.x; i < end; i += 256) {
-        const int r = (int)(i / K), k = (int)(i - (int64_t)r * K);
-        const float u = r < a.c && k < a.b ? update_of<T>(a, base + r * pitch + k) : 0.f;
-        x[flip ? (int64_t)k * N + r : (int64_t)r * N + k] = u;
-        ss = fmaf(u, u, ss);
+    for (int i = chunk * per + threadIdx.x; i < end; i += 256) {
+        const int r = i / a.b, k = i - r * a.b;
+        const float v = update_of<T>(a, base + r * pitch + k);
+        u[i] = v;
+        ss = fmaf(v, v, ss);
     }
     ss = wave_sum(ss);
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = ss;
     __syncthreads();
-    if (threadIdx.x == 0) squares[id * CHUNKS + chunk] = (red[0] + red[1]) + (red[2] + red[3]);
+    if (threadIdx.x == 0) squares[id * chunks + chunk] = (red[0] + red[1]) + (red[2] + red[3]);
+}
+
+// X0 and its transpose from u, 64 x 64 at a time (as they lie in memory: c x b)
+__global__ __launch_bounds__(256) void ks_muon_split_kernel(MuonArgs a, const float *__restrict__ u, const float *__restrict__ squares, int chunks,
+                                                            Split straight, Split turned, int R, int K)
+{
+    __shared__ float tile[64][65];
+    __shared__ float norm;
+    const int tk = K / 64, per = R / 64 * tk;
+    const int64_t id = blockIdx.x / per;
+    const int t = (int)(blockIdx.x - id * per), r0 = t / tk * 64, k0 = t % tk * 64;
+    if (threadIdx.x < 64) {
+        float ss = 0.f;
+        for (int i = threadIdx.x; i < chunks; i += 64) ss += squares[id * chunks + i];
+        ss = wave_sum(ss);
+        if (threadIdx.x == 0) norm = 1.f / (sqrtf(ss) + a.eps);
+    }
+    __syncthreads();
+    const float scale = norm;
+    const int l = threadIdx.x & 63, w = threadIdx.x >> 6;
+    u += id * a.c * a.b;
+    const int64_t base = id * R * K;
+#pragma unroll 4
+    for (int i = w; i < 64; i += 4) {
+        const int r = r0 + i, k = k0 + l;
+        tile[i][l] = r < a.c && k < a.b ? u[(int64_t)r * a.b + k] * scale : 0.f;
+    }
+    __syncthreads();
+    // lane: a row, four k at a time
+#pragma unroll
+    for (int k = 4 * w; k < 64; k += 16) {
+        straight.put(base + operand_at(r0 + l, k0 + k, K), f4{tile[l][k], tile[l][k + 1], tile[l][k + 2], tile[l][k + 3]});
+        turned.put(base + operand_at(k0 + l, r0 + k, R), f4{tile[k][l], tile[k + 1][l], tile[k + 2][l], tile[k + 3][l]});
+    }
 }
 
 enum { GRAM, POLY, APPLY };
-// C (rows x cols) of 64 x 64 tiles, K in slabs of 16.
-//   GRAM   G = s^2 X X^T      POLY   Q = p1 G + p2 G G      APPLY  X' = s (p0 X + Q X), the last one: the results
-// s = 1 / (|u| + eps) in the first step, whose X is u itself; later 1.  GRAM and POLY are symmetric: upper tiles only.
-template <typename T, int WHAT>
-__global__ __launch_bounds__(256) void ks_muon_gemm_kernel(MuonArgs a, const float *__restrict__ left, const float *__restrict__ right,
-                                                           float *__restrict__ out, const float *__restrict__ squares, int M, int N, int last)
+// C = L R^T (rows of L, rows of R), a 64 x 64 tile a workgroup; four groups of four waves share K and add up in LDS.
+//   GRAM   G = X X^T      POLY   Q = p1 G + p2 G G      APPLY  X'^T = p0 X^T + X^T Q, or the results
+// Stored are the transposes of the tiles (what a lane holds lies in a row there; G and Q are symmetric), by APPLY both.
+// (GRAM and POLY compute both triangles: with few matrices there are more CUs than tiles.)
+template <typename T, int WHAT, int GROUPS>
+__global__ __launch_bounds__(256 * GROUPS) void ks_muon_gemm_kernel(MuonArgs a, Split left, Split right, Split x, Split out, Split turned, int M, int N,
+                                                                    int last, int tiles)
 {
-    constexpr int TK = 32, LDI = TK + 4, LDO = TILE + 8;
-    __shared__ __attribute__((aligned(16))) float sl[2][TILE * LDI];
-    __shared__ __attribute__((aligned(16))) float sr[2][WHAT == APPLY ? TK * LDO : TILE * LDI];
-    const int mt = M / TILE, per = WHAT == APPLY ? mt * (N / TILE) : mt * (mt + 1) / 2;
-    const int64_t id = blockIdx.x / per;
-    int t = (int)(blockIdx.x - id * per), ti, tj;
-    if (WHAT == APPLY) {
-        ti = t % mt;
-        tj = t / mt;
-    } else {
-        ti = 0;
-        for (int rest = mt; t >= rest; --rest, ++ti) t -= rest;
-        tj = ti + t;
+    constexpr int SUMS = GROUPS > 1 ? GROUPS * 4 * 16 * 64 : 4 * 32 * 33;
+    __shared__ float sums[SUMS];
+    // a range of tiles an XCD: a matrix's operands are read through few of the L2s
+    const int per_xcd = (tiles + 7) / 8, lid = (blockIdx.x & 7) * per_xcd + (blockIdx.x >> 3);
+    if ((int)(blockIdx.x >> 3) >= per_xcd || lid >= tiles) return;
+    const int mt = M / TILE, per = WHAT == APPLY ? mt * (N / TILE) : mt * mt;
+    const int64_t id = lid / per;
+    const int t = (int)(lid - id * per), tj = t % mt, ti = t / mt;  // (tiles that share rows of L are neighbours)
+    const int K = WHAT == GRAM ? N : M, rows_l = WHAT == APPLY ? N : M;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), group = wave >> 2, quarter = wave & 3;
+    const int i0 = ti * TILE + (quarter >> 1) * 32, j0 = tj * TILE + (quarter & 1) * 32, l32 = lane & 31, lq = lane >> 5;
+    const int64_t at_l = id * rows_l * K + operand_at(i0, 0, K) + lane * 8, at_r = id * M * K + operand_at(j0, 0, K) + lane * 8;
+    const half_t *const lh = left.hi + at_l, *const ll = left.lo + at_l, *const rh = right.hi + at_r, *const rl = right.lo + at_r;
+    float16_t main, cross;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) main[e] = cross[e] = 0.f;
+    const int steps = K / (STEP * GROUPS);  // K is a multiple of 64: each group has the same number
+    struct Operands {
+        half8_t xh, xl, yh, yl;
+    };
+    auto load = [&](Operands &o, int s) {
+        const int64_t at = (int64_t)(min(s, steps - 1) * GROUPS + group) * 512;
+        o.xh = *(const half8_t *)(lh + at);
+        o.xl = *(const half8_t *)(ll + at);
+        o.yh = *(const half8_t *)(rh + at);
+        o.yl = *(const half8_t *)(rl + at);
+    };
+    Operands ring[4];
+#pragma unroll
+    for (int s = 0; s < 3; ++s) load(ring[s], s);
+    for (int s = 0; s < steps; s += 4) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            if (s + q >= steps) break;
+            load(ring[(q + 3) & 3], s + q + 3);
+            const Operands &o = ring[q];
+            main = __builtin_amdgcn_mfma_f32_32x32x16_f16(o.xh, o.yh, main, 0, 0, 0);
+            cross = __builtin_amdgcn_mfma_f32_32x32x16_f16(o.xh, o.yl, cross, 0, 0, 0);
+            cross = __builtin_amdgcn_mfma_f32_32x32x16_f16(o.xl, o.yh, cross, 0, 0, 0);
+        }
     }
-    const int K = WHAT == GRAM ? N : M, ldl = WHAT == GRAM ? N : M, ldr = WHAT == POLY ? M : N, i0 = ti * TILE, j0 = tj * TILE;
-    const float *const L = left + id * M * ldl, *const R = right + id * M * ldr;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l16 = lane & 15, q = lane >> 4;
-    const int wi = (wave >> 1) * 32, wj = (wave & 1) * 32;
-
-    f4 lr[2], rr[2];
-    auto gload = [&](int k0) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int v = tid + i * 256, row = v / (TK / 4), k = v % (TK / 4) * 4;
-            lr[i] = *(const f4 *)(L + (int64_t)(i0 + row) * ldl + k0 + k);
-            if (WHAT == APPLY) {
-                const int kk = v / (TILE / 4), col = v % (TILE / 4) * 4;
-                rr[i] = *(const f4 *)(R + (int64_t)(k0 + kk) * ldr + j0 + col);
-            } else {
-                rr[i] = *(const f4 *)(R + (int64_t)(j0 + row) * ldr + k0 + k);
-            }
-        }
-    };
-    auto lstore = [&](int buf) {
+    for (int e = 0; e < 16; ++e) main[e] = fmaf(cross[e], 1.f / SPLIT, main[e]);
+    // element e of a lane's tile: row 8 * (e / 4) + 4 * lq + e % 4, column l32.  A group finishes 16 / GROUPS of them
+    constexpr int MINE = 4 / GROUPS;  // fours of rows
+    f4 v[MINE];
+    if constexpr (GROUPS > 1) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int v = tid + i * 256, row = v / (TK / 4), k = v % (TK / 4) * 4;
-            *(f4 *)(sl[buf] + row * LDI + k) = lr[i];
-            if (WHAT == APPLY)
-                *(f4 *)(sr[buf] + v / (TILE / 4) * LDO + v % (TILE / 4) * 4) = rr[i];
-            else
-                *(f4 *)(sr[buf] + row * LDI + k) = rr[i];
-        }
-    };
-    f4 acc[2][2];
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) acc[i][j] = f4{0.f, 0.f, 0.f, 0.f};
-    gload(0);
-    lstore(0);
-    __syncthreads();
-    for (int k0 = 0, buf = 0; k0 < K; k0 += TK, buf ^= 1) {
-        if (k0 + TK < K) gload(k0 + TK);
-#pragma unroll
-        for (int k = 0; k < TK; k += 16) {
-            f4 x[2], y[2];
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                x[i] = *(const f4 *)(sl[buf] + (wi + 16 * i + l16) * LDI + k + 4 * q);
-                if (WHAT == APPLY) {
-                    const float *p = sr[buf] + (k + 4 * q) * LDO + wj + 16 * i + l16;
-                    y[i] = f4{p[0], p[LDO], p[2 * LDO], p[3 * LDO]};
-                } else {
-                    y[i] = *(const f4 *)(sr[buf] + (wj + 16 * i + l16) * LDI + k + 4 * q);
-                }
-            }
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-#pragma unroll
-                for (int i = 0; i < 2; ++i)
-#pragma unroll
-                    for (int j = 0; j < 2; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[i][e], y[j][e], acc[i][j], 0, 0, 0);
-        }
-        if (k0 + TK < K) lstore(buf ^ 1);
+        for (int e = 0; e < 16; ++e) sums[((group * 4 + quarter) * 16 + e) * 64 + lane] = main[e];
         __syncthreads();
+#pragma unroll
+        for (int k = 0; k < MINE; ++k) {
+            v[k] = f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int q = 0; q < GROUPS; ++q)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[k][e] += sums[((q * 4 + quarter) * 16 + 4 * (group * MINE + k) + e) * 64 + lane];
+        }
+        if (WHAT == APPLY) __syncthreads();
+    } else {
+#pragma unroll
+        for (int k = 0; k < MINE; ++k) v[k] = f4{main[4 * k], main[4 * k + 1], main[4 * k + 2], main[4 * k + 3]};
     }
-    float s = 1.f;
-    if (WHAT != POLY && squares) {
-        float ss = 0.f;
-        for (int i = 0; i < CHUNKS; ++i) ss += squares[id * CHUNKS + i];
-        s = 1.f / (sqrtf(ss) + a.eps);
+    float *const turn = sums + quarter * 32 * 33;  // [j][i]
+    f4 old[MINE];
+    if (WHAT != GRAM) {
+#pragma unroll
+        for (int k = 0; k < MINE; ++k) {
+            const int r = 8 * (group * MINE + k) + 4 * lq;
+            old[k] = x.get(WHAT == POLY ? id * M * M + operand_at(j0 + l32, i0 + r, M) : id * M * N + operand_at(j0 + l32, i0 + r, N));
+        }
     }
+#pragma unroll
+    for (int k = 0; k < MINE; ++k) {
+        const int r = 8 * (group * MINE + k) + 4 * lq;
+        if (WHAT == GRAM) {
+            out.put(id * M * M + operand_at(j0 + l32, i0 + r, M), v[k]);
+        } else if (WHAT == POLY) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[k][e] = fmaf(a.p2, v[k][e], a.p1 * old[k][e]);
+            out.put(id * M * M + operand_at(j0 + l32, i0 + r, M), v[k]);
+        } else {
+            // rows of X^T are i, of X are j: X[j0 + l32][i0 + r ..]
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                v[k][e] = fmaf(a.p0, old[k][e], v[k][e]);
+                turn[l32 * 33 + r + e] = v[k][e];
+            }
+            if (!last) out.put(id * M * N + operand_at(j0 + l32, i0 + r, N), v[k]);
+        }
+    }
+    if (WHAT != APPLY) return;
+    __syncthreads();
     const int64_t base = matrix_base(a, id), pitch = (int64_t)a.parts * a.b;
     const bool flip = a.c > a.b;
     const int m = flip ? a.b : a.c, n = flip ? a.c : a.b;
-    out += id * M * (WHAT == APPLY ? N : M);
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int k = 0; k < MINE; ++k) {
+        const int r = 8 * (group * MINE + k) + 4 * lq;
+        if (!last) {
+            turned.put(id * M * N + operand_at(i0 + l32, j0 + r, M), f4{turn[r * 33 + l32], turn[(r + 1) * 33 + l32], turn[(r + 2) * 33 + l32], turn[(r + 3) * 33 + l32]});
+        } else {
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int r = i0 + wi + 16 * i + 4 * q + e, c = j0 + wj + 16 * j + l16;
-                if (WHAT == GRAM) {
-                    const float v = acc[i][j][e] * s * s;
-                    out[(int64_t)r * M + c] = v;
-                    if (ti != tj) out[(int64_t)c * M + r] = v;
-                } else if (WHAT == POLY) {
-                    const float v = fmaf(a.p2, acc[i][j][e], a.p1 * L[(int64_t)r * M + c]);
-                    out[(int64_t)r * M + c] = v;
-                    if (ti != tj) out[(int64_t)c * M + r] = v;
-                } else {
-                    const float v = fmaf(a.p0, R[(int64_t)r * N + c], acc[i][j][e]) * s;
-                    if (!last)
-                        out[(int64_t)r * N + c] = v;
-                    else if (r < m && c < n)
-                        finish<T>(a, base + (flip ? (int64_t)c * pitch + r : (int64_t)r * pitch + c), v);
-                }
+            for (int e = 0; e < 4; ++e) {  // along the rows of memory
+                const int i = i0 + (flip ? r + e : l32), j = j0 + (flip ? l32 : r + e);
+                if (j < m && i < n) finish<T>(a, base + (flip ? (int64_t)i * pitch + j : (int64_t)j * pitch + i), turn[(j - j0) * 33 + i - i0]);
             }
+        }
+    }
 }
 
 // ---- choices ----------------------------------------------------------------------------------------------
@@ -374,8 +441,8 @@ template <typename T, int WAVES> int run_block(const MuonArgs &a, int64_t matric
 
 int64_t align256(int64_t v) { return (v + 255) / 256 * 256; }
 struct Space {
-    int M, N;
-    int64_t x[2], gram, poly, squares, total;
+    int M, N, chunks;
+    int64_t x[4], gram, poly, squares, u, total;  // x: two of X, two of its transpose; bytes
 };
 Space space(int64_t matrices, int c, int b)
 {
@@ -383,17 +450,18 @@ Space space(int64_t matrices, int c, int b)
     const int m = std::min(c, b), n = std::max(c, b);
     w.M = up64(m);
     w.N = up64(n);
+    w.chunks = (int)std::max<int64_t>(1, std::min<int64_t>(256, 1024 / matrices));
     int64_t at = 0;
-    auto take = [&](int64_t floats) {
+    auto take = [&](int64_t bytes) {
         const int64_t was = at;
-        at += align256(4 * floats);
+        at += align256(bytes);
         return was;
     };
-    w.x[0] = take(matrices * w.M * w.N);
-    w.x[1] = take(matrices * w.M * w.N);
-    w.gram = take(matrices * w.M * w.M);
-    w.poly = take(matrices * w.M * w.M);
-    w.squares = take(matrices * CHUNKS);
+    for (int64_t &x : w.x) x = take(4 * matrices * w.M * w.N);
+    w.gram = take(4 * matrices * w.M * w.M);
+    w.poly = take(4 * matrices * w.M * w.M);
+    w.squares = take(4 * matrices * w.chunks);
+    w.u = w.x[1];  // (the second X is written after u was read)
     w.total = at;
     return w;
 }
@@ -406,17 +474,26 @@ template <typename T> int run(const MuonArgs &a, int64_t matrices, char *ws, hip
         return tiles <= 1 ? run_block<T, 1>(a, matrices, lds, s) : tiles <= 4 ? run_block<T, 4>(a, matrices, lds, s) : run_block<T, 16>(a, matrices, lds, s);
     }
     const Space w = space(matrices, a.c, a.b);
-    const int64_t mt = w.M / TILE, half = matrices * mt * (mt + 1) / 2, full = matrices * mt * (w.N / TILE);
-    if (full > 0x7fffffffLL || matrices * CHUNKS > 0x7fffffffLL) return KSMM_ERR_TOO_LARGE;
-    float *x = (float *)(ws + w.x[0]), *y = (float *)(ws + w.x[1]), *gram = (float *)(ws + w.gram), *poly = (float *)(ws + w.poly);
-    float *const squares = (float *)(ws + w.squares);
-    hipLaunchKernelGGL((ks_muon_load_kernel<T>), dim3((unsigned)(matrices * CHUNKS)), dim3(256), 0, s, a, x, squares, w.M, w.N);
+    const int64_t mt = w.M / TILE, square = matrices * mt * mt, full = matrices * mt * (w.N / TILE);
+    if (full > 0x7fffffffLL || matrices * w.chunks > 0x7fffffffLL) return KSMM_ERR_TOO_LARGE;
+    const bool flip = a.c > a.b;
+    auto split = [&](int64_t at, int64_t values) { return Split{(half_t *)(ws + at), (half_t *)(ws + at) + values}; };
+    const int64_t values = matrices * w.M * w.N;
+    Split x = split(w.x[0], values), y = split(w.x[1], values), xt = split(w.x[2], values), yt = split(w.x[3], values);
+    const Split gram = split(w.gram, matrices * w.M * w.M), poly = split(w.poly, matrices * w.M * w.M);
+    float *const u = (float *)(ws + w.u), *const squares = (float *)(ws + w.squares);
+    hipLaunchKernelGGL((ks_muon_load_kernel<T>), dim3((unsigned)(matrices * w.chunks)), dim3(256), 0, s, a, u, squares, w.chunks);
+    hipLaunchKernelGGL(ks_muon_split_kernel, dim3((unsigned)full), dim3(256), 0, s, a, u, squares, w.chunks, flip ? xt : x, flip ? x : xt,
+                       flip ? w.N : w.M, flip ? w.M : w.N);
+    auto gemm = [&](auto fn, int groups, int64_t tiles, Split l, Split r, Split old, Split out, Split turned, bool last) {
+        hipLaunchKernelGGL(fn, dim3((unsigned)((tiles + 7) / 8 * 8)), dim3(256 * groups), 0, s, a, l, r, old, out, turned, w.M, w.N, last, (int)tiles);
+    };
     for (int i = 0; i < a.steps; ++i) {
-        const float *const sq = i == 0 ? squares : nullptr;
-        hipLaunchKernelGGL((ks_muon_gemm_kernel<T, GRAM>), dim3((unsigned)half), dim3(256), 0, s, a, x, x, gram, sq, w.M, w.N, 0);
-        hipLaunchKernelGGL((ks_muon_gemm_kernel<T, POLY>), dim3((unsigned)half), dim3(256), 0, s, a, gram, gram, poly, sq, w.M, w.N, 0);
-        hipLaunchKernelGGL((ks_muon_gemm_kernel<T, APPLY>), dim3((unsigned)full), dim3(256), 0, s, a, poly, x, y, sq, w.M, w.N, i + 1 == a.steps);
+        gemm(&ks_muon_gemm_kernel<T, GRAM, 4>, 4, square, x, x, x, gram, gram, false);
+        gemm(&ks_muon_gemm_kernel<T, POLY, 4>, 4, square, gram, gram, gram, poly, poly, false);
+        gemm(&ks_muon_gemm_kernel<T, APPLY, 1>, 1, full, xt, poly, x, y, yt, i + 1 == a.steps);
         std::swap(x, y);
+        std::swap(xt, yt);
     }
     return launched();
 }
