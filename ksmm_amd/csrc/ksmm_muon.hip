@@ -303,12 +303,13 @@ enum { GRAM, POLY, APPLY };
 //   GRAM   G = X X^T      POLY   Q = p1 G + p2 G G      APPLY  X'^T = p0 X^T + X^T Q, or the results
 // Stored are the transposes of the tiles (what a lane holds lies in a row there; G and Q are symmetric), by APPLY both.
 // (GRAM and POLY compute both triangles: with few matrices there are more CUs than tiles.)
+// A wave multiplies whole tiles of 64 x 64 (four of 32 x 32: an operand from the L1, whose 64 bytes a clock are what bounds
+// this, serves two of them); the GROUPS waves of a workgroup share K and add up in LDS.
 template <typename T, int WHAT, int GROUPS>
-__global__ __launch_bounds__(256 * GROUPS) void ks_muon_gemm_kernel(MuonArgs a, Split left, Split right, Split x, Split out, Split turned, int M, int N,
-                                                                    int last, int tiles)
+__global__ __launch_bounds__(64 * GROUPS, 2) void ks_muon_gemm_kernel(MuonArgs a, Split left, Split right, Split x, Split out, Split turned, int M, int N,
+                                                                   int last, int tiles)
 {
-    constexpr int SUMS = GROUPS > 1 ? GROUPS * 4 * 16 * 64 : 4 * 32 * 33;
-    __shared__ float sums[SUMS];
+    extern __shared__ __attribute__((aligned(16))) float sums[];  // GROUPS x 64 x 64, then 4 x 32 x 33
     // a range of tiles an XCD: a matrix's operands are read through few of the L2s
     const int per_xcd = (tiles + 7) / 8, lid = (blockIdx.x & 7) * per_xcd + (blockIdx.x >> 3);
     if ((int)(blockIdx.x >> 3) >= per_xcd || lid >= tiles) return;
@@ -316,61 +317,15 @@ __global__ __launch_bounds__(256 * GROUPS) void ks_muon_gemm_kernel(MuonArgs a, 
     const int64_t id = lid / per;
     const int t = (int)(lid - id * per), tj = t % mt, ti = t / mt;  // (tiles that share rows of L are neighbours)
     const int K = WHAT == GRAM ? N : M, rows_l = WHAT == APPLY ? N : M;
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), group = wave >> 2, quarter = wave & 3;
-    const int i0 = ti * TILE + (quarter >> 1) * 32, j0 = tj * TILE + (quarter & 1) * 32, l32 = lane & 31, lq = lane >> 5;
-    const int64_t at_l = id * rows_l * K + operand_at(i0, 0, K) + lane * 8, at_r = id * M * K + operand_at(j0, 0, K) + lane * 8;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l32 = lane & 31, lq = lane >> 5;
+    const int64_t at_l = id * rows_l * K + operand_at(ti * TILE, 0, K) + lane * 8, at_r = id * M * K + operand_at(tj * TILE, 0, K) + lane * 8;
+    const int64_t half = (int64_t)(K >> 4) * 512;  // to the other 32 rows
     const half_t *const lh = left.hi + at_l, *const ll = left.lo + at_l, *const rh = right.hi + at_r, *const rl = right.lo + at_r;
-    float16_t main, cross;
-#pragma unroll
-    for (int e = 0; e < 16; ++e) main[e] = cross[e] = 0.f;
-    const int steps = K / (STEP * GROUPS);  // K is a multiple of 64: each group has the same number
-    struct Operands {
-        half8_t xh, xl, yh, yl;
-    };
-    auto load = [&](Operands &o, int s) {
-        const int64_t at = (int64_t)(min(s, steps - 1) * GROUPS + group) * 512;
-        o.xh = *(const half8_t *)(lh + at);
-        o.xl = *(const half8_t *)(ll + at);
-        o.yh = *(const half8_t *)(rh + at);
-        o.yl = *(const half8_t *)(rl + at);
-    };
-    Operands ring[4];
-#pragma unroll
-    for (int s = 0; s < 3; ++s) load(ring[s], s);
-    for (int s = 0; s < steps; s += 4) {
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            if (s + q >= steps) break;
-            load(ring[(q + 3) & 3], s + q + 3);
-            const Operands &o = ring[q];
-            main = __builtin_amdgcn_mfma_f32_32x32x16_f16(o.xh, o.yh, main, 0, 0, 0);
-            cross = __builtin_amdgcn_mfma_f32_32x32x16_f16(o.xh, o.yl, cross, 0, 0, 0);
-            cross = __builtin_amdgcn_mfma_f32_32x32x16_f16(o.xl, o.yh, cross, 0, 0, 0);
-        }
-    }
-#pragma unroll
-    for (int e = 0; e < 16; ++e) main[e] = fmaf(cross[e], 1.f / SPLIT, main[e]);
-    // element e of a lane's tile: row 8 * (e / 4) + 4 * lq + e % 4, column l32.  A group finishes 16 / GROUPS of them
-    constexpr int MINE = 4 / GROUPS;  // fours of rows
-    f4 v[MINE];
-    if constexpr (GROUPS > 1) {
-#pragma unroll
-        for (int e = 0; e < 16; ++e) sums[((group * 4 + quarter) * 16 + e) * 64 + lane] = main[e];
-        __syncthreads();
-#pragma unroll
-        for (int k = 0; k < MINE; ++k) {
-            v[k] = f4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int q = 0; q < GROUPS; ++q)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) v[k][e] += sums[((q * 4 + quarter) * 16 + 4 * (group * MINE + k) + e) * 64 + lane];
-        }
-        if (WHAT == APPLY) __syncthreads();
-    } else {
-#pragma unroll
-        for (int k = 0; k < MINE; ++k) v[k] = f4{main[4 * k], main[4 * k + 1], main[4 * k + 2], main[4 * k + 3]};
-    }
-    float *const turn = sums + quarter * 32 * 33;  // [j][i]
+    // element e of a lane's 32 x 32: row 8 * (e / 4) + 4 * lq + e % 4, column l32.  A wave finishes MINE fours of rows of one
+    constexpr int MINE = 16 / GROUPS;
+    static_assert(MINE * GROUPS == 16 && MINE <= 4, "waves");
+    const int quarter = wave * MINE / 4, group = wave % (4 / MINE);
+    const int i0 = ti * TILE + (quarter >> 1) * 32, j0 = tj * TILE + (quarter & 1) * 32;
     f4 old[MINE];
     if (WHAT != GRAM) {
 #pragma unroll
@@ -379,6 +334,58 @@ __global__ __launch_bounds__(256 * GROUPS) void ks_muon_gemm_kernel(MuonArgs a, 
             old[k] = x.get(WHAT == POLY ? id * M * M + operand_at(j0 + l32, i0 + r, M) : id * M * N + operand_at(j0 + l32, i0 + r, N));
         }
     }
+    float16_t main[2][2], cross[2][2];
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) main[q >> 1][q & 1][e] = cross[q >> 1][q & 1][e] = 0.f;
+    struct Operands {
+        half8_t xh[2], xl[2], yh[2], yl[2];
+    };
+    const int steps = K / STEP;
+    auto load = [&](Operands &o, int s) {
+        const int64_t at = (int64_t)min(s, steps - 1) * 512;
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+            o.xh[q] = *(const half8_t *)(lh + at + q * half);
+            o.xl[q] = *(const half8_t *)(ll + at + q * half);
+            o.yh[q] = *(const half8_t *)(rh + at + q * half);
+            o.yl[q] = *(const half8_t *)(rl + at + q * half);
+        }
+    };
+    Operands ring[3];
+    load(ring[0], wave);
+    load(ring[1], wave + GROUPS);
+    for (int s = wave; s < steps; s += 3 * GROUPS) {
+#pragma unroll
+        for (int q = 0; q < 3; ++q) {
+            if (s + q * GROUPS >= steps) break;
+            load(ring[(q + 2) % 3], s + (q + 2) * GROUPS);
+            const Operands &o = ring[q];
+#pragma unroll
+            for (int p = 0; p < 4; ++p) {
+                main[p >> 1][p & 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(o.xh[p >> 1], o.yh[p & 1], main[p >> 1][p & 1], 0, 0, 0);
+                cross[p >> 1][p & 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(o.xh[p >> 1], o.yl[p & 1], cross[p >> 1][p & 1], 0, 0, 0);
+                cross[p >> 1][p & 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(o.xl[p >> 1], o.yh[p & 1], cross[p >> 1][p & 1], 0, 0, 0);
+            }
+        }
+    }
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) sums[((wave * 4 + q) * 16 + e) * 64 + lane] = fmaf(cross[q >> 1][q & 1][e], 1.f / SPLIT, main[q >> 1][q & 1][e]);
+    __syncthreads();
+    f4 v[MINE];
+#pragma unroll
+    for (int k = 0; k < MINE; ++k) {
+        v[k] = f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int q = 0; q < GROUPS; ++q)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[k][e] += sums[((q * 4 + quarter) * 16 + 4 * (group * MINE + k) + e) * 64 + lane];
+    }
+    if (WHAT == APPLY) __syncthreads();
+    float *const turn = sums + quarter * 32 * 33;  // [j][i]
 #pragma unroll
     for (int k = 0; k < MINE; ++k) {
         const int r = 8 * (group * MINE + k) + 4 * lq;
@@ -485,17 +492,21 @@ template <typename T> int run(const MuonArgs &a, int64_t matrices, char *ws, hip
     hipLaunchKernelGGL((ks_muon_load_kernel<T>), dim3((unsigned)(matrices * w.chunks)), dim3(256), 0, s, a, u, squares, w.chunks);
     hipLaunchKernelGGL(ks_muon_split_kernel, dim3((unsigned)full), dim3(256), 0, s, a, u, squares, w.chunks, flip ? xt : x, flip ? x : xt,
                        flip ? w.N : w.M, flip ? w.M : w.N);
+    int rc = KSMM_OK;
     auto gemm = [&](auto fn, int groups, int64_t tiles, Split l, Split r, Split old, Split out, Split turned, bool last) {
-        hipLaunchKernelGGL(fn, dim3((unsigned)((tiles + 7) / 8 * 8)), dim3(256 * groups), 0, s, a, l, r, old, out, turned, w.M, w.N, last, (int)tiles);
+        const int lds = groups * TILE * TILE * 4;
+        if (lds > 64 * 1024 && rc == KSMM_OK) rc = ensure_dynamic_lds((const void *)fn, lds);
+        if (rc != KSMM_OK) return;
+        hipLaunchKernelGGL(fn, dim3((unsigned)((tiles + 7) / 8 * 8)), dim3(64 * groups), lds, s, a, l, r, old, out, turned, w.M, w.N, last, (int)tiles);
     };
     for (int i = 0; i < a.steps; ++i) {
-        gemm(&ks_muon_gemm_kernel<T, GRAM, 4>, 4, square, x, x, x, gram, gram, false);
-        gemm(&ks_muon_gemm_kernel<T, POLY, 4>, 4, square, gram, gram, gram, poly, poly, false);
-        gemm(&ks_muon_gemm_kernel<T, APPLY, 1>, 1, full, xt, poly, x, y, yt, i + 1 == a.steps);
+        gemm(&ks_muon_gemm_kernel<T, GRAM, 8>, 8, square, x, x, x, gram, gram, false);
+        gemm(&ks_muon_gemm_kernel<T, POLY, 8>, 8, square, gram, gram, gram, poly, poly, false);
+        gemm(&ks_muon_gemm_kernel<T, APPLY, 4>, 4, full, xt, poly, x, y, yt, i + 1 == a.steps);
         std::swap(x, y);
         std::swap(xt, yt);
     }
-    return launched();
+    return rc == KSMM_OK ? launched() : rc;
 }
 
 int check(const ksmm_muon_desc *d, int64_t blocks, int c, int b, int parts, int dtype)
