@@ -11,8 +11,8 @@
 // Blocks that fit the LDS of a compute unit with their Gram matrix go through all steps in one launch, a workgroup
 // each (ks_muon_block_kernel).  Larger ones go step by step through tiles in global memory (ks_muon_gemm_kernel).  The
 // polynomial has slope p0 at zero: rounding errors of X grow up to p0^steps (485 for five of 3.4445) times, which is why
-// every product is fp32 (32-bit matrix instructions) whatever the type of the update.
-#include "ksmm_common.h"
+// every product is good to 22 bits with fp32 sums, whatever the type of the update.
+#include "ksmm_mfma.h"
 
 namespace ksmm {
 
@@ -68,35 +68,93 @@ __device__ __forceinline__ float wave_sum(float v)
     return v;
 }
 
-// ---- blocks that fit LDS -------------------------------------------------------------------------------
-constexpr int HELD = 8;  // 16 x 16 tiles of X a wave holds between reading the old X and writing the new one
-__host__ __device__ constexpr int up16(int v) { return (v + 15) / 16 * 16; }
-__host__ __device__ constexpr int64_t block_lds(int m, int n)
+// fp32 values as two fp16 ones, x = hi + lo / 2048: 22 bits.  A product of two such is three matrix instructions
+// (hi hi, and hi lo + lo hi in sums of their own; what lo lo would add is below the last bit), 96 clocks for 32 x 32 x 16
+// where the 32-bit instructions take 512.  |X| <= 1 here, so that no part leaves fp16's range.
+constexpr float SPLIT = 2048.f;
+__device__ __forceinline__ void split(float v, half_t &hi, half_t &lo)
 {
-    return 4 * ((int64_t)up16(m) * (up16(n) + 4) + (int64_t)up16(m) * (up16(m) + 4));
+    hi = (half_t)v;
+    lo = (half_t)((v - (float)hi) * SPLIT);
 }
 
-template <typename T, int WAVES>
+// ---- blocks that fit LDS -------------------------------------------------------------------------------
+// X and its Gram matrix (which the polynomial replaces) in LDS, hi and lo apart, sides padded to 32 with zeros; tiles of
+// 16 x 16 are dealt to the waves.  G and Q are symmetric: upper tiles only, and both operands of G G are rows.  Few of these
+// matrices fill no chip: what counts is the latency of fifteen products in a row.
+// (6,64,64,1): 28 us on 32-bit instructions; (1,128,128,3): 133.
+__host__ __device__ constexpr int up16(int v) { return (v + 15) / 16 * 16; }
+__host__ __device__ constexpr int up32(int v) { return (v + 31) / 32 * 32; }
+__host__ __device__ constexpr int64_t block_lds(int m, int n)
+{
+    return 4 * ((int64_t)up32(m) * (up32(n) + 8) + (int64_t)up32(m) * (up32(m) + 8));
+}
+
+// HELD: tiles of X a wave holds between reading the old X and writing the new one
+template <typename T, int WAVES, int HELD>
 __global__ __launch_bounds__(64 * WAVES) void ks_muon_block_kernel(MuonArgs a)
 {
-    extern __shared__ __attribute__((aligned(16))) float smem[];
+    constexpr int THREADS = 64 * WAVES, PER = HELD * 4, ONCE = PER < 16 ? PER : 16;  // elements a thread, and loaded at a time
+    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     __shared__ float red[WAVES];
     const bool flip = a.c > a.b;
-    const int m = flip ? a.b : a.c, n = flip ? a.c : a.b, M = up16(m), N = up16(n), ldx = N + 4, ldg = M + 4;
-    float *const X = smem, *const G = smem + M * ldx;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l16 = lane & 15, q = lane >> 4;
-    const int64_t base = matrix_base(a, blockIdx.x), pitch = (int64_t)a.parts * a.b;
-    const int count = a.c * a.b;
+    const int m = flip ? a.b : a.c, n = flip ? a.c : a.b, M = up32(m), N = up32(n), ldx = N + 8, ldg = M + 8;
+    half_t *const XH = (half_t *)smem, *const XL = XH + M * ldx, *const GH = XL + M * ldx, *const GL = GH + M * ldg;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int l16 = lane & 15, q = lane >> 4;
+    const int64_t base = matrix_base(a, blockIdx.x);
 
-    for (int i = tid; i < M * ldx; i += 64 * WAVES) X[i] = 0.f;
-    __syncthreads();
-    float ss = 0.f;
-    for (int i = tid; i < count; i += 64 * WAVES) {
-        const int r = i / a.b, k = i - r * a.b;
-        const float u = update_of<T>(a, base + r * pitch + k);
-        X[flip ? k * ldx + r : r * ldx + k] = u;
-        ss = fmaf(u, u, ss);
+    // the thread's elements tid, tid + THREADS, ..: row and column as stored, without a division each
+    struct Walk {
+        int r, k, dr, dk, c, b, pitch, ld;
+        bool flip;
+        __device__ __forceinline__ void next()
+        {
+            r += dr;
+            k += dk;
+            if (k >= b) {
+                k -= b;
+                ++r;
+            }
+        }
+        __device__ __forceinline__ bool in() const { return r < c; }
+        __device__ __forceinline__ int place() const { return in() ? r * pitch + k : 0; }  // in the tensors
+        __device__ __forceinline__ int inside() const { return flip ? k * ld + r : r * ld + k; }  // in X
+    };
+    const Walk start{tid / a.b, tid % a.b, THREADS / a.b, THREADS % a.b, a.c, a.b, a.parts * a.b, ldx, flip};
+    auto walk = [&]() {
+        Walk w = start;
+        asm volatile("" : "+v"(w.r), "+v"(w.k));  // (each walk is made anew: the places of one are not held for the next)
+        return w;
+    };
+    for (int i = tid; i < 2 * M * (ldx + ldg) / 8; i += THREADS) ((uint4_t *)smem)[i] = uint4_t{0u, 0u, 0u, 0u};
+    float u[PER], ss = 0.f;
+    {
+        Walk at = walk(), to = walk();
+        const T *const grad = (const T *)a.grad + base;
+#pragma unroll
+        for (int first = 0; first < PER; first += ONCE) {
+            float mom[ONCE];
+#pragma unroll
+            for (int e = 0; e < ONCE; ++e, at.next()) {
+                const float g = (float)grad[at.place()];
+                u[first + e] = at.in() ? g : 0.f;
+                if (a.m_in) mom[e] = a.m_in[base + at.place()];
+            }
+            if (a.m_in) {
+#pragma unroll
+                for (int e = 0; e < ONCE; ++e, to.next()) {
+                    const float v = fmaf(a.beta, mom[e], u[first + e]);
+                    if (to.in()) {
+                        a.m_out[base + to.place()] = v;
+                        u[first + e] = a.nesterov ? fmaf(a.beta, v, u[first + e]) : v;
+                    }
+                }
+            }
+        }
     }
+#pragma unroll
+    for (int e = 0; e < PER; ++e) ss = fmaf(u[e], u[e], ss);
     ss = wave_sum(ss);
     if (lane == 0) red[wave] = ss;
     __syncthreads();
@@ -104,113 +162,179 @@ __global__ __launch_bounds__(64 * WAVES) void ks_muon_block_kernel(MuonArgs a)
 #pragma unroll
     for (int i = 0; i < WAVES; ++i) ss += red[i];
     const float scale = 1.f / (sqrtf(ss) + a.eps);
-    for (int i = tid; i < M * ldx; i += 64 * WAVES) X[i] *= scale;
+    {
+        Walk at = walk();
+#pragma unroll
+        for (int e = 0; e < PER; ++e, at.next())
+            if (at.in()) split(u[e] * scale, XH[at.inside()], XL[at.inside()]);
+    }
     __syncthreads();
 
-    const int mt = M / 16, nt = N / 16, pairs = mt * (mt + 1) / 2, tiles = mt * nt;
-    // tile t of the upper triangle: (row, col >= row)
-    auto upper = [&](int t, int &i, int &j) {
-        i = 0;
-        int left = mt;
-        while (t >= left) {
+    const int mt = up16(m) / 16, nt = up16(n) / 16, pairs = mt * (mt + 1) / 2, tiles = mt * nt;
+    // the wave's tiles: of the upper triangle (row, col >= row), and of X
+    int pi[HELD], pj[HELD], xi[HELD], xj[HELD];
+#pragma unroll
+    for (int h = 0; h < HELD; ++h) {
+        int t = wave + h * WAVES, left = mt;
+        xi[h] = t / nt * 16;
+        xj[h] = t % nt * 16;
+        pi[h] = 0;
+        while (left > 0 && t >= left) {
             t -= left;
             --left;
-            ++i;
+            ++pi[h];
         }
-        j = i + t;
-    };
-    // S(16 rows from i0) times S'(16 rows from j0) transposed, K columns of both
-    auto rows_product = [&](const float *s, int lds, int i0, const float *t, int ldt, int j0, int K) {
-        f4 acc = {0.f, 0.f, 0.f, 0.f};
-        const float *ps = s + (i0 + l16) * lds + 4 * q, *pt = t + (j0 + l16) * ldt + 4 * q;
-        for (int k = 0; k < K; k += 16) {
-            const f4 x = *(const f4 *)(ps + k), y = *(const f4 *)(pt + k);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(x[e], y[e], acc, 0, 0, 0);
+        pj[h] = pi[h] + t;
+    }
+    // where the lane's part of a tile at (0, 0) lies: operand rows of X and G; columns of X; four of a row of G, rows of G and X
+    int at_x = l16 * ldx + 8 * q, at_g = l16 * ldg + 8 * q, at_c = (8 * q + (l16 >> 2)) * ldx + 4 * (l16 & 3);
+    int at_p = l16 * ldg + 4 * q, at_r = 4 * q * ldg + l16, at_o = 4 * q * ldx + l16;
+    // (the addresses of all tiles would be held through the steps, and spilled: each product makes its own)
+    auto fresh = [&]() { asm volatile("" : "+v"(at_x), "+v"(at_g), "+v"(at_c), "+v"(at_p), "+v"(at_r), "+v"(at_o)); };
+    // rows i0.. of (sh, sl) times rows j0.. of it, transposed, over K columns
+    auto rows_product = [&](const half_t *sh, const half_t *sl, int ld, int at, int i0, int j0, int K) {
+        const int x = at + i0 * ld, y = at + j0 * ld;
+        f4 main = {0.f, 0.f, 0.f, 0.f}, cross = {0.f, 0.f, 0.f, 0.f};
+        half8_t xh = *(const half8_t *)(sh + x), xl = *(const half8_t *)(sl + x), yh = *(const half8_t *)(sh + y), yl = *(const half8_t *)(sl + y);
+        for (int k = 32; k <= K; k += 32) {  // the next operands are read while these multiply
+            const int to = min(k, K - 32);
+            const half8_t ph = *(const half8_t *)(sh + x + to), pl = *(const half8_t *)(sl + x + to);
+            const half8_t rh = *(const half8_t *)(sh + y + to), rl = *(const half8_t *)(sl + y + to);
+            main = __builtin_amdgcn_mfma_f32_16x16x32_f16(xh, yh, main, 0, 0, 0);
+            cross = __builtin_amdgcn_mfma_f32_16x16x32_f16(xh, yl, cross, 0, 0, 0);
+            cross = __builtin_amdgcn_mfma_f32_16x16x32_f16(xl, yh, cross, 0, 0, 0);
+            xh = ph;
+            xl = pl;
+            yh = rh;
+            yl = rl;
         }
-        return acc;
-    };
-    for (int step = 0; step < a.steps; ++step) {
-        for (int t = wave; t < pairs; t += WAVES) {
-            int i, j;
-            upper(t, i, j);
-            const f4 v = rows_product(X, ldx, 16 * i, X, ldx, 16 * j, N);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int r = 16 * i + 4 * q + e, s = 16 * j + l16;
-                G[r * ldg + s] = v[e];
-                if (i != j) G[s * ldg + r] = v[e];
+        for (int e = 0; e < 4; ++e) main[e] = fmaf(cross[e], 1.f / SPLIT, main[e]);
+        return main;
+    };
+    // element e of a lane's tile: row 4 q + e, column l16
+    auto store_pair = [&](const f4 &v, int i, int j) {
+        half4_t h, l;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            half_t vh, vl;
+            split(v[e], vh, vl);
+            h[e] = vh;
+            l[e] = vl;
+            if (i != j) {
+                GH[at_r + (16 * i + e) * ldg + 16 * j] = vh;
+                GL[at_r + (16 * i + e) * ldg + 16 * j] = vl;
             }
+        }
+        *(half4_t *)(GH + at_p + 16 * j * ldg + 16 * i) = h;
+        *(half4_t *)(GL + at_p + 16 * j * ldg + 16 * i) = l;
+    };
+    auto wide = [&](const half_t *h, const half_t *l, int at) { return fmaf((float)l[at], 1.f / SPLIT, (float)h[at]); };
+    // 8 k of column l16: X[k0 + 8 q ..][j0 + l16]
+    auto columns = [&](const half_t *s, int k0, int j0) {
+        typedef short4_t __attribute__((address_space(3))) * lds_ptr;
+        typedef short short8_t __attribute__((ext_vector_type(8)));
+        const half_t *p = s + at_c + k0 * ldx + j0;
+        const short4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(p)), hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(p + 4 * ldx));
+        return __builtin_bit_cast(half8_t, short8_t{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]});
+    };
+    // the wave's tiles of X stay in registers too, unrounded
+    f4 mine[HELD];
+#pragma unroll
+    for (int h = 0; h < HELD; ++h)
+        if (wave + h * WAVES < tiles)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) mine[h][e] = wide(XH, XL, at_o + (xi[h] + e) * ldx + xj[h]);
+    for (int step = 0; step < a.steps; ++step) {
+#pragma unroll
+        for (int h = 0; h < HELD; ++h) {
+            if (wave + h * WAVES >= pairs) break;
+            fresh();
+            store_pair(rows_product(XH, XL, ldx, at_x, 16 * pi[h], 16 * pj[h], N), pi[h], pj[h]);
         }
         __syncthreads();
         f4 hold[HELD];
 #pragma unroll
         for (int h = 0; h < HELD; ++h) {
-            const int t = wave + h * WAVES;
-            if (t >= pairs) break;
-            int i, j;
-            upper(t, i, j);
-            const f4 v = rows_product(G, ldg, 16 * i, G, ldg, 16 * j, M);
+            if (wave + h * WAVES >= pairs) break;
+            fresh();
+            const int i = pi[h], j = pj[h];
+            const f4 v = rows_product(GH, GL, ldg, at_g, 16 * i, 16 * j, M);
+            const half4_t gh = *(const half4_t *)(GH + at_p + 16 * j * ldg + 16 * i), gl = *(const half4_t *)(GL + at_p + 16 * j * ldg + 16 * i);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) hold[h][e] = fmaf(a.p2, v[e], a.p1 * G[(16 * i + 4 * q + e) * ldg + 16 * j + l16]);
+            for (int e = 0; e < 4; ++e) hold[h][e] = fmaf(a.p2, v[e], a.p1 * fmaf((float)gl[e], 1.f / SPLIT, (float)gh[e]));
         }
         __syncthreads();
 #pragma unroll
         for (int h = 0; h < HELD; ++h) {
-            const int t = wave + h * WAVES;
-            if (t >= pairs) break;
-            int i, j;
-            upper(t, i, j);
+            if (wave + h * WAVES >= pairs) break;
+            fresh();
+            store_pair(hold[h], pi[h], pj[h]);
+        }
+        __syncthreads();
+#pragma unroll
+        for (int h = 0; h < HELD; ++h) {
+            if (wave + h * WAVES >= tiles) break;
+            fresh();
+            const int j0 = xj[h], x = at_g + xi[h] * ldg;
+            f4 main = {0.f, 0.f, 0.f, 0.f}, cross = {0.f, 0.f, 0.f, 0.f};
+            half8_t xh = *(const half8_t *)(GH + x), xl = *(const half8_t *)(GL + x), yh = columns(XH, 0, j0), yl = columns(XL, 0, j0);
+            for (int k = 32; k <= M; k += 32) {
+                const int to = min(k, M - 32);
+                const half8_t ph = *(const half8_t *)(GH + x + to), pl = *(const half8_t *)(GL + x + to);
+                const half8_t rh = columns(XH, to, j0), rl = columns(XL, to, j0);
+                main = __builtin_amdgcn_mfma_f32_16x16x32_f16(xh, yh, main, 0, 0, 0);
+                cross = __builtin_amdgcn_mfma_f32_16x16x32_f16(xh, yl, cross, 0, 0, 0);
+                cross = __builtin_amdgcn_mfma_f32_16x16x32_f16(xl, yh, cross, 0, 0, 0);
+                xh = ph;
+                xl = pl;
+                yh = rh;
+                yl = rl;
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) mine[h][e] = fmaf(a.p0, mine[h][e], fmaf(cross[e], 1.f / SPLIT, main[e]));
+        }
+        __syncthreads();
+#pragma unroll
+        for (int h = 0; h < HELD; ++h) {
+            if (wave + h * WAVES >= tiles) break;
+            fresh();
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const int r = 16 * i + 4 * q + e, s = 16 * j + l16;
-                G[r * ldg + s] = hold[h][e];
-                if (i != j) G[s * ldg + r] = hold[h][e];
+                const int to = at_o + (xi[h] + e) * ldx + xj[h];
+                split(mine[h][e], XH[to], XL[to]);
             }
-        }
-        __syncthreads();
-#pragma unroll
-        for (int h = 0; h < HELD; ++h) {
-            const int t = wave + h * WAVES;
-            if (t >= tiles) break;
-            const int i0 = t / nt * 16, j0 = t % nt * 16;
-            f4 acc = {0.f, 0.f, 0.f, 0.f};
-            for (int k = 0; k < M; k += 16) {
-                const f4 x = *(const f4 *)(G + (i0 + l16) * ldg + 4 * q + k);
-                const float *y = X + (k + 4 * q) * ldx + j0 + l16;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(x[e], y[e * ldx], acc, 0, 0, 0);
-            }
-#pragma unroll
-            for (int e = 0; e < 4; ++e) hold[h][e] = fmaf(a.p0, X[(i0 + 4 * q + e) * ldx + j0 + l16], acc[e]);
-        }
-        __syncthreads();
-#pragma unroll
-        for (int h = 0; h < HELD; ++h) {
-            const int t = wave + h * WAVES;
-            if (t >= tiles) break;
-            const int i0 = t / nt * 16, j0 = t % nt * 16;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) X[(i0 + 4 * q + e) * ldx + j0 + l16] = hold[h][e];
         }
         __syncthreads();
     }
-    for (int i = tid; i < count; i += 64 * WAVES) {
-        const int r = i / a.b, k = i - r * a.b;
-        finish<T>(a, base + r * pitch + k, X[flip ? k * ldx + r : r * ldx + k]);
+    Walk at = walk(), to = walk();
+#pragma unroll
+    for (int first = 0; first < PER; first += ONCE) {
+        float w[ONCE];
+        if (a.w_in) {
+#pragma unroll
+            for (int e = 0; e < ONCE; ++e, at.next())
+                w[e] = a.master_in ? a.master_in[base + at.place()] : (float)((const T *)a.w_in)[base + at.place()];
+        }
+#pragma unroll
+        for (int e = 0; e < ONCE; ++e, to.next()) {
+            if (!to.in()) continue;
+            float v = wide(XH, XL, to.inside());
+            if (a.w_in) {
+                v = fmaf(a.keep, w[e], -a.rate * v);
+                if (a.master_in) a.master_out[base + to.place()] = v;
+            }
+            ((T *)a.out)[base + to.place()] = (T)v;
+        }
     }
 }
 
 // ---- larger blocks: a launch a product --------------------------------------------------------------------
-// fp32 values as two fp16 ones, x = hi + lo / 2048: 22 bits.  A product of two such is three matrix instructions
-// (hi hi, and hi lo + lo hi in sums of their own; what lo lo would add is below the last bit), 96 clocks for 32 x 32 x 16
-// where the 32-bit instructions take 512.  |X| <= 1 here, so that no part leaves fp16's range.
 // In the workspace each matrix lies as X (M x N) and as its transpose, M and N multiples of 64 (zeros past its own
 // sides): with G and Q symmetric, every product is one of rows with rows, and its operands come straight from memory.  They
 // lie there as the instructions take them: 32 rows x 16 k are 1 KB in a row, 16 bytes a lane (operands gathered from plain
 // rows took 58 us a product of (1,1536,384,2) pairs, bound by addresses).
 constexpr int TILE = 64, STEP = 16;
-constexpr float SPLIT = 2048.f;
 __host__ __device__ constexpr int up64(int v) { return (v + 63) / 64 * 64; }
 
 // where element (r, k) of a matrix of K columns lies: lane r % 32 + 32 * (k % 16 / 8) of piece (r / 32, k / 16)
@@ -432,12 +556,12 @@ constexpr int64_t LDS_MOST = 160 * 1024 - 256;
 bool fits_lds(int m, int n)
 {
     const int64_t mt = up16(m) / 16, nt = up16(n) / 16;
-    return block_lds(m, n) <= LDS_MOST && mt * nt <= 16 * HELD && mt * (mt + 1) / 2 <= 16 * HELD;
+    return block_lds(m, n) <= LDS_MOST && mt * nt <= 16 * 8;
 }
 
-template <typename T, int WAVES> int run_block(const MuonArgs &a, int64_t matrices, int lds, hipStream_t s)
+template <typename T, int WAVES, int HELD> int run_block(const MuonArgs &a, int64_t matrices, int lds, hipStream_t s)
 {
-    const auto fn = &ks_muon_block_kernel<T, WAVES>;
+    const auto fn = &ks_muon_block_kernel<T, WAVES, HELD>;
     if (lds > 64 * 1024) {
         const int rc = ensure_dynamic_lds((const void *)fn, (int)LDS_MOST);
         if (rc != KSMM_OK) return rc;
@@ -478,7 +602,10 @@ template <typename T> int run(const MuonArgs &a, int64_t matrices, char *ws, hip
     const int m = std::min(a.c, a.b), n = std::max(a.c, a.b);
     if (fits_lds(m, n)) {
         const int lds = (int)block_lds(m, n), tiles = up16(m) / 16 * (up16(n) / 16);
-        return tiles <= 1 ? run_block<T, 1>(a, matrices, lds, s) : tiles <= 4 ? run_block<T, 4>(a, matrices, lds, s) : run_block<T, 16>(a, matrices, lds, s);
+        if (tiles <= 1) return run_block<T, 1, 1>(a, matrices, lds, s);
+        if (tiles <= 4) return run_block<T, 4, 1>(a, matrices, lds, s);
+        if (tiles <= 16) return run_block<T, 16, 1>(a, matrices, lds, s);
+        return tiles <= 64 ? run_block<T, 16, 4>(a, matrices, lds, s) : run_block<T, 16, 8>(a, matrices, lds, s);
     }
     const Space w = space(matrices, a.c, a.b);
     const int64_t mt = w.M / TILE, square = matrices * mt * mt, full = matrices * mt * (w.N / TILE);
