@@ -137,6 +137,9 @@ def gated_linear(x, factor, pattern, bias=None, act="silu", bs_last=False):
     ``x`` has a*c*d features, in the last axis, or with ``bs_last`` in the first, like the result's a*b*d.
     ``act``: "silu", "gelu" (erf form) or None.  Gradients of all three go through one call that computes
     the projections again instead of keeping them; they cannot be differentiated a second time."""
+    out = _lib.native().gated_linear(x, factor, pattern, bias, act, bs_last)
+    if out is not None:
+        return out
     if torch.is_grad_enabled() and (x.requires_grad or factor.requires_grad or (bias is not None and bias.requires_grad)):
         return KSGatedFunction.apply(x, factor, bias, tuple(pattern), act, bs_last)
     return GatedKernel.forward(x, factor, pattern, bias, act, bs_last)
@@ -317,6 +320,9 @@ def residual_norm(x, residual, gate=None, post_weight=None, weight=None, bias=No
     addition alone, n_out is None.  Missing gates and weights count as ones.  Everything has a gradient but ``alpha``;
     gradients cannot be differentiated a second time."""
     inputs = x, residual, gate, post_weight, weight, bias
+    out = _lib.native().residual_norm(*inputs, alpha, norm, eps, bs_last, need_norm)
+    if out is not None:
+        return out
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in inputs):
         out = ResidualNormFunction.apply(*inputs, float(alpha), norm, float(eps), bs_last, need_norm)
         return (residual, out) if x is None else out if need_norm else (out, None)

@@ -14,7 +14,11 @@
 #include <ATen/ATen.h>
 #include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPStream.h>
+#include <torch/csrc/autograd/function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/autograd/saved_variable.h>
 
 #include "../../include/ksmm_hip.h"
 
@@ -342,9 +346,284 @@ PyObject *py_train_backward(PyObject *, PyObject *const *args, Py_ssize_t n_args
     Py_RETURN_NONE;
 }
 
+// ---- operators around a feed-forward block ------------------------------------------------------------------
+// Their autograd nodes are C++ ones: a forward and a backward pass through Python ones took 175 us of host time, more
+// than the kernels of 25088 rows.
+
+namespace ag = torch::autograd;
+
+// a tensor argument, or none; false: neither
+bool read_optional(PyObject *o, at::Tensor *t)
+{
+    if (o == Py_None) return true;
+    if (!THPVariable_Check(o)) return false;
+    *t = THPVariable_Unpack(o);
+    return t->defined();
+}
+bool like(const at::Tensor &t, const at::Tensor &of)
+{
+    return t.scalar_type() == of.scalar_type() && t.device() == of.device() && t.is_contiguous() && !t._fw_grad(0).defined();
+}
+const void *data_of(const at::Tensor &t) { return t.defined() ? t.const_data_ptr() : nullptr; }
+void *out_of(const at::Tensor &t) { return t.defined() ? t.mutable_data_ptr() : nullptr; }
+void *stream_of(const at::Tensor &t) { return c10::hip::getCurrentHIPStream(t.device().index()).stream(); }
+void check_status(int status)
+{
+    TORCH_CHECK(status == KSMM_OK, "ksmm: ", ksmm_strerror(status), " (status ", status, ")");
+}
+// what a node returns, when its gradients are asked to be differentiated in their turn
+ag::variable_list once(ag::variable_list &&grads, const char *name)
+{
+    if (!at::GradMode::is_enabled()) return std::move(grads);
+    const auto error = std::make_shared<ag::DelayedError>(std::string(name) + ": its gradients cannot be differentiated again", (int64_t)grads.size());
+    return (*error)(std::move(grads));
+}
+
+struct NormHow {
+    double alpha, eps;
+    int kind;
+    bool bs_last;
+    int64_t batch, features, groups;
+};
+ksmm_norm_desc norm_desc(const at::Tensor (&in)[6], const NormHow &how)
+{
+    return ksmm_norm_desc{data_of(in[0]), data_of(in[1]), data_of(in[2]), data_of(in[3]), data_of(in[4]), data_of(in[5]),
+                          how.groups, (float)how.alpha, (float)how.eps, how.kind};
+}
+
+struct NormNode : ag::Node {
+    ag::SavedVariable in[6], stats;  // x, residual, gate, post_weight, weight, bias
+    NormHow how;
+    int r_at, n_at;  // which of the node's outputs r and n are, -1: none
+    std::string name() const override { return "ResidualNormBackward"; }
+    void release_variables() override
+    {
+        for (auto &v : in) v.reset_data();
+        stats.reset_data();
+    }
+    ag::variable_list apply(ag::variable_list &&grads) override
+    {
+        std::lock_guard<std::mutex> lock(mutex_);
+        at::Tensor t[6], out[6];
+        for (int i = 0; i < 6; ++i) t[i] = in[i].unpack();
+        const at::Tensor s = stats.unpack();
+        at::Tensor dr, dn;
+        if (r_at >= 0 && grads[r_at].defined()) dr = grads[r_at].contiguous();
+        if (n_at >= 0 && grads[n_at].defined()) dn = grads[n_at].contiguous();
+        ag::variable_list result(6);
+        if (!dr.defined() && !dn.defined()) return result;
+        {
+        at::NoGradGuard no_grad;
+        DeviceScope scope(t[1].device().index());
+        const bool group_gates = how.bs_last && how.groups > 1 && t[2].defined() && task_should_compute_output(2);
+        for (int i = 0; i < 6; ++i) {
+            if (!t[i].defined() || !(task_should_compute_output(i) || (i == 1 && group_gates))) continue;
+            out[i] = !dn.defined() && i >= 4 ? at::zeros_like(t[i]) : at::empty_like(t[i]);
+        }
+        const int dt = code_of(t[1].scalar_type());
+        const int64_t need = ksmm_residual_norm_backward_workspace(how.batch, how.features, how.groups, dt, how.bs_last);
+        check_status(need < 0 ? (int)need : KSMM_OK);
+        const at::Tensor ws = at::empty({need}, t[1].options().dtype(at::kByte));
+        const ksmm_norm_desc d = norm_desc(t, how);
+        check_status(ksmm_residual_norm_backward(&d, s.const_data_ptr<float>(), data_of(dr), data_of(dn), out_of(out[0]), out_of(out[1]), out_of(out[2]),
+                                                 out_of(out[3]), out_of(out[4]), out_of(out[5]), ws.mutable_data_ptr(), need, how.batch, how.features, dt,
+                                                 how.bs_last, stream_of(t[1])));
+        }
+        for (int i = 0; i < 6; ++i)
+            if (task_should_compute_output(i)) result[i] = out[i];
+        return once(std::move(result), "residual_norm");
+    }
+};
+
+// residual_norm(x, residual, gate, post_weight, weight, bias, alpha, kind, eps, bs_last, need_norm) -> (r_out, n_out) or None
+PyObject *py_residual_norm(PyObject *, PyObject *const *args, Py_ssize_t n_args)
+{
+    if (n_args != 11) {
+        PyErr_SetString(PyExc_TypeError, "residual_norm() takes 11 arguments");
+        return nullptr;
+    }
+    try {
+        at::Tensor in[6];
+        bool taken = true;
+        for (int i = 0; i < 6 && taken; ++i) taken = read_optional(args[i], &in[i]);
+        const at::Tensor &x = in[0], &res = in[1];
+        NormHow how;
+        how.alpha = PyFloat_AsDouble(args[6]);
+        how.kind = PyUnicode_Check(args[7]) ? PyUnicode_CompareWithASCIIString(args[7], "rms") == 0     ? KSMM_NORM_RMS
+                                              : PyUnicode_CompareWithASCIIString(args[7], "layer") == 0 ? KSMM_NORM_LAYER
+                                                                                                         : -1
+                                            : -1;
+        how.eps = PyFloat_AsDouble(args[8]);
+        how.bs_last = PyObject_IsTrue(args[9]) == 1;
+        const bool need_norm = PyObject_IsTrue(args[10]) == 1;
+        taken = taken && !PyErr_Occurred() && how.kind >= 0 && res.defined() && res.is_cuda() && trainable(res.scalar_type()) && res.dim() > 0 &&
+                res.numel() > 0 && (x.defined() || (need_norm && !in[2].defined() && !in[3].defined()));
+        if (taken) {
+            how.features = res.size(how.bs_last ? 0 : res.dim() - 1);
+            how.batch = res.numel() / how.features;
+            how.groups = 1;
+            for (int i = 0; i < 6 && taken; ++i) {
+                if (!in[i].defined()) continue;
+                taken = like(in[i], res);
+                if (i == 0) taken = taken && x.sizes() == res.sizes();
+                if (i >= 3) taken = taken && in[i].numel() == how.features;
+                if (i == 2) {
+                    how.groups = in[2].numel() / how.features;
+                    taken = taken && in[2].dim() > 0 && in[2].size(in[2].dim() - 1) == how.features && how.groups > 0 && how.batch % how.groups == 0;
+                }
+            }
+        }
+        if (taken) {
+            bool gradients = false;
+            if (at::GradMode::is_enabled())
+                for (const at::Tensor &t : in) gradients |= t.defined() && t.requires_grad();
+            at::Tensor r, n, stats;
+            int status;
+            {
+                WithoutGil released;
+                DeviceScope scope(res.device().index());
+                at::AutoDispatchBelowADInplaceOrView below;
+                r = x.defined() ? at::empty_like(res) : res;
+                if (need_norm) n = at::empty_like(res);
+                if (gradients) stats = at::empty({4, how.batch}, res.options().dtype(at::kFloat));
+                const ksmm_norm_desc d = norm_desc(in, how);
+                status = ksmm_residual_norm_forward(&d, x.defined() ? out_of(r) : nullptr, out_of(n), gradients ? stats.mutable_data_ptr<float>() : nullptr,
+                                                    how.batch, how.features, code_of(res.scalar_type()), how.bs_last, stream_of(res));
+            }
+            if (status == KSMM_OK) {
+                if (gradients) {
+                    std::shared_ptr<NormNode> node(new NormNode(), ag::deleteNode);
+                    node->set_next_edges(ag::collect_next_edges(in[0], in[1], in[2], in[3], in[4], in[5]));
+                    node->how = how;
+                    for (int i = 0; i < 6; ++i) node->in[i] = ag::SavedVariable(in[i], false);
+                    node->stats = ag::SavedVariable(stats, false);
+                    node->r_at = x.defined() ? 0 : -1;
+                    node->n_at = !need_norm ? -1 : x.defined() ? 1 : 0;
+                    if (x.defined()) ag::set_history(r, node);
+                    if (need_norm) ag::set_history(n, node);
+                }
+                return Py_BuildValue("(NN)", THPVariable_Wrap(r), wrapped(n));
+            }
+        }
+    } catch (const std::exception &) {
+    }
+    PyErr_Clear();
+    Py_RETURN_NONE;
+}
+
+struct GatedHow {
+    int a, b, c, d, act;
+    bool bs_last;
+    int64_t batch;
+};
+
+struct GatedNode : ag::Node {
+    ag::SavedVariable in[3];  // x, factor, bias
+    GatedHow how;
+    std::string name() const override { return "GatedLinearBackward"; }
+    void release_variables() override
+    {
+        for (auto &v : in) v.reset_data();
+    }
+    ag::variable_list apply(ag::variable_list &&grads) override
+    {
+        std::lock_guard<std::mutex> lock(mutex_);
+        ag::variable_list result(3);
+        if (!grads[0].defined()) return result;
+        at::Tensor t[3], out[3];
+        for (int i = 0; i < 3; ++i) t[i] = in[i].unpack();
+        const at::Tensor dh = grads[0].contiguous();
+        {
+            at::NoGradGuard no_grad;
+            DeviceScope scope(t[0].device().index());
+            for (int i = 0; i < 3; ++i)
+                if (t[i].defined() && task_should_compute_output(i)) out[i] = at::empty_like(t[i]);
+            const int dt = code_of(t[0].scalar_type());
+            const int64_t need = ksmm_gated_backward_workspace(how.batch, how.a, how.b, how.c, how.d, dt, how.bs_last);
+            check_status(need < 0 ? (int)need : KSMM_OK);
+            const at::Tensor ws = at::empty({need}, t[0].options().dtype(at::kByte));
+            check_status(ksmm_gated_backward(data_of(dh), data_of(t[0]), data_of(t[1]), data_of(t[2]), out_of(out[0]), out_of(out[1]), out_of(out[2]),
+                                             ws.mutable_data_ptr(), need, how.batch, how.a, how.b, how.c, how.d, dt, how.bs_last, how.act, stream_of(t[0])));
+        }
+        for (int i = 0; i < 3; ++i) result[i] = out[i];
+        return once(std::move(result), "gated_linear");
+    }
+};
+
+// gated_linear(x, factor, pattern, bias, act, bs_last) -> h or None
+PyObject *py_gated_linear(PyObject *, PyObject *const *args, Py_ssize_t n_args)
+{
+    if (n_args != 6) {
+        PyErr_SetString(PyExc_TypeError, "gated_linear() takes 6 arguments");
+        return nullptr;
+    }
+    try {
+        at::Tensor x, w, bias;
+        int64_t v[4] = {0, 0, 0, 0};
+        bool taken = THPVariable_Check(args[0]) && THPVariable_Check(args[1]) && read_optional(args[3], &bias) && PyTuple_Check(args[2]) && PyTuple_GET_SIZE(args[2]) == 4;
+        GatedHow how;
+        how.bs_last = PyObject_IsTrue(args[5]) == 1;
+        how.act = args[4] == Py_None ? KSMM_ACT_NONE : -1;
+        if (PyUnicode_Check(args[4]))
+            how.act = PyUnicode_CompareWithASCIIString(args[4], "silu") == 0   ? KSMM_ACT_SILU
+                      : PyUnicode_CompareWithASCIIString(args[4], "gelu") == 0 ? KSMM_ACT_GELU
+                      : PyUnicode_CompareWithASCIIString(args[4], "none") == 0 ? KSMM_ACT_NONE
+                                                                                : -1;
+        for (int k = 0; k < 4 && taken; ++k) {
+            v[k] = PyLong_AsLongLong(PyTuple_GET_ITEM(args[2], k));
+            taken = v[k] >= 1 && v[k] <= 0x3fffffff;
+        }
+        if (taken) {
+            x = THPVariable_Unpack(args[0]);
+            w = THPVariable_Unpack(args[1]);
+            const int64_t in_size = v[0] * v[2] * v[3], out_size = v[0] * v[1] * v[3];
+            taken = how.act >= 0 && x.is_cuda() && trainable(x.scalar_type()) && x.dim() > 0 && x.numel() > 0 && like(x, x) && like(w, x) && w.dim() == 2 &&
+                    w.size(0) == in_size && w.size(1) == 2 * v[1] && x.size(how.bs_last ? 0 : x.dim() - 1) == in_size &&
+                    (!bias.defined() || (like(bias, x) && bias.numel() == 2 * out_size));
+            if (taken) {
+                how.a = (int)v[0];
+                how.b = (int)v[1];
+                how.c = (int)v[2];
+                how.d = (int)v[3];
+                how.batch = x.numel() / in_size;
+                c10::SmallVector<int64_t, 6> shape(x.sizes().begin(), x.sizes().end());
+                shape[how.bs_last ? 0 : shape.size() - 1] = out_size;
+                const bool gradients = at::GradMode::is_enabled() && (x.requires_grad() || w.requires_grad() || (bias.defined() && bias.requires_grad()));
+                at::Tensor h;
+                int status;
+                {
+                    WithoutGil released;
+                    DeviceScope scope(x.device().index());
+                    at::AutoDispatchBelowADInplaceOrView below;
+                    h = at::empty(shape, x.options());
+                    status = ksmm_gated_forward(data_of(x), data_of(w), data_of(bias), out_of(h), how.batch, how.a, how.b, how.c, how.d,
+                                                code_of(x.scalar_type()), how.bs_last, how.act, stream_of(x));
+                }
+                if (status == KSMM_OK) {
+                    if (gradients) {
+                        std::shared_ptr<GatedNode> node(new GatedNode(), ag::deleteNode);
+                        node->set_next_edges(ag::collect_next_edges(x, w, bias));
+                        node->how = how;
+                        node->in[0] = ag::SavedVariable(x, false);
+                        node->in[1] = ag::SavedVariable(w, false);
+                        node->in[2] = ag::SavedVariable(bias, false);
+                        ag::set_history(h, node);
+                    }
+                    return THPVariable_Wrap(h);
+                }
+            }
+        }
+    } catch (const std::exception &) {
+    }
+    PyErr_Clear();
+    Py_RETURN_NONE;
+}
+
 PyMethodDef methods[] = {
     {"train_forward", (PyCFunction)(void (*)(void))py_train_forward, METH_FASTCALL, "one layer, its intermediates kept"},
     {"train_backward", (PyCFunction)(void (*)(void))py_train_backward, METH_FASTCALL, "gradients of one layer"},
+    {"residual_norm", (PyCFunction)(void (*)(void))py_residual_norm, METH_FASTCALL, "gated residual addition between two norms"},
+    {"gated_linear", (PyCFunction)(void (*)(void))py_gated_linear, METH_FASTCALL, "gated projection"},
     {"infer", (PyCFunction)(void (*)(void))py_infer, METH_FASTCALL, "one layer without gradients"},
     {nullptr, nullptr, 0, nullptr},
 };

@@ -271,3 +271,47 @@ def test_refusals():
     ]:
         with pytest.raises(error):
             call()
+
+
+def test_second_derivatives_are_refused_and_saved_tensors_guarded():
+    from ksmm_amd import gated_linear, residual_norm
+
+    with torch.enable_grad():
+        r = torch.randn(5, 32, device="cuda", requires_grad=True)
+        n = residual_norm(None, r)[1]
+        g, = torch.autograd.grad(n.sum(), r, create_graph=True)
+        with pytest.raises(RuntimeError):
+            g.sum().backward()
+        x = torch.randn(5, 32, device="cuda", requires_grad=True)
+        w = torch.randn(32, 16, device="cuda", requires_grad=True)
+        h = gated_linear(x, w, (1, 8, 32, 1))
+        g, = torch.autograd.grad(h.sum(), x, create_graph=True)
+        with pytest.raises(RuntimeError):
+            g.sum().backward()
+        h = gated_linear(x, w, (1, 8, 32, 1))
+        with torch.no_grad():
+            w.add_(1.0)
+        with pytest.raises(RuntimeError):  # changed in between
+            h.sum().backward()
+
+
+def test_through_ctypes_gives_the_same(monkeypatch):
+    """Where the CPython module is not there, the same kernels run through ctypes and Python autograd nodes."""
+    from ksmm_amd import _lib, gated_linear, residual_norm
+
+    t, dr, dn = tensors(96, 50, torch.float16, False, groups=5)
+    dev = [v.cuda().requires_grad_() for v in t.values()]
+    w = torch.randn(96, 2 * 48, device="cuda").half().requires_grad_()
+
+    def all_of():
+        with torch.enable_grad():
+            r, n = residual_norm(*dev, 0.7)
+            h = gated_linear(n, w, (1, 48, 96, 1), act="gelu")
+            return [r, n, h, *torch.autograd.grad([r, h], [*dev, w], [dr.cuda(), h.detach()])]
+
+    native = all_of()
+    assert native[1].grad_fn.name() == "ResidualNormBackward" and native[2].grad_fn.name() == "GatedLinearBackward"
+    monkeypatch.setattr(_lib, "_native", _lib._NoNative)
+    python = all_of()
+    assert "ResidualNormFunction" in python[1].grad_fn.name()
+    assert all(torch.equal(a, b) for a, b in zip(native, python))
