@@ -342,7 +342,8 @@ int ksmm_gated_backward(const void *dh, const void *x, const void *w, const void
  * the features of a row.  Tensors are (batch, features), or (features, batch) with bs_last.  gate has `groups` rows of
  * features, each for batch / groups consecutive rows of the tensors.  x NULL: r_out is the residual and is not
  * written.  n_out NULL: not wanted.  NULL gate and weight count as ones, NULL bias as zeros.
- * stats (NULL: not wanted): 4 x batch floats for the backward pass.
+ * stats (NULL: not wanted): 4 x batch floats for the backward pass.  Needs
+ * ksmm_residual_norm_forward_workspace() bytes of 16-byte aligned device memory (0: none).
  * Batch-size-first rows of up to 8192 features; batch-size-last any number. */
 typedef enum ksmm_norm_kind { KSMM_NORM_RMS = 0, KSMM_NORM_LAYER = 1 } ksmm_norm_kind;
 typedef struct ksmm_norm_desc {
@@ -351,8 +352,10 @@ typedef struct ksmm_norm_desc {
     float alpha, eps;
     int kind; /* ksmm_norm_kind */
 } ksmm_norm_desc;
-int ksmm_residual_norm_forward(const ksmm_norm_desc *desc, void *r_out, void *n_out, float *stats, int64_t batch,
-                               int64_t features, int dtype, int bs_last, void *stream);
+int64_t ksmm_residual_norm_forward_workspace(int64_t batch, int64_t features, int dtype, int bs_last);
+int ksmm_residual_norm_forward(const ksmm_norm_desc *desc, void *r_out, void *n_out, float *stats, void *workspace,
+                               int64_t workspace_bytes, int64_t batch, int64_t features, int dtype, int bs_last,
+                               void *stream);
 /* Gradients from those of the results (either may be NULL: zero).  What is not wanted is NULL; dgate of more than one
  * group in batch-size-last layout needs dresidual.  dgate, dpost_weight, dweight and dbias are sums in a fixed order. */
 int64_t ksmm_residual_norm_backward_workspace(int64_t batch, int64_t features, int64_t groups, int dtype,

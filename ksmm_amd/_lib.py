@@ -106,7 +106,8 @@ SIGNATURES = {
     "ksmm_gated_backward_workspace": (c_i64, [c_i64, c_int, c_int, c_int, c_int, c_int, c_int]),
     "ksmm_gated_backward": (c_int, [c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_i64, c_i64, c_int, c_int, c_int, c_int,
                                     c_int, c_int, c_int, c_vp]),
-    "ksmm_residual_norm_forward": (c_int, [ctypes.POINTER(KsmmNormDesc), c_vp, c_vp, c_vp, c_i64, c_i64, c_int, c_int, c_vp]),
+    "ksmm_residual_norm_forward_workspace": (c_i64, [c_i64, c_i64, c_int, c_int]),
+    "ksmm_residual_norm_forward": (c_int, [ctypes.POINTER(KsmmNormDesc), c_vp, c_vp, c_vp, c_vp, c_i64, c_i64, c_i64, c_int, c_int, c_vp]),
     "ksmm_residual_norm_backward_workspace": (c_i64, [c_i64, c_i64, c_i64, c_int, c_int]),
     "ksmm_residual_norm_backward": (c_int, [ctypes.POINTER(KsmmNormDesc), c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp,
                                             c_vp, c_i64, c_i64, c_i64, c_int, c_int, c_vp]),

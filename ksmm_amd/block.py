@@ -240,9 +240,14 @@ class NormKernel:
         stats = torch.empty(4, batch, dtype=torch.float32, device=residual.device) if need_stats else None
         if batch > 0:
             desc = NormKernel._desc(x, residual, gate, post_weight, weight, bias, alpha, norm, eps, groups)
+            dt = dtype_code(residual.dtype)
+            need = lib.ksmm_residual_norm_forward_workspace(batch, features, dt, int(bs_last))
+            if need < 0:
+                _lib.check(int(need))
+            workspace = torch.empty(need, dtype=torch.uint8, device=residual.device) if need else None
             with torch.cuda.device(residual.device):
                 _lib.check(lib.ksmm_residual_norm_forward(ctypes.byref(desc), None if x is None else r.data_ptr(), _ptr(n), _ptr(stats),
-                                                          batch, features, dtype_code(residual.dtype), int(bs_last), _stream_ptr(residual)))
+                                                          _ptr(workspace), need, batch, features, dt, int(bs_last), _stream_ptr(residual)))
         return r, n, stats
 
     @staticmethod

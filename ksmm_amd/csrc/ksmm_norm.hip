@@ -869,6 +869,263 @@ __global__ __launch_bounds__(COL_THREADS) void ks_norm_cols_bwd_kernel(NormArgs 
     }
 }
 
+// The same in steps, for many features of few columns: a launch a step, a workgroup takes 64 columns x CHUNK features, and leaves its part of the sums over features to the
+// next step.  (A step reads its operands again: what it needs of r', v and D is computed anew, unrounded.)
+//   forward   X_STATS  statistics of x       MID  r', its statistics     OUT  n
+//   backward  SUMS     sums over dn          RES  dr, sums over it       DX   dx
+// Statistics: mean and sum of squared differences of a chunk, both taken from values in registers, put together by
+// the formula for two sets, n1 n2 / (n1 + n2) (mean1 - mean2)^2.
+enum { X_STATS, MID, OUT, SUMS, RES, DX };
+constexpr int STEP_LANES = 16, STEP_COLS = 4 * STEP_LANES, STEP_FPT = 4, CHUNK = COL_THREADS / STEP_LANES * STEP_FPT;
+struct StepSpace {
+    float *x, *r, *m, *k;  // [chunk][2][batch] each
+    int tiles, chunks;
+};
+
+template <typename T, int STEP>
+__global__ __launch_bounds__(COL_THREADS, 4) void ks_norm_step_kernel(NormArgs a, NormGrads d, StepSpace sp)
+{
+    constexpr int LANES = STEP_LANES, GROUPS = COL_THREADS / LANES, FPT = STEP_FPT;
+    constexpr bool FORWARD = STEP <= OUT;
+    __shared__ float red[2 * COL_WAVES * 4 * LANES];
+    __shared__ Params held[CHUNK];
+    __shared__ float known[6][STEP_COLS];  // of a column: mean and factor of x's norm, of r's; sums
+    ColSum<LANES> sum{red};
+    const int blocks = sp.tiles * sp.chunks, per_xcd = (blocks + 7) / 8, lid = (blockIdx.x & 7) * per_xcd + (blockIdx.x >> 3);
+    if ((int)(blockIdx.x >> 3) >= per_xcd || lid >= blocks) return;
+    const int tile = lid % sp.tiles, chunk = lid / sp.tiles, H = a.features, h0 = chunk * CHUNK, h_end = min(H, h0 + CHUNK);
+    const int grp = threadIdx.x / LANES, lane4 = threadIdx.x % LANES * 4;
+    const int64_t B = a.batch, col0 = (int64_t)tile * STEP_COLS, col = col0 + lane4;
+    const int count = (int)max((int64_t)0, min((int64_t)4, B - col));  // (none: the thread adds zeros)
+    const float inv = 1.f / (float)H;
+    const T *const x = (const T *)a.x, *const res = (const T *)a.residual, *const dn = (const T *)d.dn_out, *const dr_in = (const T *)d.dr_out;
+    const bool post = a.post_weight != nullptr, one_gate = a.group_rows == B, own_gates = a.gate && !one_gate;
+    // operands
+    Raw<T> xv[FPT] = {}, rv[FPT] = {}, nv[FPT] = {}, dv[FPT] = {};
+#pragma unroll
+    for (int i = 0; i < FPT; ++i) {
+        const int h = h0 + grp + i * GROUPS;
+        if (h < h_end) {
+            if (x) xv[i] = load_four(x + h * B + col, count);
+            if (STEP != X_STATS && (FORWARD || dn)) rv[i] = load_four(res + h * B + col, count);
+            if (!FORWARD && dn) nv[i] = load_four(dn + h * B + col, count);
+            if ((STEP == RES || STEP == DX) && dr_in) dv[i] = load_four(dr_in + h * B + col, count);
+        }
+    }
+    for (int h = threadIdx.x; h < h_end - h0; h += COL_THREADS) held[h] = params_of<T>(a, one_gate, h0 + h);
+    // what the steps before left
+    if (threadIdx.x < STEP_COLS && col0 + threadIdx.x < B) {
+        const int64_t c = col0 + threadIdx.x;
+        auto statistics = [&](const float *part, int to) {
+            float n = 0.f, mean = 0.f, m2 = 0.f;
+            for (int k = 0; k < sp.chunks; ++k) {
+                const float nk = (float)(min(H, (k + 1) * CHUNK) - k * CHUNK), mk = part[(2 * k) * B + c], sk = part[(2 * k + 1) * B + c];
+                const float diff = mk - mean, both = n + nk;
+                mean = fmaf(diff, nk / both, mean);
+                m2 += sk + diff * diff * (n * nk / both);
+                n = both;
+            }
+            known[to][threadIdx.x] = mean;  // (0 without a mean: the chunks' are)
+            known[to + 1][threadIdx.x] = rsqrtf(fmaf(m2, inv, a.eps));
+        };
+        auto total = [&](const float *part, int to) {
+            float s1 = 0.f, s2 = 0.f;
+            for (int k = 0; k < sp.chunks; ++k) {
+                s1 += part[(2 * k) * B + c];
+                s2 += part[(2 * k + 1) * B + c];
+            }
+            known[to][threadIdx.x] = a.layer ? s1 * inv : 0.f;
+            known[to + 1][threadIdx.x] = s2 * inv;
+        };
+        known[0][threadIdx.x] = known[2][threadIdx.x] = 0.f;
+        known[1][threadIdx.x] = known[3][threadIdx.x] = 1.f;
+        if (FORWARD) {
+            if (STEP != X_STATS && x && post) statistics(sp.x, 0);
+            if (STEP == OUT) statistics(sp.r, 2);
+            if (STEP == (a.n_out ? OUT : MID) && a.stats && chunk == 0) {
+                for (int q = 0; q < 4; ++q) a.stats[q * B + c] = known[q][threadIdx.x];
+            }
+        } else {
+            for (int q = 0; q < 4; ++q) known[q][threadIdx.x] = a.stats[q * B + c];
+            if (STEP != SUMS && dn) total(sp.m, 4);
+        }
+    }
+    __syncthreads();
+    Four mean_x, rho_x, mean_r, rho_r, m1 = {}, m2 = {};
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+        const bool in = c < count;
+        mean_x.v[c] = in ? known[0][lane4 + c] : 0.f;
+        rho_x.v[c] = in ? known[1][lane4 + c] : 0.f;
+        mean_r.v[c] = in ? known[2][lane4 + c] : 0.f;
+        rho_r.v[c] = in ? known[3][lane4 + c] : 0.f;
+        if (!FORWARD && STEP != SUMS && dn) {
+            m1.v[c] = in ? known[4][lane4 + c] : 0.f;
+            m2.v[c] = in ? known[5][lane4 + c] : 0.f;
+        }
+    }
+    const T *gate[4];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) gate[c] = own_gates ? (const T *)a.gate + min(col + c, B - 1) / a.group_rows * H : nullptr;
+    auto factor = [&](const Params &p, int c, int h) { return own_gates ? a.alpha * (float)gate[c][h] : p.gate; };
+    auto each = [&](auto f) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < FPT; ++i) {
+            const int h = h0 + grp + i * GROUPS;
+            opaque(xv[i]);
+            opaque(rv[i]);
+            if (h < h_end) f(i, h, held[h - h0]);
+        }
+    };
+    auto get_u = [&](int i) {
+        Four u = {};
+        if (x) {
+#pragma unroll
+            for (int c = 0; c < 4; ++c) u.v[c] = post ? ((float)xv[i].v[c] - mean_x.v[c]) * rho_x.v[c] : (float)xv[i].v[c];
+        }
+        return u;
+    };
+    auto get_r = [&](int i, int h, const Params &p, const Four &u) {
+        Four r = wide_of(rv[i]);
+        if (x) {
+#pragma unroll
+            for (int c = 0; c < 4; ++c) r.v[c] = fmaf(factor(p, c, h), u.v[c] * p.post, r.v[c]);
+        }
+        return r;
+    };
+    // this chunk's statistics of value(i, h, p)
+    auto leave_statistics = [&](auto value, float *part) {
+        Four mean = {}, s = {};
+        if (a.layer) {
+            each([&](int i, int h, const Params &p) {
+                const Four v = value(i, h, p);
+#pragma unroll
+                for (int c = 0; c < 4; ++c) mean.v[c] += v.v[c];
+            });
+            sum.one(mean);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) mean.v[c] /= (float)(h_end - h0);
+        }
+        each([&](int i, int h, const Params &p) {
+            const Four v = value(i, h, p);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) s.v[c] = fmaf(v.v[c] - mean.v[c], v.v[c] - mean.v[c], s.v[c]);
+        });
+        sum.one(s);
+        if (grp == 0) {
+            store_four(part + (int64_t)(2 * chunk) * B + col, count, mean);
+            store_four(part + (int64_t)(2 * chunk + 1) * B + col, count, s);
+        }
+    };
+    auto leave_sums = [&](Four &s1, Four &s2, float *part) {
+        sum.two(s1, s2);
+        if (grp == 0) {
+            store_four(part + (int64_t)(2 * chunk) * B + col, count, s1);
+            store_four(part + (int64_t)(2 * chunk + 1) * B + col, count, s2);
+        }
+    };
+    const bool writes = threadIdx.x % LANES == 0;
+    if constexpr (STEP == X_STATS) {
+        leave_statistics([&](int i, int, const Params &) { return wide_of(xv[i]); }, sp.x);
+    } else if constexpr (STEP == MID) {
+        if (x)
+            each([&](int i, int h, const Params &p) { store_four((T *)a.r_out + h * B + col, count, get_r(i, h, p, get_u(i))); });
+        if (a.n_out) leave_statistics([&](int i, int h, const Params &p) { return get_r(i, h, p, get_u(i)); }, sp.r);
+    } else if constexpr (STEP == OUT) {
+        each([&](int i, int h, const Params &p) {
+            Four o = get_r(i, h, p, get_u(i));
+#pragma unroll
+            for (int c = 0; c < 4; ++c) o.v[c] = fmaf((o.v[c] - mean_r.v[c]) * rho_r.v[c], p.weight, p.bias);
+            store_four((T *)a.n_out + h * B + col, count, o);
+        });
+    } else if constexpr (STEP == SUMS) {
+        Four s1 = {}, s2 = {};
+        each([&](int i, int h, const Params &p) {
+            Four v = get_r(i, h, p, get_u(i));
+            const Four n = wide_of(nv[i]);
+            Four nw;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                v.v[c] = (v.v[c] - mean_r.v[c]) * rho_r.v[c];
+                nw.v[c] = n.v[c] * v.v[c];
+                s1.v[c] = fmaf(n.v[c], p.weight, s1.v[c]);
+                s2.v[c] = fmaf(n.v[c] * p.weight, v.v[c], s2.v[c]);
+            }
+            if (d.dweight) {
+                const float q = sum_lanes<LANES>(nw);
+                if (writes) d.dweight[(int64_t)tile * H + h] = q;
+            }
+            if (d.dbias) {
+                const float q = sum_lanes<LANES>(n);
+                if (writes) d.dbias[(int64_t)tile * H + h] = q;
+            }
+        });
+        leave_sums(s1, s2, sp.m);
+    } else {
+        auto get_D = [&](int i, int h, const Params &p, const Four &u) {
+            Four D = wide_of(dv[i]);
+            if (dn) {
+                const Four r = get_r(i, h, p, u);
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    const float v = (r.v[c] - mean_r.v[c]) * rho_r.v[c];
+                    D.v[c] = fmaf(rho_r.v[c], project(a, (float)nv[i].v[c] * p.weight, v, m1.v[c], m2.v[c], rho_r.v[c]), D.v[c]);
+                }
+            }
+            return D;
+        };
+        if constexpr (STEP == RES) {
+            Four k1 = {}, k2 = {};
+            each([&](int i, int h, const Params &p) {
+                const Four u = get_u(i), D = get_D(i, h, p, u);
+                if (d.dresidual) store_four((T *)d.dresidual + h * B + col, count, D);
+                if (!x) return;
+                Four q, s;
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    q.v[c] = factor(p, c, h) * D.v[c];
+                    s.v[c] = (one_gate ? D.v[c] : q.v[c]) * u.v[c];
+                    if (post) {
+                        q.v[c] *= p.post;
+                        k1.v[c] += q.v[c];
+                        k2.v[c] = fmaf(q.v[c], u.v[c], k2.v[c]);
+                    }
+                }
+                if (d.dgate || d.dpost_weight) {
+                    const float S = sum_lanes<LANES>(s);
+                    if (writes && d.dgate) d.dgate[(int64_t)tile * H + h] = a.alpha * p.post * S;
+                    if (writes && d.dpost_weight) d.dpost_weight[(int64_t)tile * H + h] = one_gate ? p.gate * S : S;
+                }
+                if (!post && d.dx) store_four((T *)d.dx + h * B + col, count, q);
+            });
+            if (x && post && d.dx) leave_sums(k1, k2, sp.k);
+        } else {
+            // (x has a norm and its gradient is wanted)
+            __syncthreads();
+            if (threadIdx.x < STEP_COLS && col0 + threadIdx.x < B) {
+                float s1 = 0.f, s2 = 0.f;
+                for (int k = 0; k < sp.chunks; ++k) {
+                    s1 += sp.k[(int64_t)(2 * k) * B + col0 + threadIdx.x];
+                    s2 += sp.k[(int64_t)(2 * k + 1) * B + col0 + threadIdx.x];
+                }
+                known[4][threadIdx.x] = a.layer ? s1 * inv : 0.f;
+                known[5][threadIdx.x] = s2 * inv;
+            }
+            __syncthreads();
+            each([&](int i, int h, const Params &p) {
+                const Four u = get_u(i);
+                Four q = get_D(i, h, p, u);
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    const float k1 = c < count ? known[4][lane4 + c] : 0.f, k2 = c < count ? known[5][lane4 + c] : 0.f;
+                    q.v[c] = rho_x.v[c] * project(a, q.v[c] * factor(p, c, h) * p.post, u.v[c], k1, k2, rho_x.v[c]);
+                }
+                store_four((T *)d.dx + h * B + col, count, q);
+            });
+        }
+    }
+}
+
 // Gradients of gates that belong to groups of columns: a wave sums a feature over a group, from the stored dr.
 template <typename T>
 __global__ __launch_bounds__(256) void ks_norm_cols_gate_kernel(NormArgs a, const T *__restrict__ dr, T *__restrict__ dgate, int64_t groups)
@@ -958,8 +1215,40 @@ NormSplit split_rows(int64_t batch, int64_t groups)
 
 int launched() { return hipGetLastError() == hipSuccess ? KSMM_OK : KSMM_ERR_LAUNCH; }
 
-template <typename T> int forward(const NormArgs &a, int bs_last, hipStream_t stream)
+// Batch-size-last in steps where features are many and columns few: tiles of columns alone then leave most of the chip
+// idle.  Forward/backward, us in one launch -> in steps: 1500 x 500 in fp32 23/52 -> 21/33, 8000 x 500 in fp16 227/457 ->
+// 60/92.  Fewer features, or more columns, are served better by the single launch, which reads its operands once: 768 x 500
+// in fp16 12/27 (steps 20/35), 8000 x 2500 in fp32 222/481 (324/512), 2000 x 4000 49/98 (78/124).
+bool in_steps(int64_t batch, int64_t features) { return features > 1024 && batch <= 2048; }
+struct Steps {
+    int tiles, chunks;
+    int64_t part;  // floats of one array of partial sums
+};
+Steps steps_of(int64_t batch, int64_t features)
 {
+    Steps s;
+    s.tiles = (int)((batch + STEP_COLS - 1) / STEP_COLS);
+    s.chunks = (int)((features + CHUNK - 1) / CHUNK);
+    s.part = 2 * (int64_t)s.chunks * batch;
+    return s;
+}
+template <typename T, int STEP> void run_step(const NormArgs &a, const NormGrads &d, const StepSpace &sp, hipStream_t stream)
+{
+    const int64_t blocks = (int64_t)sp.tiles * sp.chunks;
+    hipLaunchKernelGGL((ks_norm_step_kernel<T, STEP>), dim3((unsigned)((blocks + 7) / 8 * 8)), dim3(COL_THREADS), 0, stream, a, d, sp);
+}
+
+template <typename T> int forward(const NormArgs &a, int bs_last, float *ws, hipStream_t stream)
+{
+    if (bs_last && in_steps(a.batch, a.features)) {
+        const Steps st = steps_of(a.batch, a.features);
+        const StepSpace sp{ws, ws + st.part, nullptr, nullptr, st.tiles, st.chunks};
+        const NormGrads none{};
+        if (a.x && a.post_weight) run_step<T, X_STATS>(a, none, sp, stream);
+        run_step<T, MID>(a, none, sp, stream);
+        if (a.n_out) run_step<T, OUT>(a, none, sp, stream);
+        return launched();
+    }
     if (bs_last)
         return with_cols<T>(a.batch, a.features, [&](auto lanes, auto fpt, auto one) {
             constexpr int LANES = decltype(lanes)::value;
@@ -979,8 +1268,16 @@ template <typename T> int forward(const NormArgs &a, int bs_last, hipStream_t st
     });
 }
 
-template <typename T> int backward(const NormArgs &a, const NormGrads &partial, const NormSplit &sp, int bs_last, hipStream_t stream)
+template <typename T> int backward(const NormArgs &a, const NormGrads &partial, const NormSplit &sp, int bs_last, float *ws, hipStream_t stream)
 {
+    if (bs_last && in_steps(a.batch, a.features)) {
+        const Steps st = steps_of(a.batch, a.features);
+        const StepSpace space{nullptr, nullptr, ws, ws + st.part, st.tiles, st.chunks};
+        if (partial.dn_out) run_step<T, SUMS>(a, partial, space, stream);
+        if (partial.dresidual || a.x) run_step<T, RES>(a, partial, space, stream);
+        if (a.x && a.post_weight && partial.dx) run_step<T, DX>(a, partial, space, stream);
+        return launched();
+    }
     if (bs_last)
         return with_cols<T>(a.batch, a.features, [&](auto lanes, auto fpt, auto one) {
             constexpr int LANES = decltype(lanes)::value;
@@ -1010,18 +1307,20 @@ int64_t align256(int64_t v) { return (v + 255) / 256 * 256; }
 
 // where the partial sums of each quantity lie
 struct Layout {
-    int64_t slices, slice_bytes, gate_bytes, total;
+    int64_t slices, slice_bytes, gate_bytes, steps, total;
     NormSplit split;
 };
 Layout layout(int64_t batch, int64_t features, int64_t groups, int bs_last)
 {
     Layout l;
     l.split = split_rows(batch, groups);
-    const int cols = 4 * col_lanes(batch);
+    const bool steps = bs_last && in_steps(batch, features);
+    const int cols = steps ? STEP_COLS : 4 * col_lanes(batch);
     l.slices = bs_last ? (batch + cols - 1) / cols : l.split.ranges;
     l.slice_bytes = align256(4 * l.slices * features);
     l.gate_bytes = l.split.one_gate ? l.slice_bytes : bs_last ? 0 : align256(4 * l.split.parts * l.split.groups * features);
-    l.total = 3 * l.slice_bytes + l.gate_bytes;
+    l.steps = 3 * l.slice_bytes + l.gate_bytes;
+    l.total = l.steps + (steps ? 8 * steps_of(batch, features).part : 0);
     return l;
 }
 
@@ -1063,17 +1362,26 @@ using namespace ksmm;
 
 extern "C" {
 
-int ksmm_residual_norm_forward(const ksmm_norm_desc *desc, void *r_out, void *n_out, float *stats, int64_t batch, int64_t features,
-                               int dtype, int bs_last, void *stream)
+int64_t ksmm_residual_norm_forward_workspace(int64_t batch, int64_t features, int dtype, int bs_last)
+{
+    if (batch < 1 || features < 1) return KSMM_ERR_BAD_BATCH;
+    if (dtype != KSMM_F32 && dtype != KSMM_F16) return KSMM_ERR_BAD_DTYPE;
+    return bs_last && in_steps(batch, features) ? 8 * steps_of(batch, features).part : 0;
+}
+
+int ksmm_residual_norm_forward(const ksmm_norm_desc *desc, void *r_out, void *n_out, float *stats, void *workspace, int64_t workspace_bytes,
+                               int64_t batch, int64_t features, int dtype, int bs_last, void *stream)
 {
     const int rc = check(desc, batch, features, dtype, bs_last);
     if (rc != KSMM_OK) return rc;
     if ((desc->x && !r_out) || (!desc->x && !n_out)) return KSMM_ERR_NULL_POINTER;
+    const int64_t need = ksmm_residual_norm_forward_workspace(batch, features, dtype, bs_last);
+    if (need > 0 && (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15) != 0)) return KSMM_ERR_WORKSPACE;
     NormArgs a = args_of(desc, batch, features);
     a.r_out = desc->x ? r_out : nullptr;
     a.n_out = n_out;
     a.stats = stats;
-    return dtype == KSMM_F32 ? forward<float>(a, bs_last, (hipStream_t)stream) : forward<half_t>(a, bs_last, (hipStream_t)stream);
+    return dtype == KSMM_F32 ? forward<float>(a, bs_last, (float *)workspace, (hipStream_t)stream) : forward<half_t>(a, bs_last, (float *)workspace, (hipStream_t)stream);
 }
 
 int64_t ksmm_residual_norm_backward_workspace(int64_t batch, int64_t features, int64_t groups, int dtype, int bs_last)
@@ -1097,6 +1405,7 @@ int ksmm_residual_norm_backward(const ksmm_norm_desc *desc, const float *stats, 
     if (!workspace || workspace_bytes < l.total || ((uintptr_t)workspace & 15) != 0) return KSMM_ERR_WORKSPACE;
     const bool gate_alone = dgate && bs_last && !l.split.one_gate;
     if (gate_alone && !dresidual) return KSMM_ERR_NULL_POINTER;  // its sums read it
+    if (gate_alone && l.split.groups * features > 0x7fffffffLL) return KSMM_ERR_TOO_LARGE;
     const hipStream_t s = (hipStream_t)stream;
     NormArgs a = args_of(desc, batch, features);
     a.stats = (float *)stats;
@@ -1110,7 +1419,7 @@ int ksmm_residual_norm_backward(const ksmm_norm_desc *desc, const float *stats, 
     p.dbias = dbias && dn_out ? (float *)(ws + l.slice_bytes) : nullptr;
     p.dpost_weight = dpost_weight ? (float *)(ws + 2 * l.slice_bytes) : nullptr;
     p.dgate = dgate && !gate_alone ? (float *)(ws + 3 * l.slice_bytes) : nullptr;
-    int st = dtype == KSMM_F32 ? backward<float>(a, p, l.split, bs_last, s) : backward<half_t>(a, p, l.split, bs_last, s);
+    int st = dtype == KSMM_F32 ? backward<float>(a, p, l.split, bs_last, (float *)(ws + l.steps), s) : backward<half_t>(a, p, l.split, bs_last, (float *)(ws + l.steps), s);
     if (st != KSMM_OK) return st;
     if (gate_alone) {
         const unsigned blocks = (unsigned)((l.split.groups * features + 3) / 4);

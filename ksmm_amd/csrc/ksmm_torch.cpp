@@ -487,8 +487,14 @@ PyObject *py_residual_norm(PyObject *, PyObject *const *args, Py_ssize_t n_args)
                 if (need_norm) n = at::empty_like(res);
                 if (gradients) stats = at::empty({4, how.batch}, res.options().dtype(at::kFloat));
                 const ksmm_norm_desc d = norm_desc(in, how);
-                status = ksmm_residual_norm_forward(&d, x.defined() ? out_of(r) : nullptr, out_of(n), gradients ? stats.mutable_data_ptr<float>() : nullptr,
-                                                    how.batch, how.features, code_of(res.scalar_type()), how.bs_last, stream_of(res));
+                const int dt = code_of(res.scalar_type());
+                const int64_t need = ksmm_residual_norm_forward_workspace(how.batch, how.features, dt, how.bs_last);
+                at::Tensor ws;
+                if (need > 0) ws = at::empty({need}, res.options().dtype(at::kByte));
+                status = need < 0 ? (int)need
+                                  : ksmm_residual_norm_forward(&d, x.defined() ? out_of(r) : nullptr, out_of(n),
+                                                               gradients ? stats.mutable_data_ptr<float>() : nullptr, out_of(ws), need, how.batch,
+                                                               how.features, dt, how.bs_last, stream_of(res));
             }
             if (status == KSMM_OK) {
                 if (gradients) {

@@ -38,10 +38,10 @@ def test_norm_codes(lib, change, status):
     how = dict(batch=4, features=16, groups=1, dtype=0, kind=0, residual=64)
     how.update(change)
     desc = KsmmNormDesc(None, how["residual"], None, None, None, None, how["groups"], 1.0, 1e-6, how["kind"])
-    assert lib.ksmm_residual_norm_forward(ctypes.byref(desc), None, None, None, how["batch"], how["features"], how["dtype"], 0, None) == status
+    assert lib.ksmm_residual_norm_forward(ctypes.byref(desc), None, None, None, None, 0, how["batch"], how["features"], how["dtype"], 0, None) == status
     assert lib.ksmm_residual_norm_backward(ctypes.byref(desc), None, None, None, None, None, None, None, None, None, None, 0, how["batch"],
                                            how["features"], how["dtype"], 0, None) == status
-    assert lib.ksmm_residual_norm_forward(None, None, None, None, 1, 1, 0, 0, None) == -1
+    assert lib.ksmm_residual_norm_forward(None, None, None, None, None, 0, 1, 1, 0, 0, None) == -1
 
 
 def test_norm_backward_refuses_gradients_of_what_is_not_there(lib):
@@ -104,3 +104,13 @@ def test_muon_takes_the_factors_of_kernel_layers():
     assert {id(p) for p in KSMuon.others(model)} == {id(p) for p in model.parameters()} - {id(model.gated.factor)}
     with pytest.raises(RuntimeError):
         model.gated(torch.randn(3, 8).half())
+
+
+def test_norms_in_steps_need_a_workspace(lib):
+    from ksmm_amd._lib import KsmmNormDesc
+
+    assert lib.ksmm_residual_norm_forward_workspace(25088, 768, 1, 0) == 0 and lib.ksmm_residual_norm_forward_workspace(500, 384, 0, 1) == 0
+    need = lib.ksmm_residual_norm_forward_workspace(500, 8000, 1, 1)
+    assert need >= 500 * 8000 // 256 * 16
+    desc, p = KsmmNormDesc(64, 64, None, None, None, None, 1, 1.0, 1e-6, 0), ctypes.c_void_p(64)
+    assert lib.ksmm_residual_norm_forward(ctypes.byref(desc), p, p, None, p, need - 1, 500, 8000, 1, 1, None) == -9

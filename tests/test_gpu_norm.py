@@ -314,4 +314,24 @@ def test_through_ctypes_gives_the_same(monkeypatch):
     monkeypatch.setattr(_lib, "_native", _lib._NoNative)
     python = all_of()
     assert "ResidualNormFunction" in python[1].grad_fn.name()
-    assert all(torch.equal(a, b) for a, b in zip(native, python))
+    # (gradients of 96 x 96 weights of size one overflow now and then: NaN in both)
+    assert all(torch.allclose(a, b, rtol=0, atol=0, equal_nan=True) for a, b in zip(native, python))
+
+
+@pytest.mark.parametrize("prec", ["fp32", "fp16"])
+@pytest.mark.parametrize("features,batch,groups,post", [(1025, 130, 1, True), (1300, 66, 6, True), (1300, 66, 66, False), (2049, 2048, 1, False),
+                                                        (1300, 2100, 1, True), (1300, 2100, 4, False)])
+def test_many_features_of_few_and_of_many_columns(features, batch, groups, post, prec):
+    t, dr, dn = tensors(features, batch, DT[prec], True, groups, post=post)
+    check(prec, True, t, dr, dn, norm="layer" if post else "rms")
+
+
+@pytest.mark.parametrize("grads", ["n", "r"])
+def test_many_features_one_gradient(grads):
+    t, dr, dn = tensors(1200, 70, torch.float32, True)
+    check("fp32", True, t, dr, dn, norm="layer", grads=grads)
+
+
+def test_many_features_without_a_branch():
+    t, dr, dn = tensors(1200, 70, torch.float32, True, x=False)
+    check("fp32", True, t, dr, dn)
