@@ -489,7 +489,7 @@ template <bool LAST, int D, int TB, int MODE> struct Ring {
     static constexpr int O_CPR = LAST ? 8 : TB / WB * D * 2 / 16;      // chunks a row of them
     static constexpr int O_IT = 32 * O_CPR / 64, PIECE = 32 * O_CPR * 16;
     static constexpr int LDS_BYTES = ST * STAGE + 4 * PIECE;
-    static constexpr int STORES = UNITS * O_IT * (MODE + 1), BIASES = LAST ? 2 * BT : D * BT, EARLY = BIASES + (MODE ? UNITS * O_IT : 0);
+    static constexpr int STORES = UNITS * O_IT * (MODE + 1), BIASES = LAST ? 2 * BT : D * BT, EARLY = BIASES + (MODE ? O_IT : 0);
     static constexpr int WAIT = (ST - 2) * L;
     static_assert(W_BYTES % (16 * THREADS) == 0 && X_BYTES % (16 * THREADS) == 0 && (!LAST || D == 1) && D <= 2, "loads");
     static_assert(TB == 64 || TB == 128, "weight swizzle");
@@ -660,17 +660,15 @@ __global__ __launch_bounds__(256, 2) void ks_gated_ring_kernel(GatedArgs g, int 
         *k = (int64_t)min(n, B - 1) * out_size * parts + ((int64_t)(p.grp * parts + part) * b + min(bi, b - 8 / D)) * D;
         return n < B && bi < b;
     };
-    uint4_t dhv[MODE ? C::UNITS : 1][C::O_IT];
-    auto load_dh = [&](int t) {
-        const At p = at(t);
+    // dh of one unit: the first one's loads go out early, the next one's when its predecessor is in LDS
+    uint4_t dhv[C::O_IT];
+    auto load_dh = [&](const At &p, int u) {
 #pragma unroll
-        for (int u = 0; u < C::UNITS; ++u)
-#pragma unroll
-            for (int i = 0; i < C::O_IT; ++i) {
-                int64_t k;
-                place(p, u, i * O_STEP + o_row, 1, 0, &k);
-                dhv[MODE ? u : 0][i] = *(const uint4_t *)(dh + k);
-            }
+        for (int i = 0; i < C::O_IT; ++i) {
+            int64_t k;
+            place(p, u, i * O_STEP + o_row, 1, 0, &k);
+            dhv[i] = *(const uint4_t *)(dh + k);
+        }
     };
     auto wave_sync = [&]() {
         asm volatile("" ::: "memory");
@@ -690,8 +688,9 @@ __global__ __launch_bounds__(256, 2) void ks_gated_ring_kernel(GatedArgs g, int 
 #pragma unroll
                     for (int i = 0; i < C::O_IT; ++i) {
                         const int row = i * O_STEP + o_row;
-                        *(uint4_t *)(piece + row * (C::O_CPR * 16) + o_swizzle<C::O_CPR>(row, o_cc) * 16) = dhv[u][i];
+                        *(uint4_t *)(piece + row * (C::O_CPR * 16) + o_swizzle<C::O_CPR>(row, o_cc) * 16) = dhv[i];
                     }
+                    if (u + 1 < C::UNITS) load_dh(p, u + 1);
                     wave_sync();
                 }
                 // the lane's values of the unit: chunks of 8
@@ -782,7 +781,7 @@ __global__ __launch_bounds__(256, 2) void ks_gated_ring_kernel(GatedArgs g, int 
             issue();
             if (s == steps - C::ST + 1) {
                 load_bias(t + stride < last ? t + stride : t);
-                if constexpr (MODE == 1) load_dh(t);
+                if constexpr (MODE == 1) load_dh(at(t), 0);
             }
             const uint32_t base = read * C::STAGE;
             read = read + 1 == C::ST ? 0 : read + 1;
