@@ -114,3 +114,12 @@ def test_norms_in_steps_need_a_workspace(lib):
     assert need >= 500 * 8000 // 256 * 16
     desc, p = KsmmNormDesc(64, 64, None, None, None, None, 1, 1.0, 1e-6, 0), ctypes.c_void_p(64)
     assert lib.ksmm_residual_norm_forward(ctypes.byref(desc), p, p, None, p, need - 1, 500, 8000, 1, 1, None) == -9
+
+
+def test_train_block_refuses_nothing_to_do():
+    from ksmm_amd import train_block
+
+    assert train_block.pattern("1,2,3,4") == (1, 2, 3, 4)
+    for bad in (["--steps", "0"], ["--rows", "0"], ["--dtype", "fp8"]):
+        with pytest.raises(SystemExit):
+            train_block.main(bad)
