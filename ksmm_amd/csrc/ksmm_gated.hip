@@ -469,7 +469,8 @@ __global__ __launch_bounds__(64 * WB *WN, 2) void ks_gated_kernel(GatedArgs g, i
 // The sums start at the bias: one product of (bias, 0, ..) and (1, 0, ..).  Results go through 4 KB of LDS a wave, and
 // leave as rows of 128 bytes.
 //
-// (1,768,192,2), 25088 rows: see the table of measurements in the host code below.
+// (1,768,192,2), 25088 rows forward 62 us: 29.6 GFLOP at 480 TFLOP/s; 96 MB of x and h, 1.6 TB/s.  What is left is the vector
+// ALU's work on the results, which the other workgroup's products cover in part.
 constexpr int vmcnt_imm(int n) { return (n & 15) | (7 << 4) | (15 << 8) | (((n >> 4) & 3) << 14); }
 typedef __attribute__((address_space(3))) unsigned char *lds_bytes_t;
 
@@ -947,13 +948,33 @@ bool ring_ok(const GatedArgs &g, bool last)
     return g.d <= 2 && (int64_t)g.a * g.c * g.d * 128 < 1 << 29;
 }
 
+// Few rows or little work: tiles of 64 x 128 would leave most of the chip idle, and their time is that of one tile, whatever
+// the batch.  Workgroups of 16 outputs x 32 rows, forward, us of few rows' kernel / of tiles:
+//   fp32 batch-size-first   (1,768,192,1)  512 rows 13.1/19.1,  768 rows (1152 workgroups) 19.3/19.2
+//   fp32 batch-size-last    (1,768,192,2)  512 rows 14.9/20.8,  768 rows (2304) 20.0/20.9;  (1,768,192,1) 1024 rows (1536) 14.7/20.7
+//   fp16 batch-size-first   (6,64,64,1)    256 rows (192) 4.1/4.8,  384 rows (288) 5.1/4.8;  (1,768,192,2) 192 rows (576) 12.9/9.4
+//   fp16 batch-size-last    (1,768,192,2)  256 rows (768) 6.4/6.9,  512 rows 9.7/6.9;  (6,64,64,1) 1024 rows (768) 4.8/5.4
+// Up to 32 rows weights are read once anyway.  (Tiles need 8 outputs, and batch-size-last 16 rows.)
+template <typename T, bool LAST> bool few(const GatedArgs &g)
+{
+    const int64_t limit = sizeof(T) == 4 ? (LAST ? 2048 : 1152) : (LAST ? 768 : 256);
+    return g.batch <= 32 || g.b < 8 || (int64_t)((g.b + 15) / 16) * g.a * g.d * ((g.batch + 31) / 32) <= limit;
+}
+
+// Everything else: the ring where it can run, and the tile that goes through registers.  fp16 (1,768,192,2), 25088 rows, ring/tile:
+// 62/82 us forward, 242/262 backward (all of it), batch-size-last 54/71 and 232/260; with few tiles they are level
+// ((1,768,192,1) 3136 rows 8.3/8.2).  Weight tiles of the ring: 128 outputs halve the reads of x ((1,768,192,1), 25088 rows
+// 29.6 us for 34.8; batch-size-last (1,768,192,2) 12544 rows, 1176 tiles, 28.4 for 32.3), 64 spread better
+// (6272 rows, 588 tiles, 17.2 for 18.3; (1,768,192,1) 1576 rows 6.9 for 8.9) and waste less of a b of 64 (12.6 for 17.3).
+// Neighbouring d_i in one workgroup share cache lines batch-size-first; fp32 6272 rows, together/one by one: d = 2 99/124 us,
+// 3 25/29, 4 29/40, 8 58/71; fp16 d = 4 16/35, 16 59/120.
 template <typename T, bool LAST, int MODE> int run(const GatedArgs &g, hipStream_t s)
 {
     constexpr int TK = sizeof(T) == 4 ? 16 : 32;
-    if (g.batch <= 128 || g.b < 8) return run_few<T, LAST, MODE>(g, s);
+    if (few<T, LAST>(g)) return run_few<T, LAST, MODE>(g, s);
     if constexpr (sizeof(T) == 2) {
         if (ring_ok(g, LAST)) {
-            const bool wide = g.b % 128 == 0 || g.b > 256;
+            const bool wide = (g.b % 128 == 0 || g.b > 256) && (int64_t)((g.b + 127) / 128) * g.a * g.d * ((g.batch + 127) / 128) >= 768;
             if constexpr (LAST) {
                 return wide ? run_ring<true, 1, 128, MODE>(g, s) : run_ring<true, 1, 64, MODE>(g, s);
             } else {

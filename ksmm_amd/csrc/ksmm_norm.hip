@@ -1181,20 +1181,29 @@ template <typename T, typename F> int with_rows(int64_t features, F f)
     return KSMM_ERR_TOO_LARGE;
 }
 
-// Lanes side by side (four columns each) of a workgroup: 8, or 4 where that would leave CUs without work
-int col_lanes(int64_t batch) { return batch >= 32 * 192 ? 8 : 4; }
-template <typename T, typename F> int with_cols(int64_t batch, int64_t features, F f)
+// features a thread holds: 12 in 16 bits and 6 in 32 are what the backward pass has registers for (with 24 and 12 it
+// spills, and takes twice the time)
+template <typename T> constexpr int MOST = sizeof(T) == 2 ? 12 : 6;
+// Lanes side by side (four columns each) of a workgroup: 8, or 4 where 8 would leave CUs without work (768 x 4000 in fp16
+// forward 17.8 us for 22.5, backward 31 for 48), and where with 4 a thread holds the features that it would
+// not hold, or holds half: backward from 64 * MOST / 2 features on (8 -> 4 lanes, us: 768 x 25088 in fp16 219 -> 162, 384 x 25088 in fp32
+// 102 -> 90, but 192 x 25088 in fp16 46 -> 64), forward in fp32 above 64 * MOST (768 x 25088 112 -> 92, but 384 44 -> 49,
+// in fp16 1500 x 8000 75 -> 80).
+template <typename T> int col_lanes(int64_t batch, int64_t features, bool backward)
 {
-    // features a thread holds: 12 in 16 bits and 6 in 32 are what the backward pass has registers for (with 24 and 12 it
-    // spills, and takes twice the time)
-    constexpr int MOST = sizeof(T) == 2 ? 12 : 6;
-    const int lanes = col_lanes(batch);
+    if (batch < 32 * 192) return 4;
+    const int64_t from = backward ? 32 * MOST<T> : sizeof(T) == 4 ? 64 * MOST<T> : INT64_MAX;
+    return features > from && features <= 128 * MOST<T> ? 4 : 8;
+}
+template <typename T, typename F> int with_cols(int64_t batch, int64_t features, bool backward, F f)
+{
+    const int lanes = col_lanes<T>(batch, features, backward);
     const int64_t groups = COL_THREADS / lanes, per = (features + groups - 1) / groups;
     auto held = [&](auto lanes_of) {
         typedef std::integral_constant<bool, true> one;
-        if (per <= MOST / 2) return f(lanes_of, std::integral_constant<int, MOST / 2>(), one());
-        if (per <= MOST) return f(lanes_of, std::integral_constant<int, MOST>(), one());
-        return f(lanes_of, std::integral_constant<int, MOST / 2>(), std::integral_constant<bool, false>());
+        if (per <= MOST<T> / 2) return f(lanes_of, std::integral_constant<int, MOST<T> / 2>(), one());
+        if (per <= MOST<T>) return f(lanes_of, std::integral_constant<int, MOST<T>>(), one());
+        return f(lanes_of, std::integral_constant<int, MOST<T> / 2>(), std::integral_constant<bool, false>());
     };
     return lanes == 8 ? held(std::integral_constant<int, 8>()) : held(std::integral_constant<int, 4>());
 }
@@ -1250,7 +1259,7 @@ template <typename T> int forward(const NormArgs &a, int bs_last, float *ws, hip
         return launched();
     }
     if (bs_last)
-        return with_cols<T>(a.batch, a.features, [&](auto lanes, auto fpt, auto one) {
+        return with_cols<T>(a.batch, a.features, false, [&](auto lanes, auto fpt, auto one) {
             constexpr int LANES = decltype(lanes)::value;
             const int tiles = (int)((a.batch + 4 * LANES - 1) / (4 * LANES));
             hipLaunchKernelGGL((ks_norm_cols_kernel<T, LANES, decltype(fpt)::value, decltype(one)::value>), dim3((tiles + 7) / 8 * 8),
@@ -1279,7 +1288,7 @@ template <typename T> int backward(const NormArgs &a, const NormGrads &partial, 
         return launched();
     }
     if (bs_last)
-        return with_cols<T>(a.batch, a.features, [&](auto lanes, auto fpt, auto one) {
+        return with_cols<T>(a.batch, a.features, true, [&](auto lanes, auto fpt, auto one) {
             constexpr int LANES = decltype(lanes)::value;
             const int tiles = (int)((a.batch + 4 * LANES - 1) / (4 * LANES));
             hipLaunchKernelGGL((ks_norm_cols_bwd_kernel<T, LANES, decltype(fpt)::value, decltype(one)::value>), dim3((tiles + 7) / 8 * 8),
@@ -1310,12 +1319,12 @@ struct Layout {
     int64_t slices, slice_bytes, gate_bytes, steps, total;
     NormSplit split;
 };
-Layout layout(int64_t batch, int64_t features, int64_t groups, int bs_last)
+Layout layout(int64_t batch, int64_t features, int64_t groups, int dtype, int bs_last)
 {
     Layout l;
     l.split = split_rows(batch, groups);
     const bool steps = bs_last && in_steps(batch, features);
-    const int cols = steps ? STEP_COLS : 4 * col_lanes(batch);
+    const int cols = steps ? STEP_COLS : 4 * (dtype == KSMM_F32 ? col_lanes<float>(batch, features, true) : col_lanes<half_t>(batch, features, true));
     l.slices = bs_last ? (batch + cols - 1) / cols : l.split.ranges;
     l.slice_bytes = align256(4 * l.slices * features);
     l.gate_bytes = l.split.one_gate ? l.slice_bytes : bs_last ? 0 : align256(4 * l.split.parts * l.split.groups * features);
@@ -1388,7 +1397,7 @@ int64_t ksmm_residual_norm_backward_workspace(int64_t batch, int64_t features, i
 {
     if (batch < 1 || features < 1 || groups < 1 || batch % groups) return KSMM_ERR_BAD_BATCH;
     if (dtype != KSMM_F32 && dtype != KSMM_F16) return KSMM_ERR_BAD_DTYPE;
-    return layout(batch, features, groups, bs_last).total;
+    return layout(batch, features, groups, dtype, bs_last).total;
 }
 
 int ksmm_residual_norm_backward(const ksmm_norm_desc *desc, const float *stats, const void *dr_out, const void *dn_out, void *dx,
@@ -1401,7 +1410,7 @@ int ksmm_residual_norm_backward(const ksmm_norm_desc *desc, const float *stats, 
     if ((!desc->x && (dx || dgate || dpost_weight)) || (dgate && !desc->gate) || (dpost_weight && !desc->post_weight) ||
         (dweight && !desc->weight) || (dbias && !desc->bias))
         return KSMM_ERR_NULL_POINTER;
-    const Layout l = layout(batch, features, desc->groups, bs_last);
+    const Layout l = layout(batch, features, desc->groups, dtype, bs_last);
     if (!workspace || workspace_bytes < l.total || ((uintptr_t)workspace & 15) != 0) return KSMM_ERR_WORKSPACE;
     const bool gate_alone = dgate && bs_last && !l.split.one_gate;
     if (gate_alone && !dresidual) return KSMM_ERR_NULL_POINTER;  // its sums read it
