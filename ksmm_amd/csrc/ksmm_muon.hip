@@ -82,7 +82,7 @@ __device__ __forceinline__ void split(float v, half_t &hi, half_t &lo)
 // X and its Gram matrix (which the polynomial replaces) in LDS, hi and lo apart, sides padded to 32 with zeros; tiles of
 // 16 x 16 are dealt to the waves.  G and Q are symmetric: upper tiles only, and both operands of G G are rows.  Few of these
 // matrices fill no chip: what counts is the latency of fifteen products in a row.
-// (6,64,64,1): 28 us on 32-bit instructions; (1,128,128,3): 133.
+// (6,64,64,1) 17.7 us, (1,128,128,3) 70 (on 32-bit instructions 28 and 133).
 __host__ __device__ constexpr int up16(int v) { return (v + 15) / 16 * 16; }
 __host__ __device__ constexpr int up32(int v) { return (v + 31) / 32 * 32; }
 __host__ __device__ constexpr int64_t block_lds(int m, int n)
@@ -553,6 +553,8 @@ __global__ __launch_bounds__(64 * GROUPS, 2) void ks_muon_gemm_kernel(MuonArgs a
 int launched() { return hipGetLastError() == hipSuccess ? KSMM_OK : KSMM_ERR_LAUNCH; }
 constexpr int64_t LDS_MOST = 160 * 1024 - 256;
 
+// In one launch where X fits LDS and the waves' registers: (6,64,64,1) 17.7 us, by launches of products 73.5;
+// (1,192,48,2) of two parts 29 for 80; (1,128,128,3) 70 for 84, 64 such matrices 70 for 104.
 bool fits_lds(int m, int n)
 {
     const int64_t mt = up16(m) / 16, nt = up16(n) / 16;
@@ -626,6 +628,8 @@ template <typename T> int run(const MuonArgs &a, int64_t matrices, char *ws, hip
         if (rc != KSMM_OK) return;
         hipLaunchKernelGGL(fn, dim3((unsigned)((tiles + 7) / 8 * 8)), dim3(64 * groups), lds, s, a, l, r, old, out, turned, w.M, w.N, last, (int)tiles);
     };
+    // waves that share K: 8 for the square products, whose tiles are few, 4 for the others ((1,1536,384,2) of two parts 223 us; 4
+    // everywhere 227, 8 everywhere 241; (1,256,256,16) 115, 112, 116)
     for (int i = 0; i < a.steps; ++i) {
         gemm(&ks_muon_gemm_kernel<T, GRAM, 8>, 8, square, x, x, x, gram, gram, false);
         gemm(&ks_muon_gemm_kernel<T, POLY, 8>, 8, square, gram, gram, gram, poly, poly, false);

@@ -100,6 +100,17 @@ def test_aligned_fp16(pattern, batch, bs_last, bias):
 
 
 @pytest.mark.parametrize("bs_last", [False, True])
+@pytest.mark.parametrize("prec", ["fp32", "fp16"])
+@pytest.mark.parametrize("pattern,batch", [((8, 100, 19, 1), 1201), ((4, 100, 21, 2), 1201), ((3, 99, 20, 3), 1201), ((2, 101, 18, 4), 1201),
+                                           ((2, 100, 17, 5), 1201), ((2, 72, 20, 6), 1201), ((1, 104, 33, 8), 1201), ((8, 9, 10, 8), 1201),
+                                           ((8, 8, 3, 8), 1201), ((2, 104, 64, 4), 1208), ((16, 100, 16, 7), 77), ((24, 200, 64, 4), 40),
+                                           ((24, 200, 65, 4), 33), ((40, 128, 64, 2), 48), ((40, 128, 64, 3), 48), ((40, 100, 40, 2), 47)])
+def test_work_for_tiles(pattern, batch, prec, bs_last):
+    """Enough work for the tiles of every d, at sizes that end inside them; few rows of large factors."""
+    check(pattern, batch, prec, "silu", True, bs_last)
+
+
+@pytest.mark.parametrize("bs_last", [False, True])
 def test_no_rows_and_more_axes(bs_last):
     from ksmm_amd import GatedKernel, KSGatedLinear
 
