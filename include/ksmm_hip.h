@@ -26,8 +26,8 @@
  * remembers which kernels had their LDS limit raised, and ksmm_chain_forward_static owns one
  * fixed device buffer per GPU).  All launches go to the stream the caller passes (a
  * hipStream_t cast to void*; NULL is the legacy default stream).  Every entry point returns
- * KSMM_OK or a negative error code; ksmm_strerror() names it.  Only ksmm_factor_forward*,
- * ksmm_chain_forward* and ksmm_factor_backward* touch the GPU.
+ * KSMM_OK or a negative error code; ksmm_strerror() names it.  Only the entry points that take
+ * a stream touch the GPU.
  */
 #ifndef KSMM_HIP_H
 #define KSMM_HIP_H
@@ -318,8 +318,8 @@ int ksmm_chain_forward_static(const ksmm_factor_desc *factors, int n_factors, co
 
 /* ---- operators around a Kronecker-sparse feed-forward block (fp32 and fp16) -----------------------
  * All of them launch on the caller's stream, allocate nothing, keep nothing, and compute in fp32; results are
- * rounded once.  Every pointer needs the alignment of its elements only; workspaces 16 bytes.  Outputs must not
- * overlap inputs unless said so. */
+ * rounded once.  Every pointer needs the alignment of its elements only; workspaces 16 bytes.  Tensors written
+ * must not overlap those read unless said so (KSMM_ERR_ALIAS). */
 
 /* Gated projection: two factors of one pattern (a, b, c, d) that share their input x,
  *     h = act(G x + bias_g) * (U x + bias_u)
@@ -344,7 +344,7 @@ int ksmm_gated_backward(const void *dh, const void *x, const void *w, const void
  * written.  n_out NULL: not wanted.  NULL gate and weight count as ones, NULL bias as zeros.
  * stats (NULL: not wanted): 4 x batch floats for the backward pass.  Needs
  * ksmm_residual_norm_forward_workspace() bytes of 16-byte aligned device memory (0: none).
- * Batch-size-first rows of up to 8192 features; batch-size-last any number. */
+ * Batch-size-first rows of up to 16384 features; batch-size-last any number. */
 typedef enum ksmm_norm_kind { KSMM_NORM_RMS = 0, KSMM_NORM_LAYER = 1 } ksmm_norm_kind;
 typedef struct ksmm_norm_desc {
     const void *x, *residual, *gate, *post_weight, *weight, *bias;

@@ -445,13 +445,6 @@ int64_t wgrad_partial_bytes(int64_t batch, int a, int b, int c, int d, int dtype
     return align256(wgrad_partial_floats(batch, a, b, c, d, dtype, bs_last) * 4);
 }
 
-bool overlaps(const void *p, int64_t p_bytes, const void *q, int64_t q_bytes)
-{
-    const char *pb = (const char *)p, *qb = (const char *)q;
-    return pb < qb + q_bytes && qb < pb + p_bytes;
-}
-
-
 int check_epilogue(const ksmm_epilogue *ep)
 {
     if (!ep) return KSMM_OK;

@@ -59,6 +59,13 @@ template <> struct elem<fp8_t> {
     __device__ static __forceinline__ float load(const fp8_t *p) { return (float)fp8_to_half(p->bits); }
 };
 
+// (a NULL pointer overlaps nothing)
+static inline bool overlaps(const void *p, int64_t p_bytes, const void *q, int64_t q_bytes)
+{
+    const char *pb = (const char *)p, *qb = (const char *)q;
+    return p && q && pb < qb + q_bytes && qb < pb + p_bytes;
+}
+
 static inline size_t dtype_size(int dt)
 {
     return dt == KSMM_F32 ? 4 : dt == KSMM_F16 ? 2 : 1;

@@ -1038,6 +1038,9 @@ int ksmm_gated_forward(const void *x, const void *w, const void *bias, void *h, 
     const int rc = check(batch, a, b, c, d, dtype, act);
     if (rc != KSMM_OK) return rc;
     if (!x || !w || !h) return KSMM_ERR_NULL_POINTER;
+    const int64_t size = (int64_t)dtype_size(dtype), xs = (int64_t)a * c * d * batch * size, ws = (int64_t)a * c * d * 2 * b * size,
+                  hs = (int64_t)a * b * d * batch * size, bs = 2 * (int64_t)a * b * d * size;
+    if (overlaps(h, hs, x, xs) || overlaps(h, hs, w, ws) || overlaps(h, hs, bias, bs)) return KSMM_ERR_ALIAS;
     return gated_run(x, w, bias, nullptr, h, batch, a, b, c, d, dtype, bs_last, act, 0, (hipStream_t)stream);
 }
 
@@ -1060,6 +1063,18 @@ int ksmm_gated_backward(const void *dh, const void *x, const void *w, const void
     if (need < 0) return (int)need;
     if (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15) != 0) return KSMM_ERR_WORKSPACE;
     if (!dx && !dw && !dbias) return KSMM_OK;
+    {
+        const int64_t size = (int64_t)dtype_size(dtype), xs = (int64_t)a * c * d * batch * size, ws = (int64_t)a * c * d * 2 * b * size,
+                      hs = (int64_t)a * b * d * batch * size, bs = 2 * (int64_t)a * b * d * size;
+        const void *const in[] = {dh, x, w, bias}, *const out[] = {dx, dw, dbias, workspace};
+        const int64_t in_bytes[] = {hs, xs, ws, bs}, out_bytes[] = {xs, ws, bs, need};
+        for (int i = 0; i < 4; ++i) {
+            for (int o = 0; o < 4; ++o)
+                if (overlaps(in[i], in_bytes[i], out[o], out_bytes[o])) return KSMM_ERR_ALIAS;
+            for (int o = 0; o < i; ++o)
+                if (overlaps(out[i], out_bytes[i], out[o], out_bytes[o])) return KSMM_ERR_ALIAS;
+        }
+    }
     rc = gated_run(x, w, bias, dh, workspace, batch, a, b, c, d, dtype, bs_last, act, 1, (hipStream_t)stream);
     if (rc != KSMM_OK) return rc;
     const int64_t dz = align256(2 * (int64_t)a * b * d * batch * (int64_t)dtype_size(dtype));

@@ -1150,13 +1150,15 @@ __global__ __launch_bounds__(256) void ks_norm_cols_gate_kernel(NormArgs a, cons
 // ranges of rows that fill the chip: workgroups of 4 waves, 2 of which fit a CU in the backward pass
 constexpr int64_t FWD_RANGES = 2048, BWD_RANGES = 768;
 // widest batch-size-first row that the kernels hold
-constexpr int64_t WIDEST = 8192;
+constexpr int64_t WIDEST = 16384;
 
 template <int E, int TPR, int VPL> struct Rows {
     static constexpr int e = E, tpr = TPR, vpl = VPL;
 };
 // The kernel that holds a row in the fewest values a thread (8 to 16): fp16 768 features in 12 a lane, 3 pieces of 8 bytes,
-// are 54 us backward with both norms, in 2 pieces of 16 bytes, a third of them empty, 152.
+// are 54 us backward with both norms, in 2 pieces of 16 bytes, a third of them empty, 152.  Rates, forward/backward with both
+// norms, TB/s: 768 x 25088 in fp16 4.2/3.7, 4096 x 8192 5.0/3.5, 8192 x 4096 3.5/3.3.  Above 8192 features a thread's values
+// spill (16384 x 2048 3.7/1.5, in fp32 1.7/0.7): such rows are served, not tuned.
 template <typename T, typename F> int with_rows(int64_t features, F f)
 {
     constexpr int E = 16 / (int)sizeof(T);
@@ -1168,6 +1170,7 @@ template <typename T, typename F> int with_rows(int64_t features, F f)
         if (features <= 2048) return f(Rows<E, 256, 1>());
         if (features <= 4096) return f(Rows<E, 256, 2>());
         if (features <= 8192) return f(Rows<E, 1024, 1>());
+        if (features <= 16384) return f(Rows<E, 1024, 2>());
     } else {
         if (features <= 64) return f(Rows<E, 16, 1>());
         if (features <= 256) return f(Rows<E, 64, 1>());
@@ -1177,6 +1180,7 @@ template <typename T, typename F> int with_rows(int64_t features, F f)
         if (features <= 2048) return f(Rows<E, 256, 2>());
         if (features <= 4096) return f(Rows<E, 1024, 1>());
         if (features <= 8192) return f(Rows<E, 1024, 2>());
+        if (features <= 16384) return f(Rows<E, 1024, 4>());
     }
     return KSMM_ERR_TOO_LARGE;
 }
@@ -1386,6 +1390,10 @@ int ksmm_residual_norm_forward(const ksmm_norm_desc *desc, void *r_out, void *n_
     if ((desc->x && !r_out) || (!desc->x && !n_out)) return KSMM_ERR_NULL_POINTER;
     const int64_t need = ksmm_residual_norm_forward_workspace(batch, features, dtype, bs_last);
     if (need > 0 && (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15) != 0)) return KSMM_ERR_WORKSPACE;
+    const int64_t size = batch * features * (int64_t)dtype_size(dtype);
+    if (desc->x && (overlaps(r_out, size, desc->x, size) || overlaps(r_out, size, desc->residual, size) || overlaps(r_out, size, n_out, size)))
+        return KSMM_ERR_ALIAS;
+    if (overlaps(n_out, size, desc->x, size) || overlaps(n_out, size, desc->residual, size)) return KSMM_ERR_ALIAS;
     NormArgs a = args_of(desc, batch, features);
     a.r_out = desc->x ? r_out : nullptr;
     a.n_out = n_out;
@@ -1415,6 +1423,11 @@ int ksmm_residual_norm_backward(const ksmm_norm_desc *desc, const float *stats, 
     const bool gate_alone = dgate && bs_last && !l.split.one_gate;
     if (gate_alone && !dresidual) return KSMM_ERR_NULL_POINTER;  // its sums read it
     if (gate_alone && l.split.groups * features > 0x7fffffffLL) return KSMM_ERR_TOO_LARGE;
+    const int64_t size = batch * features * (int64_t)dtype_size(dtype);
+    const void *const in[] = {desc->x, desc->residual, dr_out, dn_out};
+    for (const void *p : in)
+        if (overlaps(dx, size, p, size) || overlaps(dresidual, size, p, size)) return KSMM_ERR_ALIAS;
+    if (overlaps(dx, size, dresidual, size)) return KSMM_ERR_ALIAS;
     const hipStream_t s = (hipStream_t)stream;
     NormArgs a = args_of(desc, batch, features);
     a.stats = (float *)stats;

@@ -31,7 +31,7 @@ def test_gated_backward_refuses_a_small_workspace(lib):
 
 @pytest.mark.parametrize("change,status", [
     ({}, -1), ({"batch": 0}, -3), ({"features": 0}, -3), ({"groups": 3}, -3), ({"groups": 0}, -3), ({"dtype": 2}, -4), ({"kind": 5}, -12),
-    ({"residual": None}, -1), ({"features": 8193}, -5)])
+    ({"residual": None}, -1), ({"features": 16385}, -5)])
 def test_norm_codes(lib, change, status):
     from ksmm_amd._lib import KsmmNormDesc
 
@@ -123,3 +123,24 @@ def test_train_block_refuses_nothing_to_do():
     for bad in (["--steps", "0"], ["--rows", "0"], ["--dtype", "fp8"]):
         with pytest.raises(SystemExit):
             train_block.main(bad)
+
+
+def test_outputs_that_lie_in_inputs_are_refused(lib):
+    from ksmm_amd._lib import KsmmNormDesc
+
+    f = lib.ksmm_gated_forward  # 4 rows of 8 features -> 8 in fp32: 128 bytes each, 512 of weights
+    assert f(4096, 8192, None, 4096 + 64, 4, 1, 8, 8, 1, 0, 0, 2, None) == -11
+    assert f(4096, 8192, None, 8192 + 500, 4, 1, 8, 8, 1, 0, 0, 2, None) == -11
+    assert f(4096, 8192, 16384, 16384 + 60, 4, 1, 8, 8, 1, 0, 0, 2, None) == -11
+    need = lib.ksmm_gated_backward_workspace(4, 1, 8, 8, 1, 0, 0)
+    g = lib.ksmm_gated_backward
+    assert g(1 << 20, 1 << 21, 1 << 22, None, 1 << 23, (1 << 23) + 64, None, 1 << 24, need, 4, 1, 8, 8, 1, 0, 0, 2, None) == -11
+    assert g(1 << 20, 1 << 21, 1 << 22, None, 1 << 23, None, None, (1 << 20) - 16, need, 4, 1, 8, 8, 1, 0, 0, 2, None) == -11
+    desc = KsmmNormDesc(1 << 20, 1 << 21, None, None, None, None, 1, 1.0, 1e-6, 0)
+    n = lib.ksmm_residual_norm_forward
+    for r, out in ((1 << 20, 1 << 22), ((1 << 21) + 60, 1 << 22), (1 << 22, 1 << 22), (1 << 22, 1 << 21)):
+        assert n(ctypes.byref(desc), r, out, None, None, 0, 4, 8, 0, 0, None) == -11
+    need = lib.ksmm_residual_norm_backward_workspace(4, 8, 1, 0, 0)
+    for dx, dr in ((1 << 20, 1 << 23), (1 << 23, 1 << 22), (1 << 23, (1 << 23) + 4)):
+        assert lib.ksmm_residual_norm_backward(ctypes.byref(desc), 1 << 19, 1 << 22, None, dx, dr, None, None, None, None, 1 << 24, need, 4, 8, 0, 0,
+                                               None) == -11

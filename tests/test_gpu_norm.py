@@ -265,7 +265,7 @@ def test_refusals():
         (ValueError, lambda: residual_norm(x, r, norm="batch")),
         (ValueError, lambda: residual_norm(None, r, need_norm=False)),
         (AssertionError, lambda: residual_norm(None, r.bfloat16())),
-        (RuntimeError, lambda: residual_norm(None, torch.ones(2, 9000, device="cuda"))),
+        (RuntimeError, lambda: residual_norm(None, torch.ones(2, 17000, device="cuda"))),
         (ValueError, lambda: ResidualNorm(32, "batch")),
         (ValueError, lambda: KSFeedForward((1, 64, 32, 1), [(1, 32, 32, 1)])),
     ]:
@@ -335,3 +335,10 @@ def test_many_features_one_gradient(grads):
 def test_many_features_without_a_branch():
     t, dr, dn = tensors(1200, 70, torch.float32, True, x=False)
     check("fp32", True, t, dr, dn)
+
+
+@pytest.mark.parametrize("prec", ["fp32", "fp16"])
+@pytest.mark.parametrize("features", [8193, 12000, 16384])
+def test_widest_rows(features, prec):
+    t, dr, dn = tensors(features, 13, DT[prec], False)
+    check(prec, False, t, dr, dn, norm="layer")
