@@ -983,11 +983,23 @@ template <typename T, bool LAST, int MODE> int run(const GatedArgs &g, hipStream
             }
         }
     }
+    // fp32, whose matrix instructions leave time to feed smaller tiles: 64 x 64 while those of 128 rows are fewer than two a place
+    // ((4,192,192,1) batch-size-last 6501 rows, 612 tiles, 46.5 us for 52.4; (1,768,192,2) 6272 rows 84 for 93, 25088 rows, 2352
+    // tiles, 299 for 291); beyond, 8 waves a tile (284 for 291, batch-size-last 260 for 264; not d = 1, 142 for 139)
+    constexpr int WN = sizeof(T) == 4 ? 4 : 2;
+    if constexpr (sizeof(T) == 4) {
+        if ((LAST || g.d <= 2) && (int64_t)((g.b + 63) / 64) * g.a * (LAST ? g.d : 1) * ((g.batch + 127) / 128) < 1024) {
+            if constexpr (LAST)
+                return run_tile<T, true, 1, false, 64, 64, TK, 2, 2, MODE>(g, s);
+            else
+                return g.d == 1 ? run_tile<T, false, 1, true, 64, 64, TK, 2, 2, MODE>(g, s) : run_tile<T, false, 2, true, 64, 64, TK, 2, 2, MODE>(g, s);
+        }
+    }
     if constexpr (LAST) {
-        return run_tile<T, true, 1, false, 64, 128, TK, 2, 2, MODE>(g, s);
+        return run_tile<T, true, 1, false, 64, 128, TK, 2, WN, MODE>(g, s);
     } else {
         if (g.d == 1) return run_tile<T, false, 1, true, 64, 128, TK, 2, 2, MODE>(g, s);
-        if (g.d == 2) return run_tile<T, false, 2, true, 64, 128, TK, 2, 2, MODE>(g, s);
+        if (g.d == 2) return run_tile<T, false, 2, true, 64, 128, TK, 2, WN, MODE>(g, s);
         if (g.d == 3) return run_tile<T, false, 3, true, 32, 128, TK, 2, 2, MODE>(g, s);
         if (g.d == 4) return run_tile<T, false, 4, true, 32, 64, TK, 2, 2, MODE>(g, s);
         if (g.d % 4 == 0) return run_tile<T, false, 4, false, 32, 64, TK, 2, 2, MODE>(g, s);

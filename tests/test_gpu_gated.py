@@ -110,6 +110,11 @@ def test_work_for_tiles(pattern, batch, prec, bs_last):
     check(pattern, batch, prec, "silu", True, bs_last)
 
 
+@pytest.mark.parametrize("pattern,batch,bs_last", [((40, 65, 6, 5), 300, True), ((60, 65, 6, 2), 1201, False), ((110, 65, 5, 1), 1201, False)])
+def test_many_tiles_fp32(pattern, batch, bs_last):
+    check(pattern, batch, "fp32", "gelu", True, bs_last)
+
+
 @pytest.mark.parametrize("bs_last", [False, True])
 def test_no_rows_and_more_axes(bs_last):
     from ksmm_amd import GatedKernel, KSGatedLinear
