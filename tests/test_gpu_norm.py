@@ -342,3 +342,24 @@ def test_many_features_without_a_branch():
 def test_widest_rows(features, prec):
     t, dr, dn = tensors(features, 13, DT[prec], False)
     check(prec, False, t, dr, dn, norm="layer")
+
+
+@pytest.mark.parametrize("bs_last", [False, True])
+def test_offsets_beyond_31_bits(bs_last):
+    """The last rows of 2.2e9 values are those of a call on them alone."""
+    from ksmm_amd import residual_norm
+
+    features, batch, last = 1100, 2_000_001, 8195
+    shape = (features, batch) if bs_last else (batch, features)
+    x, r, dn = (torch.empty(shape, dtype=torch.float16, device="cuda").normal_() for _ in range(3))
+    w = torch.ones(features, dtype=torch.float16, device="cuda")
+    tail = [(t[:, -last:] if bs_last else t[-last:]).contiguous() for t in (x, r, dn)]
+
+    def results(x, r, dn):
+        x, r = x.requires_grad_(), r.requires_grad_()
+        with torch.enable_grad():
+            out = residual_norm(x, r, None, w, w, None, 0.5, bs_last=bs_last)
+            return [t.detach() for t in out] + list(torch.autograd.grad(out[1], (x, r), dn))
+
+    for a, b in zip(results(x, r, dn), results(*tail)):
+        assert torch.equal(a[:, -last:] if bs_last else a[-last:], b)
