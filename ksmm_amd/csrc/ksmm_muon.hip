@@ -477,23 +477,31 @@ __global__ __launch_bounds__(64 * GROUPS, 2) void ks_muon_gemm_kernel(MuonArgs a
             o.yl[q] = *(const half8_t *)(rl + at + q * half);
         }
     };
+    auto multiply = [&](const Operands &o) __attribute__((always_inline)) {
+#pragma unroll
+        for (int p = 0; p < 4; ++p) {
+            main[p >> 1][p & 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(o.xh[p >> 1], o.yh[p & 1], main[p >> 1][p & 1], 0, 0, 0);
+            cross[p >> 1][p & 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(o.xh[p >> 1], o.yl[p & 1], cross[p >> 1][p & 1], 0, 0, 0);
+            cross[p >> 1][p & 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(o.xl[p >> 1], o.yh[p & 1], cross[p >> 1][p & 1], 0, 0, 0);
+        }
+    };
+    // loads run two steps ahead: the compiler must neither move them behind the products nor sink them to their use
     Operands ring[3];
     load(ring[0], wave);
     load(ring[1], wave + GROUPS);
-    for (int s = wave; s < steps; s += 3 * GROUPS) {
+    int s = wave;
+    for (; s + 2 * GROUPS < steps; s += 3 * GROUPS) {
 #pragma unroll
         for (int q = 0; q < 3; ++q) {
-            if (s + q * GROUPS >= steps) break;
             load(ring[(q + 2) % 3], s + (q + 2) * GROUPS);
-            const Operands &o = ring[q];
-#pragma unroll
-            for (int p = 0; p < 4; ++p) {
-                main[p >> 1][p & 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(o.xh[p >> 1], o.yh[p & 1], main[p >> 1][p & 1], 0, 0, 0);
-                cross[p >> 1][p & 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(o.xh[p >> 1], o.yl[p & 1], cross[p >> 1][p & 1], 0, 0, 0);
-                cross[p >> 1][p & 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(o.xl[p >> 1], o.yh[p & 1], cross[p >> 1][p & 1], 0, 0, 0);
-            }
+            asm volatile("" ::: "memory");
+            __builtin_amdgcn_sched_barrier(0);
+            multiply(ring[q]);
+            __builtin_amdgcn_sched_barrier(0);
         }
     }
+    if (s < steps) multiply(ring[0]);
+    if (s + GROUPS < steps) multiply(ring[1]);
 #pragma unroll
     for (int q = 0; q < 4; ++q)
 #pragma unroll
@@ -553,7 +561,7 @@ __global__ __launch_bounds__(64 * GROUPS, 2) void ks_muon_gemm_kernel(MuonArgs a
 int launched() { return hipGetLastError() == hipSuccess ? KSMM_OK : KSMM_ERR_LAUNCH; }
 constexpr int64_t LDS_MOST = 160 * 1024 - 256;
 
-// In one launch where X fits LDS and the waves' registers: (6,64,64,1) 17.7 us, by launches of products 73.5;
+// In one launch where X fits LDS and the waves' registers: (6,64,64,1) 17.7 us, by launches of products 73;
 // (1,192,48,2) of two parts 29 for 80; (1,128,128,3) 70 for 84, 64 such matrices 70 for 104.
 bool fits_lds(int m, int n)
 {
@@ -628,8 +636,8 @@ template <typename T> int run(const MuonArgs &a, int64_t matrices, char *ws, hip
         if (rc != KSMM_OK) return;
         hipLaunchKernelGGL(fn, dim3((unsigned)((tiles + 7) / 8 * 8)), dim3(64 * groups), lds, s, a, l, r, old, out, turned, w.M, w.N, last, (int)tiles);
     };
-    // waves that share K: 8 for the square products, whose tiles are few, 4 for the others ((1,1536,384,2) of two parts 223 us; 4
-    // everywhere 227, 8 everywhere 241; (1,256,256,16) 115, 112, 116)
+    // waves that share K: 8 for the square products, whose tiles are few, 4 for the others ((1,1536,384,2) of two parts 203 us; before
+    // loads were kept ahead 223, 4 everywhere 227, 8 everywhere 241; (1,256,256,16) 108; 115, 112, 116)
     for (int i = 0; i < a.steps; ++i) {
         gemm(&ks_muon_gemm_kernel<T, GRAM, 8>, 8, square, x, x, x, gram, gram, false);
         gemm(&ks_muon_gemm_kernel<T, POLY, 8>, 8, square, gram, gram, gram, poly, poly, false);
