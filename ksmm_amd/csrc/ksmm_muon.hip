@@ -451,13 +451,6 @@ __global__ __launch_bounds__(64 * GROUPS, 2) void ks_muon_gemm_kernel(MuonArgs a
     const int quarter = wave * MINE / 4, group = wave % (4 / MINE);
     const int i0 = ti * TILE + (quarter >> 1) * 32, j0 = tj * TILE + (quarter & 1) * 32;
     f4 old[MINE];
-    if (WHAT != GRAM) {
-#pragma unroll
-        for (int k = 0; k < MINE; ++k) {
-            const int r = 8 * (group * MINE + k) + 4 * lq;
-            old[k] = x.get(WHAT == POLY ? id * M * M + operand_at(j0 + l32, i0 + r, M) : id * M * N + operand_at(j0 + l32, i0 + r, N));
-        }
-    }
     float16_t main[2][2], cross[2][2];
 #pragma unroll
     for (int q = 0; q < 4; ++q)
@@ -498,6 +491,13 @@ __global__ __launch_bounds__(64 * GROUPS, 2) void ks_muon_gemm_kernel(MuonArgs a
             __builtin_amdgcn_sched_barrier(0);
             multiply(ring[q]);
             __builtin_amdgcn_sched_barrier(0);
+        }
+    }
+    if (WHAT != GRAM) {
+#pragma unroll
+        for (int k = 0; k < MINE; ++k) {
+            const int r = 8 * (group * MINE + k) + 4 * lq;
+            old[k] = x.get(WHAT == POLY ? id * M * M + operand_at(j0 + l32, i0 + r, M) : id * M * N + operand_at(j0 + l32, i0 + r, N));
         }
     }
     if (s < steps) multiply(ring[0]);
@@ -636,8 +636,8 @@ template <typename T> int run(const MuonArgs &a, int64_t matrices, char *ws, hip
         if (rc != KSMM_OK) return;
         hipLaunchKernelGGL(fn, dim3((unsigned)((tiles + 7) / 8 * 8)), dim3(64 * groups), lds, s, a, l, r, old, out, turned, w.M, w.N, last, (int)tiles);
     };
-    // waves that share K: 8 for the square products, whose tiles are few, 4 for the others ((1,1536,384,2) of two parts 203 us; before
-    // loads were kept ahead 223, 4 everywhere 227, 8 everywhere 241; (1,256,256,16) 108; 115, 112, 116)
+    // waves that share K: 8 for the square products, whose tiles are few, 4 for the others ((1,1536,384,2) of two parts 200 us; before
+    // loads were kept ahead 223, 4 everywhere 227, 8 everywhere 241; (1,256,256,16) 104; 115, 112, 116)
     for (int i = 0; i < a.steps; ++i) {
         gemm(&ks_muon_gemm_kernel<T, GRAM, 8>, 8, square, x, x, x, gram, gram, false);
         gemm(&ks_muon_gemm_kernel<T, POLY, 8>, 8, square, gram, gram, gram, poly, poly, false);
