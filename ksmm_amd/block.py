@@ -267,13 +267,8 @@ class NormKernel:
             needs[1] = True  # the gates' gradients are sums over it
         out = [torch.empty_like(t) if t is not None and need else None
                for t, need in zip((x, residual, gate, post_weight, weight, bias), needs)]
-        nothing = batch == 0 or (grad_r is None and grad_n is None)
-        if nothing or grad_n is None:
-            for i, t in enumerate(out):
-                if t is not None and (nothing or i >= 4):
-                    t.zero_()
-        if nothing:
-            return out
+        if batch == 0 or (grad_r is None and grad_n is None):
+            return [None if t is None else t.zero_() for t in out]
         dt = dtype_code(residual.dtype)
         need = lib.ksmm_residual_norm_backward_workspace(batch, features, groups, dt, int(bs_last))
         if need < 0:

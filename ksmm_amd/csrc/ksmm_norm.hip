@@ -1146,6 +1146,15 @@ __global__ __launch_bounds__(256) void ks_norm_cols_gate_kernel(NormArgs a, cons
     if ((threadIdx.x & 63) == 0) dgate[group * a.features + h] = (T)(a.alpha * s);
 }
 
+// Gradients of the last norm's parameters where there is none of its result.
+template <typename T> __global__ __launch_bounds__(256) void ks_norm_clear_kernel(T *__restrict__ dweight, T *__restrict__ dbias, int features)
+{
+    const int h = blockIdx.x * 256 + threadIdx.x;
+    if (h >= features) return;
+    if (dweight) dweight[h] = (T)0.f;
+    if (dbias) dbias[h] = (T)0.f;
+}
+
 // ---- choices ------------------------------------------------------------------------------------------
 // ranges of rows that fill the chip: workgroups of 4 waves, 2 of which fit a CU in the backward pass
 constexpr int64_t FWD_RANGES = 2048, BWD_RANGES = 768;
@@ -1449,6 +1458,15 @@ int ksmm_residual_norm_backward(const ksmm_norm_desc *desc, const float *stats, 
             hipLaunchKernelGGL((ks_norm_cols_gate_kernel<float>), dim3(blocks), dim3(256), 0, s, a, (const float *)dresidual, (float *)dgate, l.split.groups);
         else
             hipLaunchKernelGGL((ks_norm_cols_gate_kernel<half_t>), dim3(blocks), dim3(256), 0, s, a, (const half_t *)dresidual, (half_t *)dgate, l.split.groups);
+        st = launched();
+        if (st != KSMM_OK) return st;
+    }
+    if (!dn_out && (dweight || dbias)) {
+        const dim3 blocks((unsigned)((features + 255) / 256));
+        if (dtype == KSMM_F32)
+            hipLaunchKernelGGL((ks_norm_clear_kernel<float>), blocks, dim3(256), 0, s, (float *)dweight, (float *)dbias, (int)features);
+        else
+            hipLaunchKernelGGL((ks_norm_clear_kernel<half_t>), blocks, dim3(256), 0, s, (half_t *)dweight, (half_t *)dbias, (int)features);
         st = launched();
         if (st != KSMM_OK) return st;
     }

@@ -418,7 +418,7 @@ struct NormNode : ag::Node {
         const bool group_gates = how.bs_last && how.groups > 1 && t[2].defined() && task_should_compute_output(2);
         for (int i = 0; i < 6; ++i) {
             if (!t[i].defined() || !(task_should_compute_output(i) || (i == 1 && group_gates))) continue;
-            out[i] = !dn.defined() && i >= 4 ? at::zeros_like(t[i]) : at::empty_like(t[i]);
+            out[i] = at::empty_like(t[i]);
         }
         const int dt = code_of(t[1].scalar_type());
         const int64_t need = ksmm_residual_norm_backward_workspace(how.batch, how.features, how.groups, dt, how.bs_last);
