@@ -356,8 +356,8 @@ int64_t ksmm_residual_norm_forward_workspace(int64_t batch, int64_t features, in
 int ksmm_residual_norm_forward(const ksmm_norm_desc *desc, void *r_out, void *n_out, float *stats, void *workspace,
                                int64_t workspace_bytes, int64_t batch, int64_t features, int dtype, int bs_last,
                                void *stream);
-/* Gradients from those of the results (either may be NULL: zero, and without dn_out dweight and dbias are zeros).  What is not wanted is NULL; dgate of more than one
- * group in batch-size-last layout needs dresidual.  dgate, dpost_weight, dweight and dbias are sums in a fixed order. */
+/* Gradients from those of the results (either may be NULL: zero, and without dn_out dweight and dbias are zeros).  What is
+ * not wanted is NULL.  dgate, dpost_weight, dweight and dbias are sums in a fixed order. */
 int64_t ksmm_residual_norm_backward_workspace(int64_t batch, int64_t features, int64_t groups, int dtype,
                                               int bs_last);
 int ksmm_residual_norm_backward(const ksmm_norm_desc *desc, const float *stats, const void *dr_out,

@@ -262,9 +262,6 @@ class NormKernel:
                 _same(g, residual, name)
                 if g.shape != residual.shape:
                     raise ValueError("%s must have the residual's shape" % name)
-        needs = list(needs)
-        if needs[2] and gate is not None and groups > 1 and bs_last:
-            needs[1] = True  # the gates' gradients are sums over it
         out = [torch.empty_like(t) if t is not None and need else None
                for t, need in zip((x, residual, gate, post_weight, weight, bias), needs)]
         if batch == 0 or (grad_r is None and grad_n is None):
@@ -304,7 +301,7 @@ class ResidualNormFunction(torch.autograd.Function):
         grad_r = grads[0] if has_x else None
         grad_n = grads[-1] if need_norm else None
         out = NormKernel.backward(grad_r, grad_n, stats, *inputs, *ctx.how, needs=ctx.needs_input_grad[:6])
-        return (*(g if need else None for g, need in zip(out, ctx.needs_input_grad)), None, None, None, None, None)
+        return (*out, None, None, None, None, None)
 
 
 def residual_norm(x, residual, gate=None, post_weight=None, weight=None, bias=None, alpha=1.0, norm="rms", eps=1e-6, bs_last=False,

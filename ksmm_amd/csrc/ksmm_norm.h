@@ -18,6 +18,7 @@ struct NormGrads {
     const void *dr_out, *dn_out;  // gradients of the results, null: zero
     void *dx, *dresidual;         // null: not wanted
     float *dweight, *dbias, *dpost_weight, *dgate;  // partial sums, null: not wanted
+    float *means;                 // of dv and of dv v, a value a row each: for gates of groups batch-size-last, null: not wanted
 };
 
 // How the rows are dealt to workgroups where sums over them are taken (batch-size-first).

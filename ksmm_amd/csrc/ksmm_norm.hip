@@ -813,6 +813,10 @@ __global__ __launch_bounds__(COL_THREADS) void ks_norm_cols_bwd_kernel(NormArgs 
             m1.v[c] = a.layer ? m1.v[c] * inv : 0.f;
             m2.v[c] *= inv;
         }
+        if (d.means && grp == 0) {
+            store_four(d.means + col, count, m1);
+            store_four(d.means + B + col, count, m2);
+        }
     }
     // D of one feature
     auto get_D = [&](int i, int h, const Params &p, const Four &u) {
@@ -947,7 +951,13 @@ __global__ __launch_bounds__(COL_THREADS, 4) void ks_norm_step_kernel(NormArgs a
             }
         } else {
             for (int q = 0; q < 4; ++q) known[q][threadIdx.x] = a.stats[q * B + c];
-            if (STEP != SUMS && dn) total(sp.m, 4);
+            if (STEP != SUMS && dn) {
+                total(sp.m, 4);
+                if (STEP == RES && d.means && chunk == 0) {
+                    d.means[c] = known[4][threadIdx.x];
+                    d.means[B + c] = known[5][threadIdx.x];
+                }
+            }
         }
     }
     __syncthreads();
@@ -1126,24 +1136,48 @@ __global__ __launch_bounds__(COL_THREADS, 4) void ks_norm_step_kernel(NormArgs a
     }
 }
 
-// Gradients of gates that belong to groups of columns: a wave sums a feature over a group, from the stored dr.
-template <typename T>
-__global__ __launch_bounds__(256) void ks_norm_cols_gate_kernel(NormArgs a, const T *__restrict__ dr, T *__restrict__ dgate, int64_t groups)
+// Gradients of gates that belong to groups of columns: a wave sums four features over a group.  D is computed again, from
+// the statistics and the two means that the kernels before left (dr as it is stored would be rounded, and may have left the
+// type); a column's six floats serve the four features.
+constexpr int GATE_FEATURES = 4;
+template <typename T> __global__ __launch_bounds__(256) void ks_norm_cols_gate_kernel(NormArgs a, NormGrads d, T *__restrict__ dgate, int64_t groups)
 {
-    const int64_t wave = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6), B = a.batch;
-    const int64_t group = wave / a.features;
-    const int h = (int)(wave - group * a.features);
+    const int units = (a.features + GATE_FEATURES - 1) / GATE_FEATURES;
+    const int64_t wave = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), B = a.batch;
+    const int64_t group = wave / units;
     if (group >= groups) return;
-    const T *x = (const T *)a.x, *post = (const T *)a.post_weight;
-    const float pw = post ? (float)post[h] : 1.f;
-    float s = 0.f;
-    for (int64_t c = group * a.group_rows + (threadIdx.x & 63); c < (group + 1) * a.group_rows; c += 64) {
-        float p = (float)x[h * B + c];
-        if (post) p = (p - a.stats[c]) * a.stats[B + c] * pw;
-        s = fmaf((float)dr[h * B + c], p, s);
+    const int h0 = (int)(wave - group * units) * GATE_FEATURES, last = a.features - 1, lane = threadIdx.x & 63;
+    const T *const x = (const T *)a.x, *const res = (const T *)a.residual, *const dr = (const T *)d.dr_out, *const dn = (const T *)d.dn_out;
+    float gate[GATE_FEATURES], post[GATE_FEATURES], weight[GATE_FEATURES], s[GATE_FEATURES];
+    int64_t row[GATE_FEATURES];  // (past the last feature: the last one again, not stored)
+#pragma unroll
+    for (int i = 0; i < GATE_FEATURES; ++i) {
+        const int h = min(h0 + i, last);
+        gate[i] = a.alpha * (float)((const T *)a.gate)[group * a.features + h];
+        post[i] = a.post_weight ? (float)((const T *)a.post_weight)[h] : 1.f;
+        weight[i] = a.weight ? (float)((const T *)a.weight)[h] : 1.f;
+        row[i] = h * B;
+        s[i] = 0.f;
     }
-    s = sum64(s);
-    if ((threadIdx.x & 63) == 0) dgate[group * a.features + h] = (T)(a.alpha * s);
+    for (int64_t c = group * a.group_rows + lane; c < (group + 1) * a.group_rows; c += 64) {
+        const float mean_x = a.stats[c], rho_x = a.stats[B + c], mean_r = a.stats[2 * B + c], rho_r = a.stats[3 * B + c];
+        const float m1 = dn ? d.means[c] : 0.f, m2 = dn ? d.means[B + c] : 0.f;
+#pragma unroll
+        for (int i = 0; i < GATE_FEATURES; ++i) {
+            float p = (float)x[row[i] + c], D = dr ? (float)dr[row[i] + c] : 0.f;
+            if (a.post_weight) p = (p - mean_x) * rho_x * post[i];
+            if (dn) {
+                const float v = (fmaf(gate[i], p, (float)res[row[i] + c]) - mean_r) * rho_r;
+                D = fmaf(rho_r, project(a, (float)dn[row[i] + c] * weight[i], v, m1, m2, rho_r), D);
+            }
+            s[i] = fmaf(D, p, s[i]);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < GATE_FEATURES; ++i) {
+        s[i] = sum64(s[i]);
+        if (lane == 0 && h0 + i <= last) dgate[group * a.features + h0 + i] = (T)(a.alpha * s[i]);
+    }
 }
 
 // Gradients of the last norm's parameters where there is none of its result.
@@ -1329,7 +1363,7 @@ int64_t align256(int64_t v) { return (v + 255) / 256 * 256; }
 
 // where the partial sums of each quantity lie
 struct Layout {
-    int64_t slices, slice_bytes, gate_bytes, steps, total;
+    int64_t slices, slice_bytes, gate_bytes, steps, means, total;
     NormSplit split;
 };
 Layout layout(int64_t batch, int64_t features, int64_t groups, int dtype, int bs_last)
@@ -1342,7 +1376,8 @@ Layout layout(int64_t batch, int64_t features, int64_t groups, int dtype, int bs
     l.slice_bytes = align256(4 * l.slices * features);
     l.gate_bytes = l.split.one_gate ? l.slice_bytes : bs_last ? 0 : align256(4 * l.split.parts * l.split.groups * features);
     l.steps = 3 * l.slice_bytes + l.gate_bytes;
-    l.total = l.steps + (steps ? 8 * steps_of(batch, features).part : 0);
+    l.means = l.steps + (steps ? align256(8 * steps_of(batch, features).part) : 0);
+    l.total = l.means + (bs_last && !l.split.one_gate ? 8 * batch : 0);
     return l;
 }
 
@@ -1430,7 +1465,6 @@ int ksmm_residual_norm_backward(const ksmm_norm_desc *desc, const float *stats, 
     const Layout l = layout(batch, features, desc->groups, dtype, bs_last);
     if (!workspace || workspace_bytes < l.total || ((uintptr_t)workspace & 15) != 0) return KSMM_ERR_WORKSPACE;
     const bool gate_alone = dgate && bs_last && !l.split.one_gate;
-    if (gate_alone && !dresidual) return KSMM_ERR_NULL_POINTER;  // its sums read it
     if (gate_alone && l.split.groups * features > 0x7fffffffLL) return KSMM_ERR_TOO_LARGE;
     const int64_t size = batch * features * (int64_t)dtype_size(dtype);
     const void *const in[] = {desc->x, desc->residual, dr_out, dn_out};
@@ -1450,14 +1484,16 @@ int ksmm_residual_norm_backward(const ksmm_norm_desc *desc, const float *stats, 
     p.dbias = dbias && dn_out ? (float *)(ws + l.slice_bytes) : nullptr;
     p.dpost_weight = dpost_weight ? (float *)(ws + 2 * l.slice_bytes) : nullptr;
     p.dgate = dgate && !gate_alone ? (float *)(ws + 3 * l.slice_bytes) : nullptr;
+    p.means = gate_alone ? (float *)(ws + l.means) : nullptr;
     int st = dtype == KSMM_F32 ? backward<float>(a, p, l.split, bs_last, (float *)(ws + l.steps), s) : backward<half_t>(a, p, l.split, bs_last, (float *)(ws + l.steps), s);
     if (st != KSMM_OK) return st;
     if (gate_alone) {
-        const unsigned blocks = (unsigned)((l.split.groups * features + 3) / 4);
+        const int64_t waves = l.split.groups * ((features + GATE_FEATURES - 1) / GATE_FEATURES);
+        const dim3 blocks((unsigned)((waves + 3) / 4));
         if (dtype == KSMM_F32)
-            hipLaunchKernelGGL((ks_norm_cols_gate_kernel<float>), dim3(blocks), dim3(256), 0, s, a, (const float *)dresidual, (float *)dgate, l.split.groups);
+            hipLaunchKernelGGL((ks_norm_cols_gate_kernel<float>), blocks, dim3(256), 0, s, a, p, (float *)dgate, l.split.groups);
         else
-            hipLaunchKernelGGL((ks_norm_cols_gate_kernel<half_t>), dim3(blocks), dim3(256), 0, s, a, (const half_t *)dresidual, (half_t *)dgate, l.split.groups);
+            hipLaunchKernelGGL((ks_norm_cols_gate_kernel<half_t>), blocks, dim3(256), 0, s, a, p, (half_t *)dgate, l.split.groups);
         st = launched();
         if (st != KSMM_OK) return st;
     }

@@ -415,11 +415,8 @@ struct NormNode : ag::Node {
         {
         at::NoGradGuard no_grad;
         DeviceScope scope(t[1].device().index());
-        const bool group_gates = how.bs_last && how.groups > 1 && t[2].defined() && task_should_compute_output(2);
-        for (int i = 0; i < 6; ++i) {
-            if (!t[i].defined() || !(task_should_compute_output(i) || (i == 1 && group_gates))) continue;
-            out[i] = at::empty_like(t[i]);
-        }
+        for (int i = 0; i < 6; ++i)
+            if (t[i].defined() && task_should_compute_output(i)) out[i] = at::empty_like(t[i]);
         const int dt = code_of(t[1].scalar_type());
         const int64_t need = ksmm_residual_norm_backward_workspace(how.batch, how.features, how.groups, dt, how.bs_last);
         check_status(need < 0 ? (int)need : KSMM_OK);
@@ -429,8 +426,7 @@ struct NormNode : ag::Node {
                                                  out_of(out[3]), out_of(out[4]), out_of(out[5]), ws.mutable_data_ptr(), need, how.batch, how.features, dt,
                                                  how.bs_last, stream_of(t[1])));
         }
-        for (int i = 0; i < 6; ++i)
-            if (task_should_compute_output(i)) result[i] = out[i];
+        for (int i = 0; i < 6; ++i) result[i] = out[i];
         return once(std::move(result), "residual_norm");
     }
 };
