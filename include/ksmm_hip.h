@@ -372,7 +372,7 @@ int ksmm_residual_norm_backward(const ksmm_norm_desc *desc, const float *stats, 
  *     out = keep * weight - rate * X                            (weight NULL: out = X)
  * grad, weight and out have `dtype`; momentum is fp32.  master (NULL: none): fp32 values that the weights are
  * rounded from; they are read in place of weight, and written too.  momentum_out, master_out and out may be
- * momentum, master and weight themselves. */
+ * momentum, master and weight themselves, from the same address on. */
 typedef struct ksmm_muon_desc {
     float coefficients[3];
     float eps, beta, keep, rate;

@@ -65,6 +65,21 @@ static inline bool overlaps(const void *p, int64_t p_bytes, const void *q, int64
     const char *pb = (const char *)p, *qb = (const char *)q;
     return p && q && pb < qb + q_bytes && qb < pb + p_bytes;
 }
+// whether a result lies in an operand, or in another result (NULL and empty ones lie nowhere)
+struct Span {
+    const void *p;
+    int64_t bytes;
+};
+template <int I, int O> static inline bool any_overlap(const Span (&in)[I], const Span (&out)[O])
+{
+    for (int o = 0; o < O; ++o) {
+        for (const Span &i : in)
+            if (overlaps(out[o].p, out[o].bytes, i.p, i.bytes)) return true;
+        for (int q = 0; q < o; ++q)
+            if (overlaps(out[o].p, out[o].bytes, out[q].p, out[q].bytes)) return true;
+    }
+    return false;
+}
 
 static inline size_t dtype_size(int dt)
 {

@@ -683,6 +683,14 @@ int ksmm_muon_update(const ksmm_muon_desc *desc, const void *grad, const float *
     const int64_t need = ksmm_muon_workspace(blocks, c, b, parts);
     if (need < 0) return (int)need;
     if (need > 0 && (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15) != 0)) return KSMM_ERR_WORKSPACE;
+    {
+        // (momentum, masters and weights may be updated in their place, and nowhere else)
+        const int64_t values = blocks * parts * c * b, wide = 4 * values, size = values * (int64_t)dtype_size(dtype);
+        const bool own_m = momentum_out == momentum, own_master = master_out == master, own_w = out == weight;
+        const Span in[] = {{grad, size}, {own_m ? nullptr : momentum, wide}, {own_w ? nullptr : weight, size}, {own_master ? nullptr : master, wide}};
+        const Span written[] = {{momentum ? momentum_out : nullptr, wide}, {master ? master_out : nullptr, wide}, {out, size}, {need ? workspace : nullptr, need}};
+        if (any_overlap(in, written)) return KSMM_ERR_ALIAS;
+    }
     MuonArgs a;
     a.grad = grad;
     a.m_in = momentum;
