@@ -1411,6 +1411,16 @@ NormArgs args_of(const ksmm_norm_desc *d, int64_t batch, int64_t features)
     return a;
 }
 
+// what a call reads, but for statistics and gradients
+struct Operands {
+    Span of[6];
+};
+Operands operands_of(const NormArgs &a, int64_t groups, int dtype)
+{
+    const int64_t vector = a.features * (int64_t)dtype_size(dtype), rows = a.batch * vector;
+    return Operands{{{a.x, rows}, {a.residual, rows}, {a.gate, groups * vector}, {a.post_weight, vector}, {a.weight, vector}, {a.bias, vector}}};
+}
+
 }  // namespace
 
 }  // namespace ksmm
@@ -1434,11 +1444,10 @@ int ksmm_residual_norm_forward(const ksmm_norm_desc *desc, void *r_out, void *n_
     if ((desc->x && !r_out) || (!desc->x && !n_out)) return KSMM_ERR_NULL_POINTER;
     const int64_t need = ksmm_residual_norm_forward_workspace(batch, features, dtype, bs_last);
     if (need > 0 && (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15) != 0)) return KSMM_ERR_WORKSPACE;
-    const int64_t size = batch * features * (int64_t)dtype_size(dtype);
-    if (desc->x && (overlaps(r_out, size, desc->x, size) || overlaps(r_out, size, desc->residual, size) || overlaps(r_out, size, n_out, size)))
-        return KSMM_ERR_ALIAS;
-    if (overlaps(n_out, size, desc->x, size) || overlaps(n_out, size, desc->residual, size)) return KSMM_ERR_ALIAS;
     NormArgs a = args_of(desc, batch, features);
+    const int64_t size = batch * features * (int64_t)dtype_size(dtype);
+    const Span written[] = {{desc->x ? r_out : nullptr, size}, {n_out, size}, {stats, 16 * batch}, {need ? workspace : nullptr, need}};
+    if (any_overlap(operands_of(a, desc->groups, dtype).of, written)) return KSMM_ERR_ALIAS;
     a.r_out = desc->x ? r_out : nullptr;
     a.n_out = n_out;
     a.stats = stats;
@@ -1467,12 +1476,15 @@ int ksmm_residual_norm_backward(const ksmm_norm_desc *desc, const float *stats, 
     const bool gate_alone = dgate && bs_last && !l.split.one_gate;
     if (gate_alone && l.split.groups * features > 0x7fffffffLL) return KSMM_ERR_TOO_LARGE;
     const int64_t size = batch * features * (int64_t)dtype_size(dtype);
-    const void *const in[] = {desc->x, desc->residual, dr_out, dn_out};
-    for (const void *p : in)
-        if (overlaps(dx, size, p, size) || overlaps(dresidual, size, p, size)) return KSMM_ERR_ALIAS;
-    if (overlaps(dx, size, dresidual, size)) return KSMM_ERR_ALIAS;
-    const hipStream_t s = (hipStream_t)stream;
     NormArgs a = args_of(desc, batch, features);
+    {
+        const int64_t vector = features * (int64_t)dtype_size(dtype);
+        const Span written[] = {{dx, size}, {dresidual, size}, {dgate, desc->groups * vector}, {dpost_weight, vector}, {dweight, vector}, {dbias, vector},
+                                {workspace, l.total}};
+        const Span gradients[] = {{stats, 16 * batch}, {dr_out, size}, {dn_out, size}};
+        if (any_overlap(operands_of(a, desc->groups, dtype).of, written) || any_overlap(gradients, written)) return KSMM_ERR_ALIAS;
+    }
+    const hipStream_t s = (hipStream_t)stream;
     a.stats = (float *)stats;
     char *const ws = (char *)workspace;
     NormGrads p;
