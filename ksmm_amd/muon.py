@@ -123,6 +123,30 @@ class KSMuon(torch.optim.Optimizer):
         mine = {id(p) for p, _, _ in cls.factors_of(module)}
         return [p for p in module.parameters() if id(p) not in mine]
 
+    def load_state_dict(self, state_dict):
+        """As any optimiser's, but that the fp32 momentum and weights of fp16 factors stay fp32 (the base class rounds what it
+        loads to the parameters' type), and are copies."""
+        given = []
+
+        def seen(_, loaded):
+            given.append(loaded)
+
+        def widen(_):
+            of = [i for g in given[-1]["param_groups"] for i in g["params"]]
+            for i, p in zip(of, (p for g in self.param_groups for p in g["params"])):
+                for name in ("momentum", "master"):
+                    t = given[-1]["state"].get(i, {}).get(name)
+                    if t is not None:
+                        self.state[p][name] = t.to(device=p.device, dtype=torch.float32, copy=True).contiguous()
+
+        # (what the user's own hooks make of the state is what is loaded, and they see it as it will be)
+        hooks = self.register_load_state_dict_pre_hook(seen), self.register_load_state_dict_post_hook(widen, prepend=True)
+        try:
+            super().load_state_dict(state_dict)
+        finally:
+            for hook in hooks:
+                hook.remove()
+
     @torch.no_grad()
     def step(self, closure=None):
         loss = None

@@ -80,3 +80,45 @@ def test_norm_refuses_results_that_lie_in_operands(lib):
             for other in outs:
                 if other != o:
                     assert backward(**{o: outs[other]}) == ALIAS, (o, other)
+
+
+def optimizer(dtype):
+    """KSMuon over one CPU parameter, made without its check that factors are on a GPU."""
+    from ksmm_amd import KSMuon
+
+    p = torch.nn.Parameter(torch.randn(8, 6).to(dtype))
+    opt = KSMuon.__new__(KSMuon)
+    torch.optim.Optimizer.__init__(opt, [{"params": [p], "pattern": (1, 6, 8, 1), "parts": 1}], dict(lr=0.02, master=True))
+    return p, opt
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+def test_state_is_loaded_in_32_bits(dtype):
+    p, opt = optimizer(dtype)
+    half = dtype == torch.float16
+    opt.state[p] = {"momentum": torch.randn(8, 6), "master": torch.randn(8, 6) if half else None}
+    saved = opt.state_dict()
+    q, again = optimizer(dtype)
+    seen = []
+    again.register_load_state_dict_pre_hook(lambda o, s: seen.append("before"))
+    again.register_load_state_dict_post_hook(lambda o: seen.append([v.dtype for v in o.state[q].values() if v is not None]))
+    again.load_state_dict(saved)
+    assert seen == ["before", [torch.float32] * (2 if half else 1)]
+    assert list(again.state) == [q] and again.param_groups[0]["lr"] == 0.02
+    for name, v in opt.state[p].items():
+        if v is None:
+            assert again.state[q][name] is None
+        else:
+            assert torch.equal(again.state[q][name], v) and again.state[q][name].data_ptr() != v.data_ptr()
+    again.load_state_dict(saved)  # (the hooks it needs are gone: a second time is as the first)
+    assert len(seen) == 4
+
+
+def test_state_of_another_type_is_widened():
+    """As an optimiser that was saved in 16 bits leaves it."""
+    p, opt = optimizer(torch.float16)
+    opt.state[p] = {"momentum": torch.randn(8, 6).half(), "master": torch.randn(8, 6).half()}
+    q, again = optimizer(torch.float16)
+    again.load_state_dict(opt.state_dict())
+    assert all(v.dtype == torch.float32 for v in again.state[q].values())
+    assert torch.equal(again.state[q]["momentum"], opt.state[p]["momentum"].float())

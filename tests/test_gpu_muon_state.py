@@ -1,0 +1,64 @@
+"""KSMuon over its life: saved and resumed, next to autograd, next to others who write the weights."""
+
+import copy
+import io
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+DT = {"fp32": torch.float32, "fp16": torch.float16}
+
+PATTERNS = [((2, 24, 16, 1), 1), ((1, 20, 12, 2), 2), ((1, 130, 140, 1), 1)]
+
+
+def factors(dtype, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    return [(torch.nn.Parameter((torch.randn(a * d * c, parts * b, generator=g) * 0.2).to(dtype).cuda()), (a, b, c, d), parts)
+            for (a, b, c, d), parts in PATTERNS]
+
+
+def step(opt, fs, i):
+    g = torch.Generator().manual_seed(100 + i)
+    for p, _, _ in fs:
+        p.grad = (torch.randn(p.shape, generator=g) * 0.01).to(p.dtype).cuda()
+    opt.step()
+
+
+def tensors(opt):
+    return [v for s in opt.state.values() for v in (s["momentum"], s.get("master")) if v is not None]
+
+
+@pytest.mark.parametrize("prec", ["fp32", "fp16"])
+@pytest.mark.parametrize("model_first", [True, False])
+def test_resumed_steps_are_those_that_were_not_interrupted(prec, model_first):
+    from ksmm_amd import KSMuon
+
+    fs = factors(DT[prec])
+    opt = KSMuon(fs, lr=0.01, weight_decay=0.1)
+    for i in range(3):
+        step(opt, fs, i)
+    saved = io.BytesIO()
+    torch.save([opt.state_dict(), [p.detach() for p, _, _ in fs]], saved)
+    for i in range(3, 6):
+        step(opt, fs, i)
+    saved.seek(0)
+    state, weights = torch.load(saved, weights_only=True)
+    again = factors(DT[prec], seed=9)
+    resumed = KSMuon(again, lr=0.5)
+    if not model_first:
+        resumed.load_state_dict(state)
+    with torch.no_grad():
+        for (p, _, _), w in zip(again, weights):
+            p.copy_(w)
+    if model_first:
+        resumed.load_state_dict(state)
+    assert all(t.dtype == torch.float32 for t in tensors(resumed))
+    before = copy.deepcopy(state)
+    for i in range(3, 6):
+        step(resumed, again, i)
+    for (p, _, _), (q, _, _) in zip(fs, again):
+        assert torch.equal(p, q)
+    assert all(torch.equal(x, y) for x, y in zip(tensors(opt), tensors(resumed))) and len(tensors(opt)) == (6 if prec == "fp16" else 3)
+    for k in state["state"]:  # what was loaded from is not written
+        assert torch.equal(state["state"][k]["momentum"], before["state"][k]["momentum"])
