@@ -27,6 +27,11 @@ def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
+def _written(*tensors):
+    """Tells autograd that these were written: a kernel does not, and a graph that holds one of them must not run on."""
+    torch.autograd.graph.increment_version([t for t in tensors if not t.is_inference()])
+
+
 def _trainable_type(t, name):
     if t.dtype not in (torch.float32, torch.float16):
         raise AssertionError("Unsupported data type %s of %s: float32 and float16 are" % (t.dtype, name))
@@ -72,7 +77,8 @@ class GatedKernel:
         a, b, c, d = _check_gated(x, factor, pattern, bias, act, bs_last)
         batch = x.numel() // (a * c * d)
         shape = (a * b * d, *x.shape[1:]) if bs_last else (*x.shape[:-1], a * b * d)
-        if out is None:
+        given = out is not None
+        if not given:
             out = torch.empty(shape, dtype=x.dtype, device=x.device)
         elif tuple(out.shape) != tuple(shape) or out.dtype != x.dtype or out.device != x.device or not out.is_contiguous():
             raise ValueError("out must be a contiguous %s of shape %s" % (x.dtype, tuple(shape)))
@@ -81,6 +87,8 @@ class GatedKernel:
         with torch.cuda.device(x.device):
             _lib.check(lib.ksmm_gated_forward(x.data_ptr(), factor.data_ptr(), _ptr(bias), out.data_ptr(), batch, a, b, c, d,
                                               dtype_code(x.dtype), int(bs_last), GATED_ACTS[act], _stream_ptr(x)))
+        if given:
+            _written(out)
         return out
 
     @staticmethod

@@ -10,7 +10,7 @@ import math
 import torch
 
 from . import _lib
-from .block import KSGatedLinear, _ptr, _same, _trainable_type
+from .block import KSGatedLinear, _ptr, _same, _trainable_type, _written
 from .kernel import _check_input, _stream_ptr, dtype_code
 from .layer import KSLinear
 
@@ -82,6 +82,7 @@ def muon_update(weight, grad, momentum, pattern, parts=1, lr=0.02, beta=0.95, we
     _, b, c, _ = shape
     _launch(grad, shape, parts, steps, coefficients, eps, out, momentum, m, weight, master, master, beta, 1 - lr * weight_decay,
             lr * math.sqrt(max(1.0, b / c)), nesterov)
+    _written(*((weight, momentum) if inplace else ()), *(() if master is None else (master,)))
     return out, m
 
 

@@ -62,3 +62,37 @@ def test_resumed_steps_are_those_that_were_not_interrupted(prec, model_first):
     assert all(torch.equal(x, y) for x, y in zip(tensors(opt), tensors(resumed))) and len(tensors(opt)) == (6 if prec == "fp16" else 3)
     for k in state["state"]:  # what was loaded from is not written
         assert torch.equal(state["state"][k]["momentum"], before["state"][k]["momentum"])
+
+
+def test_autograd_sees_the_new_weights():
+    """A graph that was made with the old weights refuses to run backward, as it does behind torch's optimisers."""
+    from ksmm_amd import KSMuon, gated_linear, muon_update
+
+    pattern = (1, 16, 8, 2)
+    for prec in ("fp32", "fp16"):
+        w = torch.nn.Parameter((torch.randn(16, 32) * 0.3).to(DT[prec]).cuda())
+        x = torch.randn(5, 16, device="cuda").to(DT[prec]).requires_grad_()
+        opt = KSMuon([(w, pattern, 2)])
+        with torch.enable_grad():
+            h = gated_linear(x, w, pattern)
+            h.sum().backward(retain_graph=True)
+            opt.step()
+            with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+                h.sum().backward()
+        m, master = torch.zeros(16, 32, device="cuda"), torch.zeros(16, 32, device="cuda")
+        at = [t._version for t in (w, m, master)]
+        muon_update(w, w.grad, m, pattern, parts=2, master=master, inplace=True)
+        assert all(t._version > v for t, v in zip((w, m, master), at))
+        at = [t._version for t in (w, m, master)]
+        muon_update(w, w.grad, m, pattern, parts=2, master=master)  # writes the master alone
+        assert [t._version > v for t, v in zip((w, m, master), at)] == [False, False, True]
+
+
+def test_inference_tensors_are_updated_too():
+    from ksmm_amd import muon_update
+
+    with torch.inference_mode():
+        w, g, m = (torch.randn(16, 8, device="cuda") for _ in range(3))
+        want, want_m = muon_update(w, g, m, (1, 8, 8, 2))
+        muon_update(w, g, m, (1, 8, 8, 2), inplace=True)
+        assert torch.equal(w, want) and torch.equal(m, want_m)
