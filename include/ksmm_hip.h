@@ -371,12 +371,13 @@ int ksmm_residual_norm_backward(const ksmm_norm_desc *desc, const float *stats, 
  *     X = u / (|u|_F + eps);   steps times:  A = X X^T,  X = p0 X + (p1 A + p2 A A) X
  *     out = keep * weight - rate * X                            (weight NULL: out = X)
  * grad, weight and out have `dtype`; momentum is fp32.  master (NULL: none): fp32 values that the weights are
- * rounded from; they are read in place of weight, and written too.  momentum_out, master_out and out may be
+ * rounded from; they are read in place of weight, and written too.  follow: a weight that is not its master's rounding
+ * (somebody wrote it since) is read in place of the master.  momentum_out, master_out and out may be
  * momentum, master and weight themselves, from the same address on. */
 typedef struct ksmm_muon_desc {
     float coefficients[3];
     float eps, beta, keep, rate;
-    int steps, nesterov;
+    int steps, nesterov, follow;
 } ksmm_muon_desc;
 int64_t ksmm_muon_workspace(int64_t blocks, int c, int b, int parts);
 int ksmm_muon_update(const ksmm_muon_desc *desc, const void *grad, const float *momentum, float *momentum_out,

@@ -47,7 +47,7 @@ class KsmmNormDesc(ctypes.Structure):
 
 class KsmmMuonDesc(ctypes.Structure):
     _fields_ = [("coefficients", ctypes.c_float * 3), ("eps", ctypes.c_float), ("beta", ctypes.c_float),
-                ("keep", ctypes.c_float), ("rate", ctypes.c_float), ("steps", c_int), ("nesterov", c_int)]
+                ("keep", ctypes.c_float), ("rate", ctypes.c_float), ("steps", c_int), ("nesterov", c_int), ("follow", c_int)]
 
 
 # name -> (restype, argtypes); every symbol include/ksmm_hip.h declares

@@ -29,7 +29,7 @@ struct MuonArgs {
     float *master_out;
     void *out;               // T: w', or X
     int c, b, parts;         // blocks of c x b, `parts` side by side
-    int steps, nesterov;
+    int steps, nesterov, follow;
     float beta, keep, rate;  // w' = keep w - rate X
     float p0, p1, p2, eps;
 };
@@ -50,10 +50,19 @@ template <typename T> __device__ __forceinline__ float update_of(const MuonArgs 
     }
     return u;
 }
+// the weight that is updated: the master, or what lies in its place if that is not its rounding any more (`follow`)
+template <typename T> __device__ __forceinline__ float weight_of(const MuonArgs &a, int64_t at)
+{
+    if (!a.master_in) return (float)((const T *)a.w_in)[at];
+    const float m = a.master_in[at];
+    if (!a.follow) return m;
+    const T w = ((const T *)a.w_in)[at];
+    return (T)m == w ? m : (float)w;
+}
 template <typename T> __device__ __forceinline__ void finish(const MuonArgs &a, int64_t at, float x)
 {
     if (a.w_in) {
-        const float w = fmaf(a.keep, a.master_in ? a.master_in[at] : (float)((const T *)a.w_in)[at], -a.rate * x);
+        const float w = fmaf(a.keep, weight_of<T>(a, at), -a.rate * x);
         if (a.master_in) a.master_out[at] = w;
         ((T *)a.out)[at] = (T)w;
     } else {
@@ -313,8 +322,7 @@ __global__ __launch_bounds__(64 * WAVES) void ks_muon_block_kernel(MuonArgs a)
         float w[ONCE];
         if (a.w_in) {
 #pragma unroll
-            for (int e = 0; e < ONCE; ++e, at.next())
-                w[e] = a.master_in ? a.master_in[base + at.place()] : (float)((const T *)a.w_in)[base + at.place()];
+            for (int e = 0; e < ONCE; ++e, at.next()) w[e] = weight_of<T>(a, base + at.place());
         }
 #pragma unroll
         for (int e = 0; e < ONCE; ++e, to.next()) {
@@ -704,6 +712,7 @@ int ksmm_muon_update(const ksmm_muon_desc *desc, const void *grad, const float *
     a.parts = parts;
     a.steps = desc->steps;
     a.nesterov = desc->nesterov;
+    a.follow = desc->follow;
     a.beta = desc->beta;
     a.keep = desc->keep;
     a.rate = desc->rate;

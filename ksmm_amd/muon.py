@@ -33,14 +33,14 @@ def _check(update, pattern, parts, steps, coefficients, name):
 
 
 def _launch(grad, shape, parts, steps, coefficients, eps, out, momentum=None, momentum_out=None, weight=None, master=None,
-            master_out=None, beta=0.0, keep=1.0, rate=1.0, nesterov=True):
+            master_out=None, beta=0.0, keep=1.0, rate=1.0, nesterov=True, follow=False):
     lib = _lib.load()
     a, b, c, d = shape
     need = lib.ksmm_muon_workspace(a * d, c, b, parts)
     if need < 0:
         _lib.check(int(need))
     workspace = torch.empty(need, dtype=torch.uint8, device=grad.device) if need else None
-    desc = _lib.KsmmMuonDesc((ctypes.c_float * 3)(*coefficients), eps, beta, keep, rate, steps, int(nesterov))
+    desc = _lib.KsmmMuonDesc((ctypes.c_float * 3)(*coefficients), eps, beta, keep, rate, steps, int(nesterov), int(follow))
     with torch.cuda.device(grad.device):
         _lib.check(lib.ksmm_muon_update(ctypes.byref(desc), grad.data_ptr(), _ptr(momentum), _ptr(momentum_out), _ptr(weight),
                                         _ptr(master), _ptr(master_out), out.data_ptr(), _ptr(workspace), need, a * d, c, b, parts,
@@ -58,15 +58,16 @@ def orthogonalize(update, pattern, parts=1, steps=5, coefficients=COEFFICIENTS, 
 
 
 def muon_update(weight, grad, momentum, pattern, parts=1, lr=0.02, beta=0.95, weight_decay=0.0, nesterov=True, steps=5,
-                coefficients=COEFFICIENTS, eps=1e-7, master=None, inplace=False):
+                coefficients=COEFFICIENTS, eps=1e-7, master=None, inplace=False, follow=False):
     """(new weight, new momentum) of one step:
 
         m = beta * momentum + grad,  u = grad + beta * m (``nesterov``) or m
         w = (1 - lr * weight_decay) * weight - lr * sqrt(max(1, b / c)) * orthogonalize(u)
 
     ``weight`` and ``grad`` are kernel-format tensors of one type, ``momentum`` is fp32 and of their shape.  ``master``: fp32
-    weights that ``weight`` is rounded from; they are read instead of it and updated in place.  ``inplace``
-    writes the results over ``weight`` and ``momentum``."""
+    weights that ``weight`` is rounded from; they are read instead of it and updated in place.  ``follow``: where ``weight`` is not
+    what ``master`` rounds to, it was written since, and counts instead.  ``inplace`` writes the results over ``weight`` and
+    ``momentum``."""
     shape = _check(grad, pattern, parts, steps, coefficients, "grad")
     _same(weight, grad, "weight")
     for t, name in ((momentum, "momentum"), (master, "master")):
@@ -81,7 +82,7 @@ def muon_update(weight, grad, momentum, pattern, parts=1, lr=0.02, beta=0.95, we
     out, m = (weight, momentum) if inplace else (torch.empty_like(weight), torch.empty_like(momentum))
     _, b, c, _ = shape
     _launch(grad, shape, parts, steps, coefficients, eps, out, momentum, m, weight, master, master, beta, 1 - lr * weight_decay,
-            lr * math.sqrt(max(1.0, b / c)), nesterov)
+            lr * math.sqrt(max(1.0, b / c)), nesterov, follow)
     _written(*((weight, momentum) if inplace else ()), *(() if master is None else (master,)))
     return out, m
 
@@ -92,7 +93,8 @@ class KSMuon(torch.optim.Optimizer):
         opt = KSMuon(model)            # every such factor of a module, or a list of (parameter, pattern, parts)
 
     The other parameters (biases, norms, gates) belong to another optimiser; ``others(model)`` lists them.  fp16
-    factors are rounded from fp32 weights that the optimiser keeps (``master=False``: updated as they are)."""
+    factors are rounded from fp32 weights that the optimiser keeps (``master=False``: updated as they are); values that were
+    written into a factor since, a checkpoint's say, replace them."""
 
     def __init__(self, factors, lr=0.02, beta=0.95, weight_decay=0.0, nesterov=True, steps=5, coefficients=COEFFICIENTS, eps=1e-7,
                  master=True):
@@ -163,5 +165,5 @@ class KSMuon(torch.optim.Optimizer):
                     state["momentum"] = torch.zeros_like(p, dtype=torch.float32, memory_format=torch.contiguous_format)
                     state["master"] = p.detach().float() if g["master"] and p.dtype == torch.float16 else None
                 muon_update(p, p.grad.contiguous(), state["momentum"], g["pattern"], g["parts"], g["lr"], g["beta"], g["weight_decay"],
-                            g["nesterov"], g["steps"], g["coefficients"], g["eps"], state["master"], inplace=True)
+                            g["nesterov"], g["steps"], g["coefficients"], g["eps"], state["master"], inplace=True, follow=True)
         return loss

@@ -96,3 +96,34 @@ def test_inference_tensors_are_updated_too():
         want, want_m = muon_update(w, g, m, (1, 8, 8, 2))
         muon_update(w, g, m, (1, 8, 8, 2), inplace=True)
         assert torch.equal(w, want) and torch.equal(m, want_m)
+
+
+@pytest.mark.parametrize("how", ["copy", "data", "some"])
+def test_weights_that_others_wrote_count(how):
+    """fp32 masters stand behind fp16 weights that are still their rounding; weights loaded or changed afterwards replace them."""
+    from ksmm_amd import KSMuon
+
+    fs, new = factors(torch.float16), factors(torch.float16, seed=5)
+    opt = KSMuon(fs, lr=0.01)
+    for i in range(2):
+        step(opt, fs, i)
+    masters = [opt.state[p]["master"].clone() for p, _, _ in fs]
+    with torch.no_grad():
+        for (p, _, _), (q, _, _) in zip(fs, new):
+            if how == "copy":
+                p.copy_(q)
+            elif how == "data":  # (autograd does not see this one)
+                p.data.copy_(q)
+            else:
+                p[1].copy_(q[1])
+    # (a written value that is by chance what the master rounds to leaves it its bits)
+    want = [torch.where(p.detach() == m.half(), m, p.detach().float()) for (p, _, _), m in zip(fs, masters)]
+    assert all(not torch.equal(w, m) for w, m in zip(want, masters))
+    ref = [(torch.nn.Parameter(p.detach().clone()), pattern, parts) for p, pattern, parts in fs]
+    other = KSMuon(ref, lr=0.01)
+    for (p, _, _), (q, _, _), m in zip(fs, ref, want):
+        other.state[q] = {"momentum": opt.state[p]["momentum"].clone(), "master": m.clone()}
+    step(opt, fs, 2)
+    step(other, ref, 2)
+    for (p, _, _), (q, _, _) in zip(fs, ref):
+        assert torch.equal(p, q) and torch.equal(opt.state[p]["master"], other.state[q]["master"])
