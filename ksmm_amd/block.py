@@ -148,7 +148,8 @@ def gated_linear(x, factor, pattern, bias=None, act="silu", bs_last=False):
     out = _lib.native().gated_linear(x, factor, pattern, bias, act, bs_last)
     if out is not None:
         return out
-    if torch.is_grad_enabled() and (x.requires_grad or factor.requires_grad or (bias is not None and bias.requires_grad)):
+    if torch.jit.is_tracing() or (torch.is_grad_enabled() and (
+            x.requires_grad or factor.requires_grad or (bias is not None and bias.requires_grad))):
         return KSGatedFunction.apply(x, factor, bias, tuple(pattern), act, bs_last)
     return GatedKernel.forward(x, factor, pattern, bias, act, bs_last)
 
@@ -328,7 +329,7 @@ def residual_norm(x, residual, gate=None, post_weight=None, weight=None, bias=No
     out = _lib.native().residual_norm(*inputs, alpha, norm, eps, bs_last, need_norm)
     if out is not None:
         return out
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in inputs):
+    if torch.jit.is_tracing() or (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in inputs)):
         out = ResidualNormFunction.apply(*inputs, float(alpha), norm, float(eps), bs_last, need_norm)
         return (residual, out) if x is None else out if need_norm else (out, None)
     r, n, _ = NormKernel.forward(*inputs, alpha, norm, eps, bs_last, need_norm)

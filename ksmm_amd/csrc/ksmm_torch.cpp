@@ -19,6 +19,7 @@
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/autograd/saved_variable.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 
 #include "../../include/ksmm_hip.h"
 
@@ -352,6 +353,9 @@ PyObject *py_train_backward(PyObject *, PyObject *const *args, Py_ssize_t n_args
 
 namespace ag = torch::autograd;
 
+// torch.jit.trace records what is called through the dispatcher: of these calls the allocations alone.  The Python functions are
+// nodes of their own there.
+bool traced() { return torch::jit::tracer::isTracing(); }
 // a tensor argument, or none; false: neither
 bool read_optional(PyObject *o, at::Tensor *t)
 {
@@ -440,7 +444,7 @@ PyObject *py_residual_norm(PyObject *, PyObject *const *args, Py_ssize_t n_args)
     }
     try {
         at::Tensor in[6];
-        bool taken = true;
+        bool taken = !traced();
         for (int i = 0; i < 6 && taken; ++i) taken = read_optional(args[i], &in[i]);
         const at::Tensor &x = in[0], &res = in[1];
         NormHow how;
@@ -562,7 +566,7 @@ PyObject *py_gated_linear(PyObject *, PyObject *const *args, Py_ssize_t n_args)
     try {
         at::Tensor x, w, bias;
         int64_t v[4] = {0, 0, 0, 0};
-        bool taken = THPVariable_Check(args[0]) && THPVariable_Check(args[1]) && read_optional(args[3], &bias) && PyTuple_Check(args[2]) && PyTuple_GET_SIZE(args[2]) == 4;
+        bool taken = !traced() && THPVariable_Check(args[0]) && THPVariable_Check(args[1]) && read_optional(args[3], &bias) && PyTuple_Check(args[2]) && PyTuple_GET_SIZE(args[2]) == 4;
         GatedHow how;
         how.bs_last = PyObject_IsTrue(args[5]) == 1;
         how.act = args[4] == Py_None ? KSMM_ACT_NONE : -1;

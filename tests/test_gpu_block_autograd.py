@@ -13,6 +13,32 @@ def operands():
     return x, (torch.randn(32, 48, generator=g) / 6).cuda(), torch.randn(6, 32, generator=g).cuda(), torch.ones(32, device="cuda")
 
 
+def test_traced_functions_compute():
+    """torch.jit.trace records the operators, not the memory of the traced call's results."""
+    from ksmm_amd import gated_linear, residual_norm
+
+    x, w, r, v = operands()
+
+    def gated(x):
+        return gated_linear(x, w, (1, 24, 32, 1)) * 1.0
+
+    def norm(x, r):
+        out, n = residual_norm(x, r, weight=v)
+        return out * 1.0, n * 1.0
+
+    def only_norm(r):
+        return residual_norm(None, r, weight=v)[1] * 1.0
+
+    for grad in (False, True):
+        with torch.set_grad_enabled(grad):
+            for fn, args in ((gated, (x,)), (norm, (x, r)), (only_norm, (r,))):
+                traced = torch.jit.trace(fn, args, check_trace=False)
+                other = tuple(t * 1.5 + 0.25 for t in args)
+                got, want = traced(*other), fn(*other)
+                for a, b in zip(got if isinstance(got, tuple) else (got,), want if isinstance(want, tuple) else (want,)):
+                    assert torch.equal(a, b)
+
+
 def test_results_written_into_a_saved_tensor_are_noticed():
     from ksmm_amd import GatedKernel
 
