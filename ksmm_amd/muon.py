@@ -111,14 +111,18 @@ class KSMuon(torch.optim.Optimizer):
 
     @staticmethod
     def factors_of(module):
-        """(parameter, pattern, parts) of every factor that takes gradients."""
+        """(parameter, pattern, parts) of every factor that takes gradients; one that several modules share is one."""
         found = []
         for m in module.modules():
             if isinstance(m, KSGatedLinear):
                 found.append((m.factor, m.pattern, 2))
             elif isinstance(m, KSLinear) and m.algo == "kernel":
                 found += [(f, p, 1) for f, p in zip(m.factors, m.patterns)]
-        return [f for f in found if f[0].requires_grad]
+        once = {}
+        for f in found:
+            if f[0].requires_grad:
+                once.setdefault(id(f[0]), f)
+        return list(once.values())
 
     @classmethod
     def others(cls, module):

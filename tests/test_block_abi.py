@@ -82,6 +82,15 @@ def test_norm_refuses_results_that_lie_in_operands(lib):
                     assert backward(**{o: outs[other]}) == ALIAS, (o, other)
 
 
+def test_tied_factors_are_one():
+    from ksmm_amd import KSGatedLinear, KSMuon
+
+    first, second, other = (KSGatedLinear((2, 6, 4, 1), device="cpu") for _ in range(3))
+    second.factor = first.factor
+    found = KSMuon.factors_of(torch.nn.Sequential(first, second, other))
+    assert [id(f[0]) for f in found] == [id(first.factor), id(other.factor)]
+
+
 def optimizer(dtype):
     """KSMuon over one CPU parameter, made without its check that factors are on a GPU."""
     from ksmm_amd import KSMuon
