@@ -656,13 +656,16 @@ template <typename T> int run(const MuonArgs &a, int64_t matrices, char *ws, hip
     return rc == KSMM_OK ? launched() : rc;
 }
 
+// sizes are rounded up, and chunks and walks step over the end, in 32 bits
+bool too_large(int64_t blocks, int c, int b, int parts) { return (double)blocks * c * b * parts > 2147483647.0 - 4096.0; }
+
 int check(const ksmm_muon_desc *d, int64_t blocks, int c, int b, int parts, int dtype)
 {
     if (!d) return KSMM_ERR_NULL_POINTER;
     if (blocks < 1 || c < 1 || b < 1 || parts < 1) return KSMM_ERR_BAD_PATTERN;
     if (dtype != KSMM_F32 && dtype != KSMM_F16) return KSMM_ERR_BAD_DTYPE;
     if (d->steps < 1) return KSMM_ERR_BAD_ALGO;
-    if ((double)blocks * c * b * parts > 2147483647.0 || blocks * parts > 0x7fffffffLL) return KSMM_ERR_TOO_LARGE;
+    if (too_large(blocks, c, b, parts)) return KSMM_ERR_TOO_LARGE;
     return KSMM_OK;
 }
 
@@ -677,7 +680,7 @@ extern "C" {
 int64_t ksmm_muon_workspace(int64_t blocks, int c, int b, int parts)
 {
     if (blocks < 1 || c < 1 || b < 1 || parts < 1) return KSMM_ERR_BAD_PATTERN;
-    if ((double)blocks * c * b * parts > 2147483647.0) return KSMM_ERR_TOO_LARGE;
+    if (too_large(blocks, c, b, parts)) return KSMM_ERR_TOO_LARGE;
     return fits_lds(std::min(c, b), std::max(c, b)) ? 0 : space(blocks * parts, c, b).total;
 }
 
