@@ -85,7 +85,7 @@ def test_norm_refuses_results_that_lie_in_operands(lib):
 def test_update_refuses_sizes_whose_indexes_would_not_fit(lib):
     top = (1 << 31) - 1
     for blocks, c, b, parts in ((1, top, 1, 1), (1, 1, top, 1), (1, top - 100, 1, 1), (1, 1, 1, top), (1 << 62, 1, 1, 1), (top, 1, 1, 1),
-                                (1, 46340, 46341, 1)):
+                                (1, 46341, 46341, 1)):
         assert lib.ksmm_muon_workspace(blocks, c, b, parts) == -5, (blocks, c, b, parts)
 
 
