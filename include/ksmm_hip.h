@@ -370,6 +370,8 @@ int ksmm_residual_norm_backward(const ksmm_norm_desc *desc, const float *stats, 
  *     m' = beta m + g,   u = nesterov ? g + beta m' : m'        (momentum NULL: u = g)
  *     X = u / (|u|_F + eps);   steps times:  A = X X^T,  X = p0 X + (p1 A + p2 A A) X
  *     out = keep * weight - rate * X                            (weight NULL: out = X)
+ * X and its products are held in 22 bits (and to 1.5e-11), summed in fp32.  Coefficients and steps with which a matrix of singular
+ * values up to 1 could pass 60000 are KSMM_ERR_BAD_ALGO, as steps below 1 are.
  * grad, weight and out have `dtype`; momentum is fp32.  master (NULL: none): fp32 values that the weights are
  * rounded from; they are read in place of weight, and written too.  follow: a weight that is not its master's rounding
  * (somebody wrote it since) is read in place of the master.  momentum_out, master_out and out may be

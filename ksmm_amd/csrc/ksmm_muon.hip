@@ -11,8 +11,11 @@
 // Blocks that fit the LDS of a compute unit with their Gram matrix go through all steps in one launch, a workgroup
 // each (ks_muon_block_kernel).  Larger ones go step by step through tiles in global memory (ks_muon_gemm_kernel).  The
 // polynomial has slope p0 at zero: rounding errors of X grow up to p0^steps (485 for five of 3.4445) times, which is why
-// every product is good to 22 bits with fp32 sums, whatever the type of the update.
+// X, its Gram matrix and the polynomial of that are held in 22 bits, whatever the type of the update, and multiplied with fp32 sums.
 #include "ksmm_mfma.h"
+#include <algorithm>
+#include <cmath>
+#include <initializer_list>
 
 namespace ksmm {
 
@@ -79,7 +82,9 @@ __device__ __forceinline__ float wave_sum(float v)
 
 // fp32 values as two fp16 ones, x = hi + lo / 2048: 22 bits.  A product of two such is three matrix instructions
 // (hi hi, and hi lo + lo hi in sums of their own; what lo lo would add is below the last bit), 96 clocks for 32 x 32 x 16
-// where the 32-bit instructions take 512.  |X| <= 1 here, so that no part leaves fp16's range.
+// where the 32-bit instructions take 512.  The 22 bits are those of values from 6e-5 on; below, where hi is subnormal, they end at
+// 1.5e-11 (an entry of an orthogonal 1536 x 384 is 1e-3).  Coefficients with which a value could pass 60000 are refused (in_range).
+// (1,1536,384,2) of two parts is 5.6e-8 off in the 2-norm; the same steps in plain fp32 are 1.1e-7.
 constexpr float SPLIT = 2048.f;
 __device__ __forceinline__ void split(float v, half_t &hi, half_t &lo)
 {
@@ -659,6 +664,31 @@ template <typename T> int run(const MuonArgs &a, int64_t matrices, char *ws, hip
 // sizes are rounded up, and chunks and walks step over the end, in 32 bits
 bool too_large(int64_t blocks, int c, int b, int parts) { return (double)blocks * c * b * parts > 2147483647.0 - 4096.0; }
 
+// A step is a polynomial of the singular values, which are at most one in X0.  Whether any with such values can leave what pairs of
+// fp16 numbers hold: no entry of X, its Gram matrix or the polynomial of that is larger than the largest singular value of each.
+bool in_range(const float *p, int steps)
+{
+    const double p0 = p[0], p1 = p[1], p2 = p[2], most = 60000.0;
+    auto largest = [](double top, auto f, std::initializer_list<double> inner) {  // of |f| on [0, top]: at the top, or where its slope is zero
+        double v = std::fabs(f(top));
+        for (double at : inner)
+            if (at > 0 && at < top) v = std::max(v, std::fabs(f(at)));
+        return v;
+    };
+    const double root = 9 * p1 * p1 - 20 * p0 * p2, q = root > 0 ? std::sqrt(root) : 0.0;
+    // p0 + 3 p1 t + 5 p2 t^2 = 0, t the square of a singular value
+    const double t0 = p2 != 0 ? (-3 * p1 + q) / (10 * p2) : p1 != 0 ? -p0 / (3 * p1) : 0.0, t1 = p2 != 0 ? (-3 * p1 - q) / (10 * p2) : 0.0;
+    double s = 1.0;
+    for (int i = 0; i < steps; ++i) {
+        const double gram = s * s, poly = largest(gram, [&](double g) { return p1 * g + p2 * g * g; }, {p2 != 0 ? -p1 / (2 * p2) : 0.0});
+        const double next = largest(s, [&](double x) { return x * (p0 + x * x * (p1 + x * x * p2)); }, {t0 > 0 ? std::sqrt(t0) : 0.0, t1 > 0 ? std::sqrt(t1) : 0.0});
+        if (!(gram <= most && poly <= most && next <= most)) return false;
+        if (next == s) break;  // (and so it goes on)
+        s = next;
+    }
+    return true;
+}
+
 int check(const ksmm_muon_desc *d, int64_t blocks, int c, int b, int parts, int dtype)
 {
     if (!d) return KSMM_ERR_NULL_POINTER;
@@ -666,7 +696,7 @@ int check(const ksmm_muon_desc *d, int64_t blocks, int c, int b, int parts, int 
     if (dtype != KSMM_F32 && dtype != KSMM_F16) return KSMM_ERR_BAD_DTYPE;
     if (d->steps < 1) return KSMM_ERR_BAD_ALGO;
     if (too_large(blocks, c, b, parts)) return KSMM_ERR_TOO_LARGE;
-    return KSMM_OK;
+    return in_range(d->coefficients, d->steps) ? KSMM_OK : KSMM_ERR_BAD_ALGO;
 }
 
 }  // namespace

@@ -50,7 +50,8 @@ def _launch(grad, shape, parts, steps, coefficients, eps, out, momentum=None, mo
 def orthogonalize(update, pattern, parts=1, steps=5, coefficients=COEFFICIENTS, eps=1e-7):
     """The blocks of ``update``, a factor of ``pattern`` in kernel format (a*d*c, parts*b), made orthogonal: each
     c x b matrix X is divided by its Frobenius norm + ``eps`` and goes through ``steps`` steps of
-    X <- p0 X + (p1 A + p2 A A) X, A = X X^T.  fp32 throughout, rounded once to the update's type."""
+    X <- p0 X + (p1 A + p2 A A) X, A = X X^T.  X is held in 22 bits (and to 1.5e-11), sums are fp32; the result is rounded once to the
+    update's type.  Coefficients whose steps could take a matrix of singular values up to 1 beyond 60000 are refused."""
     shape = _check(update, pattern, parts, steps, coefficients, "update")
     out = torch.empty_like(update)
     _launch(update.detach(), shape, parts, steps, coefficients, eps, out)

@@ -1,12 +1,11 @@
 """What the C ABI of the operators around a feed-forward block refuses before anything is launched, and what its optimiser keeps of its
 state (no GPU)."""
-
 import ctypes
+
 import pytest
 import torch
 
 ALIAS = -11
-
 FAR = [(i + 1) << 28 for i in range(16)]  # addresses that are never touched: every call here is refused
 
 
@@ -87,6 +86,18 @@ def test_update_refuses_sizes_whose_indexes_would_not_fit(lib):
     for blocks, c, b, parts in ((1, top, 1, 1), (1, 1, top, 1), (1, top - 100, 1, 1), (1, 1, 1, top), (1 << 62, 1, 1, 1), (top, 1, 1, 1),
                                 (1, 46341, 46341, 1)):
         assert lib.ksmm_muon_workspace(blocks, c, b, parts) == -5, (blocks, c, b, parts)
+
+
+@pytest.mark.parametrize("coefficients,steps,status", [
+    ((3.4445, -4.7750, 2.0315), 5, -1), ((3.4445, -4.7750, 2.0315), 2000000000, -1), ((1.5, -0.5, 0.0), 100, -1), ((2.0, -1.5, 0.5), 30, -1),
+    ((20.0, 0.0, 0.0), 2, -1), ((20.0, 0.0, 0.0), 3, -6), ((1.0, 0.0, 1e6), 1, -6), ((3.4445, -4.7750, 20.0), 5, -6), ((float("nan"), 0.0, 0.0), 1, -6),
+    ((float("inf"), 0.0, 0.0), 1, -6), ((1.0, 0.0, 0.0), 2000000000, -1)])
+def test_update_refuses_coefficients_whose_steps_leave_the_range(coefficients, steps, status, lib):
+    """-1: accepted as far as the pointers, which are null here."""
+    from ksmm_amd._lib import KsmmMuonDesc
+
+    desc = KsmmMuonDesc((ctypes.c_float * 3)(*coefficients), 1e-7, 0.9, 1, 1, steps, 1)
+    assert lib.ksmm_muon_update(ctypes.byref(desc), None, None, None, None, None, None, None, None, 0, 1, 8, 8, 1, 0, None) == status
 
 
 def test_tied_factors_are_one():

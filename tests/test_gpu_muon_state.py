@@ -1,14 +1,13 @@
 """KSMuon over its life: saved and resumed, next to autograd, next to others who write the weights."""
-
 import copy
 import io
+
 import pytest
 import torch
 
 pytestmark = pytest.mark.gpu
 
 DT = {"fp32": torch.float32, "fp16": torch.float16}
-
 PATTERNS = [((2, 24, 16, 1), 1), ((1, 20, 12, 2), 2), ((1, 130, 140, 1), 1)]
 
 
@@ -127,3 +126,14 @@ def test_weights_that_others_wrote_count(how):
     step(other, ref, 2)
     for (p, _, _), (q, _, _) in zip(fs, ref):
         assert torch.equal(p, q) and torch.equal(opt.state[p]["master"], other.state[q]["master"])
+
+
+def test_coefficients_that_leave_the_range_are_refused():
+    """Iterates are held as pairs of fp16 numbers: coefficients with which a singular value of one or less could leave their range."""
+    from ksmm_amd import orthogonalize
+
+    u = torch.randn(32, 16, device="cuda")
+    for p, steps in (((20.0, 0.0, 0.0), 5), ((3.4445, -4.775, 20.0), 5), ((1.0, 0.0, 1e6), 1), ((float("nan"), 0.0, 0.0), 1)):
+        with pytest.raises(RuntimeError):
+            orthogonalize(u, (1, 16, 32, 1), steps=steps, coefficients=p)
+    assert orthogonalize(u, (1, 16, 32, 1), steps=2, coefficients=(20.0, 0.0, 0.0)).isfinite().all()
