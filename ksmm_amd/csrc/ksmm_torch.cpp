@@ -402,6 +402,7 @@ struct NormNode : ag::Node {
     std::string name() const override { return "ResidualNormBackward"; }
     void release_variables() override
     {
+        std::lock_guard<std::mutex> lock(mutex_);  // (another thread's pass may be reading them)
         for (auto &v : in) v.reset_data();
         stats.reset_data();
     }
@@ -529,6 +530,7 @@ struct GatedNode : ag::Node {
     std::string name() const override { return "GatedLinearBackward"; }
     void release_variables() override
     {
+        std::lock_guard<std::mutex> lock(mutex_);
         for (auto &v : in) v.reset_data();
     }
     ag::variable_list apply(ag::variable_list &&grads) override

@@ -1,6 +1,6 @@
 """The gated projection and the residual norm inside autograd: traced, from several threads, into tensors that are watched."""
-
 import threading
+
 import pytest
 import torch
 
@@ -50,3 +50,33 @@ def test_results_written_into_a_saved_tensor_are_noticed():
     GatedKernel.forward(x, w, (1, 24, 32, 1), out=held)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         y.backward()
+
+
+def test_one_graph_from_two_threads():
+    """Each backward pass of a shared graph gives its gradients, or says that the graph is gone."""
+    from ksmm_amd import gated_linear, residual_norm
+
+    x, w, r, v = operands()
+    for _ in range(20):
+        leaves = [t.clone().requires_grad_() for t in (x, r, w, v)]
+        with torch.enable_grad():
+            out, n = residual_norm(leaves[0], leaves[1], weight=leaves[3])
+            total = out.sum() + gated_linear(n, leaves[2], (1, 24, 32, 1)).sum()
+        want = torch.autograd.grad(total, leaves, retain_graph=True)
+        got, errors = [], []
+
+        def backward():
+            try:
+                got.append(torch.autograd.grad(total, leaves))
+            except RuntimeError as e:
+                errors.append(str(e))
+
+        threads = [threading.Thread(target=backward) for _ in range(2)]
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join(timeout=60)
+            assert not t.is_alive()
+        assert len(got) + len(errors) == 2 and all("second time" in e for e in errors), errors
+        for grads in got:
+            assert all(torch.equal(a, b) for a, b in zip(grads, want))
