@@ -464,19 +464,22 @@ __global__ __launch_bounds__(64 * WB *WN, 2) void ks_gated_kernel(GatedArgs g, i
 
 // ---- fp16 in aligned vectors: a ring of slabs ----------------------------------------------------------
 // The tile above spends its time waiting: a slab of 32 k is a quarter of a microsecond of products, its loads take two.
-// Here they go straight to LDS (no registers), three slabs of 16 k ahead; a workgroup stays for many tiles, and the first
-// slabs of the next one are on their way while this one's results leave.  Two workgroups a CU: one multiplies while the
-// other finishes a tile (GLU in the vector ALU takes as long as the products of c = 192).
+// Here they go straight to LDS (no registers), three slabs of 16 k ahead, and a workgroup stays for many tiles.  Two workgroups a CU:
+// one multiplies while the other finishes a tile (GLU in the vector ALU takes as long as the products of c = 192).
 //
-// What counts as landed is counted by hand: a slab's loads are followed by those of two more (2 * L of them), and, for three
-// iterations each, by the loads that a tile's end needs (bias of the next tile, dh; EARLY of them) and by its stores.
+// What counts as landed is counted by hand: a slab's loads are followed by those of two more (2 * L of them), and, in a tile's last two
+// iterations, by the loads that its end needs (bias of the next tile, dh; EARLY of them, each an instruction of its own in the
+// compiled code).  Those are ordinary loads, and the compiler, which does not see the ones to LDS, waits for them at the
+// head of the next tile with everything issued before: its first three slabs, and this one's stores.  So a tile begins with its slabs
+// landed, and stores do not run on behind it.
 //
 // d_i = 2: a row's (k, d_i) pairs are split into the operands of both d_i when they are read (one v_perm a register).
 // The sums start at the bias: one product of (bias, 0, ..) and (1, 0, ..).  Results go through 4 KB of LDS a wave, and
 // leave as rows of 128 bytes.
 //
-// (1,768,192,2), 25088 rows forward 62 us: 29.6 GFLOP at 480 TFLOP/s; 96 MB of x and h, 1.6 TB/s.  What is left is the vector
-// ALU's work on the results, which the other workgroup's products cover in part.
+// (1,768,192,2), 25088 rows forward 53 us: 29.6 GFLOP at 556 TFLOP/s; 96 MB of x and h, 1.8 TB/s.  The matrix cores are busy for 27 %
+// of the SIMDs' time: what is left is the wait at each tile's head, and the vector ALU's work on the results, which the other
+// workgroup's products cover in part.  MODE 1 with 128 outputs of one d_i or 64 of two spills 24 to 34 registers a lane, around its stores.
 constexpr int vmcnt_imm(int n) { return (n & 15) | (7 << 4) | (15 << 8) | (((n >> 4) & 3) << 14); }
 typedef __attribute__((address_space(3))) unsigned char *lds_bytes_t;
 
@@ -496,11 +499,11 @@ template <bool LAST, int D, int TB, int MODE> struct Ring {
     static constexpr int O_CPR = LAST ? 8 : TB / WB * D * 2 / 16;      // chunks a row of them
     static constexpr int O_IT = 32 * O_CPR / 64, PIECE = 32 * O_CPR * 16;
     static constexpr int LDS_BYTES = ST * STAGE + 4 * PIECE;
-    static constexpr int STORES = UNITS * O_IT * (MODE + 1), BIASES = LAST ? 2 * BT : D * BT, EARLY = BIASES + (MODE ? O_IT : 0);
+    static constexpr int BIASES = LAST ? 2 * BT : D * BT, EARLY = BIASES + (MODE ? O_IT : 0);
     static constexpr int WAIT = (ST - 2) * L;
     static_assert(W_BYTES % (16 * THREADS) == 0 && X_BYTES % (16 * THREADS) == 0 && (!LAST || D == 1) && D <= 2, "loads");
     static_assert(TB == 64 || TB == 128, "weight swizzle");
-    static_assert(WAIT + STORES + EARLY <= 63 && LDS_BYTES <= 80 * 1024, "ring");
+    static_assert(WAIT + EARLY <= 63 && LDS_BYTES <= 80 * 1024, "ring");
     static_assert(BT * PARTS * NT * D * 16 <= 128, "accumulators");
 };
 
@@ -747,16 +750,13 @@ __global__ __launch_bounds__(256, 2) void ks_gated_ring_kernel(GatedArgs g, int 
                 }
             }
         });
-        return p.n0 + C::TN <= B && p.b0 + TB <= b;  // all of its stores went out
     };
 
     begin_loads();
     load_bias(mine);
 #pragma unroll
     for (int s = 0; s < C::ST - 1; ++s) issue();
-    int read = 0;        // slot that is multiplied next
-    int after = 0;       // stores of the tile before that may still be counted
-    bool early = false;  // so may the loads made early in it
+    int read = 0;  // slot that is multiplied next
     for (int t = mine; t < last; t += stride) {
         const half8_t one = unit_operand((half_t)1.f);
 #pragma unroll
@@ -775,12 +775,7 @@ __global__ __launch_bounds__(256, 2) void ks_gated_ring_kernel(GatedArgs g, int 
                     }
                 }
         for (int s = 0; s < steps; ++s) {
-            const bool st = s < C::ST - 1 && after > 0, ea = s > steps - C::ST + 1 || (s == 0 && early);
-            if (st && ea)
-                __builtin_amdgcn_s_waitcnt(vmcnt_imm(C::WAIT + C::STORES + C::EARLY));
-            else if (st)
-                __builtin_amdgcn_s_waitcnt(vmcnt_imm(C::WAIT + C::STORES));
-            else if (ea)
+            if (s > steps - C::ST + 1)
                 __builtin_amdgcn_s_waitcnt(vmcnt_imm(C::WAIT + C::EARLY));
             else
                 __builtin_amdgcn_s_waitcnt(vmcnt_imm(C::WAIT));
@@ -829,8 +824,7 @@ __global__ __launch_bounds__(256, 2) void ks_gated_ring_kernel(GatedArgs g, int 
                             acc[p][q][i][j] = LAST ? op<half_t>::mfma(fx[p][j], fw, acc[p][q][i][j]) : op<half_t>::mfma(fw, fx[p][j], acc[p][q][i][j]);
                     }
         }
-        after = finish(t) ? 1 : 0;
-        early = true;
+        finish(t);
     }
     __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));  // repeated loads land before LDS goes to someone else
 }
