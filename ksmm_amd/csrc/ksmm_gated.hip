@@ -72,8 +72,8 @@ template <typename T, int ACT, bool SLOPE> __device__ __forceinline__ float acti
     return z;
 }
 
-// one branch on the activation around all of a tile's values
-template <typename F> __device__ __forceinline__ void with_act(int act, F f)
+// one branch on the activation: around all of a tile's values, or around the launch
+template <typename F> __host__ __device__ __forceinline__ void with_act(int act, F f)
 {
     if (act == KSMM_ACT_SILU)
         f(std::integral_constant<int, KSMM_ACT_SILU>());
@@ -477,9 +477,13 @@ __global__ __launch_bounds__(64 * WB *WN, 2) void ks_gated_kernel(GatedArgs g, i
 // The sums start at the bias: one product of (bias, 0, ..) and (1, 0, ..).  Results go through 4 KB of LDS a wave, and
 // leave as rows of 128 bytes.
 //
-// (1,768,192,2), 25088 rows forward 53 us: 29.6 GFLOP at 556 TFLOP/s; 96 MB of x and h, 1.8 TB/s.  The matrix cores are busy for 27 %
+// A kernel an activation: with a branch on it inside, MODE 1 with 128 outputs of one d_i or 64 of two spills 21 to 34 registers a lane
+// around its stores, and the number of one activation's registers costs the others time ((1,768,192,2), 25088 rows, a
+// training pass 285 us; in one kernel 314, and 301 while GELU had a coefficient less).
+//
+// (1,768,192,2), 25088 rows forward 52 us: 29.6 GFLOP at 566 TFLOP/s; 96 MB of x and h, 1.9 TB/s.  The matrix cores are busy for 27 %
 // of the SIMDs' time: what is left is the wait at each tile's head, and the vector ALU's work on the results, which the other
-// workgroup's products cover in part.  MODE 1 with 128 outputs of one d_i or 64 of two spills 24 to 34 registers a lane, around its stores.
+// workgroup's products cover in part.
 constexpr int vmcnt_imm(int n) { return (n & 15) | (7 << 4) | (15 << 8) | (((n >> 4) & 3) << 14); }
 typedef __attribute__((address_space(3))) unsigned char *lds_bytes_t;
 
@@ -521,7 +525,7 @@ template <bool LAST, int CPR> __device__ __forceinline__ int x_swizzle(int row, 
 }
 template <int CPR> __device__ __forceinline__ int o_swizzle(int row, int cc) { return cc ^ (CPR == 8 ? (row >> 1) & 7 : (row >> 2) & 3); }
 
-template <bool LAST, int D, int TB, int MODE>
+template <bool LAST, int D, int TB, int MODE, int ACT>
 __global__ __launch_bounds__(256, 2) void ks_gated_ring_kernel(GatedArgs g, int b_tiles, int tiles)
 {
     typedef Ring<LAST, D, TB, MODE> C;
@@ -690,66 +694,63 @@ __global__ __launch_bounds__(256, 2) void ks_gated_ring_kernel(GatedArgs g, int 
     float16_t acc[D][C::PARTS][C::BT][C::NT];
     auto finish = [&](int t) {
         const At p = at(t);
-        with_act(g.act, [&](auto act_of) {
-            constexpr int ACT = decltype(act_of)::value;
 #pragma unroll
-            for (int u = 0; u < C::UNITS; ++u) {
-                if constexpr (MODE == 1) {
+        for (int u = 0; u < C::UNITS; ++u) {
+            if constexpr (MODE == 1) {
 #pragma unroll
-                    for (int i = 0; i < C::O_IT; ++i) {
-                        const int row = i * O_STEP + o_row;
-                        *(uint4_t *)(piece + row * (C::O_CPR * 16) + o_swizzle<C::O_CPR>(row, o_cc) * 16) = dhv[i];
-                    }
-                    if (u + 1 < C::UNITS) load_dh(p, u + 1);
-                    wave_sync();
+                for (int i = 0; i < C::O_IT; ++i) {
+                    const int row = i * O_STEP + o_row;
+                    *(uint4_t *)(piece + row * (C::O_CPR * 16) + o_swizzle<C::O_CPR>(row, o_cc) * 16) = dhv[i];
                 }
-                // the lane's values of the unit: chunks of 8
-                constexpr int CHUNKS = LAST ? 4 : C::BT * D;
-                Run<half_t, 8> r1[MODE ? CHUNKS : 1];
-#pragma unroll
-                for (int k = 0; k < CHUNKS; ++k) {
-                    // LAST: j = k / 2, values 8 * (k % 2) ..; else tile i = k / D, values 8 q .. of (8 outputs x D)
-                    const int q = LAST ? k / 2 * 4 + lq * 2 + k % 2 : (k / D * 2 + lq) * D + k % D;
-                    Run<half_t, 8> in, r0;
-                    if constexpr (MODE == 1) in = __builtin_bit_cast(Run<half_t, 8>, *mine_at(q));
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        const int m = LAST ? k % 2 * 8 + e : (k % D * 8 + e) / D, pl = LAST ? 0 : (k % D * 8 + e) % D;
-                        const float gate = LAST ? acc[0][0][u % C::BT][k / 2 % C::NT][m] : acc[pl][0][k / D % C::BT][u % C::NT][m];
-                        const float up = LAST ? acc[0][C::PARTS - 1][u % C::BT][k / 2 % C::NT][m] : acc[pl][0][k / D % C::BT][u % C::NT][8 + m];
-                        float slope = 0.f;
-                        const float v = activate<half_t, ACT, MODE == 1>(gate, slope);
-                        if constexpr (MODE == 0) {
-                            r0.e[e] = (half_t)(v * up);
-                        } else {
-                            const float f = (float)in.e[e];
-                            r0.e[e] = (half_t)(f * up * slope);
-                            r1[MODE ? k : 0].e[e] = (half_t)(f * v);
-                        }
-                    }
-                    *mine_at(q) = __builtin_bit_cast(uint4_t, r0);
-                }
-#pragma unroll
-                for (int part = 0; part <= MODE; ++part) {
-                    if (part == 1) {
-#pragma unroll
-                        for (int k = 0; k < CHUNKS; ++k) {
-                            const int q = LAST ? k / 2 * 4 + lq * 2 + k % 2 : (k / D * 2 + lq) * D + k % D;
-                            *mine_at(q) = __builtin_bit_cast(uint4_t, r1[MODE ? k : 0]);
-                        }
-                    }
-                    wave_sync();
-#pragma unroll
-                    for (int i = 0; i < C::O_IT; ++i) {
-                        const int row = i * O_STEP + o_row;
-                        const uint4_t v = *(const uint4_t *)(piece + row * (C::O_CPR * 16) + o_swizzle<C::O_CPR>(row, o_cc) * 16);
-                        int64_t k;
-                        if (place(p, u, row, MODE + 1, part, &k)) *(uint4_t *)(out + k) = v;
-                    }
-                    wave_sync();
-                }
+                if (u + 1 < C::UNITS) load_dh(p, u + 1);
+                wave_sync();
             }
-        });
+            // the lane's values of the unit: chunks of 8
+            constexpr int CHUNKS = LAST ? 4 : C::BT * D;
+            Run<half_t, 8> r1[MODE ? CHUNKS : 1];
+#pragma unroll
+            for (int k = 0; k < CHUNKS; ++k) {
+                // LAST: j = k / 2, values 8 * (k % 2) ..; else tile i = k / D, values 8 q .. of (8 outputs x D)
+                const int q = LAST ? k / 2 * 4 + lq * 2 + k % 2 : (k / D * 2 + lq) * D + k % D;
+                Run<half_t, 8> in, r0;
+                if constexpr (MODE == 1) in = __builtin_bit_cast(Run<half_t, 8>, *mine_at(q));
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const int m = LAST ? k % 2 * 8 + e : (k % D * 8 + e) / D, pl = LAST ? 0 : (k % D * 8 + e) % D;
+                    const float gate = LAST ? acc[0][0][u % C::BT][k / 2 % C::NT][m] : acc[pl][0][k / D % C::BT][u % C::NT][m];
+                    const float up = LAST ? acc[0][C::PARTS - 1][u % C::BT][k / 2 % C::NT][m] : acc[pl][0][k / D % C::BT][u % C::NT][8 + m];
+                    float slope = 0.f;
+                    const float v = activate<half_t, ACT, MODE == 1>(gate, slope);
+                    if constexpr (MODE == 0) {
+                        r0.e[e] = (half_t)(v * up);
+                    } else {
+                        const float f = (float)in.e[e];
+                        r0.e[e] = (half_t)(f * up * slope);
+                        r1[MODE ? k : 0].e[e] = (half_t)(f * v);
+                    }
+                }
+                *mine_at(q) = __builtin_bit_cast(uint4_t, r0);
+            }
+#pragma unroll
+            for (int part = 0; part <= MODE; ++part) {
+                if (part == 1) {
+#pragma unroll
+                    for (int k = 0; k < CHUNKS; ++k) {
+                        const int q = LAST ? k / 2 * 4 + lq * 2 + k % 2 : (k / D * 2 + lq) * D + k % D;
+                        *mine_at(q) = __builtin_bit_cast(uint4_t, r1[MODE ? k : 0]);
+                    }
+                }
+                wave_sync();
+#pragma unroll
+                for (int i = 0; i < C::O_IT; ++i) {
+                    const int row = i * O_STEP + o_row;
+                    const uint4_t v = *(const uint4_t *)(piece + row * (C::O_CPR * 16) + o_swizzle<C::O_CPR>(row, o_cc) * 16);
+                    int64_t k;
+                    if (place(p, u, row, MODE + 1, part, &k)) *(uint4_t *)(out + k) = v;
+                }
+                wave_sync();
+            }
+        }
     };
 
     begin_loads();
@@ -932,12 +933,16 @@ template <bool LAST, int D, int TB, int MODE> int run_ring(const GatedArgs &g, h
     const int b_tiles = (g.b + TB - 1) / TB;
     const int64_t tiles = (int64_t)b_tiles * g.a * (LAST ? g.d : 1) * ((g.batch + C::TN - 1) / C::TN);
     if (tiles > 0x7ffffff0LL) return KSMM_ERR_TOO_LARGE;
-    const auto fn = &ks_gated_ring_kernel<LAST, D, TB, MODE>;
-    const int rc = ensure_dynamic_lds((const void *)fn, C::LDS_BYTES);
-    if (rc != KSMM_OK) return rc;
     const int64_t grid = std::min<int64_t>(512, (tiles + 7) / 8 * 8);  // two workgroups a CU
-    hipLaunchKernelGGL(fn, dim3((unsigned)grid), dim3(C::THREADS), C::LDS_BYTES, s, g, b_tiles, (int)tiles);
-    return launched();
+    int rc = KSMM_OK;
+    with_act(g.act, [&](auto act_of) {
+        const auto fn = &ks_gated_ring_kernel<LAST, D, TB, MODE, decltype(act_of)::value>;
+        rc = ensure_dynamic_lds((const void *)fn, C::LDS_BYTES);
+        if (rc != KSMM_OK) return;
+        hipLaunchKernelGGL(fn, dim3((unsigned)grid), dim3(C::THREADS), C::LDS_BYTES, s, g, b_tiles, (int)tiles);
+        rc = launched();
+    });
+    return rc;
 }
 // vectors of 16 bytes everywhere, and offsets inside a tile that fit 32 bits
 bool ring_ok(const GatedArgs &g, bool last)
