@@ -318,15 +318,17 @@ int ksmm_chain_forward_static(const ksmm_factor_desc *factors, int n_factors, co
 
 /* ---- operators around a Kronecker-sparse feed-forward block (fp32 and fp16) -----------------------
  * All of them launch on the caller's stream, allocate nothing, keep nothing, and compute in fp32; results are
- * rounded once.  Every pointer needs the alignment of its elements only; workspaces 16 bytes.  Tensors written
- * must not overlap those read unless said so (KSMM_ERR_ALIAS). */
+ * rounded once.  What is held in fewer bits on the way is named below.  Every pointer needs the alignment of its elements only;
+ * workspaces 16 bytes.  What is written (results, statistics, workspaces) must not overlap what is read, nor each other, unless
+ * said so (KSMM_ERR_ALIAS). */
 
 /* Gated projection: two factors of one pattern (a, b, c, d) that share their input x,
  *     h = act(G x + bias_g) * (U x + bias_u)
  * w holds both side by side, (a*d*c, 2*b), gate columns first: the kernel-format weights of ONE factor with pattern
  * (a, 2b, c, d).  bias (NULL: none) has that factor's 2*a*b*d output features; h has a*b*d.  act: any ksmm_act.
  * The backward pass computes the projections again from x, and writes what is not NULL of dx (x's shape), dw (w's)
- * and dbias (bias's).  Tensors of 2^31 elements and more (2*a*b*d x batch among them) are refused.
+ * and dbias (bias's).  The gradient of the projections themselves lies in the workspace in `dtype`: in fp16 it is rounded before the
+ * three sums over it, and an infinity beyond 65504.  Tensors of 2^31 elements and more (2*a*b*d x batch among them) are refused.
  * dw and dbias are sums in a fixed order: the same bits on every call. */
 int ksmm_gated_forward(const void *x, const void *w, const void *bias, void *h, int64_t batch, int a, int b,
                        int c, int d, int dtype, int bs_last, int act, void *stream);

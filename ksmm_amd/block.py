@@ -144,7 +144,9 @@ def gated_linear(x, factor, pattern, bias=None, act="silu", bs_last=False):
     (``pack_gated``); ``bias`` 2*a*b*d values, for each of the ``a`` groups those of the gate, then those of up.
     ``x`` has a*c*d features, in the last axis, or with ``bs_last`` in the first, like the result's a*b*d.
     ``act``: "silu", "gelu" (erf form) or None.  Gradients of all three go through one call that computes
-    the projections again instead of keeping them; they cannot be differentiated a second time."""
+    the projections again instead of keeping them; they cannot be differentiated a second time.  The gradients of the
+    projections, which those three are sums of, are held in the tensors' type: in fp16 they are rounded once before the sums, and are
+    infinities beyond 65504, as between two fp16 layers.  Who needs more than that passes fp32 tensors."""
     out = _lib.native().gated_linear(x, factor, pattern, bias, act, bs_last)
     if out is not None:
         return out

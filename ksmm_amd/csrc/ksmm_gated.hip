@@ -8,7 +8,10 @@
 // with pattern (a, 2b, c, d), which is what the gradients of input and weights run as, on the kernels that any factor
 // has.  z itself never reaches memory on the way forward; backward it is computed again, and
 //     dz[0] = dh * z1 * act'(z0),  dz[1] = dh * act(z0)
-// leave the kernel in its place (MODE 1).  Sums are fp32; h and dz are rounded once, from fp32.
+// leave the kernel in its place (MODE 1).  Sums are fp32; h is rounded once, from fp32.  So is dz, and the gradients, sums over it, once
+// more: dz in the tensors' type is what the 16-bit matrix instructions take.  In fp16 that costs gradients 2.9e-4 in the 2-norm for
+// 2.1e-4 of the last rounding alone, and the range of the type, as the same layers apart would; a training pass over
+// (1,768,192,2), 25088 rows, is 285 us, and in fp32, where dz has 32 bits, 1340.
 //
 // An MFMA tile has 32 rows of weights.  Batch-size-first these are 16 gate and 16 up columns of the same outputs, dealt
 // so that a lane (which holds rows 8j + 4*(lane/32) + i) has gate and up of 8 outputs in a row: the product needs no

@@ -72,3 +72,22 @@ def test_every_gradient_of_the_gate(n, b, bs_last, act):
     got = (g[0] if bs_last else g[:, 0]).cpu()
     off = (got.double() - want).abs() - 2 ** -22 * scale
     assert (fp16_steps(want + off.clamp_min(0), want) <= 1).all()
+
+
+@pytest.mark.parametrize("n,b,bs_last", SHAPES[:6])
+def test_gradients_of_the_projections_beyond_the_type_are_seen(n, b, bs_last):
+    """The gradients of both projections are held in the tensors' type on their way to the sums: one beyond the largest fp16 number is
+    an infinity, in every gradient that it goes into and in no other.  (Mixed-precision training scales the loss by that.)"""
+    from ksmm_amd import gated_linear
+
+    x, w, dh = torch.zeros(n, 64), torch.zeros(64, 2 * b), torch.zeros(n, b)
+    x[:, 0], x[:, 1] = 4.0, 1.0
+    w[0, :b], w[1, b:] = 1.0, 1000.0
+    dh[:, 3], dh[n // 2, 3] = 1.0, 100.0  # dz of the gate: 1.05e3, and 1.05e5
+    x, dh = ((t.t() if bs_last else t).contiguous().half().cuda() for t in (x, dh))
+    leaves = [x.requires_grad_(), w.half().cuda().requires_grad_()]
+    with torch.enable_grad():
+        dx, dw = torch.autograd.grad(gated_linear(*leaves, (1, b, 64, 1), bs_last=bs_last), leaves, dh)
+    dx = dx.t() if bs_last else dx
+    assert not dx[n // 2, 0].isfinite() and dx[:n // 2].isfinite().all() and dx[n // 2 + 1:].isfinite().all()
+    assert not dw[0, 3].isfinite() and dw[:, :3].isfinite().all() and dw[:, 4:].isfinite().all()
