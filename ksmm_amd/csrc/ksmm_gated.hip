@@ -157,14 +157,15 @@ template <typename T, int N> __device__ __forceinline__ Run<T, N> load_run(const
     }
     return r;
 }
-template <typename T, int N> __device__ __forceinline__ void store_run(T *p, int count, const Run<T, N> &r)
+// elements from `first` on (all of them in one or more 16-byte stores)
+template <typename T, int N> __device__ __forceinline__ void store_run(T *p, int first, const Run<T, N> &r)
 {
-    if (count >= N) {
+    if (first <= 0) {
         __builtin_memcpy(p, &r, sizeof(r));
     } else {
 #pragma unroll
         for (int e = 0; e < N; ++e)
-            if (e < count) p[e] = r.e[e];
+            if (e >= first) p[e] = r.e[e];
     }
 }
 
@@ -174,7 +175,9 @@ template <typename T, int N> __device__ __forceinline__ void store_run(T *p, int
 // values of a row, the E k of D neighbouring d_i, and writes them as D chunks of one d_i each (ALL: D is all of d, and
 // these values lie in a row).
 // Vectors that would cross the end of a row of weights, or of a batch-size-last row, are moved back to end with it, and
-// so are their results: some outputs are computed, and stored, twice, the same.  (b >= 8, batch-size-last batch >= 16.)
+// so are their results: some outputs are computed twice.  They are stored once, by the vector that they were in before: the compiler
+// rounds products of different places in a lane in different ways (to fp16 through fp32, or at once), and what would remain of two
+// stores is whichever comes last.  (b >= 8, batch-size-last batch >= 16.)
 template <typename T, bool LAST, int D, int TB, int TN, int TK, int WB, int WN> struct Tile {
     static constexpr int THREADS = 64 * WB * WN, E = EPV<T>;
     static constexpr int BT = TB / WB / (LAST ? 32 : 16), NT = TN / WN / 32;  // MFMA tiles a wave: outputs (16, or 32 as gate and up), rows
@@ -287,12 +290,14 @@ __global__ __launch_bounds__(64 * WB *WN, 2) void ks_gated_kernel(GatedArgs g, i
     constexpr int PARTS = LAST ? 2 : 1;  // accumulators an output tile: gate and up apart, or both in one
     float16_t acc[D][PARTS][C::BT][C::NT];
     const T *const bias = (const T *)g.bias;
-    // the lane's outputs of tile i: a run of 8 (E at a time, each moved back on its own), or one
+    // the lane's outputs of tile i: a run of 8 (E at a time, each moved back on its own), or one; and by how much they were moved
     auto run_at = [&](int i, int e) { return min(b0 + (wb * C::BT + i) * 16 + 8 * lq + e, b - E); };
+    auto run_moved = [&](int i, int e) { return b0 + (wb * C::BT + i) * 16 + 8 * lq + e - run_at(i, e); };
     auto one_at = [&](int i) {
         const int at = b0 + (wb * C::BT + i) * 32 + l32 / E * E;
         return min(at, b - E) + l32 % E;
     };
+    auto one_moved = [&](int i) { return b0 + (wb * C::BT + i) * 32 + l32 - one_at(i); };
     // the sums start at the bias: its loads go out before those of the first slab
     constexpr int BIAS = LAST ? 1 : 8 * D;
     T bv[2][C::BT][BIAS];
@@ -388,10 +393,12 @@ __global__ __launch_bounds__(64 * WB *WN, 2) void ks_gated_kernel(GatedArgs g, i
     const T *const dh = (const T *)g.dh;
     T *const out = (T *)g.out;
     const int64_t out_size = (int64_t)a * b * d;
-    with_act(g.act, [&](auto act_of) {
+    // (nearly all tiles have no vector that was moved: one branch around everything, where one at each vector took 2 to 23 % of a call)
+    auto finish_tile = [&](auto act_of, auto moved_of) {
         constexpr int ACT = decltype(act_of)::value;
-        // N values of gate and up (and of dh) at a time: a vector of the result
-        auto finish = [&](auto zg, auto zu, const T *dh_at, T *to_g, T *to_u, auto count) {
+        constexpr bool MOVED = decltype(moved_of)::value;
+        // N values of gate and up (and of dh) at a time: a vector of the result, stored from element `first` on
+        auto finish = [&](auto zg, auto zu, const T *dh_at, T *to_g, T *to_u, int first, auto count) {
             constexpr int N = decltype(count)::value;
             Run<T, N> in, r0, r1;
             if constexpr (MODE == 1) in = load_run<T, N>(dh_at, N);
@@ -408,14 +415,14 @@ __global__ __launch_bounds__(64 * WB *WN, 2) void ks_gated_kernel(GatedArgs g, i
                     r1.e[e] = (T)(t * v);
                 }
             }
-            store_run<T, N>(to_g, N, r0);
-            if constexpr (MODE == 1) store_run<T, N>(to_u, N, r1);
+            store_run<T, N>(to_g, first, r0);
+            if constexpr (MODE == 1) store_run<T, N>(to_u, first, r1);
         };
         if constexpr (LAST) {
             // a lane: one output, 16 rows of the batch in a row, E at a time
 #pragma unroll
             for (int i = 0; i < C::BT; ++i) {
-                if (b0 + (wb * C::BT + i) * 32 >= b) continue;
+                if (b0 + (wb * C::BT + i) * 32 >= b || (MOVED && l32 % E < one_moved(i))) continue;
                 const int64_t bi = one_at(i);
                 const int64_t fg = (a_i * 2 * (int64_t)b + bi) * d + d0, fh = (a_i * (int64_t)b + bi) * d + d0;
 #pragma unroll
@@ -426,7 +433,7 @@ __global__ __launch_bounds__(64 * WB *WN, 2) void ks_gated_kernel(GatedArgs g, i
                         if (at >= B) continue;
                         const int n = min(at, B - E);
                         finish([&](int e) { return acc[0][0][i][j][v + e]; }, [&](int e) { return acc[0][PARTS - 1][i][j][v + e]; },
-                               dh + fh * B + n, out + (MODE == 0 ? fh : fg) * B + n, out + (fg + (int64_t)b * d) * B + n,
+                               dh + fh * B + n, out + (MODE == 0 ? fh : fg) * B + n, out + (fg + (int64_t)b * d) * B + n, MOVED ? at - n : 0,
                                std::integral_constant<int, E>());
                     }
             }
@@ -449,19 +456,27 @@ __global__ __launch_bounds__(64 * WB *WN, 2) void ks_gated_kernel(GatedArgs g, i
                             for (int q = 0; q < D; ++q)  // vector q of the E * D values
                                 finish([&](int e) { return acc[(q * E + e) % D][0][i][j][h + (q * E + e) / D]; },
                                        [&](int e) { return acc[(q * E + e) % D][0][i][j][8 + h + (q * E + e) / D]; }, dh_n + fh + q * E,
-                                       out_n + fg + q * E, out_n + fg + (int64_t)b * D + q * E, std::integral_constant<int, E>());
+                                       out_n + fg + q * E, out_n + fg + (int64_t)b * D + q * E, MOVED ? run_moved(i, h) * D - q * E : 0,
+                                       std::integral_constant<int, E>());
                         }
                     } else {
 #pragma unroll
                         for (int h = 0; h < 8; ++h) {
+                            if (MOVED && h % E < run_moved(i, h / E * E)) continue;
                             const int64_t at = run_at(i, h / E * E) + h % E, fh = ((int64_t)a_i * b + at) * d, fg = fh + (int64_t)a_i * b * d * MODE;
                             finish([&](int e) { return acc[e][0][i][j][h]; }, [&](int e) { return acc[e][0][i][j][8 + h]; }, dh_n + fh,
-                                   out_n + fg, out_n + fg + (int64_t)b * d, std::integral_constant<int, D>());
+                                   out_n + fg, out_n + fg + (int64_t)b * d, 0, std::integral_constant<int, D>());
                         }
                     }
                 }
             }
         }
+    };
+    with_act(g.act, [&](auto act_of) {
+        if ((b0 + TB <= b || b % (LAST ? 32 : 8) == 0) && (!LAST || n0 + TN <= B || B % E == 0))
+            finish_tile(act_of, std::false_type());
+        else
+            finish_tile(act_of, std::true_type());
     });
 }
 
