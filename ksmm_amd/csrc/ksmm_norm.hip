@@ -83,11 +83,12 @@ template <int TPR> struct RowSum {
     }
 };
 
-// What a gradient dv of v = norm(t) leaves of itself: dv - v mean(dv v) - mean(dv), given the means.  (A row of one feature
-// has v^2 = 1 - eps rho^2 without a mean, which the difference would lose.)
+// What a gradient dv of v = norm(t) leaves of itself: dv - v mean(dv v) - mean(dv), given the means.  (A row of one feature has
+// v^2 = 1 - eps rho^2, and so have both of a row of two behind a mean: what is left is that part of dv, which the
+// difference would lose.)
 __device__ __forceinline__ float project(const NormArgs &a, float dv, float v, float m1, float m2, float rho)
 {
-    return a.features == 1 && !a.layer ? dv * (a.eps * rho * rho) : fmaf(-v, m2, dv) - m1;
+    return a.features == (a.layer ? 2 : 1) ? (dv - m1) * (a.eps * rho * rho) : fmaf(-v, m2, dv) - m1;
 }
 
 // ---- E elements of a row, at element alignment; past its end: zeros, and nothing stored ------------
