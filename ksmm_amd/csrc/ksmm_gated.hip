@@ -499,7 +499,7 @@ __global__ __launch_bounds__(64 * WB *WN, 2) void ks_gated_kernel(GatedArgs g, i
 // around its stores, and the number of one activation's registers costs the others time ((1,768,192,2), 25088 rows, a
 // training pass 285 us; in one kernel 314, and 301 while GELU had a coefficient less).
 //
-// (1,768,192,2), 25088 rows forward 52 us: 29.6 GFLOP at 566 TFLOP/s; 96 MB of x and h, 1.9 TB/s.  The matrix cores are busy for 27 %
+// (1,768,192,2), 25088 rows forward 52 us: 29.6 GFLOP at 566 TFLOP/s; 96 MB of x and h, 1.9 TB/s.  The matrix cores are busy for 31 %
 // of the SIMDs' time: what is left is the wait at each tile's head, and the vector ALU's work on the results, which the other
 // workgroup's products cover in part.
 constexpr int vmcnt_imm(int n) { return (n & 15) | (7 << 4) | (15 << 8) | (((n >> 4) & 3) << 14); }
@@ -985,7 +985,7 @@ template <typename T, bool LAST> bool few(const GatedArgs &g)
 }
 
 // Everything else: the ring where it can run, and the tile that goes through registers.  fp16 (1,768,192,2), 25088 rows, ring/tile:
-// 62/82 us forward, 242/262 backward (all of it), batch-size-last 54/71 and 232/260; with few tiles they are level
+// 61/73 us forward, 213/243 backward (all of it), batch-size-last 51/58 and 183/214; with few tiles they are level
 // ((1,768,192,1) 3136 rows 8.3/8.2).  Weight tiles of the ring: 128 outputs halve the reads of x ((1,768,192,1), 25088 rows
 // 29.6 us for 34.8; batch-size-last (1,768,192,2) 12544 rows, 1176 tiles, 28.4 for 32.3), 64 spread better
 // (6272 rows, 588 tiles, 17.2 for 18.3; (1,768,192,1) 1576 rows 6.9 for 8.9) and waste less of a b of 64 (12.6 for 17.3).

@@ -95,8 +95,10 @@ __device__ __forceinline__ void split(float v, half_t &hi, half_t &lo)
 // ---- blocks that fit LDS -------------------------------------------------------------------------------
 // X and its Gram matrix (which the polynomial replaces) in LDS, hi and lo apart, sides padded to 32 with zeros; tiles of
 // 16 x 16 are dealt to the waves.  G and Q are symmetric: upper tiles only, and both operands of G G are rows.  Few of these
-// matrices fill no chip: what counts is the latency of fifteen products in a row.
-// (6,64,64,1) 17.7 us, (1,128,128,3) 70 (on 32-bit instructions 28 and 133).
+// matrices fill no chip: what counts is the latency of fifteen products in a row, and for blocks that fill LDS its reads, 4 KB for
+// three instructions (128 x 128: 11 MB in five steps, 36 us at 128 bytes a clock).
+// (6,64,64,1) 17.7 us, (1,128,128,3) 70, with momentum and weights 74 (on 32-bit instructions 28 and 133).  Blocks of more than 64
+// tiles (8 a wave) spill 90 registers a thread.
 __host__ __device__ constexpr int up16(int v) { return (v + 15) / 16 * 16; }
 __host__ __device__ constexpr int up32(int v) { return (v + 31) / 32 * 32; }
 __host__ __device__ constexpr int64_t block_lds(int m, int n)

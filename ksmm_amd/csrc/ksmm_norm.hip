@@ -1204,8 +1204,9 @@ template <int E, int TPR, int VPL> struct Rows {
 };
 // The kernel that holds a row in the fewest values a thread (8 to 16): fp16 768 features in 12 a lane, 3 pieces of 8 bytes,
 // are 54 us backward with both norms, in 2 pieces of 16 bytes, a third of them empty, 152.  Rates, forward/backward with both
-// norms, TB/s: 768 x 25088 in fp16 4.2/3.7, 4096 x 8192 5.0/3.5, 8192 x 4096 3.5/3.3.  Above 8192 features a thread's values
-// spill (16384 x 2048 3.7/1.5, in fp32 1.7/0.7): such rows are served, not tuned.
+// norms, TB/s: 768 x 25088 in fp16 4.2/3.7, 4096 x 8192 5.0/3.5, 8192 x 4096 3.5/3.3.  1024 threads have 128 registers each: the
+// backward pass spills 37 to 70 of them a thread in fp32 above 4096 features, and 15 to 33 in fp16 there where 8 does not divide the row; above
+// 8192 both passes do (16384 x 2048 3.7/1.5, in fp32 1.7/0.7): such rows are served, not tuned.
 template <typename T, typename F> int with_rows(int64_t features, F f)
 {
     constexpr int E = 16 / (int)sizeof(T);
