@@ -388,6 +388,66 @@ int ksmm_muon_update(const ksmm_muon_desc *desc, const void *grad, const float *
                      const void *weight, const float *master, float *master_out, void *out, void *workspace,
                      int64_t workspace_bytes, int64_t blocks, int c, int b, int parts, int dtype, void *stream);
 
+/* ---- microscaled 4-bit numbers ----------------------------------------------------------------------
+ * An operand of the product, x (rows x a*c*d features, or a*c*d x rows with bs_last) as e2m1 codes: for each block of 32
+ * consecutive c_i (the last one of a row filled with zeros) a scale 2^e, e = max(floor(log2 max |x|) - 2, -120), as the byte
+ * e + 127, and codes of x / 2^e, rounded to the nearest, ties to the even code, at most 6.  A block that holds an infinity or a
+ * NaN has the byte 255: all of its values are NaN.
+ *   codes   (a*d, rows, 16 * ceil(c / 32)) bytes, the even c_i in the lower half of a byte; 16-byte aligned
+ *   scales  (a*d, rows, ceil(c / 32)) bytes
+ * ksmm_mx_blocks is how many scales that is.  Weights in kernel format (a*d*c, b) are such an operand of b rows, with a*d in
+ * the place of a, 1 in that of d, and bs_last.  Everything launches on the caller's stream, allocates nothing and keeps nothing;
+ * what is written must not overlap what is read. */
+int64_t ksmm_mx_blocks(int64_t rows, int a, int c, int d);
+int ksmm_mx_quantize(const void *x, void *codes, void *scales, int64_t rows, int a, int c, int d, int dtype,
+                     int bs_last, void *stream);
+/* The values that codes stand for, rounded to `dtype` (fp16: what is below 6e-8 or beyond 65504 of them). */
+int ksmm_mx_dequantize(const void *codes, const void *scales, void *x, int64_t rows, int a, int c, int d, int dtype,
+                       int bs_last, void *stream);
+/* y = act(W x + bias), W of b rows a block, or with `gated` act(G x + bias_g) * (U x + bias_u), W of 2*b rows a block, G's first,
+ * and a bias of 2*a*b*d values as for ksmm_gated_forward.  x_scales NULL: x has `dtype` and is quantised in the call; else x and
+ * x_scales are an operand of `batch` rows.  Sums are fp32; y and bias have `dtype`.  act: KSMM_ACT_SILU with `gated` only.
+ * Needs ksmm_mx_forward_workspace() bytes of 16-byte aligned device memory where x_scales is NULL (0: none). */
+int64_t ksmm_mx_forward_workspace(int64_t batch, int a, int b, int c, int d, int dtype, int bs_last, int gated);
+int ksmm_mx_forward(const void *x, const void *x_scales, const void *w, const void *w_scales, const void *bias, void *y,
+                    void *workspace, int64_t workspace_bytes, int64_t batch, int a, int b, int c, int d, int dtype,
+                    int bs_last, int act, int gated, void *stream);
+
+/* ---- AdamW over many tensors --------------------------------------------------------------------------
+ *     g = grad_scale * grad,  m' = beta1 m + (1 - beta1) g,  v' = beta2 v + (1 - beta2) g^2
+ *     w' = (1 - lr weight_decay) w - lr / (1 - beta1^t) * m' / (sqrt(v') / sqrt(1 - beta2^t) + eps)
+ * over all `count` tensors, in their place.  weight and grad have `dtype`.  master (for all of the tensors or for none): fp32 values
+ * that the weights are rounded from; follow: a weight that is not its master's rounding counts instead.  t is `step`, from 1 on,
+ * or *device_step (int64), which a captured graph reads anew on every replay.
+ * bits 32: m and v are fp32, scales is not read.  bits 8: bytes, and for each 32 consecutive values a power of two each, 2^(byte -
+ * 127), in scales (2, ceil(n / 32)), m's first.  m is e4m3fn behind 2^(floor(log2 max |m|) - 7), v an unsigned e5m3, the bits 14 to 7
+ * of an fp16 number, behind 2^(floor(log2 max v) - 14); exponents are -120 at least.  They are rounded down, or up with
+ * the probability of what is cut off, by a hash of seed + the tensor's number, step and place; v > 0 stays above zero.  Values beyond
+ * fp32 become NaN (m) or infinity (v), alone.  m and v of zeros with scales of any kind are a state to start from.
+ * What is written must not overlap anything else: no tensor may be there twice. */
+typedef struct ksmm_adamw_tensor {
+    void *weight;
+    const void *grad;
+    float *master; /* or NULL */
+    void *m, *v, *scales;
+    int64_t n;
+} ksmm_adamw_tensor;
+typedef struct ksmm_adamw_desc {
+    double lr, beta1, beta2, eps, weight_decay, grad_scale;
+    int64_t step;
+    const int64_t *device_step; /* or NULL */
+    uint32_t seed;
+    int bits, follow;
+} ksmm_adamw_desc;
+int ksmm_adamw_update(const ksmm_adamw_desc *desc, const ksmm_adamw_tensor *tensors, int count, int dtype, void *stream);
+/* What 8-bit moments stand for, as fp32. */
+typedef struct ksmm_adamw_moment {
+    const void *m, *v, *scales;
+    float *m_out, *v_out;
+    int64_t n;
+} ksmm_adamw_moment;
+int ksmm_adamw_moments(const ksmm_adamw_moment *tensors, int count, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -10,3 +10,6 @@ from .kernel import Kernel, query_tile  # noqa: F401
 from .block import (GatedKernel, KSFeedForward, KSGatedLinear, NormKernel, ResidualNorm, gated_linear,  # noqa: F401
                     pack_gated, residual_norm)
 from .muon import KSMuon, muon_update, orthogonalize  # noqa: F401
+from .mx import (KSFeedForwardMX, KSGatedLinearMX, KSLinearMX, MXFactor, MXKernel, MXLinear, MXTensor, mx_linear,  # noqa: F401
+                 pack_block, pack_mx, quantize_mx)
+from .adamw import KSAdamW, adamw_moments, adamw_update  # noqa: F401

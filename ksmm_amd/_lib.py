@@ -50,6 +50,20 @@ class KsmmMuonDesc(ctypes.Structure):
                 ("keep", ctypes.c_float), ("rate", ctypes.c_float), ("steps", c_int), ("nesterov", c_int), ("follow", c_int)]
 
 
+class KsmmAdamwTensor(ctypes.Structure):
+    _fields_ = [("weight", c_vp), ("grad", c_vp), ("master", c_vp), ("m", c_vp), ("v", c_vp), ("scales", c_vp), ("n", c_i64)]
+
+
+class KsmmAdamwDesc(ctypes.Structure):
+    _fields_ = [("lr", ctypes.c_double), ("beta1", ctypes.c_double), ("beta2", ctypes.c_double), ("eps", ctypes.c_double),
+                ("weight_decay", ctypes.c_double), ("grad_scale", ctypes.c_double), ("step", c_i64), ("device_step", c_vp),
+                ("seed", ctypes.c_uint32), ("bits", c_int), ("follow", c_int)]
+
+
+class KsmmAdamwMoment(ctypes.Structure):
+    _fields_ = [("m", c_vp), ("v", c_vp), ("scales", c_vp), ("m_out", c_vp), ("v_out", c_vp), ("n", c_i64)]
+
+
 # name -> (restype, argtypes); every symbol include/ksmm_hip.h declares
 SIGNATURES = {
     "ksmm_version": (c_int, []),
@@ -114,6 +128,14 @@ SIGNATURES = {
     "ksmm_muon_workspace": (c_i64, [c_i64, c_int, c_int, c_int]),
     "ksmm_muon_update": (c_int, [ctypes.POINTER(KsmmMuonDesc), c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_i64, c_i64,
                                  c_int, c_int, c_int, c_int, c_vp]),
+    "ksmm_mx_blocks": (c_i64, [c_i64, c_int, c_int, c_int]),
+    "ksmm_mx_quantize": (c_int, [c_vp, c_vp, c_vp, c_i64, c_int, c_int, c_int, c_int, c_int, c_vp]),
+    "ksmm_mx_dequantize": (c_int, [c_vp, c_vp, c_vp, c_i64, c_int, c_int, c_int, c_int, c_int, c_vp]),
+    "ksmm_mx_forward_workspace": (c_i64, [c_i64, c_int, c_int, c_int, c_int, c_int, c_int, c_int]),
+    "ksmm_mx_forward": (c_int, [c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_i64, c_i64, c_int, c_int, c_int, c_int, c_int, c_int,
+                                c_int, c_int, c_vp]),
+    "ksmm_adamw_update": (c_int, [ctypes.POINTER(KsmmAdamwDesc), ctypes.POINTER(KsmmAdamwTensor), c_int, c_int, c_vp]),
+    "ksmm_adamw_moments": (c_int, [ctypes.POINTER(KsmmAdamwMoment), c_int, c_vp]),
 }
 
 _lib = None

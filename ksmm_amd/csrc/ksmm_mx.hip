@@ -1,0 +1,291 @@
+// Kronecker-sparse products of microscaled 4-bit numbers (e2m1, blocks of 32 along c with a power of two in common).
+//
+//     xq[a_i, c_i, d_i, n] = 2^e rne(x / 2^e),  e = floor(log2 max |x| of the block) - 2
+//     y[a_i, b_i, d_i, n]  = act(sum_c Wq[a_i, b_i, c_i, d_i] xq[a_i, c_i, d_i, n] + bias[a_i, b_i, d_i])
+//
+// Operands are kept as the a*d matrices that the products take, (a*d, rows, c) with c in blocks of 32, the last one filled
+// with zeros: 16 bytes of codes a block, the even place in the lower half of a byte, and a byte of scale.  That is what a lane
+// of the scaled matrix instructions holds: 32 numbers of one row and their scale.
+#include "ksmm_act.h"
+#include "ksmm_mx.h"
+
+namespace ksmm {
+
+namespace {
+
+int launched() { return hipGetLastError() == hipSuccess ? KSMM_OK : KSMM_ERR_LAUNCH; }
+
+struct MxOperand {
+    const void *x;
+    uint8_t *codes, *scales;
+    int64_t rows;
+    int a, c, d, cb;
+    bool last;
+    int64_t blocks;  // a * d * rows * cb
+};
+
+// Where block i lies: its first value and the step between values of a row of c, and its place among the operand's blocks.
+// Consecutive i are consecutive in x as far as that goes.
+__device__ __forceinline__ void place(const MxOperand &p, int64_t i, int64_t *at, int64_t *step, int64_t *block, int *kb)
+{
+    int64_t n;
+    int ai, di;
+    if (p.last) {
+        n = i % p.rows;
+        i /= p.rows;
+        di = (int)(i % p.d);
+        i /= p.d;
+        *kb = (int)(i % p.cb);
+        ai = (int)(i / p.cb);
+        *step = (int64_t)p.d * p.rows;
+        *at = (((int64_t)ai * p.c + *kb * 32) * p.d + di) * p.rows + n;
+    } else {
+        di = (int)(i % p.d);
+        i /= p.d;
+        *kb = (int)(i % p.cb);
+        i /= p.cb;
+        ai = (int)(i % p.a);
+        n = i / p.a;
+        *step = p.d;
+        *at = ((n * p.a + ai) * p.c + *kb * 32) * p.d + di;
+    }
+    *block = (((int64_t)ai * p.d + di) * p.rows + n) * p.cb + *kb;
+}
+
+template <typename T> __global__ __launch_bounds__(256) void ks_mx_quantize_kernel(MxOperand p)
+{
+    for (int64_t i = blockIdx.x * 256LL + threadIdx.x; i < p.blocks; i += gridDim.x * 256LL) {
+        int64_t at, step, block;
+        int kb;
+        place(p, i, &at, &step, &block, &kb);
+        const int count = p.c - kb * 32;
+        const T *x = (const T *)p.x + at;
+        float v[4][8];
+        uint32_t top = 0;
+#pragma unroll
+        for (int k = 0; k < 32; ++k) {
+            v[k / 8][k % 8] = k < count ? (float)x[k * step] : 0.f;
+            const uint32_t bits = mx_bits(v[k / 8][k % 8]);
+            top = bits > top ? bits : top;
+        }
+        const int scale = mx_scale(top);
+        uint4_t code;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) code[q] = scale == MX_NAN ? 0 : mx_encode8(v[q], mx_power(scale));
+        *(uint4_t *)(p.codes + block * 16) = code;
+        p.scales[block] = (uint8_t)scale;
+    }
+}
+
+template <typename T> __global__ __launch_bounds__(256) void ks_mx_dequantize_kernel(MxOperand p)
+{
+    for (int64_t i = blockIdx.x * 256LL + threadIdx.x; i < p.blocks; i += gridDim.x * 256LL) {
+        int64_t at, step, block;
+        int kb;
+        place(p, i, &at, &step, &block, &kb);
+        const int count = p.c - kb * 32;
+        T *x = (T *)p.x + at;
+        const uint4_t code = *(const uint4_t *)(p.codes + block * 16);
+        const float power = mx_scale_value(p.scales[block]);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            float v[8];
+            mx_decode8(code[q], v);
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                if (q * 8 + k < count) x[(q * 8 + k) * step] = (T)(v[k] * power);
+        }
+    }
+}
+
+struct MxProduct {
+    const uint8_t *x, *x_scales, *w, *w_scales;
+    const void *bias;
+    void *y;
+    int64_t batch;
+    int a, b, c, d, cb;
+    int64_t tiles, token_tiles;
+    int b_tiles;
+};
+
+typedef int int8_v __attribute__((ext_vector_type(8)));
+
+// 32 numbers and their scale of row `row` (< rows, else zeros), block kb (< cb, else zeros)
+__device__ __forceinline__ int8_v mx_operand(const uint8_t *codes, const uint8_t *scales, int64_t row, bool there, int kb, int cb, int *scale)
+{
+    int8_v r = {0, 0, 0, 0, 0, 0, 0, 0};
+    *scale = 127;
+    if (there && kb < cb) {
+        const uint4_t v = *(const uint4_t *)(codes + (row * cb + kb) * 16);
+        r[0] = (int)v[0], r[1] = (int)v[1], r[2] = (int)v[2], r[3] = (int)v[3];
+        *scale = scales[row * cb + kb];
+    }
+    return r;
+}
+
+// A wave computes 32 outputs of 32 rows: row 8j + 4(lane / 32) + i of the tile is an output, column lane % 32 a row of the batch.
+template <typename T, bool LAST, bool GATED, int ACT> __global__ __launch_bounds__(256) void ks_mx_product_kernel(MxProduct p)
+{
+    const int lane = threadIdx.x & 63, l32 = lane & 31, half = lane >> 5;
+    const int64_t tile = blockIdx.x * 4LL + (threadIdx.x >> 6);
+    if (tile >= p.tiles) return;
+    const int bt = (int)(tile % p.b_tiles);
+    const int64_t nt = tile / p.b_tiles % p.token_tiles;
+    const int block = (int)(tile / p.b_tiles / p.token_tiles), ai = block / p.d, di = block % p.d;
+    const int rows_w = GATED ? 2 * p.b : p.b;
+    const int64_t n = nt * 32 + l32;
+    const int bi = bt * 32 + l32;
+    float16_t acc = {}, up = {};
+    for (int kb = half; kb - half < p.cb; kb += 2) {
+        int sx, sw, su;
+        const int8_v x = mx_operand(p.x, p.x_scales, (int64_t)block * p.batch + n, n < p.batch, kb, p.cb, &sx);
+        const int64_t row = (int64_t)block * rows_w + bi;
+        const int8_v w = mx_operand(p.w, p.w_scales, row, bi < p.b, kb, p.cb, &sw);
+        acc = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(w, x, acc, 4, 4, 0, sw, 0, sx);
+        if constexpr (GATED) {
+            const int8_v u = mx_operand(p.w, p.w_scales, row + p.b, bi < p.b, kb, p.cb, &su);
+            up = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(u, x, up, 4, 4, 0, su, 0, sx);
+        }
+    }
+    if (n >= p.batch) return;
+    const T *bias = (const T *)p.bias;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        const int o = bt * 32 + 8 * (i / 4) + 4 * half + (i & 3);
+        if (o >= p.b) continue;
+        float z = acc[i], slope;
+        if (bias) z += (float)bias[((int64_t)ai * rows_w + o) * p.d + di];
+        z = activate<T, ACT, false>(z, slope);
+        if constexpr (GATED) z *= up[i] + (bias ? (float)bias[((int64_t)ai * rows_w + p.b + o) * p.d + di] : 0.f);
+        const int64_t f = ((int64_t)ai * p.b + o) * p.d + di;
+        ((T *)p.y)[LAST ? f * p.batch + n : n * p.a * p.b * p.d + f] = (T)z;
+    }
+}
+
+template <typename T> int quantize(const MxOperand &p, bool back, hipStream_t s)
+{
+    const int64_t want = (p.blocks + 255) / 256;
+    const unsigned grid = (unsigned)(want < 65536 ? want : 65536);
+    if (back)
+        hipLaunchKernelGGL((ks_mx_dequantize_kernel<T>), dim3(grid), dim3(256), 0, s, p);
+    else
+        hipLaunchKernelGGL((ks_mx_quantize_kernel<T>), dim3(grid), dim3(256), 0, s, p);
+    return launched();
+}
+
+template <typename T, bool LAST, bool GATED> int product(const MxProduct &p, int act, hipStream_t s)
+{
+    const int64_t grid = (p.tiles + 3) / 4;
+    if (grid > 0x7fffffffLL) return KSMM_ERR_TOO_LARGE;
+    with_act(act, [&](auto which) {
+        hipLaunchKernelGGL((ks_mx_product_kernel<T, LAST, GATED, decltype(which)::value>), dim3((unsigned)grid), dim3(256), 0, s, p);
+    });
+    return launched();
+}
+template <typename T> int product(const MxProduct &p, bool last, bool gated, int act, hipStream_t s)
+{
+    if (last) return gated ? product<T, true, true>(p, act, s) : product<T, true, false>(p, act, s);
+    return gated ? product<T, false, true>(p, act, s) : product<T, false, false>(p, act, s);
+}
+
+// sizes of an operand; tensors of 2^31 elements and more are refused, and so are operands whose codes would take 2^35 bytes
+int check_operand(int64_t rows, int a, int c, int d, int dtype)
+{
+    if (dtype != KSMM_F32 && dtype != KSMM_F16) return KSMM_ERR_BAD_DTYPE;
+    return ksmm_validate(rows, a, 1, c, d, dtype, dtype, dtype, 0);
+}
+MxOperand operand(const void *x, void *codes, void *scales, int64_t rows, int a, int c, int d, int bs_last)
+{
+    const int cb = (int)mx_blocks(c);
+    return MxOperand{x, (uint8_t *)codes, (uint8_t *)scales, rows, a, c, d, cb, bs_last != 0, (int64_t)a * d * rows * cb};
+}
+int64_t values(int64_t rows, int a, int c, int d) { return rows * a * c * d; }
+int64_t align256(int64_t v) { return (v + 255) / 256 * 256; }
+
+}  // namespace
+
+}  // namespace ksmm
+
+using namespace ksmm;
+
+extern "C" {
+
+int64_t ksmm_mx_blocks(int64_t rows, int a, int c, int d)
+{
+    const int rc = check_operand(rows, a, c, d, KSMM_F16);
+    return rc != KSMM_OK ? rc : (int64_t)a * d * rows * mx_blocks(c);
+}
+
+static int convert(const void *x, const void *codes, const void *scales, int64_t rows, int a, int c, int d, int dtype, int bs_last,
+                   bool back, void *stream)
+{
+    const int rc = check_operand(rows, a, c, d, dtype);
+    if (rc != KSMM_OK) return rc;
+    if (!x || !codes || !scales) return KSMM_ERR_NULL_POINTER;
+    const MxOperand p = operand(x, (void *)codes, (void *)scales, rows, a, c, d, bs_last);
+    if (((uintptr_t)codes & 15) != 0) return KSMM_ERR_WORKSPACE;
+    const Span t[] = {{x, values(rows, a, c, d) * (int64_t)dtype_size(dtype)}}, q[] = {{codes, p.blocks * 16}, {scales, p.blocks}};
+    if (any_overlap(t, q) || overlaps(codes, p.blocks * 16, scales, p.blocks)) return KSMM_ERR_ALIAS;
+    return dtype == KSMM_F32 ? quantize<float>(p, back, (hipStream_t)stream) : quantize<half_t>(p, back, (hipStream_t)stream);
+}
+
+int ksmm_mx_quantize(const void *x, void *codes, void *scales, int64_t rows, int a, int c, int d, int dtype, int bs_last, void *stream)
+{
+    return convert(x, codes, scales, rows, a, c, d, dtype, bs_last, false, stream);
+}
+
+int ksmm_mx_dequantize(const void *codes, const void *scales, void *x, int64_t rows, int a, int c, int d, int dtype, int bs_last, void *stream)
+{
+    return convert(x, codes, scales, rows, a, c, d, dtype, bs_last, true, stream);
+}
+
+static int check_product(int64_t batch, int a, int b, int c, int d, int dtype, int act, int gated)
+{
+    if (dtype != KSMM_F32 && dtype != KSMM_F16) return KSMM_ERR_BAD_DTYPE;
+    if (b > 0x3fffffff || batch > 0x7fffff00) return KSMM_ERR_TOO_LARGE;
+    const int rc = ksmm_validate(batch, a, gated ? 2 * b : b, c, d, dtype, dtype, dtype, 0);
+    if (rc != KSMM_OK) return rc;
+    if (act != KSMM_ACT_NONE && act != KSMM_ACT_GELU && (act != KSMM_ACT_SILU || !gated)) return KSMM_ERR_BAD_EPILOGUE;
+    return KSMM_OK;
+}
+
+int64_t ksmm_mx_forward_workspace(int64_t batch, int a, int b, int c, int d, int dtype, int bs_last, int gated)
+{
+    const int rc = check_product(batch, a, b, c, d, dtype, KSMM_ACT_NONE, gated);
+    if (rc != KSMM_OK) return rc;
+    const int64_t blocks = (int64_t)a * d * batch * mx_blocks(c);
+    return align256(blocks * 16) + align256(blocks);
+}
+
+int ksmm_mx_forward(const void *x, const void *x_scales, const void *w, const void *w_scales, const void *bias, void *y, void *workspace,
+                    int64_t workspace_bytes, int64_t batch, int a, int b, int c, int d, int dtype, int bs_last, int act, int gated,
+                    void *stream)
+{
+    int rc = check_product(batch, a, b, c, d, dtype, act, gated);
+    if (rc != KSMM_OK) return rc;
+    if (!x || !w || !w_scales || !y) return KSMM_ERR_NULL_POINTER;
+    const int rows_w = gated ? 2 * b : b, cb = (int)mx_blocks(c);
+    const int64_t need = x_scales ? 0 : ksmm_mx_forward_workspace(batch, a, b, c, d, dtype, bs_last, gated);
+    if (((uintptr_t)w & 15) != 0 || (x_scales && ((uintptr_t)x & 15) != 0)) return KSMM_ERR_WORKSPACE;
+    if (need > 0 && (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15) != 0)) return KSMM_ERR_WORKSPACE;
+    const int64_t blocks = (int64_t)a * d * batch * cb, w_blocks = (int64_t)a * d * rows_w * cb, size = (int64_t)dtype_size(dtype);
+    const Span in[] = {{x, x_scales ? blocks * 16 : values(batch, a, c, d) * size}, {x_scales, blocks}, {w, w_blocks * 16}, {w_scales, w_blocks},
+                       {bias, (int64_t)a * rows_w * d * size}};
+    const Span out[] = {{y, values(batch, a, b, d) * size}, {need ? workspace : nullptr, need}};
+    if (any_overlap(in, out)) return KSMM_ERR_ALIAS;
+    MxProduct p{(const uint8_t *)x, (const uint8_t *)x_scales, (const uint8_t *)w, (const uint8_t *)w_scales, bias, y, batch, a, b, c, d, cb};
+    if (!x_scales) {
+        uint8_t *const codes = (uint8_t *)workspace, *const scales = codes + align256(blocks * 16);
+        rc = ksmm_mx_quantize(x, codes, scales, batch, a, c, d, dtype, bs_last, stream);
+        if (rc != KSMM_OK) return rc;
+        p.x = codes;
+        p.x_scales = scales;
+    }
+    p.b_tiles = (b + 31) / 32;
+    p.token_tiles = (batch + 31) / 32;
+    p.tiles = (int64_t)a * d * p.b_tiles * p.token_tiles;
+    return dtype == KSMM_F32 ? product<float>(p, bs_last != 0, gated != 0, act, (hipStream_t)stream)
+                             : product<half_t>(p, bs_last != 0, gated != 0, act, (hipStream_t)stream);
+}
+
+}  // extern "C"

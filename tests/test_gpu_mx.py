@@ -1,0 +1,386 @@
+"""Microscaled 4-bit numbers (quantize_mx, pack_mx, mx_linear and their modules) against the definitions in float64.
+
+Tolerances, relative Frobenius.  Codes and scales: equal.  Products: what the codes stand for is multiplied exactly (three bits by three)
+and summed in fp32; in order a sum of k terms is off by at most k 2^-24 of the sum of magnitudes, at random by sqrt(k) of it: 2e-6 for
+k up to 1024 with the fp32 activations' 1e-6.  fp16 results: the last rounding, 2^-11, or for a result below 6e-5 half of 6e-8: 4.9e-4.
+fp16 gradients of gated products: dz is rounded before the sums over it and they are once more, 2 * 2^-11 at most."""
+import pytest
+import torch
+
+from tests import mx_ref as R
+
+pytestmark = pytest.mark.gpu
+
+DT = {"fp32": torch.float32, "fp16": torch.float16}
+TOL = {"fp32": 2e-6, "fp16": 4.9e-4}
+
+
+def rel(x, y):
+    x, y = x.double().cpu(), y.double().cpu()
+    assert x.shape == y.shape
+    n = float(torch.linalg.vector_norm(y))
+    e = float(torch.linalg.vector_norm(x - y))
+    return e / n if n else e
+
+
+def rows(n, features, bs_last, dtype, seed=0, scale=1.0):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(n, features, generator=g) * scale * torch.exp2(torch.randint(-3, 4, (n, features), generator=g).float())
+    return (x.t() if bs_last else x).contiguous().to(dtype)
+
+
+def factor(pattern, gated, dtype, seed=1):
+    a, b, c, d = pattern
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(a * d * c, 2 * b if gated else b, generator=g) / c ** 0.5).to(dtype)
+
+
+def factor_rows(f, pattern):
+    """(a, d, rows, c)"""
+    a, _, c, d = pattern
+    return f.detach().cpu().reshape(a, d, c, -1).transpose(2, 3).contiguous()
+
+
+SIZES = [(1, 1, 1), (2, 31, 1), (1, 32, 1), (3, 33, 2), (1, 96, 5), (2, 64, 16), (1, 17, 40), (1, 200, 3), (4, 192, 1), (1, 256, 8), (1, 70, 64)]
+
+
+@pytest.mark.parametrize("bs_last", [False, True])
+@pytest.mark.parametrize("prec", ["fp32", "fp16"])
+@pytest.mark.parametrize("sizes", SIZES)
+def test_codes_and_scales(sizes, prec, bs_last):
+    from ksmm_amd import quantize_mx
+
+    a, c, d = sizes
+    for n in (1, 2, 31, 65, 200):
+        x = rows(n, a * c * d, bs_last, DT[prec], n)
+        q = quantize_mx(x.cuda(), sizes, bs_last)
+        code, scale = R.quantize(R.operand(x, a, c, d, bs_last).reshape(a * d, n, c))
+        assert q.codes.shape == (a * d, n, 16 * scale.shape[-1]) and q.scales.shape == scale.shape
+        assert torch.equal(q.scales.cpu().long(), scale)
+        got = R.unpacked(q.codes)
+        assert torch.equal(R.GRID[got & 7], R.GRID[code & 7]) and torch.equal(got >= 8, code >= 8)
+        back = R.tensor(R.values(code, scale, c).reshape(a, d, n, c), x.shape, bs_last)
+        assert torch.equal(q.dequantize().cpu(), back.to(DT[prec])) and q.dequantize().shape == x.shape
+        assert torch.equal(q.dequantize(torch.float32).cpu(), back.float())
+
+
+@pytest.mark.parametrize("bs_last", [False, True])
+def test_every_fp16_number_and_scale(bs_last):
+    """Each fp16 number as the largest of its block and beside each power of two above it."""
+    from ksmm_amd import quantize_mx
+
+    h = torch.arange(65536, dtype=torch.int32).to(torch.int16).view(torch.float16)
+    h = h[torch.isfinite(h)]
+    blocks = [torch.stack([h, torch.full_like(h, 2.0 ** e)], 1) for e in range(-24, 16, 3)] + [torch.stack([h, -h], 1)]
+    x = torch.cat(blocks)
+    x = x.t().contiguous() if bs_last else x
+    q = quantize_mx(x.cuda(), (1, 2, 1), bs_last)
+    code, scale = R.quantize(R.operand(x, 1, 2, 1, bs_last)[0])
+    assert torch.equal(q.scales.cpu().long(), scale)
+    back = R.tensor(R.values(code, scale, 2)[:, None], x.shape, bs_last)
+    assert torch.equal(q.dequantize(torch.float32).cpu().double(), back)
+
+
+@pytest.mark.parametrize("prec", ["fp32", "fp16"])
+@pytest.mark.parametrize("bs_last", [False, True])
+@pytest.mark.parametrize("sizes", [(1, 64, 1), (2, 40, 3), (1, 96, 2)])
+def test_infinities_and_nans_stay_in_their_block(sizes, bs_last, prec):
+    from ksmm_amd import quantize_mx
+
+    a, c, d = sizes
+    x = rows(9, a * c * d, False, DT[prec])
+    x[0, 5 * d], x[3, (c - 1) * d], x[4, 1] = float("inf"), float("nan"), -float("inf")
+    x = (x.t() if bs_last else x).contiguous()
+    q = quantize_mx(x.cuda(), sizes, bs_last)
+    code, scale = R.quantize(R.operand(x, a, c, d, bs_last))
+    assert (scale == 255).sum() == 3
+    assert torch.equal(q.scales.cpu().long().reshape(scale.shape), scale)
+    back = R.tensor(R.values(code, scale, c), x.shape, bs_last)
+    got = q.dequantize().cpu()
+    assert torch.equal(torch.isnan(got), torch.isnan(back))
+    assert torch.equal(torch.nan_to_num(got), torch.nan_to_num(back.to(DT[prec])))
+
+
+def test_ends_of_the_fp32_range():
+    from ksmm_amd import quantize_mx
+
+    x = torch.zeros(7, 32)
+    x[0, 0], x[1, 0], x[2, 0], x[3, 0], x[4, 0], x[5, 0] = 3.4e38, 2.0 ** -122, 2.0 ** -123, 1e-45, -(2.0 ** -119), 2.0 ** -126
+    q = quantize_mx(x.cuda(), (1, 32, 1))
+    code, scale = R.quantize(x)
+    assert torch.equal(q.scales.cpu().long()[0], scale)
+    assert torch.equal(q.dequantize().cpu().double(), R.values(code, scale, 32))
+
+
+PATTERNS = [(1, 1, 1, 1), (2, 5, 3, 2), (1, 32, 32, 1), (3, 33, 40, 1), (1, 64, 192, 2), (2, 20, 65, 3), (1, 100, 64, 6), (1, 16, 48, 16), (1, 130, 300, 4),
+            (6, 64, 64, 1), (1, 200, 1030, 1), (1, 8, 16, 37), (2, 96, 72, 3), (1, 48, 96, 64), (1, 768, 192, 2), (5, 34, 128, 8)]
+
+
+@pytest.mark.parametrize("bs_last", [False, True])
+@pytest.mark.parametrize("prec", ["fp32", "fp16"])
+@pytest.mark.parametrize("pattern", PATTERNS)
+def test_products(pattern, prec, bs_last):
+    from ksmm_amd import mx_linear, pack_mx, quantize_mx
+
+    a, b, c, d = pattern
+    for n, gated, act, with_bias in ((1, False, None, True), (2, True, "silu", False), (7, False, "gelu", True), (33, True, "gelu", True), (64, False, None, False),
+                                     (131, True, "silu", True), (200, True, None, False), (517, False, "gelu", False)):
+        x, f = rows(n, a * c * d, bs_last, DT[prec], n), factor(pattern, gated, DT[prec])
+        g = torch.Generator().manual_seed(2)
+        bias = (torch.randn(a * f.shape[1] * d, generator=g) * 0.1).to(DT[prec]) if with_bias else None
+        w = pack_mx(f.cuda(), pattern, gated)
+        code, scale = R.quantize(factor_rows(f, pattern).reshape(a * d, -1, c))
+        assert torch.equal(w.scales.cpu().long(), scale)
+        cuda_bias = None if bias is None else bias.cuda()
+        y = mx_linear(x.cuda(), w, bias=cuda_bias, act=act, bs_last=bs_last)
+        want = R.product(R.rounded(R.operand(x, a, c, d, bs_last)), R.rounded(factor_rows(f, pattern)), None if bias is None else bias.double(), pattern, act, gated,
+                         bs_last)
+        want = R.tensor(want, y.shape, bs_last)
+        assert y.dtype == DT[prec] and rel(y, want) <= TOL[prec], (n, gated, act)
+        # the same numbers, however they were made
+        q = quantize_mx(x.cuda(), (a, c, d), bs_last)
+        assert torch.equal(mx_linear(q, w, bias=cuda_bias, act=act, bs_last=bs_last), y)
+        assert torch.equal(mx_linear(x.cuda(), f.cuda(), pattern, bias=cuda_bias, act=act, gated=gated, bs_last=bs_last), y)
+
+
+@pytest.mark.parametrize("bs_last", [False, True])
+@pytest.mark.parametrize("prec", ["fp32", "fp16"])
+@pytest.mark.parametrize("pattern", [(1, 64, 192, 2), (3, 40, 33, 1), (1, 20, 64, 5)])
+def test_a_nan_stays_in_its_row(pattern, prec, bs_last):
+    from ksmm_amd import mx_linear, pack_mx
+
+    a, b, c, d = pattern
+    n = 70
+    x = rows(n, a * c * d, False, DT[prec])
+    clean = x.clone()
+    x[3, 2 * d] = float("nan")
+    x[68, 0] = float("inf")
+    clean[3], clean[68] = 0, 0
+    x, clean = ((t.t() if bs_last else t).contiguous().cuda() for t in (x, clean))
+    w = pack_mx(factor(pattern, False, DT[prec]).cuda(), pattern)
+    y, z = (mx_linear(t, w, bs_last=bs_last) for t in (x, clean))
+    y, z = ((t.t() if bs_last else t) for t in (y, z))
+    bad = torch.zeros(n, dtype=torch.bool)
+    bad[3] = bad[68] = True
+    assert torch.equal(y[~bad], z[~bad])
+    first = y[bad].reshape(2, a, b, d)[:, 0, :, 0]  # the block that the two belong to
+    assert torch.isnan(first).all()
+    assert int(torch.isnan(y).sum()) == first.numel()
+
+
+GRADS = [(1, 1, 1, 1), (2, 5, 3, 2), (3, 33, 40, 1), (1, 64, 192, 2), (2, 96, 72, 3), (1, 16, 48, 16)]
+
+
+@pytest.mark.parametrize("bs_last", [False, True])
+@pytest.mark.parametrize("prec", ["fp32", "fp16"])
+@pytest.mark.parametrize("pattern", GRADS)
+def test_gradients_go_straight_through(pattern, prec, bs_last):
+    from ksmm_amd import mx_linear, pack_mx
+
+    a, b, c, d = pattern
+    for n, gated, act, with_bias in ((1, False, None, True), (35, True, "silu", True), (70, False, "gelu", True), (129, True, "gelu", False), (64, False, "gelu", False)):
+        x, f = rows(n, a * c * d, bs_last, DT[prec], n), factor(pattern, gated, DT[prec])
+        g = torch.Generator().manual_seed(2)
+        bias = (torch.randn(a * f.shape[1] * d, generator=g) * 0.1).to(DT[prec]) if with_bias else None
+        dy = rows(n, a * b * d, bs_last, DT[prec], 5)
+        leaves = [t.cuda().requires_grad_(True) for t in (x, f, bias) if t is not None]
+        with torch.enable_grad():
+            y = mx_linear(leaves[0], leaves[1], pattern, bias=leaves[2] if with_bias else None, act=act, gated=gated, bs_last=bs_last)
+            got = torch.autograd.grad(y, leaves, dy.cuda())
+            xq, wq = R.rounded(R.operand(x, a, c, d, bs_last)).requires_grad_(True), R.rounded(factor_rows(f, pattern)).requires_grad_(True)
+            b64 = None if bias is None else bias.double().requires_grad_(True)
+            want = R.product(xq, wq, b64, pattern, act, gated, bs_last)
+            assert rel(y, R.tensor(want, y.shape, bs_last)) <= TOL[prec]
+            grads = torch.autograd.grad(want, [t for t in (xq, wq, b64) if t is not None], R.operand(dy, a, b, d, bs_last).double())
+        expected = [R.tensor(grads[0], x.shape, bs_last), grads[1].transpose(2, 3).reshape(f.shape)] + list(grads[2:])
+        for u, v, t in zip(got, expected, leaves):
+            assert u.dtype == t.dtype and rel(u, v) <= 2 * TOL[prec], (n, gated, act)
+        # a packed factor hands the gradient on to the input
+        with torch.enable_grad():
+            y = mx_linear(leaves[0], pack_mx(f.cuda(), pattern, gated), bias=None if bias is None else bias.cuda(), act=act, bs_last=bs_last)
+            assert torch.equal(torch.autograd.grad(y, leaves[0], dy.cuda())[0], got[0])
+
+
+def test_the_formula_of_the_gradients_against_differences():
+    for pattern, gated, name in (((2, 3, 5, 2), False, "gelu"), ((1, 4, 33, 3), True, "silu")):
+        a, b, c, d = pattern
+        g = torch.Generator().manual_seed(0)
+        x, w = torch.randn(a, d, 4, c, generator=g).double(), torch.randn(a, d, 2 * b if gated else b, c, generator=g).double()
+        bias = torch.randn(a * w.shape[2] * d, generator=g).double()
+        with torch.enable_grad():
+            args = [t.requires_grad_(True) for t in (x, w, bias)]
+            assert torch.autograd.gradcheck(lambda *t: R.product(*t, pattern, name, gated, False), args)
+
+
+def test_second_derivatives_and_quantised_inputs_are_refused():
+    from ksmm_amd import mx_linear, pack_mx, quantize_mx
+
+    with torch.enable_grad():
+        x = torch.randn(4, 64, device="cuda", requires_grad=True)
+        f = torch.randn(64, 32, device="cuda", requires_grad=True)
+        y = mx_linear(x, f, (1, 32, 64, 1))
+        (dx,) = torch.autograd.grad(y.sum(), x, create_graph=True)
+        with pytest.raises(RuntimeError):
+            dx.sum().backward()
+        with pytest.raises(RuntimeError):
+            mx_linear(quantize_mx(x, (1, 64, 1)), f, (1, 32, 64, 1))
+    w = pack_mx(f, (1, 32, 64, 1))
+    assert torch.equal(mx_linear(quantize_mx(x, (1, 64, 1)), w), mx_linear(x, w))
+
+
+@pytest.mark.parametrize("bs_last", [False, True])
+@pytest.mark.parametrize("shape", [(0,), (3, 0), (2, 5)])
+def test_batches_of_several_axes_and_of_none(shape, bs_last):
+    from ksmm_amd import mx_linear, quantize_mx
+
+    g = torch.Generator().manual_seed(0)
+    x = torch.randn(*((64, *shape) if bs_last else (*shape, 64)), generator=g).cuda()
+    f = torch.randn(64, 40, generator=g).cuda()
+    with torch.enable_grad():
+        leaves = [x.clone().requires_grad_(True), f.clone().requires_grad_(True), torch.zeros(40, device="cuda", requires_grad=True)]
+        y = mx_linear(leaves[0], leaves[1], (1, 40, 64, 1), bias=leaves[2], act="gelu", bs_last=bs_last)
+        assert y.shape == ((40, *shape) if bs_last else (*shape, 40))
+        dx, df, db = torch.autograd.grad(y.sum(), leaves)
+    assert dx.shape == x.shape and df.shape == f.shape
+    assert quantize_mx(x, (1, 64, 1), bs_last).dequantize().shape == x.shape
+    if x.numel() == 0:
+        assert not df.any() and not db.any()
+    else:
+        flat = x.reshape(64, -1) if bs_last else x.reshape(-1, 64)
+        assert torch.equal(y.reshape(40, -1) if bs_last else y.reshape(-1, 40), mx_linear(flat, f, (1, 40, 64, 1), act="gelu", bs_last=bs_last))
+
+
+def test_unaligned_tensors():
+    """Inputs, biases and results that start off a vector's boundary, whose rows are odd."""
+    from ksmm_amd import MXKernel, pack_mx, quantize_mx
+
+    for prec in ("fp32", "fp16"):
+        for pattern in ((1, 37, 65, 1), (1, 37, 33, 3), (2, 64, 64, 2)):
+            a, b, c, d = pattern
+            for bs_last in (False, True):
+                n = 67
+                x, f = rows(n, a * c * d, bs_last, DT[prec]).cuda(), factor(pattern, False, DT[prec]).cuda()
+                w = pack_mx(f, pattern)
+                bias = torch.randn(a * b * d, device="cuda").to(DT[prec])
+                y = MXKernel.forward(x, w, bias, None, bs_last)
+
+                def off(t):
+                    room = torch.empty(t.numel() + 1, dtype=t.dtype, device="cuda")
+                    room[1:].copy_(t.reshape(-1))
+                    return room[1:].view(t.shape)
+
+                out = off(torch.zeros_like(y))
+                MXKernel.forward(off(x), w, off(bias), None, bs_last, out=out)
+                assert torch.equal(out, y)
+                q, p = quantize_mx(x, (a, c, d), bs_last), quantize_mx(off(x), (a, c, d), bs_last)
+                assert torch.equal(p.codes, q.codes) and torch.equal(p.scales, q.scales)
+                p = pack_mx(off(f), pattern)
+                assert torch.equal(p.codes, w.codes) and torch.equal(p.scales, w.scales)
+
+
+def test_refusals():
+    from ksmm_amd import MXFactor, MXKernel, MXLinear, MXTensor, mx_linear, pack_mx, quantize_mx
+
+    x, f = torch.randn(4, 128, device="cuda"), torch.randn(128, 40, device="cuda")
+    p = (2, 40, 64, 1)
+    w = pack_mx(f, p)
+    q = quantize_mx(x, (2, 64, 1))
+    for call in (lambda: quantize_mx(x, (2, 64)), lambda: quantize_mx(x, (2, 32, 1)), lambda: quantize_mx(x, (0, 64, 1)), lambda: pack_mx(f, (2, 20, 64, 1)),
+                 lambda: pack_mx(f, p, gated=True), lambda: mx_linear(x, f), lambda: mx_linear(x, w, (1, 40, 128, 1)), lambda: mx_linear(x, w, gated=True),
+                 lambda: mx_linear(x, w, act="silu"), lambda: mx_linear(x, w, act="relu"), lambda: mx_linear(x[:, :64].contiguous(), w),
+                 lambda: mx_linear(x, w, bias=torch.zeros(40, device="cuda")), lambda: mx_linear(quantize_mx(x, (1, 128, 1)), w), lambda: mx_linear(q, w, bs_last=True),
+                 lambda: MXFactor(w.codes, w.scales, (2, 41, 64, 1)), lambda: MXFactor(w.codes, w.scales[:, :20].contiguous(), p), lambda: MXFactor(w.codes.float(), w.scales, p),
+                 lambda: MXTensor(q.codes, q.scales, (2, 64, 1), (5, 128), torch.float32), lambda: MXLinear([]),
+                 lambda: MXKernel.forward(x, w, out=torch.empty(4, 81, device="cuda")), lambda: MXLinear([w, w])):
+        with pytest.raises(ValueError):
+            call()
+    for call in (lambda: quantize_mx(x.cpu(), (2, 64, 1)), lambda: quantize_mx(x.t(), (2, 64, 1), True), lambda: mx_linear(x, w, bias=torch.zeros(80, device="cuda").half()),
+                 lambda: mx_linear(x, w, bias=torch.zeros(80))):
+        with pytest.raises(RuntimeError):
+            call()
+    with pytest.raises(AssertionError):
+        quantize_mx(x.double(), (2, 64, 1))
+    with pytest.raises(RuntimeError):
+        MXKernel.forward(x, w, out=x.view(-1)[:320].view(4, 80))
+
+
+def test_captured_and_replayed():
+    """Single rows from a captured graph, with eager work between the replays; two graphs at once."""
+    from ksmm_amd import mx_linear, pack_mx
+
+    pattern = (1, 768, 192, 2)
+    w = pack_mx(factor(pattern, True, torch.float16).cuda(), pattern, True)
+    graphs = []
+    for n in (1, 5):
+        x = torch.zeros(n, 384, dtype=torch.float16, device="cuda")
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            mx_linear(x, w, act="silu")
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            y = mx_linear(x, w, act="silu")
+        graphs.append((x, graph, y))
+    for i in range(4):
+        for x, graph, y in graphs:
+            new = rows(x.shape[0], 384, False, torch.float16, 10 + i).cuda()
+            x.copy_(new)
+            graph.replay()
+        for x, graph, y in graphs:
+            assert torch.equal(y, mx_linear(rows(x.shape[0], 384, False, torch.float16, 10 + i).cuda(), w, act="silu"))
+        torch.cuda.synchronize()
+
+
+def test_other_streams():
+    from ksmm_amd import mx_linear, pack_mx
+
+    pattern = (6, 64, 64, 1)
+    w = pack_mx(factor(pattern, False, torch.float16).cuda(), pattern)
+    x = rows(3000, 384, False, torch.float16).cuda()
+    want = mx_linear(x, w)
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    torch.cuda.synchronize()
+    got = []
+    for s in streams:
+        with torch.cuda.stream(s):
+            got.append(mx_linear(x, w))
+    torch.cuda.synchronize()
+    assert all(torch.equal(y, want) for y in got)
+
+
+@pytest.mark.parametrize("bs_last", [False, True])
+def test_modules(bs_last):
+    from ksmm_amd import KSFeedForwardMX, KSGatedLinearMX, KSLinear, KSLinearMX, KSMuon, MXLinear, mx_linear, pack_block
+
+    torch.manual_seed(0)
+    patterns = [(6, 64, 64, 1), (1, 768, 192, 2)]
+    x = rows(50, 384, bs_last, torch.float16).cuda()
+    layer = KSLinearMX(patterns, dtype=torch.float16, bs_last=bs_last, act="gelu")
+    y = layer(x)
+    z = mx_linear(mx_linear(x, layer.factors[0], patterns[0], bs_last=bs_last), layer.factors[1], patterns[1], bias=layer.bias, act="gelu", bs_last=bs_last)
+    assert torch.equal(y, z)
+    packed = layer.packed()
+    assert torch.equal(packed(x), y) and not list(packed.parameters()) and packed.out_size == 1536
+    layer.factors[0].data.zero_()  # (codes are a copy)
+    assert torch.equal(packed(x), y)
+    plain = KSLinear(patterns, algo="kernel", dtype=torch.float16, bs_last=bs_last, device="cuda")
+    of = MXLinear.of(plain)
+    again = MXLinear.of(KSLinear(patterns, algo="kernel", dtype=torch.float16, bs_last=bs_last, device="cuda"))
+    again.load_state_dict(of.state_dict())
+    assert torch.equal(of(x), again(x))
+
+    gated = KSGatedLinearMX((1, 768, 192, 2), bs_last=bs_last)
+    assert torch.equal(gated.packed()(x), gated(x))
+    block = KSFeedForwardMX((1, 768, 192, 2), [(1, 192, 768, 2), (6, 64, 64, 1)], bs_last=bs_last)
+    assert len(KSMuon.factors_of(block)) == 3
+    n, r = block(block.begin(x), x)
+    served = block.packed()
+    m, s = served(served.begin(x), x)
+    assert torch.equal(n, m) and torch.equal(r, s)
+    assert torch.equal(pack_block(block)(block.begin(x), x)[0], n)
+    with torch.enable_grad():
+        n, r = block(block.begin(x), x)
+        (n.float().sum() + r.float().sum()).backward()
+    assert all(p.grad is not None and torch.isfinite(p.grad).all() for p in block.parameters())
+    assert all(not any(p is q for q in block.parameters()) for p in served.parameters())
