@@ -98,16 +98,6 @@ template <typename T> __global__ __launch_bounds__(256) void ks_mx_dequantize_ke
     }
 }
 
-struct MxProduct {
-    const uint8_t *x, *x_scales, *w, *w_scales;
-    const void *bias;
-    void *y;
-    int64_t batch;
-    int a, b, c, d, cb;
-    int64_t tiles, token_tiles;
-    int b_tiles;
-};
-
 typedef int int8_v __attribute__((ext_vector_type(8)));
 
 // 32 numbers and their scale of row `row` (< rows, else zeros), block kb (< cb, else zeros)
@@ -138,7 +128,7 @@ template <typename T, bool LAST, bool GATED, int ACT> __global__ __launch_bounds
     float16_t acc = {}, up = {};
     for (int kb = half; kb - half < p.cb; kb += 2) {
         int sx, sw, su;
-        const int8_v x = mx_operand(p.x, p.x_scales, (int64_t)block * p.batch + n, n < p.batch, kb, p.cb, &sx);
+        const int8_v x = mx_operand((const uint8_t *)p.x, p.x_scales, (int64_t)block * p.batch + n, n < p.batch, kb, p.cb, &sx);
         const int64_t row = (int64_t)block * rows_w + bi;
         const int8_v w = mx_operand(p.w, p.w_scales, row, bi < p.b, kb, p.cb, &sw);
         acc = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(w, x, acc, 4, 4, 0, sw, 0, sx);
@@ -253,6 +243,7 @@ int64_t ksmm_mx_forward_workspace(int64_t batch, int a, int b, int c, int d, int
 {
     const int rc = check_product(batch, a, b, c, d, dtype, KSMM_ACT_NONE, gated);
     if (rc != KSMM_OK) return rc;
+    if (mx_in_lds(c, d, bs_last)) return 0;
     const int64_t blocks = (int64_t)a * d * batch * mx_blocks(c);
     return align256(blocks * 16) + align256(blocks);
 }
@@ -273,7 +264,10 @@ int ksmm_mx_forward(const void *x, const void *x_scales, const void *w, const vo
                        {bias, (int64_t)a * rows_w * d * size}};
     const Span out[] = {{y, values(batch, a, b, d) * size}, {need ? workspace : nullptr, need}};
     if (any_overlap(in, out)) return KSMM_ERR_ALIAS;
-    MxProduct p{(const uint8_t *)x, (const uint8_t *)x_scales, (const uint8_t *)w, (const uint8_t *)w_scales, bias, y, batch, a, b, c, d, cb};
+    MxProduct p{x, (const uint8_t *)x_scales, (const uint8_t *)w, (const uint8_t *)w_scales, bias, y, batch, a, b, c, d, cb};
+    if (mx_in_lds(c, d, bs_last))
+        return dtype == KSMM_F32 ? mx_run_float(p, bs_last != 0, gated != 0, act, (hipStream_t)stream)
+                                 : mx_run_half(p, bs_last != 0, gated != 0, act, (hipStream_t)stream);
     if (!x_scales) {
         uint8_t *const codes = (uint8_t *)workspace, *const scales = codes + align256(blocks * 16);
         rc = ksmm_mx_quantize(x, codes, scales, batch, a, c, d, dtype, bs_last, stream);
