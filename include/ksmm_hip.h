@@ -407,11 +407,12 @@ int ksmm_mx_dequantize(const void *codes, const void *scales, void *x, int64_t r
 /* y = act(W x + bias), W of b rows a block, or with `gated` act(G x + bias_g) * (U x + bias_u), W of 2*b rows a block, G's first,
  * and a bias of 2*a*b*d values as for ksmm_gated_forward.  x_scales NULL: x has `dtype` and is quantised in the call; else x and
  * x_scales are an operand of `batch` rows.  Sums are fp32; y and bias have `dtype`.  act: KSMM_ACT_SILU with `gated` only.
+ * codes_out and scales_out (NULL: not wanted): x as the operand that it was multiplied as; not written where it came as one.
  * Needs ksmm_mx_forward_workspace() bytes of 16-byte aligned device memory where x_scales is NULL (0: none). */
 int64_t ksmm_mx_forward_workspace(int64_t batch, int a, int b, int c, int d, int dtype, int bs_last, int gated);
 int ksmm_mx_forward(const void *x, const void *x_scales, const void *w, const void *w_scales, const void *bias, void *y,
-                    void *workspace, int64_t workspace_bytes, int64_t batch, int a, int b, int c, int d, int dtype,
-                    int bs_last, int act, int gated, void *stream);
+                    void *codes_out, void *scales_out, void *workspace, int64_t workspace_bytes, int64_t batch, int a,
+                    int b, int c, int d, int dtype, int bs_last, int act, int gated, void *stream);
 
 /* ---- AdamW over many tensors --------------------------------------------------------------------------
  *     g = grad_scale * grad,  m' = beta1 m + (1 - beta1) g,  v' = beta2 v + (1 - beta2) g^2

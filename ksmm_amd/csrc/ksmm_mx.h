@@ -46,61 +46,55 @@ __device__ __forceinline__ float mx_scale_value(int scale)
 }
 
 // ---- reading an operand ---------------------------------------------------------------------------------
-// A thread takes blocks of one place kb that lie side by side in memory: those of D consecutive d_i (batch-size-first), or of D
-// consecutive rows (batch-size-last).  Their 32 values of c are `step` elements apart; where that is D, they are one run of 32 * D.
+// A thread takes the blocks of one place kb of D consecutive d_i (batch-size-last D is 1): their 32 values of c are `step` elements
+// apart, and one run of 32 * D where that is D.
 typedef uint32_t uint4_any __attribute__((ext_vector_type(4), aligned(2)));  // 16 bytes at an element's alignment
 
 template <typename T, int D> struct MxGroup {
     T v[32 * D];  // value k of block j at k * D + j
 };
 
-// count: of the 32 values those that are there, here: of the D blocks; the rest is zeros
-template <typename T, int D> __device__ __forceinline__ void mx_load(MxGroup<T, D> &g, const T *x, int64_t step, int count, int here)
+// count (1 ..) of the 32 values are there.  Those behind are read as the last ones that are: that changes no largest magnitude, and
+// mx_quantize leaves them out of the codes; a branch around each load would cost more than the loads.
+template <typename T, int D> __device__ __forceinline__ void mx_load(MxGroup<T, D> &g, const T *x, int64_t step, int count)
 {
     constexpr int E = 16 / (int)sizeof(T);  // values a vector
-    if (step == D && here == D) {
-        const int have = count * D;
+    struct __attribute__((packed, aligned(sizeof(T)))) Run {
+        T e[D];
+    };
+    int last = (count < 32 ? count : 32) - 1;
+    asm volatile("" : "+v"(last));  // (offsets of 32 loads are not to be kept in registers from one step of rows to the next)
+    // (a vector that is read in another's place has the same blocks in the same places: not so where D does not divide it)
+    if (step == D && (E % D == 0 ? (last + 1) * D % E == 0 : last == 31)) {
+        const int end = (last + 1) * D / E - 1;
 #pragma unroll
         for (int j = 0; j < 32 * D / E; ++j) {
-            if ((j + 1) * E <= have) {
-                const uint4_t q = *(const uint4_any *)(x + j * E);
-                __builtin_memcpy(&g.v[j * E], &q, 16);
-            } else {
-#pragma unroll
-                for (int i = 0; i < E; ++i) g.v[j * E + i] = j * E + i < have ? x[j * E + i] : (T)0;
-            }
-        }
-    } else if (here == D) {
-        struct __attribute__((packed, aligned(sizeof(T)))) Run {
-            T e[D];
-        };
-#pragma unroll
-        for (int k = 0; k < 32; ++k) {
-            Run r = {};
-            if (k < count) r = *(const Run *)(x + k * step);
-#pragma unroll
-            for (int j = 0; j < D; ++j) g.v[k * D + j] = r.e[j];
+            const uint4_t q = *(const uint4_any *)(x + (j < end ? j : end) * E);
+            __builtin_memcpy(&g.v[j * E], &q, 16);
         }
     } else {
 #pragma unroll
-        for (int k = 0; k < 32; ++k)
+        for (int k = 0; k < 32; ++k) {
+            const Run r = *(const Run *)(x + (k < last ? k : last) * step);
 #pragma unroll
-            for (int j = 0; j < D; ++j) g.v[k * D + j] = k < count && j < here ? x[k * step + j] : (T)0;
+            for (int j = 0; j < D; ++j) g.v[k * D + j] = r.e[j];
+        }
     }
 }
 
 // block j of the group: its codes and its scale's byte
-template <typename T, int D> __device__ __forceinline__ int mx_quantize(const MxGroup<T, D> &g, int j, uint4_t &code)
+template <typename T, int D> __device__ __forceinline__ int mx_quantize(const MxGroup<T, D> &g, int j, int count, uint4_t &code)
 {
     uint32_t top = 0;
     if constexpr (sizeof(T) == 2) {
-        uint16_t most = 0;
+        typedef uint16_t ushort2_v __attribute__((ext_vector_type(2)));
+        ushort2_v most = {0, 0};
 #pragma unroll
-        for (int k = 0; k < 32; ++k) {
-            const uint16_t bits = __builtin_bit_cast(uint16_t, g.v[k * D + j]) & 0x7fffu;
-            most = bits > most ? bits : most;
+        for (int k = 0; k < 32; k += 2) {
+            const ushort2_v bits = {__builtin_bit_cast(uint16_t, g.v[k * D + j]), __builtin_bit_cast(uint16_t, g.v[(k + 1) * D + j])};
+            most = __builtin_elementwise_max(most, bits & (uint16_t)0x7fff);
         }
-        top = mx_bits((float)__builtin_bit_cast(half_t, most));
+        top = mx_bits((float)__builtin_bit_cast(half_t, (uint16_t)(most[0] > most[1] ? most[0] : most[1])));
     } else {
 #pragma unroll
         for (int k = 0; k < 32; ++k) {
@@ -124,7 +118,9 @@ template <typename T, int D> __device__ __forceinline__ int mx_quantize(const Mx
             const float e[8] = {v[0], v[D], v[2 * D], v[3 * D], v[4 * D], v[5 * D], v[6 * D], v[7 * D]};
             r = mx_encode8(e, power);
         }
-        code[q] = scale == MX_NAN ? 0 : r;
+        const int there = count - 8 * q;
+        const uint32_t mask = scale == MX_NAN || there <= 0 ? 0u : there >= 8 ? ~0u : (1u << 4 * there) - 1;
+        code[q] = r & mask;
     }
     return scale;
 }
@@ -133,6 +129,7 @@ template <typename T, int D> __device__ __forceinline__ int mx_quantize(const Mx
 struct MxProduct {
     const void *x;
     const uint8_t *x_scales;  // null: x has values
+    uint8_t *codes_out, *scales_out;  // where these go as codes, or null
     const uint8_t *w, *w_scales;
     const void *bias;
     void *y;
@@ -143,11 +140,28 @@ struct MxProduct {
     int units_per;         // of them a workgroup takes
     int b_tiles, tiles_per;  // tiles of 32 outputs, and those a workgroup takes
     int splits, unit_groups;
-    int64_t tiles, token_tiles;  // (without LDS)
+    int64_t tiles, token_tiles;  // (without LDS); steps of rows
+    int tile_rows, wave_tiles;   // rows a step, and of a workgroup's waves those that lie along the outputs
+    int row_splits, buffers;     // workgroups that share the steps
 };
-int mx_run_half(MxProduct p, bool last, bool gated, int act, hipStream_t s);
-int mx_run_float(MxProduct p, bool last, bool gated, int act, hipStream_t s);
+// by the type of x and y, the layout and whether two projections make one output
+int mx_half_first_plain(const MxProduct &p, int act, hipStream_t s);
+int mx_half_first_gated(const MxProduct &p, int act, hipStream_t s);
+int mx_half_last_plain(const MxProduct &p, int act, hipStream_t s);
+int mx_half_last_gated(const MxProduct &p, int act, hipStream_t s);
+int mx_float_first_plain(const MxProduct &p, int act, hipStream_t s);
+int mx_float_first_gated(const MxProduct &p, int act, hipStream_t s);
+int mx_float_last_plain(const MxProduct &p, int act, hipStream_t s);
+int mx_float_last_gated(const MxProduct &p, int act, hipStream_t s);
+
+// d_i that a unit takes: all of up to four, else a divisor
+inline int mx_run_of(int d) { return d <= 4 ? d : d % 4 == 0 ? 4 : d % 3 == 0 ? 3 : d % 2 == 0 ? 2 : 1; }
+// tiles of 32 rows: what 128 accumulators hold
+constexpr int mx_rows_of(int d, bool gated) { return d * (gated ? 2 : 1) <= 2 ? 4 : d * (gated ? 2 : 1) <= 4 ? 2 : 1; }
+inline int64_t mx_lds(int tt, int d, int cb) { return (int64_t)d * 32 * tt * (16 * (cb | 1) + cb); }
+constexpr int64_t MX_LDS_MOST = 80 * 1024;  // two workgroups a compute unit
+
 // whether an operand's codes fit LDS, so that it is quantised there
-bool mx_in_lds(int c, int d, int bs_last);
+inline bool mx_in_lds(int c, int d, bool last) { return mx_lds(1, last ? 1 : mx_run_of(d), (int)mx_blocks(c)) <= MX_LDS_MOST; }
 
 }  // namespace ksmm

@@ -16,84 +16,185 @@ namespace {
 int launched() { return hipGetLastError() == hipSuccess ? KSMM_OK : KSMM_ERR_LAUNCH; }
 
 struct MxOperand {
-    const void *x;
+    const void *x;  // dequantising: written
     uint8_t *codes, *scales;
     int64_t rows;
     int a, c, d, cb;
     bool last;
     int64_t blocks;  // a * d * rows * cb
 };
+constexpr int THREADS = 256;
 
-// Where block i lies: its first value and the step between values of a row of c, and its place among the operand's blocks.
-// Consecutive i are consecutive in x as far as that goes.
-__device__ __forceinline__ void place(const MxOperand &p, int64_t i, int64_t *at, int64_t *step, int64_t *block, int *kb)
+// ---- batch-size-first, all d_i of up to four in a row: four lanes a block, so that lanes that follow one another read and write 16 * D
+// bytes that do (a block a lane took 24 us for 25088 x 384 in fp16)
+template <typename T, int D, bool BACK> __global__ __launch_bounds__(THREADS) void ks_mx_rows_kernel(MxOperand p)
 {
-    int64_t n;
-    int ai, di;
-    if (p.last) {
-        n = i % p.rows;
-        i /= p.rows;
-        di = (int)(i % p.d);
-        i /= p.d;
-        *kb = (int)(i % p.cb);
-        ai = (int)(i / p.cb);
-        *step = (int64_t)p.d * p.rows;
-        *at = (((int64_t)ai * p.c + *kb * 32) * p.d + di) * p.rows + n;
-    } else {
-        di = (int)(i % p.d);
-        i /= p.d;
-        *kb = (int)(i % p.cb);
-        i /= p.cb;
-        ai = (int)(i % p.a);
-        n = i / p.a;
-        *step = p.d;
-        *at = ((n * p.a + ai) * p.c + *kb * 32) * p.d + di;
-    }
-    *block = (((int64_t)ai * p.d + di) * p.rows + n) * p.cb + *kb;
-}
-
-template <typename T> __global__ __launch_bounds__(256) void ks_mx_quantize_kernel(MxOperand p)
-{
-    for (int64_t i = blockIdx.x * 256LL + threadIdx.x; i < p.blocks; i += gridDim.x * 256LL) {
-        int64_t at, step, block;
-        int kb;
-        place(p, i, &at, &step, &block, &kb);
-        const int count = p.c - kb * 32;
-        const T *x = (const T *)p.x + at;
-        float v[4][8];
-        uint32_t top = 0;
+    constexpr int E = 16 / (int)sizeof(T), N = 8 * D;
+    const int64_t tasks = p.blocks / D * 4;
+    const int quarter = threadIdx.x & 3;
+    for (int64_t i = blockIdx.x * (int64_t)THREADS + threadIdx.x; i < tasks; i += gridDim.x * (int64_t)THREADS) {
+        int64_t t = i >> 2;
+        const int kb = (int)(t % p.cb);
+        t /= p.cb;
+        const int ai = (int)(t % p.a), count = p.c - kb * 32 - quarter * 8;
+        const int64_t n = t / p.a;
+        T *const x = (T *)p.x + ((n * p.a + ai) * p.c + kb * 32 + quarter * 8) * D;
+        T v[N];
+        if constexpr (!BACK) {
+            if (count >= 8) {
 #pragma unroll
-        for (int k = 0; k < 32; ++k) {
-            v[k / 8][k % 8] = k < count ? (float)x[k * step] : 0.f;
-            const uint32_t bits = mx_bits(v[k / 8][k % 8]);
-            top = bits > top ? bits : top;
+                for (int j = 0; j < N / E; ++j) {
+                    const uint4_t q = *(const uint4_any *)(x + j * E);
+                    __builtin_memcpy(&v[j * E], &q, 16);
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < N; ++j) v[j] = j < count * D ? x[j] : (T)0;
+            }
         }
-        const int scale = mx_scale(top);
-        uint4_t code;
 #pragma unroll
-        for (int q = 0; q < 4; ++q) code[q] = scale == MX_NAN ? 0 : mx_encode8(v[q], mx_power(scale));
-        *(uint4_t *)(p.codes + block * 16) = code;
-        p.scales[block] = (uint8_t)scale;
+        for (int j = 0; j < D; ++j) {
+            const int64_t block = (((int64_t)ai * D + j) * p.rows + n) * p.cb + kb;
+            if constexpr (BACK) {
+                float e[8];
+                mx_decode8(((const uint32_t *)p.codes)[block * 4 + quarter], e);
+                const float power = mx_scale_value(p.scales[block]);
+#pragma unroll
+                for (int k = 0; k < 8; ++k) v[k * D + j] = (T)(e[k] * power);
+            } else {
+                float e[8];
+                uint32_t top = 0;
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    e[k] = (float)v[k * D + j];
+                    top = max(top, mx_bits(e[k]));
+                }
+                top = max(top, (uint32_t)__shfl_xor((int)top, 1, 64));
+                top = max(top, (uint32_t)__shfl_xor((int)top, 2, 64));
+                const int scale = mx_scale(top);
+                ((uint32_t *)p.codes)[block * 4 + quarter] = scale == MX_NAN ? 0u : mx_encode8(e, mx_power(scale));
+                if (quarter == 0) p.scales[block] = (uint8_t)scale;
+            }
+        }
+        if constexpr (BACK) {
+            if (count >= 8) {
+#pragma unroll
+                for (int j = 0; j < N / E; ++j) {
+                    uint4_t q;
+                    __builtin_memcpy(&q, &v[j * E], 16);
+                    *(uint4_any *)(x + j * E) = q;
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < N; ++j)
+                    if (j < count * D) x[j] = v[j];
+            }
+        }
     }
 }
 
-template <typename T> __global__ __launch_bounds__(256) void ks_mx_dequantize_kernel(MxOperand p)
+// ---- batch-size-first, D of more d_i: blocks that lie side by side, a thread each
+template <typename T, int D, bool BACK> __global__ __launch_bounds__(THREADS) void ks_mx_runs_kernel(MxOperand p)
 {
-    for (int64_t i = blockIdx.x * 256LL + threadIdx.x; i < p.blocks; i += gridDim.x * 256LL) {
-        int64_t at, step, block;
-        int kb;
-        place(p, i, &at, &step, &block, &kb);
-        const int count = p.c - kb * 32;
-        T *x = (T *)p.x + at;
-        const uint4_t code = *(const uint4_t *)(p.codes + block * 16);
-        const float power = mx_scale_value(p.scales[block]);
+    struct __attribute__((packed, aligned(sizeof(T)))) Run {
+        T e[D];
+    };
+    const int64_t tasks = p.blocks / D;
+    const int runs = p.d / D;
+    for (int64_t i = blockIdx.x * (int64_t)THREADS + threadIdx.x; i < tasks; i += gridDim.x * (int64_t)THREADS) {
+        int64_t t = i;
+        const int d0 = (int)(t % runs) * D;
+        t /= runs;
+        const int kb = (int)(t % p.cb);
+        t /= p.cb;
+        const int ai = (int)(t % p.a), count = p.c - kb * 32;
+        const int64_t n = t / p.a;
+        T *const x = (T *)p.x + ((n * p.a + ai) * p.c + kb * 32) * p.d + d0;
+        MxGroup<T, D> g;
+        if constexpr (!BACK) mx_load<T, D>(g, x, p.d, count);
+#pragma unroll
+        for (int j = 0; j < D; ++j) {
+            const int64_t block = (((int64_t)ai * p.d + d0 + j) * p.rows + n) * p.cb + kb;
+            if constexpr (BACK) {
+                const uint4_t code = *(const uint4_t *)(p.codes + block * 16);
+                const float power = mx_scale_value(p.scales[block]);
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    float e[8];
+                    mx_decode8(code[q], e);
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) g.v[(8 * q + k) * D + j] = (T)(e[k] * power);
+                }
+            } else {
+                uint4_t code;
+                const int scale = mx_quantize<T, D>(g, j, count, code);
+                *(uint4_t *)(p.codes + block * 16) = code;
+                p.scales[block] = (uint8_t)scale;
+            }
+        }
+        if constexpr (BACK) {
+#pragma unroll
+            for (int k = 0; k < 32; ++k) {
+                Run r;
+#pragma unroll
+                for (int j = 0; j < D; ++j) r.e[j] = g.v[k * D + j];
+                if (k < count) *(Run *)(x + (int64_t)k * p.d) = r;
+            }
+        }
+    }
+}
+
+// ---- batch-size-last: a workgroup takes 64 rows of four blocks of a d_i.  Lanes lie along the rows in x, and along the blocks of a row
+// among the codes, which change places in LDS.
+template <typename T, bool BACK> __global__ __launch_bounds__(THREADS) void ks_mx_columns_kernel(MxOperand p, int64_t tiles)
+{
+    __shared__ uint4_t codes[64 * 4 + 4];
+    __shared__ uint8_t scales[64 * 4];
+    const int quads = (p.cb + 3) / 4;
+    int64_t t = blockIdx.x;
+    const int kb0 = (int)(t % quads) * 4;
+    t /= quads;
+    const int64_t n0 = t % tiles * 64;
+    t /= tiles;
+    const int di = (int)(t % p.d), ai = (int)(t / p.d);
+    const int row = threadIdx.x & 63, kb = kb0 + (threadIdx.x >> 6), count = p.c - kb * 32;
+    const int64_t step = (int64_t)p.d * p.rows, n = n0 + row;
+    T *const x = (T *)p.x + (((int64_t)ai * p.c + kb * 32) * p.d + di) * p.rows + n;
+    const int other = threadIdx.x >> 2, other_kb = kb0 + (threadIdx.x & 3);
+    const int64_t block = (((int64_t)ai * p.d + di) * p.rows + n0 + other) * p.cb + other_kb;
+    const bool there = n0 + other < p.rows && other_kb < p.cb;
+    // (a row's four blocks are a slot of 16 bytes each, one more for every 16 rows, so that both sides meet few of the same banks)
+    const int mine = row * 4 + (threadIdx.x >> 6) + row / 16, place = other * 4 + (threadIdx.x & 3) + other / 16;
+    if constexpr (BACK) {
+        if (there) {
+            codes[place] = *(const uint4_t *)(p.codes + block * 16);
+            scales[threadIdx.x] = p.scales[block];
+        }
+        __syncthreads();
+        if (n >= p.rows || count <= 0) return;
+        const uint4_t code = codes[mine];
+        const float power = mx_scale_value(scales[row * 4 + (threadIdx.x >> 6)]);
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-            float v[8];
-            mx_decode8(code[q], v);
+            float e[8];
+            mx_decode8(code[q], e);
 #pragma unroll
             for (int k = 0; k < 8; ++k)
-                if (q * 8 + k < count) x[(q * 8 + k) * step] = (T)(v[k] * power);
+                if (8 * q + k < count) x[(8 * q + k) * step] = (T)(e[k] * power);
+        }
+    } else {
+        if (n < p.rows && count > 0) {
+            MxGroup<T, 1> g;
+            mx_load<T, 1>(g, x, step, count);
+            uint4_t code;
+            const int scale = mx_quantize<T, 1>(g, 0, count, code);
+            codes[mine] = code;
+            scales[row * 4 + (threadIdx.x >> 6)] = (uint8_t)scale;
+        }
+        __syncthreads();
+        if (there) {
+            *(uint4_t *)(p.codes + block * 16) = codes[place];
+            p.scales[block] = scales[threadIdx.x];
         }
     }
 }
@@ -152,15 +253,32 @@ template <typename T, bool LAST, bool GATED, int ACT> __global__ __launch_bounds
     }
 }
 
-template <typename T> int quantize(const MxOperand &p, bool back, hipStream_t s)
+template <typename T, int D, bool BACK> int convert_rows(const MxOperand &p, hipStream_t s)
 {
-    const int64_t want = (p.blocks + 255) / 256;
-    const unsigned grid = (unsigned)(want < 65536 ? want : 65536);
-    if (back)
-        hipLaunchKernelGGL((ks_mx_dequantize_kernel<T>), dim3(grid), dim3(256), 0, s, p);
+    auto grid = [](int64_t tasks) {
+        const int64_t want = (tasks + THREADS - 1) / THREADS;
+        return dim3((unsigned)(want < 65536 ? want : 65536));
+    };
+    if (p.d == D)
+        hipLaunchKernelGGL((ks_mx_rows_kernel<T, D, BACK>), grid(p.blocks / D * 4), dim3(THREADS), 0, s, p);
     else
-        hipLaunchKernelGGL((ks_mx_quantize_kernel<T>), dim3(grid), dim3(256), 0, s, p);
+        hipLaunchKernelGGL((ks_mx_runs_kernel<T, D, BACK>), grid(p.blocks / D), dim3(THREADS), 0, s, p);
     return launched();
+}
+template <typename T, bool BACK> int convert(const MxOperand &p, hipStream_t s)
+{
+    if (p.last) {
+        const int64_t tiles = (p.rows + 63) / 64, grid = tiles * ((p.cb + 3) / 4) * p.a * p.d;
+        if (grid > 0x7fffffffLL) return KSMM_ERR_TOO_LARGE;
+        hipLaunchKernelGGL((ks_mx_columns_kernel<T, BACK>), dim3((unsigned)grid), dim3(THREADS), 0, s, p, tiles);
+        return launched();
+    }
+    switch (mx_run_of(p.d)) {
+    case 1: return convert_rows<T, 1, BACK>(p, s);
+    case 2: return convert_rows<T, 2, BACK>(p, s);
+    case 3: return convert_rows<T, 3, BACK>(p, s);
+    default: return convert_rows<T, 4, BACK>(p, s);
+    }
 }
 
 template <typename T, bool LAST, bool GATED> int product(const MxProduct &p, int act, hipStream_t s)
@@ -206,7 +324,7 @@ int64_t ksmm_mx_blocks(int64_t rows, int a, int c, int d)
     return rc != KSMM_OK ? rc : (int64_t)a * d * rows * mx_blocks(c);
 }
 
-static int convert(const void *x, const void *codes, const void *scales, int64_t rows, int a, int c, int d, int dtype, int bs_last,
+static int convert_operand(const void *x, const void *codes, const void *scales, int64_t rows, int a, int c, int d, int dtype, int bs_last,
                    bool back, void *stream)
 {
     const int rc = check_operand(rows, a, c, d, dtype);
@@ -216,17 +334,19 @@ static int convert(const void *x, const void *codes, const void *scales, int64_t
     if (((uintptr_t)codes & 15) != 0) return KSMM_ERR_WORKSPACE;
     const Span t[] = {{x, values(rows, a, c, d) * (int64_t)dtype_size(dtype)}}, q[] = {{codes, p.blocks * 16}, {scales, p.blocks}};
     if (any_overlap(t, q) || overlaps(codes, p.blocks * 16, scales, p.blocks)) return KSMM_ERR_ALIAS;
-    return dtype == KSMM_F32 ? quantize<float>(p, back, (hipStream_t)stream) : quantize<half_t>(p, back, (hipStream_t)stream);
+    hipStream_t s = (hipStream_t)stream;
+    if (dtype == KSMM_F32) return back ? convert<float, true>(p, s) : convert<float, false>(p, s);
+    return back ? convert<half_t, true>(p, s) : convert<half_t, false>(p, s);
 }
 
 int ksmm_mx_quantize(const void *x, void *codes, void *scales, int64_t rows, int a, int c, int d, int dtype, int bs_last, void *stream)
 {
-    return convert(x, codes, scales, rows, a, c, d, dtype, bs_last, false, stream);
+    return convert_operand(x, codes, scales, rows, a, c, d, dtype, bs_last, false, stream);
 }
 
 int ksmm_mx_dequantize(const void *codes, const void *scales, void *x, int64_t rows, int a, int c, int d, int dtype, int bs_last, void *stream)
 {
-    return convert(x, codes, scales, rows, a, c, d, dtype, bs_last, true, stream);
+    return convert_operand(x, codes, scales, rows, a, c, d, dtype, bs_last, true, stream);
 }
 
 static int check_product(int64_t batch, int a, int b, int c, int d, int dtype, int act, int gated)
@@ -243,33 +363,37 @@ int64_t ksmm_mx_forward_workspace(int64_t batch, int a, int b, int c, int d, int
 {
     const int rc = check_product(batch, a, b, c, d, dtype, KSMM_ACT_NONE, gated);
     if (rc != KSMM_OK) return rc;
-    if (mx_in_lds(c, d, bs_last)) return 0;
+    if (mx_in_lds(c, d, bs_last != 0)) return 0;
     const int64_t blocks = (int64_t)a * d * batch * mx_blocks(c);
     return align256(blocks * 16) + align256(blocks);
 }
 
-int ksmm_mx_forward(const void *x, const void *x_scales, const void *w, const void *w_scales, const void *bias, void *y, void *workspace,
-                    int64_t workspace_bytes, int64_t batch, int a, int b, int c, int d, int dtype, int bs_last, int act, int gated,
-                    void *stream)
+int ksmm_mx_forward(const void *x, const void *x_scales, const void *w, const void *w_scales, const void *bias, void *y, void *codes_out,
+                    void *scales_out, void *workspace, int64_t workspace_bytes, int64_t batch, int a, int b, int c, int d, int dtype,
+                    int bs_last, int act, int gated, void *stream)
 {
     int rc = check_product(batch, a, b, c, d, dtype, act, gated);
     if (rc != KSMM_OK) return rc;
-    if (!x || !w || !w_scales || !y) return KSMM_ERR_NULL_POINTER;
+    if (!x || !w || !w_scales || !y || (!codes_out != !scales_out)) return KSMM_ERR_NULL_POINTER;
+    if (x_scales) codes_out = scales_out = nullptr;  // (they are there)
     const int rows_w = gated ? 2 * b : b, cb = (int)mx_blocks(c);
     const int64_t need = x_scales ? 0 : ksmm_mx_forward_workspace(batch, a, b, c, d, dtype, bs_last, gated);
-    if (((uintptr_t)w & 15) != 0 || (x_scales && ((uintptr_t)x & 15) != 0)) return KSMM_ERR_WORKSPACE;
+    if (((uintptr_t)w & 15) != 0 || (x_scales && ((uintptr_t)x & 15) != 0) || ((uintptr_t)codes_out & 15) != 0) return KSMM_ERR_WORKSPACE;
     if (need > 0 && (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15) != 0)) return KSMM_ERR_WORKSPACE;
     const int64_t blocks = (int64_t)a * d * batch * cb, w_blocks = (int64_t)a * d * rows_w * cb, size = (int64_t)dtype_size(dtype);
     const Span in[] = {{x, x_scales ? blocks * 16 : values(batch, a, c, d) * size}, {x_scales, blocks}, {w, w_blocks * 16}, {w_scales, w_blocks},
                        {bias, (int64_t)a * rows_w * d * size}};
-    const Span out[] = {{y, values(batch, a, b, d) * size}, {need ? workspace : nullptr, need}};
+    const Span out[] = {{y, values(batch, a, b, d) * size}, {codes_out, blocks * 16}, {scales_out, blocks}, {need ? workspace : nullptr, need}};
     if (any_overlap(in, out)) return KSMM_ERR_ALIAS;
-    MxProduct p{x, (const uint8_t *)x_scales, (const uint8_t *)w, (const uint8_t *)w_scales, bias, y, batch, a, b, c, d, cb};
-    if (mx_in_lds(c, d, bs_last))
-        return dtype == KSMM_F32 ? mx_run_float(p, bs_last != 0, gated != 0, act, (hipStream_t)stream)
-                                 : mx_run_half(p, bs_last != 0, gated != 0, act, (hipStream_t)stream);
+    MxProduct p{x, (const uint8_t *)x_scales, (uint8_t *)codes_out, (uint8_t *)scales_out, (const uint8_t *)w, (const uint8_t *)w_scales, bias, y, batch, a, b, c, d, cb};
+    static int (*const fused[2][2][2])(const MxProduct &, int, hipStream_t) = {
+        {{mx_half_first_plain, mx_half_first_gated}, {mx_half_last_plain, mx_half_last_gated}},
+        {{mx_float_first_plain, mx_float_first_gated}, {mx_float_last_plain, mx_float_last_gated}}};
+    if (mx_in_lds(c, d, bs_last != 0))
+        return fused[dtype == KSMM_F32][bs_last != 0][gated != 0](p, act, (hipStream_t)stream);
     if (!x_scales) {
-        uint8_t *const codes = (uint8_t *)workspace, *const scales = codes + align256(blocks * 16);
+        uint8_t *const codes = codes_out ? (uint8_t *)codes_out : (uint8_t *)workspace;
+        uint8_t *const scales = codes_out ? (uint8_t *)scales_out : codes + align256(blocks * 16);
         rc = ksmm_mx_quantize(x, codes, scales, batch, a, c, d, dtype, bs_last, stream);
         if (rc != KSMM_OK) return rc;
         p.x = codes;

@@ -1,0 +1,8 @@
+// Products of microscaled 4-bit numbers: fp32, batch-size-first.
+#include "ksmm_mx_product.h"
+
+namespace ksmm {
+
+int mx_float_first_plain(const MxProduct &p, int act, hipStream_t s) { return mx_first<float, false>(p, act, s); }
+
+}  // namespace ksmm

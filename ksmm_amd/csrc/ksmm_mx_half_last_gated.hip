@@ -1,0 +1,8 @@
+// Products of microscaled 4-bit numbers: fp16, batch-size-last, gated.
+#include "ksmm_mx_product.h"
+
+namespace ksmm {
+
+int mx_half_last_gated(const MxProduct &p, int act, hipStream_t s) { return mx_last<half_t, true>(p, act, s); }
+
+}  // namespace ksmm

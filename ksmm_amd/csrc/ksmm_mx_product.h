@@ -35,6 +35,227 @@ template <typename T, int N> __device__ __forceinline__ void mx_store(T *p, cons
     }
 }
 
+// one step: which byte of the scales is a constant of the instruction
+template <bool LAST> __device__ __forceinline__ float16_t mx_step(uint4_t w, int sw, uint4_t x, int sx, int byte, float16_t c)
+{
+    const int8_v a = mx_widen(LAST ? x : w), b = mx_widen(LAST ? w : x);
+    const int sa = LAST ? sx : sw, sb = LAST ? sw : sx;
+    switch (byte) {
+    case 0: return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, b, c, 4, 4, 0, sa, 0, sb);
+    case 1: return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, b, c, 4, 4, 1, sa, 1, sb);
+    case 2: return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, b, c, 4, 4, 2, sa, 2, sb);
+    default: return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, b, c, 4, 4, 3, sa, 3, sb);
+    }
+}
+// Waits for all loads and stores.  Behind the stores of a tile that is not whole: how many those are is not known when this is
+// compiled, and without the wait the loads that are on their way are waited for with the whole tiles' stores, each time.
+__device__ __forceinline__ void mx_wait() { __builtin_amdgcn_s_waitcnt(0x0f70); }
+
+// act of a lane's results, and their stores: tile t of 32 rows of those from n0 on, tile bt of outputs
+template <typename T, bool LAST, int D, bool GATED, int ACT>
+__device__ __forceinline__ void mx_results(const MxProduct &p, const float16_t (&acc)[D][GATED ? 2 : 1], int ai, int d0, int bt, int lane, int64_t n0, int t, int here)
+{
+    constexpr int G = GATED ? 2 : 1;
+    const int l32 = lane & 31, half = lane >> 5;
+    T v[16 * D];
+#pragma unroll
+    for (int j = 0; j < D; ++j)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            float slope, z = activate<T, ACT, false>(acc[j][0][i], slope);
+            if constexpr (GATED) z *= acc[j][G - 1][i];
+            v[i * D + j] = (T)z;
+        }
+    const bool whole = (t + 1) * 32 <= here && (bt + 1) * 32 <= p.b && (LAST || p.d == D);
+    if constexpr (LAST) {
+        const int o = bt * 32 + l32, n = t * 32 + 16 * half;
+        T *const y = (T *)p.y + (((int64_t)ai * p.b + o) * p.d + d0) * p.batch + n0 + n;
+        if (whole) {
+            mx_store<T, 16>(y, v);
+        } else {
+            if (o < p.b) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    if (n + i < here) y[i] = v[i];
+            }
+            mx_wait();
+        }
+    } else {
+        const int o = bt * 32 + 16 * half, n = t * 32 + l32;
+        T *const y = (T *)p.y + (((n0 + n) * p.a + ai) * p.b + o) * p.d + d0;
+        if (whole) {
+            mx_store<T, 16 * D>(y, v);
+        } else {
+            struct __attribute__((packed, aligned(sizeof(T)))) Run {
+                T e[D];
+            };
+            if (n < here) {
+                if (p.d == D && o + 16 <= p.b) {
+                    mx_store<T, 16 * D>(y, v);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        if (o + i >= p.b) continue;
+                        Run r;
+#pragma unroll
+                        for (int j = 0; j < D; ++j) r.e[j] = v[i * D + j];
+                        *(Run *)(y + (int64_t)i * p.d) = r;
+                    }
+                }
+            }
+            mx_wait();
+        }
+    }
+}
+
+// ---- weights in registers ---------------------------------------------------------------------------------
+// A wave holds the codes of its 32 outputs (of all D, gate and up) for the whole launch, KS steps of 64 along c, and walks down the
+// batch: a workgroup's waves are WB tiles of outputs times WT runs of rows.  Each step's rows of x are quantised into one of two
+// buffers in LDS while the rows before are multiplied, and the values of the rows after are on their way in registers.
+constexpr int mx_scale_bytes(int ks) { return ks <= 4 ? 4 : ks <= 8 ? 8 : 16; }  // of a row and one half of each step
+
+template <typename T, bool LAST, int D, bool GATED, int ACT, int KS> __global__ __launch_bounds__(512) void ks_mx_held_kernel(MxProduct p)
+{
+    constexpr int G = GATED ? 2 : 1, SB = mx_scale_bytes(KS), SW = (KS + 3) / 4, R = KS > 8 ? 2 : 1;
+    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+    const int threads = blockDim.x, waves = threads >> 6, TN = p.tile_rows, buffer = D * TN * (p.slots * 16 + 2 * SB);
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l32 = lane & 31, half = lane >> 5;
+    const int run = 16 * ((l32 >> 2) & 1) + 4 * (l32 >> 3) + (l32 & 3);  // the row that this lane reads of the operand whose rows are dealt out
+    const int wb = wave & (p.wave_tiles - 1), wt = wave / p.wave_tiles, per_wave = TN / 32 / (waves / p.wave_tiles);
+    int blk = blockIdx.x;
+    const int first = blk % p.row_splits;
+    blk /= p.row_splits;
+    const int unit = blk % p.units, ai = unit / p.runs, d0 = (unit - ai * p.runs) * D, rows_w = G * p.b;
+    const int bt = blk / p.units * p.wave_tiles + wb;
+    const bool busy = bt < p.b_tiles;
+    const int wo = bt * 32 + (LAST ? l32 : run), o = wo < p.b ? wo : p.b - 1;  // (outputs behind the last one are read as the last one)
+    float *const bias = (float *)(smem + p.buffers * buffer);  // (tile of the workgroup, gate and up, D, 32 outputs)
+
+    const int tasks = TN * p.cb;
+    const bool emit = p.codes_out && blk / p.units == 0;
+    // what a thread loads for the step of rows n0 on: the blocks of task t
+    struct Load {
+        MxGroup<T, D> g;
+        int row, kb;  // none: row < 0
+    };
+    auto fetch = [&](Load &f, int t, int64_t n0) {
+        const int kb = LAST ? t / TN : t % p.cb, n = LAST ? t - kb * TN : t / p.cb;
+        f.row = t < tasks && n < p.batch - n0 ? n : -1;
+        f.kb = kb;
+        if (f.row < 0) return;
+        const T *x = (const T *)p.x + (LAST ? (((int64_t)ai * p.c + kb * 32) * p.d + d0) * p.batch + n0 + n
+                                            : (((n0 + n) * p.a + ai) * p.c + kb * 32) * p.d + d0);
+        mx_load<T, D>(f.g, x, LAST ? (int64_t)p.d * p.batch : p.d, p.c - kb * 32);
+    };
+    auto keep = [&](const Load &f, int64_t n0, int which) {
+        if (f.row < 0) return;  // (rows that are not there: whatever LDS has, they are other columns of the product)
+        uint8_t *const codes = smem + which * buffer, *const scales = codes + D * TN * p.slots * 16;
+#pragma unroll
+        for (int j = 0; j < D; ++j) {
+            const int row = j * TN + f.row;
+            uint4_t code;
+            const int scale = mx_quantize<T, D>(f.g, j, p.c - f.kb * 32, code);
+            *(uint4_t *)(codes + (row * p.slots + f.kb) * 16) = code;
+            scales[row * 2 * SB + (f.kb & 1) * SB + (f.kb >> 1)] = (uint8_t)scale;
+            if (emit) {
+                const int64_t block = (((int64_t)ai * p.d + d0 + j) * p.batch + n0 + f.row) * p.cb + f.kb;
+                *(uint4_t *)(p.codes_out + block * 16) = code;
+                p.scales_out[block] = (uint8_t)scale;
+            }
+        }
+    };
+
+    // rows, tiles of them and what is on its way
+    const int64_t row_tiles = p.token_tiles;
+    Load f[R];
+    const bool on = first + p.row_splits < row_tiles;  // more steps than one (of 512 threads, which take a step's blocks R each)
+    if (on) {
+#pragma unroll
+        for (int r = 0; r < R; ++r) fetch(f[r], threadIdx.x + r * 512, (int64_t)first * TN);
+    }
+    uint4_t w[D][G][KS];
+    int sw[D][G][SW];
+    if (busy) {
+#pragma unroll
+        for (int j = 0; j < D; ++j)
+#pragma unroll
+            for (int q = 0; q < G; ++q) {
+                const int64_t at = (((int64_t)ai * p.d + d0 + j) * rows_w + q * p.b + o) * p.cb;
+#pragma unroll
+                for (int s = 0; s < KS; ++s) {
+                    const int kb = 2 * s + half;
+                    const bool there = kb < p.cb;
+                    w[j][q][s] = there ? *(const uint4_t *)(p.w + (at + kb) * 16) : uint4_t{0, 0, 0, 0};
+                    const int scale = there ? p.w_scales[at + kb] : 127;
+                    sw[j][q][s / 4] = s % 4 ? sw[j][q][s / 4] | scale << 8 * (s % 4) : scale;
+                }
+            }
+    }
+    // (scales of blocks behind the last one are read: with weights of zeros, but not as NaN)
+    for (int k = 0; k < p.buffers; ++k)
+        for (int i = threadIdx.x; i < D * TN * SB / 2; i += threads) ((uint32_t *)(smem + k * buffer + D * TN * p.slots * 16))[i] = 0x7f7f7f7fu;
+    for (int i = threadIdx.x; i < p.wave_tiles * G * 32 * D; i += threads) {
+        const int j = i / 32 % D, q = i / 32 / D % G, out = (blk / p.units * p.wave_tiles + i / 32 / D / G) * 32 + i % 32;
+        bias[i] = p.bias && out < p.b ? (float)((const T *)p.bias)[((int64_t)ai * rows_w + q * p.b + out) * p.d + d0 + j] : 0.f;
+    }
+    __syncthreads();
+    if (on) {
+#pragma unroll
+        for (int r = 0; r < R; ++r) keep(f[r], (int64_t)first * TN, 0);
+#pragma unroll
+        for (int r = 0; r < R; ++r) fetch(f[r], threadIdx.x + r * 512, (int64_t)(first + p.row_splits) * TN);
+    } else {
+        for (int t = threadIdx.x; t < tasks; t += threads) {
+            fetch(f[0], t, (int64_t)first * TN);
+            keep(f[0], (int64_t)first * TN, 0);
+        }
+    }
+    __syncthreads();
+    int which = 0;
+    for (int64_t tile = first; tile < row_tiles; tile += p.row_splits, which ^= 1) {
+        const int64_t n0 = tile * TN;
+        const int here = (int)(p.batch - n0 < TN ? p.batch - n0 : TN);
+        if (tile + p.row_splits < row_tiles) {
+#pragma unroll
+            for (int r = 0; r < R; ++r) keep(f[r], (tile + p.row_splits) * TN, which ^ 1);
+            if (tile + 2 * p.row_splits < row_tiles) {
+#pragma unroll
+                for (int r = 0; r < R; ++r) fetch(f[r], threadIdx.x + r * 512, (tile + 2 * p.row_splits) * TN);
+            }
+        }
+        const uint8_t *const codes = smem + which * buffer, *const scales = codes + D * TN * p.slots * 16;
+        int t = wt * per_wave;
+        if (busy && t * 32 < here) {
+            do {
+                float16_t acc[D][G];
+#pragma unroll
+                for (int j = 0; j < D; ++j)
+#pragma unroll
+                    for (int q = 0; q < G; ++q)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) acc[j][q][i] = bias[((wb * G + q) * D + j) * 32 + (LAST ? l32 : 16 * half + i)];
+#pragma unroll
+                for (int j = 0; j < D; ++j) {
+                    const int row = j * TN + t * 32 + (LAST ? run : l32);
+                    int sx[SW];
+#pragma unroll
+                    for (int i = 0; i < SW; ++i) sx[i] = ((const int *)(scales + row * 2 * SB + half * SB))[i];
+#pragma unroll
+                    for (int s = 0; s < KS; ++s) {
+                        const uint4_t x = *(const uint4_t *)(codes + (row * p.slots + 2 * s + half) * 16);
+#pragma unroll
+                        for (int q = 0; q < G; ++q) acc[j][q] = mx_step<LAST>(w[j][q][s], sw[j][q][s / 4], x, sx[s / 4], s % 4, acc[j][q]);
+                    }
+                }
+                mx_results<T, LAST, D, GATED, ACT>(p, acc, ai, d0, bt, lane, n0, t, here);
+            } while (++t < (wt + 1) * per_wave && t * 32 < here);
+        } else {
+            mx_wait();
+        }
+        __syncthreads();
+    }
+}
+
 template <typename T, bool LAST, int D, int TT, bool GATED, int ACT> __global__ __launch_bounds__(64 * MX_WAVES) void ks_mx_fused_kernel(MxProduct p)
 {
     constexpr int TN = 32 * TT, G = GATED ? 2 : 1;
@@ -68,33 +289,25 @@ template <typename T, bool LAST, int D, int TT, bool GATED, int ACT> __global__ 
                 *(uint4_t *)(codes + ((size_t)row * p.slots + kb) * 16) = code;
                 scales[row * p.cb + kb] = (uint8_t)scale;
             }
-        } else if constexpr (LAST) {
-            constexpr int V = sizeof(T) == 2 ? 4 : 2;
-            for (int t = threadIdx.x; t < TN / V * p.cb; t += 64 * MX_WAVES) {
-                const int kb = t / (TN / V), n = (t - kb * (TN / V)) * V;
-                MxGroup<T, V> g;
-                const int there = here - n < 0 ? 0 : here - n < V ? here - n : V, count = p.c - kb * 32;
-                const int64_t step = (int64_t)p.d * p.batch;
-                mx_load<T, V>(g, (const T *)p.x + (((int64_t)ai * p.c + kb * 32) * p.d + d0) * p.batch + n0 + n, step, there ? count : 0, there);
-#pragma unroll
-                for (int j = 0; j < V; ++j) {
-                    uint4_t code;
-                    const int scale = mx_quantize<T, V>(g, j, code);
-                    *(uint4_t *)(codes + ((size_t)(n + j) * p.slots + kb) * 16) = code;
-                    scales[(n + j) * p.cb + kb] = (uint8_t)scale;
-                }
-            }
         } else {
             for (int t = threadIdx.x; t < TN * p.cb; t += 64 * MX_WAVES) {
-                const int n = t / p.cb, kb = t - n * p.cb;
+                const int kb = LAST ? t / TN : t % p.cb, n = LAST ? t - kb * TN : t / p.cb;
+                if (n >= here) continue;  // (whatever LDS has there, it is another column of the product)
                 MxGroup<T, D> g;
-                mx_load<T, D>(g, (const T *)p.x + (((n0 + n) * p.a + ai) * p.c + kb * 32) * p.d + d0, p.d, n < here ? p.c - kb * 32 : 0, D);
+                const T *x = (const T *)p.x + (LAST ? (((int64_t)ai * p.c + kb * 32) * p.d + d0) * p.batch + n0 + n
+                                                    : (((n0 + n) * p.a + ai) * p.c + kb * 32) * p.d + d0);
+                mx_load<T, D>(g, x, LAST ? (int64_t)p.d * p.batch : p.d, p.c - kb * 32);
 #pragma unroll
                 for (int j = 0; j < D; ++j) {
                     uint4_t code;
-                    const int scale = mx_quantize<T, D>(g, j, code);
-                    *(uint4_t *)(codes + ((size_t)(j * TN + n) * p.slots + kb) * 16) = code;
-                    scales[(j * TN + n) * p.cb + kb] = (uint8_t)scale;
+                    const int row = j * TN + n, scale = mx_quantize<T, D>(g, j, p.c - kb * 32, code);
+                    *(uint4_t *)(codes + ((size_t)row * p.slots + kb) * 16) = code;
+                    scales[row * p.cb + kb] = (uint8_t)scale;
+                    if (p.codes_out && split == 0) {
+                        const int64_t block = (((int64_t)ai * p.d + d0 + j) * p.batch + n0 + n) * p.cb + kb;
+                        *(uint4_t *)(p.codes_out + block * 16) = code;
+                        p.scales_out[block] = (uint8_t)scale;
+                    }
                 }
             }
         }
@@ -102,12 +315,22 @@ template <typename T, bool LAST, int D, int TT, bool GATED, int ACT> __global__ 
         // ---- products
         for (int bt = split * p.tiles_per + wave; bt < tile_end; bt += MX_WAVES) {
             float16_t acc[TT][D][G];
+            const T *const bias = (const T *)p.bias;
 #pragma unroll
-            for (int t = 0; t < TT; ++t)
+            for (int j = 0; j < D; ++j)
 #pragma unroll
-                for (int j = 0; j < D; ++j)
+                for (int q = 0; q < G; ++q) {
+                    float16_t add = {};
+                    if (bias) {
 #pragma unroll
-                    for (int q = 0; q < G; ++q) acc[t][j][q] = float16_t{};
+                        for (int i = 0; i < 16; ++i) {
+                            const int out = LAST ? bt * 32 + l32 : bt * 32 + 16 * half + i;
+                            add[i] = (float)bias[((int64_t)ai * rows_w + q * p.b + (out < p.b ? out : p.b - 1)) * p.d + d0 + j];
+                        }
+                    }
+#pragma unroll
+                    for (int t = 0; t < TT; ++t) acc[t][j][q] = add;
+                }
             // (outputs behind the last one are read as the last one and not stored)
             const int wo = bt * 32 + (LAST ? l32 : run), o = wo < p.b ? wo : p.b - 1;
             const int xr = LAST ? run : l32;
@@ -140,82 +363,17 @@ template <typename T, bool LAST, int D, int TT, bool GATED, int ACT> __global__ 
                             acc[t][j][q] = LAST ? mx_mfma(x, sx, w[j][q], sw[j][q], acc[t][j][q]) : mx_mfma(w[j][q], sw[j][q], x, sx, acc[t][j][q]);
                     }
             }
-            // ---- results
-            const T *const bias = (const T *)p.bias;
-            if constexpr (LAST) {
-                float add[G];
 #pragma unroll
-                for (int q = 0; q < G; ++q) add[q] = bias ? (float)bias[((int64_t)ai * rows_w + q * p.b + o) * p.d + d0] : 0.f;
-                T *const y = (T *)p.y + (((int64_t)ai * p.b + wo) * p.d + d0) * p.batch + n0;
-#pragma unroll
-                for (int t = 0; t < TT; ++t) {
-                    const int n = t * 32 + 16 * half;
-                    T v[16];
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        float slope, z = activate<T, ACT, false>(acc[t][0][0][i] + add[0], slope);
-                        if constexpr (GATED) z *= acc[t][0][G - 1][i] + add[G - 1];
-                        v[i] = (T)z;
-                    }
-                    if (wo >= p.b) continue;
-                    if (n + 16 <= here) {
-                        mx_store<T, 16>(y + n, v);
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < 16; ++i)
-                            if (n + i < here) y[n + i] = v[i];
-                    }
-                }
-            } else {
-                const int o0 = bt * 32 + 16 * half;
-#pragma unroll
-                for (int t = 0; t < TT; ++t) {
-                    const int n = t * 32 + l32;
-                    T v[16 * D];
-#pragma unroll
-                    for (int j = 0; j < D; ++j)
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) {
-                            const int oi = o0 + i < p.b ? o0 + i : p.b - 1;
-                            float slope, z = acc[t][j][0][i];
-                            if (bias) z += (float)bias[((int64_t)ai * rows_w + oi) * p.d + d0 + j];
-                            z = activate<T, ACT, false>(z, slope);
-                            if constexpr (GATED) {
-                                float u = acc[t][j][G - 1][i];
-                                if (bias) u += (float)bias[((int64_t)ai * rows_w + p.b + oi) * p.d + d0 + j];
-                                z *= u;
-                            }
-                            v[i * D + j] = (T)z;
-                        }
-                    if (n >= here) continue;
-                    T *const y = (T *)p.y + (((n0 + n) * p.a + ai) * p.b + o0) * p.d + d0;
-                    if (p.d == D && o0 + 16 <= p.b) {
-                        mx_store<T, 16 * D>(y, v);
-                    } else {
-                        struct __attribute__((packed, aligned(sizeof(T)))) Run {
-                            T e[D];
-                        };
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) {
-                            if (o0 + i >= p.b) continue;
-                            Run r;
-#pragma unroll
-                            for (int j = 0; j < D; ++j) r.e[j] = v[i * D + j];
-                            *(Run *)(y + (int64_t)i * p.d) = r;
-                        }
-                    }
-                }
-            }
+            for (int t = 0; t < TT; ++t)
+                if (t * 32 < here) mx_results<T, LAST, D, GATED, ACT>(p, acc[t], ai, d0, bt, lane, n0, t, here);
         }
     }
 }
 
-// d_i that a unit takes: all of up to four, else a divisor
-inline int mx_run_of(int d) { return d <= 4 ? d : d % 4 == 0 ? 4 : d % 3 == 0 ? 3 : d % 2 == 0 ? 2 : 1; }
-// tiles of 32 rows: what 128 accumulators hold
-constexpr int mx_rows_of(int d, bool gated) { return d * (gated ? 2 : 1) <= 2 ? 4 : d * (gated ? 2 : 1) <= 4 ? 2 : 1; }
-inline int64_t mx_lds(int tt, int d, int cb) { return (int64_t)d * 32 * tt * (16 * (cb | 1) + cb); }
-constexpr int64_t MX_LDS_MOST = 80 * 1024;  // two workgroups a compute unit
+inline int64_t mx_held_lds(int d, bool gated, int ks, int cb, int rows, int tiles, int buffers)
+{
+    return (int64_t)buffers * d * rows * ((cb | 1) * 16 + 2 * mx_scale_bytes(ks)) + (int64_t)tiles * (gated ? 2 : 1) * 32 * d * 4;
+}
 
 template <typename T, bool LAST, int D, int TT, bool GATED> int mx_launch(MxProduct p, int act, hipStream_t s)
 {
@@ -256,8 +414,77 @@ template <typename T, bool LAST, int D, int TT, bool GATED> int mx_launch(MxProd
     return rc;
 }
 
+template <typename T, bool LAST, int D, bool GATED, int KS> int mx_launch_held(MxProduct p, int act, hipStream_t s)
+{
+    constexpr int R = KS > 8 ? 2 : 1;
+    p.slots = p.cb | 1;
+    p.runs = p.d / D;
+    p.units = p.a * p.runs;
+    p.b_tiles = (p.b + 31) / 32;
+    auto tasks = [&](int rows) { return (int64_t)rows * p.cb; };
+    // eight waves: the more of them share their rows the less often these are quantised, but none should idle
+    int best = 8, idle = 1 << 30;
+    for (int tiles = 8; tiles >= 1; tiles /= 2) {
+        const int over = (p.b_tiles + tiles - 1) / tiles * tiles - p.b_tiles;
+        if (over < idle && tasks(32 * 8 / tiles) <= 512 * R) {
+            best = tiles;
+            idle = over;
+        }
+    }
+    int waves = 8;
+    p.wave_tiles = best;
+    p.tile_rows = 32 * 8 / best;
+    while (p.tile_rows < 256 && tasks(2 * p.tile_rows) <= 512 * R && mx_held_lds(D, GATED, KS, p.cb, 2 * p.tile_rows, p.wave_tiles, 2) <= 80 * 1024) p.tile_rows *= 2;
+    auto groups = [&] { return (int64_t)p.units * ((p.b_tiles + p.wave_tiles - 1) / p.wave_tiles); };
+    p.token_tiles = (p.batch + p.tile_rows - 1) / p.tile_rows;
+    if (groups() * p.token_tiles < 256) {  // few: smaller workgroups of one step each
+        for (waves = 4; waves >= 1; waves /= 2) {
+            p.wave_tiles = waves;
+            p.tile_rows = 32;
+            p.token_tiles = (p.batch + 31) / 32;
+            if (waves == 1 || groups() * p.token_tiles >= 256) break;
+        }
+    }
+    // workgroups that fit at once: a wave's registers are its weights, its sums and the values on their way
+    constexpr int REGS = D * (GATED ? 2 : 1) * (4 * KS + 16) + D * R * 8 * (int)sizeof(T) + 50;
+    const int64_t most = ((REGS > 128 ? 256 : 512) + groups() - 1) / groups();
+    p.row_splits = (int)(waves < 8 || p.token_tiles < most ? p.token_tiles : most);
+    p.buffers = p.row_splits < p.token_tiles ? 2 : 1;
+    const int64_t grid = groups() * p.row_splits;
+    if (grid > 0x7fffffffLL) return KSMM_ERR_TOO_LARGE;
+    const int lds = (int)mx_held_lds(D, GATED, KS, p.cb, p.tile_rows, p.wave_tiles, p.buffers);
+    int rc = KSMM_OK;
+    with_act(act, [&](auto which) {
+        constexpr int ACT = decltype(which)::value;
+        if constexpr (GATED || ACT != KSMM_ACT_SILU) {
+            auto fn = &ks_mx_held_kernel<T, LAST, D, GATED, ACT, KS>;
+            if (lds > 64 * 1024) rc = ensure_dynamic_lds((const void *)fn, lds);
+            if (rc != KSMM_OK) return;
+            hipLaunchKernelGGL(fn, dim3((unsigned)grid), dim3(64 * waves), lds, s, p);
+            if (hipGetLastError() != hipSuccess) rc = KSMM_ERR_LAUNCH;
+        }
+    });
+    return rc;
+}
+
+// steps of 64 along c that a kernel is made for
+template <typename T, bool LAST, int D, bool GATED, int KS, int... MORE> int mx_held(const MxProduct &p, int act, hipStream_t s)
+{
+    // registers: the weights' codes (4 a step), and the values of one row of steps on their way
+    constexpr bool fits = D * (GATED ? 2 : 1) * KS <= 16 && D * (KS > 8 ? 2 : 1) * 8 * (int)sizeof(T) <= 64;
+    if constexpr (fits) {
+        if (p.cb <= 2 * KS) return mx_launch_held<T, LAST, D, GATED, KS>(p, act, s);
+        if constexpr (sizeof...(MORE) > 0) return mx_held<T, LAST, D, GATED, MORE...>(p, act, s);
+    }
+    return KSMM_ERR_BAD_ALGO;
+}
+
 template <typename T, bool LAST, int D, bool GATED> int mx_pick(const MxProduct &p, int act, hipStream_t s)
 {
+    if (!p.x_scales) {
+        const int rc = mx_held<T, LAST, D, GATED, 1, 2, 3, 4, 6, 8, 16>(p, act, s);
+        if (rc != KSMM_ERR_BAD_ALGO) return rc;
+    }
     constexpr int TT = mx_rows_of(D, GATED);
     if constexpr (TT > 1) {
         if (p.batch > 32 && mx_lds(TT, D, p.cb) <= MX_LDS_MOST) return mx_launch<T, LAST, D, TT, GATED>(p, act, s);
@@ -265,14 +492,14 @@ template <typename T, bool LAST, int D, bool GATED> int mx_pick(const MxProduct 
     return mx_launch<T, LAST, D, 1, GATED>(p, act, s);
 }
 
-template <typename T> int mx_run(const MxProduct &p, bool last, bool gated, int act, hipStream_t s)
+template <typename T, bool GATED> int mx_last(const MxProduct &p, int act, hipStream_t s) { return mx_pick<T, true, 1, GATED>(p, act, s); }
+template <typename T, bool GATED> int mx_first(const MxProduct &p, int act, hipStream_t s)
 {
-    if (last) return gated ? mx_pick<T, true, 1, true>(p, act, s) : mx_pick<T, true, 1, false>(p, act, s);
     switch (mx_run_of(p.d)) {
-    case 1: return gated ? mx_pick<T, false, 1, true>(p, act, s) : mx_pick<T, false, 1, false>(p, act, s);
-    case 2: return gated ? mx_pick<T, false, 2, true>(p, act, s) : mx_pick<T, false, 2, false>(p, act, s);
-    case 3: return gated ? mx_pick<T, false, 3, true>(p, act, s) : mx_pick<T, false, 3, false>(p, act, s);
-    default: return gated ? mx_pick<T, false, 4, true>(p, act, s) : mx_pick<T, false, 4, false>(p, act, s);
+    case 1: return mx_pick<T, false, 1, GATED>(p, act, s);
+    case 2: return mx_pick<T, false, 2, GATED>(p, act, s);
+    case 3: return mx_pick<T, false, 3, GATED>(p, act, s);
+    default: return mx_pick<T, false, 4, GATED>(p, act, s);
     }
 }
 

@@ -173,7 +173,8 @@ class MXKernel:
     """The product as a single call on tensors, without autograd."""
 
     @staticmethod
-    def forward(x, factor, bias=None, act=None, bs_last=False, out=None, workspace=None):
+    def forward(x, factor, bias=None, act=None, bs_last=False, out=None, workspace=None, need_codes=False):
+        """The result, or with ``need_codes`` (the result, codes, scales) of x as it was multiplied."""
         lib = _lib.load()
         bs_last = bool(bs_last)
         a, b, c, d = factor.pattern
@@ -182,9 +183,13 @@ class MXKernel:
             out = torch.empty(shape, dtype=dtype, device=x.device)
         elif tuple(out.shape) != tuple(shape) or out.dtype != dtype or out.device != x.device or not out.is_contiguous():
             raise ValueError("out must be a contiguous %s of shape %s" % (dtype, tuple(shape)))
-        if batch == 0:
-            return out
         quantised = isinstance(x, MXTensor)
+        codes = scales = None
+        if need_codes:
+            codes = x.codes if quantised else torch.empty(a * d, batch, 16 * _blocks(c), dtype=torch.uint8, device=x.device)
+            scales = x.scales if quantised else torch.empty(a * d, batch, _blocks(c), dtype=torch.uint8, device=x.device)
+        if batch == 0:
+            return (out, codes, scales) if need_codes else out
         dt = dtype_code(dtype)
         need = 0
         if not quantised:
@@ -196,10 +201,11 @@ class MXKernel:
         with torch.cuda.device(x.device):
             _lib.check(lib.ksmm_mx_forward(
                 (x.codes if quantised else x).data_ptr(), x.scales.data_ptr() if quantised else None, factor.codes.data_ptr(),
-                factor.scales.data_ptr(), _ptr(bias), out.data_ptr(), workspace.data_ptr() if need > 0 else None,
+                factor.scales.data_ptr(), _ptr(bias), out.data_ptr(), None if quantised else _ptr(codes), None if quantised else _ptr(scales),
+                workspace.data_ptr() if need > 0 else None,
                 workspace.numel() * workspace.element_size() if need > 0 else 0, batch, a, b, c, d, dt, int(bs_last), GATED_ACTS[act],
                 int(factor.gated), _stream_ptr(out)))
-        return out
+        return (out, codes, scales) if need_codes else out
 
 
 class MXFunction(torch.autograd.Function):
@@ -210,12 +216,11 @@ class MXFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, factor, bias, pattern, act, gated, bs_last):
         packed = factor if isinstance(factor, MXFactor) else pack_mx(factor, pattern, gated)
-        _check_product(x, packed.device, packed.pattern, bias, act, gated, bs_last)
-        q = quantize_mx(x, (pattern[0], pattern[2], pattern[3]), bs_last)
-        ctx.save_for_backward(q.codes, q.scales, packed.codes, packed.scales, bias)
+        out, codes, scales = MXKernel.forward(x, packed, bias, act, bs_last, need_codes=True)
+        ctx.save_for_backward(codes, scales, packed.codes, packed.scales, bias)
         ctx.how = tuple(pattern), act, bool(gated), bool(bs_last), tuple(x.shape), x.dtype
         ctx.factor_dtype = None if packed is factor else factor.dtype
-        return MXKernel.forward(q, packed, bias, act, bs_last)
+        return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable

@@ -121,7 +121,7 @@ PATTERNS = [(1, 1, 1, 1), (2, 5, 3, 2), (1, 32, 32, 1), (3, 33, 40, 1), (1, 64, 
 @pytest.mark.parametrize("prec", ["fp32", "fp16"])
 @pytest.mark.parametrize("pattern", PATTERNS)
 def test_products(pattern, prec, bs_last):
-    from ksmm_amd import mx_linear, pack_mx, quantize_mx
+    from ksmm_amd import MXKernel, mx_linear, pack_mx, quantize_mx
 
     a, b, c, d = pattern
     for n, gated, act, with_bias in ((1, False, None, True), (2, True, "silu", False), (7, False, "gelu", True), (33, True, "gelu", True), (64, False, None, False),
@@ -138,8 +138,10 @@ def test_products(pattern, prec, bs_last):
                          bs_last)
         want = R.tensor(want, y.shape, bs_last)
         assert y.dtype == DT[prec] and rel(y, want) <= TOL[prec], (n, gated, act)
-        # the same numbers, however they were made
+        # the same numbers, however they were made, and handed out as they are
         q = quantize_mx(x.cuda(), (a, c, d), bs_last)
+        z, codes, scales = MXKernel.forward(x.cuda(), w, cuda_bias, act, bs_last, need_codes=True)
+        assert torch.equal(z, y) and torch.equal(codes, q.codes) and torch.equal(scales, q.scales)
         assert torch.equal(mx_linear(q, w, bias=cuda_bias, act=act, bs_last=bs_last), y)
         assert torch.equal(mx_linear(x.cuda(), f.cuda(), pattern, bias=cuda_bias, act=act, gated=gated, bs_last=bs_last), y)
 

@@ -43,7 +43,7 @@ def test_conversions_refuse(lib, back, bs_last):
 
 def test_products_refuse(lib):
     n, a, b, c, d = 9, 2, 24, 40, 3
-    names = ["x", "x_scales", "w", "w_scales", "bias", "y", "workspace"]
+    names = ["x", "x_scales", "w", "w_scales", "bias", "y", "codes", "scales", "workspace"]
     at = dict(zip(names, FAR))
     for dtype, size in ((0, 4), (1, 2)):
         for gated in (0, 1):
@@ -53,7 +53,7 @@ def test_products_refuse(lib):
 
                 def call(quantised, bytes=need, act=0, n=n, a=a, b=b, c=c, d=d, dtype=dtype, gated=gated, **change):
                     p = dict(at, **change)
-                    return lib.ksmm_mx_forward(p["x"], p["x_scales"] if quantised else None, p["w"], p["w_scales"], p["bias"], p["y"], p["workspace"], bytes, n, a, b, c, d,
+                    return lib.ksmm_mx_forward(p["x"], p["x_scales"] if quantised else None, p["w"], p["w_scales"], p["bias"], p["y"], p["codes"], p["scales"], p["workspace"], bytes, n, a, b, c, d,
                                                dtype, bs_last, act, gated, None)
 
                 for q in (False, True):
@@ -71,6 +71,10 @@ def test_products_refuse(lib):
                     for k in sizes:
                         if k != "x_scales" or q:
                             assert call(q, y=at[k] + sizes[k] - 1) == ALIAS, (q, k)
+                            if not q:  # (codes that are given are not written)
+                                assert call(q, codes=(at[k] + sizes[k] - 1) // 16 * 16) == ALIAS and call(q, scales=at[k] + sizes[k] - 1) == ALIAS, k
+                assert call(False, codes=None) == NULL and call(False, scales=None) == NULL and call(False, codes=at["codes"] + 8) == WORKSPACE
+                assert call(False, codes=at["y"]) == ALIAS and call(False, scales=at["codes"]) == ALIAS
                 assert call(True, x=at["x"] + 4) == WORKSPACE
                 if need:
                     assert call(False, bytes=need - 1) == WORKSPACE and call(False, workspace=None) == WORKSPACE and call(False, workspace=at["workspace"] + 4) == WORKSPACE
