@@ -177,6 +177,7 @@ class _NoNative:
         return None
 
     train_forward = train_backward = residual_norm = gated_linear = infer
+    mx_rows = mx_quantize = mx_dequantize = mx_linear = adamw_update = adamw_moments = infer
 
 
 def native():

@@ -44,6 +44,11 @@ def adamw_update(params, grads, exp_avgs, exp_avg_sqs, scales=None, masters=None
     ``follow``: a parameter that is not what its master rounds to was written since, and counts instead.
     ``step``: from 1 on, or an int64 tensor of one value on the device, which a captured graph reads anew on every replay.
     What a NaN or an infinity among the gradients reaches is its own element alone."""
+    if len(betas) != 2:
+        raise ValueError("betas must be two values from 0 on and below 1, not %s" % (betas,))
+    if _lib.native().adamw_update(params, grads, exp_avgs, exp_avg_sqs, scales, masters, step, lr, betas[0], betas[1], eps, weight_decay,
+                                  grad_scale, seed, follow):
+        return
     lib = _lib.load()
     params, grads = [p.detach() for p in params], [g.detach() for g in grads]
     _check_lists(params, grads=grads, exp_avgs=exp_avgs, exp_avg_sqs=exp_avg_sqs, scales=scales, masters=masters)
@@ -53,7 +58,7 @@ def adamw_update(params, grads, exp_avgs, exp_avg_sqs, scales=None, masters=None
     small = scales is not None
     if like.dtype not in (torch.float32, torch.float16):
         raise AssertionError("Unsupported data type %s of parameters: float32 and float16 are" % (like.dtype,))
-    if len(betas) != 2 or not all(0.0 <= b < 1.0 for b in betas):
+    if not all(0.0 <= b < 1.0 for b in betas):
         raise ValueError("betas must be two values from 0 on and below 1, not %s" % (betas,))
     if not all(math.isfinite(v) for v in (lr, eps, weight_decay, grad_scale)):
         raise ValueError("lr, eps, weight_decay and grad_scale must be finite")
@@ -85,6 +90,9 @@ def adamw_update(params, grads, exp_avgs, exp_avg_sqs, scales=None, masters=None
 
 def adamw_moments(exp_avgs, exp_avg_sqs, scales):
     """What moments in 8 bits stand for: two lists of float32 tensors, of the shapes of ``exp_avgs``."""
+    done = _lib.native().adamw_moments(exp_avgs, exp_avg_sqs, scales)
+    if done is not None:
+        return done
     lib = _lib.load()
     _check_lists(exp_avgs, exp_avg_sqs=exp_avg_sqs, scales=scales)
     if not exp_avgs:

@@ -15,7 +15,8 @@ constexpr float LOG2E = 1.4426950408889634f;
 // Abramowitz & Stegun 7.1.26, whose own five coefficients bound the error of erf and not that of its tail's value (5e-4 of it
 // at z = -4, 4e-3 at -6).  The six here, with p = 0.425, are the least-squares fit of e^(u^2) erfc(u) / 2, weighted anew by its own
 // error until the largest relative one is least: 1.7e-6 for u up to 5.6.
-template <typename T, int ACT, bool SLOPE> __device__ __forceinline__ float activate(float z, float &slope)
+// FIXED: the same bits in every kernel (else it is the compiler's to contract 1 - tail with the product that tail is, or not).
+template <typename T, int ACT, bool SLOPE, bool FIXED = false> __device__ __forceinline__ float activate(float z, float &slope)
 {
     if constexpr (ACT == KSMM_ACT_SILU) {
         float s;
@@ -40,8 +41,12 @@ template <typename T, int ACT, bool SLOPE> __device__ __forceinline__ float acti
             poly = fmaf(poly, t, 0.1113554886f);
             poly = fmaf(poly, t, 0.1205461711f);
             ex = __builtin_amdgcn_exp2f(-(q * q));
-            const float tail = poly * t * ex;
-            phi = z >= 0.f ? 1.f - tail : tail;
+            if constexpr (FIXED) {
+                phi = z >= 0.f ? fmaf(-(poly * t), ex, 1.f) : poly * t * ex;
+            } else {
+                const float tail = poly * t * ex;
+                phi = z >= 0.f ? 1.f - tail : tail;
+            }
         }
         if constexpr (SLOPE) slope = fmaf(z * 0.39894228040143268f, ex, phi);
         return z * phi;

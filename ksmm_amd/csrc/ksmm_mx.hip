@@ -246,8 +246,9 @@ template <typename T, bool LAST, bool GATED, int ACT> __global__ __launch_bounds
         if (o >= p.b) continue;
         float z = acc[i], slope;
         if (bias) z += (float)bias[((int64_t)ai * rows_w + o) * p.d + di];
-        z = activate<T, ACT, false>(z, slope);
+        z = activate<T, ACT, false, true>(z, slope);
         if constexpr (GATED) z *= up[i] + (bias ? (float)bias[((int64_t)ai * rows_w + p.b + o) * p.d + di] : 0.f);
+        if constexpr (sizeof(T) == 2) asm("" : "+v"(z));
         const int64_t f = ((int64_t)ai * p.b + o) * p.d + di;
         ((T *)p.y)[LAST ? f * p.batch + n : n * p.a * p.b * p.d + f] = (T)z;
     }

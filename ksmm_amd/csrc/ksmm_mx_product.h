@@ -6,6 +6,8 @@
 // row 8j + 4h + i of a tile is its row 16h + 4j + i, so that a lane ends up with 16 consecutive outputs of a row of the batch
 // (batch-size-last: 16 consecutive rows of one output), which with those of all D leave as whole vectors.
 #pragma once
+#include <algorithm>
+
 #include "ksmm_act.h"
 #include "ksmm_mx.h"
 
@@ -51,21 +53,23 @@ template <bool LAST> __device__ __forceinline__ float16_t mx_step(uint4_t w, int
 // compiled, and without the wait the loads that are on their way are waited for with the whole tiles' stores, each time.
 __device__ __forceinline__ void mx_wait() { __builtin_amdgcn_s_waitcnt(0x0f70); }
 
-// act of a lane's results, and their stores: tile t of 32 rows of those from n0 on, tile bt of outputs
-template <typename T, bool LAST, int D, bool GATED, int ACT>
-__device__ __forceinline__ void mx_results(const MxProduct &p, const float16_t (&acc)[D][GATED ? 2 : 1], int ai, int d0, int bt, int lane, int64_t n0, int t, int here)
+// act of a lane's sums of one d_i
+template <typename T, int D, bool GATED, int ACT> __device__ __forceinline__ void mx_activate(const float16_t (&acc)[GATED ? 2 : 1], int j, T (&v)[16 * D])
 {
-    constexpr int G = GATED ? 2 : 1;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        float slope, z = activate<T, ACT, false, true>(acc[0][i], slope);
+        if constexpr (GATED) z *= acc[1][i];
+        if constexpr (sizeof(T) == 2) asm("" : "+v"(z));  // (rounded to fp32 in every kernel: else the last product and this conversion can be one)
+        v[i * D + j] = (T)z;
+    }
+}
+
+// stores of a lane's results: tile t of 32 rows of those from n0 on, tile bt of outputs
+template <typename T, bool LAST, int D>
+__device__ __forceinline__ void mx_results(const MxProduct &p, const T (&v)[16 * D], int ai, int d0, int bt, int lane, int64_t n0, int t, int here)
+{
     const int l32 = lane & 31, half = lane >> 5;
-    T v[16 * D];
-#pragma unroll
-    for (int j = 0; j < D; ++j)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            float slope, z = activate<T, ACT, false>(acc[j][0][i], slope);
-            if constexpr (GATED) z *= acc[j][G - 1][i];
-            v[i * D + j] = (T)z;
-        }
     const bool whole = (t + 1) * 32 <= here && (bt + 1) * 32 <= p.b && (LAST || p.d == D);
     if constexpr (LAST) {
         const int o = bt * 32 + l32, n = t * 32 + 16 * half;
@@ -131,23 +135,23 @@ template <typename T, bool LAST, int D, bool GATED, int ACT, int KS> __global__ 
     const int wo = bt * 32 + (LAST ? l32 : run), o = wo < p.b ? wo : p.b - 1;  // (outputs behind the last one are read as the last one)
     float *const bias = (float *)(smem + p.buffers * buffer);  // (tile of the workgroup, gate and up, D, 32 outputs)
 
-    const int tasks = TN * p.cb;
+    const int tasks = TN * p.cb, batch = (int)p.batch;  // (and steps past the end are counted in 32 bits)
     const bool emit = p.codes_out && blk / p.units == 0;
     // what a thread loads for the step of rows n0 on: the blocks of task t
     struct Load {
         MxGroup<T, D> g;
         int row, kb;  // none: row < 0
     };
-    auto fetch = [&](Load &f, int t, int64_t n0) {
+    auto fetch = [&](Load &f, int t, int n0) {
         const int kb = LAST ? t / TN : t % p.cb, n = LAST ? t - kb * TN : t / p.cb;
-        f.row = t < tasks && n < p.batch - n0 ? n : -1;
+        f.row = t < tasks && n < batch - n0 ? n : -1;
         f.kb = kb;
         if (f.row < 0) return;
         const T *x = (const T *)p.x + (LAST ? (((int64_t)ai * p.c + kb * 32) * p.d + d0) * p.batch + n0 + n
-                                            : (((n0 + n) * p.a + ai) * p.c + kb * 32) * p.d + d0);
+                                            : ((((int64_t)n0 + n) * p.a + ai) * p.c + kb * 32) * p.d + d0);
         mx_load<T, D>(f.g, x, LAST ? (int64_t)p.d * p.batch : p.d, p.c - kb * 32);
     };
-    auto keep = [&](const Load &f, int64_t n0, int which) {
+    auto keep = [&](const Load &f, int n0, int which) {
         if (f.row < 0) return;  // (rows that are not there: whatever LDS has, they are other columns of the product)
         uint8_t *const codes = smem + which * buffer, *const scales = codes + D * TN * p.slots * 16;
 #pragma unroll
@@ -166,13 +170,9 @@ template <typename T, bool LAST, int D, bool GATED, int ACT, int KS> __global__ 
     };
 
     // rows, tiles of them and what is on its way
-    const int64_t row_tiles = p.token_tiles;
+    const int row_tiles = (int)p.token_tiles;
     Load f[R];
     const bool on = first + p.row_splits < row_tiles;  // more steps than one (of 512 threads, which take a step's blocks R each)
-    if (on) {
-#pragma unroll
-        for (int r = 0; r < R; ++r) fetch(f[r], threadIdx.x + r * 512, (int64_t)first * TN);
-    }
     uint4_t w[D][G][KS];
     int sw[D][G][SW];
     if (busy) {
@@ -191,6 +191,11 @@ template <typename T, bool LAST, int D, bool GATED, int ACT, int KS> __global__ 
                 }
             }
     }
+    // (behind the weights: waiting for the first rows is waiting for these too, which no step has to do again)
+    if (on) {
+#pragma unroll
+        for (int r = 0; r < R; ++r) fetch(f[r], threadIdx.x + r * 512, first * TN);
+    }
     // (scales of blocks behind the last one are read: with weights of zeros, but not as NaN)
     for (int k = 0; k < p.buffers; ++k)
         for (int i = threadIdx.x; i < D * TN * SB / 2; i += threads) ((uint32_t *)(smem + k * buffer + D * TN * p.slots * 16))[i] = 0x7f7f7f7fu;
@@ -199,55 +204,70 @@ template <typename T, bool LAST, int D, bool GATED, int ACT, int KS> __global__ 
         bias[i] = p.bias && out < p.b ? (float)((const T *)p.bias)[((int64_t)ai * rows_w + q * p.b + out) * p.d + d0 + j] : 0.f;
     }
     __syncthreads();
-    if (on) {
-#pragma unroll
-        for (int r = 0; r < R; ++r) keep(f[r], (int64_t)first * TN, 0);
-#pragma unroll
-        for (int r = 0; r < R; ++r) fetch(f[r], threadIdx.x + r * 512, (int64_t)(first + p.row_splits) * TN);
-    } else {
+    if (!on) {
         for (int t = threadIdx.x; t < tasks; t += threads) {
-            fetch(f[0], t, (int64_t)first * TN);
-            keep(f[0], (int64_t)first * TN, 0);
+            fetch(f[0], t, first * TN);
+            keep(f[0], first * TN, 0);
         }
+        __syncthreads();
     }
-    __syncthreads();
-    int which = 0;
-    for (int64_t tile = first; tile < row_tiles; tile += p.row_splits, which ^= 1) {
-        const int64_t n0 = tile * TN;
-        const int here = (int)(p.batch - n0 < TN ? p.batch - n0 : TN);
-        if (tile + p.row_splits < row_tiles) {
+    // (said to the compiler: the weights are there, and no step waits for them again, which would be for all stores before it too)
 #pragma unroll
-            for (int r = 0; r < R; ++r) keep(f[r], (tile + p.row_splits) * TN, which ^ 1);
-            if (tile + 2 * p.row_splits < row_tiles) {
+    for (int j = 0; j < D; ++j)
 #pragma unroll
-                for (int r = 0; r < R; ++r) fetch(f[r], threadIdx.x + r * 512, (tile + 2 * p.row_splits) * TN);
+        for (int q = 0; q < G; ++q) {
+#pragma unroll
+            for (int s = 0; s < KS; ++s) asm volatile("" : "+v"(w[j][q][s]));
+#pragma unroll
+            for (int s = 0; s < SW; ++s) asm volatile("" : "+v"(sw[j][q][s]));
+        }
+    mx_wait();
+    int which = on ? 1 : 0;
+    for (int tile = on ? first - p.row_splits : first; tile < row_tiles; tile += p.row_splits, which ^= 1) {
+        const int n0 = tile * TN, next = tile + p.row_splits;
+        const int here = batch - n0 < TN ? batch - n0 : TN;
+        if (next < row_tiles) {
+#pragma unroll
+            for (int r = 0; r < R; ++r) keep(f[r], next * TN, which ^ 1);
+            if (next + p.row_splits < row_tiles) {
+#pragma unroll
+                for (int r = 0; r < R; ++r) fetch(f[r], threadIdx.x + r * 512, (next + p.row_splits) * TN);
             }
         }
         const uint8_t *const codes = smem + which * buffer, *const scales = codes + D * TN * p.slots * 16;
         int t = wt * per_wave;
-        if (busy && t * 32 < here) {
+        if (busy && tile >= 0 && t * 32 < here) {
             do {
-                float16_t acc[D][G];
-#pragma unroll
-                for (int j = 0; j < D; ++j)
-#pragma unroll
-                    for (int q = 0; q < G; ++q)
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) acc[j][q][i] = bias[((wb * G + q) * D + j) * 32 + (LAST ? l32 : 16 * half + i)];
+                T v[16 * D];
 #pragma unroll
                 for (int j = 0; j < D; ++j) {
                     const int row = j * TN + t * 32 + (LAST ? run : l32);
                     int sx[SW];
 #pragma unroll
                     for (int i = 0; i < SW; ++i) sx[i] = ((const int *)(scales + row * 2 * SB + half * SB))[i];
+                    float16_t acc[G];
+                    auto steps = [&](auto biased) {
 #pragma unroll
-                    for (int s = 0; s < KS; ++s) {
-                        const uint4_t x = *(const uint4_t *)(codes + (row * p.slots + 2 * s + half) * 16);
+                        for (int q = 0; q < G; ++q) {
+                            acc[q] = float16_t{};
+                            if constexpr (decltype(biased)::value)
 #pragma unroll
-                        for (int q = 0; q < G; ++q) acc[j][q] = mx_step<LAST>(w[j][q][s], sw[j][q][s / 4], x, sx[s / 4], s % 4, acc[j][q]);
-                    }
+                                for (int i = 0; i < 16; ++i) acc[q][i] = bias[((wb * G + q) * D + j) * 32 + (LAST ? l32 : 16 * half + i)];
+                        }
+#pragma unroll
+                        for (int s = 0; s < KS; ++s) {
+                            const uint4_t x = *(const uint4_t *)(codes + (row * p.slots + 2 * s + half) * 16);
+#pragma unroll
+                            for (int q = 0; q < G; ++q) acc[q] = mx_step<LAST>(w[j][q][s], sw[j][q][s / 4], x, sx[s / 4], s % 4, acc[q]);
+                        }
+                    };
+                    if (p.bias)
+                        steps(std::true_type());
+                    else
+                        steps(std::false_type());
+                    mx_activate<T, D, GATED, ACT>(acc, j, v);
                 }
-                mx_results<T, LAST, D, GATED, ACT>(p, acc, ai, d0, bt, lane, n0, t, here);
+                mx_results<T, LAST, D>(p, v, ai, d0, bt, lane, n0, t, here);
             } while (++t < (wt + 1) * per_wave && t * 32 < here);
         } else {
             mx_wait();
@@ -365,7 +385,12 @@ template <typename T, bool LAST, int D, int TT, bool GATED, int ACT> __global__ 
             }
 #pragma unroll
             for (int t = 0; t < TT; ++t)
-                if (t * 32 < here) mx_results<T, LAST, D, GATED, ACT>(p, acc[t], ai, d0, bt, lane, n0, t, here);
+                if (t * 32 < here) {
+                    T v[16 * D];
+#pragma unroll
+                    for (int j = 0; j < D; ++j) mx_activate<T, D, GATED, ACT>(acc[t][j], j, v);
+                    mx_results<T, LAST, D>(p, v, ai, d0, bt, lane, n0, t, here);
+                }
         }
     }
 }
@@ -434,7 +459,6 @@ template <typename T, bool LAST, int D, bool GATED, int KS> int mx_launch_held(M
     int waves = 8;
     p.wave_tiles = best;
     p.tile_rows = 32 * 8 / best;
-    while (p.tile_rows < 256 && tasks(2 * p.tile_rows) <= 512 * R && mx_held_lds(D, GATED, KS, p.cb, 2 * p.tile_rows, p.wave_tiles, 2) <= 80 * 1024) p.tile_rows *= 2;
     auto groups = [&] { return (int64_t)p.units * ((p.b_tiles + p.wave_tiles - 1) / p.wave_tiles); };
     p.token_tiles = (p.batch + p.tile_rows - 1) / p.tile_rows;
     if (groups() * p.token_tiles < 256) {  // few: smaller workgroups of one step each
@@ -447,7 +471,7 @@ template <typename T, bool LAST, int D, bool GATED, int KS> int mx_launch_held(M
     }
     // workgroups that fit at once: a wave's registers are its weights, its sums and the values on their way
     constexpr int REGS = D * (GATED ? 2 : 1) * (4 * KS + 16) + D * R * 8 * (int)sizeof(T) + 50;
-    const int64_t most = ((REGS > 128 ? 256 : 512) + groups() - 1) / groups();
+    const int64_t most = std::max<int64_t>(1, (REGS > 128 ? 256 : 512) / groups());
     p.row_splits = (int)(waves < 8 || p.token_tiles < most ? p.token_tiles : most);
     p.buffers = p.row_splits < p.token_tiles ? 2 : 1;
     const int64_t grid = groups() * p.row_splits;

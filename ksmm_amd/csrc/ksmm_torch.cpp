@@ -627,11 +627,429 @@ PyObject *py_gated_linear(PyObject *, PyObject *const *args, Py_ssize_t n_args)
     Py_RETURN_NONE;
 }
 
+// ---- microscaled 4-bit numbers --------------------------------------------------------------------------------
+
+int64_t mx_blocks(int64_t c) { return (c + 31) / 32; }
+// a tuple of n sizes from 1 on
+bool read_sizes(PyObject *o, int n, int64_t *v)
+{
+    if (!PyTuple_Check(o) || PyTuple_GET_SIZE(o) != n) return false;
+    for (int k = 0; k < n; ++k) {
+        v[k] = PyLong_AsLongLong(PyTuple_GET_ITEM(o, k));
+        if (v[k] < 1 || v[k] > 0x3fffffff) return false;
+    }
+    return true;
+}
+int read_act(PyObject *o)
+{
+    if (o == Py_None) return KSMM_ACT_NONE;
+    if (!PyUnicode_Check(o)) return -1;
+    return PyUnicode_CompareWithASCIIString(o, "silu") == 0   ? KSMM_ACT_SILU
+           : PyUnicode_CompareWithASCIIString(o, "gelu") == 0 ? KSMM_ACT_GELU
+           : PyUnicode_CompareWithASCIIString(o, "none") == 0 ? KSMM_ACT_NONE
+                                                             : -1;
+}
+// codes and scales of `matrices` matrices of rows of c values; rows, or -1
+int64_t operand_rows(const at::Tensor &codes, const at::Tensor &scales, int64_t matrices, int64_t c)
+{
+    const bool fits = codes.is_cuda() && codes.scalar_type() == at::kByte && scales.scalar_type() == at::kByte && codes.device() == scales.device() &&
+                      codes.is_contiguous() && scales.is_contiguous() && codes.dim() == 3 && scales.dim() == 3 && codes.size(0) == matrices &&
+                      scales.size(0) == matrices && codes.size(1) == scales.size(1) && codes.size(2) == 16 * mx_blocks(c) &&
+                      scales.size(2) == mx_blocks(c) && ((uintptr_t)codes.const_data_ptr() & 15) == 0;
+    return fits ? codes.size(1) : -1;
+}
+
+// mx_rows(codes, scales, matrices, c) -> rows of an operand, or None
+PyObject *py_mx_rows(PyObject *, PyObject *const *args, Py_ssize_t n_args)
+{
+    if (n_args == 4 && THPVariable_Check(args[0]) && THPVariable_Check(args[1])) {
+        const int64_t matrices = PyLong_AsLongLong(args[2]), c = PyLong_AsLongLong(args[3]);
+        if (!PyErr_Occurred()) {
+            const int64_t rows = operand_rows(THPVariable_Unpack(args[0]), THPVariable_Unpack(args[1]), matrices, c);
+            if (rows >= 0) return PyLong_FromLongLong(rows);
+        }
+    }
+    PyErr_Clear();
+    Py_RETURN_NONE;
+}
+
+at::Tensor bytes_like(const at::Tensor &x, at::IntArrayRef shape) { return at::empty(shape, x.options().dtype(at::kByte)); }
+
+// mx_quantize(x, (a, c, d), bs_last) -> (codes, scales) or None
+PyObject *py_mx_quantize(PyObject *, PyObject *const *args, Py_ssize_t n_args)
+{
+    if (n_args != 3) {
+        PyErr_SetString(PyExc_TypeError, "mx_quantize() takes 3 arguments");
+        return nullptr;
+    }
+    try {
+        int64_t v[3];
+        if (!traced() && THPVariable_Check(args[0]) && read_sizes(args[1], 3, v)) {
+            const at::Tensor &x = THPVariable_Unpack(args[0]);
+            const bool bs_last = PyObject_IsTrue(args[2]) == 1;
+            const int64_t features = v[0] * v[1] * v[2];
+            if (x.is_cuda() && trainable(x.scalar_type()) && x.dim() > 0 && x.numel() > 0 && like(x, x) && x.size(bs_last ? 0 : x.dim() - 1) == features) {
+                const int64_t rows = x.numel() / features;
+                at::Tensor codes, scales;
+                int status;
+                {
+                    WithoutGil released;
+                    DeviceScope scope(x.device().index());
+                    at::AutoDispatchBelowADInplaceOrView below;
+                    codes = bytes_like(x, {v[0] * v[2], rows, 16 * mx_blocks(v[1])});
+                    scales = bytes_like(x, {v[0] * v[2], rows, mx_blocks(v[1])});
+                    status = ksmm_mx_quantize(data_of(x), out_of(codes), out_of(scales), rows, (int)v[0], (int)v[1], (int)v[2], code_of(x.scalar_type()),
+                                              bs_last, stream_of(x));
+                }
+                if (status == KSMM_OK) return Py_BuildValue("(NN)", THPVariable_Wrap(codes), THPVariable_Wrap(scales));
+            }
+        }
+    } catch (const std::exception &) {
+    }
+    PyErr_Clear();
+    Py_RETURN_NONE;
+}
+
+// mx_dequantize(codes, scales, (a, c, d), shape, half, bs_last) -> values or None
+PyObject *py_mx_dequantize(PyObject *, PyObject *const *args, Py_ssize_t n_args)
+{
+    if (n_args != 6) {
+        PyErr_SetString(PyExc_TypeError, "mx_dequantize() takes 6 arguments");
+        return nullptr;
+    }
+    try {
+        int64_t v[3];
+        if (!traced() && THPVariable_Check(args[0]) && THPVariable_Check(args[1]) && read_sizes(args[2], 3, v) && PyTuple_Check(args[3])) {
+            const at::Tensor &codes = THPVariable_Unpack(args[0]), &scales = THPVariable_Unpack(args[1]);
+            const bool half = PyObject_IsTrue(args[4]) == 1, bs_last = PyObject_IsTrue(args[5]) == 1;
+            const int64_t rows = operand_rows(codes, scales, v[0] * v[2], v[1]);
+            c10::SmallVector<int64_t, 6> shape;
+            int64_t values = 1;
+            for (Py_ssize_t i = 0; i < PyTuple_GET_SIZE(args[3]); ++i) {
+                shape.push_back(PyLong_AsLongLong(PyTuple_GET_ITEM(args[3], i)));
+                values *= shape.back();
+            }
+            if (rows > 0 && !PyErr_Occurred() && values == rows * v[0] * v[1] * v[2]) {
+                at::Tensor x;
+                int status;
+                {
+                    WithoutGil released;
+                    DeviceScope scope(codes.device().index());
+                    at::AutoDispatchBelowADInplaceOrView below;
+                    x = at::empty(shape, codes.options().dtype(half ? at::kHalf : at::kFloat));
+                    status = ksmm_mx_dequantize(data_of(codes), data_of(scales), out_of(x), rows, (int)v[0], (int)v[1], (int)v[2], half ? KSMM_F16 : KSMM_F32,
+                                                bs_last, stream_of(codes));
+                }
+                if (status == KSMM_OK) return THPVariable_Wrap(x);
+            }
+        }
+    } catch (const std::exception &) {
+    }
+    PyErr_Clear();
+    Py_RETURN_NONE;
+}
+
+struct MxHow {
+    int a, b, c, d, act, gated;
+    bool bs_last;
+    int64_t batch;
+    int rows() const { return gated ? 2 * b : b; }
+};
+int mx_forward(const void *x, const void *x_scales, const at::Tensor &w, const at::Tensor &w_scales, const at::Tensor &bias, at::Tensor &y, at::Tensor *codes,
+               at::Tensor *scales, const MxHow &h, int act)
+{
+    const int dt = code_of(y.scalar_type());
+    const int64_t need = x_scales ? 0 : ksmm_mx_forward_workspace(h.batch, h.a, h.b, h.c, h.d, dt, h.bs_last, h.gated);
+    if (need < 0) return (int)need;
+    at::Tensor ws;
+    if (need > 0) ws = bytes_like(y, {need});
+    return ksmm_mx_forward(x, x_scales, data_of(w), data_of(w_scales), data_of(bias), out_of(y), codes ? out_of(*codes) : nullptr,
+                           scales ? out_of(*scales) : nullptr, out_of(ws), need, h.batch, h.a, h.b, h.c, h.d, dt, h.bs_last, act, h.gated, stream_of(y));
+}
+
+struct MxNode : ag::Node {
+    ag::SavedVariable in[5];  // codes and scales of x and of the factor, bias
+    MxHow how;
+    c10::SmallVector<int64_t, 6> x_shape;
+    std::string name() const override { return "MXLinearBackward"; }
+    void release_variables() override
+    {
+        std::lock_guard<std::mutex> lock(mutex_);
+        for (auto &v : in) v.reset_data();
+    }
+    ag::variable_list apply(ag::variable_list &&grads) override
+    {
+        std::lock_guard<std::mutex> lock(mutex_);
+        ag::variable_list result(3);
+        if (!grads[0].defined()) return result;
+        at::Tensor t[5], out[3];
+        for (int i = 0; i < 5; ++i) t[i] = in[i].unpack();
+        const at::Tensor dy = grads[0].contiguous();
+        {
+            at::NoGradGuard no_grad;
+            DeviceScope scope(dy.device().index());
+            const int dt = code_of(dy.scalar_type());
+            void *const stream = stream_of(dy);
+            const int64_t features = (int64_t)how.a * how.c * how.d;
+            at::Tensor x = at::empty(x_shape, dy.options()), w = at::empty({features, how.rows()}, dy.options());
+            check_status(ksmm_mx_dequantize(data_of(t[0]), data_of(t[1]), out_of(x), how.batch, how.a, how.c, how.d, dt, how.bs_last, stream));
+            check_status(ksmm_mx_dequantize(data_of(t[2]), data_of(t[3]), out_of(w), how.rows(), how.a * how.d, how.c, 1, dt, 1, stream));
+            if (task_should_compute_output(0)) out[0] = at::empty(x_shape, dy.options());
+            if (task_should_compute_output(1)) out[1] = at::empty_like(w);
+            if (t[4].defined() && task_should_compute_output(2)) out[2] = at::empty_like(t[4]);
+            if (how.gated) {
+                const int64_t need = ksmm_gated_backward_workspace(how.batch, how.a, how.b, how.c, how.d, dt, how.bs_last);
+                check_status(need < 0 ? (int)need : KSMM_OK);
+                const at::Tensor ws = bytes_like(dy, {need});
+                check_status(ksmm_gated_backward(data_of(dy), data_of(x), data_of(w), data_of(t[4]), out_of(out[0]), out_of(out[1]), out_of(out[2]),
+                                                 ws.mutable_data_ptr(), need, how.batch, how.a, how.b, how.c, how.d, dt, how.bs_last, how.act, stream));
+            } else {
+                at::Tensor z;
+                if (how.act != KSMM_ACT_NONE) {  // what the activation was applied to, computed again
+                    z = at::empty_like(dy);
+                    check_status(mx_forward(data_of(t[0]), data_of(t[1]), t[2], t[3], t[4], z, nullptr, nullptr, how, KSMM_ACT_NONE));
+                }
+                const ksmm_factor_desc f{data_of(w), how.a, how.b, how.c, how.d, dt, 1.f};
+                const int64_t need = ksmm_layer_backward_workspace(&f, 1, how.batch, dt, how.bs_last, how.act);
+                check_status(need < 0 ? (int)need : KSMM_OK);
+                const at::Tensor ws = bytes_like(dy, {need});
+                const void *inputs[] = {data_of(x)};
+                void *dw[] = {out_of(out[1])};
+                check_status(ksmm_layer_backward(&f, 1, inputs, data_of(z), data_of(dy), out_of(out[0]), dw, out_of(out[2]), ws.mutable_data_ptr(), need,
+                                                 how.batch, dt, how.bs_last, how.act, stream));
+            }
+        }
+        for (int i = 0; i < 3; ++i) result[i] = out[i];
+        return once(std::move(result), "mx_linear");
+    }
+};
+
+// mx_linear(x, factor, scales, pattern, gated, bias, act, bs_last) -> y or None; scales None: a factor in kernel format, else its codes
+PyObject *py_mx_linear(PyObject *, PyObject *const *args, Py_ssize_t n_args)
+{
+    if (n_args != 8) {
+        PyErr_SetString(PyExc_TypeError, "mx_linear() takes 8 arguments");
+        return nullptr;
+    }
+    try {
+        at::Tensor w, w_scales, bias;
+        int64_t v[4];
+        MxHow h;
+        h.gated = PyObject_IsTrue(args[4]) == 1;
+        h.act = read_act(args[6]);
+        h.bs_last = PyObject_IsTrue(args[7]) == 1;
+        bool taken = !traced() && THPVariable_Check(args[0]) && read_optional(args[1], &w) && w.defined() && read_optional(args[2], &w_scales) &&
+                     read_sizes(args[3], 4, v) && read_optional(args[5], &bias) && h.act >= 0 && (h.act != KSMM_ACT_SILU || h.gated);
+        if (taken) {
+            const at::Tensor &x = THPVariable_Unpack(args[0]);
+            const int64_t features = v[0] * v[2] * v[3], rows = h.gated ? 2 * v[1] : v[1], out_features = v[0] * v[1] * v[3];
+            const bool packed = w_scales.defined();
+            taken = x.is_cuda() && trainable(x.scalar_type()) && x.dim() > 0 && x.numel() > 0 && like(x, x) && x.size(h.bs_last ? 0 : x.dim() - 1) == features &&
+                    w.device() == x.device() && (!bias.defined() || (like(bias, x) && bias.numel() == v[0] * rows * v[3]));
+            if (taken && packed) taken = operand_rows(w, w_scales, v[0] * v[3], v[2]) == rows;
+            if (taken && !packed) taken = like(w, x) && w.dim() == 2 && w.size(0) == features && w.size(1) == rows;
+            const bool gradients =
+                taken && at::GradMode::is_enabled() && (x.requires_grad() || (!packed && w.requires_grad()) || (bias.defined() && bias.requires_grad()));
+            if (taken) {
+                h.a = (int)v[0];
+                h.b = (int)v[1];
+                h.c = (int)v[2];
+                h.d = (int)v[3];
+                h.batch = x.numel() / features;
+                c10::SmallVector<int64_t, 6> shape(x.sizes().begin(), x.sizes().end());
+                shape[h.bs_last ? 0 : shape.size() - 1] = out_features;
+                at::Tensor y, codes, scales, x_codes, x_scales;
+                int status = KSMM_OK;
+                {
+                    WithoutGil released;
+                    DeviceScope scope(x.device().index());
+                    at::AutoDispatchBelowADInplaceOrView below;
+                    y = at::empty(shape, x.options());
+                    const int64_t blocks = mx_blocks(v[2]);
+                    if (packed) {
+                        codes = w;
+                        scales = w_scales;
+                    } else {
+                        codes = bytes_like(x, {v[0] * v[3], rows, 16 * blocks});
+                        scales = bytes_like(x, {v[0] * v[3], rows, blocks});
+                        status = ksmm_mx_quantize(data_of(w), out_of(codes), out_of(scales), rows, (int)(v[0] * v[3]), h.c, 1, code_of(x.scalar_type()), 1,
+                                                  stream_of(x));
+                    }
+                    if (gradients) {
+                        x_codes = bytes_like(x, {v[0] * v[3], h.batch, 16 * blocks});
+                        x_scales = bytes_like(x, {v[0] * v[3], h.batch, blocks});
+                    }
+                    if (status == KSMM_OK)
+                        status = mx_forward(data_of(x), nullptr, codes, scales, bias, y, gradients ? &x_codes : nullptr, gradients ? &x_scales : nullptr, h, h.act);
+                }
+                if (status == KSMM_OK) {
+                    if (gradients) {
+                        std::shared_ptr<MxNode> node(new MxNode(), ag::deleteNode);
+                        node->set_next_edges(ag::collect_next_edges(x, packed ? at::Tensor() : w, bias));
+                        node->how = h;
+                        node->x_shape.assign(x.sizes().begin(), x.sizes().end());
+                        const at::Tensor *const kept[] = {&x_codes, &x_scales, &codes, &scales, &bias};
+                        for (int i = 0; i < 5; ++i) node->in[i] = ag::SavedVariable(*kept[i], false);
+                        ag::set_history(y, node);
+                    }
+                    return THPVariable_Wrap(y);
+                }
+            }
+        }
+    } catch (const std::exception &) {
+    }
+    PyErr_Clear();
+    Py_RETURN_NONE;
+}
+
+// ---- AdamW ----------------------------------------------------------------------------------------------------
+
+// tensors of a list or tuple; false: something else is among them
+bool read_tensors(PyObject *o, Py_ssize_t n, std::vector<at::Tensor> *t)
+{
+    if (!(PyList_Check(o) || PyTuple_Check(o)) || PySequence_Fast_GET_SIZE(o) != n) return false;
+    t->reserve(n);
+    for (Py_ssize_t i = 0; i < n; ++i) {
+        PyObject *item = PySequence_Fast_GET_ITEM(o, i);
+        if (!THPVariable_Check(item)) return false;
+        t->push_back(THPVariable_Unpack(item));
+    }
+    return true;
+}
+bool holds(const at::Tensor &t, int64_t n, at::ScalarType type, const at::Device &device)
+{
+    return t.scalar_type() == type && t.device() == device && t.numel() == n && t.is_contiguous() && !t._fw_grad(0).defined();
+}
+int64_t moment_scales(int64_t n) { return 2 * ((n + 31) / 32); }
+
+// adamw_update(params, grads, exp_avgs, exp_avg_sqs, scales, masters, step, lr, beta1, beta2, eps, weight_decay, grad_scale, seed, follow)
+// -> True or None
+PyObject *py_adamw_update(PyObject *, PyObject *const *args, Py_ssize_t n_args)
+{
+    if (n_args != 15) {
+        PyErr_SetString(PyExc_TypeError, "adamw_update() takes 15 arguments");
+        return nullptr;
+    }
+    try {
+        const bool small = args[4] != Py_None, master = args[5] != Py_None;
+        std::vector<at::Tensor> p, g, m, v, s, w;
+        const Py_ssize_t n = PyList_Check(args[0]) || PyTuple_Check(args[0]) ? PySequence_Fast_GET_SIZE(args[0]) : 0;
+        bool taken = !traced() && n > 0 && read_tensors(args[0], n, &p) && read_tensors(args[1], n, &g) && read_tensors(args[2], n, &m) &&
+                     read_tensors(args[3], n, &v) && (!small || read_tensors(args[4], n, &s)) && (!master || read_tensors(args[5], n, &w));
+        ksmm_adamw_desc d{};
+        at::Tensor step;
+        if (taken) {
+            if (THPVariable_Check(args[6])) {
+                step = THPVariable_Unpack(args[6]);
+                d.step = 1;
+                taken = holds(step, 1, at::kLong, p[0].device());
+                if (taken) d.device_step = step.const_data_ptr<int64_t>();
+            } else {
+                d.step = PyLong_AsLongLong(args[6]);
+            }
+            d.lr = PyFloat_AsDouble(args[7]);
+            d.beta1 = PyFloat_AsDouble(args[8]);
+            d.beta2 = PyFloat_AsDouble(args[9]);
+            d.eps = PyFloat_AsDouble(args[10]);
+            d.weight_decay = PyFloat_AsDouble(args[11]);
+            d.grad_scale = PyFloat_AsDouble(args[12]);
+            d.seed = (uint32_t)PyLong_AsUnsignedLongLongMask(args[13]);
+            d.follow = PyObject_IsTrue(args[14]) == 1;
+            d.bits = small ? 8 : 32;
+            taken = taken && !PyErr_Occurred();
+        }
+        std::vector<ksmm_adamw_tensor> table(taken ? n : 0);
+        if (taken) {
+            const at::ScalarType type = p[0].scalar_type(), state = small ? at::kByte : at::kFloat;
+            const at::Device device = p[0].device();
+            taken = p[0].is_cuda() && trainable(type);
+            for (Py_ssize_t i = 0; i < n && taken; ++i) {
+                const int64_t k = p[i].numel();
+                taken = holds(p[i], k, type, device) && holds(g[i], k, type, device) && holds(m[i], k, state, device) && holds(v[i], k, state, device) &&
+                        (!small || holds(s[i], moment_scales(k), at::kByte, device)) && (!master || holds(w[i], k, at::kFloat, device));
+                if (taken)
+                    table[i] = ksmm_adamw_tensor{p[i].mutable_data_ptr(), g[i].const_data_ptr(), master ? (float *)w[i].mutable_data_ptr() : nullptr,
+                                                 m[i].mutable_data_ptr(), v[i].mutable_data_ptr(), small ? s[i].mutable_data_ptr() : nullptr, k};
+            }
+        }
+        if (taken) {
+            int status;
+            {
+                WithoutGil released;
+                DeviceScope scope(p[0].device().index());
+                status = ksmm_adamw_update(&d, table.data(), (int)n, code_of(p[0].scalar_type()), stream_of(p[0]));
+            }
+            if (status == KSMM_OK) {
+                for (const auto *list : {&p, &m, &v, &s, &w})
+                    for (const at::Tensor &t : *list)
+                        if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+                Py_RETURN_TRUE;
+            }
+        }
+    } catch (const std::exception &) {
+    }
+    PyErr_Clear();
+    Py_RETURN_NONE;
+}
+
+// adamw_moments(exp_avgs, exp_avg_sqs, scales) -> (list, list) or None
+PyObject *py_adamw_moments(PyObject *, PyObject *const *args, Py_ssize_t n_args)
+{
+    if (n_args != 3) {
+        PyErr_SetString(PyExc_TypeError, "adamw_moments() takes 3 arguments");
+        return nullptr;
+    }
+    try {
+        std::vector<at::Tensor> m, v, s, out_m, out_v;
+        const Py_ssize_t n = PyList_Check(args[0]) || PyTuple_Check(args[0]) ? PySequence_Fast_GET_SIZE(args[0]) : 0;
+        bool taken = !traced() && n > 0 && read_tensors(args[0], n, &m) && read_tensors(args[1], n, &v) && read_tensors(args[2], n, &s) && m[0].is_cuda();
+        for (Py_ssize_t i = 0; i < n && taken; ++i) {
+            const int64_t k = m[i].numel();
+            taken = holds(m[i], k, at::kByte, m[0].device()) && holds(v[i], k, at::kByte, m[0].device()) && holds(s[i], moment_scales(k), at::kByte, m[0].device());
+        }
+        if (taken) {
+            int status;
+            {
+                WithoutGil released;
+                DeviceScope scope(m[0].device().index());
+                at::AutoDispatchBelowADInplaceOrView below;
+                std::vector<ksmm_adamw_moment> table(n);
+                const auto options = m[0].options().dtype(at::kFloat);
+                for (Py_ssize_t i = 0; i < n; ++i) {
+                    out_m.push_back(at::empty(m[i].sizes(), options));
+                    out_v.push_back(at::empty(m[i].sizes(), options));
+                    table[i] = ksmm_adamw_moment{m[i].const_data_ptr(), v[i].const_data_ptr(), s[i].const_data_ptr(), out_m[i].mutable_data_ptr<float>(),
+                                                 out_v[i].mutable_data_ptr<float>(), m[i].numel()};
+                }
+                status = ksmm_adamw_moments(table.data(), (int)n, stream_of(m[0]));
+            }
+            if (status == KSMM_OK) {
+                PyObject *lists[] = {PyList_New(n), PyList_New(n)};
+                if (!lists[0] || !lists[1]) return nullptr;
+                for (Py_ssize_t i = 0; i < n; ++i) {
+                    PyList_SET_ITEM(lists[0], i, THPVariable_Wrap(out_m[i]));
+                    PyList_SET_ITEM(lists[1], i, THPVariable_Wrap(out_v[i]));
+                }
+                return Py_BuildValue("(NN)", lists[0], lists[1]);
+            }
+        }
+    } catch (const std::exception &) {
+    }
+    PyErr_Clear();
+    Py_RETURN_NONE;
+}
+
 PyMethodDef methods[] = {
     {"train_forward", (PyCFunction)(void (*)(void))py_train_forward, METH_FASTCALL, "one layer, its intermediates kept"},
     {"train_backward", (PyCFunction)(void (*)(void))py_train_backward, METH_FASTCALL, "gradients of one layer"},
     {"residual_norm", (PyCFunction)(void (*)(void))py_residual_norm, METH_FASTCALL, "gated residual addition between two norms"},
     {"gated_linear", (PyCFunction)(void (*)(void))py_gated_linear, METH_FASTCALL, "gated projection"},
+    {"mx_rows", (PyCFunction)(void (*)(void))py_mx_rows, METH_FASTCALL, "rows of a 4-bit operand"},
+    {"mx_quantize", (PyCFunction)(void (*)(void))py_mx_quantize, METH_FASTCALL, "values as 4-bit numbers"},
+    {"mx_dequantize", (PyCFunction)(void (*)(void))py_mx_dequantize, METH_FASTCALL, "what 4-bit numbers stand for"},
+    {"mx_linear", (PyCFunction)(void (*)(void))py_mx_linear, METH_FASTCALL, "product of 4-bit numbers"},
+    {"adamw_update", (PyCFunction)(void (*)(void))py_adamw_update, METH_FASTCALL, "AdamW over many tensors"},
+    {"adamw_moments", (PyCFunction)(void (*)(void))py_adamw_moments, METH_FASTCALL, "what 8-bit moments stand for"},
     {"infer", (PyCFunction)(void (*)(void))py_infer, METH_FASTCALL, "one layer without gradients"},
     {nullptr, nullptr, 0, nullptr},
 };

@@ -36,6 +36,9 @@ def _blocks(c):
 
 def _check_codes(codes, scales, matrices, c):
     """rows of an operand"""
+    rows = _lib.native().mx_rows(codes, scales, matrices, c)
+    if rows is not None:
+        return rows
     for t, name in ((codes, "codes"), (scales, "scales")):
         _check_input(t, name)
         if t.dtype != torch.uint8 or t.device != codes.device:
@@ -50,6 +53,9 @@ def _check_codes(codes, scales, matrices, c):
 
 
 def _quantize(x, rows, a, c, d, bs_last):
+    done = _lib.native().mx_quantize(x, (a, c, d), bs_last)
+    if done is not None:
+        return done
     codes = torch.empty(a * d, rows, 16 * _blocks(c), dtype=torch.uint8, device=x.device)
     scales = torch.empty(a * d, rows, _blocks(c), dtype=torch.uint8, device=x.device)
     if rows > 0:
@@ -60,6 +66,10 @@ def _quantize(x, rows, a, c, d, bs_last):
 
 
 def _dequantize(codes, scales, shape, dtype, rows, a, c, d, bs_last):
+    if dtype in (torch.float32, torch.float16):
+        x = _lib.native().mx_dequantize(codes, scales, (a, c, d), tuple(shape), dtype == torch.float16, bs_last)
+        if x is not None:
+            return x
     x = torch.empty(shape, dtype=dtype, device=codes.device)
     if rows > 0:
         with torch.cuda.device(codes.device):
@@ -284,9 +294,15 @@ def mx_linear(x, factor, pattern=None, bias=None, act=None, gated=False, bs_last
         if gated and not factor.gated:
             raise ValueError("factor is not a gated one")
         pattern, gated = factor.pattern, factor.gated
+        out = _lib.native().mx_linear(x, factor.codes, factor.scales, pattern, gated, bias, act, bs_last)
+        if out is not None:
+            return out
     elif pattern is None:
         raise ValueError("a factor in kernel format needs its pattern")
     else:
+        out = _lib.native().mx_linear(x, factor, None, pattern, gated, bias, act, bs_last)
+        if out is not None:
+            return out
         pattern = _check_factor(factor, pattern, gated)[:4]
     if torch.jit.is_tracing() or (torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in (x, factor, bias))):
         if isinstance(x, MXTensor):

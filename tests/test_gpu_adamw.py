@@ -320,3 +320,23 @@ def test_beside_muon():
     assert all(not torch.equal(p, q) and torch.isfinite(p).all() for p, q in zip(block.parameters(), before))
     served = block.packed()
     assert torch.equal(served(block.begin(x), x)[0], block(block.begin(x), x)[0])
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_without_the_native_module(monkeypatch, bits):
+    from ksmm_amd import _lib, adamw_moments, adamw_update
+
+    def everything():
+        s = make([100, 4097], "fp16", bits, True)
+        adamw_update(s["w"], s["g"], s["m"], s["v"], s["scales"], s["master"], step=torch.full((1,), 9, device="cuda"), seed=4, **HOW)
+        version = s["w"][0]._version
+        adamw_update(s["w"], s["g"], s["m"], s["v"], s["scales"], s["master"], step=10, seed=4, **HOW)
+        assert s["w"][0]._version > version
+        out = s["w"] + s["m"] + s["v"] + s["master"]
+        return out + (sum(map(list, adamw_moments(s["m"], s["v"], s["scales"])), []) if bits == 8 else [])
+
+    native = everything()
+    assert _lib.native() is not _lib._NoNative
+    monkeypatch.setattr(_lib, "_native", _lib._NoNative)
+    for x, y in zip(native, everything()):
+        assert torch.equal(x, y)

@@ -387,3 +387,31 @@ def test_modules(bs_last):
         (n.float().sum() + r.float().sum()).backward()
     assert all(p.grad is not None and torch.isfinite(p.grad).all() for p in block.parameters())
     assert all(not any(p is q for q in block.parameters()) for p in served.parameters())
+
+
+@pytest.mark.parametrize("bs_last", [False, True])
+def test_without_the_native_module(monkeypatch, bs_last):
+    """The same results, gradients among them, through ctypes alone."""
+    from ksmm_amd import _lib, mx_linear, pack_mx, quantize_mx
+
+    def everything():
+        out = []
+        for pattern, gated, act in (((2, 40, 33, 1), False, "gelu"), ((1, 64, 96, 2), True, "silu"), ((1, 24, 64, 3), False, None)):
+            a, b, c, d = pattern
+            x, f = rows(70, a * c * d, bs_last, torch.float16).cuda(), factor(pattern, gated, torch.float16).cuda()
+            bias = torch.linspace(-1, 1, a * f.shape[1] * d).half().cuda()
+            q, w = quantize_mx(x, (a, c, d), bs_last), pack_mx(f, pattern, gated)
+            out += [q.codes, q.scales, q.dequantize(), w.codes, w.dequantize(), mx_linear(x, w, bias=bias, act=act, bs_last=bs_last)]
+            leaves = [t.clone().requires_grad_(True) for t in (x, f, bias)]
+            with torch.enable_grad():
+                y = mx_linear(leaves[0], leaves[1], pattern, bias=leaves[2], act=act, gated=gated, bs_last=bs_last)
+                out += [y.detach(), *torch.autograd.grad(y, leaves, torch.ones_like(y))]
+                y = mx_linear(leaves[0], w, bias=leaves[2], act=act, bs_last=bs_last)
+                out += [y.detach(), *torch.autograd.grad(y, [leaves[0], leaves[2]], torch.ones_like(y))]
+        return out
+
+    native = everything()
+    assert _lib.native() is not _lib._NoNative
+    monkeypatch.setattr(_lib, "_native", _lib._NoNative)
+    for x, y in zip(native, everything()):
+        assert torch.equal(x, y)
