@@ -15,15 +15,14 @@
 #include <algorithm>
 #include <cfloat>
 #include <cmath>
+#include <type_traits>
 #include <vector>
 
 namespace ksmm {
 
 namespace {
 
-constexpr int PER = 8, THREADS = 256;
-constexpr int CHUNK = THREADS * PER * 2;  // values a workgroup takes
-constexpr int MOST = 64;                  // tensors a launch: their table is a kernel argument, 4 KB at most
+constexpr int PER = 8;                    // values a thread takes at a time
 
 struct Tensor {
     void *w;
@@ -33,9 +32,33 @@ struct Tensor {
     uint8_t *scales;  // m's, then v's
     uint32_t n, first;  // values, and the first workgroup; first's highest bit: every pointer allows vectors
 };
-struct Args {
-    Tensor t[MOST];
+// The tensors of a launch are a kernel argument, of 4 KB at most: without pointers that are not there more of them fit.
+template <bool MASTER, bool SCALES> struct Entry {
+    const void *p[4 + MASTER + SCALES];
+    uint32_t n, first;
+    static constexpr bool HAS_MASTER = MASTER, HAS_SCALES = SCALES;
+    __host__ __device__ void set(const Tensor &t)
+    {
+        p[0] = t.w;
+        p[1] = t.g;
+        p[2] = t.m;
+        p[3] = t.v;
+        if constexpr (MASTER) p[4] = t.master;
+        if constexpr (SCALES) p[4 + MASTER] = t.scales;
+        n = t.n;
+        first = t.first;
+    }
+    __device__ Tensor get() const
+    {
+        Tensor t{(void *)p[0], p[1], nullptr, (void *)p[2], (void *)p[3], nullptr, n, first};
+        if constexpr (MASTER) t.master = (float *)p[4];
+        if constexpr (SCALES) t.scales = (uint8_t *)p[4 + MASTER];
+        return t;
+    }
+};
+struct Common {
     int count;
+    uint32_t chunk;  // values a workgroup takes: of 256 threads two of 8 each, or where that makes few, of 64 threads one of 8 each
     uint32_t seed;  // the first tensor's
     int follow;
     float keep, lr, rate, root, eps;  // rate, root: of the step, or (with `step`) to be found from it
@@ -43,7 +66,10 @@ struct Args {
     int64_t step;
     const int64_t *device_step;
 };
-static_assert(sizeof(Args) <= 4096, "kernel arguments");
+template <typename E> struct Args : Common {
+    static constexpr int MOST = (int)((4096 - sizeof(Common)) / sizeof(E)) < 128 ? (int)((4096 - sizeof(Common)) / sizeof(E)) : 128;
+    E t[MOST];
+};
 
 __host__ __device__ __forceinline__ uint32_t mix(uint32_t x)
 {
@@ -52,18 +78,12 @@ __host__ __device__ __forceinline__ uint32_t mix(uint32_t x)
     return x ^ x >> 16;
 }
 
-// the tensor that workgroup `group` works on
-__device__ __forceinline__ int tensor_of(const Tensor *t, int count, uint32_t group)
+// the tensor that workgroup `group` works on: of all that begin at it or before, the last (every lane looks at two)
+template <typename E> __device__ __forceinline__ int tensor_of(const Args<E> &a, uint32_t group)
 {
-    int low = 0, high = count;  // low's first <= group < high's
-    while (high - low > 1) {
-        const int middle = (low + high) / 2;
-        if ((t[middle].first & 0x7fffffffu) <= group)
-            low = middle;
-        else
-            high = middle;
-    }
-    return low;
+    const int lane = threadIdx.x & 63;
+    auto before = [&](int i) { return __popcll(__ballot(i < a.count && (a.t[i].first & 0x7fffffffu) <= group)); };
+    return before(lane) + (a.count > 64 ? before(lane + 64) : 0) - 1;
 }
 
 template <typename T> struct Values {
@@ -92,7 +112,6 @@ template <typename T> __device__ __forceinline__ void store(T *p, uint32_t at, u
     }
 }
 
-__device__ __forceinline__ double power64(int e) { return __builtin_bit_cast(double, (uint64_t)(e + 1023) << 52); }
 __device__ __forceinline__ int exponent64(double v) { return (int)(__builtin_bit_cast(uint64_t, v) >> 52 & 0x7ff) - 1023; }
 __device__ __forceinline__ float scale_value(uint8_t byte)
 {
@@ -102,63 +121,80 @@ __device__ __forceinline__ float scale_value(uint8_t byte)
 // largest of the four lanes that hold a block of 32
 __device__ __forceinline__ int block_max(int v)
 {
-    v = max(v, __shfl_xor(v, 1, 64));
-    return max(v, __shfl_xor(v, 2, 64));
+    v = max(v, __builtin_amdgcn_mov_dpp(v, 0xb1, 0xf, 0xf, true));  // lanes 1 0 3 2
+    return max(v, __builtin_amdgcn_mov_dpp(v, 0x4e, 0xf, 0xf, true));  // 2 3 0 1
 }
 
 constexpr int LOWEST = -120;  // exponent of a scale
 
-// |y| 2^-e, to 3 bits behind its leading one from exponent `least` on, down or up as the dither (in 2^-16) says
-__device__ __forceinline__ float rounded(double y, int e, int least, uint32_t dither)
+// y 2^-e (y >= 0, its exponent given) to 3 bits behind its leading one from exponent `least` on, down or up as the dither (in 2^-16)
+// says, as the code of an 8-bit number: steps of its exponent E are 8 to 16 (below, of `least`, 0 to 8), and (E - least) 8 + steps
+// carries into the exponent by itself.
+__device__ __forceinline__ uint32_t rounded(double y, int exponent, int e, int least, uint32_t dither)
 {
-    const int q = max(exponent64(y) - e, least) - 3;
-    const double steps = floor(y * power64(-e - q) + (double)dither * (1.0 / 65536));
-    return (float)steps * __builtin_bit_cast(float, (uint32_t)(q + 127) << 23);
+    const int E = max(exponent - e, least);
+    const double steps = fma((double)dither, 1.0 / 65536, __builtin_ldexp(y, 3 - e - E));
+    uint32_t code = (uint32_t)(E - least) * 8 + (uint32_t)steps;
+    asm("" : "+v"(code));  // (found for every value, and not behind a branch on whether it is finite)
+    return code;
 }
 
-// e5m3 from what `rounded` gives
-__device__ __forceinline__ uint8_t e5m3(float v) { return (uint8_t)(__builtin_bit_cast(uint16_t, (half_t)v) >> 7); }
 __device__ __forceinline__ float from_e5m3(uint8_t code) { return (float)__builtin_bit_cast(half_t, (uint16_t)(code << 7)); }
 __device__ __forceinline__ float from_e4m3(uint8_t code) { return __builtin_amdgcn_cvt_f32_fp8(code, 0); }
 
-// A block's new moments as codes, and its scale; every lane of the four has eight of its values.
+// A block's new moments as codes, and its scale; every lane of the four has eight of its values.  What is 2^128 or more, or NaN, is not
+// counted among the largest.
 __device__ __forceinline__ uint8_t encode_m(const double (&m)[PER], const uint32_t (&h)[PER], Values<uint8_t> &code)
 {
-    int top = -1023;
+    int top = -1023, at[PER];
 #pragma unroll
-    for (int i = 0; i < PER; ++i) top = max(top, fabs(m[i]) <= FLT_MAX ? exponent64(m[i]) : -1023);
+    for (int i = 0; i < PER; ++i) {
+        at[i] = exponent64(m[i]);
+        top = max(top, at[i] < 128 ? at[i] : -1023);
+    }
     const int e = max(block_max(top) - 7, LOWEST);
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-        const bool finite = fabs(m[i]) <= FLT_MAX;
-        const float v = copysignf(finite ? rounded(fabs(m[i]), e, -6, h[i] & 0xffff) : 0.f, (float)m[i]);
-        code.v[i] = finite ? (uint8_t)__builtin_amdgcn_cvt_pk_fp8_f32(v, v, 0, false) : 0x7f;
+        const uint32_t sign = (uint32_t)(__builtin_bit_cast(uint64_t, m[i]) >> 63) << 7;
+        const uint32_t c = rounded(fabs(m[i]), at[i], e, -6, h[i] & 0xffff) | sign;
+        code.v[i] = (uint8_t)(at[i] < 128 ? c : 0x7f);  // (NaN)
     }
     return (uint8_t)(e + 127);
 }
 __device__ __forceinline__ uint8_t encode_v(const double (&v)[PER], const uint32_t (&h)[PER], Values<uint8_t> &code)
 {
-    int top = -1023;
+    int top = -1023, at[PER];
 #pragma unroll
-    for (int i = 0; i < PER; ++i) top = max(top, v[i] <= FLT_MAX ? exponent64(v[i]) : -1023);
+    for (int i = 0; i < PER; ++i) {
+        at[i] = exponent64(v[i]);
+        top = max(top, at[i] < 128 ? at[i] : -1023);
+    }
     const int e = max(block_max(top) - 14, LOWEST);
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-        const bool finite = v[i] <= FLT_MAX;
-        const uint8_t c = finite ? e5m3(rounded(v[i], e, -14, h[i] >> 16)) : v[i] > 0 ? 0xf8 : 0xfc;  // (infinity, NaN)
-        code.v[i] = c == 0 && v[i] > 0 ? 1 : c;
+        const uint32_t c = rounded(v[i], at[i], e, -14, h[i] >> 16), least = v[i] > 0 ? 1 : 0;
+        code.v[i] = (uint8_t)(at[i] < 128 ? max(c, least) : v[i] > 0 ? 0xf8 : 0xfc);  // (infinity, NaN)
     }
     return (uint8_t)(e + 127);
 }
 
-template <typename T, int BITS, bool MASTER> __global__ __launch_bounds__(THREADS) void ks_adamw_kernel(Args a)
+// sqrt and quotient, good to a few 2^-24 of the value: the correctly rounded ones take 25 instructions more a value.  The instruction
+// takes what is subnormal as zero, so that small values are moved up before it.
+__device__ __forceinline__ float root_of(float v)
+{
+    const bool small = v < 0x1p-96f;
+    const float r = __builtin_amdgcn_sqrtf(small ? v * 0x1p96f : v);
+    return small ? r * 0x1p-48f : r;
+}
+
+template <typename T, int BITS, bool MASTER> __global__ __launch_bounds__(256) void ks_adamw_kernel(Args<Entry<MASTER, BITS == 8>> a)
 {
 #pragma clang fp contract(off)
     __shared__ float of_step[2];
-    const int which = tensor_of(a.t, a.count, blockIdx.x);
-    const Tensor &t = a.t[which];
+    const int which = tensor_of(a, blockIdx.x);
+    const Tensor t = a.t[which].get();
     const bool aligned = t.first >> 31;
-    const uint32_t n = t.n, start = (blockIdx.x - (t.first & 0x7fffffffu)) * (uint32_t)CHUNK;
+    const uint32_t n = t.n, start = (blockIdx.x - (t.first & 0x7fffffffu)) * a.chunk;
     int64_t step = a.step;
     float rate = a.rate, root = a.root;
     if (a.device_step) {
@@ -174,7 +210,7 @@ template <typename T, int BITS, bool MASTER> __global__ __launch_bounds__(THREAD
     }
     const uint32_t key = mix(mix(a.seed + (uint32_t)which) + (uint32_t)step);
     const double beta1 = a.beta1, beta2 = a.beta2, other1 = 1.0 - beta1, other2 = 1.0 - beta2;
-    for (uint32_t at = start + threadIdx.x * PER; at < start + CHUNK; at += THREADS * PER) {
+    for (uint32_t at = start + threadIdx.x * PER; at < start + a.chunk; at += blockDim.x * PER) {
         // (the lanes of a block of 32 stay together: those behind the end hold zeros)
         if ((at & ~31u) >= n) break;
         const bool whole = aligned && at + PER <= n;
@@ -220,7 +256,7 @@ template <typename T, int BITS, bool MASTER> __global__ __launch_bounds__(THREAD
         for (int i = 0; i < PER; ++i) {
             float old = (float)w.v[i];
             if constexpr (MASTER) old = a.follow && (T)master.v[i] != w.v[i] ? old : master.v[i];
-            const float next = a.keep * old - rate * (m_new[i] / (sqrtf(v_new[i]) * root + a.eps));
+            const float next = a.keep * old - rate * (m_new[i] * __builtin_amdgcn_rcpf(root_of(v_new[i]) * root + a.eps));
             if constexpr (MASTER) master.v[i] = next;
             w.v[i] = (T)next;
         }
@@ -230,12 +266,12 @@ template <typename T, int BITS, bool MASTER> __global__ __launch_bounds__(THREAD
 }
 
 // What 8-bit moments stand for (w, master: where m and v go, as fp32).
-__global__ __launch_bounds__(THREADS) void ks_adamw_moments_kernel(Args a)
+__global__ __launch_bounds__(256) void ks_adamw_moments_kernel(Args<Entry<true, true>> a)
 {
-    const Tensor &t = a.t[tensor_of(a.t, a.count, blockIdx.x)];
+    const Tensor t = a.t[tensor_of(a, blockIdx.x)].get();
     const bool aligned = t.first >> 31;
-    const uint32_t n = t.n, start = (blockIdx.x - (t.first & 0x7fffffffu)) * (uint32_t)CHUNK, blocks = (n + 31) / 32;
-    for (uint32_t at = start + threadIdx.x * PER; at < start + CHUNK && at < n; at += THREADS * PER) {
+    const uint32_t n = t.n, start = (blockIdx.x - (t.first & 0x7fffffffu)) * a.chunk, blocks = (n + 31) / 32;
+    for (uint32_t at = start + threadIdx.x * PER; at < start + a.chunk && at < n; at += blockDim.x * PER) {
         const bool whole = aligned && at + PER <= n;
         const Values<uint8_t> cm = load((const uint8_t *)t.m, at, n, whole), cv = load((const uint8_t *)t.v, at, n, whole);
         const float sm = scale_value(t.scales[at / 32]), sv = scale_value(t.scales[blocks + at / 32]);
@@ -271,26 +307,34 @@ void add(std::vector<Range> &r, const void *p, int64_t bytes, bool written)
     if (p && bytes > 0) r.push_back(Range{(uintptr_t)p, (uintptr_t)p + (uintptr_t)bytes, written});
 }
 
-template <typename F> int in_tables(Args &a, const Tensor *all, int n, F launch)
+template <typename E, typename F> int in_tables(const Common &common, const Tensor *all, int n, F launch)
 {
+    Args<E> a;
+    (Common &)a = common;
     uint32_t groups = 0;
     int first = 0;
     const uint32_t seed = a.seed;
+    int64_t values = 0;
+    for (int i = 0; i < n; ++i) values += all[i].n;
+    // (172 thousand 8-bit values of 25 tensors: 10.6 us in workgroups of 256 threads)
+    const int threads = values < 1 << 20 ? 64 : 256;
+    a.chunk = threads == 64 ? 64 * PER : 256 * PER * 2;
     a.count = 0;
     for (int i = 0; i <= n; ++i) {
-        const uint32_t more = i < n ? (all[i].n + CHUNK - 1) / CHUNK : 0;
+        const uint32_t more = i < n ? (all[i].n + a.chunk - 1) / a.chunk : 0;
         // (a table's workgroups are counted in 31 bits)
-        if (a.count > 0 && (i == n || a.count == MOST || (uint64_t)groups + more > 0x7fffffffu)) {
+        if (a.count > 0 && (i == n || a.count == Args<E>::MOST || (uint64_t)groups + more > 0x7fffffffu)) {
             a.seed = seed + (uint32_t)first;
-            launch(groups);
+            launch(a, groups, threads);
             if (hipGetLastError() != hipSuccess) return KSMM_ERR_LAUNCH;
             groups = 0;
             a.count = 0;
         }
         if (i == n) break;
         if (a.count == 0) first = i;
-        Tensor &t = a.t[a.count++] = all[i];
+        Tensor t = all[i];
         t.first |= groups;
+        a.t[a.count++].set(t);
         groups += more;
     }
     return KSMM_OK;
@@ -330,7 +374,7 @@ int ksmm_adamw_update(const ksmm_adamw_desc *desc, const ksmm_adamw_tensor *tens
         for (int i = 0; i < count; ++i) {
             const ksmm_adamw_tensor &t = tensors[i];
             if (t.n < 0) return KSMM_ERR_BAD_BATCH;
-            if (t.n > 0x7fffffffLL - CHUNK) return KSMM_ERR_TOO_LARGE;
+            if (t.n > 0x7fffffffLL - 8192) return KSMM_ERR_TOO_LARGE;
             if (t.n > 0) {  // (pointers of empty tensors say nothing)
                 if (!any) master = t.master != nullptr;
                 any = true;
@@ -348,7 +392,7 @@ int ksmm_adamw_update(const ksmm_adamw_desc *desc, const ksmm_adamw_tensor *tens
             all.push_back(Tensor{t.weight, t.grad, t.master, t.m, t.v, (uint8_t *)t.scales, (uint32_t)t.n, vectors ? 0x80000000u : 0u});
         }
         if (any_alias(ranges)) return KSMM_ERR_ALIAS;
-        Args a{};
+        Common a{};
         const double at = (double)desc->step;
         a.seed = desc->seed;
         a.follow = desc->follow;
@@ -363,17 +407,18 @@ int ksmm_adamw_update(const ksmm_adamw_desc *desc, const ksmm_adamw_tensor *tens
         a.step = desc->step;
         a.device_step = desc->device_step;
         hipStream_t s = (hipStream_t)stream;
-        auto run = [&](auto kernel) {
-            return in_tables(a, all.data(), count, [&](uint32_t groups) {
-                if (groups > 0) hipLaunchKernelGGL(kernel, dim3(groups), dim3(THREADS), 0, s, a);
+        auto run = [&](auto of, auto masters, auto states) {
+            typedef decltype(of) T;
+            constexpr bool MASTER = decltype(masters)::value, SMALL = decltype(states)::value;
+            return in_tables<Entry<MASTER, SMALL>>(a, all.data(), count, [&](const Args<Entry<MASTER, SMALL>> &args, uint32_t groups, int threads) {
+                if (groups > 0) hipLaunchKernelGGL((ks_adamw_kernel<T, SMALL ? 8 : 32, MASTER>), dim3(groups), dim3(threads), 0, s, args);
             });
         };
-        if (dtype == KSMM_F32) {
-            if (master) return small ? run(&ks_adamw_kernel<float, 8, true>) : run(&ks_adamw_kernel<float, 32, true>);
-            return small ? run(&ks_adamw_kernel<float, 8, false>) : run(&ks_adamw_kernel<float, 32, false>);
-        }
-        if (master) return small ? run(&ks_adamw_kernel<half_t, 8, true>) : run(&ks_adamw_kernel<half_t, 32, true>);
-        return small ? run(&ks_adamw_kernel<half_t, 8, false>) : run(&ks_adamw_kernel<half_t, 32, false>);
+        auto with = [&](auto of) {
+            if (master) return small ? run(of, std::true_type(), std::true_type()) : run(of, std::true_type(), std::false_type());
+            return small ? run(of, std::false_type(), std::true_type()) : run(of, std::false_type(), std::false_type());
+        };
+        return dtype == KSMM_F32 ? with(0.f) : with((half_t)0.f);
     } catch (...) {  // (no memory for the tables)
         return KSMM_ERR_TOO_LARGE;
     }
@@ -391,7 +436,7 @@ int ksmm_adamw_moments(const ksmm_adamw_moment *tensors, int count, void *stream
         for (int i = 0; i < count; ++i) {
             const ksmm_adamw_moment &t = tensors[i];
             if (t.n < 0) return KSMM_ERR_BAD_BATCH;
-            if (t.n > 0x7fffffffLL - CHUNK) return KSMM_ERR_TOO_LARGE;
+            if (t.n > 0x7fffffffLL - 8192) return KSMM_ERR_TOO_LARGE;
             if (t.n > 0 && (!t.m || !t.v || !t.scales || !t.m_out || !t.v_out)) return KSMM_ERR_NULL_POINTER;
             add(ranges, t.m, t.n, false);
             add(ranges, t.v, t.n, false);
@@ -402,9 +447,9 @@ int ksmm_adamw_moments(const ksmm_adamw_moment *tensors, int count, void *stream
             all.push_back(Tensor{t.m_out, nullptr, t.v_out, (void *)t.m, (void *)t.v, (uint8_t *)t.scales, (uint32_t)t.n, vectors ? 0x80000000u : 0u});
         }
         if (any_alias(ranges)) return KSMM_ERR_ALIAS;
-        Args a{};
-        return in_tables(a, all.data(), count, [&](uint32_t groups) {
-            if (groups > 0) hipLaunchKernelGGL(ks_adamw_moments_kernel, dim3(groups), dim3(THREADS), 0, (hipStream_t)stream, a);
+        Common a{};
+        return in_tables<Entry<true, true>>(a, all.data(), count, [&](const Args<Entry<true, true>> &args, uint32_t groups, int threads) {
+            if (groups > 0) hipLaunchKernelGGL(ks_adamw_moments_kernel, dim3(groups), dim3(threads), 0, (hipStream_t)stream, args);
         });
     } catch (...) {
         return KSMM_ERR_TOO_LARGE;

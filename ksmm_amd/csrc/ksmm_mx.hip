@@ -69,8 +69,8 @@ template <typename T, int D, bool BACK> __global__ __launch_bounds__(THREADS) vo
                     e[k] = (float)v[k * D + j];
                     top = max(top, mx_bits(e[k]));
                 }
-                top = max(top, (uint32_t)__shfl_xor((int)top, 1, 64));
-                top = max(top, (uint32_t)__shfl_xor((int)top, 2, 64));
+                top = max(top, (uint32_t)__builtin_amdgcn_mov_dpp((int)top, 0xb1, 0xf, 0xf, true));  // lanes 1 0 3 2
+                top = max(top, (uint32_t)__builtin_amdgcn_mov_dpp((int)top, 0x4e, 0xf, 0xf, true));  // 2 3 0 1
                 const int scale = mx_scale(top);
                 ((uint32_t *)p.codes)[block * 4 + quarter] = scale == MX_NAN ? 0u : mx_encode8(e, mx_power(scale));
                 if (quarter == 0) p.scales[block] = (uint8_t)scale;

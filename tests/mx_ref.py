@@ -110,7 +110,7 @@ def _down_or_up(y, r, least):
 def encode_moments(m, v, r, s):
     n = m.numel()
     pad = -n % 32
-    finite_m, finite_v = m.abs() <= torch.finfo(torch.float32).max, v <= torch.finfo(torch.float32).max
+    finite_m, finite_v = m.abs() < 2.0 ** 128, v < 2.0 ** 128
     x, y = (torch.nn.functional.pad(torch.where(f, t, torch.zeros_like(t)), (0, pad)).reshape(-1, 32) for t, f in ((m, finite_m), (v, finite_v)))
     em = (exponent(x.abs().amax(1)) - 7).clamp(min=LOWEST)
     ev = (exponent(y.amax(1)) - 14).clamp(min=LOWEST)
