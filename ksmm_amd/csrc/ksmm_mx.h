@@ -158,7 +158,9 @@ int mx_float_last_gated(const MxProduct &p, int act, hipStream_t s);
 inline int mx_run_of(int d) { return d <= 4 ? d : d % 4 == 0 ? 4 : d % 3 == 0 ? 3 : d % 2 == 0 ? 2 : 1; }
 // tiles of 32 rows: what 128 accumulators hold
 constexpr int mx_rows_of(int d, bool gated) { return d * (gated ? 2 : 1) <= 2 ? 4 : d * (gated ? 2 : 1) <= 4 ? 2 : 1; }
-inline int64_t mx_lds(int tt, int d, int cb) { return (int64_t)d * 32 * tt * (16 * (cb | 1) + cb); }
+constexpr int MX_WAVES = 4;                           // of a workgroup that reads its weights from the caches
+constexpr int MX_LINE = 144, MX_STAGE = 32 * MX_LINE;  // LDS of a wave for its results: 128 bytes of 32 lines, 16 between them for the banks' sake
+inline int64_t mx_lds(int tt, int d, int cb) { return (int64_t)d * 32 * tt * (16 * (cb | 1) + cb) + MX_WAVES * MX_STAGE; }
 constexpr int64_t MX_LDS_MOST = 80 * 1024;  // two workgroups a compute unit
 
 // whether an operand's codes fit LDS, so that it is quantised there

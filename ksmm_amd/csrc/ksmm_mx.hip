@@ -6,8 +6,7 @@
 // Operands are kept as the a*d matrices that the products take, (a*d, rows, c) with c in blocks of 32, the last one filled
 // with zeros: 16 bytes of codes a block, the even place in the lower half of a byte, and a byte of scale.  That is what a lane
 // of the scaled matrix instructions holds: 32 numbers of one row and their scale.
-#include "ksmm_act.h"
-#include "ksmm_mx.h"
+#include "ksmm_mx_product.h"
 
 namespace ksmm {
 
@@ -199,8 +198,6 @@ template <typename T, bool BACK> __global__ __launch_bounds__(THREADS) void ks_m
     }
 }
 
-typedef int int8_v __attribute__((ext_vector_type(8)));
-
 // 32 numbers and their scale of row `row` (< rows, else zeros), block kb (< cb, else zeros)
 __device__ __forceinline__ int8_v mx_operand(const uint8_t *codes, const uint8_t *scales, int64_t row, bool there, int kb, int cb, int *scale)
 {
@@ -244,9 +241,9 @@ template <typename T, bool LAST, bool GATED, int ACT> __global__ __launch_bounds
     for (int i = 0; i < 16; ++i) {
         const int o = bt * 32 + 8 * (i / 4) + 4 * half + (i & 3);
         if (o >= p.b) continue;
-        float z = acc[i], slope;
+        float z = acc[i];
         if (bias) z += (float)bias[((int64_t)ai * rows_w + o) * p.d + di];
-        z = activate<T, ACT, false, true>(z, slope);
+        z = mx_act<T, GATED, ACT>(z);
         if constexpr (GATED) z *= up[i] + (bias ? (float)bias[((int64_t)ai * rows_w + p.b + o) * p.d + di] : 0.f);
         if constexpr (sizeof(T) == 2) asm("" : "+v"(z));
         const int64_t f = ((int64_t)ai * p.b + o) * p.d + di;

@@ -23,8 +23,6 @@ __device__ __forceinline__ float16_t mx_mfma(uint4_t a, int sa, uint4_t b, int s
     return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(mx_widen(a), mx_widen(b), c, 4, 4, 0, sa, 0, sb);
 }
 
-constexpr int MX_WAVES = 4;
-
 // N elements to p, as 16-byte stores at the elements' alignment
 template <typename T, int N> __device__ __forceinline__ void mx_store(T *p, const T (&v)[N])
 {
@@ -49,94 +47,125 @@ template <bool LAST> __device__ __forceinline__ float16_t mx_step(uint4_t w, int
     default: return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, b, c, 4, 4, 3, sa, 3, sb);
     }
 }
-// Waits for all loads and stores.  Behind the stores of a tile that is not whole: how many those are is not known when this is
-// compiled, and without the wait the loads that are on their way are waited for with the whole tiles' stores, each time.
-__device__ __forceinline__ void mx_wait() { __builtin_amdgcn_s_waitcnt(0x0f70); }
+// Of one factor in fp32 GELU is the epilogues' form (1.5e-7 of it off, 12 instructions), as everywhere; the library's erfc, which is right
+// in the smallest values too, takes five times as many, and is for those that are multiplied with another projection.
+template <typename T, bool GATED, int ACT> __device__ __forceinline__ float mx_act(float z)
+{
+    float slope;
+    if constexpr (ACT == KSMM_ACT_GELU && sizeof(T) == 4 && !GATED) return gelu_erf(z);
+    return activate<T, ACT, false, true>(z, slope);
+}
 
 // act of a lane's sums of one d_i
 template <typename T, int D, bool GATED, int ACT> __device__ __forceinline__ void mx_activate(const float16_t (&acc)[GATED ? 2 : 1], int j, T (&v)[16 * D])
 {
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-        float slope, z = activate<T, ACT, false, true>(acc[0][i], slope);
+        float z = mx_act<T, GATED, ACT>(acc[0][i]);
         if constexpr (GATED) z *= acc[1][i];
         if constexpr (sizeof(T) == 2) asm("" : "+v"(z));  // (rounded to fp32 in every kernel: else the last product and this conversion can be one)
         v[i * D + j] = (T)z;
     }
 }
 
+// Stores of a wave's tile, 32 lines (rows of the batch, or batch-size-last outputs) of 32 * D values in a row, of which every lane has a
+// half: straight from the lanes every instruction writes 64 pieces of 16 bytes apart; by way of LDS lanes that follow one another write
+// bytes that do.  `stage`: MX_STAGE bytes of the wave's own; y: the first line, `pitch` values to the next.
+template <typename T, int N> __device__ __forceinline__ void mx_store_lines(uint8_t *stage, T *y, int64_t pitch, const T (&v)[N], int lane)
+{
+    constexpr int PIECE = N * (int)sizeof(T) % 64 == 0 ? 64 : 32, PIECES = N * (int)sizeof(T) / PIECE;  // bytes of a lane at a time
+    static_assert(PIECES * PIECE == N * (int)sizeof(T), "pieces of a lane's values");
+    constexpr int CHUNKS = PIECE / 16, LANES = 2 * CHUNKS;  // of 16 bytes; lanes that share a line
+    const int l32 = lane & 31, half = lane >> 5;
+#pragma unroll
+    for (int q = 0; q < PIECES; ++q) {
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int i = 0; i < CHUNKS; ++i) __builtin_memcpy(__builtin_assume_aligned(stage + l32 * MX_LINE + half * PIECE + i * 16, 16), (const char *)v + q * PIECE + i * 16, 16);
+        __builtin_amdgcn_wave_barrier();
+        const int line = lane / LANES, chunk = lane % LANES;
+        // (both halves of a lane's values are N apart)
+        char *to = (char *)(y + line * pitch) + (chunk / CHUNKS) * (N * (int)sizeof(T)) + q * PIECE + chunk % CHUNKS * 16;
+        const int64_t step = pitch * (64 / LANES) * (int64_t)sizeof(T);
+#pragma unroll
+        for (int i = 0; i < 32 * LANES / 64; ++i) {
+            const uint4_t r = *(const uint4_t *)(stage + (line + i * (64 / LANES)) * MX_LINE + chunk * 16);
+            *(uint4_any *)to = r;
+            to += step;
+        }
+    }
+}
+
 // stores of a lane's results: tile t of 32 rows of those from n0 on, tile bt of outputs
 template <typename T, bool LAST, int D>
-__device__ __forceinline__ void mx_results(const MxProduct &p, const T (&v)[16 * D], int ai, int d0, int bt, int lane, int64_t n0, int t, int here)
+__device__ __forceinline__ void mx_results(const MxProduct &p, const T (&v)[16 * D], int ai, int d0, int bt, int lane, int64_t n0, int t, int here, uint8_t *stage)
 {
     const int l32 = lane & 31, half = lane >> 5;
-    const bool whole = (t + 1) * 32 <= here && (bt + 1) * 32 <= p.b && (LAST || p.d == D);
+    if ((t + 1) * 32 <= here && (bt + 1) * 32 <= p.b && (LAST || p.d == D)) {
+        const int64_t pitch = LAST ? (int64_t)p.d * p.batch : (int64_t)p.a * p.b * p.d;
+        T *const y = (T *)p.y + (LAST ? (((int64_t)ai * p.b + bt * 32) * p.d + d0) * p.batch + n0 + t * 32
+                                      : (((n0 + t * 32) * p.a + ai) * p.b + bt * 32) * p.d + d0);
+        mx_store_lines<T, 16 * D>(stage, y, pitch, v, lane);
+        return;
+    }
     if constexpr (LAST) {
         const int o = bt * 32 + l32, n = t * 32 + 16 * half;
         T *const y = (T *)p.y + (((int64_t)ai * p.b + o) * p.d + d0) * p.batch + n0 + n;
-        if (whole) {
-            mx_store<T, 16>(y, v);
-        } else {
-            if (o < p.b) {
+        if (o >= p.b) return;
 #pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    if (n + i < here) y[i] = v[i];
-            }
-            mx_wait();
-        }
+        for (int i = 0; i < 16; ++i)
+            if (n + i < here) y[i] = v[i];
     } else {
         const int o = bt * 32 + 16 * half, n = t * 32 + l32;
         T *const y = (T *)p.y + (((n0 + n) * p.a + ai) * p.b + o) * p.d + d0;
-        if (whole) {
+        struct __attribute__((packed, aligned(sizeof(T)))) Run {
+            T e[D];
+        };
+        if (n >= here) return;
+        if (p.d == D && o + 16 <= p.b) {
             mx_store<T, 16 * D>(y, v);
         } else {
-            struct __attribute__((packed, aligned(sizeof(T)))) Run {
-                T e[D];
-            };
-            if (n < here) {
-                if (p.d == D && o + 16 <= p.b) {
-                    mx_store<T, 16 * D>(y, v);
-                } else {
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        if (o + i >= p.b) continue;
-                        Run r;
+            for (int i = 0; i < 16; ++i) {
+                Run r;
 #pragma unroll
-                        for (int j = 0; j < D; ++j) r.e[j] = v[i * D + j];
-                        *(Run *)(y + (int64_t)i * p.d) = r;
-                    }
-                }
+                for (int j = 0; j < D; ++j) r.e[j] = v[i * D + j];
+                if (o + i < p.b) *(Run *)(y + (int64_t)i * p.d) = r;
             }
-            mx_wait();
         }
     }
 }
 
 // ---- weights in registers ---------------------------------------------------------------------------------
 // A wave holds the codes of its 32 outputs (of all D, gate and up) for the whole launch, KS steps of 64 along c, and walks down the
-// batch: a workgroup's waves are WB tiles of outputs times WT runs of rows.  Each step's rows of x are quantised into one of two
-// buffers in LDS while the rows before are multiplied, and the values of the rows after are on their way in registers.
+// batch: a workgroup's eight waves are tiles of outputs times runs of rows.  Four more waves quantise the rows of the next step into
+// the other of two buffers in LDS and have the values of the step after that on their way: waits for what is loaded would be waits for the
+// stores before it too (one counter), which only waves that store nothing do not make.
+// Where there are few steps each workgroup takes one, of fewer waves, which first quantise and then multiply.
+constexpr int MX_CONSUMERS = 8, MX_PRODUCERS = 4;
 constexpr int mx_scale_bytes(int ks) { return ks <= 4 ? 4 : ks <= 8 ? 8 : 16; }  // of a row and one half of each step
+constexpr int mx_rounds(int ks) { return ks <= 4 ? 1 : ks <= 8 ? 2 : 4; }        // blocks of 32 rows that a producer's thread takes
 
-template <typename T, bool LAST, int D, bool GATED, int ACT, int KS> __global__ __launch_bounds__(512) void ks_mx_held_kernel(MxProduct p)
+template <typename T, bool LAST, int D, bool GATED, int ACT, int KS>
+__global__ __launch_bounds__(64 * (MX_CONSUMERS + MX_PRODUCERS)) void ks_mx_held_kernel(MxProduct p)
 {
-    constexpr int G = GATED ? 2 : 1, SB = mx_scale_bytes(KS), SW = (KS + 3) / 4, R = KS > 8 ? 2 : 1;
+    constexpr int G = GATED ? 2 : 1, SB = mx_scale_bytes(KS), SW = (KS + 3) / 4, R = mx_rounds(KS);
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
-    const int threads = blockDim.x, waves = threads >> 6, TN = p.tile_rows, buffer = D * TN * (p.slots * 16 + 2 * SB);
+    const int threads = blockDim.x, TN = p.tile_rows, buffer = D * TN * (p.slots * 16 + 2 * SB);
+    const bool one = p.buffers == 1;  // one step, of all waves
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l32 = lane & 31, half = lane >> 5;
+    const int consumers = one ? threads >> 6 : MX_CONSUMERS;
     const int run = 16 * ((l32 >> 2) & 1) + 4 * (l32 >> 3) + (l32 & 3);  // the row that this lane reads of the operand whose rows are dealt out
-    const int wb = wave & (p.wave_tiles - 1), wt = wave / p.wave_tiles, per_wave = TN / 32 / (waves / p.wave_tiles);
     int blk = blockIdx.x;
     const int first = blk % p.row_splits;
     blk /= p.row_splits;
     const int unit = blk % p.units, ai = unit / p.runs, d0 = (unit - ai * p.runs) * D, rows_w = G * p.b;
-    const int bt = blk / p.units * p.wave_tiles + wb;
-    const bool busy = bt < p.b_tiles;
-    const int wo = bt * 32 + (LAST ? l32 : run), o = wo < p.b ? wo : p.b - 1;  // (outputs behind the last one are read as the last one)
+    const int tile0 = blk / p.units * p.wave_tiles;
     float *const bias = (float *)(smem + p.buffers * buffer);  // (tile of the workgroup, gate and up, D, 32 outputs)
+    uint8_t *const stage = smem + p.buffers * buffer + p.wave_tiles * G * D * 128 + wave * MX_STAGE;
+    const int tasks = TN * p.cb, batch = (int)p.batch, row_tiles = (int)p.token_tiles;  // (steps past the end are counted in 32 bits)
+    const bool emit = p.codes_out && tile0 == 0;
 
-    const int tasks = TN * p.cb, batch = (int)p.batch;  // (and steps past the end are counted in 32 bits)
-    const bool emit = p.codes_out && blk / p.units == 0;
     // what a thread loads for the step of rows n0 on: the blocks of task t
     struct Load {
         MxGroup<T, D> g;
@@ -168,14 +197,48 @@ template <typename T, bool LAST, int D, bool GATED, int ACT, int KS> __global__ 
             }
         }
     };
+    // (scales of blocks behind the last one are read: with weights of zeros, but not as NaN)
+    auto prepare = [&] {
+        for (int k = 0; k < p.buffers; ++k)
+            for (int i = threadIdx.x; i < D * TN * SB / 2; i += threads) ((uint32_t *)(smem + k * buffer + D * TN * p.slots * 16))[i] = 0x7f7f7f7fu;
+        if (p.bias)
+            for (int i = threadIdx.x; i < p.wave_tiles * G * 32 * D; i += threads) {
+                const int j = i / 32 % D, q = i / 32 / D % G, out = (tile0 + i / 32 / D / G) * 32 + i % 32;
+                bias[i] = out < p.b ? (float)((const T *)p.bias)[((int64_t)ai * rows_w + q * p.b + out) * p.d + d0 + j] : 0.f;
+            }
+    };
 
-    // rows, tiles of them and what is on its way
-    const int row_tiles = (int)p.token_tiles;
-    Load f[R];
-    const bool on = first + p.row_splits < row_tiles;  // more steps than one (of 512 threads, which take a step's blocks R each)
+    if (!one && wave >= MX_CONSUMERS) {
+        const int t0 = threadIdx.x - 64 * MX_CONSUMERS;
+        constexpr int AHEAD = std::min(R, 64 / (D * 8 * (int)sizeof(T)));  // rounds on their way: 64 registers of values
+        static_assert(R % AHEAD == 0, "rounds");
+        Load f[AHEAD];
+#pragma unroll
+        for (int r = 0; r < AHEAD; ++r) fetch(f[r], t0 + r * 64 * MX_PRODUCERS, first * TN);
+        prepare();
+        __syncthreads();
+        int which = 0;
+        for (int tile = first; tile < row_tiles; tile += p.row_splits, which ^= 1) {
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                keep(f[r % AHEAD], tile * TN, which);
+                if (r + AHEAD < R)
+                    fetch(f[r % AHEAD], t0 + (r + AHEAD) * 64 * MX_PRODUCERS, tile * TN);
+                else if (tile + p.row_splits < row_tiles)
+                    fetch(f[r % AHEAD], t0 + (r + AHEAD - R) * 64 * MX_PRODUCERS, (tile + p.row_splits) * TN);
+            }
+            __syncthreads();
+        }
+        return;
+    }
+
+    const int wb = wave & (p.wave_tiles - 1), wt = wave / p.wave_tiles, per_wave = TN / 32 / (consumers / p.wave_tiles);
+    const int bt = tile0 + wb;
+    const bool busy = bt < p.b_tiles;
     uint4_t w[D][G][KS];
     int sw[D][G][SW];
     if (busy) {
+        const int wo = bt * 32 + (LAST ? l32 : run), o = wo < p.b ? wo : p.b - 1;  // (outputs behind the last one are read as the last one)
 #pragma unroll
         for (int j = 0; j < D; ++j)
 #pragma unroll
@@ -191,25 +254,14 @@ template <typename T, bool LAST, int D, bool GATED, int ACT, int KS> __global__ 
                 }
             }
     }
-    // (behind the weights: waiting for the first rows is waiting for these too, which no step has to do again)
-    if (on) {
-#pragma unroll
-        for (int r = 0; r < R; ++r) fetch(f[r], threadIdx.x + r * 512, first * TN);
-    }
-    // (scales of blocks behind the last one are read: with weights of zeros, but not as NaN)
-    for (int k = 0; k < p.buffers; ++k)
-        for (int i = threadIdx.x; i < D * TN * SB / 2; i += threads) ((uint32_t *)(smem + k * buffer + D * TN * p.slots * 16))[i] = 0x7f7f7f7fu;
-    for (int i = threadIdx.x; i < p.wave_tiles * G * 32 * D; i += threads) {
-        const int j = i / 32 % D, q = i / 32 / D % G, out = (blk / p.units * p.wave_tiles + i / 32 / D / G) * 32 + i % 32;
-        bias[i] = p.bias && out < p.b ? (float)((const T *)p.bias)[((int64_t)ai * rows_w + q * p.b + out) * p.d + d0 + j] : 0.f;
-    }
+    prepare();
     __syncthreads();
-    if (!on) {
+    if (one) {
+        Load f;
         for (int t = threadIdx.x; t < tasks; t += threads) {
-            fetch(f[0], t, first * TN);
-            keep(f[0], first * TN, 0);
+            fetch(f, t, first * TN);
+            keep(f, first * TN, 0);
         }
-        __syncthreads();
     }
     // (said to the compiler: the weights are there, and no step waits for them again, which would be for all stores before it too)
 #pragma unroll
@@ -221,58 +273,44 @@ template <typename T, bool LAST, int D, bool GATED, int ACT, int KS> __global__ 
 #pragma unroll
             for (int s = 0; s < SW; ++s) asm volatile("" : "+v"(sw[j][q][s]));
         }
-    mx_wait();
-    int which = on ? 1 : 0;
-    for (int tile = on ? first - p.row_splits : first; tile < row_tiles; tile += p.row_splits, which ^= 1) {
-        const int n0 = tile * TN, next = tile + p.row_splits;
-        const int here = batch - n0 < TN ? batch - n0 : TN;
-        if (next < row_tiles) {
-#pragma unroll
-            for (int r = 0; r < R; ++r) keep(f[r], next * TN, which ^ 1);
-            if (next + p.row_splits < row_tiles) {
-#pragma unroll
-                for (int r = 0; r < R; ++r) fetch(f[r], threadIdx.x + r * 512, (next + p.row_splits) * TN);
-            }
-        }
-        const uint8_t *const codes = smem + which * buffer, *const scales = codes + D * TN * p.slots * 16;
-        int t = wt * per_wave;
-        if (busy && tile >= 0 && t * 32 < here) {
-            do {
-                T v[16 * D];
-#pragma unroll
-                for (int j = 0; j < D; ++j) {
-                    const int row = j * TN + t * 32 + (LAST ? run : l32);
-                    int sx[SW];
-#pragma unroll
-                    for (int i = 0; i < SW; ++i) sx[i] = ((const int *)(scales + row * 2 * SB + half * SB))[i];
-                    float16_t acc[G];
-                    auto steps = [&](auto biased) {
-#pragma unroll
-                        for (int q = 0; q < G; ++q) {
-                            acc[q] = float16_t{};
-                            if constexpr (decltype(biased)::value)
-#pragma unroll
-                                for (int i = 0; i < 16; ++i) acc[q][i] = bias[((wb * G + q) * D + j) * 32 + (LAST ? l32 : 16 * half + i)];
-                        }
-#pragma unroll
-                        for (int s = 0; s < KS; ++s) {
-                            const uint4_t x = *(const uint4_t *)(codes + (row * p.slots + 2 * s + half) * 16);
-#pragma unroll
-                            for (int q = 0; q < G; ++q) acc[q] = mx_step<LAST>(w[j][q][s], sw[j][q][s / 4], x, sx[s / 4], s % 4, acc[q]);
-                        }
-                    };
-                    if (p.bias)
-                        steps(std::true_type());
-                    else
-                        steps(std::false_type());
-                    mx_activate<T, D, GATED, ACT>(acc, j, v);
-                }
-                mx_results<T, LAST, D>(p, v, ai, d0, bt, lane, n0, t, here);
-            } while (++t < (wt + 1) * per_wave && t * 32 < here);
-        } else {
-            mx_wait();
-        }
+    int which = 0;
+    for (int tile = first; tile < row_tiles; tile += p.row_splits, which ^= 1) {
+        const int n0 = tile * TN, here = batch - n0 < TN ? batch - n0 : TN;
         __syncthreads();
+        if (!busy) continue;
+        const uint8_t *const codes = smem + which * buffer, *const scales = codes + D * TN * p.slots * 16;
+        for (int t = wt * per_wave; t < (wt + 1) * per_wave && t * 32 < here; ++t) {
+            T v[16 * D];
+#pragma unroll
+            for (int j = 0; j < D; ++j) {
+                const int row = j * TN + t * 32 + (LAST ? run : l32);
+                int sx[SW];
+#pragma unroll
+                for (int i = 0; i < SW; ++i) sx[i] = ((const int *)(scales + row * 2 * SB + half * SB))[i];
+                float16_t acc[G];
+                auto steps = [&](auto biased) {
+#pragma unroll
+                    for (int q = 0; q < G; ++q) {
+                        acc[q] = float16_t{};
+                        if constexpr (decltype(biased)::value)
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) acc[q][i] = bias[((wb * G + q) * D + j) * 32 + (LAST ? l32 : 16 * half + i)];
+                    }
+#pragma unroll
+                    for (int s = 0; s < KS; ++s) {
+                        const uint4_t x = *(const uint4_t *)(codes + (row * p.slots + 2 * s + half) * 16);
+#pragma unroll
+                        for (int q = 0; q < G; ++q) acc[q] = mx_step<LAST>(w[j][q][s], sw[j][q][s / 4], x, sx[s / 4], s % 4, acc[q]);
+                    }
+                };
+                if (p.bias)
+                    steps(std::true_type());
+                else
+                    steps(std::false_type());
+                mx_activate<T, D, GATED, ACT>(acc, j, v);
+            }
+            mx_results<T, LAST, D>(p, v, ai, d0, bt, lane, n0, t, here, stage);
+        }
     }
 }
 
@@ -280,8 +318,8 @@ template <typename T, bool LAST, int D, int TT, bool GATED, int ACT> __global__ 
 {
     constexpr int TN = 32 * TT, G = GATED ? 2 : 1;
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
-    uint8_t *const codes = smem, *const scales = smem + (size_t)D * TN * p.slots * 16;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l32 = lane & 31, half = lane >> 5;
+    uint8_t *const codes = smem + MX_WAVES * MX_STAGE, *const scales = codes + (size_t)D * TN * p.slots * 16, *const stage = smem + wave * MX_STAGE;
     const int run = 16 * ((l32 >> 2) & 1) + 4 * (l32 >> 3) + (l32 & 3);  // the row that this lane reads of the operand whose rows are dealt out
     int64_t blk = blockIdx.x;
     const int split = (int)(blk % p.splits);
@@ -389,15 +427,15 @@ template <typename T, bool LAST, int D, int TT, bool GATED, int ACT> __global__ 
                     T v[16 * D];
 #pragma unroll
                     for (int j = 0; j < D; ++j) mx_activate<T, D, GATED, ACT>(acc[t][j], j, v);
-                    mx_results<T, LAST, D>(p, v, ai, d0, bt, lane, n0, t, here);
+                    mx_results<T, LAST, D>(p, v, ai, d0, bt, lane, n0, t, here, stage);
                 }
         }
     }
 }
 
-inline int64_t mx_held_lds(int d, bool gated, int ks, int cb, int rows, int tiles, int buffers)
+inline int64_t mx_held_lds(int d, bool gated, int ks, int cb, int rows, int tiles, int buffers, int waves)
 {
-    return (int64_t)buffers * d * rows * ((cb | 1) * 16 + 2 * mx_scale_bytes(ks)) + (int64_t)tiles * (gated ? 2 : 1) * 32 * d * 4;
+    return (int64_t)buffers * d * rows * ((cb | 1) * 16 + 2 * mx_scale_bytes(ks)) + (int64_t)tiles * (gated ? 2 : 1) * 32 * d * 4 + waves * MX_STAGE;
 }
 
 template <typename T, bool LAST, int D, int TT, bool GATED> int mx_launch(MxProduct p, int act, hipStream_t s)
@@ -441,42 +479,42 @@ template <typename T, bool LAST, int D, int TT, bool GATED> int mx_launch(MxProd
 
 template <typename T, bool LAST, int D, bool GATED, int KS> int mx_launch_held(MxProduct p, int act, hipStream_t s)
 {
-    constexpr int R = KS > 8 ? 2 : 1;
+    constexpr int MOST = 64 * MX_PRODUCERS * mx_rounds(KS);  // blocks a step
     p.slots = p.cb | 1;
     p.runs = p.d / D;
     p.units = p.a * p.runs;
     p.b_tiles = (p.b + 31) / 32;
-    auto tasks = [&](int rows) { return (int64_t)rows * p.cb; };
     // eight waves: the more of them share their rows the less often these are quantised, but none should idle
-    int best = 8, idle = 1 << 30;
-    for (int tiles = 8; tiles >= 1; tiles /= 2) {
+    int waves = MX_CONSUMERS + MX_PRODUCERS, idle = 1 << 30;
+    for (int tiles = MX_CONSUMERS; tiles >= 1; tiles /= 2) {
         const int over = (p.b_tiles + tiles - 1) / tiles * tiles - p.b_tiles;
-        if (over < idle && tasks(32 * 8 / tiles) <= 512 * R) {
-            best = tiles;
+        if (over < idle && 32 * MX_CONSUMERS / tiles * p.cb <= MOST) {
+            p.wave_tiles = tiles;
             idle = over;
         }
     }
-    int waves = 8;
-    p.wave_tiles = best;
-    p.tile_rows = 32 * 8 / best;
+    p.tile_rows = 32 * MX_CONSUMERS / p.wave_tiles;
     auto groups = [&] { return (int64_t)p.units * ((p.b_tiles + p.wave_tiles - 1) / p.wave_tiles); };
     p.token_tiles = (p.batch + p.tile_rows - 1) / p.tile_rows;
-    if (groups() * p.token_tiles < 256) {  // few: smaller workgroups of one step each
+    // a workgroup a compute unit (its twelve waves take the registers of one): one more would be a second round.  Those of the same
+    // rows lie on the same XCD where that is a multiple of eight apart
+    int64_t most = std::max<int64_t>(1, 256 / groups());
+    if (most >= 8) most = most / 8 * 8;
+    p.row_splits = (int)std::min(p.token_tiles, most);
+    p.buffers = 2;
+    if (groups() * p.token_tiles < 512) {  // few: smaller workgroups of one step each
         for (waves = 4; waves >= 1; waves /= 2) {
             p.wave_tiles = waves;
             p.tile_rows = 32;
             p.token_tiles = (p.batch + 31) / 32;
             if (waves == 1 || groups() * p.token_tiles >= 256) break;
         }
+        p.row_splits = (int)p.token_tiles;
+        p.buffers = 1;
     }
-    // workgroups that fit at once: a wave's registers are its weights, its sums and the values on their way
-    constexpr int REGS = D * (GATED ? 2 : 1) * (4 * KS + 16) + D * R * 8 * (int)sizeof(T) + 50;
-    const int64_t most = std::max<int64_t>(1, (REGS > 128 ? 256 : 512) / groups());
-    p.row_splits = (int)(waves < 8 || p.token_tiles < most ? p.token_tiles : most);
-    p.buffers = p.row_splits < p.token_tiles ? 2 : 1;
     const int64_t grid = groups() * p.row_splits;
     if (grid > 0x7fffffffLL) return KSMM_ERR_TOO_LARGE;
-    const int lds = (int)mx_held_lds(D, GATED, KS, p.cb, p.tile_rows, p.wave_tiles, p.buffers);
+    const int lds = (int)mx_held_lds(D, GATED, KS, p.cb, p.tile_rows, p.wave_tiles, p.buffers, p.buffers == 1 ? waves : MX_CONSUMERS);
     int rc = KSMM_OK;
     with_act(act, [&](auto which) {
         constexpr int ACT = decltype(which)::value;
@@ -494,8 +532,8 @@ template <typename T, bool LAST, int D, bool GATED, int KS> int mx_launch_held(M
 // steps of 64 along c that a kernel is made for
 template <typename T, bool LAST, int D, bool GATED, int KS, int... MORE> int mx_held(const MxProduct &p, int act, hipStream_t s)
 {
-    // registers: the weights' codes (4 a step), and the values of one row of steps on their way
-    constexpr bool fits = D * (GATED ? 2 : 1) * KS <= 16 && D * (KS > 8 ? 2 : 1) * 8 * (int)sizeof(T) <= 64;
+    // registers (168 of them): of one wave the weights' codes (4 a step) and the results, of another the values on their way; more spill
+    constexpr bool fits = D * (GATED ? 2 : 1) * KS <= (D < 4 ? 16 : 8) && D * 8 * (int)sizeof(T) <= 64;
     if constexpr (fits) {
         if (p.cb <= 2 * KS) return mx_launch_held<T, LAST, D, GATED, KS>(p, act, s);
         if constexpr (sizeof...(MORE) > 0) return mx_held<T, LAST, D, GATED, MORE...>(p, act, s);
@@ -509,9 +547,11 @@ template <typename T, bool LAST, int D, bool GATED> int mx_pick(const MxProduct 
         const int rc = mx_held<T, LAST, D, GATED, 1, 2, 3, 4, 6, 8, 16>(p, act, s);
         if (rc != KSMM_ERR_BAD_ALGO) return rc;
     }
+    // as many rows a workgroup as accumulators hold, where that leaves two workgroups for a compute unit
     constexpr int TT = mx_rows_of(D, GATED);
     if constexpr (TT > 1) {
-        if (p.batch > 32 && mx_lds(TT, D, p.cb) <= MX_LDS_MOST) return mx_launch<T, LAST, D, TT, GATED>(p, act, s);
+        const int64_t groups = (p.batch + 32 * TT - 1) / (32 * TT) * p.a * (p.d / D) * ((p.b + 32 * MX_WAVES - 1) / (32 * MX_WAVES));
+        if (groups >= 512 && mx_lds(TT, D, p.cb) <= MX_LDS_MOST) return mx_launch<T, LAST, D, TT, GATED>(p, act, s);
     }
     return mx_launch<T, LAST, D, 1, GATED>(p, act, s);
 }
