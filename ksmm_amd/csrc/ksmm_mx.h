@@ -45,6 +45,13 @@ __device__ __forceinline__ float mx_scale_value(int scale)
     return scale == MX_NAN ? __builtin_nanf("") : scale == 0 ? __builtin_bit_cast(float, 0x00400000u) : mx_power(scale);
 }
 
+// t / d for 0 <= t, t d < 2^32 (m is less than d 2^-32 too large): a multiplication where the compiler takes 30 instructions
+struct MxDiv {
+    uint32_t d, m;
+    __device__ __forceinline__ explicit MxDiv(int d) : d((uint32_t)d), m(0xffffffffu / (uint32_t)d + 1) {}
+    __device__ __forceinline__ int operator()(int t) const { return d == 1 ? t : (int)__umulhi((uint32_t)t, m); }
+};
+
 // ---- reading an operand ---------------------------------------------------------------------------------
 // A thread takes the blocks of one place kb of D consecutive d_i (batch-size-last D is 1): their 32 values of c are `step` elements
 // apart, and one run of 32 * D where that is D.
@@ -125,6 +132,66 @@ template <typename T, int D> __device__ __forceinline__ int mx_quantize(const Mx
     return scale;
 }
 
+// ---- a quarter of a block a lane: 8 values of D consecutive d_i that are one run in memory.  Lanes that follow one another read
+// bytes that do, where a block a lane has 64 lines of the cache in every load (25088 x 768 of (1,192,768,2): 31 us for 15)
+template <typename T, int D> struct MxQuarter {
+    T v[8 * D];
+};
+// count of the 8 values are there (may be none, or more); the rest is zeros
+template <typename T, int D> __device__ __forceinline__ void mx_load(MxQuarter<T, D> &g, const T *x, int count)
+{
+    constexpr int E = 16 / (int)sizeof(T);
+    if (count >= 8) {
+#pragma unroll
+        for (int j = 0; j < 8 * D / E; ++j) {
+            const uint4_t q = *(const uint4_any *)(x + j * E);
+            __builtin_memcpy(&g.v[j * E], &q, 16);
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8 * D; ++j) g.v[j] = j < count * D ? x[j] : (T)0;
+    }
+}
+// its part of the codes of the four lanes' block j, and the scale's byte (in each of them; all four take part)
+template <typename T, int D> __device__ __forceinline__ int mx_quantize(const MxQuarter<T, D> &g, int j, uint32_t &code)
+{
+    uint32_t top = 0;
+    if constexpr (sizeof(T) == 2) {
+        uint16_t most = 0;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const uint16_t bits = __builtin_bit_cast(uint16_t, g.v[k * D + j]) & 0x7fffu;
+            most = bits > most ? bits : most;
+        }
+        top = most;
+    } else {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const uint32_t bits = mx_bits(g.v[k * D + j]);
+            top = bits > top ? bits : top;
+        }
+    }
+    top = max(top, (uint32_t)__builtin_amdgcn_mov_dpp((int)top, 0xb1, 0xf, 0xf, true));  // lanes 1 0 3 2
+    top = max(top, (uint32_t)__builtin_amdgcn_mov_dpp((int)top, 0x4e, 0xf, 0xf, true));  // 2 3 0 1
+    if constexpr (sizeof(T) == 2) top = mx_bits((float)__builtin_bit_cast(half_t, (uint16_t)top));
+    const int scale = mx_scale(top);
+    const float power = mx_power(scale);
+    uint32_t r = 0;
+    if constexpr (sizeof(T) == 2) {
+        const T *v = &g.v[j];
+        r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(r, half2_t{v[0], v[D]}, power, 0);
+        r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(r, half2_t{v[2 * D], v[3 * D]}, power, 1);
+        r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(r, half2_t{v[4 * D], v[5 * D]}, power, 2);
+        r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(r, half2_t{v[6 * D], v[7 * D]}, power, 3);
+    } else {
+        const float *v = (const float *)&g.v[j];
+        const float e[8] = {v[0], v[D], v[2 * D], v[3 * D], v[4 * D], v[5 * D], v[6 * D], v[7 * D]};
+        r = mx_encode8(e, power);
+    }
+    code = scale == MX_NAN ? 0u : r;
+    return scale;
+}
+
 // What the product kernels are given.
 struct MxProduct {
     const void *x;
@@ -135,12 +202,12 @@ struct MxProduct {
     void *y;
     int64_t batch;
     int a, b, c, d, cb;
-    int slots;             // of 16 bytes in LDS for a row's codes, odd
-    int runs, units;       // runs of D consecutive d_i, and a times as many units of work
-    int units_per;         // of them a workgroup takes
-    int b_tiles, tiles_per;  // tiles of 32 outputs, and those a workgroup takes
-    int splits, unit_groups;
+    int slots;                    // of 16 bytes in LDS for a row's codes, odd
+    int run_d, runs, units;       // d_i of a unit of work, units of an a_i and of all
+    int b_tiles, tiles_per;       // tiles of 32 outputs, and those a workgroup takes
+    int chunk_tiles, splits;      // tiles at a time, and workgroups that share the tiles
     int64_t tiles, token_tiles;  // (without LDS); steps of rows
+    int raw_rows, raw_pitch;     // rows at a time whose values go through LDS on their way to codes (0: straight), and values from one to the next
     int tile_rows, wave_tiles;   // rows a step, and of a workgroup's waves those that lie along the outputs
     int row_splits, buffers;     // workgroups that share the steps
 };
@@ -154,16 +221,39 @@ int mx_float_first_gated(const MxProduct &p, int act, hipStream_t s);
 int mx_float_last_plain(const MxProduct &p, int act, hipStream_t s);
 int mx_float_last_gated(const MxProduct &p, int act, hipStream_t s);
 
-// d_i that a unit takes: all of up to four, else a divisor
+// d_i that a thread converts together: all of up to four, else a divisor
 inline int mx_run_of(int d) { return d <= 4 ? d : d % 4 == 0 ? 4 : d % 3 == 0 ? 3 : d % 2 == 0 ? 2 : 1; }
-// tiles of 32 rows: what 128 accumulators hold
-constexpr int mx_rows_of(int d, bool gated) { return d * (gated ? 2 : 1) <= 2 ? 4 : d * (gated ? 2 : 1) <= 4 ? 2 : 1; }
-constexpr int MX_WAVES = 4;                           // of a workgroup that reads its weights from the caches
-constexpr int MX_LINE = 144, MX_STAGE = 32 * MX_LINE;  // LDS of a wave for its results: 128 bytes of 32 lines, 16 between them for the banks' sake
-inline int64_t mx_lds(int tt, int d, int cb) { return (int64_t)d * 32 * tt * (16 * (cb | 1) + cb) + MX_WAVES * MX_STAGE; }
-constexpr int64_t MX_LDS_MOST = 80 * 1024;  // two workgroups a compute unit
 
+// Weights from the caches: d_i of a workgroup (16 of more are pieces of 32 bytes at least), tiles of outputs at a time (a wave each,
+// or with d_i of their own some), and LDS
+constexpr int MX_WAVES = 8;
+constexpr int MX_LINE = 144, MX_STAGE = 32 * MX_LINE;  // of a wave for its results: 128 bytes of 32 lines, 16 between them for the banks' sake
+constexpr int64_t MX_LDS_MOST = 80 * 1024;             // two workgroups a compute unit
+constexpr int64_t MX_LDS_ALL = 160 * 1024;
+inline int mx_unit_of(int d, bool last) { return last ? 1 : d <= 16 ? d : 16; }
+inline int mx_chunk_of(int unit, bool last) { return last || unit == 1 ? MX_WAVES : unit < MX_WAVES ? MX_WAVES / unit : 1; }
+inline int64_t mx_codes_lds(int tt, int c, int d, bool last)
+{
+    const int64_t cb = mx_blocks(c), unit = mx_unit_of(d, last), rows = 32 * tt;
+    return unit * rows * (cb | 1) * 16 + (unit * rows * cb + 15) / 16 * 16;
+}
+// Five d_i and more go through LDS on their way to codes: bytes of a row (16 more than its vectors: rows meet other banks), and rows at a
+// time, all of them or as few times as two workgroups a compute unit allow
+inline int64_t mx_raw_row(int c, int d, int size) { return ((int64_t)mx_unit_of(d, false) * c * size + 15) / 16 * 16 + 16; }
+inline int mx_raw_rows(int tt, int c, int d, int size)
+{
+    const int64_t fit = (MX_LDS_MOST - mx_codes_lds(tt, c, d, false)) / mx_raw_row(c, d, size), rows = 32 * tt;
+    const int64_t times = fit < 1 ? rows : (rows + fit - 1) / fit;
+    return (int)((rows + times - 1) / times);
+}
+inline int64_t mx_wide_lds(int tt, int c, int d, int size, bool last)
+{
+    if (last) return mx_codes_lds(tt, c, d, last) + MX_WAVES * MX_STAGE;
+    const int64_t unit = mx_unit_of(d, last), results = 32 * tt * (mx_chunk_of((int)unit, last) * 32 * unit * size + 4);
+    const int64_t raw = d > 4 ? mx_raw_rows(tt, c, d, size) * mx_raw_row(c, d, size) : 0;
+    return mx_codes_lds(tt, c, d, last) + (results > raw ? results : raw);
+}
 // whether an operand's codes fit LDS, so that it is quantised there
-inline bool mx_in_lds(int c, int d, bool last) { return mx_lds(1, last ? 1 : mx_run_of(d), (int)mx_blocks(c)) <= MX_LDS_MOST; }
+inline bool mx_in_lds(int c, int d, int size, bool last) { return mx_wide_lds(1, c, d, size, last) <= MX_LDS_ALL; }
 
 }  // namespace ksmm

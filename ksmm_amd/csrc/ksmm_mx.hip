@@ -361,7 +361,7 @@ int64_t ksmm_mx_forward_workspace(int64_t batch, int a, int b, int c, int d, int
 {
     const int rc = check_product(batch, a, b, c, d, dtype, KSMM_ACT_NONE, gated);
     if (rc != KSMM_OK) return rc;
-    if (mx_in_lds(c, d, bs_last != 0)) return 0;
+    if (mx_in_lds(c, d, (int)dtype_size(dtype), bs_last != 0)) return 0;
     const int64_t blocks = (int64_t)a * d * batch * mx_blocks(c);
     return align256(blocks * 16) + align256(blocks);
 }
@@ -387,7 +387,7 @@ int ksmm_mx_forward(const void *x, const void *x_scales, const void *w, const vo
     static int (*const fused[2][2][2])(const MxProduct &, int, hipStream_t) = {
         {{mx_half_first_plain, mx_half_first_gated}, {mx_half_last_plain, mx_half_last_gated}},
         {{mx_float_first_plain, mx_float_first_gated}, {mx_float_last_plain, mx_float_last_gated}}};
-    if (mx_in_lds(c, d, bs_last != 0))
+    if (mx_in_lds(c, d, (int)dtype_size(dtype), bs_last != 0))
         return fused[dtype == KSMM_F32][bs_last != 0][gated != 0](p, act, (hipStream_t)stream);
     if (!x_scales) {
         uint8_t *const codes = codes_out ? (uint8_t *)codes_out : (uint8_t *)workspace;

@@ -7,6 +7,7 @@
 // (batch-size-last: 16 consecutive rows of one output), which with those of all D leave as whole vectors.
 #pragma once
 #include <algorithm>
+#include <type_traits>
 
 #include "ksmm_act.h"
 #include "ksmm_mx.h"
@@ -101,7 +102,7 @@ template <typename T, bool LAST, int D>
 __device__ __forceinline__ void mx_results(const MxProduct &p, const T (&v)[16 * D], int ai, int d0, int bt, int lane, int64_t n0, int t, int here, uint8_t *stage)
 {
     const int l32 = lane & 31, half = lane >> 5;
-    if ((t + 1) * 32 <= here && (bt + 1) * 32 <= p.b && (LAST || p.d == D)) {
+    if ((t + 1) * 32 <= here && (bt + 1) * 32 <= p.b) {
         const int64_t pitch = LAST ? (int64_t)p.d * p.batch : (int64_t)p.a * p.b * p.d;
         T *const y = (T *)p.y + (LAST ? (((int64_t)ai * p.b + bt * 32) * p.d + d0) * p.batch + n0 + t * 32
                                       : (((n0 + t * 32) * p.a + ai) * p.b + bt * 32) * p.d + d0);
@@ -122,7 +123,7 @@ __device__ __forceinline__ void mx_results(const MxProduct &p, const T (&v)[16 *
             T e[D];
         };
         if (n >= here) return;
-        if (p.d == D && o + 16 <= p.b) {
+        if (o + 16 <= p.b) {
             mx_store<T, 16 * D>(y, v);
         } else {
 #pragma unroll
@@ -144,12 +145,24 @@ __device__ __forceinline__ void mx_results(const MxProduct &p, const T (&v)[16 *
 // Where there are few steps each workgroup takes one, of fewer waves, which first quantise and then multiply.
 constexpr int MX_CONSUMERS = 8, MX_PRODUCERS = 4;
 constexpr int mx_scale_bytes(int ks) { return ks <= 4 ? 4 : ks <= 8 ? 8 : 16; }  // of a row and one half of each step
-constexpr int mx_rounds(int ks) { return ks <= 4 ? 1 : ks <= 8 ? 2 : 4; }        // blocks of 32 rows that a producer's thread takes
+// blocks of 32 rows, or quarters of them, that a producer's thread takes, and of these those on their way at once: 64 registers of values
+constexpr int mx_rounds(int ks, int quarters) { return quarters == 1 ? (ks + 3) / 4 : ks; }
+// Lanes a block.  Four of them read what is one run in memory with a quarter of the lines a load, but find the scale four times: in fp32
+// (1,768,192,2) gated takes 58 us for 64, in fp16 36 for 29.  (Of 16 steps the rounds would be too many to keep; blocks of three d_i that
+// end inside 32 are read three values at a time: (1,192,48,3) in fp16 27 us for 13.)
+template <typename T> constexpr int mx_quarters(bool last, int ks, int d) { return last || ks > 8 || (sizeof(T) == 2 && d != 3) ? 1 : 4; }
+constexpr int mx_ahead(int rounds, int registers)
+{
+    int n = 64 / registers < 8 ? 64 / registers : 8;
+    if (n > rounds) n = rounds;
+    while (rounds % n) --n;
+    return n;
+}
 
 template <typename T, bool LAST, int D, bool GATED, int ACT, int KS>
 __global__ __launch_bounds__(64 * (MX_CONSUMERS + MX_PRODUCERS)) void ks_mx_held_kernel(MxProduct p)
 {
-    constexpr int G = GATED ? 2 : 1, SB = mx_scale_bytes(KS), SW = (KS + 3) / 4, R = mx_rounds(KS);
+    constexpr int G = GATED ? 2 : 1, SB = mx_scale_bytes(KS), SW = (KS + 3) / 4, R = mx_rounds(KS, mx_quarters<T>(LAST, KS, D));
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     const int threads = blockDim.x, TN = p.tile_rows, buffer = D * TN * (p.slots * 16 + 2 * SB);
     const bool one = p.buffers == 1;  // one step, of all waves
@@ -166,34 +179,51 @@ __global__ __launch_bounds__(64 * (MX_CONSUMERS + MX_PRODUCERS)) void ks_mx_held
     const int tasks = TN * p.cb, batch = (int)p.batch, row_tiles = (int)p.token_tiles;  // (steps past the end are counted in 32 bits)
     const bool emit = p.codes_out && tile0 == 0;
 
-    // what a thread loads for the step of rows n0 on: the blocks of task t
-    struct Load {
-        MxGroup<T, D> g;
-        int row, kb;  // none: row < 0
+    // what a thread loads for the step of rows n0 on: the blocks of task t, or batch-size-first a quarter of them
+    constexpr int Q = mx_quarters<T>(LAST, KS, D);
+    typedef std::conditional_t<Q == 1, MxGroup<T, D>, MxQuarter<T, D>> Load;
+    const MxDiv by(LAST ? TN : p.cb);
+    const int quarter = threadIdx.x & 3;  // (batch-size-first: a thread has the same of all its blocks)
+    // row * 256 + kb of task t
+    auto place = [&](int t) {
+        const int u = t / Q, v = by(u), rest = u - v * (LAST ? TN : p.cb);
+        return LAST ? rest * 256 + v : v * 256 + rest;
     };
-    auto fetch = [&](Load &f, int t, int n0) {
-        const int kb = LAST ? t / TN : t % p.cb, n = LAST ? t - kb * TN : t / p.cb;
-        f.row = t < tasks && n < batch - n0 ? n : -1;
-        f.kb = kb;
-        if (f.row < 0) return;
-        const T *x = (const T *)p.x + (LAST ? (((int64_t)ai * p.c + kb * 32) * p.d + d0) * p.batch + n0 + n
-                                            : ((((int64_t)n0 + n) * p.a + ai) * p.c + kb * 32) * p.d + d0);
-        mx_load<T, D>(f.g, x, LAST ? (int64_t)p.d * p.batch : p.d, p.c - kb * 32);
+    // rows that are not there: whatever LDS has, they are other columns of the product
+    auto there = [&](int t, int at, int n0) { return t < tasks * Q && (at >> 8) < batch - n0; };
+    auto fetch = [&](Load &f, int t, int at, int n0) {
+        if (!there(t, at, n0)) return;
+        const int n = at >> 8, kb = at & 255;
+        if constexpr (LAST)
+            mx_load<T, 1>(f, (const T *)p.x + (((int64_t)ai * p.c + kb * 32) * p.d + d0) * p.batch + n0 + n, (int64_t)p.d * p.batch, p.c - kb * 32);
+        else if constexpr (Q == 1)
+            mx_load<T, D>(f, (const T *)p.x + ((((int64_t)n0 + n) * p.a + ai) * p.c + kb * 32) * D, D, p.c - kb * 32);
+        else
+            mx_load<T, D>(f, (const T *)p.x + ((((int64_t)n0 + n) * p.a + ai) * p.c + kb * 32 + quarter * 8) * D, p.c - kb * 32 - quarter * 8);
     };
-    auto keep = [&](const Load &f, int n0, int which) {
-        if (f.row < 0) return;  // (rows that are not there: whatever LDS has, they are other columns of the product)
+    auto keep = [&](const Load &f, int t, int at, int n0, int which) {
+        if (!there(t, at, n0)) return;
+        const int n = at >> 8, kb = at & 255;
         uint8_t *const codes = smem + which * buffer, *const scales = codes + D * TN * p.slots * 16;
 #pragma unroll
         for (int j = 0; j < D; ++j) {
-            const int row = j * TN + f.row;
-            uint4_t code;
-            const int scale = mx_quantize<T, D>(f.g, j, p.c - f.kb * 32, code);
-            *(uint4_t *)(codes + (row * p.slots + f.kb) * 16) = code;
-            scales[row * 2 * SB + (f.kb & 1) * SB + (f.kb >> 1)] = (uint8_t)scale;
-            if (emit) {
-                const int64_t block = (((int64_t)ai * p.d + d0 + j) * p.batch + n0 + f.row) * p.cb + f.kb;
-                *(uint4_t *)(p.codes_out + block * 16) = code;
-                p.scales_out[block] = (uint8_t)scale;
+            const int row = j * TN + n;
+            const int64_t block = (((int64_t)ai * p.d + d0 + j) * p.batch + n0 + n) * p.cb + kb;
+            int scale;
+            if constexpr (Q == 1) {
+                uint4_t code;
+                scale = mx_quantize<T, D>(f, j, p.c - kb * 32, code);
+                *(uint4_t *)(codes + (row * p.slots + kb) * 16) = code;
+                if (emit) *(uint4_t *)(p.codes_out + block * 16) = code;
+            } else {
+                uint32_t code;
+                scale = mx_quantize<T, D>(f, j, code);
+                *(uint32_t *)(codes + (row * p.slots + kb) * 16 + quarter * 4) = code;
+                if (emit) *(uint32_t *)(p.codes_out + block * 16 + quarter * 4) = code;
+            }
+            if (Q == 1 || quarter == 0) {
+                scales[row * 2 * SB + (kb & 1) * SB + (kb >> 1)] = (uint8_t)scale;
+                if (emit) p.scales_out[block] = (uint8_t)scale;
             }
         }
     };
@@ -210,22 +240,23 @@ __global__ __launch_bounds__(64 * (MX_CONSUMERS + MX_PRODUCERS)) void ks_mx_held
 
     if (!one && wave >= MX_CONSUMERS) {
         const int t0 = threadIdx.x - 64 * MX_CONSUMERS;
-        constexpr int AHEAD = std::min(R, 64 / (D * 8 * (int)sizeof(T)));  // rounds on their way: 64 registers of values
-        static_assert(R % AHEAD == 0, "rounds");
+        constexpr int AHEAD = mx_ahead(R, D * (int)sizeof(T) * 8 / Q);
         Load f[AHEAD];
+        int at[R];
 #pragma unroll
-        for (int r = 0; r < AHEAD; ++r) fetch(f[r], t0 + r * 64 * MX_PRODUCERS, first * TN);
+        for (int r = 0; r < R; ++r) at[r] = place(t0 + r * 64 * MX_PRODUCERS);
+#pragma unroll
+        for (int r = 0; r < AHEAD; ++r) fetch(f[r], t0 + r * 64 * MX_PRODUCERS, at[r], first * TN);
         prepare();
         __syncthreads();
         int which = 0;
         for (int tile = first; tile < row_tiles; tile += p.row_splits, which ^= 1) {
 #pragma unroll
             for (int r = 0; r < R; ++r) {
-                keep(f[r % AHEAD], tile * TN, which);
-                if (r + AHEAD < R)
-                    fetch(f[r % AHEAD], t0 + (r + AHEAD) * 64 * MX_PRODUCERS, tile * TN);
-                else if (tile + p.row_splits < row_tiles)
-                    fetch(f[r % AHEAD], t0 + (r + AHEAD - R) * 64 * MX_PRODUCERS, (tile + p.row_splits) * TN);
+                keep(f[r % AHEAD], t0 + r * 64 * MX_PRODUCERS, at[r], tile * TN, which);
+                const int next = (r + AHEAD) % R;
+                if (r + AHEAD < R || tile + p.row_splits < row_tiles)
+                    fetch(f[r % AHEAD], t0 + next * 64 * MX_PRODUCERS, at[next], (r + AHEAD < R ? tile : tile + p.row_splits) * TN);
             }
             __syncthreads();
         }
@@ -258,9 +289,10 @@ __global__ __launch_bounds__(64 * (MX_CONSUMERS + MX_PRODUCERS)) void ks_mx_held
     __syncthreads();
     if (one) {
         Load f;
-        for (int t = threadIdx.x; t < tasks; t += threads) {
-            fetch(f, t, first * TN);
-            keep(f, first * TN, 0);
+        for (int t = threadIdx.x; t < tasks * Q; t += threads) {
+            const int at = place(t);
+            fetch(f, t, at, first * TN);
+            keep(f, t, at, first * TN, 0);
         }
     }
     // (said to the compiler: the weights are there, and no step waits for them again, which would be for all stores before it too)
@@ -314,121 +346,226 @@ __global__ __launch_bounds__(64 * (MX_CONSUMERS + MX_PRODUCERS)) void ks_mx_held
     }
 }
 
-template <typename T, bool LAST, int D, int TT, bool GATED, int ACT> __global__ __launch_bounds__(64 * MX_WAVES) void ks_mx_fused_kernel(MxProduct p)
+// ---- weights from the caches: more of them than registers hold, or d_i that no thread takes together ------------------------------
+// A workgroup quantises 32 * TT rows of a unit (one a_i; all d_i, or runs of 16 of more) into LDS; its waves take tiles of 32 outputs
+// of one d_i each, and leave their results in LDS, from where they go out a line of a row, all d_i, at a time (batch-size-last, where
+// a unit is one d_i, straight from the wave).  The codes of a step along c are on their way while the step before is multiplied.
+// D: d_i that a thread quantises together (1: all of one, or of five and more).
+template <typename T, bool LAST, int D, int TT, bool GATED, int ACT> __global__ __launch_bounds__(64 * MX_WAVES) void ks_mx_wide_kernel(MxProduct p)
 {
     constexpr int TN = 32 * TT, G = GATED ? 2 : 1;
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l32 = lane & 31, half = lane >> 5;
-    uint8_t *const codes = smem + MX_WAVES * MX_STAGE, *const scales = codes + (size_t)D * TN * p.slots * 16, *const stage = smem + wave * MX_STAGE;
     const int run = 16 * ((l32 >> 2) & 1) + 4 * (l32 >> 3) + (l32 & 3);  // the row that this lane reads of the operand whose rows are dealt out
+    uint8_t *const codes = smem, *const scales = codes + (size_t)p.run_d * TN * p.slots * 16;
+    T *const stage = (T *)(scales + (p.run_d * TN * p.cb + 15) / 16 * 16);  // of the workgroup: rows of `pitch`; batch-size-last of the waves
     int64_t blk = blockIdx.x;
     const int split = (int)(blk % p.splits);
     blk /= p.splits;
-    const int first_unit = (int)(blk % p.unit_groups) * p.units_per;
-    const int64_t n0 = blk / p.unit_groups * TN;
-    const int here = (int)(p.batch - n0 < TN ? p.batch - n0 : TN);  // rows of the batch
-    const int rows_w = G * p.b, last_unit = first_unit + p.units_per < p.units ? first_unit + p.units_per : p.units;
-    const int tile_end = (split + 1) * p.tiles_per < p.b_tiles ? (split + 1) * p.tiles_per : p.b_tiles;
-
-    for (int unit = first_unit; unit < last_unit; ++unit) {
-        const int ai = unit / p.runs, d0 = (unit - ai * p.runs) * D;
-        if (unit > first_unit) __syncthreads();  // (the codes before are no longer read)
-        // ---- x into LDS
-        if (p.x_scales) {
-            for (int t = threadIdx.x; t < D * TN * p.cb; t += 64 * MX_WAVES) {
-                const int kb = t % p.cb, row = t / p.cb, j = row / TN, n = row - j * TN;
-                uint4_t code = {0, 0, 0, 0};
-                int scale = 127;
-                if (n < here) {
-                    const int64_t block = (((int64_t)ai * p.d + d0 + j) * p.batch + n0 + n) * p.cb + kb;
-                    code = *(const uint4_t *)((const uint8_t *)p.x + block * 16);
-                    scale = p.x_scales[block];
-                }
-                *(uint4_t *)(codes + ((size_t)row * p.slots + kb) * 16) = code;
-                scales[row * p.cb + kb] = (uint8_t)scale;
-            }
-        } else {
-            for (int t = threadIdx.x; t < TN * p.cb; t += 64 * MX_WAVES) {
-                const int kb = LAST ? t / TN : t % p.cb, n = LAST ? t - kb * TN : t / p.cb;
-                if (n >= here) continue;  // (whatever LDS has there, it is another column of the product)
-                MxGroup<T, D> g;
-                const T *x = (const T *)p.x + (LAST ? (((int64_t)ai * p.c + kb * 32) * p.d + d0) * p.batch + n0 + n
-                                                    : (((n0 + n) * p.a + ai) * p.c + kb * 32) * p.d + d0);
-                mx_load<T, D>(g, x, LAST ? (int64_t)p.d * p.batch : p.d, p.c - kb * 32);
+    const int unit = (int)(blk % p.units), ai = unit / p.runs, d0 = (unit - ai * p.runs) * p.run_d;
+    const int64_t n0 = blk / p.units * TN;
+    const int here = (int)(p.batch - n0 < TN ? p.batch - n0 : TN);                 // rows of the batch
+    const int dc = LAST ? 1 : p.d - d0 < p.run_d ? p.d - d0 : p.run_d;             // d_i of the unit
+    const int rows_w = G * p.b, pitch = p.chunk_tiles * 32 * p.run_d + 4 / (int)sizeof(T);  // (an odd number of words: rows meet other banks)
+    // ---- x into LDS
+    auto keep = [&](int j, int n, int kb, uint4_t code, int scale, bool emit) {
+        const int row = j * TN + n;
+        *(uint4_t *)(codes + ((size_t)row * p.slots + kb) * 16) = code;
+        scales[row * p.cb + kb] = (uint8_t)scale;
+        if (emit) {
+            const int64_t block = (((int64_t)ai * p.d + d0 + j) * p.batch + n0 + n) * p.cb + kb;
+            *(uint4_t *)(p.codes_out + block * 16) = code;
+            p.scales_out[block] = (uint8_t)scale;
+        }
+    };
+    const bool emit = p.codes_out && split == 0;
+    const MxDiv by_cb(p.cb), by_dc(dc);
+    if (p.x_scales) {  // as codes: they are copied
+        for (int t = threadIdx.x; t < TN * p.cb * dc; t += 64 * MX_WAVES) {
+            const int u = by_cb(t), kb = t - u * p.cb, j = u / TN, n = u - j * TN;
+            if (n >= here) continue;
+            const int64_t block = (((int64_t)ai * p.d + d0 + j) * p.batch + n0 + n) * p.cb + kb;
+            keep(j, n, kb, *(const uint4_t *)((const uint8_t *)p.x + block * 16), p.x_scales[block], false);
+        }
+    } else if constexpr (LAST) {
+        for (int t = threadIdx.x; t < TN * p.cb; t += 64 * MX_WAVES) {
+            const int kb = t / TN, n = t - kb * TN;
+            if (n >= here) continue;  // (whatever LDS has there, it is another column of the product)
+            MxGroup<T, 1> g;
+            mx_load<T, 1>(g, (const T *)p.x + (((int64_t)ai * p.c + kb * 32) * p.d + d0) * p.batch + n0 + n, (int64_t)p.d * p.batch, p.c - kb * 32);
+            uint4_t code;
+            const int scale = mx_quantize<T, 1>(g, 0, p.c - kb * 32, code);
+            keep(0, n, kb, code, scale, emit);
+        }
+    } else if (p.d == D) {
+        for (int t = threadIdx.x; t < TN * p.cb * 4; t += 64 * MX_WAVES) {
+            const int u = t / 4, quarter = t & 3, n = by_cb(u), kb = u - n * p.cb;
+            if (n >= here) continue;
+            MxQuarter<T, D> g;
+            mx_load<T, D>(g, (const T *)p.x + (((n0 + n) * p.a + ai) * p.c + kb * 32 + quarter * 8) * D, p.c - kb * 32 - quarter * 8);
 #pragma unroll
-                for (int j = 0; j < D; ++j) {
-                    uint4_t code;
-                    const int row = j * TN + n, scale = mx_quantize<T, D>(g, j, p.c - kb * 32, code);
-                    *(uint4_t *)(codes + ((size_t)row * p.slots + kb) * 16) = code;
+            for (int j = 0; j < D; ++j) {
+                uint32_t code;
+                const int row = j * TN + n, scale = mx_quantize<T, D>(g, j, code);
+                const int64_t block = (((int64_t)ai * p.d + d0 + j) * p.batch + n0 + n) * p.cb + kb;
+                ((uint32_t *)(codes + ((size_t)row * p.slots + kb) * 16))[quarter] = code;
+                if (emit) ((uint32_t *)(p.codes_out + block * 16))[quarter] = code;
+                if (quarter == 0) {
                     scales[row * p.cb + kb] = (uint8_t)scale;
-                    if (p.codes_out && split == 0) {
-                        const int64_t block = (((int64_t)ai * p.d + d0 + j) * p.batch + n0 + n) * p.cb + kb;
-                        *(uint4_t *)(p.codes_out + block * 16) = code;
-                        p.scales_out[block] = (uint8_t)scale;
-                    }
+                    if (emit) p.scales_out[block] = (uint8_t)scale;
                 }
             }
         }
-        __syncthreads();
-        // ---- products
-        for (int bt = split * p.tiles_per + wave; bt < tile_end; bt += MX_WAVES) {
-            float16_t acc[TT][D][G];
-            const T *const bias = (const T *)p.bias;
+    } else if constexpr (D == 1) {
+        // five d_i and more: as they lie into LDS, where a thread gathers a block
+        constexpr int E = 16 / (int)sizeof(T), AHEAD = 4;
+        const bool whole = dc == p.d;
+        const int length = whole ? p.c * dc : dc, vectors = (length + E - 1) / E, lines = whole ? 1 : p.c;  // runs of a row
+        const MxDiv by_vectors(vectors), by_lines(lines);
+        for (int first = 0; first < here; first += p.raw_rows) {
+            const int rows = here - first < p.raw_rows ? here - first : p.raw_rows, total = rows * lines * vectors;
+            if (first > 0) __syncthreads();
+            for (int i0 = threadIdx.x; i0 < total; i0 += 64 * MX_WAVES * AHEAD) {
+                uint4_t q[AHEAD];
+                int to[AHEAD], left[AHEAD];
 #pragma unroll
-            for (int j = 0; j < D; ++j)
+                for (int r = 0; r < AHEAD; ++r) {
+                    const int i = i0 + r * 64 * MX_WAVES < total ? i0 + r * 64 * MX_WAVES : i0;  // (behind the end the first one again)
+                    const int u = by_vectors(i), e = (i - u * vectors) * E, n = by_lines(u), line = u - n * lines;
+                    const T *from = (const T *)p.x + (((n0 + first + n) * p.a + ai) * p.c + line) * p.d + d0 + e;
+                    left[r] = length - e;
+                    to[r] = n * p.raw_pitch + line * dc + e;
+                    if (left[r] >= E) {
+                        q[r] = *(const uint4_any *)from;
+                    } else {
+                        T v[E];
 #pragma unroll
-                for (int q = 0; q < G; ++q) {
-                    float16_t add = {};
-                    if (bias) {
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) {
-                            const int out = LAST ? bt * 32 + l32 : bt * 32 + 16 * half + i;
-                            add[i] = (float)bias[((int64_t)ai * rows_w + q * p.b + (out < p.b ? out : p.b - 1)) * p.d + d0 + j];
-                        }
+                        for (int k = 0; k < E; ++k) v[k] = from[k < left[r] ? k : 0];
+                        __builtin_memcpy(&q[r], v, 16);
                     }
-#pragma unroll
-                    for (int t = 0; t < TT; ++t) acc[t][j][q] = add;
                 }
+#pragma unroll
+                for (int r = 0; r < AHEAD; ++r) {
+                    if (whole || dc % E == 0) {
+                        __builtin_memcpy(__builtin_assume_aligned(stage + to[r], 16), &q[r], 16);
+                    } else {
+                        T v[E];
+                        __builtin_memcpy(v, &q[r], 16);
+#pragma unroll
+                        for (int k = 0; k < E; ++k)
+                            if (k < left[r]) stage[to[r] + k] = v[k];
+                    }
+                }
+            }
+            __syncthreads();
+            const MxDiv by_rows(rows);
+            for (int t = threadIdx.x; t < rows * p.cb * dc; t += 64 * MX_WAVES) {
+                const int u = by_dc(t), j = t - u * dc, kb = by_rows(u), n = u - kb * rows, count = p.c - kb * 32, last = (count < 32 ? count : 32) - 1;
+                const T *from = stage + n * p.raw_pitch + kb * 32 * dc + j;
+                MxGroup<T, 1> g;
+#pragma unroll
+                for (int k = 0; k < 32; ++k) g.v[k] = from[(k < last ? k : last) * dc];
+                uint4_t code;
+                const int scale = mx_quantize<T, 1>(g, 0, count, code);
+                keep(j, first + n, kb, code, scale, emit);
+            }
+        }
+    }
+    __syncthreads();
+    // ---- products, a chunk of tiles of outputs at a time
+    const T *const bias = (const T *)p.bias;
+    const int chunk_end = (split + 1) * p.tiles_per < p.b_tiles ? (split + 1) * p.tiles_per : p.b_tiles;
+    for (int chunk = split * p.tiles_per; chunk < chunk_end; chunk += p.chunk_tiles) {
+        const int jobs = (chunk_end - chunk < p.chunk_tiles ? chunk_end - chunk : p.chunk_tiles) * dc;
+        for (int job = wave; job < jobs; job += MX_WAVES) {
+            const int job_tile = by_dc(job), j = job - job_tile * dc, bt = chunk + job_tile;
             // (outputs behind the last one are read as the last one and not stored)
             const int wo = bt * 32 + (LAST ? l32 : run), o = wo < p.b ? wo : p.b - 1;
-            const int xr = LAST ? run : l32;
-            int64_t at[D][G];
+            int64_t at[G];
 #pragma unroll
-            for (int j = 0; j < D; ++j)
+            for (int q = 0; q < G; ++q) at[q] = (((int64_t)ai * p.d + d0 + j) * rows_w + q * p.b + o) * p.cb;
+            struct Step {
+                uint4_t w[G];
+                int s[G];
+            };
+            auto load = [&](int kb, Step &k) {
+                const bool there = kb < p.cb;
 #pragma unroll
-                for (int q = 0; q < G; ++q) at[j][q] = (((int64_t)ai * p.d + d0 + j) * rows_w + q * p.b + o) * p.cb;
+                for (int q = 0; q < G; ++q) {
+                    k.w[q] = there ? *(const uint4_t *)(p.w + (at[q] + kb) * 16) : uint4_t{0, 0, 0, 0};
+                    k.s[q] = there ? p.w_scales[at[q] + kb] : 127;
+                }
+            };
+            Step now;
+            load(half, now);
+            float16_t acc[TT][G];
+#pragma unroll
+            for (int q = 0; q < G; ++q) {
+                float16_t add = {};
+                if (bias) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const int out = LAST ? bt * 32 + l32 : bt * 32 + 16 * half + i;
+                        add[i] = (float)bias[((int64_t)ai * rows_w + q * p.b + (out < p.b ? out : p.b - 1)) * p.d + d0 + j];
+                    }
+                }
+#pragma unroll
+                for (int t = 0; t < TT; ++t) acc[t][q] = add;
+            }
             for (int k0 = 0; k0 < p.cb; k0 += 2) {
                 const int kb = k0 + half;
-                const bool there = kb < p.cb;
-                uint4_t w[D][G];
-                int sw[D][G];
+                Step next = now;
+                if (k0 + 2 < p.cb) load(kb + 2, next);
 #pragma unroll
-                for (int j = 0; j < D; ++j)
+                for (int t = 0; t < TT; ++t) {
+                    const int row = j * TN + t * 32 + (LAST ? run : l32);
+                    const bool there = kb < p.cb;
+                    const uint4_t x = there ? *(const uint4_t *)(codes + ((size_t)row * p.slots + kb) * 16) : uint4_t{0, 0, 0, 0};
+                    const int sx = there ? scales[row * p.cb + kb] : 127;
 #pragma unroll
-                    for (int q = 0; q < G; ++q) {
-                        w[j][q] = there ? *(const uint4_t *)(p.w + (at[j][q] + kb) * 16) : uint4_t{0, 0, 0, 0};
-                        sw[j][q] = there ? p.w_scales[at[j][q] + kb] : 127;
-                    }
-#pragma unroll
-                for (int t = 0; t < TT; ++t)
-#pragma unroll
-                    for (int j = 0; j < D; ++j) {
-                        const int row = j * TN + t * 32 + xr;
-                        const uint4_t x = there ? *(const uint4_t *)(codes + ((size_t)row * p.slots + kb) * 16) : uint4_t{0, 0, 0, 0};
-                        const int sx = there ? scales[row * p.cb + kb] : 127;
-#pragma unroll
-                        for (int q = 0; q < G; ++q)
-                            acc[t][j][q] = LAST ? mx_mfma(x, sx, w[j][q], sw[j][q], acc[t][j][q]) : mx_mfma(w[j][q], sw[j][q], x, sx, acc[t][j][q]);
-                    }
+                    for (int q = 0; q < G; ++q) acc[t][q] = LAST ? mx_mfma(x, sx, now.w[q], now.s[q], acc[t][q]) : mx_mfma(now.w[q], now.s[q], x, sx, acc[t][q]);
+                }
+                now = next;
             }
 #pragma unroll
-            for (int t = 0; t < TT; ++t)
-                if (t * 32 < here) {
-                    T v[16 * D];
+            for (int t = 0; t < TT; ++t) {
+                T v[16];
+                mx_activate<T, 1, GATED, ACT>(acc[t], 0, v);
+                if constexpr (LAST) {
+                    if (t * 32 < here) mx_results<T, true, 1>(p, v, ai, d0, bt, lane, n0, t, here, (uint8_t *)stage + wave * MX_STAGE);
+                } else {
+                    T *const to = stage + (t * 32 + l32) * pitch + ((bt - chunk) * 32 + 16 * half) * dc + j;
 #pragma unroll
-                    for (int j = 0; j < D; ++j) mx_activate<T, D, GATED, ACT>(acc[t][j], j, v);
-                    mx_results<T, LAST, D>(p, v, ai, d0, bt, lane, n0, t, here, stage);
+                    for (int i = 0; i < 16; ++i) to[i * dc] = v[i];
                 }
+            }
+        }
+        if constexpr (!LAST) {
+            __syncthreads();
+            // pieces of a line that lie together: all of it, or with more d_i than the unit's, those of an output
+            constexpr int E = 16 / (int)sizeof(T);
+            const int outs = (chunk + p.chunk_tiles) * 32 < p.b ? p.chunk_tiles * 32 : p.b - chunk * 32, tiles_out = (chunk_end - chunk) * 32;
+            const int lines = outs < tiles_out ? outs : tiles_out;  // outputs of the chunk
+            const int piece = dc == p.d ? lines * dc : dc, pieces = dc == p.d ? 1 : lines, vectors = (piece + E - 1) / E;
+            const MxDiv by_vectors(vectors), by_pieces(pieces);
+            for (int i = threadIdx.x; i < here * pieces * vectors; i += 64 * MX_WAVES) {
+                const int u = by_vectors(i), e = (i - u * vectors) * E, n = by_pieces(u), q = u - n * pieces;
+                const T *from = stage + n * pitch + q * dc + e;
+                T *to = (T *)p.y + (((n0 + n) * p.a + ai) * p.b + chunk * 32 + q) * p.d + d0 + e;
+                if (e + E <= piece) {
+                    T v[E];
+                    if (sizeof(T) == 4 || dc % 2 == 0 || pieces == 1) {  // (words)
+                        __builtin_memcpy(v, __builtin_assume_aligned(from, 4), 16);
+                    } else {
+#pragma unroll
+                        for (int k = 0; k < E; ++k) v[k] = from[k];
+                    }
+                    mx_store<T, E>(to, v);
+                } else {
+                    for (int k = 0; k < piece - e; ++k) to[k] = from[k];
+                }
+            }
+            __syncthreads();
         }
     }
 }
@@ -438,36 +575,32 @@ inline int64_t mx_held_lds(int d, bool gated, int ks, int cb, int rows, int tile
     return (int64_t)buffers * d * rows * ((cb | 1) * 16 + 2 * mx_scale_bytes(ks)) + (int64_t)tiles * (gated ? 2 : 1) * 32 * d * 4 + waves * MX_STAGE;
 }
 
-template <typename T, bool LAST, int D, int TT, bool GATED> int mx_launch(MxProduct p, int act, hipStream_t s)
+template <typename T, bool LAST, int D, int TT, bool GATED> int mx_launch_wide(MxProduct p, int act, hipStream_t s)
 {
     p.slots = p.cb | 1;
-    p.runs = p.d / D;
+    p.run_d = mx_unit_of(p.d, LAST);
+    p.runs = (p.d + p.run_d - 1) / p.run_d;
     p.units = p.a * p.runs;
     p.b_tiles = (p.b + 31) / 32;
+    p.chunk_tiles = mx_chunk_of(p.run_d, LAST);
     p.token_tiles = (p.batch + 32 * TT - 1) / (32 * TT);
-    // units whose values share a line of 128 bytes go to one workgroup, unless there are few
-    p.units_per = 1;
-    if (!LAST) {
-        const int64_t bytes = (int64_t)(p.d == D ? p.c * D : D) * (int64_t)sizeof(T);
-        const int64_t share = bytes >= 128 ? 1 : 128 / bytes;
-        if (p.token_tiles * p.units / share >= 1024) p.units_per = (int)(share < p.units ? share : p.units);
-    }
-    p.unit_groups = (p.units + p.units_per - 1) / p.units_per;
     // outputs are split over workgroups, each of which quantises its rows anew, until there are 1024
-    const int64_t groups = p.token_tiles * p.unit_groups;
-    const int most = (p.b_tiles + MX_WAVES - 1) / MX_WAVES;
+    const int64_t groups = p.token_tiles * p.units;
+    const int most = (p.b_tiles + p.chunk_tiles - 1) / p.chunk_tiles;
     const int64_t want = groups >= 1024 ? 1 : (1024 + groups - 1) / groups;
     p.splits = (int)(want < most ? want : most);
-    p.tiles_per = (p.b_tiles + p.splits - 1) / p.splits;
+    p.tiles_per = (most + p.splits - 1) / p.splits * p.chunk_tiles;
     p.splits = (p.b_tiles + p.tiles_per - 1) / p.tiles_per;
     const int64_t grid = groups * p.splits;
     if (grid > 0x7fffffffLL) return KSMM_ERR_TOO_LARGE;
-    const int lds = (int)mx_lds(TT, D, p.cb);
+    const int lds = (int)mx_wide_lds(TT, p.c, p.d, (int)sizeof(T), LAST);
+    p.raw_pitch = (int)(mx_raw_row(p.c, p.d, (int)sizeof(T)) / (int)sizeof(T));
+    p.raw_rows = mx_raw_rows(TT, p.c, p.d, (int)sizeof(T));
     int rc = KSMM_OK;
     with_act(act, [&](auto which) {
         constexpr int ACT = decltype(which)::value;
         if constexpr (GATED || ACT != KSMM_ACT_SILU) {
-            auto fn = &ks_mx_fused_kernel<T, LAST, D, TT, GATED, ACT>;
+            auto fn = &ks_mx_wide_kernel<T, LAST, D, TT, GATED, ACT>;
             if (lds > 64 * 1024) rc = ensure_dynamic_lds((const void *)fn, lds);
             if (rc != KSMM_OK) return;
             hipLaunchKernelGGL(fn, dim3((unsigned)grid), dim3(64 * MX_WAVES), lds, s, p);
@@ -477,11 +610,18 @@ template <typename T, bool LAST, int D, int TT, bool GATED> int mx_launch(MxProd
     return rc;
 }
 
+// registers of a thread
+inline int mx_registers(const void *kernel)
+{
+    hipFuncAttributes a;
+    return hipFuncGetAttributes(&a, kernel) == hipSuccess ? a.numRegs : 512;
+}
+
 template <typename T, bool LAST, int D, bool GATED, int KS> int mx_launch_held(MxProduct p, int act, hipStream_t s)
 {
-    constexpr int MOST = 64 * MX_PRODUCERS * mx_rounds(KS);  // blocks a step
+    constexpr int Q = mx_quarters<T>(LAST, KS, D), MOST = 64 * MX_PRODUCERS * mx_rounds(KS, Q) / Q;  // blocks a step
     p.slots = p.cb | 1;
-    p.runs = p.d / D;
+    p.runs = LAST ? p.d : 1;
     p.units = p.a * p.runs;
     p.b_tiles = (p.b + 31) / 32;
     // eight waves: the more of them share their rows the less often these are quantised, but none should idle
@@ -496,10 +636,22 @@ template <typename T, bool LAST, int D, bool GATED, int KS> int mx_launch_held(M
     p.tile_rows = 32 * MX_CONSUMERS / p.wave_tiles;
     auto groups = [&] { return (int64_t)p.units * ((p.b_tiles + p.wave_tiles - 1) / p.wave_tiles); };
     p.token_tiles = (p.batch + p.tile_rows - 1) / p.tile_rows;
-    // a workgroup a compute unit (its twelve waves take the registers of one): one more would be a second round.  Those of the same
-    // rows lie on the same XCD where that is a multiple of eight apart
-    int64_t most = std::max<int64_t>(1, 256 / groups());
-    if (most >= 8) most = most / 8 * 8;
+    // a workgroup a compute unit, or two where the registers of both fit: one more would be a second round.  Those of the same rows lie on
+    // the same XCD where that is a multiple of eight apart
+    auto most_of = [&](int a_unit) {
+        const int64_t most = std::max<int64_t>(1, 256 * a_unit / groups());
+        return most >= 8 ? most / 8 * 8 : most;
+    };
+    int64_t most = most_of(1);
+    if (p.token_tiles > most && mx_held_lds(D, GATED, KS, p.cb, p.tile_rows, p.wave_tiles, 2, MX_CONSUMERS) <= 80 * 1024) {
+        with_act(act, [&](auto which) {
+            constexpr int ACT = decltype(which)::value;
+            if constexpr (GATED || ACT != KSMM_ACT_SILU) {
+                static const int registers = mx_registers((const void *)&ks_mx_held_kernel<T, LAST, D, GATED, ACT, KS>);
+                if (registers <= 80) most = most_of(2);  // (six waves of each SIMD's 512)
+            }
+        });
+    }
     p.row_splits = (int)std::min(p.token_tiles, most);
     p.buffers = 2;
     if (groups() * p.token_tiles < 512) {  // few: smaller workgroups of one step each
@@ -532,8 +684,9 @@ template <typename T, bool LAST, int D, bool GATED, int KS> int mx_launch_held(M
 // steps of 64 along c that a kernel is made for
 template <typename T, bool LAST, int D, bool GATED, int KS, int... MORE> int mx_held(const MxProduct &p, int act, hipStream_t s)
 {
-    // registers (168 of them): of one wave the weights' codes (4 a step) and the results, of another the values on their way; more spill
-    constexpr bool fits = D * (GATED ? 2 : 1) * KS <= (D < 4 ? 16 : 8) && D * 8 * (int)sizeof(T) <= 64;
+    // registers (168 of them): the weights' codes, sums and results of a wave; with more it spills (4 d_i: all of them live longer)
+    constexpr int SIZE = (int)sizeof(T), HELD = 4 * D * (GATED ? 2 : 1) * KS + 16 * (GATED ? 2 : 1) + 4 * D * SIZE;
+    constexpr bool fits = D < 4 ? HELD <= (D == 3 ? 104 : 112) : SIZE == 2 && D * (GATED ? 2 : 1) * KS <= 8;
     if constexpr (fits) {
         if (p.cb <= 2 * KS) return mx_launch_held<T, LAST, D, GATED, KS>(p, act, s);
         if constexpr (sizeof...(MORE) > 0) return mx_held<T, LAST, D, GATED, MORE...>(p, act, s);
@@ -543,27 +696,25 @@ template <typename T, bool LAST, int D, bool GATED, int KS, int... MORE> int mx_
 
 template <typename T, bool LAST, int D, bool GATED> int mx_pick(const MxProduct &p, int act, hipStream_t s)
 {
-    if (!p.x_scales) {
+    if (!p.x_scales && (LAST || p.d == D)) {
         const int rc = mx_held<T, LAST, D, GATED, 1, 2, 3, 4, 6, 8, 16>(p, act, s);
         if (rc != KSMM_ERR_BAD_ALGO) return rc;
     }
-    // as many rows a workgroup as accumulators hold, where that leaves two workgroups for a compute unit
-    constexpr int TT = mx_rows_of(D, GATED);
-    if constexpr (TT > 1) {
-        const int64_t groups = (p.batch + 32 * TT - 1) / (32 * TT) * p.a * (p.d / D) * ((p.b + 32 * MX_WAVES - 1) / (32 * MX_WAVES));
-        if (groups >= 512 && mx_lds(TT, D, p.cb) <= MX_LDS_MOST) return mx_launch<T, LAST, D, TT, GATED>(p, act, s);
-    }
-    return mx_launch<T, LAST, D, 1, GATED>(p, act, s);
+    // twice the rows for the same weights, where that leaves two workgroups for a compute unit
+    const int unit = mx_unit_of(p.d, LAST), chunk = mx_chunk_of(unit, LAST);
+    const int64_t groups = (p.batch + 63) / 64 * p.a * ((p.d + unit - 1) / unit) * ((p.b + 32 * chunk - 1) / (32 * chunk));
+    if (groups >= 512 && mx_wide_lds(2, p.c, p.d, (int)sizeof(T), LAST) <= MX_LDS_MOST) return mx_launch_wide<T, LAST, D, 2, GATED>(p, act, s);
+    return mx_launch_wide<T, LAST, D, 1, GATED>(p, act, s);
 }
 
 template <typename T, bool GATED> int mx_last(const MxProduct &p, int act, hipStream_t s) { return mx_pick<T, true, 1, GATED>(p, act, s); }
 template <typename T, bool GATED> int mx_first(const MxProduct &p, int act, hipStream_t s)
 {
-    switch (mx_run_of(p.d)) {
-    case 1: return mx_pick<T, false, 1, GATED>(p, act, s);
+    switch (p.d) {
     case 2: return mx_pick<T, false, 2, GATED>(p, act, s);
     case 3: return mx_pick<T, false, 3, GATED>(p, act, s);
-    default: return mx_pick<T, false, 4, GATED>(p, act, s);
+    case 4: return mx_pick<T, false, 4, GATED>(p, act, s);
+    default: return mx_pick<T, false, 1, GATED>(p, act, s);
     }
 }
 

@@ -114,7 +114,8 @@ def test_ends_of_the_fp32_range():
 
 
 PATTERNS = [(1, 1, 1, 1), (2, 5, 3, 2), (1, 32, 32, 1), (3, 33, 40, 1), (1, 64, 192, 2), (2, 20, 65, 3), (1, 100, 64, 6), (1, 16, 48, 16), (1, 130, 300, 4),
-            (6, 64, 64, 1), (1, 200, 1030, 1), (1, 8, 16, 37), (2, 96, 72, 3), (1, 48, 96, 64), (1, 768, 192, 2), (5, 34, 128, 8), (1, 9, 5000, 1), (1, 9, 1400, 4), (40, 16, 16, 1), (70, 4, 4, 1)]
+            (6, 64, 64, 1), (1, 200, 1030, 1), (1, 8, 16, 37), (2, 96, 72, 3), (1, 48, 96, 64), (1, 768, 192, 2), (5, 34, 128, 8), (1, 9, 5000, 1), (1, 9, 1400, 4), (40, 16, 16, 1), (70, 4, 4, 1),
+            (1, 40, 70, 17), (1, 33, 33, 20), (1, 24, 3000, 5), (2, 64, 64, 7), (1, 70, 384, 4)]
 
 
 @pytest.mark.parametrize("bs_last", [False, True])
