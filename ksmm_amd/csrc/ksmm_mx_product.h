@@ -266,8 +266,12 @@ __global__ __launch_bounds__(64 * (MX_CONSUMERS + MX_PRODUCERS)) void ks_mx_held
     const int wb = wave & (p.wave_tiles - 1), wt = wave / p.wave_tiles, per_wave = TN / 32 / (consumers / p.wave_tiles);
     const int bt = tile0 + wb;
     const bool busy = bt < p.b_tiles;
+    // (one step: its rows are on their way before the weights are, so that it waits for both at once)
+    Load f;
+    const int at = one ? place(threadIdx.x) : 0;
+    if (one) fetch(f, threadIdx.x, at, first * TN);
     uint4_t w[D][G][KS];
-    int sw[D][G][SW];
+    int sw[D][G][SW], scale[D][G][KS];
     if (busy) {
         const int wo = bt * 32 + (LAST ? l32 : run), o = wo < p.b ? wo : p.b - 1;  // (outputs behind the last one are read as the last one)
 #pragma unroll
@@ -280,21 +284,26 @@ __global__ __launch_bounds__(64 * (MX_CONSUMERS + MX_PRODUCERS)) void ks_mx_held
                     const int kb = 2 * s + half;
                     const bool there = kb < p.cb;
                     w[j][q][s] = there ? *(const uint4_t *)(p.w + (at + kb) * 16) : uint4_t{0, 0, 0, 0};
-                    const int scale = there ? p.w_scales[at + kb] : 127;
-                    sw[j][q][s / 4] = s % 4 ? sw[j][q][s / 4] | scale << 8 * (s % 4) : scale;
+                    scale[j][q][s] = there ? p.w_scales[at + kb] : 127;
                 }
             }
     }
     prepare();
     __syncthreads();
     if (one) {
-        Load f;
-        for (int t = threadIdx.x; t < tasks * Q; t += threads) {
-            const int at = place(t);
-            fetch(f, t, at, first * TN);
-            keep(f, t, at, first * TN, 0);
+        keep(f, threadIdx.x, at, first * TN, 0);
+        for (int t = threadIdx.x + threads; t < tasks * Q; t += threads) {
+            const int more = place(t);
+            fetch(f, t, more, first * TN);
+            keep(f, t, more, first * TN, 0);
         }
     }
+#pragma unroll
+    for (int j = 0; j < D; ++j)
+#pragma unroll
+        for (int q = 0; q < G; ++q)
+#pragma unroll
+            for (int s = 0; s < KS; ++s) sw[j][q][s / 4] = s % 4 ? sw[j][q][s / 4] | scale[j][q][s] << 8 * (s % 4) : scale[j][q][s];
     // (said to the compiler: the weights are there, and no step waits for them again, which would be for all stores before it too)
 #pragma unroll
     for (int j = 0; j < D; ++j)
