@@ -340,3 +340,56 @@ def test_without_the_native_module(monkeypatch, bits):
     monkeypatch.setattr(_lib, "_native", _lib._NoNative)
     for x, y in zip(native, everything()):
         assert torch.equal(x, y)
+
+
+def test_places_beyond_31_bits_of_bytes():
+    """A tensor of almost 2^31 values: its ends as tensors of their own, rounded by the hash of their own places."""
+    from ksmm_amd import adamw_moments, adamw_update
+
+    n, k = (1 << 31) - 16384, 4096
+    w = torch.zeros(n, dtype=torch.float16, device="cuda")
+    g = torch.zeros(n, dtype=torch.float16, device="cuda")
+    m, v, s = torch.zeros(n, dtype=torch.uint8, device="cuda"), torch.zeros(n, dtype=torch.uint8, device="cuda"), torch.zeros(2, n // 32, dtype=torch.uint8, device="cuda")
+    part = make([k], "fp16", 8, False)
+    for at in (0, n - k):
+        w[at:at + k], g[at:at + k], m[at:at + k], v[at:at + k] = part["w"][0], part["g"][0], part["m"][0], part["v"][0]
+        s[:, at // 32:(at + k) // 32] = part["scales"][0]
+    adamw_update([w], [g], [m], [v], [s], step=5, seed=2, **HOW)
+    m0, v0 = R.decode_moments(part["m"][0], part["v"][0], part["scales"][0])
+    w1, m1, v1 = R.adamw(part["w"][0].cpu().double(), part["g"][0], m0, v0, 5, HOW["lr"], HOW["betas"], HOW["eps"], HOW["weight_decay"], HOW["grad_scale"])
+    key = R._mix((R._mix(2) + 5) & 0xFFFFFFFF)
+    for at in (0, n - k):
+        h = R._mix(torch.arange(at, at + k, dtype=torch.int64) ^ key)
+        cm, cv, sc = R.encode_moments(m1, v1, (h & 0xFFFF).double() / 65536, (h >> 16).double() / 65536)
+        assert torch.equal(s[:, at // 32:(at + k) // 32].cpu(), sc)
+        got = R.decode_moments(m[at:at + k], v[at:at + k], s[:, at // 32:(at + k) // 32])
+        assert all(torch.equal(x, y) for x, y in zip(got, R.decode_moments(cm, cv, sc)))
+        assert float((w[at:at + k].cpu().double() - w1).abs().max()) <= 2.0 ** -11 * float(w1.abs().max()) + 1e-6
+    assert not w[k:k + 1000].any() and not m[n // 2:n // 2 + 1000].any()
+
+
+def test_threads_at_once():
+    import threading
+
+    from ksmm_amd import adamw_update
+
+    alone, sets = [], []
+    for i in range(4):
+        s = make([1000 + i, 77], "fp32", 8, False, seed=i)
+        adamw_update(s["w"], s["g"], s["m"], s["v"], s["scales"], seed=i, **HOW)
+        alone.append(s)
+        sets.append(make([1000 + i, 77], "fp32", 8, False, seed=i))
+    torch.cuda.synchronize()
+
+    def work(s, i):
+        with torch.no_grad(), torch.cuda.stream(torch.cuda.Stream()):
+            adamw_update(s["w"], s["g"], s["m"], s["v"], s["scales"], seed=i, **HOW)
+            torch.cuda.current_stream().synchronize()
+
+    threads = [threading.Thread(target=work, args=(s, i)) for i, s in enumerate(sets)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for x, y in zip(alone, sets):
+        assert all(torch.equal(p, q) for k in ("w", "m", "v", "scales") for p, q in zip(x[k], y[k]))

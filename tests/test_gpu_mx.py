@@ -416,3 +416,119 @@ def test_without_the_native_module(monkeypatch, bs_last):
     monkeypatch.setattr(_lib, "_native", _lib._NoNative)
     for x, y in zip(native, everything()):
         assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("bs_last", [False, True])
+@pytest.mark.parametrize("pattern", [(1, 6, 9000, 1), (1, 5, 1200, 16), (2, 40, 2500, 2)])
+def test_more_than_local_memory_holds(pattern, bs_last):
+    """c so large that a workgroup cannot keep the codes of 32 rows."""
+    from ksmm_amd import MXKernel, mx_linear, pack_mx, quantize_mx
+
+    a, b, c, d = pattern
+    for prec in ("fp16", "fp32"):
+        for n, gated, act in ((3, True, "silu"), (70, False, "gelu")):
+            x, f = rows(n, a * c * d, bs_last, DT[prec], n).cuda(), factor(pattern, gated, DT[prec]).cuda()
+            w, q = pack_mx(f, pattern, gated), quantize_mx(x, (a, c, d), bs_last)
+            y, codes, scales = MXKernel.forward(x, w, None, act, bs_last, need_codes=True)
+            want = R.product(R.rounded(R.operand(x, a, c, d, bs_last)), R.rounded(factor_rows(f, pattern)), None, pattern, act, gated, bs_last)
+            # (sums of 9000 terms in fp32, at random: sqrt(9000) 2^-24, 6e-6 of the sum's deviation)
+            assert rel(y, R.tensor(want, y.shape, bs_last)) <= max(TOL[prec], 6e-6)
+            assert torch.equal(codes, q.codes) and torch.equal(scales, q.scales) and torch.equal(mx_linear(q, w, act=act, bs_last=bs_last), y)
+
+
+@pytest.mark.parametrize("bs_last", [False, True])
+def test_offsets_beyond_31_bits(bs_last):
+    """Tensors of almost 2^31 elements: their last rows as a tensor of their own."""
+    from ksmm_amd import MXKernel, mx_linear, pack_mx, quantize_mx
+
+    pattern, n = (1, 64, 64, 1), (1 << 25) - 4096
+    w = pack_mx(factor(pattern, False, torch.float16).cuda(), pattern)
+    part = rows(100, 64, False, torch.float16).cuda()
+    x = torch.zeros((64, n) if bs_last else (n, 64), dtype=torch.float16, device="cuda")
+    for at in (0, n // 2 + 7, n - 100):
+        if bs_last:
+            x[:, at:at + 100] = part.t()
+        else:
+            x[at:at + 100] = part
+    y, codes, scales = MXKernel.forward(x, w, None, None, bs_last, need_codes=True)
+    small = (part.t() if bs_last else part).contiguous()
+    want, q = mx_linear(small, w, bs_last=bs_last), quantize_mx(small, (1, 64, 1), bs_last)
+    big = quantize_mx(x, (1, 64, 1), bs_last)
+    assert torch.equal(big.codes, codes) and torch.equal(big.scales, scales)
+    back = big.dequantize()
+    for at in (0, n // 2 + 7, n - 100):
+        assert torch.equal(y[:, at:at + 100] if bs_last else y[at:at + 100], want)
+        assert torch.equal(codes[:, at:at + 100], q.codes) and torch.equal(scales[:, at:at + 100], q.scales)
+        assert torch.equal(back[:, at:at + 100] if bs_last else back[at:at + 100], q.dequantize())
+    assert not (y[:, 200:300] if bs_last else y[200:300]).any()
+
+
+def test_traced_modules_compute():
+    from ksmm_amd import KSLinearMX
+
+    torch.manual_seed(0)
+    layer = KSLinearMX([(6, 64, 64, 1), (1, 96, 192, 2)], dtype=torch.float16)
+    x, other = (torch.randn(9, 384, device="cuda").half() for _ in range(2))
+    traced = torch.jit.trace(layer, (x,), check_trace=False)
+    assert torch.equal(traced(other), layer(other))
+
+
+def test_threads_at_once():
+    """Calls of several threads on streams of their own."""
+    import threading
+
+    from ksmm_amd import mx_linear, pack_mx
+
+    pattern = (1, 96, 192, 2)
+    f = factor(pattern, True, torch.float16).cuda()
+    w = pack_mx(f, pattern, True)
+    xs = [rows(300 + 7 * i, 384, False, torch.float16, i).cuda() for i in range(4)]
+    want = [mx_linear(x, w, act="silu") for x in xs]
+    torch.cuda.synchronize()
+    got = [None] * 4
+
+    def work(i):
+        with torch.no_grad(), torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(10):
+                got[i] = mx_linear(xs[i], w, act="silu")
+            torch.cuda.current_stream().synchronize()
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert all(torch.equal(x, y) for x, y in zip(got, want))
+
+
+@pytest.mark.parametrize("gated", [False, True])
+def test_captured_training(gated):
+    """Forward and backward pass of a captured step, replayed on new inputs."""
+    from ksmm_amd import mx_linear
+
+    pattern = (1, 96, 64, 2)
+    x = rows(70, 128, False, torch.float16).cuda().requires_grad_(True)
+    f = factor(pattern, gated, torch.float16).cuda().requires_grad_(True)
+    dy = rows(70, 192, False, torch.float16, 3).cuda()
+
+    def step():
+        with torch.enable_grad():
+            y = mx_linear(x, f, pattern, act="gelu", gated=gated)
+            return (y.detach(), *torch.autograd.grad(y, (x, f), dy))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for i in range(4):
+        with torch.no_grad():
+            x.copy_(rows(70, 128, False, torch.float16, 20 + i).cuda())
+            f.copy_(factor(pattern, gated, torch.float16, 30 + i).cuda())
+        graph.replay()
+        torch.cuda.synchronize()
+        for got, want in zip(out, step()):
+            assert torch.equal(got, want), i
