@@ -14,6 +14,7 @@
 #include <ATen/ATen.h>
 #include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPStream.h>
+#include <hip/hip_runtime_api.h>
 #include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
@@ -767,6 +768,20 @@ int mx_forward(const void *x, const void *x_scales, const at::Tensor &w, const a
                            scales ? out_of(*scales) : nullptr, out_of(ws), need, h.batch, h.a, h.b, h.c, h.d, dt, h.bs_last, act, h.gated, stream_of(y));
 }
 
+// A pass that is being captured is refused where it comes to a node of the default stream: a leaf that an eager graph outside still
+// holds.  The engine would make the default stream wait for the captured one, which is an error where nothing catches it.
+void refuse_outside(const ag::edge_list &edges, void *stream)
+{
+    for (const ag::Edge &e : edges) {
+        const auto other = e.function ? e.function->stream() : c10::nullopt;
+        if (!other || other->id() != 0 || !stream) continue;
+        hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+        if (hipStreamIsCapturing((hipStream_t)stream, &status) != hipSuccess) status = hipStreamCaptureStatusNone;
+        TORCH_CHECK(status == hipStreamCaptureStatusNone,
+                    "mx_linear: a backward pass cannot be captured while a graph of the same leaves from outside the capture is alive; drop what holds it first");
+    }
+}
+
 struct MxNode : ag::Node {
     ag::SavedVariable in[5];  // codes and scales of x and of the factor, bias
     MxHow how;
@@ -790,6 +805,7 @@ struct MxNode : ag::Node {
             DeviceScope scope(dy.device().index());
             const int dt = code_of(dy.scalar_type());
             void *const stream = stream_of(dy);
+            refuse_outside(next_edges(), stream);
             const int64_t features = (int64_t)how.a * how.c * how.d;
             at::Tensor x = at::empty(x_shape, dy.options()), w = at::empty({features, how.rows()}, dy.options());
             check_status(ksmm_mx_dequantize(data_of(t[0]), data_of(t[1]), out_of(x), how.batch, how.a, how.c, how.d, dt, how.bs_last, stream));

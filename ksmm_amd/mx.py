@@ -206,6 +206,8 @@ class MXKernel:
             need = lib.ksmm_mx_forward_workspace(batch, a, b, c, d, dt, int(bs_last), int(factor.gated))
             if need < 0:
                 _lib.check(int(need))
+            if workspace is not None and (workspace.device != x.device or not workspace.is_contiguous()):
+                raise ValueError("workspace must be contiguous on %s" % (x.device,))
             if need > 0 and (workspace is None or workspace.numel() * workspace.element_size() < need):
                 workspace = torch.empty(need, dtype=torch.uint8, device=x.device)
         with torch.cuda.device(x.device):
@@ -408,6 +410,6 @@ class KSFeedForwardMX(KSFeedForward):
 def pack_block(block):
     """A copy of a ``KSFeedForward`` whose factors are packed; its norm is copied too."""
     new = copy.copy(block)
-    new._modules = dict(block._modules)
+    new._modules, new._parameters, new._buffers = dict(block._modules), dict(block._parameters), dict(block._buffers)
     new.gated, new.down, new.norm = MXLinear.of(block.gated), MXLinear.of(block.down), copy.deepcopy(block.norm)
     return new

@@ -306,6 +306,9 @@ def test_refusals():
         quantize_mx(x.double(), (2, 64, 1))
     with pytest.raises(RuntimeError):
         MXKernel.forward(x, w, out=x.view(-1)[:320].view(4, 80))
+    for ws in (torch.empty(1 << 20, dtype=torch.uint8), torch.empty(8, 8, dtype=torch.uint8, device="cuda").t()):
+        with pytest.raises(ValueError):
+            MXKernel.forward(x, w, workspace=ws)
 
 
 def test_captured_and_replayed():
@@ -532,3 +535,41 @@ def test_captured_training(gated):
         torch.cuda.synchronize()
         for got, want in zip(out, step()):
             assert torch.equal(got, want), i
+
+
+@pytest.mark.parametrize("leaf", ["x", "factor", "bias"])
+@torch.enable_grad()
+def test_captured_backward_beside_an_eager_graph_of_its_leaves(leaf):
+    """Refused before anything is enqueued: the eager graph's nodes of the leaves belong to the default stream."""
+    from ksmm_amd import mx_linear
+
+    pattern = (1, 40, 64, 2)
+    x = rows(9, 128, False, torch.float16).cuda().requires_grad_(leaf == "x")
+    f = factor(pattern, False, torch.float16).cuda().requires_grad_(leaf == "factor")
+    bias = torch.zeros(80, device="cuda").half().requires_grad_(leaf == "bias")
+    leaves = [t for t in (x, f, bias) if t.requires_grad]
+    dy = rows(9, 80, False, torch.float16, 3).cuda()
+    torch.autograd.grad(mx_linear(x, f, pattern, bias), leaves, dy)
+    eager = mx_linear(x, f, pattern, bias)
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="cannot be captured"):
+        with torch.cuda.graph(graph):
+            torch.autograd.grad(mx_linear(x, f, pattern, bias), leaves, dy)
+    want = torch.autograd.grad(eager, leaves, dy)
+    del eager, graph
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = torch.autograd.grad(mx_linear(x, f, pattern, bias), leaves, dy)
+    for _ in range(2):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got[0], want[0])
+
+
+def test_packed_blocks_are_their_own():
+    from ksmm_amd import KSFeedForward, pack_block
+
+    block = KSFeedForward((1, 64, 32, 2), [(1, 32, 64, 2)])
+    new = pack_block(block)
+    new.register_buffer("more", torch.zeros(1))
+    assert not hasattr(block, "more") and "gated" in block._modules and type(block.gated) is not type(new.gated)

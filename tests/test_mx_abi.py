@@ -41,15 +41,16 @@ def test_conversions_refuse(lib, back, bs_last):
     assert call(x=codes + 16 * blocks - 1) == ALIAS and call(scales=codes + 16 * blocks - 1) == ALIAS
 
 
-def test_products_refuse(lib):
-    n, a, b, c, d = 9, 2, 24, 40, 3
+@pytest.mark.parametrize("c", [40, 9000])
+def test_products_refuse(lib, c):
+    n, a, b, d = 9, 2, 24, 3
     names = ["x", "x_scales", "w", "w_scales", "bias", "y", "codes", "scales", "workspace"]
     at = dict(zip(names, FAR))
     for dtype, size in ((0, 4), (1, 2)):
         for gated in (0, 1):
             for bs_last in (0, 1):
                 need = lib.ksmm_mx_forward_workspace(n, a, b, c, d, dtype, bs_last, gated)
-                assert need >= 0
+                assert (need > 0) == (c == 9000)
 
                 def call(quantised, bytes=need, act=0, n=n, a=a, b=b, c=c, d=d, dtype=dtype, gated=gated, **change):
                     p = dict(at, **change)
@@ -65,7 +66,7 @@ def test_products_refuse(lib):
                         assert call(q, act=2) == EPILOGUE
                     assert call(q, w=at["w"] + 8) == WORKSPACE
                     rows = b * (1 + gated)
-                    blocks = 2 * a * d
+                    blocks = (c + 31) // 32 * a * d
                     sizes = {"x": n * blocks * 16 if q else n * a * c * d * size, "x_scales": n * blocks, "w": rows * blocks * 16, "w_scales": rows * blocks,
                              "bias": a * rows * d * size}
                     for k in sizes:
@@ -105,7 +106,7 @@ def test_steps_refuse(lib, bits):
         return lib.ksmm_adamw_update(ctypes.byref(d or desc(bits)), t if t is not None else table(), count, dtype, None)
 
     nan, inf = float("nan"), float("inf")
-    for change in (dict(beta1=1.0), dict(beta2=1.0), dict(beta1=-0.1), dict(beta2=nan), dict(lr=inf), dict(eps=nan), dict(weight_decay=inf), dict(grad_scale=nan), dict(step=0),
+    for change in (dict(beta1=1.0), dict(beta2=1.0), dict(beta1=-0.1), dict(beta2=nan), dict(lr=inf), dict(eps=nan), dict(eps=1e-38), dict(weight_decay=inf), dict(grad_scale=nan), dict(step=0),
                    dict(step=-5)):
         assert call(desc(bits, **change)) == ALGO, change
     assert call(desc(16)) == DTYPE and call(dtype=2) == DTYPE and call(count=-1) == BATCH
