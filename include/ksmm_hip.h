@@ -424,7 +424,7 @@ int ksmm_mx_forward(const void *x, const void *x_scales, const void *w, const vo
  * 127), in scales (2, ceil(n / 32)), m's first.  m is e4m3fn behind 2^(floor(log2 max |m|) - 7), v an unsigned e5m3, the bits 14 to 7
  * of an fp16 number, behind 2^(floor(log2 max v) - 14); exponents are -120 at least.  They are rounded down, or up with
  * the probability of what is cut off, by a hash of seed + the tensor's number, step and place; v > 0 stays above zero.  Values beyond
- * fp32 become NaN (m) or infinity (v), alone.  m and v of zeros with scales of any kind are a state to start from.
+ * fp32 become NaN (m) or infinity (v), alone.  Zeros everywhere are a state to start from.  eps: none below 2^-126 but 0.
  * What is written must not overlap anything else: no tensor may be there twice. */
 typedef struct ksmm_adamw_tensor {
     void *weight;

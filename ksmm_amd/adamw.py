@@ -42,7 +42,7 @@ def adamw_update(params, grads, exp_avgs, exp_avg_sqs, scales=None, masters=None
     their mean is kept.  Zeros everywhere are a state to start from.
     ``masters``: fp32 weights that the parameters are rounded from; they are read instead of them and written too.
     ``follow``: a parameter that is not what its master rounds to was written since, and counts instead.
-    ``step``: from 1 on, or an int64 tensor of one value on the device, which a captured graph reads anew on every replay.
+    ``eps``: 0, or 2^-126 and more.  ``step``: from 1 on, or an int64 tensor of one value on the device, which a captured graph reads anew on every replay.
     What a NaN or an infinity among the gradients reaches is its own element alone."""
     if len(betas) != 2:
         raise ValueError("betas must be two values from 0 on and below 1, not %s" % (betas,))
@@ -122,7 +122,7 @@ class KSAdamW(torch.optim.Optimizer):
     rounded from fp32 weights that the optimiser keeps (``master=False``: updated as they are); values that were written into
     a parameter since replace them.  ``grad_scale`` multiplies the gradients: one over a loss's scale.  ``capturable``: the count of steps is
     a tensor of the group's on its one device, so that a captured step counts on with every replay (a step before the capture sets the
-    state up)."""
+    state up; without either a capture is refused)."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01, bits=32, master=True, grad_scale=1.0, seed=0,
                  capturable=False):
@@ -192,8 +192,11 @@ class KSAdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
+        capturing = torch.cuda.is_current_stream_capturing()
         for g in self.param_groups:
             sets = {}
+            if capturing and not (g["capturable"] and g.get("step") is not None and all(self.state[p] for p in g["params"] if p.grad is not None)):
+                raise RuntimeError("a captured step needs capturable=True and a step before the capture: it would not count, or begin anew on every replay")
             if g["capturable"]:
                 if g.get("step") is None:
                     g["step"] = torch.zeros(1, dtype=torch.int64, device=g["params"][0].device)

@@ -61,8 +61,8 @@ struct Common {
     uint32_t chunk;  // values a workgroup takes: of 256 threads two of 8 each, or where that makes few, of 64 threads one of 8 each
     uint32_t seed;  // the first tensor's
     int follow;
-    float keep, lr, rate, root, eps;  // rate, root: of the step, or (with `step`) to be found from it
-    double beta1, beta2, scale;
+    float keep, rate, root, eps;  // rate, root: of the step, or (with `device_step`) to be found from it
+    double lr, beta1, beta2, scale;
     int64_t step;
     const int64_t *device_step;
 };
@@ -201,7 +201,7 @@ template <typename T, int BITS, bool MASTER> __global__ __launch_bounds__(256) v
         step = *a.device_step;
         if (threadIdx.x == 0) {
             const double at = step < 1 ? 1.0 : (double)step;
-            of_step[0] = (float)((double)a.lr / (1.0 - pow(a.beta1, at)));
+            of_step[0] = (float)(a.lr / (1.0 - pow(a.beta1, at)));
             of_step[1] = (float)(1.0 / sqrt(1.0 - pow(a.beta2, at)));
         }
         __syncthreads();
@@ -361,6 +361,7 @@ int ksmm_adamw_update(const ksmm_adamw_desc *desc, const ksmm_adamw_tensor *tens
         if (!(b >= 0.0 && b < 1.0)) return KSMM_ERR_BAD_ALGO;
     for (double r : rates)
         if (!std::isfinite(r)) return KSMM_ERR_BAD_ALGO;
+    if (desc->eps != 0.0 && std::fabs(desc->eps) < FLT_MIN) return KSMM_ERR_BAD_ALGO;  // (0 / eps is 0: its reciprocal has to be a number)
     if (!desc->device_step && desc->step < 1) return KSMM_ERR_BAD_ALGO;
     const int64_t size = (int64_t)dtype_size(dtype);
     const bool small = desc->bits == 8;
@@ -397,7 +398,7 @@ int ksmm_adamw_update(const ksmm_adamw_desc *desc, const ksmm_adamw_tensor *tens
         a.seed = desc->seed;
         a.follow = desc->follow;
         a.keep = (float)(1.0 - desc->lr * desc->weight_decay);
-        a.lr = (float)desc->lr;
+        a.lr = desc->lr;
         a.rate = desc->device_step ? 0.f : (float)(desc->lr / (1.0 - std::pow(desc->beta1, at)));
         a.root = desc->device_step ? 0.f : (float)(1.0 / std::sqrt(1.0 - std::pow(desc->beta2, at)));
         a.eps = (float)desc->eps;

@@ -393,3 +393,20 @@ def test_threads_at_once():
         t.join()
     for x, y in zip(alone, sets):
         assert all(torch.equal(p, q) for k in ("w", "m", "v", "scales") for p, q in zip(x[k], y[k]))
+
+
+def test_captures_that_would_not_count_are_refused():
+    from ksmm_amd import KSAdamW
+
+    for how, before in ((dict(), 1), (dict(capturable=True), 0)):
+        ps = params("fp16")
+        opt = KSAdamW(ps, **how)
+        for p, g in zip(ps, grads_of(ps, 0)):
+            p.grad = g.clone()
+        for _ in range(before):
+            opt.step()
+        kept = [p.detach().clone() for p in ps]
+        with pytest.raises(RuntimeError, match="captur"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                opt.step()
+        assert all(torch.equal(p, k) for p, k in zip(ps, kept))
