@@ -48,7 +48,8 @@ __device__ __forceinline__ float mx_scale_value(int scale)
 // t / d for 0 <= t, t d < 2^32 (m is less than d 2^-32 too large): a multiplication where the compiler takes 30 instructions
 struct MxDiv {
     uint32_t d, m;
-    __device__ __forceinline__ explicit MxDiv(int d) : d((uint32_t)d), m(0xffffffffu / (uint32_t)d + 1) {}
+    MxDiv() = default;
+    __host__ __device__ __forceinline__ explicit MxDiv(int d) : d((uint32_t)d), m(0xffffffffu / (uint32_t)d + 1) {}
     __device__ __forceinline__ int operator()(int t) const { return d == 1 ? t : (int)__umulhi((uint32_t)t, m); }
 };
 
@@ -137,7 +138,8 @@ template <typename T, int D> __device__ __forceinline__ int mx_quantize(const Mx
 template <typename T, int D> struct MxQuarter {
     T v[8 * D];
 };
-// count of the 8 values are there (may be none, or more); the rest is zeros
+// count of the 8 values are there (may be none, or more); the rest is zeros.  (Values that are not are read as the last that is, in this
+// quarter or one before: a branch around each load is a wait of its own)
 template <typename T, int D> __device__ __forceinline__ void mx_load(MxQuarter<T, D> &g, const T *x, int count)
 {
     constexpr int E = 16 / (int)sizeof(T);
@@ -148,8 +150,15 @@ template <typename T, int D> __device__ __forceinline__ void mx_load(MxQuarter<T
             __builtin_memcpy(&g.v[j * E], &q, 16);
         }
     } else {
+        struct __attribute__((packed, aligned(sizeof(T)))) Run {
+            T e[D];
+        } r[8];
 #pragma unroll
-        for (int j = 0; j < 8 * D; ++j) g.v[j] = j < count * D ? x[j] : (T)0;
+        for (int k = 0; k < 8; ++k) r[k] = *(const Run *)(x + (k < count ? k : count - 1) * D);
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+#pragma unroll
+            for (int j = 0; j < D; ++j) g.v[k * D + j] = k < count ? r[k].e[j] : (T)0;
     }
 }
 // its part of the codes of the four lanes' block j, and the scale's byte (in each of them; all four take part)
@@ -209,7 +218,8 @@ struct MxProduct {
     int64_t tiles, token_tiles;  // (without LDS); steps of rows
     int raw_rows, raw_pitch;     // rows at a time whose values go through LDS on their way to codes (0: straight), and values from one to the next
     int tile_rows, wave_tiles;   // rows a step, and of a workgroup's waves those that lie along the outputs
-    int row_splits, buffers;     // workgroups that share the steps
+    int row_splits;              // workgroups that share the steps
+    MxDiv by_cb, by_run_d;
 };
 // by the type of x and y, the layout and whether two projections make one output
 int mx_half_first_plain(const MxProduct &p, int act, hipStream_t s);

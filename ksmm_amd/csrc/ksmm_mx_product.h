@@ -142,7 +142,6 @@ __device__ __forceinline__ void mx_results(const MxProduct &p, const T (&v)[16 *
 // batch: a workgroup's eight waves are tiles of outputs times runs of rows.  Four more waves quantise the rows of the next step into
 // the other of two buffers in LDS and have the values of the step after that on their way: waits for what is loaded would be waits for the
 // stores before it too (one counter), which only waves that store nothing do not make.
-// Where there are few steps each workgroup takes one, of fewer waves, which first quantise and then multiply.
 constexpr int MX_CONSUMERS = 8, MX_PRODUCERS = 4;
 constexpr int mx_scale_bytes(int ks) { return ks <= 4 ? 4 : ks <= 8 ? 8 : 16; }  // of a row and one half of each step
 // blocks of 32 rows, or quarters of them, that a producer's thread takes, and of these those on their way at once: 64 registers of values
@@ -164,18 +163,17 @@ __global__ __launch_bounds__(64 * (MX_CONSUMERS + MX_PRODUCERS)) void ks_mx_held
 {
     constexpr int G = GATED ? 2 : 1, SB = mx_scale_bytes(KS), SW = (KS + 3) / 4, R = mx_rounds(KS, mx_quarters<T>(LAST, KS, D));
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
-    const int threads = blockDim.x, TN = p.tile_rows, buffer = D * TN * (p.slots * 16 + 2 * SB);
-    const bool one = p.buffers == 1;  // one step, of all waves
+    constexpr int threads = 64 * (MX_CONSUMERS + MX_PRODUCERS);
+    const int TN = p.tile_rows, buffer = D * TN * (p.slots * 16 + 2 * SB);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l32 = lane & 31, half = lane >> 5;
-    const int consumers = one ? threads >> 6 : MX_CONSUMERS;
     const int run = 16 * ((l32 >> 2) & 1) + 4 * (l32 >> 3) + (l32 & 3);  // the row that this lane reads of the operand whose rows are dealt out
     int blk = blockIdx.x;
     const int first = blk % p.row_splits;
     blk /= p.row_splits;
     const int unit = blk % p.units, ai = unit / p.runs, d0 = (unit - ai * p.runs) * D, rows_w = G * p.b;
     const int tile0 = blk / p.units * p.wave_tiles;
-    float *const bias = (float *)(smem + p.buffers * buffer);  // (tile of the workgroup, gate and up, D, 32 outputs)
-    uint8_t *const stage = smem + p.buffers * buffer + p.wave_tiles * G * D * 128 + wave * MX_STAGE;
+    float *const bias = (float *)(smem + 2 * buffer);  // (tile of the workgroup, gate and up, D, 32 outputs)
+    uint8_t *const stage = smem + 2 * buffer + p.wave_tiles * G * D * 128 + wave * MX_STAGE;
     const int tasks = TN * p.cb, batch = (int)p.batch, row_tiles = (int)p.token_tiles;  // (steps past the end are counted in 32 bits)
     const bool emit = p.codes_out && tile0 == 0;
 
@@ -229,7 +227,7 @@ __global__ __launch_bounds__(64 * (MX_CONSUMERS + MX_PRODUCERS)) void ks_mx_held
     };
     // (scales of blocks behind the last one are read: with weights of zeros, but not as NaN)
     auto prepare = [&] {
-        for (int k = 0; k < p.buffers; ++k)
+        for (int k = 0; k < 2; ++k)
             for (int i = threadIdx.x; i < D * TN * SB / 2; i += threads) ((uint32_t *)(smem + k * buffer + D * TN * p.slots * 16))[i] = 0x7f7f7f7fu;
         if (p.bias)
             for (int i = threadIdx.x; i < p.wave_tiles * G * 32 * D; i += threads) {
@@ -238,7 +236,7 @@ __global__ __launch_bounds__(64 * (MX_CONSUMERS + MX_PRODUCERS)) void ks_mx_held
             }
     };
 
-    if (!one && wave >= MX_CONSUMERS) {
+    if (wave >= MX_CONSUMERS) {
         const int t0 = threadIdx.x - 64 * MX_CONSUMERS;
         constexpr int AHEAD = mx_ahead(R, D * (int)sizeof(T) * 8 / Q);
         Load f[AHEAD];
@@ -263,13 +261,9 @@ __global__ __launch_bounds__(64 * (MX_CONSUMERS + MX_PRODUCERS)) void ks_mx_held
         return;
     }
 
-    const int wb = wave & (p.wave_tiles - 1), wt = wave / p.wave_tiles, per_wave = TN / 32 / (consumers / p.wave_tiles);
+    const int wb = wave & (p.wave_tiles - 1), wt = wave / p.wave_tiles, per_wave = TN / 32 / (MX_CONSUMERS / p.wave_tiles);
     const int bt = tile0 + wb;
     const bool busy = bt < p.b_tiles;
-    // (one step: its rows are on their way before the weights are, so that it waits for both at once)
-    Load f;
-    const int at = one ? place(threadIdx.x) : 0;
-    if (one) fetch(f, threadIdx.x, at, first * TN);
     uint4_t w[D][G][KS];
     int sw[D][G][SW], scale[D][G][KS];
     if (busy) {
@@ -290,14 +284,6 @@ __global__ __launch_bounds__(64 * (MX_CONSUMERS + MX_PRODUCERS)) void ks_mx_held
     }
     prepare();
     __syncthreads();
-    if (one) {
-        keep(f, threadIdx.x, at, first * TN, 0);
-        for (int t = threadIdx.x + threads; t < tasks * Q; t += threads) {
-            const int more = place(t);
-            fetch(f, t, more, first * TN);
-            keep(f, t, more, first * TN, 0);
-        }
-    }
 #pragma unroll
     for (int j = 0; j < D; ++j)
 #pragma unroll
@@ -355,11 +341,14 @@ __global__ __launch_bounds__(64 * (MX_CONSUMERS + MX_PRODUCERS)) void ks_mx_held
     }
 }
 
-// ---- weights from the caches: more of them than registers hold, or d_i that no thread takes together ------------------------------
+// ---- weights from the caches: few rows, more weights than registers hold, or d_i that no thread takes together --------------------
 // A workgroup quantises 32 * TT rows of a unit (one a_i; all d_i, or runs of 16 of more) into LDS; its waves take tiles of 32 outputs
 // of one d_i each, and leave their results in LDS, from where they go out a line of a row, all d_i, at a time (batch-size-last, where
-// a unit is one d_i, straight from the wave).  The codes of a step along c are on their way while the step before is multiplied.
-// D: d_i that a thread quantises together (1: all of one, or of five and more).
+// a unit is one d_i, and where a tile is all of a workgroup's, straight from the wave).  Four steps along c of codes are on their way, the
+// first ones before x is.  Of few rows a launch is bound by what follows one another, not by a rate: eight waves quantise, chunks of
+// outputs are as small as one workgroup a compute unit allows (see mx_launch_wide), and what divides is multiplied with.
+// D: all d_i of up to four, which a thread quantises together; 0: five and more; -1: x comes as codes.  (Kernels of their own: what they do not
+// run of the others' instructions costs a launch of few rows a tenth.)
 template <typename T, bool LAST, int D, int TT, bool GATED, int ACT> __global__ __launch_bounds__(64 * MX_WAVES) void ks_mx_wide_kernel(MxProduct p)
 {
     constexpr int TN = 32 * TT, G = GATED ? 2 : 1;
@@ -368,11 +357,9 @@ template <typename T, bool LAST, int D, int TT, bool GATED, int ACT> __global__ 
     const int run = 16 * ((l32 >> 2) & 1) + 4 * (l32 >> 3) + (l32 & 3);  // the row that this lane reads of the operand whose rows are dealt out
     uint8_t *const codes = smem, *const scales = codes + (size_t)p.run_d * TN * p.slots * 16;
     T *const stage = (T *)(scales + (p.run_d * TN * p.cb + 15) / 16 * 16);  // of the workgroup: rows of `pitch`; batch-size-last of the waves
-    int64_t blk = blockIdx.x;
-    const int split = (int)(blk % p.splits);
-    blk /= p.splits;
-    const int unit = (int)(blk % p.units), ai = unit / p.runs, d0 = (unit - ai * p.runs) * p.run_d;
-    const int64_t n0 = blk / p.units * TN;
+    const uint32_t rest = blockIdx.x / (uint32_t)p.splits, split = blockIdx.x - rest * (uint32_t)p.splits, tile = rest / (uint32_t)p.units;
+    const int unit = (int)(rest - tile * (uint32_t)p.units), ai = p.runs == 1 ? unit : unit / p.runs, d0 = (unit - ai * p.runs) * p.run_d;
+    const int64_t n0 = (int64_t)tile * TN;
     const int here = (int)(p.batch - n0 < TN ? p.batch - n0 : TN);                 // rows of the batch
     const int dc = LAST ? 1 : p.d - d0 < p.run_d ? p.d - d0 : p.run_d;             // d_i of the unit
     const int rows_w = G * p.b, pitch = p.chunk_tiles * 32 * p.run_d + 4 / (int)sizeof(T);  // (an odd number of words: rows meet other banks)
@@ -388,8 +375,40 @@ template <typename T, bool LAST, int D, int TT, bool GATED, int ACT> __global__ 
         }
     };
     const bool emit = p.codes_out && split == 0;
-    const MxDiv by_cb(p.cb), by_dc(dc);
-    if (p.x_scales) {  // as codes: they are copied
+    const MxDiv by_cb = p.by_cb, by_dc = dc == p.run_d ? p.by_run_d : MxDiv(dc);
+    const int chunk_first = (int)split * p.tiles_per, chunk_end = chunk_first + p.tiles_per < p.b_tiles ? chunk_first + p.tiles_per : p.b_tiles;
+    // ---- a wave's work: a tile of outputs of one d_i, and the codes of its next AHEAD steps along c
+    constexpr int AHEAD = 4;
+    struct {
+        int j, bt;
+        int64_t at[G];
+        uint4_t w[AHEAD][G];
+        int s[AHEAD][G];
+    } job;
+    auto load = [&](int kb, int r) {
+        const bool there = kb < p.cb;
+#pragma unroll
+        for (int q = 0; q < G; ++q) {
+            job.w[r][q] = there ? *(const uint4_t *)(p.w + (job.at[q] + kb) * 16) : uint4_t{0, 0, 0, 0};
+            job.s[r][q] = there ? p.w_scales[job.at[q] + kb] : 127;
+        }
+    };
+    auto begin = [&](int chunk, int i) {
+        const int tile = by_dc(i);
+        job.j = i - tile * dc;
+        job.bt = chunk + tile;
+        // (outputs behind the last one are read as the last one and not stored)
+        const int wo = job.bt * 32 + (LAST ? l32 : run), o = wo < p.b ? wo : p.b - 1;
+#pragma unroll
+        for (int q = 0; q < G; ++q) job.at[q] = (((int64_t)ai * p.d + d0 + job.j) * rows_w + q * p.b + o) * p.cb;
+#pragma unroll
+        for (int r = 0; r < AHEAD; ++r)
+            if (2 * r < p.cb) load(2 * r + half, r);
+    };
+    auto jobs_of = [&](int chunk) { return (chunk_end - chunk < p.chunk_tiles ? chunk_end - chunk : p.chunk_tiles) * dc; };
+    // (the first ones are on their way before x is)
+    if (wave < jobs_of(chunk_first)) begin(chunk_first, wave);
+    if constexpr (D < 0) {  // they are copied
         for (int t = threadIdx.x; t < TN * p.cb * dc; t += 64 * MX_WAVES) {
             const int u = by_cb(t), kb = t - u * p.cb, j = u / TN, n = u - j * TN;
             if (n >= here) continue;
@@ -406,27 +425,38 @@ template <typename T, bool LAST, int D, int TT, bool GATED, int ACT> __global__ 
             const int scale = mx_quantize<T, 1>(g, 0, p.c - kb * 32, code);
             keep(0, n, kb, code, scale, emit);
         }
-    } else if (p.d == D) {
-        for (int t = threadIdx.x; t < TN * p.cb * 4; t += 64 * MX_WAVES) {
-            const int u = t / 4, quarter = t & 3, n = by_cb(u), kb = u - n * p.cb;
-            if (n >= here) continue;
-            MxQuarter<T, D> g;
-            mx_load<T, D>(g, (const T *)p.x + (((n0 + n) * p.a + ai) * p.c + kb * 32 + quarter * 8) * D, p.c - kb * 32 - quarter * 8);
+    } else if constexpr (D > 0) {
+        constexpr int SIZE = 2 * D * (int)sizeof(T), TIMES = 64 / SIZE < 4 ? 64 / SIZE : 4;  // (64 registers of values on their way)
+        const int total = here * p.cb * 4, quarter = threadIdx.x & 3;
+        for (int t0 = threadIdx.x; t0 < total; t0 += 64 * MX_WAVES * TIMES) {
+            MxQuarter<T, D> g[TIMES];
+            int n[TIMES], kb[TIMES];
 #pragma unroll
-            for (int j = 0; j < D; ++j) {
-                uint32_t code;
-                const int row = j * TN + n, scale = mx_quantize<T, D>(g, j, code);
-                const int64_t block = (((int64_t)ai * p.d + d0 + j) * p.batch + n0 + n) * p.cb + kb;
-                ((uint32_t *)(codes + ((size_t)row * p.slots + kb) * 16))[quarter] = code;
-                if (emit) ((uint32_t *)(p.codes_out + block * 16))[quarter] = code;
-                if (quarter == 0) {
-                    scales[row * p.cb + kb] = (uint8_t)scale;
-                    if (emit) p.scales_out[block] = (uint8_t)scale;
+            for (int r = 0; r < TIMES; ++r) {
+                const int t = t0 + r * 64 * MX_WAVES, u = t / 4;
+                n[r] = by_cb(u);
+                kb[r] = u - n[r] * p.cb;
+                if (t < total) mx_load<T, D>(g[r], (const T *)p.x + (((n0 + n[r]) * p.a + ai) * p.c + kb[r] * 32 + quarter * 8) * D, p.c - kb[r] * 32 - quarter * 8);
+            }
+#pragma unroll
+            for (int r = 0; r < TIMES; ++r) {
+                if (t0 + r * 64 * MX_WAVES >= total) break;
+#pragma unroll
+                for (int j = 0; j < D; ++j) {
+                    uint32_t code;
+                    const int row = j * TN + n[r], scale = mx_quantize<T, D>(g[r], j, code);
+                    const int64_t block = (((int64_t)ai * p.d + d0 + j) * p.batch + n0 + n[r]) * p.cb + kb[r];
+                    ((uint32_t *)(codes + ((size_t)row * p.slots + kb[r]) * 16))[quarter] = code;
+                    if (emit) ((uint32_t *)(p.codes_out + block * 16))[quarter] = code;
+                    if (quarter == 0) {
+                        scales[row * p.cb + kb[r]] = (uint8_t)scale;
+                        if (emit) p.scales_out[block] = (uint8_t)scale;
+                    }
                 }
             }
         }
-    } else if constexpr (D == 1) {
-        // five d_i and more: as they lie into LDS, where a thread gathers a block
+    } else {
+        // as they lie into LDS, where a thread gathers a block
         constexpr int E = 16 / (int)sizeof(T), AHEAD = 4;
         const bool whole = dc == p.d;
         const int length = whole ? p.c * dc : dc, vectors = (length + E - 1) / E, lines = whole ? 1 : p.c;  // runs of a row
@@ -482,31 +512,13 @@ template <typename T, bool LAST, int D, int TT, bool GATED, int ACT> __global__ 
     }
     __syncthreads();
     // ---- products, a chunk of tiles of outputs at a time
+    const bool alone = !LAST && (D == 1 || D == -1) && p.d == 1 && p.chunk_tiles == 1;  // (one wave's lines are all there is)
     const T *const bias = (const T *)p.bias;
-    const int chunk_end = (split + 1) * p.tiles_per < p.b_tiles ? (split + 1) * p.tiles_per : p.b_tiles;
-    for (int chunk = split * p.tiles_per; chunk < chunk_end; chunk += p.chunk_tiles) {
-        const int jobs = (chunk_end - chunk < p.chunk_tiles ? chunk_end - chunk : p.chunk_tiles) * dc;
-        for (int job = wave; job < jobs; job += MX_WAVES) {
-            const int job_tile = by_dc(job), j = job - job_tile * dc, bt = chunk + job_tile;
-            // (outputs behind the last one are read as the last one and not stored)
-            const int wo = bt * 32 + (LAST ? l32 : run), o = wo < p.b ? wo : p.b - 1;
-            int64_t at[G];
-#pragma unroll
-            for (int q = 0; q < G; ++q) at[q] = (((int64_t)ai * p.d + d0 + j) * rows_w + q * p.b + o) * p.cb;
-            struct Step {
-                uint4_t w[G];
-                int s[G];
-            };
-            auto load = [&](int kb, Step &k) {
-                const bool there = kb < p.cb;
-#pragma unroll
-                for (int q = 0; q < G; ++q) {
-                    k.w[q] = there ? *(const uint4_t *)(p.w + (at[q] + kb) * 16) : uint4_t{0, 0, 0, 0};
-                    k.s[q] = there ? p.w_scales[at[q] + kb] : 127;
-                }
-            };
-            Step now;
-            load(half, now);
+    for (int chunk = chunk_first; chunk < chunk_end; chunk += p.chunk_tiles) {
+        const int jobs = jobs_of(chunk);
+        for (int i = wave; i < jobs; i += MX_WAVES) {
+            if (chunk > chunk_first || i > wave) begin(chunk, i);
+            const int j = job.j, bt = job.bt;
             float16_t acc[TT][G];
 #pragma unroll
             for (int q = 0; q < G; ++q) {
@@ -521,27 +533,42 @@ template <typename T, bool LAST, int D, int TT, bool GATED, int ACT> __global__ 
 #pragma unroll
                 for (int t = 0; t < TT; ++t) acc[t][q] = add;
             }
-            for (int k0 = 0; k0 < p.cb; k0 += 2) {
-                const int kb = k0 + half;
-                Step next = now;
-                if (k0 + 2 < p.cb) load(kb + 2, next);
+            constexpr int XS = TT == 1 ? AHEAD : 1;  // steps whose codes of x are read at once
+            for (int k0 = 0; k0 < p.cb; k0 += 2 * AHEAD) {
 #pragma unroll
-                for (int t = 0; t < TT; ++t) {
-                    const int row = j * TN + t * 32 + (LAST ? run : l32);
-                    const bool there = kb < p.cb;
-                    const uint4_t x = there ? *(const uint4_t *)(codes + ((size_t)row * p.slots + kb) * 16) : uint4_t{0, 0, 0, 0};
-                    const int sx = there ? scales[row * p.cb + kb] : 127;
+                for (int r0 = 0; r0 < AHEAD; r0 += XS) {
+                    uint4_t x[XS][TT];
+                    int sx[XS][TT];
 #pragma unroll
-                    for (int q = 0; q < G; ++q) acc[t][q] = LAST ? mx_mfma(x, sx, now.w[q], now.s[q], acc[t][q]) : mx_mfma(now.w[q], now.s[q], x, sx, acc[t][q]);
+                    for (int r = 0; r < XS; ++r) {
+                        const int kb = k0 + 2 * (r0 + r) + half, at = kb < p.cb ? kb : p.cb - 1;  // (behind the last block: with weights of zeros, but not as NaN)
+#pragma unroll
+                        for (int t = 0; t < TT; ++t) {
+                            const int row = j * TN + t * 32 + (LAST ? run : l32);
+                            x[r][t] = *(const uint4_t *)(codes + ((size_t)row * p.slots + at) * 16);
+                            sx[r][t] = kb < p.cb ? scales[row * p.cb + at] : 127;
+                        }
+                    }
+#pragma unroll
+                    for (int r = 0; r < XS; ++r) {
+                        const int k = k0 + 2 * (r0 + r);
+                        if (k >= p.cb) break;
+                        const auto &w = job.w[r0 + r];
+                        const auto &sw = job.s[r0 + r];
+#pragma unroll
+                        for (int t = 0; t < TT; ++t)
+#pragma unroll
+                            for (int q = 0; q < G; ++q) acc[t][q] = LAST ? mx_mfma(x[r][t], sx[r][t], w[q], sw[q], acc[t][q]) : mx_mfma(w[q], sw[q], x[r][t], sx[r][t], acc[t][q]);
+                        if (k + 2 * AHEAD < p.cb) load(k + 2 * AHEAD + half, r0 + r);
+                    }
                 }
-                now = next;
             }
 #pragma unroll
             for (int t = 0; t < TT; ++t) {
                 T v[16];
                 mx_activate<T, 1, GATED, ACT>(acc[t], 0, v);
-                if constexpr (LAST) {
-                    if (t * 32 < here) mx_results<T, true, 1>(p, v, ai, d0, bt, lane, n0, t, here, (uint8_t *)stage + wave * MX_STAGE);
+                if (LAST || alone) {
+                    if (t * 32 < here) mx_results<T, LAST, 1>(p, v, ai, d0, bt, lane, n0, t, here, (uint8_t *)stage + wave * MX_STAGE);
                 } else {
                     T *const to = stage + (t * 32 + l32) * pitch + ((bt - chunk) * 32 + 16 * half) * dc + j;
 #pragma unroll
@@ -549,7 +576,7 @@ template <typename T, bool LAST, int D, int TT, bool GATED, int ACT> __global__ 
                 }
             }
         }
-        if constexpr (!LAST) {
+        if (!LAST && !alone) {
             __syncthreads();
             // pieces of a line that lie together: all of it, or with more d_i than the unit's, those of an output
             constexpr int E = 16 / (int)sizeof(T);
@@ -579,9 +606,9 @@ template <typename T, bool LAST, int D, int TT, bool GATED, int ACT> __global__ 
     }
 }
 
-inline int64_t mx_held_lds(int d, bool gated, int ks, int cb, int rows, int tiles, int buffers, int waves)
+inline int64_t mx_held_lds(int d, bool gated, int ks, int cb, int rows, int tiles)
 {
-    return (int64_t)buffers * d * rows * ((cb | 1) * 16 + 2 * mx_scale_bytes(ks)) + (int64_t)tiles * (gated ? 2 : 1) * 32 * d * 4 + waves * MX_STAGE;
+    return 2LL * d * rows * ((cb | 1) * 16 + 2 * mx_scale_bytes(ks)) + (int64_t)tiles * (gated ? 2 : 1) * 32 * d * 4 + MX_CONSUMERS * MX_STAGE;
 }
 
 template <typename T, bool LAST, int D, int TT, bool GATED> int mx_launch_wide(MxProduct p, int act, hipStream_t s)
@@ -593,8 +620,10 @@ template <typename T, bool LAST, int D, int TT, bool GATED> int mx_launch_wide(M
     p.b_tiles = (p.b + 31) / 32;
     p.chunk_tiles = mx_chunk_of(p.run_d, LAST);
     p.token_tiles = (p.batch + 32 * TT - 1) / (32 * TT);
-    // outputs are split over workgroups, each of which quantises its rows anew, until there are 1024
+    // outputs are split over workgroups, each of which quantises its rows anew, until there are 1024; and where there is less than one for a
+    // compute unit, into smaller chunks, so that more of them load the weights
     const int64_t groups = p.token_tiles * p.units;
+    while (p.chunk_tiles > 1 && groups * ((p.b_tiles + p.chunk_tiles / 2 - 1) / (p.chunk_tiles / 2)) <= 256) p.chunk_tiles /= 2;
     const int most = (p.b_tiles + p.chunk_tiles - 1) / p.chunk_tiles;
     const int64_t want = groups >= 1024 ? 1 : (1024 + groups - 1) / groups;
     p.splits = (int)(want < most ? want : most);
@@ -603,6 +632,8 @@ template <typename T, bool LAST, int D, int TT, bool GATED> int mx_launch_wide(M
     const int64_t grid = groups * p.splits;
     if (grid > 0x7fffffffLL) return KSMM_ERR_TOO_LARGE;
     const int lds = (int)mx_wide_lds(TT, p.c, p.d, (int)sizeof(T), LAST);
+    p.by_cb = MxDiv(p.cb);
+    p.by_run_d = MxDiv(p.run_d);
     p.raw_pitch = (int)(mx_raw_row(p.c, p.d, (int)sizeof(T)) / (int)sizeof(T));
     p.raw_rows = mx_raw_rows(TT, p.c, p.d, (int)sizeof(T));
     int rc = KSMM_OK;
@@ -634,7 +665,7 @@ template <typename T, bool LAST, int D, bool GATED, int KS> int mx_launch_held(M
     p.units = p.a * p.runs;
     p.b_tiles = (p.b + 31) / 32;
     // eight waves: the more of them share their rows the less often these are quantised, but none should idle
-    int waves = MX_CONSUMERS + MX_PRODUCERS, idle = 1 << 30;
+    int idle = 1 << 30;
     for (int tiles = MX_CONSUMERS; tiles >= 1; tiles /= 2) {
         const int over = (p.b_tiles + tiles - 1) / tiles * tiles - p.b_tiles;
         if (over < idle && 32 * MX_CONSUMERS / tiles * p.cb <= MOST) {
@@ -652,7 +683,7 @@ template <typename T, bool LAST, int D, bool GATED, int KS> int mx_launch_held(M
         return most >= 8 ? most / 8 * 8 : most;
     };
     int64_t most = most_of(1);
-    if (p.token_tiles > most && mx_held_lds(D, GATED, KS, p.cb, p.tile_rows, p.wave_tiles, 2, MX_CONSUMERS) <= 80 * 1024) {
+    if (p.token_tiles > most && mx_held_lds(D, GATED, KS, p.cb, p.tile_rows, p.wave_tiles) <= 80 * 1024) {
         with_act(act, [&](auto which) {
             constexpr int ACT = decltype(which)::value;
             if constexpr (GATED || ACT != KSMM_ACT_SILU) {
@@ -662,20 +693,9 @@ template <typename T, bool LAST, int D, bool GATED, int KS> int mx_launch_held(M
         });
     }
     p.row_splits = (int)std::min(p.token_tiles, most);
-    p.buffers = 2;
-    if (groups() * p.token_tiles < 512) {  // few: smaller workgroups of one step each
-        for (waves = 4; waves >= 1; waves /= 2) {
-            p.wave_tiles = waves;
-            p.tile_rows = 32;
-            p.token_tiles = (p.batch + 31) / 32;
-            if (waves == 1 || groups() * p.token_tiles >= 256) break;
-        }
-        p.row_splits = (int)p.token_tiles;
-        p.buffers = 1;
-    }
     const int64_t grid = groups() * p.row_splits;
     if (grid > 0x7fffffffLL) return KSMM_ERR_TOO_LARGE;
-    const int lds = (int)mx_held_lds(D, GATED, KS, p.cb, p.tile_rows, p.wave_tiles, p.buffers, p.buffers == 1 ? waves : MX_CONSUMERS);
+    const int lds = (int)mx_held_lds(D, GATED, KS, p.cb, p.tile_rows, p.wave_tiles);
     int rc = KSMM_OK;
     with_act(act, [&](auto which) {
         constexpr int ACT = decltype(which)::value;
@@ -683,7 +703,7 @@ template <typename T, bool LAST, int D, bool GATED, int KS> int mx_launch_held(M
             auto fn = &ks_mx_held_kernel<T, LAST, D, GATED, ACT, KS>;
             if (lds > 64 * 1024) rc = ensure_dynamic_lds((const void *)fn, lds);
             if (rc != KSMM_OK) return;
-            hipLaunchKernelGGL(fn, dim3((unsigned)grid), dim3(64 * waves), lds, s, p);
+            hipLaunchKernelGGL(fn, dim3((unsigned)grid), dim3(64 * (MX_CONSUMERS + MX_PRODUCERS)), lds, s, p);
             if (hipGetLastError() != hipSuccess) rc = KSMM_ERR_LAUNCH;
         }
     });
@@ -705,25 +725,34 @@ template <typename T, bool LAST, int D, bool GATED, int KS, int... MORE> int mx_
 
 template <typename T, bool LAST, int D, bool GATED> int mx_pick(const MxProduct &p, int act, hipStream_t s)
 {
-    if (!p.x_scales && (LAST || p.d == D)) {
-        const int rc = mx_held<T, LAST, D, GATED, 1, 2, 3, 4, 6, 8, 16>(p, act, s);
-        if (rc != KSMM_ERR_BAD_ALGO) return rc;
+    const int unit = mx_unit_of(p.d, LAST), chunk = mx_chunk_of(unit, LAST);
+    auto groups = [&](int rows) { return (p.batch + rows - 1) / rows * p.a * ((p.d + unit - 1) / unit) * ((p.b + 32 * chunk - 1) / (32 * chunk)); };
+    if constexpr (D > 0) {
+        // fewer than these are done sooner by workgroups of one step, which all begin at once: (1,768,192,2) gated fp16 of 32 rows in 4.9 us
+        // for 7.2, of 1000 in 6.6 for 7.8; with 252 of them 4000 rows of (2,96,72,3) in fp32 take 9.4 for 8.2
+        if (groups(32) > 192) {
+            const int rc = mx_held<T, LAST, D, GATED, 1, 2, 3, 4, 6, 8, 16>(p, act, s);
+            if (rc != KSMM_ERR_BAD_ALGO) return rc;
+        }
     }
     // twice the rows for the same weights, where that leaves two workgroups for a compute unit
-    const int unit = mx_unit_of(p.d, LAST), chunk = mx_chunk_of(unit, LAST);
-    const int64_t groups = (p.batch + 63) / 64 * p.a * ((p.d + unit - 1) / unit) * ((p.b + 32 * chunk - 1) / (32 * chunk));
-    if (groups >= 512 && mx_wide_lds(2, p.c, p.d, (int)sizeof(T), LAST) <= MX_LDS_MOST) return mx_launch_wide<T, LAST, D, 2, GATED>(p, act, s);
+    if (groups(64) >= 512 && mx_wide_lds(2, p.c, p.d, (int)sizeof(T), LAST) <= MX_LDS_MOST) return mx_launch_wide<T, LAST, D, 2, GATED>(p, act, s);
     return mx_launch_wide<T, LAST, D, 1, GATED>(p, act, s);
 }
 
-template <typename T, bool GATED> int mx_last(const MxProduct &p, int act, hipStream_t s) { return mx_pick<T, true, 1, GATED>(p, act, s); }
+template <typename T, bool GATED> int mx_last(const MxProduct &p, int act, hipStream_t s)
+{
+    return p.x_scales ? mx_pick<T, true, -1, GATED>(p, act, s) : mx_pick<T, true, 1, GATED>(p, act, s);
+}
 template <typename T, bool GATED> int mx_first(const MxProduct &p, int act, hipStream_t s)
 {
-    switch (p.d) {
+    switch (p.x_scales ? -1 : p.d) {
+    case -1: return mx_pick<T, false, -1, GATED>(p, act, s);
+    case 1: return mx_pick<T, false, 1, GATED>(p, act, s);
     case 2: return mx_pick<T, false, 2, GATED>(p, act, s);
     case 3: return mx_pick<T, false, 3, GATED>(p, act, s);
     case 4: return mx_pick<T, false, 4, GATED>(p, act, s);
-    default: return mx_pick<T, false, 1, GATED>(p, act, s);
+    default: return mx_pick<T, false, 0, GATED>(p, act, s);
     }
 }
 
