@@ -153,6 +153,7 @@ template <typename T, int D> __device__ __forceinline__ void mx_load(MxQuarter<T
         struct __attribute__((packed, aligned(sizeof(T)))) Run {
             T e[D];
         } r[8];
+        asm volatile("" : "+v"(count));  // (as above)
 #pragma unroll
         for (int k = 0; k < 8; ++k) r[k] = *(const Run *)(x + (k < count ? k : count - 1) * D);
 #pragma unroll
@@ -209,6 +210,7 @@ struct MxProduct {
     const uint8_t *w, *w_scales;
     const void *bias;
     void *y;
+    const void *dy;  // (gradients only)
     int64_t batch;
     int a, b, c, d, cb;
     int slots;                    // of 16 bytes in LDS for a row's codes, odd
@@ -221,6 +223,8 @@ struct MxProduct {
     int row_splits;              // workgroups that share the steps
     MxDiv by_cb, by_run_d;
 };
+int mx_slope_half(const MxProduct &p, bool last, bool gated, int act, hipStream_t s);
+int mx_slope_float(const MxProduct &p, bool last, bool gated, int act, hipStream_t s);
 // by the type of x and y, the layout and whether two projections make one output
 int mx_half_first_plain(const MxProduct &p, int act, hipStream_t s);
 int mx_half_first_gated(const MxProduct &p, int act, hipStream_t s);

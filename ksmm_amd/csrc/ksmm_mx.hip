@@ -383,7 +383,7 @@ int ksmm_mx_forward(const void *x, const void *x_scales, const void *w, const vo
                        {bias, (int64_t)a * rows_w * d * size}};
     const Span out[] = {{y, values(batch, a, b, d) * size}, {codes_out, blocks * 16}, {scales_out, blocks}, {need ? workspace : nullptr, need}};
     if (any_overlap(in, out)) return KSMM_ERR_ALIAS;
-    MxProduct p{x, (const uint8_t *)x_scales, (uint8_t *)codes_out, (uint8_t *)scales_out, (const uint8_t *)w, (const uint8_t *)w_scales, bias, y, batch, a, b, c, d, cb};
+    MxProduct p{x, (const uint8_t *)x_scales, (uint8_t *)codes_out, (uint8_t *)scales_out, (const uint8_t *)w, (const uint8_t *)w_scales, bias, y, nullptr, batch, a, b, c, d, cb};
     static int (*const fused[2][2][2])(const MxProduct &, int, hipStream_t) = {
         {{mx_half_first_plain, mx_half_first_gated}, {mx_half_last_plain, mx_half_last_gated}},
         {{mx_float_first_plain, mx_float_first_gated}, {mx_float_last_plain, mx_float_last_gated}}};
@@ -402,6 +402,26 @@ int ksmm_mx_forward(const void *x, const void *x_scales, const void *w, const vo
     p.tiles = (int64_t)a * d * p.b_tiles * p.token_tiles;
     return dtype == KSMM_F32 ? product<float>(p, bs_last != 0, gated != 0, act, (hipStream_t)stream)
                              : product<half_t>(p, bs_last != 0, gated != 0, act, (hipStream_t)stream);
+}
+
+int ksmm_mx_slope(const void *x, const void *x_scales, const void *w, const void *w_scales, const void *bias, const void *dy, void *dz, int64_t batch,
+                  int a, int b, int c, int d, int dtype, int bs_last, int act, int gated, void *stream)
+{
+    const int rc = check_product(batch, a, b, c, d, dtype, act, gated);
+    if (rc != KSMM_OK) return rc;
+    if (!gated && act == KSMM_ACT_NONE) return KSMM_ERR_BAD_EPILOGUE;
+    const int rows_w = gated ? 2 * b : b, cb = (int)mx_blocks(c);
+    MxProduct p{x, (const uint8_t *)x_scales, nullptr, nullptr, (const uint8_t *)w, (const uint8_t *)w_scales, bias, dz, dy, batch, a, b, c, d, cb};
+    if (dz) {
+        if (!x || !x_scales || !w || !w_scales || !dy) return KSMM_ERR_NULL_POINTER;
+        const int64_t blocks = (int64_t)a * d * batch * cb, w_blocks = (int64_t)a * d * rows_w * cb, size = (int64_t)dtype_size(dtype);
+        if (((uintptr_t)w & 15) != 0 || ((uintptr_t)x & 15) != 0) return KSMM_ERR_WORKSPACE;
+        const Span in[] = {{x, blocks * 16}, {x_scales, blocks}, {w, w_blocks * 16}, {w_scales, w_blocks}, {bias, (int64_t)a * rows_w * d * size},
+                           {dy, values(batch, a, b, d) * size}};
+        const Span out[] = {{dz, values(batch, a, rows_w, d) * size}};
+        if (any_overlap(in, out)) return KSMM_ERR_ALIAS;
+    }
+    return (dtype == KSMM_F32 ? mx_slope_float : mx_slope_half)(p, bs_last != 0, gated != 0, act, (hipStream_t)stream);
 }
 
 }  // extern "C"

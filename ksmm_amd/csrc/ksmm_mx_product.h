@@ -97,28 +97,29 @@ template <typename T, int N> __device__ __forceinline__ void mx_store_lines(uint
     }
 }
 
-// stores of a lane's results: tile t of 32 rows of those from n0 on, tile bt of outputs
+// stores of a lane's results: tile t of 32 rows of those from n0 on, tile bt of the p.b outputs that begin at `from` of an a_i's `rows`
 template <typename T, bool LAST, int D>
-__device__ __forceinline__ void mx_results(const MxProduct &p, const T (&v)[16 * D], int ai, int d0, int bt, int lane, int64_t n0, int t, int here, uint8_t *stage)
+__device__ __forceinline__ void mx_results(const MxProduct &p, const T (&v)[16 * D], int ai, int d0, int bt, int lane, int64_t n0, int t, int here, uint8_t *stage,
+                                           int rows, int from = 0)
 {
     const int l32 = lane & 31, half = lane >> 5;
     if ((t + 1) * 32 <= here && (bt + 1) * 32 <= p.b) {
-        const int64_t pitch = LAST ? (int64_t)p.d * p.batch : (int64_t)p.a * p.b * p.d;
-        T *const y = (T *)p.y + (LAST ? (((int64_t)ai * p.b + bt * 32) * p.d + d0) * p.batch + n0 + t * 32
-                                      : (((n0 + t * 32) * p.a + ai) * p.b + bt * 32) * p.d + d0);
+        const int64_t pitch = LAST ? (int64_t)p.d * p.batch : (int64_t)p.a * rows * p.d;
+        T *const y = (T *)p.y + (LAST ? (((int64_t)ai * rows + from + bt * 32) * p.d + d0) * p.batch + n0 + t * 32
+                                      : (((n0 + t * 32) * p.a + ai) * rows + from + bt * 32) * p.d + d0);
         mx_store_lines<T, 16 * D>(stage, y, pitch, v, lane);
         return;
     }
     if constexpr (LAST) {
         const int o = bt * 32 + l32, n = t * 32 + 16 * half;
-        T *const y = (T *)p.y + (((int64_t)ai * p.b + o) * p.d + d0) * p.batch + n0 + n;
+        T *const y = (T *)p.y + (((int64_t)ai * rows + from + o) * p.d + d0) * p.batch + n0 + n;
         if (o >= p.b) return;
 #pragma unroll
         for (int i = 0; i < 16; ++i)
             if (n + i < here) y[i] = v[i];
     } else {
         const int o = bt * 32 + 16 * half, n = t * 32 + l32;
-        T *const y = (T *)p.y + (((n0 + n) * p.a + ai) * p.b + o) * p.d + d0;
+        T *const y = (T *)p.y + (((n0 + n) * p.a + ai) * rows + from + o) * p.d + d0;
         struct __attribute__((packed, aligned(sizeof(T)))) Run {
             T e[D];
         };
@@ -158,21 +159,97 @@ constexpr int mx_ahead(int rounds, int registers)
     return n;
 }
 
+// the weights of a wave's 32 outputs, those of tile bt
+template <bool LAST, int D, int G, int KS> struct MxHeld {
+    static constexpr int SB = mx_scale_bytes(KS), SW = (KS + 3) / 4;
+    uint4_t w[D][G][KS];
+    int sw[D][G][SW], scale[D][G][KS];
+    __device__ __forceinline__ void load(const MxProduct &p, int ai, int d0, int bt, int l32, int run, int half)
+    {
+        const int wo = bt * 32 + (LAST ? l32 : run), o = wo < p.b ? wo : p.b - 1;  // (outputs behind the last one are read as the last one)
+#pragma unroll
+        for (int j = 0; j < D; ++j)
+#pragma unroll
+            for (int q = 0; q < G; ++q) {
+                const int64_t at = (((int64_t)ai * p.d + d0 + j) * (G * p.b) + q * p.b + o) * p.cb;
+#pragma unroll
+                for (int s = 0; s < KS; ++s) {
+                    const int kb = 2 * s + half;
+                    const bool there = kb < p.cb;
+                    w[j][q][s] = there ? *(const uint4_t *)(p.w + (at + kb) * 16) : uint4_t{0, 0, 0, 0};
+                    scale[j][q][s] = there ? p.w_scales[at + kb] : 127;
+                }
+            }
+    }
+    // (said to the compiler: the weights are there, and no step waits for them again, which would be for all stores before it too)
+    __device__ __forceinline__ void arrived()
+    {
+#pragma unroll
+        for (int j = 0; j < D; ++j)
+#pragma unroll
+            for (int q = 0; q < G; ++q) {
+#pragma unroll
+                for (int s = 0; s < KS; ++s) sw[j][q][s / 4] = s % 4 ? sw[j][q][s / 4] | scale[j][q][s] << 8 * (s % 4) : scale[j][q][s];
+#pragma unroll
+                for (int s = 0; s < KS; ++s) asm volatile("" : "+v"(w[j][q][s]));
+#pragma unroll
+                for (int s = 0; s < SW; ++s) asm volatile("" : "+v"(sw[j][q][s]));
+            }
+    }
+    // sums of row `row` of x in LDS with d_i j's weights; bias: of the wave's tile, or null
+    __device__ __forceinline__ void sums(const uint8_t *codes, const uint8_t *scales, int slots, int row, int j, int l32, int half, const float *bias, float16_t (&acc)[G]) const
+    {
+        int sx[SW];
+#pragma unroll
+        for (int i = 0; i < SW; ++i) sx[i] = ((const int *)(scales + row * 2 * SB + half * SB))[i];
+        auto steps = [&](auto biased) {
+#pragma unroll
+            for (int q = 0; q < G; ++q) {
+                acc[q] = float16_t{};
+                if constexpr (decltype(biased)::value)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) acc[q][i] = bias[(q * D + j) * 32 + (LAST ? l32 : 16 * half + i)];
+            }
+#pragma unroll
+            for (int s = 0; s < KS; ++s) {
+                const uint4_t x = *(const uint4_t *)(codes + (row * slots + 2 * s + half) * 16);
+#pragma unroll
+                for (int q = 0; q < G; ++q) acc[q] = mx_step<LAST>(w[j][q][s], sw[j][q][s / 4], x, sx[s / 4], s % 4, acc[q]);
+            }
+        };
+        if (bias)
+            steps(std::true_type());
+        else
+            steps(std::false_type());
+    }
+};
+// scales of blocks behind the last one, of `words` words each `apart` bytes from the other buffer's: they are read, with weights of zeros, but
+// not as NaN; and the biases of `tiles` tiles from tile0 on, (tile, gate and up, D, 32 outputs)
+template <typename T, int D, int G> __device__ __forceinline__ void mx_prepare(const MxProduct &p, uint8_t *scales, int apart, int words, float *bias, int ai, int d0, int tile0)
+{
+    for (int k = 0; k < 2; ++k)
+        for (int i = threadIdx.x; i < words; i += blockDim.x) ((uint32_t *)(scales + k * apart))[i] = 0x7f7f7f7fu;
+    if (p.bias)
+        for (int i = threadIdx.x; i < p.wave_tiles * G * 32 * D; i += blockDim.x) {
+            const int j = i / 32 % D, q = i / 32 / D % G, out = (tile0 + i / 32 / D / G) * 32 + i % 32;
+            bias[i] = out < p.b ? (float)((const T *)p.bias)[((int64_t)ai * (G * p.b) + q * p.b + out) * p.d + d0 + j] : 0.f;
+        }
+}
+
 template <typename T, bool LAST, int D, bool GATED, int ACT, int KS>
 __global__ __launch_bounds__(64 * (MX_CONSUMERS + MX_PRODUCERS)) void ks_mx_held_kernel(MxProduct p)
 {
-    constexpr int G = GATED ? 2 : 1, SB = mx_scale_bytes(KS), SW = (KS + 3) / 4, R = mx_rounds(KS, mx_quarters<T>(LAST, KS, D));
+    constexpr int G = GATED ? 2 : 1, SB = mx_scale_bytes(KS), R = mx_rounds(KS, mx_quarters<T>(LAST, KS, D));
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
-    constexpr int threads = 64 * (MX_CONSUMERS + MX_PRODUCERS);
     const int TN = p.tile_rows, buffer = D * TN * (p.slots * 16 + 2 * SB);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l32 = lane & 31, half = lane >> 5;
     const int run = 16 * ((l32 >> 2) & 1) + 4 * (l32 >> 3) + (l32 & 3);  // the row that this lane reads of the operand whose rows are dealt out
     int blk = blockIdx.x;
     const int first = blk % p.row_splits;
     blk /= p.row_splits;
-    const int unit = blk % p.units, ai = unit / p.runs, d0 = (unit - ai * p.runs) * D, rows_w = G * p.b;
+    const int unit = blk % p.units, ai = unit / p.runs, d0 = (unit - ai * p.runs) * D;
     const int tile0 = blk / p.units * p.wave_tiles;
-    float *const bias = (float *)(smem + 2 * buffer);  // (tile of the workgroup, gate and up, D, 32 outputs)
+    float *const bias = (float *)(smem + 2 * buffer);
     uint8_t *const stage = smem + 2 * buffer + p.wave_tiles * G * D * 128 + wave * MX_STAGE;
     const int tasks = TN * p.cb, batch = (int)p.batch, row_tiles = (int)p.token_tiles;  // (steps past the end are counted in 32 bits)
     const bool emit = p.codes_out && tile0 == 0;
@@ -225,16 +302,7 @@ __global__ __launch_bounds__(64 * (MX_CONSUMERS + MX_PRODUCERS)) void ks_mx_held
             }
         }
     };
-    // (scales of blocks behind the last one are read: with weights of zeros, but not as NaN)
-    auto prepare = [&] {
-        for (int k = 0; k < 2; ++k)
-            for (int i = threadIdx.x; i < D * TN * SB / 2; i += threads) ((uint32_t *)(smem + k * buffer + D * TN * p.slots * 16))[i] = 0x7f7f7f7fu;
-        if (p.bias)
-            for (int i = threadIdx.x; i < p.wave_tiles * G * 32 * D; i += threads) {
-                const int j = i / 32 % D, q = i / 32 / D % G, out = (tile0 + i / 32 / D / G) * 32 + i % 32;
-                bias[i] = out < p.b ? (float)((const T *)p.bias)[((int64_t)ai * rows_w + q * p.b + out) * p.d + d0 + j] : 0.f;
-            }
-    };
+    auto prepare = [&] { mx_prepare<T, D, G>(p, smem + D * TN * p.slots * 16, buffer, D * TN * SB / 2, bias, ai, d0, tile0); };
 
     if (wave >= MX_CONSUMERS) {
         const int t0 = threadIdx.x - 64 * MX_CONSUMERS;
@@ -264,42 +332,11 @@ __global__ __launch_bounds__(64 * (MX_CONSUMERS + MX_PRODUCERS)) void ks_mx_held
     const int wb = wave & (p.wave_tiles - 1), wt = wave / p.wave_tiles, per_wave = TN / 32 / (MX_CONSUMERS / p.wave_tiles);
     const int bt = tile0 + wb;
     const bool busy = bt < p.b_tiles;
-    uint4_t w[D][G][KS];
-    int sw[D][G][SW], scale[D][G][KS];
-    if (busy) {
-        const int wo = bt * 32 + (LAST ? l32 : run), o = wo < p.b ? wo : p.b - 1;  // (outputs behind the last one are read as the last one)
-#pragma unroll
-        for (int j = 0; j < D; ++j)
-#pragma unroll
-            for (int q = 0; q < G; ++q) {
-                const int64_t at = (((int64_t)ai * p.d + d0 + j) * rows_w + q * p.b + o) * p.cb;
-#pragma unroll
-                for (int s = 0; s < KS; ++s) {
-                    const int kb = 2 * s + half;
-                    const bool there = kb < p.cb;
-                    w[j][q][s] = there ? *(const uint4_t *)(p.w + (at + kb) * 16) : uint4_t{0, 0, 0, 0};
-                    scale[j][q][s] = there ? p.w_scales[at + kb] : 127;
-                }
-            }
-    }
+    MxHeld<LAST, D, G, KS> held;
+    if (busy) held.load(p, ai, d0, bt, l32, run, half);
     prepare();
     __syncthreads();
-#pragma unroll
-    for (int j = 0; j < D; ++j)
-#pragma unroll
-        for (int q = 0; q < G; ++q)
-#pragma unroll
-            for (int s = 0; s < KS; ++s) sw[j][q][s / 4] = s % 4 ? sw[j][q][s / 4] | scale[j][q][s] << 8 * (s % 4) : scale[j][q][s];
-    // (said to the compiler: the weights are there, and no step waits for them again, which would be for all stores before it too)
-#pragma unroll
-    for (int j = 0; j < D; ++j)
-#pragma unroll
-        for (int q = 0; q < G; ++q) {
-#pragma unroll
-            for (int s = 0; s < KS; ++s) asm volatile("" : "+v"(w[j][q][s]));
-#pragma unroll
-            for (int s = 0; s < SW; ++s) asm volatile("" : "+v"(sw[j][q][s]));
-        }
+    held.arrived();
     int which = 0;
     for (int tile = first; tile < row_tiles; tile += p.row_splits, which ^= 1) {
         const int n0 = tile * TN, here = batch - n0 < TN ? batch - n0 : TN;
@@ -310,33 +347,11 @@ __global__ __launch_bounds__(64 * (MX_CONSUMERS + MX_PRODUCERS)) void ks_mx_held
             T v[16 * D];
 #pragma unroll
             for (int j = 0; j < D; ++j) {
-                const int row = j * TN + t * 32 + (LAST ? run : l32);
-                int sx[SW];
-#pragma unroll
-                for (int i = 0; i < SW; ++i) sx[i] = ((const int *)(scales + row * 2 * SB + half * SB))[i];
                 float16_t acc[G];
-                auto steps = [&](auto biased) {
-#pragma unroll
-                    for (int q = 0; q < G; ++q) {
-                        acc[q] = float16_t{};
-                        if constexpr (decltype(biased)::value)
-#pragma unroll
-                            for (int i = 0; i < 16; ++i) acc[q][i] = bias[((wb * G + q) * D + j) * 32 + (LAST ? l32 : 16 * half + i)];
-                    }
-#pragma unroll
-                    for (int s = 0; s < KS; ++s) {
-                        const uint4_t x = *(const uint4_t *)(codes + (row * p.slots + 2 * s + half) * 16);
-#pragma unroll
-                        for (int q = 0; q < G; ++q) acc[q] = mx_step<LAST>(w[j][q][s], sw[j][q][s / 4], x, sx[s / 4], s % 4, acc[q]);
-                    }
-                };
-                if (p.bias)
-                    steps(std::true_type());
-                else
-                    steps(std::false_type());
+                held.sums(codes, scales, p.slots, j * TN + t * 32 + (LAST ? run : l32), j, l32, half, p.bias ? bias + wb * G * D * 32 : nullptr, acc);
                 mx_activate<T, D, GATED, ACT>(acc, j, v);
             }
-            mx_results<T, LAST, D>(p, v, ai, d0, bt, lane, n0, t, here, stage);
+            mx_results<T, LAST, D>(p, v, ai, d0, bt, lane, n0, t, here, stage, p.b);
         }
     }
 }
@@ -568,7 +583,7 @@ template <typename T, bool LAST, int D, int TT, bool GATED, int ACT> __global__ 
                 T v[16];
                 mx_activate<T, 1, GATED, ACT>(acc[t], 0, v);
                 if (LAST || alone) {
-                    if (t * 32 < here) mx_results<T, LAST, 1>(p, v, ai, d0, bt, lane, n0, t, here, (uint8_t *)stage + wave * MX_STAGE);
+                    if (t * 32 < here) mx_results<T, LAST, 1>(p, v, ai, d0, bt, lane, n0, t, here, (uint8_t *)stage + wave * MX_STAGE, p.b);
                 } else {
                     T *const to = stage + (t * 32 + l32) * pitch + ((bt - chunk) * 32 + 16 * half) * dc + j;
 #pragma unroll
@@ -657,43 +672,50 @@ inline int mx_registers(const void *kernel)
     return hipFuncGetAttributes(&a, kernel) == hipSuccess ? a.numRegs : 512;
 }
 
-template <typename T, bool LAST, int D, bool GATED, int KS> int mx_launch_held(MxProduct p, int act, hipStream_t s)
+// sizes of a launch whose weights are held: `most` blocks a step of a workgroup
+inline void mx_held_sizes(MxProduct &p, bool last, int most)
 {
-    constexpr int Q = mx_quarters<T>(LAST, KS, D), MOST = 64 * MX_PRODUCERS * mx_rounds(KS, Q) / Q;  // blocks a step
     p.slots = p.cb | 1;
-    p.runs = LAST ? p.d : 1;
+    p.runs = last ? p.d : 1;
     p.units = p.a * p.runs;
     p.b_tiles = (p.b + 31) / 32;
     // eight waves: the more of them share their rows the less often these are quantised, but none should idle
     int idle = 1 << 30;
     for (int tiles = MX_CONSUMERS; tiles >= 1; tiles /= 2) {
         const int over = (p.b_tiles + tiles - 1) / tiles * tiles - p.b_tiles;
-        if (over < idle && 32 * MX_CONSUMERS / tiles * p.cb <= MOST) {
+        if (over < idle && 32 * MX_CONSUMERS / tiles * p.cb <= most) {
             p.wave_tiles = tiles;
             idle = over;
         }
     }
     p.tile_rows = 32 * MX_CONSUMERS / p.wave_tiles;
-    auto groups = [&] { return (int64_t)p.units * ((p.b_tiles + p.wave_tiles - 1) / p.wave_tiles); };
     p.token_tiles = (p.batch + p.tile_rows - 1) / p.tile_rows;
-    // a workgroup a compute unit, or two where the registers of both fit: one more would be a second round.  Those of the same rows lie on
-    // the same XCD where that is a multiple of eight apart
-    auto most_of = [&](int a_unit) {
-        const int64_t most = std::max<int64_t>(1, 256 * a_unit / groups());
-        return most >= 8 ? most / 8 * 8 : most;
-    };
-    int64_t most = most_of(1);
+}
+inline int64_t mx_held_groups(const MxProduct &p) { return (int64_t)p.units * ((p.b_tiles + p.wave_tiles - 1) / p.wave_tiles); }
+// workgroups that share the steps of one tile of outputs: one a compute unit, or two where the registers of both fit; one more would be a
+// second round.  Those of the same rows lie on the same XCD where that is a multiple of eight apart
+inline int64_t mx_held_splits(const MxProduct &p, int a_unit)
+{
+    const int64_t most = std::max<int64_t>(1, 256 * a_unit / mx_held_groups(p));
+    return most >= 8 ? most / 8 * 8 : most;
+}
+
+template <typename T, bool LAST, int D, bool GATED, int KS> int mx_launch_held(MxProduct p, int act, hipStream_t s)
+{
+    constexpr int Q = mx_quarters<T>(LAST, KS, D);
+    mx_held_sizes(p, LAST, 64 * MX_PRODUCERS * mx_rounds(KS, Q) / Q);
+    int64_t most = mx_held_splits(p, 1);
     if (p.token_tiles > most && mx_held_lds(D, GATED, KS, p.cb, p.tile_rows, p.wave_tiles) <= 80 * 1024) {
         with_act(act, [&](auto which) {
             constexpr int ACT = decltype(which)::value;
             if constexpr (GATED || ACT != KSMM_ACT_SILU) {
                 static const int registers = mx_registers((const void *)&ks_mx_held_kernel<T, LAST, D, GATED, ACT, KS>);
-                if (registers <= 80) most = most_of(2);  // (six waves of each SIMD's 512)
+                if (registers <= 80) most = mx_held_splits(p, 2);  // (six waves of each SIMD's 512)
             }
         });
     }
     p.row_splits = (int)std::min(p.token_tiles, most);
-    const int64_t grid = groups() * p.row_splits;
+    const int64_t grid = mx_held_groups(p) * p.row_splits;
     if (grid > 0x7fffffffLL) return KSMM_ERR_TOO_LARGE;
     const int lds = (int)mx_held_lds(D, GATED, KS, p.cb, p.tile_rows, p.wave_tiles);
     int rc = KSMM_OK;

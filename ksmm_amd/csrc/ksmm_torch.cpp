@@ -787,6 +787,16 @@ struct MxNode : ag::Node {
     MxHow how;
     c10::SmallVector<int64_t, 6> x_shape;
     std::string name() const override { return "MXLinearBackward"; }
+    void layer_backward(const ksmm_factor_desc &f, const at::Tensor &x, const at::Tensor &z, const at::Tensor &dy, at::Tensor (&out)[3], int act, int dt, void *stream)
+    {
+        const int64_t need = ksmm_layer_backward_workspace(&f, 1, how.batch, dt, how.bs_last, act);
+        check_status(need < 0 ? (int)need : KSMM_OK);
+        const at::Tensor ws = bytes_like(dy, {need});
+        const void *inputs[] = {data_of(x)};
+        void *dw[] = {out_of(out[1])};
+        check_status(ksmm_layer_backward(&f, 1, inputs, data_of(z), data_of(dy), out_of(out[0]), dw, out_of(out[2]), ws.mutable_data_ptr(), need, how.batch, dt,
+                                         how.bs_last, act, stream));
+    }
     void release_variables() override
     {
         std::lock_guard<std::mutex> lock(mutex_);
@@ -813,26 +823,31 @@ struct MxNode : ag::Node {
             if (task_should_compute_output(0)) out[0] = at::empty(x_shape, dy.options());
             if (task_should_compute_output(1)) out[1] = at::empty_like(w);
             if (t[4].defined() && task_should_compute_output(2)) out[2] = at::empty_like(t[4]);
-            if (how.gated) {
+            // what the activation was applied to is computed again, with the gradients of it where there is a kernel for both
+            const bool nothing = how.act == KSMM_ACT_NONE && !how.gated;
+            auto slope = [&](void *dz) {
+                return ksmm_mx_slope(data_of(t[0]), data_of(t[1]), data_of(t[2]), data_of(t[3]), data_of(t[4]), data_of(dy), dz, how.batch, how.a, how.b, how.c, how.d,
+                                     dt, how.bs_last, how.act, how.gated, stream);
+            };
+            if (nothing || slope(nullptr) == KSMM_OK) {
+                at::Tensor dz = dy;
+                if (!nothing) {
+                    dz = at::empty({how.batch * how.a * how.rows() * how.d}, dy.options());
+                    check_status(slope(out_of(dz)));
+                }
+                const ksmm_factor_desc f{data_of(w), how.a, how.rows(), how.c, how.d, dt, 1.f};
+                layer_backward(f, x, at::Tensor(), dz, out, KSMM_ACT_NONE, dt, stream);
+            } else if (how.gated) {
                 const int64_t need = ksmm_gated_backward_workspace(how.batch, how.a, how.b, how.c, how.d, dt, how.bs_last);
                 check_status(need < 0 ? (int)need : KSMM_OK);
                 const at::Tensor ws = bytes_like(dy, {need});
                 check_status(ksmm_gated_backward(data_of(dy), data_of(x), data_of(w), data_of(t[4]), out_of(out[0]), out_of(out[1]), out_of(out[2]),
                                                  ws.mutable_data_ptr(), need, how.batch, how.a, how.b, how.c, how.d, dt, how.bs_last, how.act, stream));
             } else {
-                at::Tensor z;
-                if (how.act != KSMM_ACT_NONE) {  // what the activation was applied to, computed again
-                    z = at::empty_like(dy);
-                    check_status(mx_forward(data_of(t[0]), data_of(t[1]), t[2], t[3], t[4], z, nullptr, nullptr, how, KSMM_ACT_NONE));
-                }
+                at::Tensor z = at::empty_like(dy);
+                check_status(mx_forward(data_of(t[0]), data_of(t[1]), t[2], t[3], t[4], z, nullptr, nullptr, how, KSMM_ACT_NONE));
                 const ksmm_factor_desc f{data_of(w), how.a, how.b, how.c, how.d, dt, 1.f};
-                const int64_t need = ksmm_layer_backward_workspace(&f, 1, how.batch, dt, how.bs_last, how.act);
-                check_status(need < 0 ? (int)need : KSMM_OK);
-                const at::Tensor ws = bytes_like(dy, {need});
-                const void *inputs[] = {data_of(x)};
-                void *dw[] = {out_of(out[1])};
-                check_status(ksmm_layer_backward(&f, 1, inputs, data_of(z), data_of(dy), out_of(out[0]), dw, out_of(out[2]), ws.mutable_data_ptr(), need,
-                                                 how.batch, dt, how.bs_last, how.act, stream));
+                layer_backward(f, x, z, dy, out, how.act, dt, stream);
             }
         }
         for (int i = 0; i < 3; ++i) result[i] = out[i];

@@ -246,13 +246,35 @@ class MXFunction(torch.autograd.Function):
         packed = MXFactor(w_codes, w_scales, pattern, gated)
         w = packed.dequantize(dtype)
         grad = grad.contiguous()
-        if gated:
+        dz = _slope(grad, q, packed, bias, act, bs_last) if grad.numel() > 0 and (gated or act not in (None, "none")) else None
+        if dz is not None:  # those of a layer without an activation, of the gate's and the other projection's outputs side by side
+            packed = MXFactor(w_codes, w_scales, (a, packed.codes.size(1), c, d))
+            dx, dw, dbias = _backward(dz, q, packed, w, bias, None, bs_last, need_x, need_w, need_b)
+        elif gated:
             dx, dw, dbias = GatedKernel.backward(grad, q.dequantize(), w, pattern, bias, act, bs_last, need_x, need_w, need_b)
         else:
             dx, dw, dbias = _backward(grad, q, packed, w, bias, act, bs_last, need_x, need_w, need_b)
         if dw is not None and dw.dtype != ctx.factor_dtype:
             dw = dw.to(ctx.factor_dtype)
         return dx, dw, dbias, None, None, None, None
+
+
+def _slope(grad, q, packed, bias, act, bs_last):
+    """The gradient of what the activation was applied to, or None where no kernel computes both."""
+    lib = _lib.load()
+    a, b, c, d = packed.pattern
+    rows, batch = packed.codes.size(1), q.codes.size(1)
+
+    def call(out):
+        return lib.ksmm_mx_slope(q.codes.data_ptr(), q.scales.data_ptr(), packed.codes.data_ptr(), packed.scales.data_ptr(), _ptr(bias), grad.data_ptr(),
+                                 _ptr(out), batch, a, b, c, d, dtype_code(grad.dtype), int(bs_last), GATED_ACTS[act], int(packed.gated), _stream_ptr(grad))
+
+    if call(None) != 0:
+        return None
+    out = torch.empty((a * rows * d, batch) if bs_last else (batch, a * rows * d), dtype=grad.dtype, device=grad.device)
+    with torch.cuda.device(grad.device):
+        _lib.check(call(out))
+    return out
 
 
 def _backward(grad, q, packed, w, bias, act, bs_last, need_x, need_w, need_b):

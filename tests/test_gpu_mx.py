@@ -573,3 +573,45 @@ def test_packed_blocks_are_their_own():
     new = pack_block(block)
     new.register_buffer("more", torch.zeros(1))
     assert not hasattr(block, "more") and "gated" in block._modules and type(block.gated) is not type(new.gated)
+
+
+SLOPES = [(1, 1, 1, 1), (2, 5, 3, 2), (1, 32, 32, 1), (3, 33, 40, 1), (1, 64, 192, 2), (2, 96, 72, 2), (1, 130, 120, 1), (1, 768, 192, 2), (6, 64, 64, 1), (1, 200, 250, 1), (4, 192, 192, 1),
+          (2, 24, 70, 3), (1, 40, 16, 5), (1, 48, 400, 1)]
+
+
+@pytest.mark.parametrize("bs_last", [False, True])
+@pytest.mark.parametrize("prec", ["fp32", "fp16"])
+@pytest.mark.parametrize("pattern", SLOPES)
+def test_gradients_of_what_activations_are_applied_to(pattern, prec, bs_last):
+    """In fp16 they are rounded once, 2^-11 of each; fp32 as its sums are."""
+    from ksmm_amd import _lib, pack_mx, quantize_mx
+    from ksmm_amd.mx import _slope
+
+    a, b, c, d = pattern
+    for n, gated, act, with_bias in ((1, True, "silu", True), (7, False, "gelu", True), (33, True, "gelu", False), (200, True, None, True), (517, False, "gelu", False),
+                                     (1000, True, "silu", False)):
+        x, f = rows(n, a * c * d, bs_last, DT[prec], n), factor(pattern, gated, DT[prec])
+        total = a * b * d * (1 + gated)
+        bias = torch.linspace(-1, 1, total).to(DT[prec]) if with_bias else None
+        dy = rows(n, a * b * d, bs_last, DT[prec], n + 1)
+        q, w = quantize_mx(x.cuda(), (a, c, d), bs_last), pack_mx(f.cuda(), pattern, gated)
+        got = _slope(dy.cuda(), q, w, None if bias is None else bias.cuda(), act, bs_last)
+        taken = (bs_last or d <= (2 if prec == "fp16" else 1)) and c <= 256
+        assert (got is not None) or not taken
+        if got is None:
+            continue
+        xr = R.rounded(R.operand(x, a, c, d, bs_last))
+        with torch.enable_grad():
+            z = (xr @ R.rounded(factor_rows(f, pattern)).transpose(2, 3)).double()
+            if bias is not None:
+                z = z + bias.double().reshape(a, -1, d).permute(0, 2, 1).unsqueeze(2)
+            z = z.detach().requires_grad_(True)
+            y = R.act(act, z[..., :b]) * z[..., b:] if gated else R.act(act, z)
+            want, = torch.autograd.grad(y, z, R.operand(dy, a, b, d, bs_last).double())
+        assert rel(got, R.tensor(want, got.shape, bs_last)) <= (2.0 ** -11 + 1e-5 if prec == "fp16" else TOL[prec]), (n, gated, act)
+        if n == 517:  # nothing behind the end is written
+            room = torch.full((got.numel() + 64,), 7.0, dtype=DT[prec], device="cuda")
+            out = room[:got.numel()]
+            rc = _lib.load().ksmm_mx_slope(q.codes.data_ptr(), q.scales.data_ptr(), w.codes.data_ptr(), w.scales.data_ptr(), None, dy.cuda().data_ptr(), out.data_ptr(), n, a, b, c, d,
+                                           0 if prec == "fp32" else 1, int(bs_last), 1, int(gated), torch.cuda.current_stream().cuda_stream)
+            assert rc == 0 and torch.equal(out, got.flatten()) and (room[got.numel():] == 7).all()

@@ -83,6 +83,35 @@ def test_products_refuse(lib, c):
                         assert call(False, workspace=at[k]) == ALIAS
 
 
+@pytest.mark.parametrize("gated", [0, 1])
+@pytest.mark.parametrize("dtype", [0, 1])
+def test_slopes_refuse(lib, dtype, gated):
+    n, a, b, c, d, size = 9, 2, 24, 40, 1, (4, 2)[dtype]
+    names = ["x", "x_scales", "w", "w_scales", "bias", "dy", "dz"]
+    at = dict(zip(names, FAR))
+
+    def call(n=n, a=a, b=b, c=c, d=d, dtype=dtype, bs_last=0, act=1, **change):
+        p = dict(at, **change)
+        return lib.ksmm_mx_slope(*(p[k] for k in names), n, a, b, c, d, dtype, bs_last, act, gated, None)
+
+    for k in ("x", "x_scales", "w", "w_scales", "dy"):
+        assert call(**{k: None}) == NULL
+    assert call(n=0) == BATCH and call(c=0) == PATTERN and call(dtype=2) == DTYPE and call(n=0x7fffffff) == LARGE and call(act=3) == EPILOGUE
+    if not gated:
+        assert call(act=0) == EPILOGUE and call(act=2) == EPILOGUE
+    assert call(w=at["w"] + 8) == WORKSPACE and call(x=at["x"] + 4) == WORKSPACE
+    rows = b * (1 + gated)
+    sizes = {"x": n * a * 2 * 16, "x_scales": n * a * 2, "w": rows * a * 2 * 16, "w_scales": rows * a * 2, "bias": a * rows * size, "dy": n * a * b * size}
+    for k in sizes:
+        assert call(dz=at[k] + sizes[k] - 1) == ALIAS, k
+    # what there is a kernel for is said without a launch
+    for bs_last in (0, 1):
+        assert call(dz=None, bs_last=bs_last) == 0
+        assert call(dz=None, bs_last=bs_last, d=2) == (0 if bs_last or dtype == 1 else ALGO)
+        assert call(dz=None, bs_last=bs_last, d=3) == (0 if bs_last else ALGO) and call(dz=None, bs_last=bs_last, c=2000) == ALGO
+        assert call(bs_last=bs_last, c=2000) == ALGO
+
+
 def table(count=2, n=100, small=True, master=True):
     from ksmm_amd._lib import KsmmAdamwTensor
 
