@@ -21,7 +21,23 @@ struct MxOperand {
     int a, c, d, cb;
     bool last;
     int64_t blocks;  // a * d * rows * cb
+    bool small;      // tasks that the two divide by multiplying
+    MxDiv by_cb, by_a;
 };
+// task t as (n, ai, kb), t = (n a + ai) cb + kb
+__device__ __forceinline__ int64_t mx_place(const MxOperand &p, int64_t t, int &ai, int &kb)
+{
+    if (p.small) {
+        const int i = (int)t, u = p.by_cb(i), n = p.by_a(u);
+        kb = i - u * p.cb;
+        ai = u - n * p.a;
+        return n;
+    }
+    const int64_t u = t / p.cb, n = u / p.a;
+    kb = (int)(t - u * p.cb);
+    ai = (int)(u - n * p.a);
+    return n;
+}
 constexpr int THREADS = 256;
 
 // ---- batch-size-first, all d_i of up to four in a row: four lanes a block, so that lanes that follow one another read and write 16 * D
@@ -32,11 +48,9 @@ template <typename T, int D, bool BACK> __global__ __launch_bounds__(THREADS) vo
     const int64_t tasks = p.blocks / D * 4;
     const int quarter = threadIdx.x & 3;
     for (int64_t i = blockIdx.x * (int64_t)THREADS + threadIdx.x; i < tasks; i += gridDim.x * (int64_t)THREADS) {
-        int64_t t = i >> 2;
-        const int kb = (int)(t % p.cb);
-        t /= p.cb;
-        const int ai = (int)(t % p.a), count = p.c - kb * 32 - quarter * 8;
-        const int64_t n = t / p.a;
+        int ai, kb;
+        const int64_t n = mx_place(p, i >> 2, ai, kb);
+        const int count = p.c - kb * 32 - quarter * 8;
         T *const x = (T *)p.x + ((n * p.a + ai) * p.c + kb * 32 + quarter * 8) * D;
         T v[N];
         if constexpr (!BACK) {
@@ -101,13 +115,10 @@ template <typename T, int D, bool BACK> __global__ __launch_bounds__(THREADS) vo
     const int64_t tasks = p.blocks / D;
     const int runs = p.d / D;
     for (int64_t i = blockIdx.x * (int64_t)THREADS + threadIdx.x; i < tasks; i += gridDim.x * (int64_t)THREADS) {
-        int64_t t = i;
-        const int d0 = (int)(t % runs) * D;
-        t /= runs;
-        const int kb = (int)(t % p.cb);
-        t /= p.cb;
-        const int ai = (int)(t % p.a), count = p.c - kb * 32;
-        const int64_t n = t / p.a;
+        const int64_t t = i / runs;
+        int ai, kb;
+        const int64_t n = mx_place(p, t, ai, kb);
+        const int d0 = (int)(i - t * runs) * D, count = p.c - kb * 32;
         T *const x = (T *)p.x + ((n * p.a + ai) * p.c + kb * 32) * p.d + d0;
         MxGroup<T, D> g;
         if constexpr (!BACK) mx_load<T, D>(g, x, p.d, count);
@@ -149,13 +160,10 @@ template <typename T, bool BACK> __global__ __launch_bounds__(THREADS) void ks_m
 {
     __shared__ uint4_t codes[64 * 4 + 4];
     __shared__ uint8_t scales[64 * 4];
-    const int quads = (p.cb + 3) / 4;
-    int64_t t = blockIdx.x;
-    const int kb0 = (int)(t % quads) * 4;
-    t /= quads;
-    const int64_t n0 = t % tiles * 64;
-    t /= tiles;
-    const int di = (int)(t % p.d), ai = (int)(t / p.d);
+    // (in 32 bits: a workgroup begins with these, and lives for 32 loads)
+    const uint32_t quads = (uint32_t)(p.cb + 3) / 4, u = blockIdx.x / quads, row_tiles = (uint32_t)tiles, block_at = u / row_tiles;
+    const int kb0 = (int)(blockIdx.x - u * quads) * 4, ai = (int)(block_at / (uint32_t)p.d), di = (int)block_at - ai * p.d;
+    const int64_t n0 = (int64_t)(u - block_at * row_tiles) * 64;
     const int row = threadIdx.x & 63, kb = kb0 + (threadIdx.x >> 6), count = p.c - kb * 32;
     const int64_t step = (int64_t)p.d * p.rows, n = n0 + row;
     T *const x = (T *)p.x + (((int64_t)ai * p.c + kb * 32) * p.d + di) * p.rows + n;
@@ -303,7 +311,10 @@ int check_operand(int64_t rows, int a, int c, int d, int dtype)
 MxOperand operand(const void *x, void *codes, void *scales, int64_t rows, int a, int c, int d, int bs_last)
 {
     const int cb = (int)mx_blocks(c);
-    return MxOperand{x, (uint8_t *)codes, (uint8_t *)scales, rows, a, c, d, cb, bs_last != 0, (int64_t)a * d * rows * cb};
+    // (MxDiv: t d < 2^32 of the largest t)
+    const int64_t tasks = (int64_t)a * rows * cb;
+    return MxOperand{x,  (uint8_t *)codes, (uint8_t *)scales, rows, a, c, d, cb, bs_last != 0, (int64_t)a * d * rows * cb, tasks < (1LL << 32) / std::max(a, cb) && tasks < 1LL << 31,
+                     MxDiv(cb), MxDiv(a)};
 }
 int64_t values(int64_t rows, int a, int c, int d) { return rows * a * c * d; }
 int64_t align256(int64_t v) { return (v + 255) / 256 * 256; }

@@ -252,7 +252,7 @@ __global__ __launch_bounds__(64 * (MX_CONSUMERS + MX_PRODUCERS)) void ks_mx_held
     float *const bias = (float *)(smem + 2 * buffer);
     uint8_t *const stage = smem + 2 * buffer + p.wave_tiles * G * D * 128 + wave * MX_STAGE;
     const int tasks = TN * p.cb, batch = (int)p.batch, row_tiles = (int)p.token_tiles;  // (steps past the end are counted in 32 bits)
-    const bool emit = p.codes_out && tile0 == 0;
+    const int turns = p.codes_out ? p.splits : 0, mine = blk / p.units;  // (workgroups of the same rows hand out the codes in turn)
 
     // what a thread loads for the step of rows n0 on: the blocks of task t, or batch-size-first a quarter of them
     constexpr int Q = mx_quarters<T>(LAST, KS, D);
@@ -276,7 +276,7 @@ __global__ __launch_bounds__(64 * (MX_CONSUMERS + MX_PRODUCERS)) void ks_mx_held
         else
             mx_load<T, D>(f, (const T *)p.x + ((((int64_t)n0 + n) * p.a + ai) * p.c + kb * 32 + quarter * 8) * D, p.c - kb * 32 - quarter * 8);
     };
-    auto keep = [&](const Load &f, int t, int at, int n0, int which) {
+    auto keep = [&](const Load &f, int t, int at, int n0, int which, bool emit) {
         if (!there(t, at, n0)) return;
         const int n = at >> 8, kb = at & 255;
         uint8_t *const codes = smem + which * buffer, *const scales = codes + D * TN * p.slots * 16;
@@ -315,11 +315,13 @@ __global__ __launch_bounds__(64 * (MX_CONSUMERS + MX_PRODUCERS)) void ks_mx_held
         for (int r = 0; r < AHEAD; ++r) fetch(f[r], t0 + r * 64 * MX_PRODUCERS, at[r], first * TN);
         prepare();
         __syncthreads();
-        int which = 0;
+        int which = 0, turn = turns ? 0 : -1;
         for (int tile = first; tile < row_tiles; tile += p.row_splits, which ^= 1) {
+            const bool emit = turn == mine;
+            if (turns) turn = turn + 1 < turns ? turn + 1 : 0;
 #pragma unroll
             for (int r = 0; r < R; ++r) {
-                keep(f[r % AHEAD], t0 + r * 64 * MX_PRODUCERS, at[r], tile * TN, which);
+                keep(f[r % AHEAD], t0 + r * 64 * MX_PRODUCERS, at[r], tile * TN, which, emit);
                 const int next = (r + AHEAD) % R;
                 if (r + AHEAD < R || tile + p.row_splits < row_tiles)
                     fetch(f[r % AHEAD], t0 + next * 64 * MX_PRODUCERS, at[next], (r + AHEAD < R ? tile : tile + p.row_splits) * TN);
@@ -690,8 +692,9 @@ inline void mx_held_sizes(MxProduct &p, bool last, int most)
     }
     p.tile_rows = 32 * MX_CONSUMERS / p.wave_tiles;
     p.token_tiles = (p.batch + p.tile_rows - 1) / p.tile_rows;
+    p.splits = (p.b_tiles + p.wave_tiles - 1) / p.wave_tiles;
 }
-inline int64_t mx_held_groups(const MxProduct &p) { return (int64_t)p.units * ((p.b_tiles + p.wave_tiles - 1) / p.wave_tiles); }
+inline int64_t mx_held_groups(const MxProduct &p) { return (int64_t)p.units * p.splits; }
 // workgroups that share the steps of one tile of outputs: one a compute unit, or two where the registers of both fit; one more would be a
 // second round.  Those of the same rows lie on the same XCD where that is a multiple of eight apart
 inline int64_t mx_held_splits(const MxProduct &p, int a_unit)
