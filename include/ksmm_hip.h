@@ -417,7 +417,7 @@ int ksmm_mx_forward(const void *x, const void *x_scales, const void *w, const vo
 /* Gradients of what the activation was applied to, which is computed again from the operands' codes: with `gated` dz of 2*b rows a block,
  * dy u act'(g) and dy act(g) in G's and U's places, else dy act'(z), rounded to `dtype`; they are those of a layer of the pattern
  * (a, 2*b or b, c, d) without an activation.  KSMM_ERR_BAD_ALGO: there is no kernel for the pattern (batch-size-first
- * d above 2, in fp32 above 1, or weights that registers do not hold); dz NULL: only that is found, nothing is launched. */
+ * d above 4, in fp32 above 2, or weights that registers do not hold); dz NULL: only that is found, nothing is launched. */
 int ksmm_mx_slope(const void *x, const void *x_scales, const void *w, const void *w_scales, const void *bias, const void *dy,
                   void *dz, int64_t batch, int a, int b, int c, int d, int dtype, int bs_last, int act, int gated,
                   void *stream);

@@ -623,9 +623,9 @@ template <typename T, bool LAST, int D, int TT, bool GATED, int ACT> __global__ 
     }
 }
 
-inline int64_t mx_held_lds(int d, bool gated, int ks, int cb, int rows, int tiles)
+inline int64_t mx_held_lds(int d, bool gated, int ks, int cb, int rows, int tiles, int consumers)
 {
-    return 2LL * d * rows * ((cb | 1) * 16 + 2 * mx_scale_bytes(ks)) + (int64_t)tiles * (gated ? 2 : 1) * 32 * d * 4 + MX_CONSUMERS * MX_STAGE;
+    return 2LL * d * rows * ((cb | 1) * 16 + 2 * mx_scale_bytes(ks)) + (int64_t)tiles * (gated ? 2 : 1) * 32 * d * 4 + consumers * MX_STAGE;
 }
 
 template <typename T, bool LAST, int D, int TT, bool GATED> int mx_launch_wide(MxProduct p, int act, hipStream_t s)
@@ -674,25 +674,31 @@ inline int mx_registers(const void *kernel)
     return hipFuncGetAttributes(&a, kernel) == hipSuccess ? a.numRegs : 512;
 }
 
-// sizes of a launch whose weights are held: `most` blocks a step of a workgroup
-inline void mx_held_sizes(MxProduct &p, bool last, int most)
+// the rest of the sizes, with `tiles` of outputs a workgroup
+inline void mx_held_tiles(MxProduct &p, int consumers, int tiles)
+{
+    p.wave_tiles = tiles;
+    p.tile_rows = 32 * consumers / tiles;
+    p.token_tiles = (p.batch + p.tile_rows - 1) / p.tile_rows;
+    p.splits = (p.b_tiles + tiles - 1) / tiles;
+}
+// sizes of a launch whose weights are held by `consumers` waves: `most` blocks a step of a workgroup
+inline void mx_held_sizes(MxProduct &p, bool last, int consumers, int most)
 {
     p.slots = p.cb | 1;
     p.runs = last ? p.d : 1;
     p.units = p.a * p.runs;
     p.b_tiles = (p.b + 31) / 32;
-    // eight waves: the more of them share their rows the less often these are quantised, but none should idle
+    // the more waves share their rows the less often these are quantised, but none should idle
     int idle = 1 << 30;
-    for (int tiles = MX_CONSUMERS; tiles >= 1; tiles /= 2) {
+    for (int tiles = consumers; tiles >= 1; tiles /= 2) {
         const int over = (p.b_tiles + tiles - 1) / tiles * tiles - p.b_tiles;
-        if (over < idle && 32 * MX_CONSUMERS / tiles * p.cb <= most) {
+        if (over < idle && 32 * consumers / tiles * p.cb <= most) {
             p.wave_tiles = tiles;
             idle = over;
         }
     }
-    p.tile_rows = 32 * MX_CONSUMERS / p.wave_tiles;
-    p.token_tiles = (p.batch + p.tile_rows - 1) / p.tile_rows;
-    p.splits = (p.b_tiles + p.wave_tiles - 1) / p.wave_tiles;
+    mx_held_tiles(p, consumers, p.wave_tiles);
 }
 inline int64_t mx_held_groups(const MxProduct &p) { return (int64_t)p.units * p.splits; }
 // workgroups that share the steps of one tile of outputs: one a compute unit, or two where the registers of both fit; one more would be a
@@ -706,9 +712,9 @@ inline int64_t mx_held_splits(const MxProduct &p, int a_unit)
 template <typename T, bool LAST, int D, bool GATED, int KS> int mx_launch_held(MxProduct p, int act, hipStream_t s)
 {
     constexpr int Q = mx_quarters<T>(LAST, KS, D);
-    mx_held_sizes(p, LAST, 64 * MX_PRODUCERS * mx_rounds(KS, Q) / Q);
+    mx_held_sizes(p, LAST, MX_CONSUMERS, 64 * MX_PRODUCERS * mx_rounds(KS, Q) / Q);
     int64_t most = mx_held_splits(p, 1);
-    if (p.token_tiles > most && mx_held_lds(D, GATED, KS, p.cb, p.tile_rows, p.wave_tiles) <= 80 * 1024) {
+    if (p.token_tiles > most && mx_held_lds(D, GATED, KS, p.cb, p.tile_rows, p.wave_tiles, MX_CONSUMERS) <= 80 * 1024) {
         with_act(act, [&](auto which) {
             constexpr int ACT = decltype(which)::value;
             if constexpr (GATED || ACT != KSMM_ACT_SILU) {
@@ -720,7 +726,7 @@ template <typename T, bool LAST, int D, bool GATED, int KS> int mx_launch_held(M
     p.row_splits = (int)std::min(p.token_tiles, most);
     const int64_t grid = mx_held_groups(p) * p.row_splits;
     if (grid > 0x7fffffffLL) return KSMM_ERR_TOO_LARGE;
-    const int lds = (int)mx_held_lds(D, GATED, KS, p.cb, p.tile_rows, p.wave_tiles);
+    const int lds = (int)mx_held_lds(D, GATED, KS, p.cb, p.tile_rows, p.wave_tiles, MX_CONSUMERS);
     int rc = KSMM_OK;
     with_act(act, [&](auto which) {
         constexpr int ACT = decltype(which)::value;

@@ -4,7 +4,7 @@
 //
 // What is kept of the forward pass are the operands' codes, 17 bytes for 32 values; of a call that writes z and another one that reads it
 // again two of the five passes over tensors of b features are left out.  The work is that of the forward kernel whose weights are in
-// registers: eight waves multiply and store, four bring the next step's codes of x and its dy into LDS, as they lie.
+// registers: eight waves (four) multiply and store, four bring the next step's codes of x and its dy into LDS, as they lie.
 // What bounds it: HBM.  (1,768,192,2) gated in fp16, 25088 rows: 236 MB in 46 us, 5.1 TB/s, what a copy reaches; the kernel that multiplies
 // the values in fp16 once more takes 80.
 #pragma once
@@ -14,14 +14,17 @@ namespace ksmm {
 
 namespace {
 
+// waves that multiply: with more than 4 bytes of D a value the dy of eight would not fit LDS, nor their registers the gradients
+template <typename T, int D> constexpr int mx_slope_waves() { return D * (int)sizeof(T) <= 4 ? MX_CONSUMERS : MX_CONSUMERS / 2; }
+
 // bytes from one line of dy in LDS (a row of the batch; batch-size-last an output) to the next: 16 more than there are, for the banks' sake
 template <typename T, bool LAST, int D> __host__ __device__ constexpr int mx_dy_pitch(int rows, int tiles) { return (LAST ? rows : tiles * 32 * D) * (int)sizeof(T) + 16; }
 
 template <typename T, bool LAST, int D, bool GATED, int ACT, int KS>
-__global__ __launch_bounds__(64 * (MX_CONSUMERS + MX_PRODUCERS)) void ks_mx_slope_kernel(MxProduct p)
+__global__ __launch_bounds__(64 * (mx_slope_waves<T, D>() + MX_PRODUCERS)) void ks_mx_slope_kernel(MxProduct p)
 {
-    constexpr int G = GATED ? 2 : 1, SB = mx_scale_bytes(KS), R = mx_rounds(KS, 1), E = 16 / (int)sizeof(T), THREADS = 64 * MX_PRODUCERS;
-    constexpr int V = 32 * MX_CONSUMERS * 32 * D / E / THREADS;  // vectors of dy that a producer's thread takes
+    constexpr int G = GATED ? 2 : 1, SB = mx_scale_bytes(KS), R = mx_rounds(KS, 1), E = 16 / (int)sizeof(T), THREADS = 64 * MX_PRODUCERS, C = mx_slope_waves<T, D>();
+    constexpr int V = 32 * C * 32 * D / E / THREADS;  // vectors of dy that a producer's thread takes
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     const int TN = p.tile_rows, pitch = mx_dy_pitch<T, LAST, D>(TN, p.wave_tiles), scales_at = D * TN * p.slots * 16, dy_at = scales_at + D * TN * 2 * SB;
     const int buffer = dy_at + (LAST ? p.wave_tiles * 32 : TN) * pitch;
@@ -37,8 +40,8 @@ __global__ __launch_bounds__(64 * (MX_CONSUMERS + MX_PRODUCERS)) void ks_mx_slop
     const int tasks = TN * p.cb, batch = (int)p.batch, row_tiles = (int)p.token_tiles;
     auto prepare = [&] { mx_prepare<T, D, G>(p, smem + scales_at, buffer, D * TN * SB / 2, bias, ai, d0, tile0); };
 
-    if (wave >= MX_CONSUMERS) {
-        const int t0 = threadIdx.x - 64 * MX_CONSUMERS;
+    if (wave >= C) {
+        const int t0 = threadIdx.x - 64 * C;
         const MxDiv by_cb(p.cb), by_line(LAST ? TN / E : p.wave_tiles * 32 * D / E);
         const int outs = p.b - tile0 * 32;  // from the workgroup's first tile on
         uint4_t code[D][R], dy[V];
@@ -114,7 +117,7 @@ __global__ __launch_bounds__(64 * (MX_CONSUMERS + MX_PRODUCERS)) void ks_mx_slop
         return;
     }
 
-    const int wb = wave & (p.wave_tiles - 1), wt = wave / p.wave_tiles, per_wave = TN / 32 / (MX_CONSUMERS / p.wave_tiles);
+    const int wb = wave & (p.wave_tiles - 1), wt = wave / p.wave_tiles, per_wave = TN / 32 / (C / p.wave_tiles);
     const int bt = tile0 + wb;
     const bool busy = bt < p.b_tiles;
     MxHeld<LAST, D, G, KS> held;
@@ -161,8 +164,13 @@ __global__ __launch_bounds__(64 * (MX_CONSUMERS + MX_PRODUCERS)) void ks_mx_slop
 
 template <typename T, bool LAST, int D, bool GATED, int KS> int mx_launch_slope(MxProduct p, int act, hipStream_t s)
 {
-    mx_held_sizes(p, LAST, 64 * MX_PRODUCERS * mx_rounds(KS, 1));
-    const int64_t lds = mx_held_lds(D, GATED, KS, p.cb, p.tile_rows, p.wave_tiles) + 2LL * (LAST ? p.wave_tiles * 32 : p.tile_rows) * mx_dy_pitch<T, LAST, D>(p.tile_rows, p.wave_tiles);
+    constexpr int C = mx_slope_waves<T, D>();
+    mx_held_sizes(p, LAST, C, 64 * MX_PRODUCERS * mx_rounds(KS, 1));
+    auto bytes = [&] {
+        return mx_held_lds(D, GATED, KS, p.cb, p.tile_rows, p.wave_tiles, C) + 2LL * (LAST ? p.wave_tiles * 32 : p.tile_rows) * mx_dy_pitch<T, LAST, D>(p.tile_rows, p.wave_tiles);
+    };
+    while (bytes() > MX_LDS_ALL && p.wave_tiles < C) mx_held_tiles(p, C, 2 * p.wave_tiles);  // (fewer rows of codes)
+    const int64_t lds = bytes();
     if (lds > MX_LDS_ALL) return KSMM_ERR_BAD_ALGO;
     p.row_splits = (int)std::min(p.token_tiles, mx_held_splits(p, 1));
     const int64_t grid = mx_held_groups(p) * p.row_splits;
@@ -175,7 +183,7 @@ template <typename T, bool LAST, int D, bool GATED, int KS> int mx_launch_slope(
             auto fn = &ks_mx_slope_kernel<T, LAST, D, GATED, ACT, KS>;
             if (lds > 64 * 1024) rc = ensure_dynamic_lds((const void *)fn, (int)lds);
             if (rc != KSMM_OK) return;
-            hipLaunchKernelGGL(fn, dim3((unsigned)grid), dim3(64 * (MX_CONSUMERS + MX_PRODUCERS)), lds, s, p);
+            hipLaunchKernelGGL(fn, dim3((unsigned)grid), dim3(64 * (C + MX_PRODUCERS)), lds, s, p);
             if (hipGetLastError() != hipSuccess) rc = KSMM_ERR_LAUNCH;
         }
     });
@@ -184,9 +192,9 @@ template <typename T, bool LAST, int D, bool GATED, int KS> int mx_launch_slope(
 
 template <typename T, bool LAST, int D, bool GATED, int KS, int... MORE> int mx_slope_steps(const MxProduct &p, int act, hipStream_t s)
 {
-    // registers: the weights' codes, sums, and gradients of gate and up
+    // registers, 168 of them or 256: the weights' codes, sums, and gradients of gate and up
     constexpr int G = GATED ? 2 : 1, HELD = 4 * D * G * KS + 16 * G + 4 * D * G * (int)sizeof(T);
-    if constexpr (HELD <= 112) {
+    if constexpr (HELD <= (mx_slope_waves<T, D>() == MX_CONSUMERS ? 112 : 176)) {
         if (p.cb <= 2 * KS) return mx_launch_slope<T, LAST, D, GATED, KS>(p, act, s);
         if constexpr (sizeof...(MORE) > 0) return mx_slope_steps<T, LAST, D, GATED, MORE...>(p, act, s);
     }

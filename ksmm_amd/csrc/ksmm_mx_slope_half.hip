@@ -1,4 +1,4 @@
-// Gradients of what activations were applied to, of products of microscaled 4-bit numbers: fp16.  (The gradients of three d_i, gate and up, do not fit the registers.)
+// Gradients of what activations were applied to, of products of microscaled 4-bit numbers: fp16.
 #include "ksmm_mx_slope.h"
 
 namespace ksmm {
@@ -9,6 +9,8 @@ int mx_slope_half(const MxProduct &p, bool last, bool gated, int act, hipStream_
     switch (p.d) {
     case 1: return mx_slope<half_t, false, 1>(p, gated, act, s);
     case 2: return mx_slope<half_t, false, 2>(p, gated, act, s);
+    case 3: return mx_slope<half_t, false, 3>(p, gated, act, s);
+    case 4: return mx_slope<half_t, false, 4>(p, gated, act, s);
     default: return KSMM_ERR_BAD_ALGO;
     }
 }

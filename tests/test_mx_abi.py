@@ -107,8 +107,8 @@ def test_slopes_refuse(lib, dtype, gated):
     # what there is a kernel for is said without a launch
     for bs_last in (0, 1):
         assert call(dz=None, bs_last=bs_last) == 0
-        assert call(dz=None, bs_last=bs_last, d=2) == (0 if bs_last or dtype == 1 else ALGO)
-        assert call(dz=None, bs_last=bs_last, d=3) == (0 if bs_last else ALGO) and call(dz=None, bs_last=bs_last, c=2000) == ALGO
+        assert call(dz=None, bs_last=bs_last, d=2) == 0 and call(dz=None, bs_last=bs_last, d=3) == (0 if bs_last or dtype == 1 else ALGO)
+        assert call(dz=None, bs_last=bs_last, d=5) == (0 if bs_last else ALGO) and call(dz=None, bs_last=bs_last, c=2000) == ALGO
         assert call(bs_last=bs_last, c=2000) == ALGO
 
 
