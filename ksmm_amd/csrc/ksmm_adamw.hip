@@ -10,7 +10,10 @@
 // every run.  A v above zero never becomes zero.  New moments are computed in 64 bits, where the decision of a value next to
 // a border does not depend on the order of roundings; the weights take them in 32.
 //
-// What bounds it: HBM, 16 bytes a weight in fp16 with 8-bit moments and fp32 weights behind them, 28 in fp32.
+// What bounds it: HBM, 16 bytes a weight in fp16 with 8-bit moments and fp32 weights behind them, 28 in fp32.  10.9 million values of 72
+// tensors in fp32: 306 MB in 60-65 us, 4.7-5.1 TB/s; 14.4 million with 8-bit moments: 257 MB in 64, 4 TB/s, of which the vector ALU is
+// busy for half (64-bit moments, codes); what they stand for 25 us.  A value costs one read and one write of each tensor whatever
+// the order, so that all there is to choose is how many are on their way: eight a thread, vectors of 8 to 32 bytes.
 #include "ksmm_common.h"
 #include <algorithm>
 #include <cfloat>

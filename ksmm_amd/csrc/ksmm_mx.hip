@@ -6,6 +6,10 @@
 // Operands are kept as the a*d matrices that the products take, (a*d, rows, c) with c in blocks of 32, the last one filled
 // with zeros: 16 bytes of codes a block, the even place in the lower half of a byte, and a byte of scale.  That is what a lane
 // of the scaled matrix instructions holds: 32 numbers of one row and their scale.
+//
+// Here: conversions, the products of rows whose codes no workgroup's LDS holds, and the C entry points.  Conversions are bound by HBM:
+// 25088 x 384 in fp16 to codes 24.4 MB in 6.4 us and back in 7.6, 768 x 6501 in fp32 batch-size-last 8.4 and 7.4; of that 2 us are a
+// launch's start and end.
 #include "ksmm_mx_product.h"
 
 namespace ksmm {
@@ -219,6 +223,8 @@ __device__ __forceinline__ int8_v mx_operand(const uint8_t *codes, const uint8_t
     return r;
 }
 
+// Codes beyond LDS (c of 8500 and more): operands from the caches, x quantised in a launch before.  (1,512,9000,1) fp16: one row 38 us, 4096 rows
+// 139, 272 TF (c of 8000, which LDS holds: 20 and 81).
 // A wave computes 32 outputs of 32 rows: row 8j + 4(lane / 32) + i of the tile is an output, column lane % 32 a row of the batch.
 template <typename T, bool LAST, bool GATED, int ACT> __global__ __launch_bounds__(256) void ks_mx_product_kernel(MxProduct p)
 {
