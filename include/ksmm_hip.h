@@ -404,6 +404,9 @@ int ksmm_mx_quantize(const void *x, void *codes, void *scales, int64_t rows, int
 /* The values that codes stand for, rounded to `dtype` (fp16: what is below 6e-8 or beyond 65504 of them). */
 int ksmm_mx_dequantize(const void *codes, const void *scales, void *x, int64_t rows, int a, int c, int d, int dtype,
                        int bs_last, void *stream);
+/* Both operands of a product, x of `batch` rows and W of `rows` (in kernel format), in one launch: for its gradients. */
+int ksmm_mx_values(const void *x_codes, const void *x_scales, void *x, const void *w_codes, const void *w_scales, void *w,
+                   int64_t batch, int64_t rows, int a, int c, int d, int dtype, int bs_last, void *stream);
 /* y = act(W x + bias), W of b rows a block, or with `gated` act(G x + bias_g) * (U x + bias_u), W of 2*b rows a block, G's first,
  * and a bias of 2*a*b*d values as for ksmm_gated_forward.  x_scales NULL: x has `dtype` and is quantised in the call; else x and
  * x_scales are an operand of `batch` rows.  Sums are fp32; y and bias have `dtype`.  act: KSMM_ACT_SILU with `gated` only.

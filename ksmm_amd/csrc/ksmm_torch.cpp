@@ -818,8 +818,8 @@ struct MxNode : ag::Node {
             refuse_outside(next_edges(), stream);
             const int64_t features = (int64_t)how.a * how.c * how.d;
             at::Tensor x = at::empty(x_shape, dy.options()), w = at::empty({features, how.rows()}, dy.options());
-            check_status(ksmm_mx_dequantize(data_of(t[0]), data_of(t[1]), out_of(x), how.batch, how.a, how.c, how.d, dt, how.bs_last, stream));
-            check_status(ksmm_mx_dequantize(data_of(t[2]), data_of(t[3]), out_of(w), how.rows(), how.a * how.d, how.c, 1, dt, 1, stream));
+            check_status(ksmm_mx_values(data_of(t[0]), data_of(t[1]), out_of(x), data_of(t[2]), data_of(t[3]), out_of(w), how.batch, how.rows(), how.a, how.c, how.d, dt,
+                                        how.bs_last, stream));
             if (task_should_compute_output(0)) out[0] = at::empty(x_shape, dy.options());
             if (task_should_compute_output(1)) out[1] = at::empty_like(w);
             if (t[4].defined() && task_should_compute_output(2)) out[2] = at::empty_like(t[4]);

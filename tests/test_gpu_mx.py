@@ -615,3 +615,45 @@ def test_gradients_of_what_activations_are_applied_to(pattern, prec, bs_last):
             rc = _lib.load().ksmm_mx_slope(q.codes.data_ptr(), q.scales.data_ptr(), w.codes.data_ptr(), w.scales.data_ptr(), None, dy.cuda().data_ptr(), out.data_ptr(), n, a, b, c, d,
                                            0 if prec == "fp32" else 1, int(bs_last), 1, int(gated), torch.cuda.current_stream().cuda_stream)
             assert rc == 0 and torch.equal(out, got.flatten()) and (room[got.numel():] == 7).all()
+
+
+@pytest.mark.parametrize("bs_last", [False, True])
+@pytest.mark.parametrize("prec", ["fp32", "fp16"])
+@pytest.mark.parametrize("pattern", [(1, 1, 1, 1), (2, 5, 3, 2), (3, 33, 40, 1), (2, 20, 65, 3), (1, 100, 64, 6), (1, 9, 130, 4), (5, 34, 128, 8), (1, 8, 16, 37)])
+def test_both_operands_as_values(pattern, prec, bs_last):
+    from ksmm_amd import _lib, pack_mx, quantize_mx
+
+    a, b, c, d = pattern
+    for n, gated in ((1, False), (70, True), (517, False)):
+        q = quantize_mx(rows(n, a * c * d, bs_last, DT[prec], n).cuda(), (a, c, d), bs_last)
+        w = pack_mx(factor(pattern, gated, DT[prec]).cuda(), pattern, gated)
+        room = [torch.full((a * c * d * k + 64,), 7.0, dtype=DT[prec], device="cuda") for k in (n, w.codes.size(1))]
+        rc = _lib.load().ksmm_mx_values(q.codes.data_ptr(), q.scales.data_ptr(), room[0].data_ptr(), w.codes.data_ptr(), w.scales.data_ptr(), room[1].data_ptr(), n, w.codes.size(1),
+                                        a, c, d, 0 if prec == "fp32" else 1, int(bs_last), torch.cuda.current_stream().cuda_stream)
+        assert rc == 0
+        for got, want in zip(room, (q.dequantize(), w.dequantize(DT[prec]))):
+            assert torch.equal(got[:-64], want.flatten()) and (got[-64:] == 7).all()
+
+
+@pytest.mark.parametrize("bs_last", [False, True])
+def test_training_beyond_31_bits(bs_last):
+    """Gradients of almost 2^31 elements behind an activation: those of rows alone."""
+    from ksmm_amd import pack_mx, quantize_mx
+    from ksmm_amd.mx import _slope
+
+    pattern, n = (1, 64, 64, 1), (1 << 25) - 4096
+    w = pack_mx(factor(pattern, False, torch.float16).cuda(), pattern)
+    part, dpart = rows(100, 64, False, torch.float16).cuda(), rows(100, 64, False, torch.float16, 1).cuda()
+    x, dy = (torch.zeros((64, n) if bs_last else (n, 64), dtype=torch.float16, device="cuda") for _ in range(2))
+    for at in (0, n // 2 + 7, n - 100):
+        for whole, piece in ((x, part), (dy, dpart)):
+            if bs_last:
+                whole[:, at:at + 100] = piece.t()
+            else:
+                whole[at:at + 100] = piece
+    small, dsmall = ((t.t() if bs_last else t).contiguous() for t in (part, dpart))
+    want = _slope(dsmall, quantize_mx(small, (1, 64, 1), bs_last), w, None, "gelu", bs_last)
+    got = _slope(dy, quantize_mx(x, (1, 64, 1), bs_last), w, None, "gelu", bs_last)
+    for at in (0, n // 2 + 7, n - 100):
+        assert torch.equal(got[:, at:at + 100] if bs_last else got[at:at + 100], want)
+    assert not (got[:, 200:300] if bs_last else got[200:300]).any()

@@ -41,6 +41,28 @@ def test_conversions_refuse(lib, back, bs_last):
     assert call(x=codes + 16 * blocks - 1) == ALIAS and call(scales=codes + 16 * blocks - 1) == ALIAS
 
 
+@pytest.mark.parametrize("bs_last", [0, 1])
+def test_values_of_both_operands_refuse(lib, bs_last):
+    batch, rows, a, c, d = 10, 7, 2, 40, 3
+    names = ["x_codes", "x_scales", "x", "w_codes", "w_scales", "w"]
+    at = dict(zip(names, FAR))
+
+    def call(batch=batch, rows=rows, a=a, c=c, d=d, dtype=1, **change):
+        p = dict(at, **change)
+        return lib.ksmm_mx_values(*(p[k] for k in names), batch, rows, a, c, d, dtype, bs_last, None)
+
+    for k in names:
+        assert call(**{k: None}) == NULL
+    assert call(batch=0) == BATCH and call(rows=0) == BATCH and call(a=0) == PATTERN and call(d=0) == PATTERN and call(dtype=2) == DTYPE
+    assert call(batch=1 << 30) == LARGE and call(rows=1 << 30) == LARGE and call(a=1 << 20, d=1 << 20, c=1) == LARGE
+    assert call(x_codes=at["x_codes"] + 8) == WORKSPACE and call(w_codes=at["w_codes"] + 4) == WORKSPACE
+    sizes = {"x_codes": batch * a * d * 32, "x_scales": batch * a * d * 2, "w_codes": rows * a * d * 32, "w_scales": rows * a * d * 2}
+    for out, other in (("x", "w"), ("w", "x")):
+        for k in sizes:
+            assert call(**{out: at[k] + sizes[k] - 1}) == ALIAS
+        assert call(**{out: at[other] + 2}) == ALIAS
+
+
 @pytest.mark.parametrize("c", [40, 9000])
 def test_products_refuse(lib, c):
     n, a, b, d = 9, 2, 24, 3
