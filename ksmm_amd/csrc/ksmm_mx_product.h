@@ -156,6 +156,9 @@ constexpr int mx_rounds(int ks, int quarters) { return quarters == 1 ? (ks + 3) 
 // (1,768,192,2) gated takes 58 us for 64, in fp16 36 for 29.  (Of 16 steps the rounds would be too many to keep; blocks of three d_i that
 // end inside 32 are read three values at a time: (1,192,48,3) in fp16 27 us for 13.)
 template <typename T> constexpr int mx_quarters(bool last, int ks, int d) { return last || ks > 8 || (sizeof(T) == 2 && d != 3) ? 1 : 4; }
+// Rows that a lane reads together, batch-size-last: of 2-byte values two, 256 bytes a load instead of 128, where that leaves the producers
+// work ((1,192,768,2) 25088 rows 40.7 -> 35.2 us, (1,48,48,16) 32 -> 29; of three steps, 96 pairs a step for 256 threads, (1,768,192,2) 42.5 -> 44.5)
+template <typename T> constexpr int mx_pairs(bool last, int ks) { return last && sizeof(T) == 2 && (ks == 1 || ks > 4) ? 2 : 1; }
 constexpr int mx_ahead(int rounds, int registers)
 {
     int n = 64 / registers < 8 ? 64 / registers : 8;
@@ -244,7 +247,8 @@ template <typename T, int D, int G> __device__ __forceinline__ void mx_prepare(c
 template <typename T, bool LAST, int D, bool GATED, int ACT, int KS>
 __global__ __launch_bounds__(64 * (MX_CONSUMERS + MX_PRODUCERS)) void ks_mx_held_kernel(MxProduct p)
 {
-    constexpr int G = GATED ? 2 : 1, SB = mx_scale_bytes(KS), R = mx_rounds(KS, mx_quarters<T>(LAST, KS, D));
+    constexpr int G = GATED ? 2 : 1, SB = mx_scale_bytes(KS), P = mx_pairs<T>(LAST, KS), R = (mx_rounds(KS, mx_quarters<T>(LAST, KS, D)) + P - 1) / P;
+    constexpr int BLOCKS = LAST ? P : D;  // of a task: rows, or d_i of one
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     const int TN = p.tile_rows, buffer = D * TN * (p.slots * 16 + 2 * SB);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l32 = lane & 31, half = lane >> 5;
@@ -256,18 +260,18 @@ __global__ __launch_bounds__(64 * (MX_CONSUMERS + MX_PRODUCERS)) void ks_mx_held
     const int tile0 = blk / p.units * p.wave_tiles;
     float *const bias = (float *)(smem + 2 * buffer);
     uint8_t *const stage = smem + 2 * buffer + p.wave_tiles * G * D * 128 + wave * MX_STAGE;
-    const int tasks = TN * p.cb, batch = (int)p.batch, row_tiles = (int)p.token_tiles;  // (steps past the end are counted in 32 bits)
+    const int tasks = TN / P * p.cb, batch = (int)p.batch, row_tiles = (int)p.token_tiles;  // (steps past the end are counted in 32 bits)
     const int turns = p.codes_out ? p.splits : 0, mine = blk / p.units;  // (workgroups of the same rows hand out the codes in turn)
 
     // what a thread loads for the step of rows n0 on: the blocks of task t, or batch-size-first a quarter of them
     constexpr int Q = mx_quarters<T>(LAST, KS, D);
-    typedef std::conditional_t<Q == 1, MxGroup<T, D>, MxQuarter<T, D>> Load;
-    const MxDiv by(LAST ? TN : p.cb);
+    typedef std::conditional_t<Q == 1, MxGroup<T, BLOCKS>, MxQuarter<T, D>> Load;
+    const MxDiv by(LAST ? TN / P : p.cb);
     const int quarter = threadIdx.x & 3;  // (batch-size-first: a thread has the same of all its blocks)
     // row * 256 + kb of task t
     auto place = [&](int t) {
-        const int u = t / Q, v = by(u), rest = u - v * (LAST ? TN : p.cb);
-        return LAST ? rest * 256 + v : v * 256 + rest;
+        const int u = t / Q, v = by(u), rest = u - v * (LAST ? TN / P : p.cb);
+        return LAST ? rest * P * 256 + v : v * 256 + rest;
     };
     // rows that are not there: whatever LDS has, they are other columns of the product
     auto there = [&](int t, int at, int n0) { return t < tasks * Q && (at >> 8) < batch - n0; };
@@ -275,7 +279,7 @@ __global__ __launch_bounds__(64 * (MX_CONSUMERS + MX_PRODUCERS)) void ks_mx_held
         if (!there(t, at, n0)) return;
         const int n = at >> 8, kb = at & 255;
         if constexpr (LAST)
-            mx_load<T, 1>(f, (const T *)p.x + (((int64_t)ai * p.c + kb * 32) * p.d + d0) * p.batch + n0 + n, (int64_t)p.d * p.batch, p.c - kb * 32);
+            mx_load<T, P>(f, (const T *)p.x + (((int64_t)ai * p.c + kb * 32) * p.d + d0) * p.batch + (n0 + n < batch - P ? n0 + n : batch - P), (int64_t)p.d * p.batch, p.c - kb * 32);
         else if constexpr (Q == 1)
             mx_load<T, D>(f, (const T *)p.x + ((((int64_t)n0 + n) * p.a + ai) * p.c + kb * 32) * D, D, p.c - kb * 32);
         else
@@ -286,13 +290,15 @@ __global__ __launch_bounds__(64 * (MX_CONSUMERS + MX_PRODUCERS)) void ks_mx_held
         const int n = at >> 8, kb = at & 255;
         uint8_t *const codes = smem + which * buffer, *const scales = codes + D * TN * p.slots * 16;
 #pragma unroll
-        for (int j = 0; j < D; ++j) {
-            const int row = j * TN + n;
-            const int64_t block = (((int64_t)ai * p.d + d0 + j) * p.batch + n0 + n) * p.cb + kb;
+        for (int j = 0; j < BLOCKS; ++j) {
+            // (of two rows the last one of the batch goes with the one before it, which has been found once already, here or a step ago)
+            const int at_row = LAST ? (n < batch - n0 - P ? n : batch - n0 - P) + j : n, row = LAST ? at_row : j * TN + n;
+            if (P > 1 && row < 0) continue;
+            const int64_t block = (((int64_t)ai * p.d + d0 + (LAST ? 0 : j)) * p.batch + n0 + at_row) * p.cb + kb;
             int scale;
             if constexpr (Q == 1) {
                 uint4_t code;
-                scale = mx_quantize<T, D>(f, j, p.c - kb * 32, code);
+                scale = mx_quantize<T, BLOCKS>(f, j, p.c - kb * 32, code);
                 *(uint4_t *)(codes + (row * p.slots + kb) * 16) = code;
                 if (emit) *(uint4_t *)(p.codes_out + block * 16) = code;
             } else {
@@ -311,7 +317,7 @@ __global__ __launch_bounds__(64 * (MX_CONSUMERS + MX_PRODUCERS)) void ks_mx_held
 
     if (wave >= MX_CONSUMERS) {
         const int t0 = threadIdx.x - 64 * MX_CONSUMERS;
-        constexpr int AHEAD = mx_ahead(R, D * (int)sizeof(T) * 8 / Q);
+        constexpr int AHEAD = mx_ahead(R, BLOCKS * (int)sizeof(T) * 8 / Q);
         Load f[AHEAD];
         int at[R];
 #pragma unroll
@@ -438,14 +444,20 @@ template <typename T, bool LAST, int D, int TT, bool GATED, int ACT> __global__ 
             keep(j, n, kb, *(const uint4_t *)((const uint8_t *)p.x + block * 16), p.x_scales[block], false);
         }
     } else if constexpr (LAST) {
-        for (int t = threadIdx.x; t < TN * p.cb; t += 64 * MX_WAVES) {
-            const int kb = t / TN, n = t - kb * TN;
+        constexpr int P = TT == 1 ? 1 : mx_pairs<T>(true, 16);  // ((1,1024,1024,1) fp16, 25088 rows 86 -> 60 us)
+        for (int t = threadIdx.x; t < TN / P * p.cb; t += 64 * MX_WAVES) {
+            const int kb = t / (TN / P), n = (t - kb * (TN / P)) * P;
             if (n >= here) continue;  // (whatever LDS has there, it is another column of the product)
-            MxGroup<T, 1> g;
-            mx_load<T, 1>(g, (const T *)p.x + (((int64_t)ai * p.c + kb * 32) * p.d + d0) * p.batch + n0 + n, (int64_t)p.d * p.batch, p.c - kb * 32);
-            uint4_t code;
-            const int scale = mx_quantize<T, 1>(g, 0, p.c - kb * 32, code);
-            keep(0, n, kb, code, scale, emit);
+            // (of two rows the last one of the batch goes with the one before it)
+            const int first = n < here - P ? n : here - P;
+            MxGroup<T, P> g;
+            mx_load<T, P>(g, (const T *)p.x + (((int64_t)ai * p.c + kb * 32) * p.d + d0) * p.batch + n0 + first, (int64_t)p.d * p.batch, p.c - kb * 32);
+#pragma unroll
+            for (int j = 0; j < P; ++j) {
+                uint4_t code;
+                const int scale = mx_quantize<T, P>(g, j, p.c - kb * 32, code);
+                if (P == 1 || first + j >= 0) keep(0, first + j, kb, code, scale, emit);
+            }
         }
     } else if constexpr (D > 0) {
         constexpr int SIZE = 2 * D * (int)sizeof(T), TIMES = 64 / SIZE < 4 ? 64 / SIZE : 4;  // (64 registers of values on their way)
@@ -716,8 +728,8 @@ inline int64_t mx_held_splits(const MxProduct &p, int a_unit)
 
 template <typename T, bool LAST, int D, bool GATED, int KS> int mx_launch_held(MxProduct p, int act, hipStream_t s)
 {
-    constexpr int Q = mx_quarters<T>(LAST, KS, D);
-    mx_held_sizes(p, LAST, MX_CONSUMERS, 64 * MX_PRODUCERS * mx_rounds(KS, Q) / Q);
+    constexpr int Q = mx_quarters<T>(LAST, KS, D), P = mx_pairs<T>(LAST, KS);
+    mx_held_sizes(p, LAST, MX_CONSUMERS, 64 * MX_PRODUCERS * P * ((mx_rounds(KS, Q) + P - 1) / P) / Q);
     int64_t most = mx_held_splits(p, 1);
     if (p.token_tiles > most && mx_held_lds(D, GATED, KS, p.cb, p.tile_rows, p.wave_tiles, MX_CONSUMERS) <= 80 * 1024) {
         with_act(act, [&](auto which) {
@@ -766,7 +778,7 @@ template <typename T, bool LAST, int D, bool GATED> int mx_pick(const MxProduct 
     if constexpr (D > 0) {
         // fewer than these are done sooner by workgroups of one step, which all begin at once: (1,768,192,2) gated fp16 of 32 rows in 4.9 us
         // for 7.2, of 1000 in 6.6 for 7.8; with 252 of them 4000 rows of (2,96,72,3) in fp32 take 9.4 for 8.2
-        if (groups(32) > 192) {
+        if (groups(32) > 192 && p.batch >= mx_pairs<T>(LAST, 1)) {
             const int rc = mx_held<T, LAST, D, GATED, 1, 2, 3, 4, 6, 8, 16>(p, act, s);
             if (rc != KSMM_ERR_BAD_ALGO) return rc;
         }
@@ -774,7 +786,7 @@ template <typename T, bool LAST, int D, bool GATED> int mx_pick(const MxProduct 
     // twice the rows for the same weights, where that leaves a workgroup for a compute unit without splits, or there are many more weights than x
     // ((1,1536,384,2) gated fp16 of 3136 rows 35 -> 28 us, (1,128,128,8) 12 -> 17)
     const bool many = (p.batch + 63) / 64 * p.a * ((p.d + unit - 1) / unit) >= 256, heavy = (GATED ? 2 : 1) * p.b >= 256 * (int)sizeof(T) && groups(64) >= 256;
-    if ((many || heavy) && mx_wide_lds(2, p.c, p.d, (int)sizeof(T), LAST) <= MX_LDS_MOST) return mx_launch_wide<T, LAST, D, 2, GATED>(p, act, s);
+    if (p.batch > 32 && (many || heavy) && mx_wide_lds(2, p.c, p.d, (int)sizeof(T), LAST) <= MX_LDS_MOST) return mx_launch_wide<T, LAST, D, 2, GATED>(p, act, s);
     return mx_launch_wide<T, LAST, D, 1, GATED>(p, act, s);
 }
 

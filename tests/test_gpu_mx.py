@@ -657,3 +657,19 @@ def test_training_beyond_31_bits(bs_last):
     for at in (0, n // 2 + 7, n - 100):
         assert torch.equal(got[:, at:at + 100] if bs_last else got[at:at + 100], want)
     assert not (got[:, 200:300] if bs_last else got[200:300]).any()
+
+
+@pytest.mark.parametrize("prec", ["fp32", "fp16"])
+@pytest.mark.parametrize("pattern", [(200, 4, 4, 1), (300, 4, 4, 1), (1, 40, 48, 200), (1, 40, 3000, 270), (1, 300, 1030, 1), (2, 70, 600, 1)])
+def test_last_rows_of_the_batch_feature_major(pattern, prec):
+    """One row, and odd numbers of them: rows that are read in pairs."""
+    from ksmm_amd import MXKernel, mx_linear, pack_mx, quantize_mx
+
+    a, b, c, d = pattern
+    for n in (1, 2, 3, 31, 33, 65, 129) + ((257,) if a * c * d < 100000 else ()) + ((12801, 16385) if a * c * d < 1100 else ()):
+        x = rows(n, a * c * d, True, DT[prec], n).cuda()
+        w, q = pack_mx(factor(pattern, False, DT[prec]).cuda(), pattern), quantize_mx(x, (a, c, d), True)
+        y, codes, scales = MXKernel.forward(x, w, None, None, True, need_codes=True)
+        assert torch.equal(codes, q.codes) and torch.equal(scales, q.scales) and torch.equal(y, mx_linear(q, w, bs_last=True))
+        want = R.product(R.rounded(R.operand(x[:, -3:].contiguous(), a, c, d, True)), R.rounded(factor_rows(factor(pattern, False, DT[prec]), pattern)), None, pattern, None, False, True)
+        assert rel(y[:, -3:], R.tensor(want, (a * b * d, min(n, 3)), True)) <= TOL[prec]
