@@ -11,9 +11,10 @@
 // a border does not depend on the order of roundings; the weights take them in 32.
 //
 // What bounds it: HBM, 16 bytes a weight in fp16 with 8-bit moments and fp32 weights behind them, 28 in fp32.  10.9 million values of 72
-// tensors in fp32: 306 MB in 60-65 us, 4.7-5.1 TB/s; 14.4 million with 8-bit moments: 257 MB in 64, 4 TB/s, of which the vector ALU is
+// tensors in fp32: 306 MB in 61 us, 5.0 TB/s; 14.4 million with 8-bit moments: 257 MB in 63, 4.1 TB/s, of which the vector ALU is
 // busy for half (64-bit moments, codes); what they stand for 25 us.  A value costs one read and one write of each tensor whatever
-// the order, so that all there is to choose is how many are on their way: eight a thread, vectors of 8 to 32 bytes.
+// the order, so that all there is to choose is how many are on their way: four a thread, vectors of 4 to 16
+// bytes (eight: 65 us for 61, and 64.5 for 63).
 #include "ksmm_common.h"
 #include <algorithm>
 #include <cfloat>
@@ -25,7 +26,7 @@ namespace ksmm {
 
 namespace {
 
-constexpr int PER = 8;                    // values a thread takes at a time
+constexpr int PER = 4;                    // values a thread takes at a time
 
 struct Tensor {
     void *w;
@@ -61,7 +62,7 @@ template <bool MASTER, bool SCALES> struct Entry {
 };
 struct Common {
     int count;
-    uint32_t chunk;  // values a workgroup takes: of 256 threads two of 8 each, or where that makes few, of 64 threads one of 8 each
+    uint32_t chunk;  // values a workgroup takes: 256 threads' once (8-bit moments: twice), or where that makes few, of 64 threads
     uint32_t seed;  // the first tensor's
     int follow;
     float keep, rate, root, eps;  // rate, root: of the step, or (with `device_step`) to be found from it
@@ -121,11 +122,12 @@ __device__ __forceinline__ float scale_value(uint8_t byte)
     return byte ? __builtin_bit_cast(float, (uint32_t)byte << 23) : __builtin_bit_cast(float, 0x00400000u);
 }
 
-// largest of the four lanes that hold a block of 32
+// largest of the eight lanes that hold a block of 32
 __device__ __forceinline__ int block_max(int v)
 {
     v = max(v, __builtin_amdgcn_mov_dpp(v, 0xb1, 0xf, 0xf, true));  // lanes 1 0 3 2
-    return max(v, __builtin_amdgcn_mov_dpp(v, 0x4e, 0xf, 0xf, true));  // 2 3 0 1
+    v = max(v, __builtin_amdgcn_mov_dpp(v, 0x4e, 0xf, 0xf, true));  // 2 3 0 1
+    return max(v, __builtin_amdgcn_mov_dpp(v, 0x141, 0xf, 0xf, true));  // 7 6 5 4 3 2 1 0: the other four's
 }
 
 constexpr int LOWEST = -120;  // exponent of a scale
@@ -145,7 +147,7 @@ __device__ __forceinline__ uint32_t rounded(double y, int exponent, int e, int l
 __device__ __forceinline__ float from_e5m3(uint8_t code) { return (float)__builtin_bit_cast(half_t, (uint16_t)(code << 7)); }
 __device__ __forceinline__ float from_e4m3(uint8_t code) { return __builtin_amdgcn_cvt_f32_fp8(code, 0); }
 
-// A block's new moments as codes, and its scale; every lane of the four has eight of its values.  What is 2^128 or more, or NaN, is not
+// A block's new moments as codes, and its scale; every lane of the eight has four of its values.  What is 2^128 or more, or NaN, is not
 // counted among the largest.
 __device__ __forceinline__ uint8_t encode_m(const double (&m)[PER], const uint32_t (&h)[PER], Values<uint8_t> &code)
 {
@@ -321,7 +323,8 @@ template <typename E, typename F> int in_tables(const Common &common, const Tens
     for (int i = 0; i < n; ++i) values += all[i].n;
     // (172 thousand 8-bit values of 25 tensors: 10.6 us in workgroups of 256 threads)
     const int threads = values < 1 << 20 ? 64 : 256;
-    a.chunk = threads == 64 ? 64 * PER : 256 * PER * 2;
+    // (28 bytes a value: 61 us once, 62.6 twice, 67 four times; 8-bit moments 95, 90.5 and 95 with the launch that gives them back)
+    a.chunk = threads * PER * (threads == 256 && E::HAS_SCALES ? 2 : 1);
     a.count = 0;
     for (int i = 0; i <= n; ++i) {
         const uint32_t more = i < n ? (all[i].n + a.chunk - 1) / a.chunk : 0;
