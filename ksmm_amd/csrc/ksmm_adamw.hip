@@ -11,10 +11,10 @@
 // a border does not depend on the order of roundings; the weights take them in 32.
 //
 // What bounds it: HBM, 16 bytes a weight in fp16 with 8-bit moments and fp32 weights behind them, 28 in fp32.  10.9 million values of 72
-// tensors in fp32: 306 MB in 61 us, 5.0 TB/s; 14.4 million with 8-bit moments: 257 MB in 63, 4.1 TB/s, of which the vector ALU is
-// busy for half (64-bit moments, codes); what they stand for 25 us.  A value costs one read and one write of each tensor whatever
+// tensors in fp32: 306 MB in 61 us, 5.0 TB/s; 14.4 million with 8-bit moments: 257 MB in 64, 4 TB/s, of which the vector ALU is
+// busy for half (64-bit moments, codes); what they stand for 23 us.  A value costs one read and one write of each tensor whatever
 // the order, so that all there is to choose is how many are on their way: four a thread, vectors of 4 to 16
-// bytes (eight: 65 us for 61, and 64.5 for 63).
+// bytes (eight: 65 us for 61, the same for 64, 25 for 23).
 #include "ksmm_common.h"
 #include <algorithm>
 #include <cfloat>
@@ -395,7 +395,8 @@ int ksmm_adamw_update(const ksmm_adamw_desc *desc, const ksmm_adamw_tensor *tens
             add(ranges, t.m, state, true);
             add(ranges, t.v, state, true);
             if (small) add(ranges, t.scales, 2 * ((t.n + 31) / 32), true);
-            const bool vectors = aligned(t.weight, 16) && aligned(t.grad, 16) && aligned(t.master, 16) && aligned(t.m, small ? 8 : 16) && aligned(t.v, small ? 8 : 16);
+            const bool vectors = aligned(t.weight, PER * (int)size) && aligned(t.grad, PER * (int)size) && aligned(t.master, PER * 4) && aligned(t.m, small ? PER : PER * 4) &&
+                                 aligned(t.v, small ? PER : PER * 4);
             all.push_back(Tensor{t.weight, t.grad, t.master, t.m, t.v, (uint8_t *)t.scales, (uint32_t)t.n, vectors ? 0x80000000u : 0u});
         }
         if (any_alias(ranges)) return KSMM_ERR_ALIAS;
@@ -450,7 +451,7 @@ int ksmm_adamw_moments(const ksmm_adamw_moment *tensors, int count, void *stream
             add(ranges, t.scales, 2 * ((t.n + 31) / 32), false);
             add(ranges, t.m_out, 4 * t.n, true);
             add(ranges, t.v_out, 4 * t.n, true);
-            const bool vectors = aligned(t.m, 8) && aligned(t.v, 8) && aligned(t.m_out, 16) && aligned(t.v_out, 16);
+            const bool vectors = aligned(t.m, PER) && aligned(t.v, PER) && aligned(t.m_out, PER * 4) && aligned(t.v_out, PER * 4);
             all.push_back(Tensor{t.m_out, nullptr, t.v_out, (void *)t.m, (void *)t.v, (uint8_t *)t.scales, (uint32_t)t.n, vectors ? 0x80000000u : 0u});
         }
         if (any_alias(ranges)) return KSMM_ERR_ALIAS;
