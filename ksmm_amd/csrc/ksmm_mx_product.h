@@ -675,7 +675,7 @@ template <typename T, bool LAST, int D, int TT, bool GATED> int mx_launch_wide(M
         constexpr int ACT = decltype(which)::value;
         if constexpr (GATED || ACT != KSMM_ACT_SILU) {
             auto fn = &ks_mx_wide_kernel<T, LAST, D, TT, GATED, ACT>;
-            if (lds > 64 * 1024) rc = ensure_dynamic_lds((const void *)fn, lds);
+            if (lds > 64 * 1024) rc = ensure_dynamic_lds((const void *)fn, (int)MX_LDS_ALL);  // (set once a kernel: for all of its sizes)
             if (rc != KSMM_OK) return;
             hipLaunchKernelGGL(fn, dim3((unsigned)grid), dim3(64 * MX_WAVES), lds, s, p);
             if (hipGetLastError() != hipSuccess) rc = KSMM_ERR_LAUNCH;
@@ -749,7 +749,7 @@ template <typename T, bool LAST, int D, bool GATED, int KS> int mx_launch_held(M
         constexpr int ACT = decltype(which)::value;
         if constexpr (GATED || ACT != KSMM_ACT_SILU) {
             auto fn = &ks_mx_held_kernel<T, LAST, D, GATED, ACT, KS>;
-            if (lds > 64 * 1024) rc = ensure_dynamic_lds((const void *)fn, lds);
+            if (lds > 64 * 1024) rc = ensure_dynamic_lds((const void *)fn, (int)MX_LDS_ALL);  // (set once a kernel: for all of its sizes)
             if (rc != KSMM_OK) return;
             hipLaunchKernelGGL(fn, dim3((unsigned)grid), dim3(64 * (MX_CONSUMERS + MX_PRODUCERS)), lds, s, p);
             if (hipGetLastError() != hipSuccess) rc = KSMM_ERR_LAUNCH;

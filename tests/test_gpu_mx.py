@@ -673,3 +673,16 @@ def test_last_rows_of_the_batch_feature_major(pattern, prec):
         assert torch.equal(codes, q.codes) and torch.equal(scales, q.scales) and torch.equal(y, mx_linear(q, w, bs_last=True))
         want = R.product(R.rounded(R.operand(x[:, -3:].contiguous(), a, c, d, True)), R.rounded(factor_rows(factor(pattern, False, DT[prec]), pattern)), None, pattern, None, False, True)
         assert rel(y[:, -3:], R.tensor(want, (a * b * d, min(n, 3)), True)) <= TOL[prec]
+
+
+@pytest.mark.parametrize("bs_last", [False, True])
+def test_local_memory_of_a_kernel_grows_from_call_to_call(bs_last):
+    """The same kernel with 70, 100 and 150 KB of it, in that order."""
+    from ksmm_amd import mx_linear, pack_mx
+
+    for c in (2100 if bs_last else 3200, 5000, 7200 if bs_last else 8000):
+        pattern = (1, 24, c, 1)
+        x, f = rows(9, c, bs_last, torch.float32, 1), factor(pattern, True, torch.float32)
+        y = mx_linear(x.cuda(), pack_mx(f.cuda(), pattern, True), act="gelu", bs_last=bs_last)
+        want = R.product(R.rounded(R.operand(x, 1, c, 1, bs_last)), R.rounded(factor_rows(f, pattern)), None, pattern, "gelu", True, bs_last)
+        assert rel(y, R.tensor(want, y.shape, bs_last)) <= 6e-6
