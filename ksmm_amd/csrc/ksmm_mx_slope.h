@@ -7,6 +7,9 @@
 // registers: eight waves (four) multiply and store, four bring the next step's codes of x and its dy into LDS, as they lie.
 // What bounds it: HBM.  (1,768,192,2) gated in fp16, 25088 rows: 236 MB in 46 us, 5.1 TB/s, what a copy reaches; the kernel that multiplies
 // the values in fp16 once more takes 80.
+// dz has the tensors' type, as gradients between two layers have: in fp16 it is rounded before dx, dW and dbias sum it, 2.9e-4 off
+// (rms) for 2.1e-4 of one rounding alone.  In 32 bits its traffic would be 390 MB for 236, and dx and dW, 115 us of a pass, were on fp32
+// matrix cores, at an eighth of the rate.
 #pragma once
 #include "ksmm_mx_product.h"
 
