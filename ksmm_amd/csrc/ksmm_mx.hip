@@ -234,9 +234,9 @@ template <typename T, int D> __global__ __launch_bounds__(THREADS) void ks_mx_va
     if constexpr (D == 0) {
         mx_columns<T, true>(x, group);
     } else {
-        if (x.d == D)
+        if (D == 3 || x.d == D)
             mx_rows<T, D, true>(x, group, groups);
-        else
+        else if constexpr (D != 3)
             mx_runs<T, D, true>(x, group, groups);
     }
 }
@@ -305,9 +305,9 @@ int64_t groups_of(const MxOperand &p)
 }
 template <typename T, int D, bool BACK> int convert_rows(const MxOperand &p, hipStream_t s)
 {
-    if (p.d == D)
+    if (D == 3 || p.d == D)  // (never three of more)
         hipLaunchKernelGGL((ks_mx_rows_kernel<T, D, BACK>), dim3((unsigned)groups_of(p)), dim3(THREADS), 0, s, p);
-    else
+    else if constexpr (D != 3)
         hipLaunchKernelGGL((ks_mx_runs_kernel<T, D, BACK>), dim3((unsigned)groups_of(p)), dim3(THREADS), 0, s, p);
     return launched();
 }
