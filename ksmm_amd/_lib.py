@@ -14,6 +14,7 @@ KSMM_F32, KSMM_F16, KSMM_FP8_E4M3 = 0, 1, 2
 ALGO_AUTO, ALGO_GENERIC, ALGO_WAVE, ALGO_TILE = 0, 1, 2, 3
 MAX_FACTORS = 16
 ACT_NONE, ACT_GELU, ACT_SILU = 0, 1, 2
+ERR_LAUNCH = -7
 NORM_RMS, NORM_LAYER = 0, 1
 ABI_VERSION = 2
 

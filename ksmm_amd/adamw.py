@@ -46,8 +46,11 @@ def adamw_update(params, grads, exp_avgs, exp_avg_sqs, scales=None, masters=None
     What a NaN or an infinity among the gradients reaches is its own element alone."""
     if len(betas) != 2:
         raise ValueError("betas must be two values from 0 on and below 1, not %s" % (betas,))
-    if _lib.native().adamw_update(params, grads, exp_avgs, exp_avg_sqs, scales, masters, step, lr, betas[0], betas[1], eps, weight_decay,
-                                  grad_scale, seed, follow):
+    done = _lib.native().adamw_update(params, grads, exp_avgs, exp_avg_sqs, scales, masters, step, lr, betas[0], betas[1], eps, weight_decay,
+                                      grad_scale, seed, follow)
+    if done is not None:
+        if done is not True:  # a launch failed: others may have been made, and a second call would update their tensors twice
+            _lib.check(done)
         return
     lib = _lib.load()
     params, grads = [p.detach() for p in params], [g.detach() for g in grads]
@@ -84,8 +87,10 @@ def adamw_update(params, grads, exp_avgs, exp_avg_sqs, scales=None, masters=None
     desc = _lib.KsmmAdamwDesc(lr, betas[0], betas[1], eps, weight_decay, grad_scale, 1 if on_device else int(step),
                               step.data_ptr() if on_device else None, seed & 0xffffffff, 8 if small else 32, int(follow))
     with torch.cuda.device(like.device):
-        _lib.check(lib.ksmm_adamw_update(ctypes.byref(desc), table, len(params), dtype_code(like.dtype), _stream_ptr(like)))
-    _written(*params, *exp_avgs, *exp_avg_sqs, *(scales or ()), *(masters or ()))
+        status = lib.ksmm_adamw_update(ctypes.byref(desc), table, len(params), dtype_code(like.dtype), _stream_ptr(like))
+    if status in (0, _lib.ERR_LAUNCH):  # (of several launches some may have been made)
+        _written(*params, *exp_avgs, *exp_avg_sqs, *(scales or ()), *(masters or ()))
+    _lib.check(status)
 
 
 def adamw_moments(exp_avgs, exp_avg_sqs, scales):

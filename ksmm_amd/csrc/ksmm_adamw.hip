@@ -93,7 +93,7 @@ template <typename E> __device__ __forceinline__ int tensor_of(const Args<E> &a,
 template <typename T> struct Values {
     T v[PER];
 };
-// values at .. at + 7, as far as they are there; `whole`: all of them, at a vector's alignment
+// values at .. at + 3, as far as they are there; `whole`: all of them, at a vector's alignment
 template <typename T> __device__ __forceinline__ Values<T> load(const T *p, uint32_t at, uint32_t n, bool whole)
 {
     Values<T> r;
@@ -331,8 +331,10 @@ template <typename E, typename F> int in_tables(const Common &common, const Tens
         // (a table's workgroups are counted in 31 bits)
         if (a.count > 0 && (i == n || a.count == Args<E>::MOST || (uint64_t)groups + more > 0x7fffffffu)) {
             a.seed = seed + (uint32_t)first;
-            launch(a, groups, threads);
-            if (hipGetLastError() != hipSuccess) return KSMM_ERR_LAUNCH;
+            if (groups > 0) {
+                const int rc = launch(a, groups, threads);
+                if (rc != KSMM_OK) return rc;
+            }
             groups = 0;
             a.count = 0;
         }
@@ -419,7 +421,7 @@ int ksmm_adamw_update(const ksmm_adamw_desc *desc, const ksmm_adamw_tensor *tens
             typedef decltype(of) T;
             constexpr bool MASTER = decltype(masters)::value, SMALL = decltype(states)::value;
             return in_tables<Entry<MASTER, SMALL>>(a, all.data(), count, [&](const Args<Entry<MASTER, SMALL>> &args, uint32_t groups, int threads) {
-                if (groups > 0) hipLaunchKernelGGL((ks_adamw_kernel<T, SMALL ? 8 : 32, MASTER>), dim3(groups), dim3(threads), 0, s, args);
+                return launch_kernel(&ks_adamw_kernel<T, SMALL ? 8 : 32, MASTER>, groups, threads, 0, s, args);
             });
         };
         auto with = [&](auto of) {
@@ -457,7 +459,7 @@ int ksmm_adamw_moments(const ksmm_adamw_moment *tensors, int count, void *stream
         if (any_alias(ranges)) return KSMM_ERR_ALIAS;
         Common a{};
         return in_tables<Entry<true, true>>(a, all.data(), count, [&](const Args<Entry<true, true>> &args, uint32_t groups, int threads) {
-            if (groups > 0) hipLaunchKernelGGL(ks_adamw_moments_kernel, dim3(groups), dim3(threads), 0, (hipStream_t)stream, args);
+            return launch_kernel(&ks_adamw_moments_kernel, groups, threads, 0, (hipStream_t)stream, args);
         });
     } catch (...) {
         return KSMM_ERR_TOO_LARGE;

@@ -86,6 +86,19 @@ static inline size_t dtype_size(int dt)
     return dt == KSMM_F32 ? 4 : dt == KSMM_F16 ? 2 : 1;
 }
 
+// A launch and its own status: hipGetLastError() would also give, and clear, what an earlier call on the thread left behind.
+template <typename P> struct SameType {
+    typedef P type;
+};
+template <typename... P>
+static inline int launch_kernel(void (*fn)(P...), unsigned groups, unsigned threads, size_t lds, hipStream_t s, const typename SameType<P>::type &...p)
+{
+    void *args[] = {(void *)&p...};
+    if (hipLaunchKernel((const void *)fn, dim3(groups), dim3(threads), args, lds, s) == hipSuccess) return KSMM_OK;
+    (void)hipGetLastError();  // (it is told here)
+    return KSMM_ERR_LAUNCH;
+}
+
 // One factor problem, as the launchers see it.
 struct Problem {
     const void *x;

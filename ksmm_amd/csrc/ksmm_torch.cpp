@@ -954,7 +954,7 @@ bool holds(const at::Tensor &t, int64_t n, at::ScalarType type, const at::Device
 int64_t moment_scales(int64_t n) { return 2 * ((n + 31) / 32); }
 
 // adamw_update(params, grads, exp_avgs, exp_avg_sqs, scales, masters, step, lr, beta1, beta2, eps, weight_decay, grad_scale, seed, follow)
-// -> True or None
+// -> True, None, or the status of a launch that failed: tensors may have been updated by then, and the call is not to be made again
 PyObject *py_adamw_update(PyObject *, PyObject *const *args, Py_ssize_t n_args)
 {
     if (n_args != 15) {
@@ -1010,11 +1010,12 @@ PyObject *py_adamw_update(PyObject *, PyObject *const *args, Py_ssize_t n_args)
                 DeviceScope scope(p[0].device().index());
                 status = ksmm_adamw_update(&d, table.data(), (int)n, code_of(p[0].scalar_type()), stream_of(p[0]));
             }
-            if (status == KSMM_OK) {
+            if (status == KSMM_OK || status == KSMM_ERR_LAUNCH) {
                 for (const auto *list : {&p, &m, &v, &s, &w})
                     for (const at::Tensor &t : *list)
                         if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
-                Py_RETURN_TRUE;
+                if (status == KSMM_OK) Py_RETURN_TRUE;
+                return PyLong_FromLong(status);
             }
         }
     } catch (const std::exception &) {
