@@ -16,7 +16,7 @@ import torch
 from torch import nn
 
 from . import _lib
-from .block import GATED_ACTS, GatedKernel, KSFeedForward, KSGatedLinear, _ptr, _same, _trainable_type
+from .block import GATED_ACTS, GatedKernel, KSFeedForward, KSGatedLinear, _ptr, _trainable_type, _written
 from .kernel import Kernel, _check_input, _stream_ptr, dtype_code
 from .layer import KSLinear
 
@@ -189,7 +189,8 @@ class MXKernel:
         bs_last = bool(bs_last)
         a, b, c, d = factor.pattern
         batch, dtype, shape = _check_product(x, factor.device, factor.pattern, bias, act, factor.gated, bs_last)
-        if out is None:
+        given = out is not None
+        if not given:
             out = torch.empty(shape, dtype=dtype, device=x.device)
         elif tuple(out.shape) != tuple(shape) or out.dtype != dtype or out.device != x.device or not out.is_contiguous():
             raise ValueError("out must be a contiguous %s of shape %s" % (dtype, tuple(shape)))
@@ -217,6 +218,8 @@ class MXKernel:
                 workspace.data_ptr() if need > 0 else None,
                 workspace.numel() * workspace.element_size() if need > 0 else 0, batch, a, b, c, d, dt, int(bs_last), GATED_ACTS[act],
                 int(factor.gated), _stream_ptr(out)))
+        if given:
+            _written(out)
         return (out, codes, scales) if need_codes else out
 
 
