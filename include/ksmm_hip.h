@@ -417,6 +417,11 @@ int ksmm_mx_forward(const void *x, const void *x_scales, const void *w, const vo
                     void *codes_out, void *scales_out, void *workspace, int64_t workspace_bytes, int64_t batch, int a,
                     int b, int c, int d, int dtype, int bs_last, int act, int gated, void *stream);
 
+/* z = W x + bias of one factor, what its activation was applied to, rounded to `dtype`, in fp16 to 65504 at most: beyond it an activation
+ * has the slope that it has there, where that of an infinity is none.  Operands as above. */
+int ksmm_mx_sums(const void *x, const void *x_scales, const void *w, const void *w_scales, const void *bias, void *z, int64_t batch, int a,
+                 int b, int c, int d, int dtype, int bs_last, void *stream);
+
 /* Gradients of what the activation was applied to, which is computed again from the operands' codes: with `gated` dz of 2*b rows a block,
  * dy u act'(g) and dy act(g) in G's and U's places, else dy act'(z), rounded to `dtype`; they are those of a layer of the pattern
  * (a, 2*b or b, c, d) without an activation.  KSMM_ERR_BAD_ALGO: there is no kernel for the pattern (batch-size-first

@@ -136,6 +136,7 @@ SIGNATURES = {
     "ksmm_mx_forward": (c_int, [c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_i64, c_i64, c_int, c_int, c_int, c_int, c_int, c_int,
                                 c_int, c_int, c_vp]),
     "ksmm_mx_values": (c_int, [c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_i64, c_i64, c_int, c_int, c_int, c_int, c_int, c_vp]),
+    "ksmm_mx_sums": (c_int, [c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_i64, c_int, c_int, c_int, c_int, c_int, c_int, c_vp]),
     "ksmm_mx_slope": (c_int, [c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_i64, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_vp]),
     "ksmm_adamw_update": (c_int, [ctypes.POINTER(KsmmAdamwDesc), ctypes.POINTER(KsmmAdamwTensor), c_int, c_int, c_vp]),
     "ksmm_adamw_moments": (c_int, [ctypes.POINTER(KsmmAdamwMoment), c_int, c_vp]),

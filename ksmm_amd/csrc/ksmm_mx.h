@@ -211,6 +211,7 @@ struct MxProduct {
     const void *bias;
     void *y;
     const void *dy;  // (gradients only)
+    bool finite;     // of codes, without an activation: results beyond the type's range are its largest (gradients only)
     int64_t batch;
     int a, b, c, d, cb;
     int slots;                    // of 16 bytes in LDS for a row's codes, odd

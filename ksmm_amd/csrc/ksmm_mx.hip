@@ -288,6 +288,8 @@ template <typename T, bool LAST, bool GATED, int ACT> __global__ __launch_bounds
         if (o >= p.b) continue;
         float z = acc[i];
         if (bias) z += (float)bias[((int64_t)ai * rows_w + o) * p.d + di];
+        if constexpr (!GATED && ACT == KSMM_ACT_NONE && sizeof(T) == 2)
+            if (p.finite) z = mx_within_half(z);
         z = mx_act<T, GATED, ACT>(z);
         if constexpr (GATED) z *= up[i] + (bias ? (float)bias[((int64_t)ai * rows_w + p.b + o) * p.d + di] : 0.f);
         if constexpr (sizeof(T) == 2) asm("" : "+v"(z));
@@ -350,8 +352,11 @@ template <typename T, bool LAST, bool GATED> int product(const MxProduct &p, int
     });
     return launched();
 }
-template <typename T> int product(const MxProduct &p, bool last, bool gated, int act, hipStream_t s)
+template <typename T> int product(MxProduct p, bool last, bool gated, int act, hipStream_t s)
 {
+    p.b_tiles = (p.b + 31) / 32;
+    p.token_tiles = (p.batch + 31) / 32;
+    p.tiles = (int64_t)p.a * p.d * p.b_tiles * p.token_tiles;
     if (last) return gated ? product<T, true, true>(p, act, s) : product<T, true, false>(p, act, s);
     return gated ? product<T, false, true>(p, act, s) : product<T, false, false>(p, act, s);
 }
@@ -448,6 +453,16 @@ int64_t ksmm_mx_forward_workspace(int64_t batch, int a, int b, int c, int d, int
     return align256(blocks * 16) + align256(blocks);
 }
 
+// the product of an operand, or of values whose codes LDS holds
+static int launch_product(const MxProduct &p, int dtype, bool last, bool gated, int act, hipStream_t s)
+{
+    static int (*const fused[2][2][2])(const MxProduct &, int, hipStream_t) = {
+        {{mx_half_first_plain, mx_half_first_gated}, {mx_half_last_plain, mx_half_last_gated}},
+        {{mx_float_first_plain, mx_float_first_gated}, {mx_float_last_plain, mx_float_last_gated}}};
+    if (mx_in_lds(p.c, p.d, (int)dtype_size(dtype), last)) return fused[dtype == KSMM_F32][last][gated](p, act, s);
+    return dtype == KSMM_F32 ? product<float>(p, last, gated, act, s) : product<half_t>(p, last, gated, act, s);
+}
+
 int ksmm_mx_forward(const void *x, const void *x_scales, const void *w, const void *w_scales, const void *bias, void *y, void *codes_out,
                     void *scales_out, void *workspace, int64_t workspace_bytes, int64_t batch, int a, int b, int c, int d, int dtype,
                     int bs_last, int act, int gated, void *stream)
@@ -465,13 +480,9 @@ int ksmm_mx_forward(const void *x, const void *x_scales, const void *w, const vo
                        {bias, (int64_t)a * rows_w * d * size}};
     const Span out[] = {{y, values(batch, a, b, d) * size}, {codes_out, blocks * 16}, {scales_out, blocks}, {need ? workspace : nullptr, need}};
     if (any_overlap(in, out)) return KSMM_ERR_ALIAS;
-    MxProduct p{x, (const uint8_t *)x_scales, (uint8_t *)codes_out, (uint8_t *)scales_out, (const uint8_t *)w, (const uint8_t *)w_scales, bias, y, nullptr, batch, a, b, c, d, cb};
-    static int (*const fused[2][2][2])(const MxProduct &, int, hipStream_t) = {
-        {{mx_half_first_plain, mx_half_first_gated}, {mx_half_last_plain, mx_half_last_gated}},
-        {{mx_float_first_plain, mx_float_first_gated}, {mx_float_last_plain, mx_float_last_gated}}};
-    if (mx_in_lds(c, d, (int)dtype_size(dtype), bs_last != 0))
-        return fused[dtype == KSMM_F32][bs_last != 0][gated != 0](p, act, (hipStream_t)stream);
-    if (!x_scales) {
+    MxProduct p{x, (const uint8_t *)x_scales, (uint8_t *)codes_out, (uint8_t *)scales_out, (const uint8_t *)w, (const uint8_t *)w_scales, bias, y, nullptr, false, batch, a, b, c, d, cb};
+    hipStream_t s = (hipStream_t)stream;
+    if (need > 0) {  // (no workgroup's LDS holds the codes: x is quantised in a launch of its own)
         uint8_t *const codes = codes_out ? (uint8_t *)codes_out : (uint8_t *)workspace;
         uint8_t *const scales = codes_out ? (uint8_t *)scales_out : codes + align256(blocks * 16);
         rc = ksmm_mx_quantize(x, codes, scales, batch, a, c, d, dtype, bs_last, stream);
@@ -479,11 +490,23 @@ int ksmm_mx_forward(const void *x, const void *x_scales, const void *w, const vo
         p.x = codes;
         p.x_scales = scales;
     }
-    p.b_tiles = (b + 31) / 32;
-    p.token_tiles = (batch + 31) / 32;
-    p.tiles = (int64_t)a * d * p.b_tiles * p.token_tiles;
-    return dtype == KSMM_F32 ? product<float>(p, bs_last != 0, gated != 0, act, (hipStream_t)stream)
-                             : product<half_t>(p, bs_last != 0, gated != 0, act, (hipStream_t)stream);
+    return launch_product(p, dtype, bs_last != 0, gated != 0, act, s);
+}
+
+int ksmm_mx_sums(const void *x, const void *x_scales, const void *w, const void *w_scales, const void *bias, void *z, int64_t batch, int a, int b, int c, int d,
+                 int dtype, int bs_last, void *stream)
+{
+    const int rc = check_product(batch, a, b, c, d, dtype, KSMM_ACT_NONE, 0);
+    if (rc != KSMM_OK) return rc;
+    if (!x || !x_scales || !w || !w_scales || !z) return KSMM_ERR_NULL_POINTER;
+    if (((uintptr_t)w & 15) != 0 || ((uintptr_t)x & 15) != 0) return KSMM_ERR_WORKSPACE;
+    const int cb = (int)mx_blocks(c);
+    const int64_t blocks = (int64_t)a * d * batch * cb, w_blocks = (int64_t)a * d * b * cb, size = (int64_t)dtype_size(dtype);
+    const Span in[] = {{x, blocks * 16}, {x_scales, blocks}, {w, w_blocks * 16}, {w_scales, w_blocks}, {bias, (int64_t)a * b * d * size}};
+    const Span out[] = {{z, values(batch, a, b, d) * size}};
+    if (any_overlap(in, out)) return KSMM_ERR_ALIAS;
+    const MxProduct p{x, (const uint8_t *)x_scales, nullptr, nullptr, (const uint8_t *)w, (const uint8_t *)w_scales, bias, z, nullptr, true, batch, a, b, c, d, cb};
+    return launch_product(p, dtype, bs_last != 0, false, KSMM_ACT_NONE, (hipStream_t)stream);
 }
 
 int ksmm_mx_slope(const void *x, const void *x_scales, const void *w, const void *w_scales, const void *bias, const void *dy, void *dz, int64_t batch,
@@ -493,7 +516,7 @@ int ksmm_mx_slope(const void *x, const void *x_scales, const void *w, const void
     if (rc != KSMM_OK) return rc;
     if (!gated && act == KSMM_ACT_NONE) return KSMM_ERR_BAD_EPILOGUE;
     const int rows_w = gated ? 2 * b : b, cb = (int)mx_blocks(c);
-    MxProduct p{x, (const uint8_t *)x_scales, nullptr, nullptr, (const uint8_t *)w, (const uint8_t *)w_scales, bias, dz, dy, batch, a, b, c, d, cb};
+    MxProduct p{x, (const uint8_t *)x_scales, nullptr, nullptr, (const uint8_t *)w, (const uint8_t *)w_scales, bias, dz, dy, false, batch, a, b, c, d, cb};
     if (dz) {
         if (!x || !x_scales || !w || !w_scales || !dy) return KSMM_ERR_NULL_POINTER;
         const int64_t blocks = (int64_t)a * d * batch * cb, w_blocks = (int64_t)a * d * rows_w * cb, size = (int64_t)dtype_size(dtype);

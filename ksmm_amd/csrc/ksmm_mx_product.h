@@ -62,6 +62,9 @@ template <typename T, bool GATED, int ACT> __device__ __forceinline__ float mx_a
     return activate<T, ACT, false, true>(z, slope);
 }
 
+// in fp16's range (NaN stays)
+__device__ __forceinline__ float mx_within_half(float z) { return z > 65504.f ? 65504.f : z < -65504.f ? -65504.f : z; }
+
 // act of a lane's sums of one d_i
 template <typename T, int D, bool GATED, int ACT> __device__ __forceinline__ void mx_activate(const float16_t (&acc)[GATED ? 2 : 1], int j, T (&v)[16 * D])
 {
@@ -600,6 +603,12 @@ template <typename T, bool LAST, int D, int TT, bool GATED, int ACT> __global__ 
 #pragma unroll
             for (int t = 0; t < TT; ++t) {
                 T v[16];
+                if constexpr (D == -1 && !GATED && ACT == KSMM_ACT_NONE && sizeof(T) == 2) {
+                    if (p.finite) {
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) acc[t][0][i] = mx_within_half(acc[t][0][i]);
+                    }
+                }
                 mx_activate<T, 1, GATED, ACT>(acc[t], 0, v);
                 if (LAST || alone) {
                     if (t * 32 < here) mx_results<T, LAST, 1>(p, v, ai, d0, bt, lane, n0, t, here, (uint8_t *)stage + wave * MX_STAGE, p.b);

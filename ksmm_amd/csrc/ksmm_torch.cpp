@@ -845,7 +845,10 @@ struct MxNode : ag::Node {
                                                  ws.mutable_data_ptr(), need, how.batch, how.a, how.b, how.c, how.d, dt, how.bs_last, how.act, stream));
             } else {
                 at::Tensor z = at::empty_like(dy);
-                check_status(mx_forward(data_of(t[0]), data_of(t[1]), t[2], t[3], t[4], z, nullptr, nullptr, how, KSMM_ACT_NONE));
+                // (in the tensors' type: z in 32 bits beside fp16 took a pass of (1,128,128,8), 25088 rows from 240 to 280 us, for gradients 2.93e-4
+                // off instead of 2.99e-4)
+                check_status(ksmm_mx_sums(data_of(t[0]), data_of(t[1]), data_of(t[2]), data_of(t[3]), data_of(t[4]), out_of(z), how.batch, how.a, how.b, how.c, how.d, dt,
+                                          how.bs_last, stream));
                 const ksmm_factor_desc f{data_of(w), how.a, how.b, how.c, how.d, dt, 1.f};
                 layer_backward(f, x, z, dy, out, how.act, dt, stream);
             }

@@ -291,7 +291,10 @@ def _backward(grad, q, packed, w, bias, act, bs_last, need_x, need_w, need_b):
     act = None if act == "none" else act
     z = None
     if act is not None:  # what the activation was applied to, computed again
-        z = MXKernel.forward(q, packed, bias, None, bs_last).view(flat.shape)
+        z = torch.empty_like(flat)
+        with torch.cuda.device(grad.device):
+            _lib.check(_lib.load().ksmm_mx_sums(q.codes.data_ptr(), q.scales.data_ptr(), packed.codes.data_ptr(), packed.scales.data_ptr(), _ptr(bias), z.data_ptr(),
+                                                q.codes.size(1), a, b, c, d, dtype_code(q.dtype), int(bs_last), _stream_ptr(grad)))
     need_b = need_b and bias is not None
     x = q.dequantize()
     x = x.view(a * c * d, -1) if bs_last else x.view(-1, a * c * d)
@@ -314,7 +317,8 @@ def mx_linear(x, factor, pattern=None, bias=None, act=None, gated=False, bs_last
     the call.  ``bias`` has x's type.  ``act``: None, "gelu" (erf form), and with ``gated`` "silu".  The result has x's type.
     Gradients of x, of a factor in kernel format and of the bias are those of the product of the quantised values, handed
     straight through the roundings; they cannot be differentiated a second time.  In fp16 the gradients of the
-    projections are held in fp16 between the steps, as ``gated_linear`` holds them."""
+    projections are held in fp16 between the steps, as ``gated_linear`` holds them; and where no kernel has both, what GELU is applied to is too
+    (at most 65504): of one factor batch-size-first d of 5 and more, or c that registers do not hold."""
     if isinstance(factor, MXFactor):
         if pattern is not None and tuple(pattern) != factor.pattern:
             raise ValueError("factor has the pattern %s, not %s" % (factor.pattern, tuple(pattern)))

@@ -27,3 +27,69 @@ def test_a_given_result_counts_as_written():
     with torch.inference_mode():  # (tensors without a count)
         out = torch.empty(5, 40, device="cuda")
         assert torch.equal(MXKernel.forward(x, w, out=out), MXKernel.forward(x, w))
+
+
+FAR = [(1, 16, 64, 5), (2, 8, 33, 6), (1, 12, 40, 17), (1, 20, 400, 4), (1, 40, 600, 1), (1, 6, 9000, 1)]
+
+
+@pytest.mark.parametrize("native", [True, False])
+@pytest.mark.parametrize("bs_last", [False, True])
+@pytest.mark.parametrize("pattern", FAR)
+def test_gradients_far_below_zero(monkeypatch, pattern, bs_last, native):
+    """GELU of what fp16 does not hold: its result is zero, and so is its slope.  dz is rounded once, the sums over it once more: twice 2^-11."""
+    from ksmm_amd import _lib, mx_linear
+
+    if not native:
+        monkeypatch.setattr(_lib, "_native", _lib._NoNative)
+    a, b, c, d = pattern
+    n = 37
+    x, f = rows(n, a * c * d, bs_last, torch.float16, 1), factor(pattern, False, torch.float16)
+    f[:, 0] = -64.0  # z of the first output of a block: -64 |x| summed, below -65504 with the rows made large
+    x = x.abs().clamp(max=8.0)
+    if bs_last:
+        x[:, :5] = 512.0
+    else:
+        x[:5] = 512.0
+    dy = rows(n, a * b * d, bs_last, torch.float16, 5)
+    leaves = [t.cuda().requires_grad_(True) for t in (x, f)]
+    bias = torch.linspace(-1, 1, a * b * d).half().cuda().requires_grad_(True)
+    with torch.enable_grad():
+        y = mx_linear(leaves[0], leaves[1], pattern, bias=bias, act="gelu", bs_last=bs_last)
+        got = torch.autograd.grad(y, [*leaves, bias], dy.cuda())
+        xq, wq = R.rounded(R.operand(x, a, c, d, bs_last)).requires_grad_(True), R.rounded(factor_rows(f, pattern)).requires_grad_(True)
+        b64 = bias.detach().cpu().double().requires_grad_(True)
+        want = R.product(xq, wq, b64, pattern, "gelu", False, bs_last)
+        assert float(R.product(xq, wq, b64, pattern, None, False, bs_last).min()) < -65520
+        grads = torch.autograd.grad(want, [xq, wq, b64], R.operand(dy, a, b, d, bs_last).double())
+    assert torch.isfinite(y).all()
+    for u, v in zip(got, [R.tensor(grads[0], x.shape, bs_last), grads[1].transpose(2, 3).reshape(f.shape), grads[2]]):
+        assert torch.isfinite(u).all() and rel(u, v) <= 2 * TOL["fp16"]
+
+
+@pytest.mark.parametrize("bs_last", [False, True])
+@pytest.mark.parametrize("prec", ["fp32", "fp16"])
+@pytest.mark.parametrize("pattern", [(1, 40, 16, 5), (2, 24, 70, 3), (2, 33, 33, 17), (1, 70, 64, 16), (1, 6, 9000, 1), (1, 5, 1200, 16)])
+def test_sums_for_gradients(pattern, prec, bs_last):
+    """What GELU is applied to: the product's result without it, but that fp16 ends at 65504, and a NaN is none.  Nothing behind the end is written."""
+    from ksmm_amd import _lib, mx_linear, pack_mx, quantize_mx
+    from ksmm_amd.mx import _ptr
+
+    a, b, c, d = pattern
+    for n, with_bias in ((1, True), (33, False), (70, True), (517, False)):
+        x, f = rows(n, a * c * d, False, DT[prec], n), factor(pattern, False, DT[prec])
+        x[0] *= 1000
+        f[:, 0] *= 1000
+        f[:, 1] *= -1000
+        x[n // 2, 0] = float("nan")
+        x = (x.t() if bs_last else x).contiguous()
+        bias = torch.linspace(-1, 1, a * b * d).to(DT[prec]).cuda() if with_bias else None
+        q, w = quantize_mx(x.cuda(), (a, c, d), bs_last), pack_mx(f.cuda(), pattern)
+        y = mx_linear(q, w, bias=bias, bs_last=bs_last)
+        room = torch.full((y.numel() + 64,), 7.0, dtype=DT[prec], device="cuda")
+        assert _lib.load().ksmm_mx_sums(q.codes.data_ptr(), q.scales.data_ptr(), w.codes.data_ptr(), w.scales.data_ptr(), _ptr(bias), room.data_ptr(), n, a, b, c, d,
+                                        0 if prec == "fp32" else 1, int(bs_last), torch.cuda.current_stream().cuda_stream) == 0
+        z = room[:-64].view(y.shape)
+        assert torch.isnan(y).any() and (prec == "fp32" or n == 1 or torch.isinf(y).any())
+        assert torch.equal(torch.isnan(z), torch.isnan(y))
+        want = y.clamp(-65504, 65504) if prec == "fp16" else y
+        assert torch.equal(torch.nan_to_num(z), torch.nan_to_num(want)) and (room[-64:] == 7).all()

@@ -239,3 +239,26 @@ def test_modules_refuse():
         MXLinear.of(torch.nn.Linear(2, 2))
     with pytest.raises((RuntimeError, ValueError)):
         adamw_update([torch.zeros(2)], [torch.zeros(2)], [torch.zeros(2)], [torch.zeros(2)])
+
+
+@pytest.mark.parametrize("dtype", [0, 1])
+@pytest.mark.parametrize("c,d", [(40, 1), (40, 5), (9000, 1)])
+def test_sums_refuse(lib, c, d, dtype):
+    n, a, b, size = 9, 2, 24, (4, 2)[dtype]
+    names = ["x", "x_scales", "w", "w_scales", "bias", "z"]
+    at = dict(zip(names, FAR))
+
+    def call(n=n, a=a, b=b, c=c, d=d, dtype=dtype, bs_last=0, **change):
+        p = dict(at, **change)
+        return lib.ksmm_mx_sums(*(p[k] for k in names), n, a, b, c, d, dtype, bs_last, None)
+
+    for bs_last in (0, 1):
+        for k in ("x", "x_scales", "w", "w_scales", "z"):
+            assert call(bs_last=bs_last, **{k: None}) == NULL
+        assert call(bs_last=bs_last, n=0) == BATCH and call(bs_last=bs_last, b=0) == PATTERN and call(bs_last=bs_last, dtype=2) == DTYPE
+        assert call(bs_last=bs_last, n=0x7fffffff) == LARGE and call(bs_last=bs_last, w=at["w"] + 8) == WORKSPACE and call(bs_last=bs_last, x=at["x"] + 4) == WORKSPACE
+        blocks = (c + 31) // 32 * a * d
+        sizes = {"x": n * blocks * 16, "x_scales": n * blocks, "w": b * blocks * 16, "w_scales": b * blocks, "bias": a * b * d * size}
+        for k in sizes:
+            assert call(bs_last=bs_last, z=at[k] + sizes[k] - 1) == ALIAS, k
+        assert call(bs_last=bs_last, z=at["x"] - size * n * a * b * d + 1) == ALIAS
