@@ -752,7 +752,7 @@ PyObject *py_mx_dequantize(PyObject *, PyObject *const *args, Py_ssize_t n_args)
 
 struct MxHow {
     int a, b, c, d, act, gated;
-    bool bs_last;
+    bool bs_last, wide;  // wide: fp16 may not have the factor's values, gradients are computed in fp32
     int64_t batch;
     int rows() const { return gated ? 2 * b : b; }
 };
@@ -809,13 +809,15 @@ struct MxNode : ag::Node {
         if (!grads[0].defined()) return result;
         at::Tensor t[5], out[3];
         for (int i = 0; i < 5; ++i) t[i] = in[i].unpack();
-        const at::Tensor dy = grads[0].contiguous();
+        const at::ScalarType type = grads[0].scalar_type(), held = how.wide ? at::kFloat : type;
         {
             at::NoGradGuard no_grad;
-            DeviceScope scope(dy.device().index());
-            const int dt = code_of(dy.scalar_type());
-            void *const stream = stream_of(dy);
+            DeviceScope scope(grads[0].device().index());
+            void *const stream = stream_of(grads[0]);
             refuse_outside(next_edges(), stream);
+            const at::Tensor dy = grads[0].to(held).contiguous();
+            if (t[4].defined()) t[4] = t[4].to(held);
+            const int dt = code_of(held);
             const int64_t features = (int64_t)how.a * how.c * how.d;
             at::Tensor x = at::empty(x_shape, dy.options()), w = at::empty({features, how.rows()}, dy.options());
             check_status(ksmm_mx_values(data_of(t[0]), data_of(t[1]), out_of(x), data_of(t[2]), data_of(t[3]), out_of(w), how.batch, how.rows(), how.a, how.c, how.d, dt,
@@ -852,17 +854,19 @@ struct MxNode : ag::Node {
                 const ksmm_factor_desc f{data_of(w), how.a, how.b, how.c, how.d, dt, 1.f};
                 layer_backward(f, x, z, dy, out, how.act, dt, stream);
             }
+            for (int i = 0; i < 3; ++i)
+                if (out[i].defined()) result[i] = out[i].to(type);
         }
-        for (int i = 0; i < 3; ++i) result[i] = out[i];
         return once(std::move(result), "mx_linear");
     }
 };
 
-// mx_linear(x, factor, scales, pattern, gated, bias, act, bs_last) -> y or None; scales None: a factor in kernel format, else its codes
+// mx_linear(x, factor, scales, pattern, gated, bias, act, bs_last, wide) -> y or None; scales None: a factor in kernel format, else its codes,
+// with `wide` of values that fp16 may not have
 PyObject *py_mx_linear(PyObject *, PyObject *const *args, Py_ssize_t n_args)
 {
-    if (n_args != 8) {
-        PyErr_SetString(PyExc_TypeError, "mx_linear() takes 8 arguments");
+    if (n_args != 9) {
+        PyErr_SetString(PyExc_TypeError, "mx_linear() takes 9 arguments");
         return nullptr;
     }
     try {
@@ -890,6 +894,7 @@ PyObject *py_mx_linear(PyObject *, PyObject *const *args, Py_ssize_t n_args)
                 h.c = (int)v[2];
                 h.d = (int)v[3];
                 h.batch = x.numel() / features;
+                h.wide = PyObject_IsTrue(args[8]) == 1 && x.scalar_type() == at::kHalf;
                 c10::SmallVector<int64_t, 6> shape(x.sizes().begin(), x.sizes().end());
                 shape[h.bs_last ? 0 : shape.size() - 1] = out_features;
                 at::Tensor y, codes, scales, x_codes, x_scales;

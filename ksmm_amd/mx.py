@@ -115,11 +115,12 @@ def quantize_mx(x, sizes, bs_last=False):
 
 class MXFactor:
     """A factor of ``pattern`` (a, b, c, d) as microscaled 4-bit numbers: ``codes`` (a*d, b, 16 * ceil(c / 32)) and ``scales``
-    (a*d, b, ceil(c / 32)), uint8; with ``gated`` two of them side by side, 2*b rows, the gate's first."""
+    (a*d, b, ceil(c / 32)), uint8; with ``gated`` two of them side by side, 2*b rows, the gate's first.  ``dtype``: what they were made
+    from.  Numbers of float16 are all float16 values; of float32, or of what is not said, gradients of fp16 inputs are computed in 32 bits."""
 
-    def __init__(self, codes, scales, pattern, gated=False):
+    def __init__(self, codes, scales, pattern, gated=False, dtype=None):
         self.pattern = a, b, c, d = _sizes(pattern, 4, "pattern")
-        self.codes, self.scales, self.gated = codes, scales, bool(gated)
+        self.codes, self.scales, self.gated, self.dtype = codes, scales, bool(gated), dtype
         rows = _check_codes(codes, scales, a * d, c)
         if rows != (2 * b if gated else b):
             raise ValueError("codes must have %d rows, not %d" % (2 * b if gated else b, rows))
@@ -149,7 +150,7 @@ def pack_mx(factor, pattern, gated=False):
     """A factor in kernel format, (a*d*c, b) or with ``gated`` (a*d*c, 2*b), as an ``MXFactor``."""
     a, b, c, d = _check_factor(factor, pattern, gated)
     codes, scales = _quantize(factor.detach(), factor.size(1), a * d, c, 1, True)
-    return MXFactor(codes, scales, (a, b, c, d), gated)
+    return MXFactor(codes, scales, (a, b, c, d), gated, factor.dtype)
 
 
 def _check_product(x, device, pattern, bias, act, gated, bs_last):
@@ -226,15 +227,15 @@ class MXKernel:
 class MXFunction(torch.autograd.Function):
     """``apply(x, factor, bias, pattern, act, gated, bs_last)``: both operands are quantised, and kept so (17 bytes for 32 values)
     for the gradients, which are those of the product of what the codes stand for.  ``factor``: in kernel format, or an
-    ``MXFactor``, which takes no gradient."""
+    ``MXFactor``, which takes no gradient; where fp16 may not have its values, those of fp16 tensors are computed in fp32."""
 
     @staticmethod
     def forward(ctx, x, factor, bias, pattern, act, gated, bs_last):
         packed = factor if isinstance(factor, MXFactor) else pack_mx(factor, pattern, gated)
         out, codes, scales = MXKernel.forward(x, packed, bias, act, bs_last, need_codes=True)
         ctx.save_for_backward(codes, scales, packed.codes, packed.scales, bias)
-        ctx.how = tuple(pattern), act, bool(gated), bool(bs_last), tuple(x.shape), x.dtype
-        ctx.factor_dtype = None if packed is factor else factor.dtype
+        ctx.how = tuple(pattern), act, bool(gated), bool(bs_last), tuple(x.shape), torch.float32 if packed.dtype != torch.float16 else x.dtype
+        ctx.dtype, ctx.factor_dtype = x.dtype, None if packed is factor else factor.dtype
         return out
 
     @staticmethod
@@ -248,7 +249,7 @@ class MXFunction(torch.autograd.Function):
         q = MXTensor(x_codes, x_scales, (a, c, d), shape, dtype, bs_last)
         packed = MXFactor(w_codes, w_scales, pattern, gated)
         w = packed.dequantize(dtype)
-        grad = grad.contiguous()
+        grad, bias = grad.to(dtype).contiguous(), None if bias is None else bias.to(dtype)
         dz = _slope(grad, q, packed, bias, act, bs_last) if grad.numel() > 0 and (gated or act not in (None, "none")) else None
         if dz is not None:  # those of a layer without an activation, of the gate's and the other projection's outputs side by side
             packed = MXFactor(w_codes, w_scales, (a, packed.codes.size(1), c, d))
@@ -257,9 +258,8 @@ class MXFunction(torch.autograd.Function):
             dx, dw, dbias = GatedKernel.backward(grad, q.dequantize(), w, pattern, bias, act, bs_last, need_x, need_w, need_b)
         else:
             dx, dw, dbias = _backward(grad, q, packed, w, bias, act, bs_last, need_x, need_w, need_b)
-        if dw is not None and dw.dtype != ctx.factor_dtype:
-            dw = dw.to(ctx.factor_dtype)
-        return dx, dw, dbias, None, None, None, None
+        dx, dbias = (None if t is None else t.to(ctx.dtype) for t in (dx, dbias))
+        return dx, None if dw is None else dw.to(ctx.factor_dtype), dbias, None, None, None, None
 
 
 def _slope(grad, q, packed, bias, act, bs_last):
@@ -318,20 +318,21 @@ def mx_linear(x, factor, pattern=None, bias=None, act=None, gated=False, bs_last
     Gradients of x, of a factor in kernel format and of the bias are those of the product of the quantised values, handed
     straight through the roundings; they cannot be differentiated a second time.  In fp16 the gradients of the
     projections are held in fp16 between the steps, as ``gated_linear`` holds them; and where no kernel has both, what GELU is applied to is too
-    (at most 65504): of one factor batch-size-first d of 5 and more, or c that registers do not hold."""
+    (at most 65504): of one factor batch-size-first d of 5 and more, or c that registers do not hold.  Through an ``MXFactor`` that was not made
+    from fp16 values the gradients of fp16 tensors are computed in fp32, and rounded at the end."""
     if isinstance(factor, MXFactor):
         if pattern is not None and tuple(pattern) != factor.pattern:
             raise ValueError("factor has the pattern %s, not %s" % (factor.pattern, tuple(pattern)))
         if gated and not factor.gated:
             raise ValueError("factor is not a gated one")
         pattern, gated = factor.pattern, factor.gated
-        out = _lib.native().mx_linear(x, factor.codes, factor.scales, pattern, gated, bias, act, bs_last)
+        out = _lib.native().mx_linear(x, factor.codes, factor.scales, pattern, gated, bias, act, bs_last, factor.dtype != torch.float16)
         if out is not None:
             return out
     elif pattern is None:
         raise ValueError("a factor in kernel format needs its pattern")
     else:
-        out = _lib.native().mx_linear(x, factor, None, pattern, gated, bias, act, bs_last)
+        out = _lib.native().mx_linear(x, factor, None, pattern, gated, bias, act, bs_last, False)
         if out is not None:
             return out
         pattern = _check_factor(factor, pattern, gated)[:4]
@@ -379,6 +380,13 @@ def _chain(x, factors, patterns, bias, act, bs_last):
     return x
 
 
+def _type_of(scales):
+    """float16 where all of a factor's numbers are float16 values, else float32.  6 * 2^13 and 0.5 * 2^-23 are; of 2^-77 and less (and of zeros)
+    nothing is left in a float16 gradient."""
+    fine = ((scales >= 104) & (scales <= 140)) | (scales <= 50) | (scales == 255)
+    return torch.float16 if bool(fine.all()) else torch.float32
+
+
 class MXLinear(nn.Module):
     """A layer of packed factors, the first one applied first: what ``KSLinearMX.packed()`` gives, or of any
     ``KSLinear(algo='kernel')`` or ``KSGatedLinear`` ``MXLinear.of``.  Codes and scales are buffers, a copy of the factors as they
@@ -388,7 +396,7 @@ class MXLinear(nn.Module):
         super().__init__()
         if not factors:
             raise ValueError("no factors")
-        self.patterns, self.gated = [f.pattern for f in factors], [f.gated for f in factors]
+        self.patterns, self.gated, self.dtypes = [f.pattern for f in factors], [f.gated for f in factors], [f.dtype for f in factors]
         if any(self.gated[:-1]):
             raise ValueError("only the last factor may be gated")
         for p, q in zip(self.patterns, self.patterns[1:]):
@@ -413,8 +421,15 @@ class MXLinear(nn.Module):
         return cls([pack_mx(f, p) for f, p in zip(layer.factors, layer.patterns)], layer.bias, layer.act, layer.bs_last)
 
     def factors(self):
-        return [MXFactor(getattr(self, "codes%d" % i), getattr(self, "scales%d" % i), p, g)
-                for i, (p, g) in enumerate(zip(self.patterns, self.gated))]
+        return [MXFactor(getattr(self, "codes%d" % i), getattr(self, "scales%d" % i), p, g, t)
+                for i, (p, g, t) in enumerate(zip(self.patterns, self.gated, self.dtypes))]
+
+    def _load_from_state_dict(self, state_dict, prefix, *how):
+        super()._load_from_state_dict(state_dict, prefix, *how)
+        for i in range(len(self.dtypes)):
+            scales = state_dict.get("%sscales%d" % (prefix, i))
+            if scales is not None:
+                self.dtypes[i] = _type_of(scales)
 
     def forward(self, x):
         return _chain(x, self.factors(), self.patterns, self.bias, self.act, self.bs_last)

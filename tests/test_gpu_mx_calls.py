@@ -93,3 +93,80 @@ def test_sums_for_gradients(pattern, prec, bs_last):
         assert torch.equal(torch.isnan(z), torch.isnan(y))
         want = y.clamp(-65504, 65504) if prec == "fp16" else y
         assert torch.equal(torch.nan_to_num(z), torch.nan_to_num(want)) and (room[-64:] == 7).all()
+
+
+def wide(gated, seed=0):
+    """A factor in fp32 whose first block lies beyond fp16's range and whose second one below it, and an input and gradient for it.
+
+    Products of the first are 2^8 (gated dz 2^-7), of gradients 2^12; of the second 2^-12."""
+    g = torch.Generator().manual_seed(seed)
+    pattern, n = (2, 24, 64, 1), 41
+    a, b, c, d = pattern
+    f = torch.randn(a, c, 2 * b if gated else b, generator=g) * torch.tensor([2.0 ** 17, 2.0 ** -27]).view(2, 1, 1)
+    x = torch.randn(n, a, c, generator=g) * torch.tensor([2.0 ** -12, 1.0]).view(1, 2, 1)
+    dy = torch.randn(n, a, b, generator=g) * torch.tensor([2.0 ** -15, 2.0 ** 13]).view(1, 2, 1)
+    return pattern, f.reshape(a * d * c, -1), x.reshape(n, -1).half(), dy.reshape(n, -1).half()
+
+
+def wide_gradients(pattern, f, x, dy, bias, act, gated):
+    a, b, c, d = pattern
+    with torch.enable_grad():
+        xq, wq = R.rounded(R.operand(x, a, c, d, False)).requires_grad_(True), R.rounded(factor_rows(f, pattern))
+        b64 = bias.double().requires_grad_(True)
+        want = R.product(xq, wq, b64, pattern, act, gated, False)
+        dx, db = torch.autograd.grad(want, [xq, b64], R.operand(dy, a, b, d, False).double())
+    return R.tensor(dx, x.shape, False), db
+
+
+@pytest.mark.parametrize("native", [True, False])
+@pytest.mark.parametrize("gated,act", [(False, None), (False, "gelu"), (True, "silu"), (True, None)])
+@pytest.mark.parametrize("made", ["packed", "by hand"])
+def test_gradients_through_values_beyond_fp16(monkeypatch, made, gated, act, native):
+    """Codes of fp32 weights hold values that fp16 has not: gradients of fp16 inputs are rounded once for all that, at the end."""
+    from ksmm_amd import MXFactor, _lib, mx_linear, pack_mx
+
+    if not native:
+        monkeypatch.setattr(_lib, "_native", _lib._NoNative)
+    pattern, f, x, dy = wide(gated)
+    w = pack_mx(f.cuda(), pattern, gated)
+    if made == "by hand":
+        w = MXFactor(w.codes, w.scales, pattern, gated)
+    bias = torch.linspace(-1, 1, f.shape[1] * 2).half()
+    leaves = [t.cuda().requires_grad_(True) for t in (x, bias)]
+    with torch.enable_grad():
+        y = mx_linear(leaves[0], w, bias=leaves[1], act=act)
+        dx, db = torch.autograd.grad(y, leaves, dy.cuda())
+    assert y.dtype == dx.dtype == db.dtype == torch.float16
+    want, want_b = wide_gradients(pattern, f, x, dy, bias, act, gated)
+    for part in (slice(0, 64), slice(64, 128)):
+        # (a value is rounded to 2^-11 of it, or to 2^-25 where the type has no more)
+        assert rel(dx[:, part], want[:, part]) <= TOL["fp16"] + 2.0 ** -25 * want[:, part].numel() ** 0.5 / float(want[:, part].norm())
+    fine = want_b.abs() < 65504
+    assert fine.sum() >= 24 and rel(db.cpu()[fine], want_b[fine]) <= TOL["fp16"]
+
+
+def test_gradients_through_loaded_codes():
+    from ksmm_amd import KSLinear, MXLinear
+
+    pattern, f, x, dy = wide(False)
+    layers = {}
+    for dtype in (torch.float32, torch.float16):
+        layer = KSLinear([pattern], algo="kernel", bias=False, dtype=dtype, device="cuda")
+        layer.factors[0].data.copy_(f.clamp(-60000, 60000))
+        layers[dtype] = MXLinear.of(layer)
+    layer = KSLinear([pattern], algo="kernel", bias=False, dtype=torch.float32, device="cuda")
+    layer.factors[0].data.copy_(f)
+    full = MXLinear.of(layer)
+    layers[torch.float16].load_state_dict(full.state_dict())
+    want, _ = wide_gradients(pattern, f, x, dy, torch.zeros(48), None, False)
+    for served in (full, layers[torch.float16]):
+        with torch.enable_grad():
+            leaf = x.cuda().requires_grad_(True)
+            dx, = torch.autograd.grad(served(leaf), leaf, dy.cuda())
+        assert rel(dx, want) <= TOL["fp16"] and rel(dx[:, 64:], want[:, 64:]) <= 2 * TOL["fp16"]
+    # and back: codes of fp16 weights
+    narrow = MXLinear.of(KSLinear([pattern], algo="kernel", bias=False, dtype=torch.float16, device="cuda"))
+    full.load_state_dict(narrow.state_dict())
+    with torch.enable_grad():
+        leaf = x.cuda().requires_grad_(True)
+        assert torch.equal(*(torch.autograd.grad(m(leaf), leaf, dy.cuda())[0] for m in (full, narrow)))
