@@ -14,6 +14,7 @@ import math
 
 import torch
 from torch import nn
+from torch.autograd import forward_ad
 
 from . import _lib
 from .block import GATED_ACTS, GatedKernel, KSFeedForward, KSGatedLinear, _ptr, _trainable_type, _written
@@ -316,7 +317,7 @@ def mx_linear(x, factor, pattern=None, bias=None, act=None, gated=False, bs_last
     ``factor``: an ``MXFactor`` (``pattern`` and ``gated`` are its own then), or a factor in kernel format, which is quantised in
     the call.  ``bias`` has x's type.  ``act``: None, "gelu" (erf form), and with ``gated`` "silu".  The result has x's type.
     Gradients of x, of a factor in kernel format and of the bias are those of the product of the quantised values, handed
-    straight through the roundings; they cannot be differentiated a second time.  In fp16 the gradients of the
+    straight through the roundings; they cannot be differentiated a second time, nor in forward mode.  In fp16 the gradients of the
     projections are held in fp16 between the steps, as ``gated_linear`` holds them; and where no kernel has both, what GELU is applied to is too
     (at most 65504): of one factor batch-size-first d of 5 and more, or c that registers do not hold.  Through an ``MXFactor`` that was not made
     from fp16 values the gradients of fp16 tensors are computed in fp32, and rounded at the end."""
@@ -336,6 +337,8 @@ def mx_linear(x, factor, pattern=None, bias=None, act=None, gated=False, bs_last
         if out is not None:
             return out
         pattern = _check_factor(factor, pattern, gated)[:4]
+    if forward_ad._current_level >= 0 and any(isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None for t in (x, factor, bias)):
+        raise RuntimeError("mx_linear has no forward-mode derivative: a tangent would be lost")
     if torch.jit.is_tracing() or (torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in (x, factor, bias))):
         if isinstance(x, MXTensor):
             raise RuntimeError("a quantised input has no gradient: pass the tensor, or call without gradients")

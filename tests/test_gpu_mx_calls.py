@@ -170,3 +170,23 @@ def test_gradients_through_loaded_codes():
     with torch.enable_grad():
         leaf = x.cuda().requires_grad_(True)
         assert torch.equal(*(torch.autograd.grad(m(leaf), leaf, dy.cuda())[0] for m in (full, narrow)))
+
+
+def test_forward_mode_is_refused():
+    """A tangent would be lost."""
+    from torch.autograd import forward_ad
+
+    from ksmm_amd import KSLinearMX, MXLinear, mx_linear, pack_mx, quantize_mx
+
+    pattern = (1, 40, 64, 1)
+    x, f, bias = rows(5, 64, False, torch.float32).cuda(), factor(pattern, False, torch.float32).cuda(), torch.zeros(40, device="cuda")
+    w = pack_mx(f, pattern)
+    layer = KSLinearMX([pattern], dtype=torch.float32, bias=False)
+    with forward_ad.dual_level():
+        dx, df, db = (forward_ad.make_dual(t, torch.ones_like(t)) for t in (x, f, bias))
+        for call in (lambda: mx_linear(dx, w), lambda: mx_linear(dx, f, pattern), lambda: mx_linear(x, df, pattern), lambda: mx_linear(x, w, bias=db),
+                     lambda: mx_linear(quantize_mx(x, (1, 64, 1)), w, bias=db), lambda: layer(dx), lambda: layer.packed()(dx)):
+            for on in (False, True):
+                with torch.set_grad_enabled(on), pytest.raises(RuntimeError, match="forward-mode"):
+                    call()
+        assert torch.equal(mx_linear(x, w), mx_linear(x, f, pattern))  # (tensors without one)

@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from ksmm_amd import KSAdamW, _lib, adamw_update
+from ksmm_amd import _lib, adamw_update, mx
 
 
 class Native:
@@ -27,3 +27,33 @@ def test_a_step_whose_launch_failed_is_not_made_again(monkeypatch):
     with pytest.raises(_lib.KsmmError) as e:
         adamw_update(t, t, t, t)
     assert e.value.status == -7 and native.calls == 1
+
+
+def test_a_tangent_is_refused(monkeypatch):
+    """Forward-mode derivatives, whichever tensor has one: no kernel is reached."""
+    from torch.autograd import forward_ad
+
+    class Declines:
+        @staticmethod
+        def mx_linear(*args):
+            return None
+
+    def reached(*args, **kw):
+        raise AssertionError("a kernel is reached")
+
+    monkeypatch.setattr(_lib, "native", lambda: Declines)
+    monkeypatch.setattr(mx.MXKernel, "forward", staticmethod(reached))
+    monkeypatch.setattr(mx.MXFunction, "apply", reached)
+    monkeypatch.setattr(mx, "_check_factor", lambda factor, pattern, gated: pattern)
+    packed = object.__new__(mx.MXFactor)
+    packed.codes = packed.scales = torch.zeros(1, dtype=torch.uint8)
+    packed.pattern, packed.gated, packed.dtype = (1, 4, 8, 1), False, torch.float32
+    x, factor, bias = torch.ones(2, 8), torch.ones(8, 4), torch.ones(4)
+    with forward_ad.dual_level():
+        dual = [forward_ad.make_dual(t, torch.ones_like(t)) for t in (x, factor, bias)]
+        for args in ((dual[0], packed), (dual[0], factor, packed.pattern), (x, dual[1], packed.pattern), (x, packed, None, dual[2])):
+            for on in (False, True):
+                with torch.set_grad_enabled(on), pytest.raises(RuntimeError, match="forward-mode"):
+                    mx.mx_linear(*args)
+        with pytest.raises(AssertionError, match="reached"):
+            mx.mx_linear(x, packed)
