@@ -123,7 +123,8 @@ class KSAdamW(torch.optim.Optimizer):
         opt = KSAdamW(model.parameters(), lr=1e-3)                  # of everything
         muon, rest = KSMuon(model), KSAdamW(KSMuon.others(model))   # beside the factors' own updates
 
-    ``bits``: 32, or 8 for moments that take 2.06 bytes a weight instead of 8 (``adamw_update`` says how).  fp16 parameters are
+    ``bits``: 32, or 8 for moments that take 2.06 bytes a weight instead of 8 (``adamw_update`` says how; the tensors' numbers go on over
+    all groups).  fp16 parameters are
     rounded from fp32 weights that the optimiser keeps (``master=False``: updated as they are); values that were written into
     a parameter since replace them.  ``grad_scale`` multiplies the gradients: one over a loss's scale.  ``capturable``: the count of steps is
     a tensor of the group's on its one device, so that a captured step counts on with every replay (a step before the capture sets the
@@ -198,6 +199,7 @@ class KSAdamW(torch.optim.Optimizer):
             with torch.enable_grad():
                 loss = closure()
         capturing = torch.cuda.is_current_stream_capturing()
+        number = 0  # of tensors whose step was made: those of all groups and types are rounded by numbers of their own
         for g in self.param_groups:
             sets = {}
             if capturing and not (g["capturable"] and g.get("step") is not None and all(self.state[p] for p in g["params"] if p.grad is not None)):
@@ -221,5 +223,6 @@ class KSAdamW(torch.optim.Optimizer):
                 adamw_update(ps, [p.grad.contiguous() for p in ps], [s["exp_avg"] for s in states], [s["exp_avg_sq"] for s in states],
                              [s["scales"] for s in states] if small else None, [s["master"] for s in states] if master else None,
                              g["step"] if count is None else count, g["lr"], g["betas"], g["eps"], g["weight_decay"], g["grad_scale"],
-                             g["seed"], follow=True)
+                             g["seed"] + number, follow=True)
+                number += len(ps)
         return loss

@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from ksmm_amd import _lib, adamw_update, mx
+from ksmm_amd import KSAdamW, _lib, adamw, adamw_update, mx
 
 
 class Native:
@@ -57,3 +57,24 @@ def test_a_tangent_is_refused(monkeypatch):
                     mx.mx_linear(*args)
         with pytest.raises(AssertionError, match="reached"):
             mx.mx_linear(x, packed)
+
+
+def test_no_two_tensors_of_a_step_are_rounded_alike(monkeypatch):
+    """Seeds and numbers in a call of all groups, types and counts of steps; of one group they are those of its list."""
+    seeds = []
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    monkeypatch.setattr(adamw, "adamw_update", lambda params, grads, m, v, scales, masters, step, *how, **kw: seeds.append([how[5] + i for i in range(len(params))]))
+    ps = [torch.nn.Parameter(torch.zeros(40, dtype=t)) for t in (torch.float32, torch.float16, torch.float32, torch.float32, torch.float16)]
+
+    def step(opt, of):
+        seeds.clear()
+        for p in ps:
+            p.grad = torch.ones_like(p) if any(p is q for q in of) else None
+        opt.step()
+        return [s for call in seeds for s in call]
+
+    opt = KSAdamW([{"params": ps[:3]}, {"params": ps[3:4], "weight_decay": 0.0}, {"params": ps[4:]}], bits=8, seed=7)
+    for of in (ps, ps[1:], ps[::2], ps):  # (counts of steps that differ, too)
+        found = step(opt, of)
+        assert len(found) == len(of) == len(set(found)), found
+    assert sorted(step(KSAdamW(ps[:1] + ps[2:4], bits=8, seed=7), ps)) == [7, 8, 9]
