@@ -16,8 +16,6 @@ namespace ksmm {
 
 namespace {
 
-int launched() { return hipGetLastError() == hipSuccess ? KSMM_OK : KSMM_ERR_LAUNCH; }
-
 struct MxOperand {
     const void *x;  // dequantising: written
     uint8_t *codes, *scales;
@@ -307,19 +305,15 @@ int64_t groups_of(const MxOperand &p)
 }
 template <typename T, int D, bool BACK> int convert_rows(const MxOperand &p, hipStream_t s)
 {
-    if (D == 3 || p.d == D)  // (never three of more)
-        hipLaunchKernelGGL((ks_mx_rows_kernel<T, D, BACK>), dim3((unsigned)groups_of(p)), dim3(THREADS), 0, s, p);
-    else if constexpr (D != 3)
-        hipLaunchKernelGGL((ks_mx_runs_kernel<T, D, BACK>), dim3((unsigned)groups_of(p)), dim3(THREADS), 0, s, p);
-    return launched();
+    const unsigned groups = (unsigned)groups_of(p);
+    if constexpr (D != 3)  // (never three of more)
+        if (p.d != D) return launch_kernel(&ks_mx_runs_kernel<T, D, BACK>, groups, THREADS, 0, s, p);
+    return launch_kernel(&ks_mx_rows_kernel<T, D, BACK>, groups, THREADS, 0, s, p);
 }
 template <typename T, bool BACK> int convert(const MxOperand &p, hipStream_t s)
 {
     if (groups_of(p) > 0x7fffffffLL) return KSMM_ERR_TOO_LARGE;
-    if (p.last) {
-        hipLaunchKernelGGL((ks_mx_columns_kernel<T, BACK>), dim3((unsigned)groups_of(p)), dim3(THREADS), 0, s, p);
-        return launched();
-    }
+    if (p.last) return launch_kernel(&ks_mx_columns_kernel<T, BACK>, (unsigned)groups_of(p), THREADS, 0, s, p);
     switch (mx_run_of(p.d)) {
     case 1: return convert_rows<T, 1, BACK>(p, s);
     case 2: return convert_rows<T, 2, BACK>(p, s);
@@ -332,25 +326,23 @@ template <typename T> int values_of(const MxOperand &x, const MxOperand &w, hipS
 {
     const int64_t x_groups = groups_of(x), w_groups = groups_of(w);
     if (x_groups + w_groups > 0x7fffffffLL) return KSMM_ERR_TOO_LARGE;
-    const dim3 grid((unsigned)(x_groups + w_groups)), threads(THREADS);
+    auto launch = [&](auto fn) { return launch_kernel(fn, (unsigned)(x_groups + w_groups), THREADS, 0, s, x, w, (uint32_t)w_groups); };
     switch (x.last ? 0 : mx_run_of(x.d)) {
-    case 0: hipLaunchKernelGGL((ks_mx_values_kernel<T, 0>), grid, threads, 0, s, x, w, (uint32_t)w_groups); break;
-    case 1: hipLaunchKernelGGL((ks_mx_values_kernel<T, 1>), grid, threads, 0, s, x, w, (uint32_t)w_groups); break;
-    case 2: hipLaunchKernelGGL((ks_mx_values_kernel<T, 2>), grid, threads, 0, s, x, w, (uint32_t)w_groups); break;
-    case 3: hipLaunchKernelGGL((ks_mx_values_kernel<T, 3>), grid, threads, 0, s, x, w, (uint32_t)w_groups); break;
-    default: hipLaunchKernelGGL((ks_mx_values_kernel<T, 4>), grid, threads, 0, s, x, w, (uint32_t)w_groups);
+    case 0: return launch(&ks_mx_values_kernel<T, 0>);
+    case 1: return launch(&ks_mx_values_kernel<T, 1>);
+    case 2: return launch(&ks_mx_values_kernel<T, 2>);
+    case 3: return launch(&ks_mx_values_kernel<T, 3>);
+    default: return launch(&ks_mx_values_kernel<T, 4>);
     }
-    return launched();
 }
 
 template <typename T, bool LAST, bool GATED> int product(const MxProduct &p, int act, hipStream_t s)
 {
     const int64_t grid = (p.tiles + 3) / 4;
     if (grid > 0x7fffffffLL) return KSMM_ERR_TOO_LARGE;
-    with_act(act, [&](auto which) {
-        hipLaunchKernelGGL((ks_mx_product_kernel<T, LAST, GATED, decltype(which)::value>), dim3((unsigned)grid), dim3(256), 0, s, p);
-    });
-    return launched();
+    int rc = KSMM_OK;
+    with_act(act, [&](auto which) { rc = launch_kernel(&ks_mx_product_kernel<T, LAST, GATED, decltype(which)::value>, (unsigned)grid, 256, 0, s, p); });
+    return rc;
 }
 template <typename T> int product(MxProduct p, bool last, bool gated, int act, hipStream_t s)
 {

@@ -685,9 +685,7 @@ template <typename T, bool LAST, int D, int TT, bool GATED> int mx_launch_wide(M
         if constexpr (GATED || ACT != KSMM_ACT_SILU) {
             auto fn = &ks_mx_wide_kernel<T, LAST, D, TT, GATED, ACT>;
             if (lds > 64 * 1024) rc = ensure_dynamic_lds((const void *)fn, (int)MX_LDS_ALL);  // (set once a kernel: for all of its sizes)
-            if (rc != KSMM_OK) return;
-            hipLaunchKernelGGL(fn, dim3((unsigned)grid), dim3(64 * MX_WAVES), lds, s, p);
-            if (hipGetLastError() != hipSuccess) rc = KSMM_ERR_LAUNCH;
+            if (rc == KSMM_OK) rc = launch_kernel(fn, (unsigned)grid, 64 * MX_WAVES, lds, s, p);
         }
     });
     return rc;
@@ -697,7 +695,9 @@ template <typename T, bool LAST, int D, int TT, bool GATED> int mx_launch_wide(M
 inline int mx_registers(const void *kernel)
 {
     hipFuncAttributes a;
-    return hipFuncGetAttributes(&a, kernel) == hipSuccess ? a.numRegs : 512;
+    if (hipFuncGetAttributes(&a, kernel) == hipSuccess) return a.numRegs;
+    (void)hipGetLastError();  // (its answer is not needed)
+    return 512;
 }
 
 // the rest of the sizes, with `tiles` of outputs a workgroup
@@ -759,9 +759,7 @@ template <typename T, bool LAST, int D, bool GATED, int KS> int mx_launch_held(M
         if constexpr (GATED || ACT != KSMM_ACT_SILU) {
             auto fn = &ks_mx_held_kernel<T, LAST, D, GATED, ACT, KS>;
             if (lds > 64 * 1024) rc = ensure_dynamic_lds((const void *)fn, (int)MX_LDS_ALL);  // (set once a kernel: for all of its sizes)
-            if (rc != KSMM_OK) return;
-            hipLaunchKernelGGL(fn, dim3((unsigned)grid), dim3(64 * (MX_CONSUMERS + MX_PRODUCERS)), lds, s, p);
-            if (hipGetLastError() != hipSuccess) rc = KSMM_ERR_LAUNCH;
+            if (rc == KSMM_OK) rc = launch_kernel(fn, (unsigned)grid, 64 * (MX_CONSUMERS + MX_PRODUCERS), lds, s, p);
         }
     });
     return rc;

@@ -185,9 +185,7 @@ template <typename T, bool LAST, int D, bool GATED, int KS> int mx_launch_slope(
         if constexpr (GATED || ACT == KSMM_ACT_GELU) {
             auto fn = &ks_mx_slope_kernel<T, LAST, D, GATED, ACT, KS>;
             if (lds > 64 * 1024) rc = ensure_dynamic_lds((const void *)fn, (int)MX_LDS_ALL);  // (set once a kernel: for all of its sizes)
-            if (rc != KSMM_OK) return;
-            hipLaunchKernelGGL(fn, dim3((unsigned)grid), dim3(64 * (C + MX_PRODUCERS)), lds, s, p);
-            if (hipGetLastError() != hipSuccess) rc = KSMM_ERR_LAUNCH;
+            if (rc == KSMM_OK) rc = launch_kernel(fn, (unsigned)grid, 64 * (C + MX_PRODUCERS), lds, s, p);
         }
     });
     return rc;

@@ -190,3 +190,30 @@ def test_forward_mode_is_refused():
                 with torch.set_grad_enabled(on), pytest.raises(RuntimeError, match="forward-mode"):
                     call()
         assert torch.equal(mx_linear(x, w), mx_linear(x, f, pattern))  # (tensors without one)
+
+
+@pytest.mark.parametrize("native", [True, False])
+def test_an_error_from_before_is_not_the_calls_own(monkeypatch, native):
+    """What an earlier call on the thread left is neither taken for a launch's own nor cleared."""
+    from ksmm_amd import _lib, mx_linear, pack_mx, quantize_mx
+    from ksmm_amd.mx import _slope
+
+    lib = _lib.load()
+    if not native:
+        monkeypatch.setattr(_lib, "_native", _lib._NoNative)
+    pattern = (1, 40, 64, 2)
+    x, f, dy = rows(70, 128, False, torch.float16).cuda(), factor(pattern, False, torch.float16).cuda(), rows(70, 80, False, torch.float16, 1).cuda()
+    got = []
+    for before in (False, True):
+        w, q = pack_mx(f, pattern), quantize_mx(x, (1, 64, 2))
+        torch.cuda.synchronize()
+        if before:
+            assert lib.hipSetDevice(1 << 20) != 0
+        try:
+            now = [pack_mx(f, pattern).codes, quantize_mx(x, (1, 64, 2)).codes, q.dequantize(), mx_linear(x, w, act="gelu"), mx_linear(q, w), mx_linear(x, f, pattern),
+                   _slope(dy, q, w, None, "gelu", False)]
+        finally:
+            left = lib.hipGetLastError()
+        assert (left != 0) == before
+        got.append(now)
+    assert all(torch.equal(x, y) for x, y in zip(*got))
