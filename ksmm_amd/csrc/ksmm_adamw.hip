@@ -328,8 +328,7 @@ template <typename E, typename F> int in_tables(const Common &common, const Tens
     a.count = 0;
     for (int i = 0; i <= n; ++i) {
         const uint32_t more = i < n ? (all[i].n + a.chunk - 1) / a.chunk : 0;
-        // (a table's workgroups are counted in 31 bits)
-        if (a.count > 0 && (i == n || a.count == Args<E>::MOST || (uint64_t)groups + more > 0x7fffffffu)) {
+        if (a.count > 0 && (i == n || a.count == Args<E>::MOST || (int64_t)groups + more > THREADS_MOST / threads)) {
             a.seed = seed + (uint32_t)first;
             if (groups > 0) {
                 const int rc = launch(a, groups, threads);

@@ -99,6 +99,19 @@ static inline int launch_kernel(void (*fn)(P...), unsigned groups, unsigned thre
     return KSMM_ERR_LAUNCH;
 }
 
+// Workgroups in as many launches as it takes, launch(first, count): one of 2^32 threads and more starts what is left of them without 2^32,
+// and reports no error.
+constexpr int64_t THREADS_MOST = 0xffffffffLL;
+template <typename F> static inline int in_launches(int64_t groups, int threads, F launch)
+{
+    const int64_t most = THREADS_MOST / threads;
+    for (int64_t first = 0; first < groups; first += most) {
+        const int rc = launch((uint32_t)first, (unsigned)(groups - first < most ? groups - first : most));
+        if (rc != KSMM_OK) return rc;
+    }
+    return KSMM_OK;
+}
+
 // One factor problem, as the launchers see it.
 struct Problem {
     const void *x;

@@ -216,9 +216,9 @@ template <typename T, int D, bool BACK> __global__ __launch_bounds__(THREADS) vo
 {
     mx_runs<T, D, BACK>(p, blockIdx.x, gridDim.x);
 }
-template <typename T, bool BACK> __global__ __launch_bounds__(THREADS) void ks_mx_columns_kernel(MxOperand p)
+template <typename T, bool BACK> __global__ __launch_bounds__(THREADS) void ks_mx_columns_kernel(MxOperand p, uint32_t first)
 {
-    mx_columns<T, BACK>(p, blockIdx.x);
+    mx_columns<T, BACK>(p, first + blockIdx.x);
 }
 // ---- both operands of a product back to values, for its gradients: workgroups of the one behind those of the other (a launch each for
 // (2,96,72,3) fp32, 1970 rows takes 6.6 us, this one 3.9).  D: d_i of x together, 0 batch-size-last
@@ -313,7 +313,8 @@ template <typename T, int D, bool BACK> int convert_rows(const MxOperand &p, hip
 template <typename T, bool BACK> int convert(const MxOperand &p, hipStream_t s)
 {
     if (groups_of(p) > 0x7fffffffLL) return KSMM_ERR_TOO_LARGE;
-    if (p.last) return launch_kernel(&ks_mx_columns_kernel<T, BACK>, (unsigned)groups_of(p), THREADS, 0, s, p);
+    if (p.last)
+        return in_launches(groups_of(p), THREADS, [&](uint32_t first, unsigned groups) { return launch_kernel(&ks_mx_columns_kernel<T, BACK>, groups, THREADS, 0, s, p, first); });
     switch (mx_run_of(p.d)) {
     case 1: return convert_rows<T, 1, BACK>(p, s);
     case 2: return convert_rows<T, 2, BACK>(p, s);
@@ -325,7 +326,10 @@ template <typename T, bool BACK> int convert(const MxOperand &p, hipStream_t s)
 template <typename T> int values_of(const MxOperand &x, const MxOperand &w, hipStream_t s)
 {
     const int64_t x_groups = groups_of(x), w_groups = groups_of(w);
-    if (x_groups + w_groups > 0x7fffffffLL) return KSMM_ERR_TOO_LARGE;
+    if (x_groups + w_groups > THREADS_MOST / THREADS) {
+        const int rc = convert<T, true>(w, s);
+        return rc == KSMM_OK ? convert<T, true>(x, s) : rc;
+    }
     auto launch = [&](auto fn) { return launch_kernel(fn, (unsigned)(x_groups + w_groups), THREADS, 0, s, x, w, (uint32_t)w_groups); };
     switch (x.last ? 0 : mx_run_of(x.d)) {
     case 0: return launch(&ks_mx_values_kernel<T, 0>);

@@ -256,7 +256,7 @@ __global__ __launch_bounds__(64 * (MX_CONSUMERS + MX_PRODUCERS)) void ks_mx_held
     const int TN = p.tile_rows, buffer = D * TN * (p.slots * 16 + 2 * SB);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l32 = lane & 31, half = lane >> 5;
     const int run = 16 * ((l32 >> 2) & 1) + 4 * (l32 >> 3) + (l32 & 3);  // the row that this lane reads of the operand whose rows are dealt out
-    int blk = blockIdx.x;
+    int blk = (int)(p.first + blockIdx.x);
     const int first = blk % p.row_splits;
     blk /= p.row_splits;
     const int unit = blk % p.units, ai = unit / p.runs, d0 = (unit - ai * p.runs) * D;
@@ -388,7 +388,7 @@ template <typename T, bool LAST, int D, int TT, bool GATED, int ACT> __global__ 
     const int run = 16 * ((l32 >> 2) & 1) + 4 * (l32 >> 3) + (l32 & 3);  // the row that this lane reads of the operand whose rows are dealt out
     uint8_t *const codes = smem, *const scales = codes + (size_t)p.run_d * TN * p.slots * 16;
     T *const stage = (T *)(scales + (p.run_d * TN * p.cb + 15) / 16 * 16);  // of the workgroup: rows of `pitch`; batch-size-last of the waves
-    const uint32_t rest = blockIdx.x / (uint32_t)p.splits, split = blockIdx.x - rest * (uint32_t)p.splits, tile = rest / (uint32_t)p.units;
+    const uint32_t group = p.first + blockIdx.x, rest = group / (uint32_t)p.splits, split = group - rest * (uint32_t)p.splits, tile = rest / (uint32_t)p.units;
     const int unit = (int)(rest - tile * (uint32_t)p.units), ai = p.runs == 1 ? unit : unit / p.runs, d0 = (unit - ai * p.runs) * p.run_d;
     const int64_t n0 = (int64_t)tile * TN;
     const int here = (int)(p.batch - n0 < TN ? p.batch - n0 : TN);                 // rows of the batch
@@ -649,6 +649,15 @@ template <typename T, bool LAST, int D, int TT, bool GATED, int ACT> __global__ 
     }
 }
 
+// `grid` workgroups of a kernel
+inline int mx_launch(void (*fn)(MxProduct), MxProduct p, int64_t grid, int threads, int64_t lds, hipStream_t s)
+{
+    return in_launches(grid, threads, [&](uint32_t first, unsigned groups) {
+        p.first = first;
+        return launch_kernel(fn, groups, (unsigned)threads, (size_t)lds, s, p);
+    });
+}
+
 inline int64_t mx_held_lds(int d, bool gated, int ks, int cb, int rows, int tiles, int consumers)
 {
     return 2LL * d * rows * ((cb | 1) * 16 + 2 * mx_scale_bytes(ks)) + (int64_t)tiles * (gated ? 2 : 1) * 32 * d * 4 + consumers * MX_STAGE;
@@ -685,7 +694,7 @@ template <typename T, bool LAST, int D, int TT, bool GATED> int mx_launch_wide(M
         if constexpr (GATED || ACT != KSMM_ACT_SILU) {
             auto fn = &ks_mx_wide_kernel<T, LAST, D, TT, GATED, ACT>;
             if (lds > 64 * 1024) rc = ensure_dynamic_lds((const void *)fn, (int)MX_LDS_ALL);  // (set once a kernel: for all of its sizes)
-            if (rc == KSMM_OK) rc = launch_kernel(fn, (unsigned)grid, 64 * MX_WAVES, lds, s, p);
+            if (rc == KSMM_OK) rc = mx_launch(fn, p, grid, 64 * MX_WAVES, lds, s);
         }
     });
     return rc;
@@ -759,7 +768,7 @@ template <typename T, bool LAST, int D, bool GATED, int KS> int mx_launch_held(M
         if constexpr (GATED || ACT != KSMM_ACT_SILU) {
             auto fn = &ks_mx_held_kernel<T, LAST, D, GATED, ACT, KS>;
             if (lds > 64 * 1024) rc = ensure_dynamic_lds((const void *)fn, (int)MX_LDS_ALL);  // (set once a kernel: for all of its sizes)
-            if (rc == KSMM_OK) rc = launch_kernel(fn, (unsigned)grid, 64 * (MX_CONSUMERS + MX_PRODUCERS), lds, s, p);
+            if (rc == KSMM_OK) rc = mx_launch(fn, p, grid, 64 * (MX_CONSUMERS + MX_PRODUCERS), lds, s);
         }
     });
     return rc;

@@ -33,7 +33,7 @@ __global__ __launch_bounds__(64 * (mx_slope_waves<T, D>() + MX_PRODUCERS)) void 
     const int buffer = dy_at + (LAST ? p.wave_tiles * 32 : TN) * pitch;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l32 = lane & 31, half = lane >> 5;
     const int run = 16 * ((l32 >> 2) & 1) + 4 * (l32 >> 3) + (l32 & 3);  // the row that this lane reads of the operand whose rows are dealt out
-    int blk = blockIdx.x;
+    int blk = (int)(p.first + blockIdx.x);
     const int first = blk % p.row_splits;
     blk /= p.row_splits;
     const int unit = blk % p.units, ai = unit / p.runs, d0 = (unit - ai * p.runs) * D;
@@ -185,7 +185,7 @@ template <typename T, bool LAST, int D, bool GATED, int KS> int mx_launch_slope(
         if constexpr (GATED || ACT == KSMM_ACT_GELU) {
             auto fn = &ks_mx_slope_kernel<T, LAST, D, GATED, ACT, KS>;
             if (lds > 64 * 1024) rc = ensure_dynamic_lds((const void *)fn, (int)MX_LDS_ALL);  // (set once a kernel: for all of its sizes)
-            if (rc == KSMM_OK) rc = launch_kernel(fn, (unsigned)grid, 64 * (C + MX_PRODUCERS), lds, s, p);
+            if (rc == KSMM_OK) rc = mx_launch(fn, p, grid, 64 * (C + MX_PRODUCERS), lds, s);
         }
     });
     return rc;

@@ -217,3 +217,32 @@ def test_an_error_from_before_is_not_the_calls_own(monkeypatch, native):
         assert (left != 0) == before
         got.append(now)
     assert all(torch.equal(x, y) for x, y in zip(*got))
+
+
+@pytest.mark.parametrize("bs_last", [False, True])
+@pytest.mark.parametrize("prec", ["fp32", "fp16"])
+def test_more_workgroups_than_a_launch_takes(prec, bs_last):
+    """2^32 threads and more: blocks of one number each, whose product is that of two numbers."""
+    from ksmm_amd import MXKernel, pack_mx, quantize_mx
+    from ksmm_amd.mx import _slope
+
+    a = 16_800_000
+    g = torch.Generator(device="cuda").manual_seed(0)
+    f = torch.randn(a, 1, device="cuda", generator=g).to(DT[prec])
+    w = pack_mx(f, (a, 1, 1, 1))
+    wq = w.dequantize(torch.float32).flatten()
+    assert bool(((wq - f.flatten().float()).abs() <= 0.25 * f.flatten().float().abs()).all())  # (saturation: 7.99 of 8 is 6)
+    for n in (1, 3):
+        x = torch.randn(*((a, n) if bs_last else (n, a)), device="cuda", generator=g).to(DT[prec])
+        q = quantize_mx(x, (a, 1, 1), bs_last)
+        xq = q.dequantize(torch.float32)
+        z = xq * (wq.unsqueeze(1) if bs_last else wq)  # (exact: three bits by three)
+        y, codes, scales = MXKernel.forward(x, w, None, None, bs_last, need_codes=True)
+        assert torch.equal(y, z.to(DT[prec])) and torch.equal(codes, q.codes) and torch.equal(scales, q.scales)
+        assert torch.equal(MXKernel.forward(q, w, None, None, bs_last), y)
+        del y, codes, scales
+        dz = _slope(torch.ones_like(x), q, w, None, "gelu", bs_last)
+        with torch.enable_grad():
+            z.requires_grad_(True)
+            want, = torch.autograd.grad(torch.nn.functional.gelu(z).sum(), z)
+        assert bool(((dz.float() - want).abs() <= (2.0 ** -11 if prec == "fp16" else 2e-6) * want.abs() + 2e-6).all())
