@@ -454,9 +454,15 @@ class KSFeedForwardMX(KSFeedForward):
         return pack_block(self)
 
 
+def _shell(module):
+    """A copy of a module with what it has, whose modules, parameters, buffers and hooks are registered for itself."""
+    new = copy.copy(module)
+    new.__dict__.update({k: v.copy() for k, v in module.__dict__.items() if isinstance(v, (dict, set))})
+    return new
+
+
 def pack_block(block):
     """A copy of a ``KSFeedForward`` whose factors are packed; its norm is copied too."""
-    new = copy.copy(block)
-    new._modules, new._parameters, new._buffers = dict(block._modules), dict(block._parameters), dict(block._buffers)
+    new = _shell(block)
     new.gated, new.down, new.norm = MXLinear.of(block.gated), MXLinear.of(block.down), copy.deepcopy(block.norm)
     return new

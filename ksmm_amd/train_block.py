@@ -8,7 +8,6 @@ random rows.  ``KSMuon`` updates the factors, SGD with momentum the norms' weigh
 come from packed factors.  A single row runs as a captured graph, whose results are compared with the eager ones.  One JSON
 line: losses (of the targets' variance, before and after), time of a training step, time of a row."""
 import argparse
-import copy
 import json
 import time
 
@@ -18,7 +17,7 @@ from torch import nn
 from .adamw import KSAdamW
 from .block import KSFeedForward
 from .muon import KSMuon
-from .mx import KSFeedForwardMX, pack_block
+from .mx import KSFeedForwardMX, _shell, pack_block
 
 
 class KSStack(nn.Module):
@@ -31,8 +30,8 @@ class KSStack(nn.Module):
 
     def packed(self):
         """A copy whose factors are microscaled 4-bit numbers."""
-        new = copy.copy(self)
-        new._modules = {"blocks": nn.ModuleList(pack_block(b) for b in self.blocks)}
+        new = _shell(self)
+        new.blocks = nn.ModuleList(pack_block(b) for b in self.blocks)
         return new
 
     def forward(self, residual):

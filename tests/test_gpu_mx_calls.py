@@ -246,3 +246,19 @@ def test_more_workgroups_than_a_launch_takes(prec, bs_last):
             z.requires_grad_(True)
             want, = torch.autograd.grad(torch.nn.functional.gelu(z).sum(), z)
         assert bool(((dz.float() - want).abs() <= (2.0 ** -11 if prec == "fp16" else 2e-6) * want.abs() + 2e-6).all())
+
+
+def test_copies_have_hooks_of_their_own():
+    from ksmm_amd import KSFeedForwardMX
+    from ksmm_amd.train_block import KSStack
+
+    block = KSFeedForwardMX((1, 64, 32, 2), [(1, 32, 64, 2)])
+    stack = KSStack((1, 64, 32, 2), [(1, 32, 64, 2)], 1, mx=True)
+    for module in (block, stack):
+        copy = module.packed()
+        calls = []
+        copy.register_forward_hook(lambda *a: calls.append("copy"))
+        copy.register_forward_pre_hook(lambda *a: calls.append("copy"))
+        assert not module._forward_hooks and not module._forward_pre_hooks
+        copy.register_buffer("more", torch.zeros(1), persistent=False)
+        assert not hasattr(module, "more") and not module._non_persistent_buffers_set
