@@ -53,7 +53,7 @@ typedef enum ksmm_status {
     KSMM_ERR_BAD_PATTERN = -2,    /* a, b, c or d < 1                                         */
     KSMM_ERR_BAD_BATCH = -3,      /* batch < 1                                                */
     KSMM_ERR_BAD_DTYPE = -4,      /* (x, w, y) type combination not in the list above         */
-    KSMM_ERR_TOO_LARGE = -5,      /* a tensor has 2^31 elements or more                       */
+    KSMM_ERR_TOO_LARGE = -5,      /* a tensor has 2^31 elements or more, or a launch would have 2^32 threads */
     KSMM_ERR_BAD_ALGO = -6,       /* forced kernel id unknown, or it cannot run this problem  */
     KSMM_ERR_LAUNCH = -7,         /* HIP reported an error at launch                          */
     KSMM_ERR_CHAIN_MISMATCH = -8, /* output size of factor i != input size of factor i+1      */

@@ -232,7 +232,7 @@ int launch(const void *dy, const void *z, void *dz, float *part, void *dbias, in
            hipStream_t s)
 {
     const int64_t blocks = bs_last ? (features * p.splits + 3) / 4 : p.splits * p.col_blocks;
-    if (blocks > 0x7fffffffLL) return KSMM_ERR_TOO_LARGE;
+    if (blocks > THREADS_MOST / 256) return KSMM_ERR_TOO_LARGE;
     if (bs_last)
         hipLaunchKernelGGL((ks_act_bwd_bl_kernel<T, VEC, ACT>), dim3((unsigned)blocks), dim3(256), 0, s, (const T *)dy, (const T *)z,
                            (T *)dz, part, (T *)dbias, batch, features, (int)p.splits, p.size);

@@ -553,7 +553,7 @@ int launch_wgrad_bl(const void *dy, const void *x, float *acc, int64_t batch, in
 {
     const auto [splits, cols] = wgrad_bl_split(batch, a, b, c, d, elem<T>::dtype);
     const int64_t waves = (int64_t)a * d * splits, blocks = (waves + 3) / 4;
-    if (blocks > 0x7fffffffLL) return KSMM_ERR_TOO_LARGE;
+    if (blocks > THREADS_MOST / 256) return KSMM_ERR_TOO_LARGE;
     *splits_used = (int)splits;
     const bool whole = wgrad_aligned(dy, x, batch, elem<T>::dtype);
     auto fn = whole ? &ks_wgrad_bl_kernel<T, 1, true, false> : &ks_wgrad_bl_kernel<T, 1, false, true>;
@@ -574,7 +574,7 @@ int launch_wgrad_tiled(const void *dy, const void *x, float *acc, int64_t batch,
     int64_t splits, cols;
     wgrad_tiled_splits(batch, tiles, &splits, &cols);
     const int64_t blocks = tiles * splits;
-    if (blocks > 0x7fffffffLL) return KSMM_ERR_TOO_LARGE;
+    if (blocks > THREADS_MOST / 256) return KSMM_ERR_TOO_LARGE;
     *splits_used = (int)splits;
     const int64_t slice = (int64_t)a * b * c * d;
     if (bs_last)
@@ -594,7 +594,7 @@ int launch_wgrad_gemm_tile(const void *dy, const void *x, float *acc, int64_t ba
     const int64_t tiles = (int64_t)a * d * m_tiles * n_tiles;
     const auto [splits, cols] = wgrad_gemm_split(batch, a, b, c, d, elem<T>::dtype);
     const int64_t blocks = (splits * tiles + 7) / 8 * 8;
-    if (blocks > 0x7fffffffLL) return KSMM_ERR_TOO_LARGE;
+    if (blocks > THREADS_MOST / 256) return KSMM_ERR_TOO_LARGE;
     *splits_used = (int)splits;
     const auto fn = wgrad_aligned(dy, x, batch, elem<T>::dtype) ? &ks_wgrad_gemm_kernel<T, TM, TN, false> : &ks_wgrad_gemm_kernel<T, TM, TN, true>;
     const int lds = 2 * (TM + TN) * 128;
@@ -647,7 +647,7 @@ int block_transpose_run(const TransposeJob *jobs, int n, int dtype, hipStream_t 
         // 11.7 / 12.5, (16,64,64,16) 8.9 / 10.3, (6,192,192,16) 19 / 28.
         if (total <= squares * 512 || total <= 1 << 18) o.b_tiles = 0;
         blocks += o.b_tiles ? squares : (total + 255) / 256;
-        if (blocks > 0x7fffffffLL) return KSMM_ERR_TOO_LARGE;
+        if (blocks > THREADS_MOST / 256) return KSMM_ERR_TOO_LARGE;
     }
     if (n < 1) return KSMM_OK;
     if (dtype == KSMM_F32)
@@ -689,7 +689,7 @@ int finish_run(const FinishJob *jobs, int n, int dtype, hipStream_t stream)
         o.first = (uint32_t)blocks;
         const int64_t per = finish_outputs(j.n, j.splits);
         blocks += (j.n + per - 1) / per;
-        if (blocks > 0x7fffffffLL) return KSMM_ERR_TOO_LARGE;
+        if (blocks > THREADS_MOST / 256) return KSMM_ERR_TOO_LARGE;
     }
     if (f.jobs < 1) return KSMM_OK;
     if (dtype == KSMM_F32)

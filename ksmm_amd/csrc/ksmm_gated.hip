@@ -871,7 +871,7 @@ template <typename T, bool LAST, int MODE> int run_few(const GatedArgs &g, hipSt
 {
     const int b_tiles = (g.b + 15) / 16;
     const int64_t blocks = (int64_t)b_tiles * g.a * g.d * ((g.batch + 31) / 32);
-    if (blocks > 0x7ffffff0LL) return KSMM_ERR_TOO_LARGE;
+    if (blocks > THREADS_MOST / (64 * FEW_WAVES) - 8) return KSMM_ERR_TOO_LARGE;
     hipLaunchKernelGGL((ks_gated_few_kernel<T, LAST, MODE>), dim3((unsigned)((blocks + 7) / 8 * 8)), dim3(64 * FEW_WAVES), 0, s, g, b_tiles, (int)blocks);
     return launched();
 }
@@ -881,7 +881,7 @@ template <typename T, bool LAST, int D, bool ALL, int TB, int TN, int TK, int WB
     typedef Tile<T, LAST, D, TB, TN, TK, WB, WN> C;
     const int b_tiles = (g.b + TB - 1) / TB;
     const int64_t n_tiles = (g.batch + TN - 1) / TN, blocks = (int64_t)b_tiles * g.a * (g.d / D) * n_tiles;
-    if (blocks > 0x7ffffff0LL) return KSMM_ERR_TOO_LARGE;
+    if (blocks > THREADS_MOST / C::THREADS - 8) return KSMM_ERR_TOO_LARGE;
     const auto fn = &ks_gated_kernel<T, LAST, D, ALL, TB, TN, TK, WB, WN, MODE>;
     if (C::LDS_BYTES > 64 * 1024) {
         const int rc = ensure_dynamic_lds((const void *)fn, C::LDS_BYTES);

@@ -1522,7 +1522,7 @@ int gemm_run(const Problem &p, int variant, bool launch, ksmm_tile *tile)
     const int64_t blocks = groups * m_tiles * n_tiles;
     int64_t grid = (blocks + 7) / 8 * 8;
     if (t.pers && grid > 256 * t.pers) grid = 256 * t.pers;  // persistent workgroups: pers per CU
-    if (grid > 0x7fffffffLL) return KSMM_ERR_TOO_LARGE;
+    if (grid > THREADS_MOST / t.threads) return KSMM_ERR_TOO_LARGE;
     if (tile) {
         tile->algo = KSMM_ALGO_TILE;
         tile->variant = (4 << 24) | pick;

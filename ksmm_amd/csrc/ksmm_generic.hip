@@ -196,7 +196,7 @@ int generic_run(const Problem &p, int variant, bool launch, ksmm_tile *tile)
         const int bt = 8;
         const int64_t n_blocks = (p.batch / vec + 255) / 256, b_chunks = (p.b + bt - 1) / bt;
         const int64_t grid = (int64_t)p.a * p.d * n_blocks * b_chunks;
-        if (grid > 0x7fffffffLL) return KSMM_ERR_TOO_LARGE;
+        if (grid > THREADS_MOST / 256) return KSMM_ERR_TOO_LARGE;
         if (tile) {
             tile->algo = KSMM_ALGO_GENERIC;
             tile->variant = 1;
@@ -222,7 +222,7 @@ int generic_run(const Problem &p, int variant, bool launch, ksmm_tile *tile)
     const int64_t fast = p.bs_last ? p.batch : out_size;
     const int64_t slow = p.bs_last ? out_size : p.batch;
     const int64_t nblocks = ((fast + threads - 1) / threads) * slow;
-    if (nblocks > 0x7fffffffLL) return KSMM_ERR_TOO_LARGE;
+    if (nblocks > THREADS_MOST / threads) return KSMM_ERR_TOO_LARGE;
     dim3 grid((unsigned)nblocks, 1, 1);
     if (tile) {
         tile->algo = KSMM_ALGO_GENERIC;

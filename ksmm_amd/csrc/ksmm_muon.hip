@@ -591,6 +591,7 @@ template <typename T, int WAVES, int HELD> int run_block(const MuonArgs &a, int6
         const int rc = ensure_dynamic_lds((const void *)fn, (int)LDS_MOST);
         if (rc != KSMM_OK) return rc;
     }
+    if (matrices > THREADS_MOST / (64 * WAVES)) return KSMM_ERR_TOO_LARGE;
     hipLaunchKernelGGL(fn, dim3((unsigned)matrices), dim3(64 * WAVES), lds, s, a);
     return launched();
 }
@@ -634,7 +635,7 @@ template <typename T> int run(const MuonArgs &a, int64_t matrices, char *ws, hip
     }
     const Space w = space(matrices, a.c, a.b);
     const int64_t mt = w.M / TILE, square = matrices * mt * mt, full = matrices * mt * (w.N / TILE);
-    if (full > 0x7fffffffLL || matrices * w.chunks > 0x7fffffffLL) return KSMM_ERR_TOO_LARGE;
+    if (full > THREADS_MOST / 512 - 8 || matrices * w.chunks > THREADS_MOST / 256) return KSMM_ERR_TOO_LARGE;
     const bool flip = a.c > a.b;
     auto split = [&](int64_t at, int64_t values) { return Split{(half_t *)(ws + at), (half_t *)(ws + at) + values}; };
     const int64_t values = matrices * w.M * w.N;

@@ -1314,6 +1314,7 @@ template <typename T> int forward(const NormArgs &a, int bs_last, float *ws, hip
         return with_cols<T>(a.batch, a.features, false, [&](auto lanes, auto fpt, auto one) {
             constexpr int LANES = decltype(lanes)::value;
             const int tiles = (int)((a.batch + 4 * LANES - 1) / (4 * LANES));
+            if (tiles > THREADS_MOST / COL_THREADS - 8) return (int)KSMM_ERR_TOO_LARGE;
             hipLaunchKernelGGL((ks_norm_cols_kernel<T, LANES, decltype(fpt)::value, decltype(one)::value>), dim3((tiles + 7) / 8 * 8),
                                dim3(COL_THREADS), 0, stream, a, tiles);
             return launched();
@@ -1343,6 +1344,7 @@ template <typename T> int backward(const NormArgs &a, const NormGrads &partial, 
         return with_cols<T>(a.batch, a.features, true, [&](auto lanes, auto fpt, auto one) {
             constexpr int LANES = decltype(lanes)::value;
             const int tiles = (int)((a.batch + 4 * LANES - 1) / (4 * LANES));
+            if (tiles > THREADS_MOST / COL_THREADS - 8) return (int)KSMM_ERR_TOO_LARGE;
             hipLaunchKernelGGL((ks_norm_cols_bwd_kernel<T, LANES, decltype(fpt)::value, decltype(one)::value>), dim3((tiles + 7) / 8 * 8),
                                dim3(COL_THREADS), 0, stream, a, partial, tiles);
             return launched();

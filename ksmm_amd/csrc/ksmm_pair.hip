@@ -348,7 +348,7 @@ bool pair_plan(const ksmm_factor_desc *f, int n, int64_t batch, int x_dtype, int
     p->m_tiles = (b1 + 64 * s.mg - 1) / (64 * s.mg);
     p->tiles = (int64_t)f[1].a * (d1 / p->dg) * p->m_tiles;
     p->grid = p->tiles * ((batch + 16 * s.nt - 1) / (16 * s.nt));
-    return p->grid <= 0x7fffffffLL;
+    return p->grid <= THREADS_MOST / (64 * PAIR_WAVES);
 }
 
 }  // namespace

@@ -248,7 +248,7 @@ int decode_run(const DecodeJob *jobs, int n, hipStream_t stream)
         d.job[i].n = jobs[i].n;
         d.job[i].first = (uint32_t)blocks;
         blocks += (jobs[i].n + 256 * RUN - 1) / (256 * RUN);
-        if (blocks > 0x7fffffffLL) return KSMM_ERR_TOO_LARGE;
+        if (blocks > THREADS_MOST / 256) return KSMM_ERR_TOO_LARGE;
     }
     if (blocks < 1) return KSMM_OK;
     hipLaunchKernelGGL(ks_decode_kernel, dim3((unsigned)blocks), dim3(256), 0, stream, d);

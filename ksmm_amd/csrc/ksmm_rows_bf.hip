@@ -623,7 +623,7 @@ int rows_bf_run(const Problem &p, int variant, bool launch, ksmm_tile *tile)
     if (wgs > n_tiles) wgs = n_tiles;
     // (groups of one a_i that take the same tiles sit 8 block indices apart: see the kernels)
     const int64_t grid = t.ag ? ag * wgs : 8 * (int64_t)(p.d / t.dd) * (((int64_t)p.a * wgs + 7) / 8);
-    if (grid > 0x7fffffffLL) return KSMM_ERR_TOO_LARGE;
+    if (grid > THREADS_MOST / (64 * nw)) return KSMM_ERR_TOO_LARGE;
     if (tile) {
         tile->algo = KSMM_ALGO_WAVE;
         tile->variant = 1000 + pick;

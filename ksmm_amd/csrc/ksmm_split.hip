@@ -358,7 +358,7 @@ int split_run(const Problem &p, int variant, bool launch, ksmm_tile *tile)
     if (ks > steps) ks = steps;
     const int64_t d_groups = p.d / t.dd, tiles = (int64_t)p.a * d_groups * m_tiles;
     const int64_t n_tiles = (p.batch + tn - 1) / tn, grid = (tiles + 7) / 8 * 8 * n_tiles;
-    if (grid > 0x7fffffffLL) return KSMM_ERR_TOO_LARGE;
+    if (grid > THREADS_MOST / (64 * ks)) return KSMM_ERR_TOO_LARGE;
     const int lds = ks > 1 ? ks * tiles_w * 1024 : 0;  // at most 64 KB
     if (tile) {
         tile->algo = KSMM_ALGO_TILE;

@@ -431,7 +431,7 @@ int stream_run(const Problem &p, int variant, bool launch, ksmm_tile *tile)
     const int64_t n_tiles = (p.batch + t.tn - 1) / t.tn;
     if (wgs > n_tiles) wgs = n_tiles;
     const int64_t grid = groups * wgs;
-    if (grid > 0x7fffffffLL) return KSMM_ERR_TOO_LARGE;
+    if (grid > THREADS_MOST / t.threads) return KSMM_ERR_TOO_LARGE;
     if (tile) {
         tile->algo = KSMM_ALGO_TILE;
         tile->variant = (2 << 24) | pick;

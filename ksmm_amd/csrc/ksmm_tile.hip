@@ -515,7 +515,7 @@ int ws_run(const Problem &p, int variant, int wgs_hint, bool launch, ksmm_tile *
     if (wgs > n_tiles) wgs = n_tiles;
     if (wgs < 1) wgs = 1;
     const int64_t grid = groups * wgs;
-    if (grid > 0x7fffffffLL) return KSMM_ERR_TOO_LARGE;
+    if (grid > THREADS_MOST / t.threads) return KSMM_ERR_TOO_LARGE;
     if (tile) {
         tile->algo = KSMM_ALGO_TILE;
         tile->variant = (1 << 24) | pick;
@@ -726,7 +726,7 @@ int tile_run(const Problem &p, int variant, bool launch, ksmm_tile *tile)
     const int64_t n_tiles = (p.batch + t.tn - 1) / t.tn;
     const int64_t blocks = (int64_t)p.a * p.d * m_tiles * n_tiles;
     const int64_t grid = (blocks + 7) / 8 * 8;
-    if (grid > 0x7fffffffLL) return KSMM_ERR_TOO_LARGE;
+    if (grid > THREADS_MOST / t.threads) return KSMM_ERR_TOO_LARGE;
     if (tile) {
         tile->algo = KSMM_ALGO_TILE;
         tile->variant = pick | (ragged ? 1 << 8 : 0);

@@ -1298,7 +1298,7 @@ int tile_bf_run(const Problem &p, int variant, bool launch, ksmm_tile *tile)
     const int64_t n_tiles = (p.batch + t.tn - 1) / t.tn;
     const int64_t blocks = (int64_t)p.a * (p.d / t.dd) * m_tiles * n_tiles;
     const int64_t grid = (blocks + 7) / 8 * 8;
-    if (grid > 0x7fffffffLL) return KSMM_ERR_TOO_LARGE;
+    if (grid > THREADS_MOST / t.threads) return KSMM_ERR_TOO_LARGE;
     if (tile) {
         tile->algo = KSMM_ALGO_TILE;
         tile->variant = (3 << 24) | pick;

@@ -180,7 +180,7 @@ int repitch_run(const void *in, void *out, int64_t rows, int64_t cols_in, int64_
     const bool vout = cols_out % v == 0 && ((uintptr_t)out & 15) == 0;
     const int64_t vec_per_row = (cols_out + v - 1) / v;
     const int64_t blocks = (rows * vec_per_row + 255) / 256;
-    if (blocks > 0x7fffffffLL) return KSMM_ERR_TOO_LARGE;
+    if (blocks > THREADS_MOST / 256) return KSMM_ERR_TOO_LARGE;
     const void *fn = elem_bytes == 4 ? repitch_fn<4>(vin, vout)
                                      : elem_bytes == 2 ? repitch_fn<2>(vin, vout) : repitch_fn<1>(vin, vout);
     int ci = (int)cols_in, co = (int)cols_out, vpr = (int)vec_per_row;
@@ -205,7 +205,7 @@ int transpose_run(const void *in, void *out, int64_t rows, int64_t cols, int ele
     const void *fn = elem_bytes == 4 ? transpose_fn<4>(vin, vout)
                                      : elem_bytes == 2 ? transpose_fn<2>(vin, vout) : transpose_fn<1>(vin, vout);
     const int64_t tiles_r = (rows + TT - 1) / TT, tiles_c = (cols + TT - 1) / TT;
-    if (tiles_r * tiles_c > 0x7fffffffLL) return KSMM_ERR_TOO_LARGE;
+    if (tiles_r * tiles_c > THREADS_MOST / 256) return KSMM_ERR_TOO_LARGE;
     int rows_i = (int)rows, cols_i = (int)cols, tiles_c_i = (int)tiles_c, ip = (int)in_pitch, op = (int)out_pitch;
     void *args[] = {(void *)&in, (void *)&out, &rows_i, &cols_i, &tiles_c_i, &ip, &op};
     hipError_t e = hipLaunchKernel(fn, dim3((unsigned)(tiles_r * tiles_c)), dim3(256), args, 0, stream);

@@ -846,7 +846,7 @@ int wave_run(const Problem &p, int variant, bool launch, ksmm_tile *tile)
         const int64_t n_slabs = (n_tiles + iters - 1) / iters;
         const int64_t waves = groups * n_slabs;
         const int64_t blocks = (waves + wpw - 1) / wpw;
-        if (blocks > 0x7fffffffLL) return KSMM_ERR_TOO_LARGE;
+        if (blocks > THREADS_MOST / (64 * wpw)) return KSMM_ERR_TOO_LARGE;
         const int lds = wpw * ks * 1024;
         if (tile) {
             tile->algo = KSMM_ALGO_WAVE;
@@ -907,7 +907,7 @@ int wave_run(const Problem &p, int variant, bool launch, ksmm_tile *tile)
     const int64_t m_split = p.b / in.b;
     if (combo == 0 && !in.ring && m_split > wpb && m_split % wpb == 0)
         blocks = 8 * (m_split / wpb) * (((int64_t)p.a * p.d * n_slabs + 7) / 8);
-    if (blocks > 0x7fffffffLL) return KSMM_ERR_TOO_LARGE;
+    if (blocks > THREADS_MOST / (64 * wpb)) return KSMM_ERR_TOO_LARGE;
     if (tile) {
         tile->algo = KSMM_ALGO_WAVE;
         tile->variant = pick | (iters_field << 8) | (rr << 16);

@@ -362,7 +362,7 @@ template <typename T, int TT, bool TWO> int launch(const void *dy, const void *x
     constexpr int CH = TT == 1 ? 16 : TT == 2 ? 8 : 4;
     const int64_t tiles = (int64_t)g.a_groups * g.d_groups * g.m_groups * g.n_groups;
     const int64_t blocks = g.splits >= 8 ? (int64_t)((g.splits + 7) / 8 * 8) * tiles : g.splits * tiles;
-    if (blocks > 0x7fffffffLL) return KSMM_ERR_TOO_LARGE;
+    if (blocks > THREADS_MOST / (64 * g.ta * g.td * g.wm * g.wn)) return KSMM_ERR_TOO_LARGE;
     const int lds = (TWO ? 2 : 1) * (g.ta * g.td * (g.wm + g.wn) * 16 * TT * CH + 1) * 16;
     constexpr int MOST = (TWO ? 2 : 1) * (8 * 2 * 16 * TT * CH + 1) * 16;  // eight waves (the limit is set once a kernel)
     const int rc = ensure_dynamic_lds((const void *)ks_wgrad_bf_kernel<T, TT, CH, TWO>, MOST);

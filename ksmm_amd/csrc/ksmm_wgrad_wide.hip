@@ -303,7 +303,7 @@ int wgrad_wide_run(const void *dy, const void *x, void *dw, float *acc, int64_t 
     if (!p.inst) return KSMM_ERR_BAD_ALGO;
     *splits = p.g.splits;
     const int64_t blocks = ((int64_t)p.g.splits * p.g.tiles + 7) / 8 * 8;
-    if (blocks > 0x7fffffffLL) return KSMM_ERR_TOO_LARGE;
+    if (blocks > THREADS_MOST / p.inst->threads) return KSMM_ERR_TOO_LARGE;
     const int rc = ensure_dynamic_lds(p.inst->fn, p.inst->lds);
     if (rc != KSMM_OK) return rc;
     void *args[] = {(void *)&dy, (void *)&x, (void *)&acc, (void *)&dw, &p.g};
