@@ -1011,7 +1011,7 @@ const char *ksmm_strerror(int status)
     case KSMM_ERR_BAD_PATTERN: return "pattern (a,b,c,d) must be four positive integers";
     case KSMM_ERR_BAD_BATCH: return "batch size must be positive";
     case KSMM_ERR_BAD_DTYPE: return "unsupported data type combination";
-    case KSMM_ERR_TOO_LARGE: return "tensor too large (2^31 elements or more)";
+    case KSMM_ERR_TOO_LARGE: return "tensor too large (2^31 elements or more), or a launch of 2^32 threads or more";
     case KSMM_ERR_BAD_ALGO: return "kernel family/variant unknown or not applicable to this problem";
     case KSMM_ERR_LAUNCH: return "HIP kernel launch failed";
     case KSMM_ERR_CHAIN_MISMATCH: return "consecutive factors have incompatible sizes";

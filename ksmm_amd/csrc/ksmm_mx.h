@@ -212,6 +212,7 @@ struct MxProduct {
     void *y;
     const void *dy;  // (gradients only)
     bool finite;     // of codes, without an activation: results beyond the type's range are its largest (gradients only)
+    uint32_t first;  // workgroup of the launch, of all
     int64_t batch;
     int a, b, c, d, cb;
     int slots;                    // of 16 bytes in LDS for a row's codes, odd
@@ -222,7 +223,6 @@ struct MxProduct {
     int raw_rows, raw_pitch;     // rows at a time whose values go through LDS on their way to codes (0: straight), and values from one to the next
     int tile_rows, wave_tiles;   // rows a step, and of a workgroup's waves those that lie along the outputs
     int row_splits;              // workgroups that share the steps
-    uint32_t first;              // workgroup of the launch, of all
     MxDiv by_cb, by_run_d;
 };
 int mx_slope_half(const MxProduct &p, bool last, bool gated, int act, hipStream_t s);

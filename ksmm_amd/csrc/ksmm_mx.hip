@@ -22,6 +22,7 @@ struct MxOperand {
     int64_t rows;
     int a, c, d, cb;
     bool last;
+    uint32_t first;  // workgroup of the launch, of all (batch-size-last)
     int64_t blocks;  // a * d * rows * cb
     bool small;      // tasks that the two divide by multiplying
     MxDiv by_cb, by_a;
@@ -216,9 +217,9 @@ template <typename T, int D, bool BACK> __global__ __launch_bounds__(THREADS) vo
 {
     mx_runs<T, D, BACK>(p, blockIdx.x, gridDim.x);
 }
-template <typename T, bool BACK> __global__ __launch_bounds__(THREADS) void ks_mx_columns_kernel(MxOperand p, uint32_t first)
+template <typename T, bool BACK> __global__ __launch_bounds__(THREADS) void ks_mx_columns_kernel(MxOperand p)
 {
-    mx_columns<T, BACK>(p, first + blockIdx.x);
+    mx_columns<T, BACK>(p, p.first + blockIdx.x);
 }
 // ---- both operands of a product back to values, for its gradients: workgroups of the one behind those of the other (a launch each for
 // (2,96,72,3) fp32, 1970 rows takes 6.6 us, this one 3.9).  D: d_i of x together, 0 batch-size-last
@@ -314,7 +315,11 @@ template <typename T, bool BACK> int convert(const MxOperand &p, hipStream_t s)
 {
     if (groups_of(p) > 0x7fffffffLL) return KSMM_ERR_TOO_LARGE;
     if (p.last)
-        return in_launches(groups_of(p), THREADS, [&](uint32_t first, unsigned groups) { return launch_kernel(&ks_mx_columns_kernel<T, BACK>, groups, THREADS, 0, s, p, first); });
+        return in_launches(groups_of(p), THREADS, [&](uint32_t first, unsigned groups) {
+            MxOperand part = p;
+            part.first = first;
+            return launch_kernel(&ks_mx_columns_kernel<T, BACK>, groups, THREADS, 0, s, part);
+        });
     switch (mx_run_of(p.d)) {
     case 1: return convert_rows<T, 1, BACK>(p, s);
     case 2: return convert_rows<T, 2, BACK>(p, s);
@@ -368,7 +373,7 @@ MxOperand operand(const void *x, void *codes, void *scales, int64_t rows, int a,
     const int cb = (int)mx_blocks(c);
     // (MxDiv: t d < 2^32 of the largest t)
     const int64_t tasks = (int64_t)a * rows * cb;
-    return MxOperand{x,  (uint8_t *)codes, (uint8_t *)scales, rows, a, c, d, cb, bs_last != 0, (int64_t)a * d * rows * cb, tasks < (1LL << 32) / std::max(a, cb) && tasks < 1LL << 31,
+    return MxOperand{x,  (uint8_t *)codes, (uint8_t *)scales, rows, a, c, d, cb, bs_last != 0, 0, (int64_t)a * d * rows * cb, tasks < (1LL << 32) / std::max(a, cb) && tasks < 1LL << 31,
                      MxDiv(cb), MxDiv(a)};
 }
 int64_t values(int64_t rows, int a, int c, int d) { return rows * a * c * d; }
@@ -476,7 +481,7 @@ int ksmm_mx_forward(const void *x, const void *x_scales, const void *w, const vo
                        {bias, (int64_t)a * rows_w * d * size}};
     const Span out[] = {{y, values(batch, a, b, d) * size}, {codes_out, blocks * 16}, {scales_out, blocks}, {need ? workspace : nullptr, need}};
     if (any_overlap(in, out)) return KSMM_ERR_ALIAS;
-    MxProduct p{x, (const uint8_t *)x_scales, (uint8_t *)codes_out, (uint8_t *)scales_out, (const uint8_t *)w, (const uint8_t *)w_scales, bias, y, nullptr, false, batch, a, b, c, d, cb};
+    MxProduct p{x, (const uint8_t *)x_scales, (uint8_t *)codes_out, (uint8_t *)scales_out, (const uint8_t *)w, (const uint8_t *)w_scales, bias, y, nullptr, false, 0, batch, a, b, c, d, cb};
     hipStream_t s = (hipStream_t)stream;
     if (need > 0) {  // (no workgroup's LDS holds the codes: x is quantised in a launch of its own)
         uint8_t *const codes = codes_out ? (uint8_t *)codes_out : (uint8_t *)workspace;
@@ -501,7 +506,7 @@ int ksmm_mx_sums(const void *x, const void *x_scales, const void *w, const void 
     const Span in[] = {{x, blocks * 16}, {x_scales, blocks}, {w, w_blocks * 16}, {w_scales, w_blocks}, {bias, (int64_t)a * b * d * size}};
     const Span out[] = {{z, values(batch, a, b, d) * size}};
     if (any_overlap(in, out)) return KSMM_ERR_ALIAS;
-    const MxProduct p{x, (const uint8_t *)x_scales, nullptr, nullptr, (const uint8_t *)w, (const uint8_t *)w_scales, bias, z, nullptr, true, batch, a, b, c, d, cb};
+    const MxProduct p{x, (const uint8_t *)x_scales, nullptr, nullptr, (const uint8_t *)w, (const uint8_t *)w_scales, bias, z, nullptr, true, 0, batch, a, b, c, d, cb};
     return launch_product(p, dtype, bs_last != 0, false, KSMM_ACT_NONE, (hipStream_t)stream);
 }
 
@@ -512,7 +517,7 @@ int ksmm_mx_slope(const void *x, const void *x_scales, const void *w, const void
     if (rc != KSMM_OK) return rc;
     if (!gated && act == KSMM_ACT_NONE) return KSMM_ERR_BAD_EPILOGUE;
     const int rows_w = gated ? 2 * b : b, cb = (int)mx_blocks(c);
-    MxProduct p{x, (const uint8_t *)x_scales, nullptr, nullptr, (const uint8_t *)w, (const uint8_t *)w_scales, bias, dz, dy, false, batch, a, b, c, d, cb};
+    MxProduct p{x, (const uint8_t *)x_scales, nullptr, nullptr, (const uint8_t *)w, (const uint8_t *)w_scales, bias, dz, dy, false, 0, batch, a, b, c, d, cb};
     if (dz) {
         if (!x || !x_scales || !w || !w_scales || !dy) return KSMM_ERR_NULL_POINTER;
         const int64_t blocks = (int64_t)a * d * batch * cb, w_blocks = (int64_t)a * d * rows_w * cb, size = (int64_t)dtype_size(dtype);
