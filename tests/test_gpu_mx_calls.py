@@ -262,3 +262,20 @@ def test_copies_have_hooks_of_their_own():
         assert not module._forward_hooks and not module._forward_pre_hooks
         copy.register_buffer("more", torch.zeros(1), persistent=False)
         assert not hasattr(module, "more") and not module._non_persistent_buffers_set
+
+
+@pytest.mark.parametrize("bs_last", [False, True])
+@pytest.mark.parametrize("pattern", [(1, 2000, 1, 1), (1, 500, 40, 4), (2, 200, 33, 5), (1, 2000, 9000, 1)])
+def test_gelu_in_fp32_far_below_zero(pattern, bs_last):
+    """Of one factor, relative to its value: 1e-6, and what an exponent of 0.72 z^2 is off by, four times 2^-24 of it: 1.2e-7 z^2."""
+    from ksmm_amd import mx_linear, pack_mx
+
+    a, b, c, d = pattern
+    w = pack_mx(factor(pattern, False, torch.float32).cuda(), pattern)
+    z = torch.linspace(-12, 6, a * b * d)  # (the bias: sums of zeros are exact)
+    for n in (1, 300):
+        x = torch.zeros((a * c * d, n) if bs_last else (n, a * c * d), device="cuda")
+        y = mx_linear(x, w, bias=z.cuda(), act="gelu", bs_last=bs_last).cpu().double()
+        want = z.double() * torch.special.erfc(-z.double() * 0.5 ** 0.5) / 2
+        off = ((y.t() if bs_last else y) - want).abs()
+        assert bool((off <= (1e-6 + 1.2e-7 * z.double().square()) * want.abs()).all())
