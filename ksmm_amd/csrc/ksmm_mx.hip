@@ -7,8 +7,9 @@
 // with zeros: 16 bytes of codes a block, the even place in the lower half of a byte, and a byte of scale.  That is what a lane
 // of the scaled matrix instructions holds: 32 numbers of one row and their scale.
 //
-// Here: conversions, the products of rows whose codes no workgroup's LDS holds, and the C entry points.  Conversions are bound by HBM:
-// 25088 x 384 in fp16 to codes 24.4 MB in 6.4 us and back in 7.6, 768 x 6501 in fp32 batch-size-last 8.4 and 7.4; of that 2 us are a
+// Here: conversions, the products of rows whose codes no workgroup's LDS holds, and the C entry points.  Conversions are short workgroups, of
+// which each loads once and waits for it: 24.4 MB of 25088 x 384 in fp16 take 6.6 to 7.0 us to codes and 8.0 back (medians, of one run's dispatches
+// 6.3 and 7.8 at least), 22.6 MB of 768 x 6501 in fp32 batch-size-last 8.7 and 7.8, where a copy takes 4.7 and 4.4; of that 2 us are a
 // launch's start and end.
 #include "ksmm_mx_product.h"
 

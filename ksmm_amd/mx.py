@@ -432,7 +432,7 @@ class MXLinear(nn.Module):
         for i in range(len(self.dtypes)):
             scales = state_dict.get("%sscales%d" % (prefix, i))
             if scales is not None:
-                self.dtypes[i] = _type_of(scales)
+                self.dtypes[i] = None if scales.is_meta else _type_of(scales)
 
     def forward(self, x):
         return _chain(x, self.factors(), self.patterns, self.bias, self.act, self.bs_last)

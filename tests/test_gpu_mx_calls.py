@@ -95,16 +95,16 @@ def test_sums_for_gradients(pattern, prec, bs_last):
         assert torch.equal(torch.nan_to_num(z), torch.nan_to_num(want)) and (room[-64:] == 7).all()
 
 
-def wide(gated, seed=0):
+def wide(gated, d=1, seed=0):
     """A factor in fp32 whose first block lies beyond fp16's range and whose second one below it, and an input and gradient for it.
 
     Products of the first are 2^8 (gated dz 2^-7), of gradients 2^12; of the second 2^-12."""
     g = torch.Generator().manual_seed(seed)
-    pattern, n = (2, 24, 64, 1), 41
+    pattern, n = (2, 24, 64, d), 41
     a, b, c, d = pattern
-    f = torch.randn(a, c, 2 * b if gated else b, generator=g) * torch.tensor([2.0 ** 17, 2.0 ** -27]).view(2, 1, 1)
-    x = torch.randn(n, a, c, generator=g) * torch.tensor([2.0 ** -12, 1.0]).view(1, 2, 1)
-    dy = torch.randn(n, a, b, generator=g) * torch.tensor([2.0 ** -15, 2.0 ** 13]).view(1, 2, 1)
+    f = torch.randn(a, d * c, 2 * b if gated else b, generator=g) * torch.tensor([2.0 ** 17, 2.0 ** -27]).view(2, 1, 1)
+    x = torch.randn(n, a, c * d, generator=g) * torch.tensor([2.0 ** -12, 1.0]).view(1, 2, 1)
+    dy = torch.randn(n, a, b * d, generator=g) * torch.tensor([2.0 ** -15, 2.0 ** 13]).view(1, 2, 1)
     return pattern, f.reshape(a * d * c, -1), x.reshape(n, -1).half(), dy.reshape(n, -1).half()
 
 
@@ -121,24 +121,25 @@ def wide_gradients(pattern, f, x, dy, bias, act, gated):
 @pytest.mark.parametrize("native", [True, False])
 @pytest.mark.parametrize("gated,act", [(False, None), (False, "gelu"), (True, "silu"), (True, None)])
 @pytest.mark.parametrize("made", ["packed", "by hand"])
-def test_gradients_through_values_beyond_fp16(monkeypatch, made, gated, act, native):
+@pytest.mark.parametrize("d", [1, 5])
+def test_gradients_through_values_beyond_fp16(monkeypatch, d, made, gated, act, native):
     """Codes of fp32 weights hold values that fp16 has not: gradients of fp16 inputs are rounded once for all that, at the end."""
     from ksmm_amd import MXFactor, _lib, mx_linear, pack_mx
 
     if not native:
         monkeypatch.setattr(_lib, "_native", _lib._NoNative)
-    pattern, f, x, dy = wide(gated)
+    pattern, f, x, dy = wide(gated, d)
     w = pack_mx(f.cuda(), pattern, gated)
     if made == "by hand":
         w = MXFactor(w.codes, w.scales, pattern, gated)
-    bias = torch.linspace(-1, 1, f.shape[1] * 2).half()
+    bias = torch.linspace(-1, 1, f.shape[1] * 2 * d).half()
     leaves = [t.cuda().requires_grad_(True) for t in (x, bias)]
     with torch.enable_grad():
         y = mx_linear(leaves[0], w, bias=leaves[1], act=act)
         dx, db = torch.autograd.grad(y, leaves, dy.cuda())
     assert y.dtype == dx.dtype == db.dtype == torch.float16
     want, want_b = wide_gradients(pattern, f, x, dy, bias, act, gated)
-    for part in (slice(0, 64), slice(64, 128)):
+    for part in (slice(0, 64 * d), slice(64 * d, None)):
         # (a value is rounded to 2^-11 of it, or to 2^-25 where the type has no more)
         assert rel(dx[:, part], want[:, part]) <= TOL["fp16"] + 2.0 ** -25 * want[:, part].numel() ** 0.5 / float(want[:, part].norm())
     fine = want_b.abs() < 65504
@@ -279,3 +280,19 @@ def test_gelu_in_fp32_far_below_zero(pattern, bs_last):
         want = z.double() * torch.special.erfc(-z.double() * 0.5 ** 0.5) / 2
         off = ((y.t() if bs_last else y) - want).abs()
         assert bool((off <= (1e-6 + 1.2e-7 * z.double().square()) * want.abs()).all())
+
+
+@pytest.mark.parametrize("bs_last", [False, True])
+@pytest.mark.parametrize("shape", [(0,), (3, 0)])
+def test_gated_batches_of_none(shape, bs_last):
+    from ksmm_amd import mx_linear
+
+    for d in (1, 5):
+        pattern = (1, 40, 64, d)
+        x = torch.zeros(*((64 * d, *shape) if bs_last else (*shape, 64 * d)), device="cuda")
+        with torch.enable_grad():
+            leaves = [x.requires_grad_(True), torch.ones(64 * d, 80, device="cuda", requires_grad=True), torch.zeros(80 * d, device="cuda", requires_grad=True)]
+            y = mx_linear(leaves[0], leaves[1], pattern, bias=leaves[2], act="silu", gated=True, bs_last=bs_last)
+            dx, df, db = torch.autograd.grad(y.sum(), leaves)
+        assert y.shape == ((40 * d, *shape) if bs_last else (*shape, 40 * d)) and dx.shape == x.shape
+        assert not df.any() and not db.any() and df.shape == (64 * d, 80)
