@@ -573,7 +573,6 @@ __global__ __launch_bounds__(64 * GROUPS, 2) void ks_muon_gemm_kernel(MuonArgs a
 }
 
 // ---- choices ----------------------------------------------------------------------------------------------
-int launched() { return hipGetLastError() == hipSuccess ? KSMM_OK : KSMM_ERR_LAUNCH; }
 constexpr int64_t LDS_MOST = 160 * 1024 - 256;
 
 // In one launch where X fits LDS and the waves' registers: (6,64,64,1) 17.7 us, by launches of products 73;
@@ -592,8 +591,7 @@ template <typename T, int WAVES, int HELD> int run_block(const MuonArgs &a, int6
         if (rc != KSMM_OK) return rc;
     }
     if (matrices > THREADS_MOST / (64 * WAVES)) return KSMM_ERR_TOO_LARGE;
-    hipLaunchKernelGGL(fn, dim3((unsigned)matrices), dim3(64 * WAVES), lds, s, a);
-    return launched();
+    return launch_kernel(fn, (unsigned)matrices, 64 * WAVES, lds, s, a);
 }
 
 int64_t align256(int64_t v) { return (v + 255) / 256 * 256; }
@@ -642,15 +640,12 @@ template <typename T> int run(const MuonArgs &a, int64_t matrices, char *ws, hip
     Split x = split(w.x[0], values), y = split(w.x[1], values), xt = split(w.x[2], values), yt = split(w.x[3], values);
     const Split gram = split(w.gram, matrices * w.M * w.M), poly = split(w.poly, matrices * w.M * w.M);
     float *const u = (float *)(ws + w.u), *const squares = (float *)(ws + w.squares);
-    hipLaunchKernelGGL((ks_muon_load_kernel<T>), dim3((unsigned)(matrices * w.chunks)), dim3(256), 0, s, a, u, squares, w.chunks);
-    hipLaunchKernelGGL(ks_muon_split_kernel, dim3((unsigned)full), dim3(256), 0, s, a, u, squares, w.chunks, flip ? xt : x, flip ? x : xt,
-                       flip ? w.N : w.M, flip ? w.M : w.N);
-    int rc = KSMM_OK;
+    int rc = launch_kernel(&ks_muon_load_kernel<T>, (unsigned)(matrices * w.chunks), 256, 0, s, a, u, squares, w.chunks);
+    if (rc == KSMM_OK) rc = launch_kernel(&ks_muon_split_kernel, (unsigned)full, 256, 0, s, a, u, squares, w.chunks, flip ? xt : x, flip ? x : xt, flip ? w.N : w.M, flip ? w.M : w.N);
     auto gemm = [&](auto fn, int groups, int64_t tiles, Split l, Split r, Split old, Split out, Split turned, bool last) {
         const int lds = groups * TILE * TILE * 4;
         if (lds > 64 * 1024 && rc == KSMM_OK) rc = ensure_dynamic_lds((const void *)fn, lds);
-        if (rc != KSMM_OK) return;
-        hipLaunchKernelGGL(fn, dim3((unsigned)((tiles + 7) / 8 * 8)), dim3(64 * groups), lds, s, a, l, r, old, out, turned, w.M, w.N, last, (int)tiles);
+        if (rc == KSMM_OK) rc = launch_kernel(fn, (unsigned)((tiles + 7) / 8 * 8), 64 * groups, lds, s, a, l, r, old, out, turned, w.M, w.N, last, (int)tiles);
     };
     // waves that share K: 8 for the square products, whose tiles are few, 4 for the others ((1,1536,384,2) of two parts 200 us; before
     // loads were kept ahead 223, 4 everywhere 227, 8 everywhere 241; (1,256,256,16) 104; 115, 112, 116)
@@ -661,7 +656,7 @@ template <typename T> int run(const MuonArgs &a, int64_t matrices, char *ws, hip
         std::swap(x, y);
         std::swap(xt, yt);
     }
-    return rc == KSMM_OK ? launched() : rc;
+    return rc;
 }
 
 // sizes are rounded up, and chunks and walks step over the end, in 32 bits
